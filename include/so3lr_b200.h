@@ -329,6 +329,182 @@ int so3lr_last_stats(const so3lr_handle *h, long long *sr_edges, long long *sr_p
  * PersistentCache before Kokkos::finalize, pair_so3lr_native_mpi.cpp:1070-1086). */
 void so3lr_destroy(so3lr_handle *h);
 
+/* ---- Row-wise feed-forward layers in low precision (no counterpart in the reference) ----
+ *
+ * The row-wise half of a transformer block over per-atom (or per-token) features,
+ * as a caller trains it next to this library's evaluations or serves it in 8
+ * bits: RMS norm with the residual's addition, a product of 8-bit integers with
+ * row and channel scales, and the gated feed-forward block with its gradients.
+ *
+ * Conventions of these entry points, besides the ones above:
+ *   - No handle. Every pointer is device memory of the calling thread's current
+ *     CUDA device; `stream` is a cudaStream_t of that device (NULL: the default
+ *     stream). The work is asynchronous on `stream`: a call returns when its
+ *     kernels are queued, allocates nothing and may be captured in a graph.
+ *   - A matrix is row-major with unit column stride and a row stride in elements
+ *     (inputs: any stride >= 0, so a row may be broadcast; outputs: at least the
+ *     row's length). Any alignment of the element type is accepted; rows that
+ *     start on 16-byte boundaries run faster.
+ *   - Sizes are at least 1, but `rows` may be 0: the call then writes only what
+ *     does not depend on rows (weight gradients: zeros).
+ *   - `workspace` is scratch of at least the bytes the matching _workspace
+ *     function returns for the same arguments (-1: invalid sizes), 256-byte
+ *     aligned; its contents mean nothing between calls. Calls that may overlap
+ *     need workspaces of their own.
+ *   - Elements are SO3LR_FLOAT32, SO3LR_BFLOAT16 or SO3LR_FLOAT16. Sums, norms and
+ *     activations are computed in float32 (8-bit products: int32) in a fixed
+ *     order: repeated calls return the same bits. */
+#define SO3LR_FLOAT32 0
+#define SO3LR_BFLOAT16 1
+#define SO3LR_FLOAT16 2
+
+/* RMS norm with the residual's addition, width <= 16384:
+ *   s = x + residual, rounded to the element type (x itself without a residual)
+ *   y = s * weight / sqrt(mean(s^2) + eps)
+ * The norm is of s as stored, so so3lr_rms_norm_backward, which has only the
+ * stored s, returns the gradient of exactly what ran. The result goes to `y`, or,
+ * when `codes` is given instead, into 8 bits with a scale for each row:
+ *   scale = max|y| / 127, code = y / scale rounded to nearest (ties to even)
+ * A row of zeros gets scale 0 and codes 0; a row that holds an infinity or a NaN
+ * gets scale NaN and codes 0. s, y may be the memory of x or residual. */
+typedef struct {
+  long long rows, width;
+  int dtype;                  /* x, residual, s, y */
+  int weight_dtype;           /* dtype or SO3LR_FLOAT32 */
+  double eps;                 /* >= 0 */
+  const void *x;
+  long long x_stride;
+  const void *residual;       /* optional */
+  long long residual_stride;
+  const void *weight;         /* width */
+  void *s;                    /* with a residual: required; without: must be NULL */
+  long long s_stride;
+  void *y;                    /* exactly one of y and codes */
+  long long y_stride;
+  signed char *codes;
+  long long codes_stride;
+  float *scales;              /* rows, with codes */
+} so3lr_rms_norm_args;
+int so3lr_rms_norm(const so3lr_rms_norm_args *args, void *stream, char *err, size_t errlen);
+
+/* Gradients of so3lr_rms_norm: with xh = s / sqrt(mean(s^2) + eps) and a = dy * weight,
+ *   dx = (a - xh mean(a xh)) / sqrt(mean(s^2) + eps) + ds   (also the residual's gradient)
+ *   dweight = sum over rows of dy xh
+ * ds is the gradient that reaches s directly (the residual stream); optional. */
+typedef struct {
+  long long rows, width;
+  int dtype;                  /* dy, s, ds, dx */
+  int weight_dtype;           /* weight, dweight */
+  double eps;
+  const void *dy;
+  long long dy_stride;
+  const void *s;
+  long long s_stride;
+  const void *weight;
+  const void *ds;             /* optional */
+  long long ds_stride;
+  void *dx;                   /* may be the memory of dy or ds */
+  long long dx_stride;
+  void *dweight;              /* width */
+} so3lr_rms_norm_backward_args;
+long long so3lr_rms_norm_backward_workspace(const so3lr_rms_norm_backward_args *args);
+int so3lr_rms_norm_backward(const so3lr_rms_norm_backward_args *args, void *workspace, long long workspace_bytes,
+                            void *stream, char *err, size_t errlen);
+
+/* Product of 8-bit integers, k <= 131071 (an int32 sum cannot overflow):
+ *   y[t][n] = (sum_k a[t][k] b[n][k]) a_scales[t] b_scales[n] + bias[n] */
+typedef struct {
+  long long rows, n, k;
+  int out_dtype;
+  const signed char *a;       /* rows x k */
+  long long a_stride;
+  const float *a_scales;      /* rows */
+  const signed char *b;       /* n x k: output channels are rows */
+  long long b_stride;
+  const float *b_scales;      /* n */
+  const float *bias;          /* n, optional */
+  void *y;                    /* rows x n */
+  long long y_stride;
+} so3lr_int8_linear_args;
+long long so3lr_int8_linear_workspace(const so3lr_int8_linear_args *args);
+int so3lr_int8_linear(const so3lr_int8_linear_args *args, void *workspace, long long workspace_bytes, void *stream,
+                      char *err, size_t errlen);
+
+/* silu(g) * u of rows [g | u] (2 hidden wide, hidden <= 32768), in 8 bits with a
+ * scale for each row as in so3lr_rms_norm: what stands between the two 8-bit
+ * products of a feed-forward block. silu(g) = g / (1 + exp(-g)). */
+typedef struct {
+  long long rows, hidden;
+  int dtype;
+  const void *gu;
+  long long gu_stride;
+  signed char *codes;         /* rows x hidden */
+  long long codes_stride;
+  float *scales;              /* rows */
+} so3lr_gate_int8_args;
+int so3lr_gate_int8(const so3lr_gate_int8_args *args, void *stream, char *err, size_t errlen);
+
+/* out = codes * scale of the row. */
+typedef struct {
+  long long rows, width;
+  int dtype;
+  const signed char *codes;
+  long long codes_stride;
+  const float *scales;
+  void *out;
+  long long out_stride;
+} so3lr_dequantize_int8_args;
+int so3lr_dequantize_int8(const so3lr_dequantize_int8_args *args, void *stream, char *err, size_t errlen);
+
+/* Gated feed-forward block, bfloat16 or float16:
+ *   h = silu(x Wg^T) * (x Wu^T)    (hidden wide; rounded to the element type between the products)
+ *   y = h Wd^T
+ * Weights are stored with output channels as rows. */
+typedef struct {
+  long long rows, width, hidden;
+  int dtype;
+  const void *x;              /* rows x width */
+  long long x_stride;
+  const void *w_gate;         /* hidden x width */
+  long long w_gate_stride;
+  const void *w_up;           /* hidden x width */
+  long long w_up_stride;
+  const void *w_down;         /* width x hidden */
+  long long w_down_stride;
+  void *y;                    /* rows x width */
+  long long y_stride;
+} so3lr_feed_forward_args;
+long long so3lr_feed_forward_workspace(const so3lr_feed_forward_args *args);
+int so3lr_feed_forward(const so3lr_feed_forward_args *args, void *workspace, long long workspace_bytes, void *stream,
+                       char *err, size_t errlen);
+
+/* Gradients of so3lr_feed_forward for dy: with g, u the two projections (computed
+ * again, so nothing is kept from the forward pass), sg = 1 / (1 + exp(-g)),
+ *   dh = dy Wd,  du = dh g sg,  dg = dh u sg (1 + g (1 - sg))
+ *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h */
+typedef struct {
+  long long rows, width, hidden;
+  int dtype;
+  const void *dy;             /* rows x width */
+  long long dy_stride;
+  const void *x;
+  long long x_stride;
+  const void *w_gate;
+  long long w_gate_stride;
+  const void *w_up;
+  long long w_up_stride;
+  const void *w_down;
+  long long w_down_stride;
+  void *dx;                   /* rows x width */
+  long long dx_stride;
+  void *dw_gate;              /* hidden x width, contiguous */
+  void *dw_up;                /* hidden x width, contiguous */
+  void *dw_down;              /* width x hidden, contiguous */
+} so3lr_feed_forward_backward_args;
+long long so3lr_feed_forward_backward_workspace(const so3lr_feed_forward_backward_args *args);
+int so3lr_feed_forward_backward(const so3lr_feed_forward_backward_args *args, void *workspace,
+                                long long workspace_bytes, void *stream, char *err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,34 @@
+// Row-wise feed-forward layers (include/so3lr_b200.h, "Row-wise feed-forward
+// layers"): launchers behind the C entry points of layers.cpp. Arguments have
+// been checked there.
+#pragma once
+
+#include <cstddef>
+
+#include "../../include/so3lr_b200.h"
+#include "common.cuh"
+
+namespace so3lr_b200 {
+
+// A matrix operand: element (r, c) at data + r * row + c * col, in elements.
+struct View {
+  const void *data;
+  long long row, col;
+};
+
+// rows.cu
+void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s);
+long long rms_norm_backward_bytes(const so3lr_rms_norm_backward_args &a);
+void launch_rms_norm_backward(const so3lr_rms_norm_backward_args &a, void *workspace, cudaStream_t s);
+void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s);
+void launch_dequantize_int8(const so3lr_dequantize_int8_args &a, cudaStream_t s);
+
+// dense.cu
+long long int8_linear_bytes(const so3lr_int8_linear_args &a);
+void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s);
+long long feed_forward_bytes(const so3lr_feed_forward_args &a);
+void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s);
+long long feed_forward_backward_bytes(const so3lr_feed_forward_backward_args &a);
+void launch_feed_forward_backward(const so3lr_feed_forward_backward_args &a, void *workspace, cudaStream_t s);
+
+}  // namespace so3lr_b200
