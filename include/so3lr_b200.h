@@ -473,13 +473,15 @@ typedef struct {
   long long w_down_stride;
   void *y;                    /* rows x width */
   long long y_stride;
+  void *h;                    /* optional: rows x hidden, contiguous; h as the second product reads it,
+                                 which so3lr_feed_forward_backward needs */
 } so3lr_feed_forward_args;
 long long so3lr_feed_forward_workspace(const so3lr_feed_forward_args *args);
 int so3lr_feed_forward(const so3lr_feed_forward_args *args, void *workspace, long long workspace_bytes, void *stream,
                        char *err, size_t errlen);
 
 /* Gradients of so3lr_feed_forward for dy: with g, u the two projections (computed
- * again, so nothing is kept from the forward pass), sg = 1 / (1 + exp(-g)),
+ * again, so that only h is kept from the forward pass), sg = 1 / (1 + exp(-g)),
  *   dh = dy Wd,  du = dh g sg,  dg = dh u sg (1 + g (1 - sg))
  *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h */
 typedef struct {
@@ -495,6 +497,7 @@ typedef struct {
   long long w_up_stride;
   const void *w_down;
   long long w_down_stride;
+  const void *h;              /* rows x hidden, contiguous, from the forward pass */
   void *dx;                   /* rows x width */
   long long dx_stride;
   void *dw_gate;              /* hidden x width, contiguous */

@@ -1,81 +1,603 @@
-// Products of the feed-forward layers: simple kernels, one thread per output
-// element from 16 x 16 shared-memory tiles, operands through strided views.
+// Dense products of the feed-forward layers on the tcgen05 tensor cores: 8-bit
+// products with row and channel scales, the gated block's forward pass and its
+// gradients.
+//
+// One persistent kernel. A CTA pair computes a tile of 256 rows x 256 accumulator
+// columns; each CTA stages its 128 rows of A and its 128 rows of B (half the
+// tile's columns) per K block of 128 bytes, six blocks deep, with TMA into
+// 128-byte-swizzled tiles. Against one CTA per 128 x 256 tile this reads a third
+// less from L2 per product, which is what bounds a tile loop at this size.
+// Warp 0 loads, warp 1 of the leader issues the MMAs, warps 2-9 read the
+// accumulators (TMEM lane = row) and write the results; two accumulator buffers of
+// 256 columns, so that a tile's epilogue runs under the next tile's MMAs.
+//
+// Operands are K-major (the contraction runs along the row) or MN-major (it runs
+// down the rows): the gradients need transposed operands, and the tensor core
+// reads them in place. An operand whose rows do not start on 16-byte boundaries
+// (TMA's rule) is first copied into padded rows.
+//
+// Products with few tiles and a long contraction are split along K: each part
+// writes raw 32-bit sums, k_join adds them in order.
+#include <mutex>
+
 #include "layers_common.cuh"
+#include "model_host.hpp"
+#include "tensor_core.cuh"
 
 namespace so3lr_b200 {
 namespace {
 
-constexpr int kTile = 16;
+constexpr int kPairs = kSmCount / 2;
+constexpr int kTileM = 256, kTileN = 256;   // of a CTA pair
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (2 + kEpiWarps) * 32;
+constexpr uint32_t kOperand = 128 * 128;    // 128 rows of 128 bytes: one operand tile of a CTA, 16 KB
+constexpr uint32_t kStaging = 4096;         // of an epilogue warp: 32 rows x 32 values
+constexpr int kBarBytes = 256;
+constexpr int kMaxMaps = 6, kMaxProblems = 3, kMaxStages = 6;
 
-template <class T>
-__device__ __forceinline__ auto at(const View &v, long long r, long long c) {
-  return static_cast<const T *>(v.data)[r * v.row + c * v.col];
-}
+// What the kernel computes.
+enum Mode {
+  kPlain,     // C = A B^T, one or two K segments (A1 B1^T + A2 B2^T)
+  kInt8,      // C = (A B^T) a_scale b_scale + bias
+  kGated,     // C = silu(A G^T) * (A U^T): 128 columns of G and 128 of U per tile
+  kGatedBack  // g, u as above and dh = DY Wd: C = dg, C2 = du
+};
+template <int MODE>
+struct Shape {
+  // x, dy, one of Wg / Wu, 64 columns of Wd per CTA and K block, else A and B
+  static constexpr uint32_t kStage = MODE == kGatedBack ? 3 * kOperand + kOperand / 2 : 2 * kOperand;
+  static constexpr int kStages = MODE == kGatedBack ? 3 : 6;
+  static constexpr int kBuffers = MODE == kGatedBack ? 1 : 2;  // accumulators of 384 or 256 columns in 512
+  static constexpr uint32_t kSmem = kStage * kStages + kEpiWarps * kStaging + kBarBytes + 1024;
+  static constexpr int kColumns = MODE == kGated || MODE == kGatedBack ? 128 : kTileN;  // result columns per tile
+};
 
-// one element of A (m x k) times B (n x k), transposed; all threads of the block call it
-template <class T, class Acc>
-__device__ Acc product(const View &A, const View &B, long long m, long long n, long long k, long long row,
-                       long long col) {
-  __shared__ Acc ta[kTile][kTile + 1], tb[kTile][kTile + 1];
-  Acc sum = 0;
-  const long long brow = col - threadIdx.x + threadIdx.y;
-  for (long long k0 = 0; k0 < k; k0 += kTile) {
-    const long long c = k0 + threadIdx.x;
-    ta[threadIdx.y][threadIdx.x] = row < m && c < k ? Acc(at<T>(A, row, c)) : Acc(0);
-    tb[threadIdx.y][threadIdx.x] = brow < n && c < k ? Acc(at<T>(B, brow, c)) : Acc(0);
-    __syncthreads();
+struct Problem {
+  int a[2], b[2];                // tensor maps of the K segments
+  int kb0, kb;                   // K blocks of the first segment, of both
+  int m, n;                      // result
+  int tiles_m, tiles_n, splits;
+  int first;                     // its first work item
+  void *c;
+  long long ldc;
+  long long partial;             // offset of its raw sums (splits > 1): [splits][m][ldp]
+  int ldp;
+};
+struct Params {
+  CUtensorMap map[kMaxMaps];
+  Problem prob[kMaxProblems];
+  int problems, items;
+  void *c2;                      // du
+  const float *a_scales, *b_scales, *bias;
+  uint32_t *partial;
+  int *err;
+};
+
+struct Item {
+  int prob, m0, n0, kb_begin, kb_end, split;
+};
+template <int MODE>
+__device__ __forceinline__ Item item_of(const Params &p, int it) {
+  Item w;
+  w.prob = 0;
 #pragma unroll
-    for (int i = 0; i < kTile; ++i) sum += ta[threadIdx.y][i] * tb[threadIdx.x][i];
-    __syncthreads();
-  }
-  return sum;
+  for (int i = 1; i < kMaxProblems; ++i)
+    if (i < p.problems && it >= p.prob[i].first) w.prob = i;
+  const Problem &q = p.prob[w.prob];
+  const int r = it - q.first;
+  w.split = r % q.splits;
+  const int tile = r / q.splits;
+  // groups of 8 row tiles, columns outer: the tiles in flight share their operands in L2
+  const int group = tile / (8 * q.tiles_n), rows = min(8, q.tiles_m - 8 * group), t = tile - group * 8 * q.tiles_n;
+  w.m0 = (8 * group + t % rows) * kTileM;
+  w.n0 = (t / rows) * Shape<MODE>::kColumns;
+  w.kb_begin = int((long long)q.kb * w.split / q.splits);
+  w.kb_end = int((long long)q.kb * (w.split + 1) / q.splits);
+  return w;
 }
 
-__device__ __forceinline__ long long tile_row() { return (long long)blockIdx.x * kTile + threadIdx.y; }
-__device__ __forceinline__ long long tile_col() { return (long long)blockIdx.y * kTile + threadIdx.x; }
-dim3 grid_of(long long m, long long n) {
-  return dim3(unsigned((m + kTile - 1) / kTile), unsigned((n + kTile - 1) / kTile));
-}
-
+// 32 values of each of the warp's 32 rows (lane = row) to C through the warp's
+// staging, which turns them into stores of whole 64- or 128-byte row segments.
+// 16-byte pieces of a staged row are permuted with the row: no bank conflicts.
 template <class O>
-__global__ void k_int8_linear(const so3lr_int8_linear_args a) {
-  const long long r = tile_row(), c = tile_col();
-  const int sum = product<signed char, int>(View{a.a, a.a_stride, 1}, View{a.b, a.b_stride, 1}, a.rows, a.n, a.k, r, c);
-  if (r >= a.rows || c >= a.n) return;
-  float y = float(sum) * a.a_scales[r] * a.b_scales[c];
-  if (a.bias) y += a.bias[c];
-  static_cast<O *>(a.y)[r * a.y_stride + c] = from_float<O>(y);
+__device__ __forceinline__ void store32(unsigned char *stage, int lane, const float (&v)[32], O *c, long long ldc,
+                                        int rows, int cols, bool wide) {
+  constexpr int kPer = 16 / sizeof(O), kPieces = 32 / kPer;  // 4 pieces of 16-bit values, 8 of 32-bit ones
+  const int row_bytes = 32 * sizeof(O);
+  auto slot = [&](int r, int piece) {
+    return stage + r * row_bytes + 16 * (piece ^ (sizeof(O) == 2 ? (r >> 1) & 3 : r & 7));
+  };
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    Chunk<O, kPer> out;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) out.e[j] = from_float<O>(v[i * kPer + j]);
+    store_chunk<O, kPer>(reinterpret_cast<O *>(slot(lane, i)), out);
+  }
+  __syncwarp();
+  const int piece = lane % kPieces;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int r = i * (32 / kPieces) + lane / kPieces;
+    const Chunk<O, kPer> out = load_chunk<O, kPer>(reinterpret_cast<const O *>(slot(r, piece)));
+    if (r < rows) {
+      O *dst = c + r * ldc + piece * kPer;
+      const int left = cols - piece * kPer;
+      if (wide && left >= kPer)
+        store_chunk<O, kPer>(dst, out);
+      else
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (j < left) dst[j] = out.e[j];
+    }
+  }
+  __syncwarp();
 }
 
-// C = A1 B1^T (+ A2 B2^T)
-template <class T>
-__global__ void k_product(View A1, View B1, View A2, View B2, long long m, long long n, long long k, T *C,
-                          long long c_stride) {
-  const long long r = tile_row(), c = tile_col();
-  float v = product<T, float>(A1, B1, m, n, k, r, c);
-  if (A2.data) v += product<T, float>(A2, B2, m, n, k, r, c);
-  if (r < m && c < n) C[r * c_stride + c] = from_float<T>(v);
+__device__ __forceinline__ void to_floats(const uint32_t (&r)[32], float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-template <class T>
-__global__ void k_gated(View X, View G, View U, long long m, long long n, long long k, T *H) {
-  const long long r = tile_row(), c = tile_col();
-  const float g = product<T, float>(X, G, m, n, k, r, c), u = product<T, float>(X, U, m, n, k, r, c);
-  if (r < m && c < n) H[r * n + c] = from_float<T>(silu_f32(g) * u);
+template <int MODE, class T, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense(const __grid_constant__ Params p) {
+  using S = Shape<MODE>;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = tc::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  unsigned char *sm = smem_raw + (base - raw);
+  unsigned char *staging = sm + S::kStage * S::kStages;
+  unsigned char *bar_mem = staging + kEpiWarps * kStaging;
+  const uint32_t bars = tc::smem_u32(bar_mem);
+  auto full = [&](int s) { return bars + 8u * s; };                      // K block landed in both CTAs (leader)
+  auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };      // MMAs done with it (both)
+  auto acc_full = [&](int b) { return bars + 8u * (2 * kMaxStages + b); };       // accumulator complete (both)
+  auto acc_empty = [&](int b) { return bars + 8u * (2 * kMaxStages + 2 + b); };  // read by both CTAs (leader)
+  const uint32_t drain = bars + 8u * (2 * kMaxStages + 4);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar_mem + 8 * (2 * kMaxStages + 5));
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  volatile int *issued = reinterpret_cast<volatile int *>(tmem_slot + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(tc::cluster_rank());
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      tc::mbar_init(full(s), 1);
+      tc::mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      tc::mbar_init(acc_full(b), 1);
+      tc::mbar_init(acc_empty(b), 2 * kEpiWarps);
+    }
+    tc::mbar_init(drain, 1);
+    *abort_flag = 0;
+    *issued = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc::smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::cluster_sync();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------- loads
+    if (lane == 0) {
+      int n = 0;
+      bool ok = true;
+      for (int it = pair; it < p.items && ok; it += pairs) {
+        const Item w = item_of<MODE>(p, it);
+        const Problem &q = p.prob[w.prob];
+        for (int kb = w.kb_begin; kb < w.kb_end; ++kb, ++n) {
+          const int s = n % S::kStages;
+          ok = tc::mbar_wait(empty(s), ((n / S::kStages) & 1) ^ 1, abort_flag, p.err, 1);
+          if (!ok) break;
+          if (rank == 0) tc::mbar_expect_tx(full(s), 2 * S::kStage);
+          const uint32_t bar = tc::at_leader(full(s)), dst = base + s * S::kStage;
+          constexpr int kElems = MODE == kInt8 ? 128 : 64;  // of a K block
+          if (MODE == kGated || MODE == kGatedBack) {
+            const int k = kb * 64;
+            tc::tma_load(dst, &p.map[0], k, w.m0 + 128 * rank, bar);                  // x
+            tc::tma_load(dst + kOperand, &p.map[1 + rank], k, w.n0, bar);             // Wg | Wu
+            if (MODE == kGatedBack) {
+              tc::tma_load(dst + 2 * kOperand, &p.map[3], k, w.m0 + 128 * rank, bar); // dy
+              tc::tma_load(dst + 3 * kOperand, &p.map[4], w.n0 + 64 * rank, k, bar);  // Wd
+            }
+          } else {
+            const int seg = kb >= q.kb0 ? 1 : 0, k = (kb - (seg ? q.kb0 : 0)) * kElems;
+            const CUtensorMap *a = &p.map[q.a[seg]], *b = &p.map[q.b[seg]];
+            const int m = w.m0 + 128 * rank, c = w.n0 + 128 * rank;
+            if (A_MN) {
+              tc::tma_load(dst, a, m, k, bar);
+              tc::tma_load(dst + kOperand / 2, a, m + 64, k, bar);
+            } else {
+              tc::tma_load(dst, a, k, m, bar);
+            }
+            if (B_MN) {
+              tc::tma_load(dst + kOperand, b, c, k, bar);
+              tc::tma_load(dst + kOperand + kOperand / 2, b, c + 64, k, bar);
+            } else {
+              tc::tma_load(dst + kOperand, b, k, c, bar);
+            }
+          }
+          *issued = n + 1;
+        }
+      }
+      // every release of a K block has reached this CTA before it may leave
+      for (int i = max(0, n - S::kStages); i < n && ok; ++i)
+        ok = tc::mbar_wait(empty(i % S::kStages), (i / S::kStages) & 1, abort_flag, p.err, 6);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // -------------------------------------------------------------------- MMAs
+    if (rank == 0 && lane == 0) {
+      constexpr bool kI8 = MODE == kInt8;
+      constexpr uint32_t kAb = kI8 || std::is_same<T, __nv_bfloat16>::value ? 1 : 0;  // s8 / bf16, or f16
+      constexpr uint32_t kId = tc::idesc(kI8 ? 2 : 1, kAb, A_MN, B_MN, 256);
+      constexpr uint32_t kIdDh = tc::idesc(1, kAb, false, true, 128);
+      int n = 0, done = 0;
+      bool ok = true;
+      for (int it = pair; it < p.items && ok; it += pairs, ++done) {
+        const Item w = item_of<MODE>(p, it);
+        const int buf = done % S::kBuffers;
+        ok = tc::mbar_wait(acc_empty(buf), ((done / S::kBuffers) & 1) ^ 1, abort_flag, p.err, 2);
+        if (!ok) break;
+        tc::fence_after();
+        const uint32_t d = tmem + 256u * buf;
+        for (int kb = w.kb_begin; kb < w.kb_end; ++kb, ++n) {
+          const int s = n % S::kStages;
+          ok = tc::mbar_wait(full(s), (n / S::kStages) & 1, abort_flag, p.err, 3);
+          if (!ok) break;
+          tc::fence_after();
+          const uint32_t a = base + s * S::kStage, b = a + kOperand;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const uint64_t da = A_MN ? tc::desc_mn(a + 2048 * ks, kOperand / 2) : tc::desc_k(a + 32 * ks);
+            const uint64_t db = B_MN ? tc::desc_mn(b + 2048 * ks, kOperand / 2) : tc::desc_k(b + 32 * ks);
+            tc::mma<kI8>(d, da, db, kId, kb > w.kb_begin || ks > 0);
+            if (MODE == kGatedBack)
+              tc::mma<false>(d + 256, tc::desc_k(a + 2 * kOperand + 32 * ks),
+                             tc::desc_mn(a + 3 * kOperand + 2048 * ks, kOperand / 2), kIdDh,
+                             kb > w.kb_begin || ks > 0);
+          }
+          tc::commit_pair(empty(s));
+        }
+        if (!ok) break;
+        tc::commit_pair(acc_full(buf));
+      }
+      // every MMA has completed and, after a wait that gave up, so have the copies in flight (bounded)
+      tc::commit_pair(drain);
+      tc::mbar_wait(drain, 0, abort_flag, p.err, 4);
+      if (!ok) {
+        const long long t0 = clock64();
+        for (int i = n; i < *issued; ++i)
+          while (!tc::mbar_try(full(i % S::kStages), (i / S::kStages) & 1) && clock64() - t0 < tc::kWaitCycles) {
+          }
+      }
+    } else if (lane == 0) {
+      tc::mbar_wait(drain, 0, abort_flag, p.err, 4);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    unsigned char *stage = staging + (warp - 2) * kStaging;
+    const uint32_t lanes = tmem + (uint32_t(32 * quad) << 16);
+    int done = 0;
+    for (int it = pair; it < p.items; it += pairs, ++done) {
+      const Item w = item_of<MODE>(p, it);
+      const Problem &q = p.prob[w.prob];
+      const int buf = done % S::kBuffers;
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(acc_full(buf), (done / S::kBuffers) & 1, abort_flag, p.err, 5)))
+        break;
+      tc::fence_after();
+      const uint32_t acc = lanes + 256u * buf;
+      auto release = [&] {  // this warp has read its part of the accumulator
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(tc::at_leader(acc_empty(buf)));
+      };
+      const int row0 = w.m0 + 128 * rank + 32 * quad, rows = min(32, q.m - row0);
+      if (MODE == kPlain || MODE == kInt8) {
+        const bool split = q.splits > 1;
+        const float sa = MODE == kInt8 && !split && lane < rows ? p.a_scales[row0 + lane] : 0.0f;
+        const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % 16 == 0;
+        for (int j = 0; j < 4; ++j) {
+          const int col = 128 * half + 32 * j, c0 = w.n0 + col;
+          uint32_t r[32];
+          tc::tmem_ld32(acc + col, r);
+          tc::wait_ld(r);
+          if (j == 3) release();
+          if (rows <= 0 || c0 >= q.n) continue;
+          float v[32];
+          if (split) {
+            to_floats(r, v);  // raw 32-bit sums, float or int
+            store32<float>(stage, lane, v,
+                           reinterpret_cast<float *>(p.partial) + q.partial + ((long long)w.split * q.m + row0) * q.ldp + c0,
+                           q.ldp, rows, q.n - c0, true);
+            continue;
+          }
+          if (MODE == kInt8) {
+            const bool live = c0 + lane < q.n;
+            const float sb = live ? p.b_scales[c0 + lane] : 0.0f, bias = live && p.bias ? p.bias[c0 + lane] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float s = __shfl_sync(0xffffffffu, sb, i), t = __shfl_sync(0xffffffffu, bias, i);
+              v[i] = fmaf(float(int(r[i])) * sa, s, t);
+            }
+          } else {
+            to_floats(r, v);
+          }
+          store32<T>(stage, lane, v, static_cast<T *>(q.c) + row0 * q.ldc + c0, q.ldc, rows, q.n - c0, wide);
+        }
+      } else {
+        const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % 16 == 0;
+        for (int j = 0; j < 2; ++j) {
+          const int col = 64 * half + 32 * j, c0 = w.n0 + col;
+          uint32_t g[32], u[32];
+          tc::tmem_ld32(acc + col, g);
+          tc::tmem_ld32(acc + 128 + col, u);
+          if (MODE == kGated) {
+            tc::wait_ld(g);
+            tc::wait_ld(u);
+            if (j == 1) release();
+            if (rows <= 0 || c0 >= q.n) continue;
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = silu_f32(__uint_as_float(g[i])) * __uint_as_float(u[i]);
+            store32<T>(stage, lane, v, static_cast<T *>(q.c) + row0 * q.ldc + c0, q.ldc, rows, q.n - c0, wide);
+          } else {
+            uint32_t dh[32];
+            tc::tmem_ld32(acc + 256 + col, dh);
+            tc::wait_ld(g);
+            tc::wait_ld(u);
+            tc::wait_ld(dh);
+            if (j == 1) release();
+            if (rows <= 0 || c0 >= q.n) continue;
+            float dg[32], du[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float gi = __uint_as_float(g[i]), d = __uint_as_float(dh[i]);
+              const float sg = __fdividef(1.0f, 1.0f + __expf(-gi));
+              du[i] = d * (gi * sg);
+              dg[i] = d * __uint_as_float(u[i]) * (sg * fmaf(gi, 1.0f - sg, 1.0f));
+            }
+            const long long at = row0 * q.ldc + c0;
+            store32<T>(stage, lane, dg, static_cast<T *>(q.c) + at, q.ldc, rows, q.n - c0, wide);
+            store32<T>(stage, lane, du, static_cast<T *>(p.c2) + at, q.ldc, rows, q.n - c0, wide);
+          }
+        }
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::cluster_sync();  // neither CTA leaves while the other may still signal it
+  tc::fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-template <class T>
-__global__ void k_gated_backward(View X, View G, View U, View DY, View DT, long long m, long long n, long long k,
-                                 T *H, T *DG, T *DU) {
-  const long long r = tile_row(), c = tile_col();
-  const float g = product<T, float>(X, G, m, n, k, r, c), u = product<T, float>(X, U, m, n, k, r, c);
-  const float dh = product<T, float>(DY, DT, m, n, k, r, c);
-  if (r >= m || c >= n) return;
-  const float sg = __fdividef(1.0f, 1.0f + __expf(-g));
-  H[r * n + c] = from_float<T>(g * sg * u);
-  DU[r * n + c] = from_float<T>(dh * g * sg);
-  DG[r * n + c] = from_float<T>(dh * u * sg * (1.0f + g * (1.0f - sg)));
+// C = the sum over `splits` of raw [m][ldp] sums, in order; 8-bit products get their scales here
+template <class T, bool INT8>
+__global__ void k_join(const uint32_t *__restrict__ partial, int splits, int m, int n, int ldp, T *__restrict__ c,
+                       long long ldc, const float *__restrict__ a_scales, const float *__restrict__ b_scales,
+                       const float *__restrict__ bias, bool wide) {
+  const int per_row = ldp / 4;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < (long long)m * per_row;
+       i += (long long)gridDim.x * blockDim.x) {
+    const int row = int(i / per_row), col = int(i - (long long)row * per_row) * 4;
+    float f[4] = {0, 0, 0, 0};
+    int s[4] = {0, 0, 0, 0};
+    for (int k = 0; k < splits; ++k) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(partial + ((long long)k * m + row) * ldp + col);
+      const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (INT8)
+          s[j] += int(e[j]);
+        else
+          f[j] += __uint_as_float(e[j]);
+      }
+    }
+    Chunk<T, 4> out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (INT8 && col + j < n)
+        f[j] = fmaf(float(s[j]) * a_scales[row], b_scales[col + j], bias ? bias[col + j] : 0.0f);
+      out.e[j] = from_float<T>(f[j]);
+    }
+    T *dst = c + row * ldc + col;
+    if (wide && col + 4 <= n)
+      store_chunk<T, 4>(dst, out);
+    else
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < n) dst[j] = out.e[j];
+  }
 }
+
+// rows copied to rows that start on 16-byte boundaries (the rest of a padded row is not read)
+template <class T>
+__global__ void k_repack(long long rows, int cols, const T *__restrict__ src, long long stride, T *__restrict__ dst,
+                         int ld) {
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * cols;
+       i += (long long)gridDim.x * blockDim.x) {
+    const long long r = i / cols;
+    const int c = int(i - r * cols);
+    dst[r * ld + c] = src[r * stride + c];
+  }
+}
+
+// -------------------------------------------------------------------- host side
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    SO3_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !p) throw Error("cuTensorMapEncodeTiled: the driver does not have it");
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// Where a kernel whose wait gave up says so (page-locked host memory that every
+// device writes); looked at before the next call queues work.
+int *gave_up_flag() {
+  static int *flag = [] {
+    // allowed while another stream of the thread is being captured: it is no stream operation
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SO3_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    void *p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    SO3_CUDA(e);
+    *static_cast<volatile int *>(p) = 0;
+    return static_cast<int *>(p);
+  }();
+  return flag;
+}
+void check_gave_up() {
+  const int where = *static_cast<volatile int *>(gave_up_flag());
+  if (where)
+    throw Error("feed-forward layers: a kernel of an earlier call gave up waiting (stage " + std::to_string(where) +
+                "); its results are not valid");
+}
+
+// Scratch handed out from the caller's workspace; with base == nullptr only counted.
+class Scratch {
+ public:
+  explicit Scratch(void *base) : base_(static_cast<char *>(base)) {}
+  void *take(long long bytes) {
+    void *p = base_ + used_;
+    used_ += (bytes + 255) / 256 * 256;
+    return p;
+  }
+  long long used() const { return used_; }
+
+ private:
+  char *base_;
+  long long used_ = 0;
+};
+
+// A row-major operand [rows][cols].
+struct Operand {
+  const void *data;
+  long long stride;
+  long long rows, cols;
+};
+
+// Builds and queues products; with `dry` only the scratch is counted, so that the
+// workspace sizes come from the code that uses the workspace.
+class Dense {
+ public:
+  Dense(void *workspace, int elem, cudaStream_t stream, bool dry)
+      : scratch_(workspace), elem_(elem), stream_(stream), dry_(dry) {
+    if (!dry) check_gave_up();
+  }
+  Scratch &scratch() { return scratch_; }
+  bool dry() const { return dry_; }
+  cudaStream_t stream() const { return stream_; }
+
+  // the operand as TMA reads it: in place, or copied to padded rows
+  Operand ready(Operand o) {
+    const bool in_place = reinterpret_cast<uintptr_t>(o.data) % 16 == 0 &&
+                          (o.rows == 1 || (o.stride * elem_ % 16 == 0 && o.stride >= o.cols));
+    if (in_place) return o;
+    const int ld = int(padded(o.cols));
+    void *p = scratch_.take(o.rows * ld * elem_);
+    if (!dry_) {
+      const unsigned grid = unsigned(std::min<long long>((o.rows * o.cols + 255) / 256, kSmCount * 32));
+      if (elem_ == 1)
+        k_repack<<<grid, 256, 0, stream_>>>(o.rows, int(o.cols), static_cast<const uint8_t *>(o.data), o.stride,
+                                            static_cast<uint8_t *>(p), ld);
+      else
+        k_repack<<<grid, 256, 0, stream_>>>(o.rows, int(o.cols), static_cast<const uint16_t *>(o.data), o.stride,
+                                            static_cast<uint16_t *>(p), ld);
+      SO3_LAUNCH("repack");
+    }
+    return Operand{p, ld, o.rows, o.cols};
+  }
+  long long padded(long long cols) const { return (cols * elem_ + 15) / 16 * 16 / elem_; }
+
+  // A tensor map whose boxes are 128 bytes of `box_rows` rows.
+  CUtensorMap map(const Operand &o, int box_rows) const {
+    CUtensorMap m;
+    const cuuint64_t dims[2] = {cuuint64_t(o.cols), cuuint64_t(o.rows)};
+    const cuuint64_t stride[1] = {cuuint64_t((o.rows == 1 ? padded(o.cols) : o.stride) * elem_)};
+    const cuuint32_t box[2] = {cuuint32_t(128 / elem_), cuuint32_t(box_rows)}, step[2] = {1, 1};
+    const CUresult r = encode_tiled()(
+        &m, elem_ == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+        const_cast<void *>(o.data), dims, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw Error("cuTensorMapEncodeTiled failed with " + std::to_string(int(r)));
+    return m;
+  }
+
+  // Work items of the problems; a problem list that leaves most CTA pairs idle is
+  // split along K, at least four K blocks to a part.
+  template <int MODE>
+  void plan(Params &p, bool may_split) {
+    long long tiles = 0;
+    int kb = 1 << 30;
+    for (int i = 0; i < p.problems; ++i) {
+      Problem &q = p.prob[i];
+      q.tiles_m = (q.m - 1) / kTileM + 1;
+      q.tiles_n = (q.n - 1) / Shape<MODE>::kColumns + 1;
+      tiles += (long long)q.tiles_m * q.tiles_n;
+      kb = std::min(kb, q.kb);
+    }
+    if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
+    const int splits = may_split ? std::max(1, std::min(int(kPairs / tiles), kb / 4)) : 1;
+    long long partial = 0;
+    p.items = 0;
+    for (int i = 0; i < p.problems; ++i) {
+      Problem &q = p.prob[i];
+      q.splits = splits;
+      q.first = p.items;
+      p.items += q.tiles_m * q.tiles_n * splits;
+      q.ldp = (q.n + 3) / 4 * 4;
+      q.partial = partial;
+      if (splits > 1) partial += (long long)splits * q.m * q.ldp;
+    }
+    p.partial = splits > 1 ? static_cast<uint32_t *>(scratch_.take(partial * 4)) : nullptr;
+  }
+
+  template <int MODE, class T, bool A_MN, bool B_MN>
+  void run(Params &p) {
+    const void *fn = reinterpret_cast<const void *>(&k_dense<MODE, T, A_MN, B_MN>);
+    allow_dynamic_smem(fn, Shape<MODE>::kSmem);
+    p.err = gave_up_flag();
+    k_dense<MODE, T, A_MN, B_MN>
+        <<<2 * std::min(kPairs, p.items), kThreads, Shape<MODE>::kSmem, stream_>>>(p);
+    SO3_LAUNCH("dense");
+    for (int i = 0; i < p.problems; ++i) {
+      const Problem &q = p.prob[i];
+      if (q.splits == 1) continue;
+      const long long total = (long long)q.m * (q.ldp / 4);
+      const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % (4 * sizeof(T)) == 0;
+      k_join<T, MODE == kInt8><<<unsigned(std::min<long long>((total + 255) / 256, kSmCount * 16)), 256, 0, stream_>>>(
+          p.partial + q.partial, q.splits, q.m, q.n, q.ldp, static_cast<T *>(q.c), q.ldc, p.a_scales, p.b_scales,
+          p.bias, wide);
+      SO3_LAUNCH("join");
+    }
+  }
+
+ private:
+  Scratch scratch_;
+  int elem_;
+  cudaStream_t stream_;
+  bool dry_;
+};
+
+int blocks_of(long long k, int per) { return int((k + per - 1) / per); }
 
 template <class F>
 void by_half(int dtype, F &&f) {
@@ -84,62 +606,195 @@ void by_half(int dtype, F &&f) {
   else
     f(__half{});
 }
-const dim3 kBlock(kTile, kTile);
+
+// ------------------------------------------------------------------ 8-bit product
+template <class O>
+void int8_linear(Dense &d, const so3lr_int8_linear_args &a) {
+  Params p{};
+  const Operand x = d.ready(Operand{a.a, a.a_stride, a.rows, a.k}), w = d.ready(Operand{a.b, a.b_stride, a.n, a.k});
+  p.problems = 1;
+  p.a_scales = a.a_scales;
+  p.b_scales = a.b_scales;
+  p.bias = a.bias;
+  Problem &q = p.prob[0];
+  q.a[0] = 0;
+  q.b[0] = 1;
+  q.kb = q.kb0 = blocks_of(a.k, 128);
+  q.m = int(a.rows);
+  q.n = int(a.n);
+  q.c = a.y;
+  q.ldc = a.y_stride;
+  d.plan<kInt8>(p, true);
+  if (d.dry()) return;
+  p.map[0] = d.map(x, 128);
+  p.map[1] = d.map(w, 128);
+  d.run<kInt8, O, false, false>(p);
+}
+
+// ------------------------------------------------------------------- feed-forward
+template <class T>
+void feed_forward(Dense &d, const so3lr_feed_forward_args &a) {
+  const Operand x = d.ready(Operand{a.x, a.x_stride, a.rows, a.width});
+  const Operand g = d.ready(Operand{a.w_gate, a.w_gate_stride, a.hidden, a.width});
+  const Operand u = d.ready(Operand{a.w_up, a.w_up_stride, a.hidden, a.width});
+  const Operand w = d.ready(Operand{a.w_down, a.w_down_stride, a.width, a.hidden});
+  Operand h{a.h, a.hidden, a.rows, a.hidden};
+  if (!a.h) {
+    h.stride = d.padded(a.hidden);
+    h.data = d.scratch().take(a.rows * h.stride * 2);
+  }
+  {
+    Params p{};
+    p.problems = 1;
+    Problem &q = p.prob[0];
+    q.kb = q.kb0 = blocks_of(a.width, 64);
+    q.m = int(a.rows);
+    q.n = int(a.hidden);
+    q.c = const_cast<void *>(h.data);
+    q.ldc = h.stride;
+    d.plan<kGated>(p, false);
+    if (!d.dry()) {
+      p.map[0] = d.map(x, 128);
+      p.map[1] = d.map(g, 128);
+      p.map[2] = d.map(u, 128);
+      d.run<kGated, T, false, false>(p);
+    }
+  }
+  const Operand hr = d.ready(h);
+  Params p{};
+  p.problems = 1;
+  Problem &q = p.prob[0];
+  q.a[0] = 0;
+  q.b[0] = 1;
+  q.kb = q.kb0 = blocks_of(a.hidden, 64);
+  q.m = int(a.rows);
+  q.n = int(a.width);
+  q.c = a.y;
+  q.ldc = a.y_stride;
+  d.plan<kPlain>(p, true);
+  if (d.dry()) return;
+  p.map[0] = d.map(hr, 128);
+  p.map[1] = d.map(w, 128);
+  d.run<kPlain, T, false, false>(p);
+}
 
 template <class T>
-void multiply(View A, View B, View A2, View B2, long long m, long long n, long long k, void *c, long long c_stride,
-              cudaStream_t s) {
-  k_product<T><<<grid_of(m, n), kBlock, 0, s>>>(A, B, A2, B2, m, n, k, static_cast<T *>(c), c_stride);
-  SO3_LAUNCH("product");
+void feed_forward_backward(Dense &d, const so3lr_feed_forward_backward_args &a) {
+  const Operand x = d.ready(Operand{a.x, a.x_stride, a.rows, a.width});
+  const Operand dy = d.ready(Operand{a.dy, a.dy_stride, a.rows, a.width});
+  const Operand g = d.ready(Operand{a.w_gate, a.w_gate_stride, a.hidden, a.width});
+  const Operand u = d.ready(Operand{a.w_up, a.w_up_stride, a.hidden, a.width});
+  const Operand w = d.ready(Operand{a.w_down, a.w_down_stride, a.width, a.hidden});
+  const Operand h = d.ready(Operand{a.h, a.hidden, a.rows, a.hidden});
+  const long long ld = d.padded(a.hidden);
+  Operand dg{d.scratch().take(a.rows * ld * 2), ld, a.rows, a.hidden}, du = dg;
+  du.data = d.scratch().take(a.rows * ld * 2);
+  {
+    Params p{};
+    p.problems = 1;
+    Problem &q = p.prob[0];
+    q.kb = q.kb0 = blocks_of(a.width, 64);
+    q.m = int(a.rows);
+    q.n = int(a.hidden);
+    q.c = const_cast<void *>(dg.data);
+    q.ldc = ld;
+    p.c2 = const_cast<void *>(du.data);
+    d.plan<kGatedBack>(p, false);
+    if (!d.dry()) {
+      p.map[0] = d.map(x, 128);
+      p.map[1] = d.map(g, 128);
+      p.map[2] = d.map(u, 128);
+      p.map[3] = d.map(dy, 128);
+      p.map[4] = d.map(w, 64);
+      d.run<kGatedBack, T, false, false>(p);
+    }
+  }
+  {  // dx = dg Wg + du Wu: one contraction over both
+    Params p{};
+    p.problems = 1;
+    Problem &q = p.prob[0];
+    q.a[0] = 0;
+    q.a[1] = 1;
+    q.b[0] = 2;
+    q.b[1] = 3;
+    q.kb0 = blocks_of(a.hidden, 64);
+    q.kb = 2 * q.kb0;
+    q.m = int(a.rows);
+    q.n = int(a.width);
+    q.c = a.dx;
+    q.ldc = a.dx_stride;
+    d.plan<kPlain>(p, true);
+    if (!d.dry()) {
+      p.map[0] = d.map(dg, 128);
+      p.map[1] = d.map(du, 128);
+      p.map[2] = d.map(g, 64);
+      p.map[3] = d.map(u, 64);
+      d.run<kPlain, T, false, true>(p);
+    }
+  }
+  // the three weight gradients, contracted over the rows, in one launch
+  Params p{};
+  p.problems = 3;
+  for (int i = 0; i < 3; ++i) {
+    Problem &q = p.prob[i];
+    q.a[0] = i;              // dg, du, dy
+    q.b[0] = i < 2 ? 3 : 4;  // x, x, h
+    q.kb = q.kb0 = blocks_of(a.rows, 64);
+    q.m = int(i < 2 ? a.hidden : a.width);
+    q.n = int(i < 2 ? a.width : a.hidden);
+    q.c = i == 0 ? a.dw_gate : i == 1 ? a.dw_up : a.dw_down;
+    q.ldc = q.n;
+  }
+  d.plan<kPlain>(p, true);
+  if (d.dry()) return;
+  p.map[0] = d.map(dg, 64);
+  p.map[1] = d.map(du, 64);
+  p.map[2] = d.map(dy, 64);
+  p.map[3] = d.map(x, 64);
+  p.map[4] = d.map(h, 64);
+  d.run<kPlain, T, true, true>(p);
+}
+
+template <class A, class F>
+long long dry_run(const A &a, int elem, F &&f) {
+  if (a.rows == 0) return 0;
+  Dense d(nullptr, elem, nullptr, true);
+  f(d);
+  return d.scratch().used();
 }
 
 }  // namespace
 
-long long int8_linear_bytes(const so3lr_int8_linear_args &) { return 0; }
-void launch_int8_linear(const so3lr_int8_linear_args &a, void *, cudaStream_t s) {
-  const dim3 grid = grid_of(a.rows, a.n);
+long long int8_linear_bytes(const so3lr_int8_linear_args &a) {
+  return dry_run(a, 1, [&](Dense &d) { int8_linear<float>(d, a); });
+}
+void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s) {
+  Dense d(workspace, 1, s, false);
   if (a.out_dtype == SO3LR_FLOAT32)
-    k_int8_linear<float><<<grid, kBlock, 0, s>>>(a);
-  else if (a.out_dtype == SO3LR_BFLOAT16)
-    k_int8_linear<__nv_bfloat16><<<grid, kBlock, 0, s>>>(a);
+    int8_linear<float>(d, a);
   else
-    k_int8_linear<__half><<<grid, kBlock, 0, s>>>(a);
-  SO3_LAUNCH("int8_linear");
+    by_half(a.out_dtype, [&](auto t) { int8_linear<decltype(t)>(d, a); });
 }
 
-long long feed_forward_bytes(const so3lr_feed_forward_args &a) { return a.rows * a.hidden * 2; }
+long long feed_forward_bytes(const so3lr_feed_forward_args &a) {
+  return dry_run(a, 2, [&](Dense &d) { feed_forward<__half>(d, a); });
+}
 void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s) {
-  by_half(a.dtype, [&](auto t) {
-    using T = decltype(t);
-    k_gated<T><<<grid_of(a.rows, a.hidden), kBlock, 0, s>>>(
-        View{a.x, a.x_stride, 1}, View{a.w_gate, a.w_gate_stride, 1}, View{a.w_up, a.w_up_stride, 1}, a.rows,
-        a.hidden, a.width, static_cast<T *>(workspace));
-    SO3_LAUNCH("gated");
-    multiply<T>(View{workspace, a.hidden, 1}, View{a.w_down, a.w_down_stride, 1}, View{}, View{}, a.rows, a.width,
-                a.hidden, a.y, a.y_stride, s);
-  });
+  Dense d(workspace, 2, s, false);
+  by_half(a.dtype, [&](auto t) { feed_forward<decltype(t)>(d, a); });
 }
 
 long long feed_forward_backward_bytes(const so3lr_feed_forward_backward_args &a) {
-  return 3 * a.rows * a.hidden * 2;
+  return dry_run(a, 2, [&](Dense &d) { feed_forward_backward<__half>(d, a); });
 }
 void launch_feed_forward_backward(const so3lr_feed_forward_backward_args &a, void *workspace, cudaStream_t s) {
-  by_half(a.dtype, [&](auto t) {
-    using T = decltype(t);
-    const long long R = a.rows, D = a.width, H = a.hidden;
-    T *h = static_cast<T *>(workspace), *dg = h + R * H, *du = dg + R * H;
-    if (R > 0) {
-      k_gated_backward<T><<<grid_of(R, H), kBlock, 0, s>>>(
-          View{a.x, a.x_stride, 1}, View{a.w_gate, a.w_gate_stride, 1}, View{a.w_up, a.w_up_stride, 1},
-          View{a.dy, a.dy_stride, 1}, View{a.w_down, 1, a.w_down_stride}, R, H, D, h, dg, du);
-      SO3_LAUNCH("gated_backward");
-      multiply<T>(View{dg, H, 1}, View{a.w_gate, 1, a.w_gate_stride}, View{du, H, 1}, View{a.w_up, 1, a.w_up_stride},
-                  R, D, H, a.dx, a.dx_stride, s);
-    }
-    multiply<T>(View{dg, 1, H}, View{a.x, 1, a.x_stride}, View{}, View{}, H, D, R, a.dw_gate, D, s);
-    multiply<T>(View{du, 1, H}, View{a.x, 1, a.x_stride}, View{}, View{}, H, D, R, a.dw_up, D, s);
-    multiply<T>(View{a.dy, 1, a.dy_stride}, View{h, 1, H}, View{}, View{}, D, H, R, a.dw_down, H, s);
-  });
+  if (a.rows == 0) {
+    const std::size_t bytes = std::size_t(a.hidden) * a.width * 2;
+    for (void *w : {a.dw_gate, a.dw_up, a.dw_down}) SO3_CUDA(cudaMemsetAsync(w, 0, bytes, s));
+    return;
+  }
+  Dense d(workspace, 2, s, false);
+  by_half(a.dtype, [&](auto t) { feed_forward_backward<decltype(t)>(d, a); });
 }
 
 }  // namespace so3lr_b200

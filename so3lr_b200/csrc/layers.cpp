@@ -192,12 +192,14 @@ void check(const so3lr_feed_forward_args *a) {
   check_feed_forward_sizes(call, a);
   check_feed_forward_inputs(call, a);
   matrix(call, "y", a->y, a->y_stride, a->rows, a->width, 2, true);
+  if (a->h) matrix(call, "h", a->h, a->hidden, a->rows, a->hidden, 2, true);
 }
 void check(const so3lr_feed_forward_backward_args *a) {
   const char *call = "so3lr_feed_forward_backward";
   check_feed_forward_sizes(call, a);
   check_feed_forward_inputs(call, a);
   matrix(call, "dy", a->dy, a->dy_stride, a->rows, a->width, 2, false);
+  matrix(call, "h", a->h, a->hidden, a->rows, a->hidden, 2, false);
   matrix(call, "dx", a->dx, a->dx_stride, a->rows, a->width, 2, true);
   pointer(call, "dw_gate", a->dw_gate, 2);
   pointer(call, "dw_up", a->dw_up, 2);

@@ -10,11 +10,6 @@
 
 namespace so3lr_b200 {
 
-// A matrix operand: element (r, c) at data + r * row + c * col, in elements.
-struct View {
-  const void *data;
-  long long row, col;
-};
 
 // rows.cu
 void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s);

@@ -71,13 +71,13 @@ class _DequantizeInt8(C.Structure):
 class _FeedForward(C.Structure):
     _fields_ = [("rows", _ll), ("width", _ll), ("hidden", _ll), ("dtype", _i), ("x", _p), ("x_stride", _ll),
                 ("w_gate", _p), ("w_gate_stride", _ll), ("w_up", _p), ("w_up_stride", _ll), ("w_down", _p),
-                ("w_down_stride", _ll), ("y", _p), ("y_stride", _ll)]
+                ("w_down_stride", _ll), ("y", _p), ("y_stride", _ll), ("h", _p)]
 
 
 class _FeedForwardBackward(C.Structure):
     _fields_ = [("rows", _ll), ("width", _ll), ("hidden", _ll), ("dtype", _i), ("dy", _p), ("dy_stride", _ll),
                 ("x", _p), ("x_stride", _ll), ("w_gate", _p), ("w_gate_stride", _ll), ("w_up", _p),
-                ("w_up_stride", _ll), ("w_down", _p), ("w_down_stride", _ll), ("dx", _p), ("dx_stride", _ll),
+                ("w_up_stride", _ll), ("w_down", _p), ("w_down_stride", _ll), ("h", _p), ("dx", _p), ("dx_stride", _ll),
                 ("dw_gate", _p), ("dw_up", _p), ("dw_down", _p)]
 
 
@@ -345,16 +345,17 @@ def _ffn_operands(x, w_gate, w_up, w_down):
     return x2, g, u, d, t, hidden
 
 
-def _ffn(x, w_gate, w_up, w_down):
+def _ffn(x, w_gate, w_up, w_down, keep=False):
     x2, g, u, d, t, hidden = _ffn_operands(x, w_gate, w_up, w_down)
     rows, width = x2.shape
     y = torch.empty((rows, width), dtype=x2.dtype, device=x2.device)
+    h = torch.empty((rows, hidden), dtype=x2.dtype, device=x2.device) if keep else None
     if rows:
         _queue("so3lr_feed_forward",
                _FeedForward(rows, width, hidden, t, x2.data_ptr(), x2.stride(0), g.data_ptr(), g.stride(0),
-                            u.data_ptr(), u.stride(0), d.data_ptr(), d.stride(0), y.data_ptr(), width),
-               x2.device, scratch=True)
-    return _shaped(y, x)
+                            u.data_ptr(), u.stride(0), d.data_ptr(), d.stride(0), y.data_ptr(), width,
+                            h.data_ptr() if keep else None), x2.device, scratch=True)
+    return _shaped(y, x), h
 
 
 class _FeedForwardFunction(torch.autograd.Function):
@@ -376,21 +377,24 @@ def feed_forward(x, w_gate, w_up, w_down):
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
                                     w_down.requires_grad):
         return _FeedForwardFunction.apply(x, w_gate, w_up, w_down)
-    return _ffn(x, w_gate, w_up, w_down)
+    return _ffn(x, w_gate, w_up, w_down)[0]
 
 
 def feed_forward_train(x, w_gate, w_up, w_down):
     """(y, saved): feed_forward, and what feed_forward_backward needs of it."""
-    return _ffn(x, w_gate, w_up, w_down), (x, w_gate, w_up, w_down)
+    y, h = _ffn(x, w_gate, w_up, w_down, keep=True)
+    return y, (x, w_gate, w_up, w_down, h)
 
 
 def feed_forward_backward(dy, saved):
     """(dx, dw_gate, dw_up, dw_down) for the gradient dy of feed_forward_train's y."""
-    x, w_gate, w_up, w_down = saved
+    x, w_gate, w_up, w_down, h = saved
     x2, g, u, d, t, hidden = _ffn_operands(x, w_gate, w_up, w_down)
     rows, width = x2.shape
     dev = x2.device
     d2 = _rows(dy, "dy", dev, x2.dtype, width, rows)
+    if h.shape != (rows, hidden) or h.dtype != x2.dtype or not h.is_contiguous():
+        raise ValueError("saved does not come from feed_forward_train")
     dx = torch.empty((rows, width), dtype=x2.dtype, device=dev)
     dwg = torch.empty((hidden, width), dtype=x2.dtype, device=dev)
     dwu = torch.empty((hidden, width), dtype=x2.dtype, device=dev)
@@ -398,7 +402,7 @@ def feed_forward_backward(dy, saved):
     _queue("so3lr_feed_forward_backward",
            _FeedForwardBackward(rows, width, hidden, t, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0),
                                 g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0), d.data_ptr(), d.stride(0),
-                                dx.data_ptr(), width, dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr()),
+                                h.data_ptr(), dx.data_ptr(), width, dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr()),
            dev, scratch=True)
     return _shaped(dx, x), dwg, dwu, dwd
 
