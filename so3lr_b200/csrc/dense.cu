@@ -363,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const float gi = __uint_as_float(g[i]), d = __uint_as_float(dh[i]);
-              const float sg = __fdividef(1.0f, 1.0f + __expf(-gi));
+              const float sg = sigmoid_f32(gi);
               du[i] = d * (gi * sg);
               dg[i] = d * __uint_as_float(u[i]) * (sg * fmaf(gi, 1.0f - sg, 1.0f));
             }
@@ -446,29 +446,6 @@ EncodeTiled encode_tiled() {
     return reinterpret_cast<EncodeTiled>(p);
   }();
   return fn;
-}
-
-// Where a kernel whose wait gave up says so (page-locked host memory that every
-// device writes); looked at before the next call queues work.
-int *gave_up_flag() {
-  static int *flag = [] {
-    // allowed while another stream of the thread is being captured: it is no stream operation
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    SO3_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-    void *p = nullptr;
-    const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    SO3_CUDA(e);
-    *static_cast<volatile int *>(p) = 0;
-    return static_cast<int *>(p);
-  }();
-  return flag;
-}
-void check_gave_up() {
-  const int where = *static_cast<volatile int *>(gave_up_flag());
-  if (where)
-    throw Error("feed-forward layers: a kernel of an earlier call gave up waiting (stage " + std::to_string(where) +
-                "); its results are not valid");
 }
 
 // Scratch handed out from the caller's workspace; with base == nullptr only counted.
@@ -765,10 +742,35 @@ long long dry_run(const A &a, int elem, F &&f) {
 
 }  // namespace
 
+// Where a kernel whose wait gave up says so (page-locked host memory that every
+// device writes); looked at before the next call queues work.
+int *gave_up_flag() {
+  static int *flag = [] {
+    // allowed while another stream of the thread is being captured: it is no stream operation
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SO3_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    void *p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    SO3_CUDA(e);
+    *static_cast<volatile int *>(p) = 0;
+    return static_cast<int *>(p);
+  }();
+  return flag;
+}
+void check_gave_up() {
+  const int where = *static_cast<volatile int *>(gave_up_flag());
+  if (where)
+    throw Error("feed-forward layers: a kernel of an earlier call gave up waiting (stage " + std::to_string(where) +
+                "); its results are not valid");
+}
+
 long long int8_linear_bytes(const so3lr_int8_linear_args &a) {
+  if (a.rows <= kFewRows) return 0;
   return dry_run(a, 1, [&](Dense &d) { int8_linear<float>(d, a); });
 }
 void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s) {
+  if (a.rows <= kFewRows) return launch_int8_linear_few(a, s);
   Dense d(workspace, 1, s, false);
   if (a.out_dtype == SO3LR_FLOAT32)
     int8_linear<float>(d, a);
@@ -776,10 +778,14 @@ void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaSt
     by_half(a.out_dtype, [&](auto t) { int8_linear<decltype(t)>(d, a); });
 }
 
+// rows of the hidden layer of a few rows, on 16-byte boundaries
+static long long few_stride(const so3lr_feed_forward_args &a) { return (a.hidden + 7) / 8 * 8; }
 long long feed_forward_bytes(const so3lr_feed_forward_args &a) {
+  if (a.rows <= kFewRows) return a.h ? 0 : a.rows * few_stride(a) * 2;
   return dry_run(a, 2, [&](Dense &d) { feed_forward<__half>(d, a); });
 }
 void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s) {
+  if (a.rows <= kFewRows) return launch_feed_forward_few(a, a.h ? a.h : workspace, a.h ? a.hidden : few_stride(a), s);
   Dense d(workspace, 2, s, false);
   by_half(a.dtype, [&](auto t) { feed_forward<decltype(t)>(d, a); });
 }

@@ -1,0 +1,183 @@
+// Dense products of the feed-forward layers for up to kFewRows rows (single atoms or
+// tokens, small batches). All that counts is reading the weights once, at HBM's rate:
+// a block takes 8 output channels and its warps split the contraction, so that a
+// 4096 x 4096 weight has 512 blocks. The products run on warp-level MMAs
+// (m16n8k16 / m16n8k32, rows as M, channels as N) straight from registers: a tile of
+// the tcgen05 kernel would be filled to a few of its 256 rows and would need its
+// operands in shared memory first.
+//
+// Contraction order: an MMA takes two 4-byte words of each lane's operands. A lane
+// loads 16 contiguous bytes (words 0..3) of its row and of its channel at the same
+// place, feeds words 0, 1 to one MMA and 2, 3 to the next; both operands use the
+// same permutation of the contraction, so the sums are those of the formula.
+#include "layers_common.cuh"
+#include "model_host.hpp"
+
+namespace so3lr_b200 {
+namespace {
+
+__device__ __forceinline__ void mma_words(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_words(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_words(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1, signed char) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <class E, class Acc>
+__device__ __forceinline__ void mma_step(Acc (&c)[4], const uint4 &x0, const uint4 &x1, const uint4 &w) {
+  mma_words(c, x0.x, x1.x, x0.y, x1.y, w.x, w.y, E{});
+  mma_words(c, x0.z, x1.z, x0.w, x1.w, w.z, w.w, E{});
+}
+
+// 16 bytes of a row from element k on; elements past the row's end read as zero
+template <class E, bool ALIGNED, bool WEIGHT>
+__device__ __forceinline__ uint4 load16(const E *p, int k, int length) {
+  constexpr int kPer = 16 / sizeof(E);
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (ALIGNED && k + kPer <= length) {
+    if (WEIGHT)  // read once: not kept in L1
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "l"(p + k));
+    else
+      v = *reinterpret_cast<const uint4 *>(p + k);
+  } else {
+    alignas(16) E e[kPer] = {};
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (k + i < length) e[i] = p[k + i];
+    v = *reinterpret_cast<const uint4 *>(e);
+  }
+  return v;
+}
+
+struct FewArgs {
+  int rows, n, k;
+  const void *x;
+  long long x_stride;
+  const void *w, *w2;            // w2: the up projection (GATED)
+  long long w_stride, w2_stride;
+  void *y;
+  long long y_stride;
+  const float *a_scales, *b_scales, *bias;  // 8-bit products
+};
+
+// y = x w^T (8 bits: scaled), or silu(x w^T) * (x w2^T). TWO: more than 8 rows.
+template <class E, class O, bool GATED, bool TWO, bool ALIGNED>
+__global__ void __launch_bounds__(256) k_few_rows(const FewArgs a) {
+  constexpr bool kInt8 = std::is_same<E, signed char>::value;
+  using Acc = typename std::conditional<kInt8, int, float>::type;
+  constexpr int kPer = 16 / sizeof(E), kUnroll = GATED ? 4 : 8, kOut = GATED ? 2 : 1;
+  __shared__ Acc part[8][kOut][16][8];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n = blockIdx.x * 8 + g;
+  const E *w = static_cast<const E *>(a.w) + n * a.w_stride, *w2 = static_cast<const E *>(a.w2) + n * a.w2_stride;
+  const E *x0 = static_cast<const E *>(a.x) + g * a.x_stride, *x1 = x0 + 8 * a.x_stride;
+  const bool live_n = n < a.n, live0 = g < a.rows, live1 = TWO && g + 8 < a.rows;
+  const int steps = (a.k + 4 * kPer - 1) / (4 * kPer);
+  const int begin = int((long long)steps * warp / warps), end = int((long long)steps * (warp + 1) / warps);
+  Acc acc[kOut][4] = {};
+  for (int st = begin; st < end; st += kUnroll) {
+    uint4 vw[kUnroll], vw2[GATED ? kUnroll : 1], v0[kUnroll], v1[TWO ? kUnroll : 1];
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = ((st + i) * 4 + t) * kPer;
+      const bool in = st + i < end && k < a.k;
+      vw[i] = in && live_n ? load16<E, ALIGNED, true>(w, k, a.k) : zero;
+      if (GATED) vw2[i] = in && live_n ? load16<E, ALIGNED, true>(w2, k, a.k) : zero;
+      v0[i] = in && live0 ? load16<E, ALIGNED, false>(x0, k, a.k) : zero;
+      if (TWO) v1[i] = in && live1 ? load16<E, ALIGNED, false>(x1, k, a.k) : zero;
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      mma_step<E>(acc[0], v0[i], TWO ? v1[i] : zero, vw[i]);
+      if (GATED) mma_step<E>(acc[kOut - 1], v0[i], TWO ? v1[i] : zero, vw2[i]);
+    }
+  }
+#pragma unroll
+  for (int o = 0; o < kOut; ++o) {
+    part[warp][o][g][2 * t] = acc[o][0];
+    part[warp][o][g][2 * t + 1] = acc[o][1];
+    part[warp][o][g + 8][2 * t] = acc[o][2];
+    part[warp][o][g + 8][2 * t + 1] = acc[o][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 8 * a.rows; i += blockDim.x) {
+    const int row = i >> 3, c = blockIdx.x * 8 + (i & 7);
+    if (c >= a.n) continue;
+    Acc sum[kOut] = {};
+    for (int k = 0; k < warps; ++k)
+#pragma unroll
+      for (int o = 0; o < kOut; ++o) sum[o] += part[k][o][row][i & 7];
+    float y;
+    if (kInt8)
+      y = fmaf(float(sum[0]) * a.a_scales[row], a.b_scales[c], a.bias ? a.bias[c] : 0.0f);
+    else if (GATED)
+      y = silu_f32(float(sum[0])) * float(sum[kOut - 1]);
+    else
+      y = float(sum[0]);
+    static_cast<O *>(a.y)[row * a.y_stride + c] = from_float<O>(y);
+  }
+}
+
+bool rows_aligned(const void *p, long long stride, long long rows, int size) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || stride * size % 16 == 0));
+}
+
+template <class E, class O, bool GATED>
+void run(const FewArgs &a, cudaStream_t s) {
+  constexpr int kPer = 16 / sizeof(E);
+  const bool aligned = rows_aligned(a.x, a.x_stride, a.rows, sizeof(E)) && rows_aligned(a.w, a.w_stride, a.n, sizeof(E)) &&
+                       rows_aligned(a.w2, a.w2_stride, a.n, sizeof(E));
+  // up to 8 warps split the contraction, at least two steps of 64 bytes to each
+  const int steps = (a.k + 4 * kPer - 1) / (4 * kPer), warps = std::max(1, std::min(8, steps / 2));
+  const unsigned grid = unsigned((a.n + 7) / 8), block = unsigned(32 * warps);
+  if (a.rows > 8)
+    aligned ? k_few_rows<E, O, GATED, true, true><<<grid, block, 0, s>>>(a)
+            : k_few_rows<E, O, GATED, true, false><<<grid, block, 0, s>>>(a);
+  else
+    aligned ? k_few_rows<E, O, GATED, false, true><<<grid, block, 0, s>>>(a)
+            : k_few_rows<E, O, GATED, false, false><<<grid, block, 0, s>>>(a);
+  SO3_LAUNCH("few_rows");
+}
+
+}  // namespace
+
+void launch_int8_linear_few(const so3lr_int8_linear_args &l, cudaStream_t s) {
+  const FewArgs a{int(l.rows), int(l.n), int(l.k), l.a, l.a_stride, l.b, nullptr, l.b_stride, 0, l.y, l.y_stride,
+                  l.a_scales, l.b_scales, l.bias};
+  if (l.out_dtype == SO3LR_FLOAT32)
+    run<signed char, float, false>(a, s);
+  else if (l.out_dtype == SO3LR_BFLOAT16)
+    run<signed char, __nv_bfloat16, false>(a, s);
+  else
+    run<signed char, __half, false>(a, s);
+}
+
+void launch_feed_forward_few(const so3lr_feed_forward_args &f, void *h, long long h_stride, cudaStream_t s) {
+  const FewArgs up{int(f.rows), int(f.hidden), int(f.width), f.x, f.x_stride, f.w_gate, f.w_up, f.w_gate_stride,
+                   f.w_up_stride, h, h_stride, nullptr, nullptr, nullptr};
+  const FewArgs down{int(f.rows), int(f.width), int(f.hidden), h, h_stride, f.w_down, nullptr, f.w_down_stride, 0,
+                     f.y, f.y_stride, nullptr, nullptr, nullptr};
+  if (f.dtype == SO3LR_BFLOAT16) {
+    run<__nv_bfloat16, __nv_bfloat16, true>(up, s);
+    run<__nv_bfloat16, __nv_bfloat16, false>(down, s);
+  } else {
+    run<__half, __half, true>(up, s);
+    run<__half, __half, false>(down, s);
+  }
+}
+
+}  // namespace so3lr_b200

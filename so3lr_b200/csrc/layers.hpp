@@ -19,11 +19,20 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s);
 void launch_dequantize_int8(const so3lr_dequantize_int8_args &a, cudaStream_t s);
 
 // dense.cu
+// Where a kernel whose bounded wait gave up says so, and the refusal of further calls after that.
+int *gave_up_flag();
+void check_gave_up();
 long long int8_linear_bytes(const so3lr_int8_linear_args &a);
 void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s);
 long long feed_forward_bytes(const so3lr_feed_forward_args &a);
 void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s);
 long long feed_forward_backward_bytes(const so3lr_feed_forward_backward_args &a);
 void launch_feed_forward_backward(const so3lr_feed_forward_backward_args &a, void *workspace, cudaStream_t s);
+
+// few_rows.cu: the forward products for at most kFewRows rows, any alignment, no
+// workspace but the hidden layer's
+constexpr int kFewRows = 16;
+void launch_int8_linear_few(const so3lr_int8_linear_args &a, cudaStream_t s);
+void launch_feed_forward_few(const so3lr_feed_forward_args &a, void *h, long long h_stride, cudaStream_t s);
 
 }  // namespace so3lr_b200

@@ -46,14 +46,29 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// silu(g) = g / (1 + exp(-g)). exp(-g) overflows to infinity for g < -88 and the
-// quotient is then 0, as it should be to float32's range.
-__device__ __forceinline__ float silu_f32(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
+// 1 / (1 + exp(-g)) with the hardware's exponential and reciprocal (both within 2
+// units in the last place). exp(-g) overflows to infinity for g < -88, and the
+// result is then 0, as it should be to float32's range; the flushed denormals of
+// either do not show beside 1.
+__device__ __forceinline__ float sigmoid_f32(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+__device__ __forceinline__ float silu_f32(float g) { return g * sigmoid_f32(g); }
 
-// max|v| of a row from the bits of |v|, which order like the values with
-// infinities and NaN on top. Row scale: 0 for a row whose scale would not be a
-// normal number (its reciprocal could overflow), NaN for one that holds an
-// infinity or a NaN; `inv` is then 0, which makes every code 0.
+// |result| = max(|a|, |b|), a NaN if either is one (the sign is the product of
+// theirs): one instruction per element of a row's maximum
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Row scale from the bits of max|v|, which order like the values with infinities
+// and NaN on top: 0 for a row whose scale would not be a normal number (its
+// reciprocal could overflow), NaN for one that holds an infinity or a NaN. `inv` is
+// then 0, which makes every code 0.
 __device__ __forceinline__ float row_scale(uint32_t top_bits, float &inv) {
   inv = 0.0f;
   if (top_bits > 0x7f7fffffu) return __uint_as_float(0x7fc00000u);
@@ -62,9 +77,32 @@ __device__ __forceinline__ float row_scale(uint32_t top_bits, float &inv) {
   inv = 1.0f / scale;
   return scale;
 }
-__device__ __forceinline__ signed char to_code(float v, float inv) {
-  // a NaN can only meet inv = 0 here; __float2int_rn turns the NaN product into 0
-  return static_cast<signed char>(max(-127, min(127, __float2int_rn(v * inv))));
+// VEC codes of a row: v inv rounded to nearest even. Adding 1.5 2^23 leaves the
+// rounded integer in the low bits of the sum (a float-to-int conversion runs at an
+// eighth of the rate); |v inv| <= 127 (1 + 2^-22), so the low byte is the code.
+template <int VEC>
+__device__ __forceinline__ Chunk<signed char, VEC> to_codes(const float *v, float inv) {
+  Chunk<signed char, VEC> out;
+  uint32_t q[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) q[i] = __float_as_uint(fmaf(v[i], inv, 12582912.0f));
+  if (VEC % 4 == 0) {
+    const uint32_t live = inv != 0.0f ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const uint32_t lo = __byte_perm(q[4 * i], q[4 * i + 1], 0x0040), hi = __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040);
+      reinterpret_cast<uint32_t *>(&out)[i] = __byte_perm(lo, hi, 0x5410) & live;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out.e[i] = inv != 0.0f ? static_cast<signed char>(q[i] & 0xff) : 0;
+  }
+  return out;
+}
+// The float of a signed byte, without the slow int-to-float conversion: the byte
+// + 128 in the low bits of 2^23
+__device__ __forceinline__ float byte_to_float(uint32_t flipped, int i) {
+  return __uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
 }
 
 }  // namespace so3lr_b200

@@ -6,15 +6,16 @@
 // A row belongs to one warp (up to 16 elements per lane, so that short rows need
 // no block barrier) or to one block. A thread holds N chunks of VEC elements:
 // 16-byte chunks where every row starts on a 16-byte boundary, single elements
-// otherwise (odd widths, views).
+// otherwise (odd widths, views). Eight elements a thread keep the registers low and
+// so the bytes in flight high; sixteen only where a row would not fit otherwise.
 #include "layers_common.cuh"
 #include "model_host.hpp"
+#include "tensor_core.cuh"
 
 namespace so3lr_b200 {
 namespace {
 
 constexpr int kWarpRows = 8;     // rows of a block when a warp owns a row
-constexpr int kPerThread = 16;   // elements a thread holds at most (norm)
 
 // The threads of one row: a warp or the whole block. Reductions run in a fixed
 // order and return the same value to every thread of the row.
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
     }
   }
   const float rstd = 1.0f / sqrtf(team.sum(sq, slot) / float(width) + float(a.eps));
-  uint32_t top = 0;
+  float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = (j * team.size + team.t) * VEC;
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
         const float y = v[j * VEC + i] * rstd * to_float(cw[j].e[i]);
         v[j * VEC + i] = y;
         if (QUANT)
-          top = ::max(top, __float_as_uint(y) & 0x7fffffffu);
+          top = max_abs(top, y);
         else
           out.e[i] = from_float<T>(y);
       }
@@ -122,24 +123,21 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
   }
   if (!QUANT) return;
   float inv;
-  const float scale = row_scale(team.max(top, slot_max), inv);
+  const float scale = row_scale(team.max(__float_as_uint(top) & 0x7fffffffu, slot_max), inv);
   if (team.t == 0) a.scales[row] = scale;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = (j * team.size + team.t) * VEC;
-    if (c < width) {
-      Chunk<signed char, VEC> out;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out.e[i] = to_code(v[j * VEC + i], inv);
-      store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, out);
-    }
+    if (c < width)
+      store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
   }
 }
 
 // dx = rstd (a - xh mean(a xh)) + ds with a = dy w, xh = s rstd; each block also
 // sums dy xh over its rows (a fixed set, in order) into one row of `partial`.
-template <class T, class W, int VEC, int N, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial) {
+template <class T, class W, int VEC, int N, int MAXT>
+__global__ void __launch_bounds__(MAXT) k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial) {
+  constexpr bool WARP = MAXT == 32 * kWarpRows;
   __shared__ float2 slot[2][32];
   extern __shared__ float column[];  // WARP: kWarpRows x width
   const RowTeam<WARP> team;
@@ -229,6 +227,126 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm_backw
   }
 }
 
+// A ring of rows in shared memory, filled by bulk copies: what is in flight costs no
+// registers, so a block that walks over rows keeps the memory system busy while it
+// reduces and writes the current one. One block barrier after the last read of a
+// stage, thread 0 may refill it.
+struct RowRing {
+  uint32_t bars, buffer, stage_bytes;
+  int stages;
+  unsigned char *mem;
+  int *err;
+  volatile int *abort_flag;
+
+  __device__ RowRing(unsigned char *smem, uint32_t bytes, int nstages, int *error)
+      : stage_bytes(bytes), stages(nstages), mem(smem + 128), err(error) {
+    bars = tc::smem_u32(smem);
+    buffer = bars + 128;
+    abort_flag = reinterpret_cast<volatile int *>(smem + 120);
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) tc::mbar_init(bars + 8 * i, 1);
+      *abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+  }
+  __device__ const unsigned char *stage(int i) const { return mem + (i % stages) * stage_bytes; }
+  // waits for the i-th row of this block; after a wait that gave up (reported in *err) nothing waits again
+  __device__ void wait(int i) const { tc::mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, abort_flag, err, 7); }
+  // thread 0: the copies of the i-th row
+  __device__ uint32_t expect(int i, uint32_t bytes) const {
+    tc::mbar_expect_tx(bars + 8 * (i % stages), bytes);
+    return buffer + (i % stages) * stage_bytes;
+  }
+  __device__ uint32_t bar(int i) const { return bars + 8 * (i % stages); }
+};
+constexpr int kRingHeader = 128, kRingStages = 8;
+
+// k_rms_norm_backward for rows on 16-byte boundaries that need a block: 16 elements a
+// thread, rows through a ring. Bound by instruction issue before it is bound by HBM:
+// the row's reduction costs each warp about a hundred instructions, so fewer and
+// fuller warps are faster (8 elements a thread: 115 us at 16384 x 4096 bfloat16).
+template <class T, class W>
+__global__ void __launch_bounds__(512)
+    k_rms_norm_backward_ring(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, int stages, int *err) {
+  constexpr int VEC = 16 / sizeof(T), N = 16 / VEC;
+  __shared__ float2 slot[2][32];
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
+  const uint32_t row_bytes = width * sizeof(T), tensors = a.ds ? 3 : 2;
+  const RowRing ring(smem, tensors * row_bytes, stages, err);
+  const RowTeam<false> team;
+  const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
+  auto fetch = [&](int i) {
+    const long long row = blockIdx.x + (long long)i * gridDim.x;
+    const uint32_t dst = ring.expect(i, tensors * row_bytes);
+    tc::bulk_load(dst, static_cast<const T *>(a.s) + row * a.s_stride, row_bytes, ring.bar(i));
+    tc::bulk_load(dst + row_bytes, static_cast<const T *>(a.dy) + row * a.dy_stride, row_bytes, ring.bar(i));
+    if (a.ds)
+      tc::bulk_load(dst + 2 * row_bytes, static_cast<const T *>(a.ds) + row * a.ds_stride, row_bytes, ring.bar(i));
+  };
+  if (t == 0)
+    for (int i = 0; i < min(stages, rows); ++i) fetch(i);
+  Chunk<W, VEC> cw[N];
+  float dw[16];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = (j * size + t) * VEC;
+    if (c < width) cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dw[j * VEC + i] = 0.0f;
+  }
+  const float per = 1.0f / float(width);
+  for (int k = 0; k < rows; ++k) {
+    ring.wait(k);
+    const T *s = reinterpret_cast<const T *>(ring.stage(k));
+    Chunk<T, VEC> cs[N], cd[N], ce[N];
+    float sq = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        cs[j] = load_chunk<T, VEC>(s + c);
+        cd[j] = load_chunk<T, VEC>(s + width + c);
+        if (a.ds) ce[j] = load_chunk<T, VEC>(s + 2 * width + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float f = to_float(cs[j].e[i]);
+          sq = fmaf(f, f, sq);
+          dot = fmaf(f, to_float(cd[j].e[i]) * to_float(cw[j].e[i]), dot);
+        }
+      }
+    }
+    const float2 total = team.sum2(sq, dot, slot[k & 1]);  // a barrier: every thread has read the stage
+    if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
+    const float rstd = 1.0f / sqrtf(total.x * per + float(a.eps));
+    const float back = -(total.y * rstd * per) * rstd * rstd;  // - mean(a xh) rstd^2, times s
+    T *dx = static_cast<T *>(a.dx) + (blockIdx.x + (long long)k * gridDim.x) * a.dx_stride;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        Chunk<T, VEC> out;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float f = to_float(cs[j].e[i]), d = to_float(cd[j].e[i]);
+          dw[j * VEC + i] = fmaf(d, f * rstd, dw[j * VEC + i]);
+          const float rest = a.ds ? fmaf(f, back, to_float(ce[j].e[i])) : f * back;
+          out.e[i] = from_float<T>(fmaf(d * to_float(cw[j].e[i]), rstd, rest));
+        }
+        store_chunk<T, VEC>(dx + c, out);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = (j * size + t) * VEC;
+    if (c < width)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) partial[(size_t)blockIdx.x * width + c + i] = dw[j * VEC + i];
+  }
+}
+
 // column sums of `partial` (nparts x width) in a fixed order: 32 columns per
 // block, part k summed by thread row k % 32, then the 32 thread rows in order
 template <class W>
@@ -237,7 +355,7 @@ __global__ void k_column_sum(int nparts, int width, const float *__restrict__ pa
   const int c = blockIdx.x * 32 + threadIdx.x;
   float total = 0.0f;
   if (c < width)
-#pragma unroll 4
+#pragma unroll 8
     for (int k = threadIdx.y; k < nparts; k += 32) total += partial[(size_t)k * width + c];
   part[threadIdx.y][threadIdx.x] = total;
   __syncthreads();
@@ -249,8 +367,10 @@ __global__ void k_column_sum(int nparts, int width, const float *__restrict__ pa
   }
 }
 
+// 8-bit rows of silu(g) u
 template <class T, int VEC, int N, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_gate_int8(const so3lr_gate_int8_args a) {
+__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024, VEC *N == 8 && !WARP ? 2 : 1)
+    k_gate_int8(const so3lr_gate_int8_args a) {
   __shared__ uint32_t slot[32];
   const RowTeam<WARP> team;
   const long long row = WARP ? (long long)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
@@ -266,8 +386,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_gate_int8(cons
       cu[j] = load_chunk<T, VEC>(u + c);
     }
   }
-  float v[N * VEC];
-  uint32_t top = 0;
+  float v[N * VEC], top = 0.0f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = (j * team.size + team.t) * VEC;
@@ -275,21 +394,66 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_gate_int8(cons
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         v[j * VEC + i] = silu_f32(to_float(cg[j].e[i])) * to_float(cu[j].e[i]);
-        top = ::max(top, __float_as_uint(v[j * VEC + i]) & 0x7fffffffu);
+        top = max_abs(top, v[j * VEC + i]);
       }
     }
   }
   float inv;
-  const float scale = row_scale(team.max(top, slot), inv);
+  const float scale = row_scale(team.max(__float_as_uint(top) & 0x7fffffffu, slot), inv);
   if (team.t == 0) a.scales[row] = scale;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = (j * team.size + team.t) * VEC;
-    if (c < hidden) {
-      Chunk<signed char, VEC> out;
+    if (c < hidden)
+      store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
+  }
+}
+
+// k_gate_int8 for many rows on 16-byte boundaries: PER elements a thread, rows through a ring
+template <class T, int PER, int MAXT>
+__global__ void __launch_bounds__(MAXT) k_gate_int8_ring(const so3lr_gate_int8_args a, int stages, int *err) {
+  constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
+  __shared__ uint32_t slot[2][32];
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int hidden = int(a.hidden), t = threadIdx.x, size = blockDim.x;
+  const uint32_t row_bytes = 2 * hidden * sizeof(T);
+  const RowRing ring(smem, row_bytes, stages, err);
+  const RowTeam<false> team;
+  const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
+  auto fetch = [&](int i) {
+    const long long row = blockIdx.x + (long long)i * gridDim.x;
+    const uint32_t dst = ring.expect(i, row_bytes);
+    tc::bulk_load(dst, static_cast<const T *>(a.gu) + row * a.gu_stride, row_bytes, ring.bar(i));
+  };
+  if (t == 0)
+    for (int i = 0; i < min(stages, rows); ++i) fetch(i);
+  for (int k = 0; k < rows; ++k) {
+    ring.wait(k);
+    const T *g = reinterpret_cast<const T *>(ring.stage(k)), *u = g + hidden;
+    float v[PER], top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out.e[i] = to_code(v[j * VEC + i], inv);
-      store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, out);
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < hidden) {
+        const Chunk<T, VEC> cg = load_chunk<T, VEC>(g + c), cu = load_chunk<T, VEC>(u + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          v[j * VEC + i] = silu_f32(to_float(cg.e[i])) * to_float(cu.e[i]);
+          top = max_abs(top, v[j * VEC + i]);
+        }
+      }
+    }
+    float inv;
+    const uint32_t bits = team.max(__float_as_uint(top) & 0x7fffffffu, slot[k & 1]);  // every thread has read the stage
+    if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
+    const float scale = row_scale(bits, inv);
+    const long long row = blockIdx.x + (long long)k * gridDim.x;
+    if (t == 0) a.scales[row] = scale;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < hidden)
+        store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
     }
   }
 }
@@ -301,12 +465,23 @@ __global__ void k_dequantize_int8(const so3lr_dequantize_int8_args a) {
        i += (long long)gridDim.x * blockDim.x) {
     const long long row = total < (1LL << 31) ? uint32_t(i) / uint32_t(per_row) : i / per_row;
     const long long c = (i - row * per_row) * VEC;
-    const float scale = a.scales[row];
     const Chunk<signed char, VEC> q = load_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c);
-    Chunk<T, VEC> out;
+    const float scale = a.scales[row];
+    T *dst = static_cast<T *>(a.out) + row * a.out_stride + c;
+    if (VEC == 16) {
+      constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) out.e[k] = from_float<T>(float(q.e[k]) * scale);
-    store_chunk<T, VEC>(static_cast<T *>(a.out) + row * a.out_stride + c, out);
+      for (int j = 0; j < VEC; j += kPer) {
+        Chunk<T, kPer> out;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          out.e[k] = from_float<T>(
+              byte_to_float(reinterpret_cast<const uint32_t *>(&q)[(j + k) / 4] ^ 0x80808080u, (j + k) % 4) * scale);
+        store_chunk<T, kPer>(dst + j, out);
+      }
+    } else {
+      dst[0] = from_float<T>(float(q.e[0]) * scale);
+    }
   }
 }
 
@@ -315,9 +490,11 @@ bool aligned(const void *p, long long stride, int size, int bytes) {
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (stride * size) % bytes == 0);
 }
 
-// Threads that hold a row of `width` elements, PER of them each: a warp where one
+// Threads that hold a row of `width` elements, `per` of them each: a warp where one
 // suffices, else a block of whole warps.
 int row_threads(long long width, int per) { return int((width + 32LL * per - 1) / (32LL * per)) * 32; }
+// Elements a thread holds: 8, or 16 where that keeps the row in one warp or in one block.
+int per_thread(long long width) { return width <= 256 || (width > 512 && width <= 8192) ? 8 : 16; }
 
 template <class F>
 void by_type(int dtype, F &&f) {
@@ -353,28 +530,65 @@ void norm_forward(const so3lr_rms_norm_args &a, cudaStream_t s) {
   SO3_LAUNCH("rms_norm");
 }
 
-int backward_blocks(long long rows, int threads) {
+// Blocks of a kernel that walks over rows
+int walking_blocks(long long rows, int threads) {
   const bool warp = threads == 32;
   const long long want = warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
-  const int per_sm = warp ? 4 : std::max(1, std::min(8, 1024 / threads));
+  const int per_sm = warp ? 4 : std::max(1, std::min(4, 1536 / threads));
   return int(std::min<long long>(want, (long long)kSmCount * per_sm));
 }
 
+// Ring of a kernel that walks over rows: two blocks an SM, shared memory for up to
+// kRingStages rows. stages < 2: the row is too long.
+struct RingPlan {
+  int grid, stages, smem;
+};
+RingPlan ring_plan(long long rows, long long row_bytes) {
+  const long long room = 110 * 1024 - kRingHeader;
+  RingPlan p;
+  p.grid = int(std::min<long long>(rows, 2LL * kSmCount));
+  p.stages = int(std::min<long long>(kRingStages, room / row_bytes));
+  p.smem = int(kRingHeader + p.stages * row_bytes);
+  return p;
+}
+// The ring kernel's blocks, 0 where the direct loads serve: rows of a warp, unaligned
+// rows, and rows too long for the ring
+RingPlan backward_ring(const so3lr_rms_norm_backward_args &a) {
+  const int e = a.dtype == SO3LR_FLOAT32 ? 4 : 2;
+  const bool wide = a.width * e % 16 == 0 && aligned(a.dy, a.dy_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
+                    aligned(a.ds, a.ds_stride, e, 16) && aligned(a.dx, a.dx_stride, e, 16) &&
+                    aligned(a.weight, 0, 1, 16);
+  if (!wide || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
+  const RingPlan p = ring_plan(a.rows, 3 * a.width * e);
+  return p.stages < 2 ? RingPlan{0, 0, 0} : p;
+}
+int backward_parts(const so3lr_rms_norm_backward_args &a) {
+  const RingPlan r = backward_ring(a);
+  return r.stages ? r.grid : walking_blocks(a.rows, row_threads(a.width, per_thread(a.width)));
+}
+
 template <class T, class W, int VEC, int N>
-void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, cudaStream_t s) {
+void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int grid, cudaStream_t s) {
   const int threads = row_threads(a.width, VEC * N);
-  const int grid = backward_blocks(a.rows, threads);
-  if (grid > 0) {
-    if (threads == 32)
-      k_rms_norm_backward<T, W, VEC, N, true>
-          <<<grid, 32 * kWarpRows, kWarpRows * a.width * sizeof(float), s>>>(a, partial);
-    else
-      k_rms_norm_backward<T, W, VEC, N, false><<<grid, threads, 0, s>>>(a, partial);
-    SO3_LAUNCH("rms_norm_backward");
-  }
-  k_column_sum<W><<<unsigned((a.width + 31) / 32), dim3(32, 32), 0, s>>>(grid, int(a.width), partial,
-                                                                        static_cast<W *>(a.dweight));
-  SO3_LAUNCH("column_sum");
+  if (threads == 32)
+    k_rms_norm_backward<T, W, VEC, N, 32 * kWarpRows>
+        <<<grid, 32 * kWarpRows, kWarpRows * a.width * sizeof(float), s>>>(a, partial);
+  else if (threads <= 512)
+    k_rms_norm_backward<T, W, VEC, N, 512><<<grid, threads, 0, s>>>(a, partial);
+  else
+    k_rms_norm_backward<T, W, VEC, N, 1024><<<grid, threads, 0, s>>>(a, partial);
+  SO3_LAUNCH("rms_norm_backward");
+}
+template <class T, class W>
+void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, const RingPlan &r, cudaStream_t s) {
+  check_gave_up();
+  const int threads = row_threads(a.width, 16);
+  auto run = [&](auto fn) {
+    allow_dynamic_smem(reinterpret_cast<const void *>(fn), 227 * 1024 - 1024);
+    fn<<<r.grid, threads, r.smem, s>>>(a, partial, r.stages, gave_up_flag());
+  };
+  run(&k_rms_norm_backward_ring<T, W>);
+  SO3_LAUNCH("rms_norm_backward_ring");
 }
 
 template <class T, int VEC, int N>
@@ -385,6 +599,21 @@ void gate(const so3lr_gate_int8_args &a, cudaStream_t s) {
   else
     k_gate_int8<T, VEC, N, false><<<unsigned(a.rows), threads, 0, s>>>(a);
   SO3_LAUNCH("gate_int8");
+}
+int ring_per_thread(long long hidden) { return hidden <= 4096 ? 16 : 32; }
+template <class T>
+void gate_ring(const so3lr_gate_int8_args &a, const RingPlan &r, cudaStream_t s) {
+  check_gave_up();
+  const int threads = row_threads(a.hidden, ring_per_thread(a.hidden));
+  auto run = [&](auto fn) {
+    allow_dynamic_smem(reinterpret_cast<const void *>(fn), 227 * 1024 - 1024);
+    fn<<<r.grid, threads, r.smem, s>>>(a, r.stages, gave_up_flag());
+  };
+  if (ring_per_thread(a.hidden) == 16)
+    run(&k_gate_int8_ring<T, 16, 256>);
+  else
+    run(&k_gate_int8_ring<T, 32, 512>);
+  SO3_LAUNCH("gate_int8_ring");
 }
 
 }  // namespace
@@ -400,16 +629,16 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
                         aligned(a.residual, a.residual_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
                         aligned(a.y, a.y_stride, e, 16) && aligned(a.codes, a.codes_stride, 1, V) &&
                         aligned(a.weight, 0, 1, 16);
-      if (!wide)
-        norm_forward<T, W, 1, kPerThread>(a, s);
+      if (per_thread(a.width) == 8)
+        wide ? norm_forward<T, W, V, 8 / V>(a, s) : norm_forward<T, W, 1, 8>(a, s);
       else
-        norm_forward<T, W, V, kPerThread / V>(a, s);
+        wide ? norm_forward<T, W, V, 16 / V>(a, s) : norm_forward<T, W, 1, 16>(a, s);
     });
   });
 }
 
 long long rms_norm_backward_bytes(const so3lr_rms_norm_backward_args &a) {
-  return (long long)backward_blocks(a.rows, row_threads(a.width, kPerThread)) * a.width * 4;
+  return (long long)backward_parts(a) * a.width * 4;
 }
 
 void launch_rms_norm_backward(const so3lr_rms_norm_backward_args &a, void *workspace, cudaStream_t s) {
@@ -423,10 +652,20 @@ void launch_rms_norm_backward(const so3lr_rms_norm_backward_args &a, void *works
                         aligned(a.ds, a.ds_stride, e, 16) && aligned(a.dx, a.dx_stride, e, 16) &&
                         aligned(a.weight, 0, 1, 16);
       float *partial = static_cast<float *>(workspace);
-      if (!wide)
-        norm_backward<T, W, 1, kPerThread>(a, partial, s);
-      else
-        norm_backward<T, W, V, kPerThread / V>(a, partial, s);
+      const RingPlan r = backward_ring(a);
+      const int parts = backward_parts(a);
+      if (parts > 0) {
+        if (r.stages)
+          norm_backward_ring<T, W>(a, partial, r, s);
+        else if (per_thread(a.width) == 8)
+          wide ? norm_backward<T, W, V, 8 / V>(a, partial, parts, s) : norm_backward<T, W, 1, 8>(a, partial, parts, s);
+        else
+          wide ? norm_backward<T, W, V, 16 / V>(a, partial, parts, s)
+               : norm_backward<T, W, 1, 16>(a, partial, parts, s);
+      }
+      k_column_sum<W><<<unsigned((a.width + 31) / 32), dim3(32, 32), 0, s>>>(parts, int(a.width), partial,
+                                                                            static_cast<W *>(a.dweight));
+      SO3_LAUNCH("column_sum");
     });
   });
 }
@@ -438,12 +677,17 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s) {
     const int e = sizeof(T);
     const bool wide = a.hidden % V == 0 && aligned(a.gu, a.gu_stride, e, 16) && aligned(a.codes, a.codes_stride, 1, V);
     // up to 32 elements per thread: 32768 columns in a block of 1,024 threads
-    if (!wide)
-      gate<T, 1, 32>(a, s);
-    else if (a.hidden <= 1024 * kPerThread)
-      gate<T, V, kPerThread / V>(a, s);
+    const int per = a.hidden > 16384 ? 32 : per_thread(a.hidden);
+    // the ring where a block has several rows to walk over, and a row needs a block
+    const RingPlan r = ring_plan(a.rows, 2 * a.hidden * e);
+    if (wide && a.hidden > 512 && a.hidden <= 16384 && r.stages >= 2 && a.rows > 2 * r.grid)
+      gate_ring<T>(a, r, s);
+    else if (per == 32)
+      wide ? gate<T, V, 32 / V>(a, s) : gate<T, 1, 32>(a, s);
+    else if (per == 8)
+      wide ? gate<T, V, 8 / V>(a, s) : gate<T, 1, 8>(a, s);
     else
-      gate<T, V, 32 / V>(a, s);
+      wide ? gate<T, V, 16 / V>(a, s) : gate<T, 1, 16>(a, s);
   });
 }
 
@@ -451,11 +695,12 @@ void launch_dequantize_int8(const so3lr_dequantize_int8_args &a, cudaStream_t s)
   by_type(a.dtype, [&](auto t) {
     using T = decltype(t);
     const int e = sizeof(T);
-    const bool wide = a.width % 8 == 0 && aligned(a.codes, a.codes_stride, 1, 8) && aligned(a.out, a.out_stride, e, 16);
-    const long long total = a.rows * (wide ? a.width / 8 : a.width);
+    const bool wide =
+        a.width % 16 == 0 && aligned(a.codes, a.codes_stride, 1, 16) && aligned(a.out, a.out_stride, e, 16);
+    const long long total = a.rows * (wide ? a.width / 16 : a.width);
     const unsigned grid = unsigned(std::min<long long>((total + 255) / 256, kSmCount * 64));
     if (wide)
-      k_dequantize_int8<T, 8><<<grid, 256, 0, s>>>(a);
+      k_dequantize_int8<T, 16><<<grid, 256, 0, s>>>(a);
     else
       k_dequantize_int8<T, 1><<<grid, 256, 0, s>>>(a);
     SO3_LAUNCH("dequantize_int8");

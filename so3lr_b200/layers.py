@@ -25,6 +25,7 @@ There is no CPU path: a tensor that is not on a GPU is refused.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -81,64 +82,80 @@ class _FeedForwardBackward(C.Structure):
                 ("dw_gate", _p), ("dw_up", _p), ("dw_down", _p)]
 
 
-_LIB = None
 _ERR_BYTES = 1024
+_LOCAL = threading.local()  # a message buffer for each thread
+_CALLS: dict = {}
 
 
 def _lib():
-    global _LIB
-    if _LIB is None:
-        lib = load_library()
+    lib = load_library()
+    if not _CALLS:
         plain = {"so3lr_rms_norm": _RmsNorm, "so3lr_gate_int8": _GateInt8, "so3lr_dequantize_int8": _DequantizeInt8}
         scratch = {"so3lr_rms_norm_backward": _RmsNormBackward, "so3lr_int8_linear": _Int8Linear,
                    "so3lr_feed_forward": _FeedForward, "so3lr_feed_forward_backward": _FeedForwardBackward}
+        calls = {}
         for name, args in plain.items():
-            getattr(lib, name).argtypes = [C.POINTER(args), _p, _p, C.c_size_t]
+            calls[args] = getattr(lib, name), None
+            calls[args][0].argtypes = [C.POINTER(args), _p, _p, C.c_size_t]
         for name, args in scratch.items():
-            getattr(lib, name).argtypes = [C.POINTER(args), _p, _ll, _p, _p, C.c_size_t]
-            size = getattr(lib, name + "_workspace")
-            size.argtypes, size.restype = [C.POINTER(args)], _ll
-        _LIB = lib
-    return _LIB
+            calls[args] = getattr(lib, name), getattr(lib, name + "_workspace")
+            calls[args][0].argtypes = [C.POINTER(args), _p, _ll, _p, _p, C.c_size_t]
+            calls[args][1].argtypes, calls[args][1].restype = [C.POINTER(args)], _ll
+        _CALLS.update(calls)
+    return lib
 
 
-def _queue(name: str, args, device: torch.device, scratch: bool = False) -> None:
-    """One C call on the current stream of `device`, made this thread's device for it."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _queue(name, args, device, scratch)
-    lib = _lib()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    err = C.create_string_buffer(_ERR_BYTES)
-    if scratch:
-        need = getattr(lib, name + "_workspace")(args)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-        rc = getattr(lib, name)(args, ws.data_ptr() if need > 0 else None, max(need, 0), stream, err, _ERR_BYTES)
+# the current stream's handle without the Stream object that torch.cuda.current_stream makes (2 us)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _queue(args, like: torch.Tensor) -> None:
+    """The C call of `args` on the current stream of like's device, made this thread's device for it."""
+    index = like.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _queue(args, like)
+    try:
+        call, size = _CALLS[type(args)]
+        err = _LOCAL.err
+    except (KeyError, AttributeError):
+        _lib()
+        call, size = _CALLS[type(args)]
+        err = _LOCAL.err = C.create_string_buffer(_ERR_BYTES)
+    if size is None:
+        rc = call(args, _raw_stream(index), err, _ERR_BYTES)
     else:
-        rc = getattr(lib, name)(args, stream, err, _ERR_BYTES)
+        need = size(args)
+        if need > 0:
+            ws = like.new_empty(need, dtype=torch.uint8)
+            rc = call(args, ws.data_ptr(), need, _raw_stream(index), err, _ERR_BYTES)
+        else:
+            rc = call(args, None, 0, _raw_stream(index), err, _ERR_BYTES)
     if rc != 0:
         raise So3lrError(err.value.decode(errors="replace") or f"status {rc}")
 
 
-def _rows(t: torch.Tensor, what: str, device=None, dtype=None, width=None, rows=None) -> torch.Tensor:
+def _rows(t: torch.Tensor, what: str, like=None, dtype=None, width=None, rows=None) -> torch.Tensor:
     """`t` as a 2-D view of rows with a contiguous last dimension, checked."""
     if not isinstance(t, torch.Tensor) or t.dim() < 1:
         raise ValueError(f"{what} must be a tensor with at least one dimension")
     if not t.is_cuda:
         raise ValueError(f"{what} must be on a CUDA device, got {t.device} (there is no CPU path)")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the other tensors are on {device}")
+    if like is not None and t.get_device() != like.get_device():
+        raise ValueError(f"{what} is on {t.device}, the other tensors are on {like.device}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
     if t.dim() != 2:
         t = t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2) if t.is_contiguous() else _fold(t, what)
-    if width is not None and t.shape[1] != width:
-        raise ValueError(f"{what} must have rows of {width} elements, got {t.shape[1]}")
-    if rows is not None and t.shape[0] != rows:
-        raise ValueError(f"{what} must have {rows} rows, got {t.shape[0]}")
-    if t.shape[1] < 1:
+    n, w = t.shape
+    if width is not None and w != width:
+        raise ValueError(f"{what} must have rows of {width} elements, got {w}")
+    if rows is not None and n != rows:
+        raise ValueError(f"{what} must have {rows} rows, got {n}")
+    if w < 1:
         raise ValueError(f"{what} must have rows of at least one element")
-    if t.stride(1) != 1 and t.shape[1] != 1:
+    if t.stride(1) != 1 and w != 1:
         raise ValueError(f"{what} must have a contiguous last dimension")
     return t
 
@@ -155,25 +172,28 @@ def _dense_rows(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _vector(t: torch.Tensor, what: str, device, dtypes, length: int) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.shape[0] != length or t.device != device:
-        raise ValueError(f"{what} must be a 1-D tensor of {length} elements on {device}")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{what} must be one of {', '.join(map(str, dtypes))}, got {t.dtype}")
+def _vector(t: torch.Tensor, what: str, like, dtype, length: int, or_dtype=None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.shape != (length,) or t.get_device() != like.get_device():
+        raise ValueError(f"{what} must be a 1-D tensor of {length} elements on {like.device}")
+    if t.dtype != dtype and t.dtype != or_dtype:
+        raise ValueError(f"{what} must be {dtype}{f' or {or_dtype}' if or_dtype else ''}, got {t.dtype}")
     if length > 1 and t.stride(0) != 1:
         raise ValueError(f"{what} must be contiguous")
     return t
 
 
 def _type_of(t: torch.Tensor, what: str, types=_TYPES) -> int:
-    if t.dtype not in types:
+    code = types.get(t.dtype)
+    if code is None:
         raise ValueError(f"{what} must be one of {', '.join(map(str, types))}, got {t.dtype}")
-    return types[t.dtype]
+    return code
 
 
-def _codes_like(rows: int, width: int, device) -> torch.Tensor:
+def _codes_like(like: torch.Tensor, rows: int, width: int) -> torch.Tensor:
     """8-bit rows that start on 16-byte boundaries, as int8_linear reads them without a copy."""
-    return torch.empty((rows, (width + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :width]
+    if width % 16 == 0:
+        return like.new_empty((rows, width), dtype=torch.int8)
+    return like.new_empty((rows, (width + 15) // 16 * 16), dtype=torch.int8)[:, :width]
 
 
 def _shaped(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
@@ -184,29 +204,26 @@ def _shaped(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
 def _norm(x, weight, residual, eps, quantize):
     x2 = _rows(x, "x")
     rows, width = x2.shape
-    dev = x2.device
     t = _type_of(x2, "x")
-    weight = _vector(weight, "weight", dev, (x2.dtype, torch.float32), width)
-    if residual is None:
-        r2 = s = None
-    else:
+    _vector(weight, "weight", x2, x2.dtype, width, torch.float32)
+    r_ptr, r_stride, s, s_ptr = None, 0, x, None
+    if residual is not None:
         if residual.shape != x.shape:
             raise ValueError(f"residual must have the shape of x, {tuple(x.shape)}, got {tuple(residual.shape)}")
-        r2 = _rows(residual, "residual", dev, x2.dtype, width, rows)
-        s = torch.empty((rows, width), dtype=x2.dtype, device=dev)
-    a = _RmsNorm(rows, width, t, _TYPES[weight.dtype], eps, x2.data_ptr(), x2.stride(0))
-    a.weight = weight.data_ptr()
-    if s is not None:
-        a.residual, a.residual_stride, a.s, a.s_stride = r2.data_ptr(), r2.stride(0), s.data_ptr(), width
+        r2 = _rows(residual, "residual", x2, x2.dtype)
+        s = x2.new_empty((rows, width))
+        r_ptr, r_stride, s_ptr = r2.data_ptr(), r2.stride(0), s.data_ptr()
+        s = _shaped(s, x)
     if quantize:
-        y, scales = _codes_like(rows, width, dev), torch.empty(rows, dtype=torch.float32, device=dev)
-        a.codes, a.codes_stride, a.scales = y.data_ptr(), y.stride(0), scales.data_ptr()
+        y, scales = _codes_like(x2, rows, width), x2.new_empty(rows, dtype=torch.float32)
+        out = (None, 0, y.data_ptr(), y.stride(0), scales.data_ptr())
     else:
-        y, scales = torch.empty((rows, width), dtype=x2.dtype, device=dev), None
-        a.y, a.y_stride = y.data_ptr(), width
+        y, scales = x2.new_empty((rows, width)), None
+        out = (y.data_ptr(), width, None, 0, None)
     if rows:
-        _queue("so3lr_rms_norm", a, dev)
-    return y, scales, x if s is None else _shaped(s, x)
+        _queue(_RmsNorm(rows, width, t, _TYPES[weight.dtype], eps, x2.data_ptr(), x2.stride(0), r_ptr, r_stride,
+                        weight.data_ptr(), s_ptr, width, *out), x2)
+    return y, scales, s
 
 
 class _NormFunction(torch.autograd.Function):
@@ -249,18 +266,16 @@ def rms_norm_backward(dy, s, weight, ds=None, *, eps: float = 1e-6):
     of s; dx is also the residual's gradient."""
     s2 = _rows(s, "s")
     rows, width = s2.shape
-    dev = s2.device
     t = _type_of(s2, "s")
-    weight = _vector(weight, "weight", dev, (s2.dtype, torch.float32), width)
-    d2 = _rows(dy, "dy", dev, s2.dtype, width, rows)
-    dx = torch.empty((rows, width), dtype=s2.dtype, device=dev)
-    dw = torch.empty(width, dtype=weight.dtype, device=dev)
-    a = _RmsNormBackward(rows, width, t, _TYPES[weight.dtype], eps, d2.data_ptr(), d2.stride(0), s2.data_ptr(),
-                         s2.stride(0), weight.data_ptr(), None, 0, dx.data_ptr(), width, dw.data_ptr())
+    _vector(weight, "weight", s2, s2.dtype, width, torch.float32)
+    d2 = _rows(dy, "dy", s2, s2.dtype, width, rows)
+    e_ptr, e_stride = None, 0
     if ds is not None:
-        e2 = _rows(ds, "ds", dev, s2.dtype, width, rows)
-        a.ds, a.ds_stride = e2.data_ptr(), e2.stride(0)
-    _queue("so3lr_rms_norm_backward", a, dev, scratch=True)
+        e2 = _rows(ds, "ds", s2, s2.dtype, width, rows)
+        e_ptr, e_stride = e2.data_ptr(), e2.stride(0)
+    dx, dw = s2.new_empty((rows, width)), torch.empty_like(weight)
+    _queue(_RmsNormBackward(rows, width, t, _TYPES[weight.dtype], eps, d2.data_ptr(), d2.stride(0), s2.data_ptr(),
+                            s2.stride(0), weight.data_ptr(), e_ptr, e_stride, dx.data_ptr(), width, dw.data_ptr()), s2)
     return _shaped(dx, s), dw
 
 
@@ -270,23 +285,22 @@ def int8_linear(a, a_scales, b, b_scales, bias=None, *, out_dtype=torch.bfloat16
     [..., k] and b [n, k] int8, scales and bias float32, y [..., n] of out_dtype."""
     a2 = _rows(a, "a", dtype=torch.int8)
     rows, k = a2.shape
-    dev = a2.device
-    b2 = _rows(b, "b", dev, torch.int8, k)
+    b2 = _rows(b, "b", a2, torch.int8, k)
     n = b2.shape[0]
-    if out_dtype not in _TYPES:
+    t = _TYPES.get(out_dtype)
+    if t is None:
         raise ValueError(f"out_dtype must be one of {', '.join(map(str, _TYPES))}, got {out_dtype}")
-    a_scales = _vector(a_scales, "a_scales", dev, (torch.float32,), rows)
-    b_scales = _vector(b_scales, "b_scales", dev, (torch.float32,), n)
+    _vector(a_scales, "a_scales", a2, torch.float32, rows)
+    _vector(b_scales, "b_scales", a2, torch.float32, n)
     if bias is not None:
-        bias = _vector(bias, "bias", dev, (torch.float32,), n)
+        _vector(bias, "bias", a2, torch.float32, n)
     if n < 1:
         raise ValueError("b must have at least one row")
-    y = torch.empty((rows, n), dtype=out_dtype, device=dev)
+    y = a2.new_empty((rows, n), dtype=out_dtype)
     if rows:
-        _queue("so3lr_int8_linear",
-               _Int8Linear(rows, n, k, _TYPES[out_dtype], a2.data_ptr(), a2.stride(0), a_scales.data_ptr(),
-                           b2.data_ptr(), b2.stride(0), b_scales.data_ptr(),
-                           None if bias is None else bias.data_ptr(), y.data_ptr(), n), dev, scratch=True)
+        _queue(_Int8Linear(rows, n, k, t, a2.data_ptr(), a2.stride(0), a_scales.data_ptr(), b2.data_ptr(),
+                           b2.stride(0), b_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                           y.data_ptr(), n), a2)
     return _shaped(y, a)
 
 
@@ -297,11 +311,10 @@ def gate_int8(gu):
     rows, width = x.shape
     if width % 2:
         raise ValueError(f"gu must hold g and u side by side: an even width, got {width}")
-    codes = _codes_like(rows, width // 2, x.device)
-    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    codes, scales = _codes_like(x, rows, width // 2), x.new_empty(rows, dtype=torch.float32)
     if rows:
-        _queue("so3lr_gate_int8", _GateInt8(rows, width // 2, t, x.data_ptr(), x.stride(0), codes.data_ptr(),
-                                            codes.stride(0), scales.data_ptr()), x.device)
+        _queue(_GateInt8(rows, width // 2, t, x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0),
+                         scales.data_ptr()), x)
     return codes, scales
 
 
@@ -309,13 +322,13 @@ def dequantize_int8(codes, scales, dtype=torch.bfloat16):
     """codes * scales[:, None], rounded to dtype."""
     c = _rows(codes, "codes", dtype=torch.int8)
     rows, width = c.shape
-    if dtype not in _TYPES:
+    t = _TYPES.get(dtype)
+    if t is None:
         raise ValueError(f"dtype must be one of {', '.join(map(str, _TYPES))}, got {dtype}")
-    scales = _vector(scales, "scales", c.device, (torch.float32,), rows)
-    out = torch.empty((rows, width), dtype=dtype, device=c.device)
+    _vector(scales, "scales", c, torch.float32, rows)
+    out = c.new_empty((rows, width), dtype=dtype)
     if rows:
-        _queue("so3lr_dequantize_int8", _DequantizeInt8(rows, width, _TYPES[dtype], c.data_ptr(), c.stride(0),
-                                                        scales.data_ptr(), out.data_ptr(), width), c.device)
+        _queue(_DequantizeInt8(rows, width, t, c.data_ptr(), c.stride(0), scales.data_ptr(), out.data_ptr(), width), c)
     return _shaped(out, codes)
 
 
@@ -326,7 +339,7 @@ def quantize_weight(w):
     _type_of(w2, "w")
     f = w2.detach().float()
     scales = f.abs().amax(1) / 127.0
-    codes = _codes_like(w2.shape[0], w2.shape[1], w2.device)
+    codes = _codes_like(w2, *w2.shape)
     codes.copy_(torch.round(f / torch.where(scales > 0, scales, 1.0)[:, None]).clamp_(-127, 127))
     return codes, scales
 
@@ -335,26 +348,24 @@ def quantize_weight(w):
 def _ffn_operands(x, w_gate, w_up, w_down):
     x2 = _rows(x, "x")
     t = _type_of(x2, "x", _HALF)
-    width, dev = x2.shape[1], x2.device
-    g = _rows(w_gate, "w_gate", dev, x2.dtype, width)
+    width, dtype = x2.shape[1], x2.dtype
+    g = _rows(w_gate, "w_gate", x2, dtype, width)
     hidden = g.shape[0]
     if hidden < 1:
         raise ValueError("w_gate must have at least one row")
-    u = _rows(w_up, "w_up", dev, x2.dtype, width, hidden)
-    d = _rows(w_down, "w_down", dev, x2.dtype, hidden, width)
-    return x2, g, u, d, t, hidden
+    u = _rows(w_up, "w_up", x2, dtype, width, hidden)
+    d = _rows(w_down, "w_down", x2, dtype, hidden, width)
+    return x2, t, hidden, (x2.data_ptr(), x2.stride(0), g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0),
+                           d.data_ptr(), d.stride(0))
 
 
 def _ffn(x, w_gate, w_up, w_down, keep=False):
-    x2, g, u, d, t, hidden = _ffn_operands(x, w_gate, w_up, w_down)
+    x2, t, hidden, operands = _ffn_operands(x, w_gate, w_up, w_down)
     rows, width = x2.shape
-    y = torch.empty((rows, width), dtype=x2.dtype, device=x2.device)
-    h = torch.empty((rows, hidden), dtype=x2.dtype, device=x2.device) if keep else None
+    y = x2.new_empty((rows, width))
+    h = x2.new_empty((rows, hidden)) if keep else None
     if rows:
-        _queue("so3lr_feed_forward",
-               _FeedForward(rows, width, hidden, t, x2.data_ptr(), x2.stride(0), g.data_ptr(), g.stride(0),
-                            u.data_ptr(), u.stride(0), d.data_ptr(), d.stride(0), y.data_ptr(), width,
-                            h.data_ptr() if keep else None), x2.device, scratch=True)
+        _queue(_FeedForward(rows, width, hidden, t, *operands, y.data_ptr(), width, h.data_ptr() if keep else None), x2)
     return _shaped(y, x), h
 
 
@@ -389,21 +400,15 @@ def feed_forward_train(x, w_gate, w_up, w_down):
 def feed_forward_backward(dy, saved):
     """(dx, dw_gate, dw_up, dw_down) for the gradient dy of feed_forward_train's y."""
     x, w_gate, w_up, w_down, h = saved
-    x2, g, u, d, t, hidden = _ffn_operands(x, w_gate, w_up, w_down)
+    x2, t, hidden, operands = _ffn_operands(x, w_gate, w_up, w_down)
     rows, width = x2.shape
-    dev = x2.device
-    d2 = _rows(dy, "dy", dev, x2.dtype, width, rows)
+    d2 = _rows(dy, "dy", x2, x2.dtype, width, rows)
     if h.shape != (rows, hidden) or h.dtype != x2.dtype or not h.is_contiguous():
         raise ValueError("saved does not come from feed_forward_train")
-    dx = torch.empty((rows, width), dtype=x2.dtype, device=dev)
-    dwg = torch.empty((hidden, width), dtype=x2.dtype, device=dev)
-    dwu = torch.empty((hidden, width), dtype=x2.dtype, device=dev)
-    dwd = torch.empty((width, hidden), dtype=x2.dtype, device=dev)
-    _queue("so3lr_feed_forward_backward",
-           _FeedForwardBackward(rows, width, hidden, t, d2.data_ptr(), d2.stride(0), x2.data_ptr(), x2.stride(0),
-                                g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0), d.data_ptr(), d.stride(0),
-                                h.data_ptr(), dx.data_ptr(), width, dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr()),
-           dev, scratch=True)
+    dx = x2.new_empty((rows, width))
+    dwg, dwu, dwd = x2.new_empty((hidden, width)), x2.new_empty((hidden, width)), x2.new_empty((width, hidden))
+    _queue(_FeedForwardBackward(rows, width, hidden, t, d2.data_ptr(), d2.stride(0), *operands, h.data_ptr(),
+                                dx.data_ptr(), width, dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr()), x2)
     return _shaped(dx, x), dwg, dwu, dwd
 
 
