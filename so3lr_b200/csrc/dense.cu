@@ -7,7 +7,7 @@
 // tile's columns) per K block of 128 bytes, six blocks deep, with TMA into
 // 128-byte-swizzled tiles. Against one CTA per 128 x 256 tile this reads a third
 // less from L2 per product, which is what bounds a tile loop at this size.
-// Warp 0 loads, warp 1 of the leader issues the MMAs, warps 2-9 read the
+// Warp 0 loads, warp 1 of the leader issues the MMAs, warps 2-17 read the
 // accumulators (TMEM lane = row) and write the results; two accumulator buffers of
 // 256 columns, so that a tile's epilogue runs under the next tile's MMAs.
 //
@@ -29,10 +29,10 @@ namespace {
 
 constexpr int kPairs = kSmCount / 2;
 constexpr int kTileM = 256, kTileN = 256;   // of a CTA pair
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;  // four a scheduler: with two the epilogue's latencies show
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr uint32_t kOperand = 128 * 128;    // 128 rows of 128 bytes: one operand tile of a CTA, 16 KB
-constexpr uint32_t kStaging = 4096;         // of an epilogue warp: 32 rows x 32 values
+constexpr uint32_t kStaging = 2048;         // of an epilogue warp: 32 rows x 64 bytes
 constexpr int kBarBytes = 256;
 constexpr int kMaxMaps = 6, kMaxProblems = 3, kMaxStages = 6;
 
@@ -97,47 +97,40 @@ __device__ __forceinline__ Item item_of(const Params &p, int it) {
   return w;
 }
 
-// 32 values of each of the warp's 32 rows (lane = row) to C through the warp's
-// staging, which turns them into stores of whole 64- or 128-byte row segments.
-// 16-byte pieces of a staged row are permuted with the row: no bank conflicts.
+// 64 bytes of each of the warp's 32 rows (lane = row) to C through the warp's staging,
+// which turns them into stores of whole row segments. The 16-byte pieces of a staged
+// row are permuted with the row: no bank conflicts either way. `cols`: columns left
+// in the row from c on; `wide`: the rows of C start on 16-byte boundaries.
 template <class O>
-__device__ __forceinline__ void store32(unsigned char *stage, int lane, const float (&v)[32], O *c, long long ldc,
-                                        int rows, int cols, bool wide) {
-  constexpr int kPer = 16 / sizeof(O), kPieces = 32 / kPer;  // 4 pieces of 16-bit values, 8 of 32-bit ones
-  const int row_bytes = 32 * sizeof(O);
+__device__ __forceinline__ void store_rows(unsigned char *stage, int lane, const Chunk<O, 16 / sizeof(O)> (&v)[4],
+                                           O *c, long long ldc, int rows, int cols, bool wide) {
+  constexpr int kPer = 16 / sizeof(O);
   auto slot = [&](int r, int piece) {
-    return stage + r * row_bytes + 16 * (piece ^ (sizeof(O) == 2 ? (r >> 1) & 3 : r & 7));
+    return reinterpret_cast<O *>(stage + 64 * r + 16 * (piece ^ ((r >> 1) & 3)));
   };
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    Chunk<O, kPer> out;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) out.e[j] = from_float<O>(v[i * kPer + j]);
-    store_chunk<O, kPer>(reinterpret_cast<O *>(slot(lane, i)), out);
-  }
+  for (int i = 0; i < 4; ++i) store_chunk<O, kPer>(slot(lane, i), v[i]);
   __syncwarp();
-  const int piece = lane % kPieces;
+  const int piece = lane & 3, left = cols - piece * kPer;
+  c += (lane >> 2) * ldc + piece * kPer;
+  if (wide && left >= kPer) {
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int r = i * (32 / kPieces) + lane / kPieces;
-    const Chunk<O, kPer> out = load_chunk<O, kPer>(reinterpret_cast<const O *>(slot(r, piece)));
-    if (r < rows) {
-      O *dst = c + r * ldc + piece * kPer;
-      const int left = cols - piece * kPer;
-      if (wide && left >= kPer)
-        store_chunk<O, kPer>(dst, out);
-      else
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (j < left) dst[j] = out.e[j];
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (r < rows) store_chunk<O, kPer>(c + 8 * i * ldc, load_chunk<O, kPer>(slot(r, piece)));
+    }
+  } else if (left > 0) {
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (r < rows)
+        for (int j = 0; j < min(left, kPer); ++j) c[8 * i * ldc + j] = slot(r, piece)[j];
     }
   }
   __syncwarp();
 }
-
-__device__ __forceinline__ void to_floats(const uint32_t (&r)[32], float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+template <class O, int N>
+__device__ __forceinline__ void put(Chunk<O, N> &chunk, int i, float v) {
+  chunk.e[i] = from_float<O>(v);
 }
 
 template <int MODE, class T, bool A_MN, bool B_MN>
@@ -285,7 +278,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue
-    const int quad = warp & 3, half = (warp - 2) >> 2;
+    // warp: TMEM lanes 32 (warp % 4) .. + 31, a quarter of the columns
+    const int quad = warp & 3, part = (warp - 2) >> 2;
     unsigned char *stage = staging + (warp - 2) * kStaging;
     const uint32_t lanes = tmem + (uint32_t(32 * quad) << 16);
     int done = 0;
@@ -303,75 +297,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
         if (lane == 0) tc::mbar_arrive_cluster(tc::at_leader(acc_empty(buf)));
       };
       const int row0 = w.m0 + 128 * rank + 32 * quad, rows = min(32, q.m - row0);
+      constexpr int kPer = 16 / sizeof(T);
+      const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % 16 == 0;
       if (MODE == kPlain || MODE == kInt8) {
         const bool split = q.splits > 1;
         const float sa = MODE == kInt8 && !split && lane < rows ? p.a_scales[row0 + lane] : 0.0f;
-        const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % 16 == 0;
-        for (int j = 0; j < 4; ++j) {
-          const int col = 128 * half + 32 * j, c0 = w.n0 + col;
+        for (int j = 0; j < 2; ++j) {
+          const int col = 64 * part + 32 * j, c0 = w.n0 + col;
           uint32_t r[32];
           tc::tmem_ld32(acc + col, r);
           tc::wait_ld(r);
-          if (j == 3) release();
+          if (j == 1) release();
           if (rows <= 0 || c0 >= q.n) continue;
-          float v[32];
-          if (split) {
-            to_floats(r, v);  // raw 32-bit sums, float or int
-            store32<float>(stage, lane, v,
-                           reinterpret_cast<float *>(p.partial) + q.partial + ((long long)w.split * q.m + row0) * q.ldp + c0,
-                           q.ldp, rows, q.n - c0, true);
+          if (split) {  // raw 32-bit sums, float or int
+            uint32_t *dst = p.partial + q.partial + ((long long)w.split * q.m + row0) * q.ldp + c0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              Chunk<float, 4> v[4];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i / 4].e[i % 4] = __uint_as_float(r[16 * h + i]);
+              store_rows<float>(stage, lane, v, reinterpret_cast<float *>(dst) + 16 * h, q.ldp, rows,
+                                q.n - c0 - 16 * h, true);
+            }
             continue;
           }
-          if (MODE == kInt8) {
-            const bool live = c0 + lane < q.n;
-            const float sb = live ? p.b_scales[c0 + lane] : 0.0f, bias = live && p.bias ? p.bias[c0 + lane] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float s = __shfl_sync(0xffffffffu, sb, i), t = __shfl_sync(0xffffffffu, bias, i);
-              v[i] = fmaf(float(int(r[i])) * sa, s, t);
-            }
-          } else {
-            to_floats(r, v);
+          float sb = 0.0f, bias = 0.0f;
+          if (MODE == kInt8 && c0 + lane < q.n) {
+            sb = p.b_scales[c0 + lane];
+            bias = p.bias ? p.bias[c0 + lane] : 0.0f;
           }
-          store32<T>(stage, lane, v, static_cast<T *>(q.c) + row0 * q.ldc + c0, q.ldc, rows, q.n - c0, wide);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // 32 columns of 2 bytes, or twice 16 of 4
+            constexpr int kCols = 4 * kPer;
+            if (h * kCols >= 32) break;
+            Chunk<T, kPer> v[4];
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) {
+              const int k = (h * kCols + i) % 32;
+              float f = __uint_as_float(r[k]);
+              if (MODE == kInt8)
+                f = fmaf(float(int(r[k])) * sa, __shfl_sync(0xffffffffu, sb, k), __shfl_sync(0xffffffffu, bias, k));
+              put(v[i / kPer], i % kPer, f);
+            }
+            store_rows<T>(stage, lane, v, static_cast<T *>(q.c) + row0 * q.ldc + c0 + h * kCols, q.ldc, rows,
+                          q.n - c0 - h * kCols, wide);
+          }
         }
       } else {
-        const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % 16 == 0;
-        for (int j = 0; j < 2; ++j) {
-          const int col = 64 * half + 32 * j, c0 = w.n0 + col;
-          uint32_t g[32], u[32];
-          tc::tmem_ld32(acc + col, g);
-          tc::tmem_ld32(acc + 128 + col, u);
-          if (MODE == kGated) {
-            tc::wait_ld(g);
-            tc::wait_ld(u);
-            if (j == 1) release();
-            if (rows <= 0 || c0 >= q.n) continue;
-            float v[32];
+        const int col = 32 * part, c0 = w.n0 + col;
+        const bool live = rows > 0 && c0 < q.n;
+        const long long at = row0 * q.ldc + c0;
+        Chunk<T, 8> out[4], out2[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = silu_f32(__uint_as_float(g[i])) * __uint_as_float(u[i]);
-            store32<T>(stage, lane, v, static_cast<T *>(q.c) + row0 * q.ldc + c0, q.ldc, rows, q.n - c0, wide);
-          } else {
-            uint32_t dh[32];
-            tc::tmem_ld32(acc + 256 + col, dh);
-            tc::wait_ld(g);
-            tc::wait_ld(u);
-            tc::wait_ld(dh);
-            if (j == 1) release();
-            if (rows <= 0 || c0 >= q.n) continue;
-            float dg[32], du[32];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t g[16], u[16], dh[16];
+          tc::tmem_ld16(acc + col + 16 * h, g);
+          tc::tmem_ld16(acc + 128 + col + 16 * h, u);
+          if (MODE == kGatedBack) tc::tmem_ld16(acc + 256 + col + 16 * h, dh);
+          tc::wait_ld(g);
+          tc::wait_ld(u);
+          if (MODE == kGatedBack) tc::wait_ld(dh);
+          if (h == 1) release();
+          if (!live) continue;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float gi = __uint_as_float(g[i]), d = __uint_as_float(dh[i]);
-              const float sg = sigmoid_f32(gi);
-              du[i] = d * (gi * sg);
-              dg[i] = d * __uint_as_float(u[i]) * (sg * fmaf(gi, 1.0f - sg, 1.0f));
+          for (int i = 0; i < 16; ++i) {
+            const float gi = __uint_as_float(g[i]), ui = __uint_as_float(u[i]), sg = sigmoid_f32(gi);
+            if (MODE == kGated) {
+              put(out[2 * h + i / 8], i % 8, gi * sg * ui);
+            } else {
+              const float d = __uint_as_float(dh[i]);
+              put(out2[2 * h + i / 8], i % 8, d * (gi * sg));
+              put(out[2 * h + i / 8], i % 8, d * ui * (sg * fmaf(gi, 1.0f - sg, 1.0f)));
             }
-            const long long at = row0 * q.ldc + c0;
-            store32<T>(stage, lane, dg, static_cast<T *>(q.c) + at, q.ldc, rows, q.n - c0, wide);
-            store32<T>(stage, lane, du, static_cast<T *>(p.c2) + at, q.ldc, rows, q.n - c0, wide);
           }
         }
+        if (!live) continue;
+        // only the 16-bit types have these modes
+        using H = typename std::conditional<sizeof(T) == 2, T, __half>::type;
+        auto &o1 = reinterpret_cast<Chunk<H, 8>(&)[4]>(out);
+        auto &o2 = reinterpret_cast<Chunk<H, 8>(&)[4]>(out2);
+        store_rows<H>(stage, lane, o1, static_cast<H *>(q.c) + at, q.ldc, rows, q.n - c0, wide);
+        if (MODE == kGatedBack)
+          store_rows<H>(stage, lane, o2, static_cast<H *>(p.c2) + at, q.ldc, rows, q.n - c0, wide);
       }
     }
   }
