@@ -475,13 +475,18 @@ typedef struct {
   long long y_stride;
   void *h;                    /* optional: rows x hidden, contiguous; h as the second product reads it,
                                  which so3lr_feed_forward_backward needs */
+  float *gu;                  /* optional: so3lr_feed_forward_keep bytes, 16-byte aligned; the two projections
+                                 in float32 for so3lr_feed_forward_backward, which otherwise computes them again */
 } so3lr_feed_forward_args;
+/* Bytes of `gu` worth keeping for the backward pass: 0 where computing the
+ * projections again is cheaper than writing and reading them (narrow layers). */
+long long so3lr_feed_forward_keep(const so3lr_feed_forward_args *args);
 long long so3lr_feed_forward_workspace(const so3lr_feed_forward_args *args);
 int so3lr_feed_forward(const so3lr_feed_forward_args *args, void *workspace, long long workspace_bytes, void *stream,
                        char *err, size_t errlen);
 
-/* Gradients of so3lr_feed_forward for dy: with g, u the two projections (computed
- * again, so that only h is kept from the forward pass), sg = 1 / (1 + exp(-g)),
+/* Gradients of so3lr_feed_forward for dy: with g, u the two projections (kept by
+ * the forward pass, or computed again), sg = 1 / (1 + exp(-g)),
  *   dh = dy Wd,  du = dh g sg,  dg = dh u sg (1 + g (1 - sg))
  *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h */
 typedef struct {
@@ -498,6 +503,7 @@ typedef struct {
   const void *w_down;
   long long w_down_stride;
   const void *h;              /* rows x hidden, contiguous, from the forward pass */
+  const float *gu;            /* from the forward pass, or NULL */
   void *dx;                   /* rows x width */
   long long dx_stride;
   void *dw_gate;              /* hidden x width, contiguous */

@@ -8,16 +8,20 @@ Every translation unit is compiled with
 translation units whose code depends on the model width are compiled once per
 supported width (``-DSO3LR_FEATURES=128`` and ``=256``; the mixed-precision
 filter kernels exist for F = 128 only). Object files are cached under
-``so3lr_b200/_build`` and rebuilt when a source or header is newer.
+``so3lr_b200/_build`` and rebuilt when a source or header is newer. Where torch is
+installed, the Python module of the row-wise feed-forward layers is compiled
+against it and linked to the library.
 """
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.util
 import os
 import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = pathlib.Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
@@ -76,6 +80,37 @@ def _compile(unit, newest_header: float, force: bool, verbose: bool) -> pathlib.
     return obj
 
 
+def torch_module() -> pathlib.Path | None:
+    """The Python module of the feed-forward layers (binding/layers_binding.cpp),
+    compiled against the torch that is installed; None without torch (the rest of
+    the package does not need it)."""
+    if importlib.util.find_spec("torch") is None:
+        return None
+    return HERE / ("_layers" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_torch_module(force: bool = False) -> pathlib.Path | None:
+    out = torch_module()
+    if out is None:
+        return None
+    src, header = HERE / "binding" / "layers_binding.cpp", INCLUDE / "so3lr_b200.h"
+    newest = max(f.stat().st_mtime for f in (src, header, pathlib.Path(__file__)))
+    if not force and out.exists() and out.stat().st_mtime >= newest:
+        return out
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    includes = include_paths("cuda") + [sysconfig.get_paths()["include"], str(INCLUDE)]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", str(src), "-o", str(out),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    cmd += [f"-I{p}" for p in includes] + [f"-L{p}" for p in library_paths("cuda")]
+    cmd += [f"-L{HERE}", "-Wl,-rpath,$ORIGIN", "-lso3lr_b200", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+            "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    return out
+
+
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     BUILD.mkdir(exist_ok=True)
     newest_header = max([h.stat().st_mtime for h in headers()] + [pathlib.Path(__file__).stat().st_mtime])
@@ -87,6 +122,7 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    build_torch_module(force)
     return LIB
 
 

@@ -41,7 +41,8 @@ enum Mode {
   kPlain,     // C = A B^T, one or two K segments (A1 B1^T + A2 B2^T)
   kInt8,      // C = (A B^T) a_scale b_scale + bias
   kGated,     // C = silu(A G^T) * (A U^T): 128 columns of G and 128 of U per tile
-  kGatedBack  // g, u as above and dh = DY Wd: C = dg, C2 = du
+  kGatedBack, // g, u as above and dh = DY Wd: C = dg, C2 = du
+  kKeptBack   // the same with g, u read from the forward pass: dh alone is computed
 };
 template <int MODE>
 struct Shape {
@@ -69,6 +70,7 @@ struct Params {
   Problem prob[kMaxProblems];
   int problems, items;
   void *c2;                      // du
+  float *gu;                     // kept projections, see gu_index
   const float *a_scales, *b_scales, *bias;
   uint32_t *partial;
   int *err;
@@ -95,6 +97,12 @@ __device__ __forceinline__ Item item_of(const Params &p, int it) {
   w.kb_begin = int((long long)q.kb * w.split / q.splits);
   w.kb_end = int((long long)q.kb * (w.split + 1) / q.splits);
   return w;
+}
+
+// Kept projections: g (which = 0) and u (1) of row r, hidden column c, blocks of 32
+// rows so that a warp (lane = row) moves whole 128-byte lines straight from registers
+__device__ __forceinline__ size_t gu_index(long long row, int c, int which, int hidden) {
+  return ((size_t(row >> 5) * hidden + c) * 2 + which) * 32 + (row & 31);
 }
 
 // 64 bytes of each of the warp's 32 rows (lane = row) to C through the warp's staging,
@@ -343,6 +351,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
                           q.n - c0 - h * kCols, wide);
           }
         }
+      } else if (MODE == kKeptBack) {
+        for (int j = 0; j < 2; ++j) {
+          const int col = 64 * part + 32 * j, c0 = w.n0 + col;
+          const bool live = rows > 0 && c0 < q.n;
+          Chunk<T, kPer> out[4], out2[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float g[16], u[16];
+            uint32_t dh[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int c = c0 + 16 * h + i;
+              const bool in = live && c < q.n;
+              g[i] = in ? __ldcs(p.gu + gu_index(row0 + lane, c, 0, q.n)) : 0.0f;
+              u[i] = in ? __ldcs(p.gu + gu_index(row0 + lane, c, 1, q.n)) : 0.0f;
+            }
+            tc::tmem_ld16(acc + col + 16 * h, dh);
+            tc::wait_ld(dh);
+            if (j == 1 && h == 1) release();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float d = __uint_as_float(dh[i]), sg = sigmoid_f32(g[i]);
+              put(out2[2 * h + i / 8], i % 8, d * (g[i] * sg));
+              put(out[2 * h + i / 8], i % 8, d * u[i] * (sg * fmaf(g[i], 1.0f - sg, 1.0f)));
+            }
+          }
+          if (!live) continue;
+          const long long at = row0 * q.ldc + c0;
+          store_rows<T>(stage, lane, out, static_cast<T *>(q.c) + at, q.ldc, rows, q.n - c0, wide);
+          store_rows<T>(stage, lane, out2, static_cast<T *>(p.c2) + at, q.ldc, rows, q.n - c0, wide);
+        }
       } else {
         const int col = 32 * part, c0 = w.n0 + col;
         const bool live = rows > 0 && c0 < q.n;
@@ -359,6 +398,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           if (MODE == kGatedBack) tc::wait_ld(dh);
           if (h == 1) release();
           if (!live) continue;
+          if (MODE == kGated && p.gu) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int c = c0 + 16 * h + i;
+              if (c < q.n) {
+                p.gu[gu_index(row0 + lane, c, 0, q.n)] = __uint_as_float(g[i]);
+                p.gu[gu_index(row0 + lane, c, 1, q.n)] = __uint_as_float(u[i]);
+              }
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float gi = __uint_as_float(g[i]), ui = __uint_as_float(u[i]), sg = sigmoid_f32(gi);
@@ -488,7 +537,6 @@ class Dense {
   }
   Scratch &scratch() { return scratch_; }
   bool dry() const { return dry_; }
-  cudaStream_t stream() const { return stream_; }
 
   // the operand as TMA reads it: in place, or copied to padded rows
   Operand ready(Operand o) {
@@ -616,6 +664,11 @@ void int8_linear(Dense &d, const so3lr_int8_linear_args &a) {
 }
 
 // ------------------------------------------------------------------- feed-forward
+// Keeping g and u costs 16 bytes of HBM traffic an element, computing them again 4
+// width operations: at this card's 1.6 PFLOP/s and 6.5 TB/s the two are even near a
+// width of 1024.
+bool keeps(long long width) { return width >= 1024; }
+
 template <class T>
 void feed_forward(Dense &d, const so3lr_feed_forward_args &a) {
   const Operand x = d.ready(Operand{a.x, a.x_stride, a.rows, a.width});
@@ -636,6 +689,7 @@ void feed_forward(Dense &d, const so3lr_feed_forward_args &a) {
     q.n = int(a.hidden);
     q.c = const_cast<void *>(h.data);
     q.ldc = h.stride;
+    p.gu = a.gu;
     d.plan<kGated>(p, false);
     if (!d.dry()) {
       p.map[0] = d.map(x, 128);
@@ -683,8 +737,19 @@ void feed_forward_backward(Dense &d, const so3lr_feed_forward_backward_args &a) 
     q.c = const_cast<void *>(dg.data);
     q.ldc = ld;
     p.c2 = const_cast<void *>(du.data);
-    d.plan<kGatedBack>(p, false);
-    if (!d.dry()) {
+    if (a.gu) {
+      p.gu = const_cast<float *>(a.gu);
+      q.a[0] = 0;
+      q.b[0] = 1;
+      d.plan<kKeptBack>(p, false);
+    } else {
+      d.plan<kGatedBack>(p, false);
+    }
+    if (a.gu && !d.dry()) {
+      p.map[0] = d.map(dy, 128);
+      p.map[1] = d.map(w, 64);
+      d.run<kKeptBack, T, false, true>(p);
+    } else if (!d.dry()) {
       p.map[0] = d.map(x, 128);
       p.map[1] = d.map(g, 128);
       p.map[2] = d.map(u, 128);
@@ -785,14 +850,18 @@ void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaSt
     by_half(a.out_dtype, [&](auto t) { int8_linear<decltype(t)>(d, a); });
 }
 
+long long feed_forward_keep(const so3lr_feed_forward_args &a) {
+  return a.rows > kFewRows && keeps(a.width) ? (a.rows + 31) / 32 * 32 * a.hidden * 8 : 0;
+}
 // rows of the hidden layer of a few rows, on 16-byte boundaries
 static long long few_stride(const so3lr_feed_forward_args &a) { return (a.hidden + 7) / 8 * 8; }
 long long feed_forward_bytes(const so3lr_feed_forward_args &a) {
-  if (a.rows <= kFewRows) return a.h ? 0 : a.rows * few_stride(a) * 2;
+  if (a.rows <= kFewRows && !a.gu) return a.h ? 0 : a.rows * few_stride(a) * 2;
   return dry_run(a, 2, [&](Dense &d) { feed_forward<__half>(d, a); });
 }
 void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s) {
-  if (a.rows <= kFewRows) return launch_feed_forward_few(a, a.h ? a.h : workspace, a.h ? a.hidden : few_stride(a), s);
+  if (a.rows <= kFewRows && !a.gu)
+    return launch_feed_forward_few(a, a.h ? a.h : workspace, a.h ? a.hidden : few_stride(a), s);
   Dense d(workspace, 2, s, false);
   by_half(a.dtype, [&](auto t) { feed_forward<decltype(t)>(d, a); });
 }

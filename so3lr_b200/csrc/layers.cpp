@@ -193,6 +193,7 @@ void check(const so3lr_feed_forward_args *a) {
   check_feed_forward_inputs(call, a);
   matrix(call, "y", a->y, a->y_stride, a->rows, a->width, 2, true);
   if (a->h) matrix(call, "h", a->h, a->hidden, a->rows, a->hidden, 2, true);
+  if (a->gu) pointer(call, "gu", a->gu, 16);
 }
 void check(const so3lr_feed_forward_backward_args *a) {
   const char *call = "so3lr_feed_forward_backward";
@@ -200,6 +201,7 @@ void check(const so3lr_feed_forward_backward_args *a) {
   check_feed_forward_inputs(call, a);
   matrix(call, "dy", a->dy, a->dy_stride, a->rows, a->width, 2, false);
   matrix(call, "h", a->h, a->hidden, a->rows, a->hidden, 2, false);
+  if (a->gu) pointer(call, "gu", a->gu, 16);
   matrix(call, "dx", a->dx, a->dx_stride, a->rows, a->width, 2, true);
   pointer(call, "dw_gate", a->dw_gate, 2);
   pointer(call, "dw_up", a->dw_up, 2);
@@ -265,6 +267,12 @@ long long so3lr_feed_forward_workspace(const so3lr_feed_forward_args *args) {
   return sized([&] {
     check_feed_forward_sizes("so3lr_feed_forward", args);
     return so3lr_b200::feed_forward_bytes(*args);
+  });
+}
+long long so3lr_feed_forward_keep(const so3lr_feed_forward_args *args) {
+  return sized([&] {
+    check_feed_forward_sizes("so3lr_feed_forward", args);
+    return so3lr_b200::feed_forward_keep(*args);
   });
 }
 int so3lr_feed_forward(const so3lr_feed_forward_args *args, void *workspace, long long workspace_bytes, void *stream,

@@ -24,6 +24,7 @@ int *gave_up_flag();
 void check_gave_up();
 long long int8_linear_bytes(const so3lr_int8_linear_args &a);
 void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s);
+long long feed_forward_keep(const so3lr_feed_forward_args &a);
 long long feed_forward_bytes(const so3lr_feed_forward_args &a);
 void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s);
 long long feed_forward_backward_bytes(const so3lr_feed_forward_backward_args &a);

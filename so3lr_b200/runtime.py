@@ -32,7 +32,7 @@ EXPORTED = (
     # row-wise feed-forward layers (bound in layers.py)
     "so3lr_rms_norm", "so3lr_rms_norm_backward_workspace", "so3lr_rms_norm_backward", "so3lr_int8_linear_workspace",
     "so3lr_int8_linear", "so3lr_gate_int8", "so3lr_dequantize_int8", "so3lr_feed_forward_workspace",
-    "so3lr_feed_forward", "so3lr_feed_forward_backward_workspace", "so3lr_feed_forward_backward",
+    "so3lr_feed_forward_keep", "so3lr_feed_forward", "so3lr_feed_forward_backward_workspace", "so3lr_feed_forward_backward",
 )
 
 _dp = C.POINTER(C.c_double)

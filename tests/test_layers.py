@@ -10,9 +10,6 @@ times the unit roundoff is allowed for each). Where a bound over the whole sum
 would hide a lost term, the 2-norm of the error is held as well: two independent
 roundings to the type, 2 u relative.
 """
-import ctypes as C
-
-import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -324,7 +321,8 @@ def _ffn_ref(x, wg, wu, wd, dy, dtype):
 
 FFN_SIZES = [(1, 1, 1), (1, 64, 64), (1, 128, 512), (2, 33, 70), (3, 128, 300), (4, 256, 1024), (5, 7, 3), (8, 520, 1368),
              (9, 256, 256), (17, 100, 333), (33, 128, 512), (64, 64, 4096), (100, 136, 200), (128, 128, 128),
-             (129, 130, 131), (192, 256, 1024), (257, 264, 520), (777, 520, 1368), (3000, 256, 512)]
+             (129, 130, 131), (192, 256, 1024), (257, 264, 520), (777, 520, 1368), (3000, 256, 512), (5, 1024, 72), (40, 1024, 200),
+             (333, 1032, 260), (300, 2048, 131)]
 
 
 @pytest.mark.parametrize("dtype", HALF)
@@ -340,6 +338,19 @@ def test_feed_forward_and_gradients(layers, rows, width, hidden, dtype):
         if want.numel() >= 1000:
             off = float((got[name].double() - want).norm() / want.norm())
             assert off <= 2 * U[dtype], (name, off)
+
+
+def test_feed_forward_saved_of_another_call(layers):
+    x, wg, wu, wd, dy = _ffn_inputs(40, 1024, 64, torch.bfloat16)
+    _, saved = layers.feed_forward_train(x, wg, wu, wd)
+    assert saved[5] is not None
+    for wrong in (saved[:4] + (saved[4][:39], saved[5]), saved[:5] + (saved[5][:-1],), (x[:8],) + saved[1:]):
+        with pytest.raises(ValueError):
+            layers.feed_forward_backward(dy[:wrong[0].shape[0]], wrong)
+    # without the kept projections they are computed again: the same gradients within their roundings
+    for a, b in zip(layers.feed_forward_backward(dy, saved), layers.feed_forward_backward(dy, saved[:5] + (None,))):
+        off = float((a.double() - b.double()).norm() / a.double().norm())
+        assert off <= 2 * U[torch.bfloat16], off
 
 
 def test_feed_forward_layouts(layers):
