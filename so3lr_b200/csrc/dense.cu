@@ -360,12 +360,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           for (int h = 0; h < 2; ++h) {
             float g[16], u[16];
             uint32_t dh[16];
+            const float *gu = p.gu + gu_index(row0 + lane, c0 + 16 * h, 0, q.n);
+            const int left = live ? q.n - c0 - 16 * h : 0;
+            if (left >= 16) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int c = c0 + 16 * h + i;
-              const bool in = live && c < q.n;
-              g[i] = in ? __ldcs(p.gu + gu_index(row0 + lane, c, 0, q.n)) : 0.0f;
-              u[i] = in ? __ldcs(p.gu + gu_index(row0 + lane, c, 1, q.n)) : 0.0f;
+              for (int i = 0; i < 16; ++i) {
+                g[i] = __ldcs(gu + 64 * i);
+                u[i] = __ldcs(gu + 64 * i + 32);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                g[i] = i < left ? gu[64 * i] : 0.0f;
+                u[i] = i < left ? gu[64 * i + 32] : 0.0f;
+              }
             }
             tc::tmem_ld16(acc + col + 16 * h, dh);
             tc::wait_ld(dh);
@@ -399,14 +407,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           if (h == 1) release();
           if (!live) continue;
           if (MODE == kGated && p.gu) {
+            float *gu = p.gu + gu_index(row0 + lane, c0 + 16 * h, 0, q.n);
+            const int left = q.n - c0 - 16 * h;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int c = c0 + 16 * h + i;
-              if (c < q.n) {
-                p.gu[gu_index(row0 + lane, c, 0, q.n)] = __uint_as_float(g[i]);
-                p.gu[gu_index(row0 + lane, c, 1, q.n)] = __uint_as_float(u[i]);
+            for (int i = 0; i < 16; ++i)
+              if (i < left) {
+                __stcs(gu + 64 * i, __uint_as_float(g[i]));
+                __stcs(gu + 64 * i + 32, __uint_as_float(u[i]));
               }
-            }
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
