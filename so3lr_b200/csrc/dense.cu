@@ -16,8 +16,9 @@
 // reads them in place. An operand whose rows do not start on 16-byte boundaries
 // (TMA's rule) is first copied into padded rows.
 //
-// Products with few tiles and a long contraction are split along K: each part
-// writes raw 32-bit sums, k_join adds them in order.
+// Tiles beyond the last whole wave (one tile a CTA pair) of a long contraction are
+// split along K, so that they fill the pairs too: each part writes raw 32-bit sums,
+// k_join adds them in order.
 #include <mutex>
 
 #include "layers_common.cuh"
@@ -58,44 +59,50 @@ struct Problem {
   int a[2], b[2];                // tensor maps of the K segments
   int kb0, kb;                   // K blocks of the first segment, of both
   int m, n;                      // result
-  int tiles_m, tiles_n, splits;
-  int first;                     // its first work item
+  int tiles_m, tiles_n;
+  int first;                     // its first tile
   void *c;
   long long ldc;
-  long long partial;             // offset of its raw sums (splits > 1): [splits][m][ldp]
-  int ldp;
 };
 struct Params {
   CUtensorMap map[kMaxMaps];
   Problem prob[kMaxProblems];
   int problems, items;
+  int whole, splits;             // tiles done by one work item each; parts of each tile after those
   void *c2;                      // du
   float *gu;                     // kept projections, see gu_index
   const float *a_scales, *b_scales, *bias;
-  uint32_t *partial;
+  uint32_t *partial;             // raw sums: [tile - whole][part][kTileM][kTileN]
   int *err;
 };
 
 struct Item {
-  int prob, m0, n0, kb_begin, kb_end, split;
+  int prob, m0, n0, kb_begin, kb_end;
+  uint32_t *partial;  // where raw sums go; nullptr: the item is a whole tile
 };
 template <int MODE>
 __device__ __forceinline__ Item item_of(const Params &p, int it) {
   Item w;
+  int tile = it, part = 0, parts = 1;
+  w.partial = nullptr;
+  if (it >= p.whole) {
+    parts = p.splits;
+    part = (it - p.whole) % parts;
+    tile = p.whole + (it - p.whole) / parts;
+    if (parts > 1) w.partial = p.partial + (size_t)(it - p.whole) * (kTileM * kTileN);
+  }
   w.prob = 0;
 #pragma unroll
   for (int i = 1; i < kMaxProblems; ++i)
-    if (i < p.problems && it >= p.prob[i].first) w.prob = i;
+    if (i < p.problems && tile >= p.prob[i].first) w.prob = i;
   const Problem &q = p.prob[w.prob];
-  const int r = it - q.first;
-  w.split = r % q.splits;
-  const int tile = r / q.splits;
   // groups of 8 row tiles, columns outer: the tiles in flight share their operands in L2
+  tile -= q.first;
   const int group = tile / (8 * q.tiles_n), rows = min(8, q.tiles_m - 8 * group), t = tile - group * 8 * q.tiles_n;
   w.m0 = (8 * group + t % rows) * kTileM;
   w.n0 = (t / rows) * Shape<MODE>::kColumns;
-  w.kb_begin = int((long long)q.kb * w.split / q.splits);
-  w.kb_end = int((long long)q.kb * (w.split + 1) / q.splits);
+  w.kb_begin = int((long long)q.kb * part / parts);
+  w.kb_end = int((long long)q.kb * (part + 1) / parts);
   return w;
 }
 
@@ -119,20 +126,21 @@ __device__ __forceinline__ void store_rows(unsigned char *stage, int lane, const
 #pragma unroll
   for (int i = 0; i < 4; ++i) store_chunk<O, kPer>(slot(lane, i), v[i]);
   __syncwarp();
-  const int piece = lane & 3, left = cols - piece * kPer;
-  c += (lane >> 2) * ldc + piece * kPer;
-  if (wide && left >= kPer) {
+  if (wide && cols >= 4 * kPer) {  // 16 bytes a lane, 8 rows at a time
+    const int piece = lane & 3;
+    c += (lane >> 2) * ldc + piece * kPer;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 8 * i + (lane >> 2);
       if (r < rows) store_chunk<O, kPer>(c + 8 * i * ldc, load_chunk<O, kPer>(slot(r, piece)));
     }
-  } else if (left > 0) {
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      if (r < rows)
-        for (int j = 0; j < min(left, kPer); ++j) c[8 * i * ldc + j] = slot(r, piece)[j];
-    }
+  } else {  // one element a lane: still whole row segments
+    constexpr int kElems = 4 * kPer, kRows = 32 / kElems;
+    const int e = lane % kElems, r0 = lane / kElems;
+    c += r0 * ldc + e;
+    if (e < cols)
+#pragma unroll 8
+      for (int r = r0; r < rows; r += kRows, c += kRows * ldc) *c = slot(r, e / kPer)[e % kPer];
   }
   __syncwarp();
 }
@@ -308,7 +316,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       constexpr int kPer = 16 / sizeof(T);
       const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % 16 == 0;
       if (MODE == kPlain || MODE == kInt8) {
-        const bool split = q.splits > 1;
+        const bool split = w.partial != nullptr;
         const float sa = MODE == kInt8 && !split && lane < rows ? p.a_scales[row0 + lane] : 0.0f;
         for (int j = 0; j < 2; ++j) {
           const int col = 64 * part + 32 * j, c0 = w.n0 + col;
@@ -318,14 +326,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           if (j == 1) release();
           if (rows <= 0 || c0 >= q.n) continue;
           if (split) {  // raw 32-bit sums, float or int
-            uint32_t *dst = p.partial + q.partial + ((long long)w.split * q.m + row0) * q.ldp + c0;
+            uint32_t *dst = w.partial + (128 * rank + 32 * quad) * kTileN + col;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               Chunk<float, 4> v[4];
 #pragma unroll
               for (int i = 0; i < 16; ++i) v[i / 4].e[i % 4] = __uint_as_float(r[16 * h + i]);
-              store_rows<float>(stage, lane, v, reinterpret_cast<float *>(dst) + 16 * h, q.ldp, rows,
-                                q.n - c0 - 16 * h, true);
+              store_rows<float>(stage, lane, v, reinterpret_cast<float *>(dst) + 16 * h, kTileN, rows, 16, true);
             }
             continue;
           }
@@ -446,23 +453,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// C = the sum over `splits` of raw [m][ldp] sums, in order; 8-bit products get their scales here
-template <class T, bool INT8>
-__global__ void k_join(const uint32_t *__restrict__ partial, int splits, int m, int n, int ldp, T *__restrict__ c,
-                       long long ldc, const float *__restrict__ a_scales, const float *__restrict__ b_scales,
-                       const float *__restrict__ bias, bool wide) {
-  const int per_row = ldp / 4;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < (long long)m * per_row;
-       i += (long long)gridDim.x * blockDim.x) {
-    const int row = int(i / per_row), col = int(i - (long long)row * per_row) * 4;
+// C of the split tiles = the sum of their parts, in order; 8-bit products get their
+// scales here. A block does 16 rows of a tile, a thread 4 columns of 4 of them.
+template <int MODE, class T>
+__global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) {
+  const Item w = item_of<MODE>(p, p.whole + blockIdx.y * p.splits);
+  const Problem &q = p.prob[w.prob];
+  const int col = w.n0 + 4 * (threadIdx.x & 63);
+  if (col >= q.n) return;
+  const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % (4 * sizeof(T)) == 0 && col + 4 <= q.n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 16 * blockIdx.x + 4 * i + (threadIdx.x >> 6), row = w.m0 + r;
+    if (row >= q.m) break;
     float f[4] = {0, 0, 0, 0};
     int s[4] = {0, 0, 0, 0};
-    for (int k = 0; k < splits; ++k) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(partial + ((long long)k * m + row) * ldp + col);
+    for (int k = 0; k < p.splits; ++k) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(w.partial + ((size_t)k * kTileM + r) * kTileN + col - w.n0);
       const uint32_t e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (INT8)
+        if (MODE == kInt8)
           s[j] += int(e[j]);
         else
           f[j] += __uint_as_float(e[j]);
@@ -471,17 +482,17 @@ __global__ void k_join(const uint32_t *__restrict__ partial, int splits, int m, 
     Chunk<T, 4> out;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (INT8 && col + j < n)
-        f[j] = fmaf(float(s[j]) * a_scales[row], b_scales[col + j], bias ? bias[col + j] : 0.0f);
+      if (MODE == kInt8 && col + j < q.n)
+        f[j] = fmaf(float(s[j]) * p.a_scales[row], p.b_scales[col + j], p.bias ? p.bias[col + j] : 0.0f);
       out.e[j] = from_float<T>(f[j]);
     }
-    T *dst = c + row * ldc + col;
-    if (wide && col + 4 <= n)
+    T *dst = static_cast<T *>(q.c) + row * q.ldc + col;
+    if (wide)
       store_chunk<T, 4>(dst, out);
     else
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (col + j < n) dst[j] = out.e[j];
+        if (col + j < q.n) dst[j] = out.e[j];
   }
 }
 
@@ -581,8 +592,9 @@ class Dense {
     return m;
   }
 
-  // Work items of the problems; a problem list that leaves most CTA pairs idle is
-  // split along K, at least four K blocks to a part.
+  // Work items of the problems. The tiles after the last whole wave are split along K
+  // where that leaves no pair idle and saves more than the join costs: 24 K blocks
+  // take a pair about 7 us, a join with its launch 4 to 5.
   template <int MODE>
   void plan(Params &p, bool may_split) {
     long long tiles = 0;
@@ -591,23 +603,18 @@ class Dense {
       Problem &q = p.prob[i];
       q.tiles_m = (q.m - 1) / kTileM + 1;
       q.tiles_n = (q.n - 1) / Shape<MODE>::kColumns + 1;
+      q.first = int(tiles);
       tiles += (long long)q.tiles_m * q.tiles_n;
       kb = std::min(kb, q.kb);
+      if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
     }
-    if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
-    const int splits = may_split ? std::max(1, std::min(int(kPairs / tiles), kb / 4)) : 1;
-    long long partial = 0;
-    p.items = 0;
-    for (int i = 0; i < p.problems; ++i) {
-      Problem &q = p.prob[i];
-      q.splits = splits;
-      q.first = p.items;
-      p.items += q.tiles_m * q.tiles_n * splits;
-      q.ldp = (q.n + 3) / 4 * 4;
-      q.partial = partial;
-      if (splits > 1) partial += (long long)splits * q.m * q.ldp;
-    }
-    p.partial = splits > 1 ? static_cast<uint32_t *>(scratch_.take(partial * 4)) : nullptr;
+    const int rest = int(tiles % kPairs);
+    p.splits = may_split && rest > 0 && kb >= 24 ? std::max(1, std::min(kPairs / rest, kb / 8)) : 1;
+    p.whole = int(tiles) - (p.splits > 1 ? rest : 0);
+    p.items = p.whole + (p.splits > 1 ? rest * p.splits : 0);
+    p.partial = p.splits > 1
+                    ? static_cast<uint32_t *>(scratch_.take((long long)rest * p.splits * kTileM * kTileN * 4))
+                    : nullptr;
   }
 
   template <int MODE, class T, bool A_MN, bool B_MN>
@@ -618,14 +625,9 @@ class Dense {
     k_dense<MODE, T, A_MN, B_MN>
         <<<2 * std::min(kPairs, p.items), kThreads, Shape<MODE>::kSmem, stream_>>>(p);
     SO3_LAUNCH("dense");
-    for (int i = 0; i < p.problems; ++i) {
-      const Problem &q = p.prob[i];
-      if (q.splits == 1) continue;
-      const long long total = (long long)q.m * (q.ldp / 4);
-      const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % (4 * sizeof(T)) == 0;
-      k_join<T, MODE == kInt8><<<unsigned(std::min<long long>((total + 255) / 256, kSmCount * 16)), 256, 0, stream_>>>(
-          p.partial + q.partial, q.splits, q.m, q.n, q.ldp, static_cast<T *>(q.c), q.ldc, p.a_scales, p.b_scales,
-          p.bias, wide);
+    if constexpr (MODE == kPlain || MODE == kInt8) {
+      if (p.splits == 1) return;
+      k_join<MODE, T><<<dim3(kTileM / 16, (p.items - p.whole) / p.splits), 256, 0, stream_>>>(p);
       SO3_LAUNCH("join");
     }
   }
