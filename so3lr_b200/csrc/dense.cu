@@ -67,7 +67,7 @@ struct Problem {
 struct Params {
   CUtensorMap map[kMaxMaps];
   Problem prob[kMaxProblems];
-  int problems, items;
+  int problems, items, maps;
   int whole, splits;             // tiles done by one work item each; parts of each tile after those
   void *c2;                      // du
   float *gu;                     // kept projections, see gu_index
@@ -170,6 +170,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   const int rank = int(tc::cluster_rank());
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
+  dependents_may_start();
+  if (warp == 2 && lane < p.maps) tc::prefetch_map(&p.map[lane]);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       tc::mbar_init(full(s), 1);
@@ -193,6 +195,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   tc::cluster_sync();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_predecessors();
 
   if (warp == 0) {
     // ------------------------------------------------------------------- loads
@@ -457,6 +460,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
 // scales here. A block does 16 rows of a tile, a thread 4 columns of 4 of them.
 template <int MODE, class T>
 __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) {
+  dependents_may_start();
+  wait_for_predecessors();
   const Item w = item_of<MODE>(p, p.whole + blockIdx.y * p.splits);
   const Problem &q = p.prob[w.prob];
   const int col = w.n0 + 4 * (threadIdx.x & 63);
@@ -468,6 +473,7 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) 
     if (row >= q.m) break;
     float f[4] = {0, 0, 0, 0};
     int s[4] = {0, 0, 0, 0};
+#pragma unroll 4
     for (int k = 0; k < p.splits; ++k) {
       const uint4 v = *reinterpret_cast<const uint4 *>(w.partial + ((size_t)k * kTileM + r) * kTileN + col - w.n0);
       const uint32_t e[4] = {v.x, v.y, v.z, v.w};
@@ -500,6 +506,8 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) 
 template <class T>
 __global__ void k_repack(long long rows, int cols, const T *__restrict__ src, long long stride, T *__restrict__ dst,
                          int ld) {
+  dependents_may_start();
+  wait_for_predecessors();
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * cols;
        i += (long long)gridDim.x * blockDim.x) {
     const long long r = i / cols;
@@ -567,12 +575,11 @@ class Dense {
     if (!dry_) {
       const unsigned grid = unsigned(std::min<long long>((o.rows * o.cols + 255) / 256, kSmCount * 32));
       if (elem_ == 1)
-        k_repack<<<grid, 256, 0, stream_>>>(o.rows, int(o.cols), static_cast<const uint8_t *>(o.data), o.stride,
-                                            static_cast<uint8_t *>(p), ld);
+        launch(k_repack<uint8_t>, grid, 256, 0, stream_, o.rows, int(o.cols), static_cast<const uint8_t *>(o.data),
+               o.stride, static_cast<uint8_t *>(p), ld);
       else
-        k_repack<<<grid, 256, 0, stream_>>>(o.rows, int(o.cols), static_cast<const uint16_t *>(o.data), o.stride,
-                                            static_cast<uint16_t *>(p), ld);
-      SO3_LAUNCH("repack");
+        launch(k_repack<uint16_t>, grid, 256, 0, stream_, o.rows, int(o.cols), static_cast<const uint16_t *>(o.data),
+               o.stride, static_cast<uint16_t *>(p), ld);
     }
     return Operand{p, ld, o.rows, o.cols};
   }
@@ -622,13 +629,10 @@ class Dense {
     const void *fn = reinterpret_cast<const void *>(&k_dense<MODE, T, A_MN, B_MN>);
     allow_dynamic_smem(fn, Shape<MODE>::kSmem);
     p.err = gave_up_flag();
-    k_dense<MODE, T, A_MN, B_MN>
-        <<<2 * std::min(kPairs, p.items), kThreads, Shape<MODE>::kSmem, stream_>>>(p);
-    SO3_LAUNCH("dense");
+    launch(k_dense<MODE, T, A_MN, B_MN>, 2 * std::min(kPairs, p.items), kThreads, Shape<MODE>::kSmem, stream_, p);
     if constexpr (MODE == kPlain || MODE == kInt8) {
       if (p.splits == 1) return;
-      k_join<MODE, T><<<dim3(kTileM / 16, (p.items - p.whole) / p.splits), 256, 0, stream_>>>(p);
-      SO3_LAUNCH("join");
+      launch(k_join<MODE, T>, dim3(kTileM / 16, (p.items - p.whole) / p.splits), 256, 0, stream_, p);
     }
   }
 
@@ -668,6 +672,7 @@ void int8_linear(Dense &d, const so3lr_int8_linear_args &a) {
   q.ldc = a.y_stride;
   d.plan<kInt8>(p, true);
   if (d.dry()) return;
+  p.maps = 2;
   p.map[0] = d.map(x, 128);
   p.map[1] = d.map(w, 128);
   d.run<kInt8, O, false, false>(p);
@@ -702,6 +707,7 @@ void feed_forward(Dense &d, const so3lr_feed_forward_args &a) {
     p.gu = a.gu;
     d.plan<kGated>(p, false);
     if (!d.dry()) {
+      p.maps = 3;
       p.map[0] = d.map(x, 128);
       p.map[1] = d.map(g, 128);
       p.map[2] = d.map(u, 128);
@@ -721,6 +727,7 @@ void feed_forward(Dense &d, const so3lr_feed_forward_args &a) {
   q.ldc = a.y_stride;
   d.plan<kPlain>(p, true);
   if (d.dry()) return;
+  p.maps = 2;
   p.map[0] = d.map(hr, 128);
   p.map[1] = d.map(w, 128);
   d.run<kPlain, T, false, false>(p);
@@ -756,10 +763,12 @@ void feed_forward_backward(Dense &d, const so3lr_feed_forward_backward_args &a) 
       d.plan<kGatedBack>(p, false);
     }
     if (a.gu && !d.dry()) {
+      p.maps = 2;
       p.map[0] = d.map(dy, 128);
       p.map[1] = d.map(w, 64);
       d.run<kKeptBack, T, false, true>(p);
     } else if (!d.dry()) {
+      p.maps = 5;
       p.map[0] = d.map(x, 128);
       p.map[1] = d.map(g, 128);
       p.map[2] = d.map(u, 128);
@@ -784,6 +793,7 @@ void feed_forward_backward(Dense &d, const so3lr_feed_forward_backward_args &a) 
     q.ldc = a.dx_stride;
     d.plan<kPlain>(p, true);
     if (!d.dry()) {
+      p.maps = 4;
       p.map[0] = d.map(dg, 128);
       p.map[1] = d.map(du, 128);
       p.map[2] = d.map(g, 64);
@@ -806,6 +816,7 @@ void feed_forward_backward(Dense &d, const so3lr_feed_forward_backward_args &a) 
   }
   d.plan<kPlain>(p, true);
   if (d.dry()) return;
+  p.maps = 5;
   p.map[0] = d.map(dg, 64);
   p.map[1] = d.map(du, 64);
   p.map[2] = d.map(dy, 64);

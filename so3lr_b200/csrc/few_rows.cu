@@ -89,6 +89,19 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   const bool live_n = n < a.n, live0 = g < a.rows, live1 = TWO && g + 8 < a.rows;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer);
   const int begin = int((long long)steps * warp / warps), end = int((long long)steps * (warp + 1) / warps);
+  dependents_may_start();
+  // the first weights on their way to L2, which needs no order with the kernel before
+  if (ALIGNED && live_n) {
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int k = ((begin + i) * 4 + t) * kPer;
+      if (begin + i < end && k < a.k) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(w + k));
+        if (GATED) asm volatile("prefetch.global.L2 [%0];" ::"l"(w2 + k));
+      }
+    }
+  }
+  wait_for_predecessors();
   Acc acc[kOut][4] = {};
   for (int st = begin; st < end; st += kUnroll) {
     uint4 vw[kUnroll], vw2[GATED ? kUnroll : 1], v0[kUnroll], v1[TWO ? kUnroll : 1];
@@ -154,12 +167,11 @@ void run(const FewArgs &a, cudaStream_t s) {
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer), warps = std::max(1, std::min(most, steps / 4));
   const unsigned block = unsigned(32 * warps);
   if (a.rows > 8)
-    aligned ? k_few_rows<E, O, GATED, true, true><<<grid, block, 0, s>>>(a)
-            : k_few_rows<E, O, GATED, true, false><<<grid, block, 0, s>>>(a);
+    aligned ? launch(k_few_rows<E, O, GATED, true, true>, grid, block, 0, s, a)
+            : launch(k_few_rows<E, O, GATED, true, false>, grid, block, 0, s, a);
   else
-    aligned ? k_few_rows<E, O, GATED, false, true><<<grid, block, 0, s>>>(a)
-            : k_few_rows<E, O, GATED, false, false><<<grid, block, 0, s>>>(a);
-  SO3_LAUNCH("few_rows");
+    aligned ? launch(k_few_rows<E, O, GATED, false, true>, grid, block, 0, s, a)
+            : launch(k_few_rows<E, O, GATED, false, false>, grid, block, 0, s, a);
 }
 
 }  // namespace

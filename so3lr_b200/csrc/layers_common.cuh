@@ -6,12 +6,39 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <utility>
 
 #include "layers.hpp"
 
 namespace so3lr_b200 {
 
 constexpr int kSmCount = 148;  // B200
+
+// Programmatic dependent launch. Every kernel of the layers is launched so that it may
+// start while the kernel before it on the stream finishes: it lets its own successor
+// start (dependents_may_start) and touches no global memory before
+// wait_for_predecessors, which returns when everything before it on the stream has
+// completed and is visible. What runs ahead is launch latency and set-up (barriers,
+// TMEM, tensor maps), 1 to 2 us of a small call's kernels.
+__device__ __forceinline__ void dependents_may_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_predecessors() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... P, class... A>
+void launch(void (*kernel)(P...), dim3 grid, dim3 block, std::size_t smem, cudaStream_t stream, A &&...args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  ++launch_counter();
+  SO3_CUDA(cudaLaunchKernelEx(&config, kernel, std::forward<A>(args)...));
+}
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -65,6 +65,8 @@ template <class T, class W, int VEC, int N, bool WARP, bool QUANT>
 __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const so3lr_rms_norm_args a) {
   __shared__ float slot[32];
   __shared__ uint32_t slot_max[32];
+  dependents_may_start();
+  wait_for_predecessors();
   const RowTeam<WARP> team;
   const long long row = WARP ? (long long)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= a.rows) return;  // whole warps (WARP) only: a block row always exists
@@ -140,6 +142,8 @@ __global__ void __launch_bounds__(MAXT) k_rms_norm_backward(const so3lr_rms_norm
   constexpr bool WARP = MAXT == 32 * kWarpRows;
   __shared__ float2 slot[2][32];
   extern __shared__ float column[];  // WARP: kWarpRows x width
+  dependents_may_start();
+  wait_for_predecessors();
   const RowTeam<WARP> team;
   const int width = int(a.width);
   const int teams = WARP ? kWarpRows : 1, team_id = WARP ? threadIdx.x >> 5 : 0;
@@ -274,7 +278,9 @@ __global__ void __launch_bounds__(512)
   extern __shared__ __align__(128) unsigned char smem[];
   const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
   const uint32_t row_bytes = width * sizeof(T), tensors = a.ds ? 3 : 2;
+  dependents_may_start();
   const RowRing ring(smem, tensors * row_bytes, stages, err);
+  wait_for_predecessors();
   const RowTeam<false> team;
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
   auto fetch = [&](int i) {
@@ -352,6 +358,8 @@ __global__ void __launch_bounds__(512)
 template <class W>
 __global__ void k_column_sum(int nparts, int width, const float *__restrict__ partial, W *__restrict__ out) {
   __shared__ float part[32][33];
+  dependents_may_start();
+  wait_for_predecessors();
   const int c = blockIdx.x * 32 + threadIdx.x;
   float total = 0.0f;
   if (c < width)
@@ -372,6 +380,8 @@ template <class T, int VEC, int N, bool WARP>
 __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024, VEC *N == 8 && !WARP ? 2 : 1)
     k_gate_int8(const so3lr_gate_int8_args a) {
   __shared__ uint32_t slot[32];
+  dependents_may_start();
+  wait_for_predecessors();
   const RowTeam<WARP> team;
   const long long row = WARP ? (long long)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= a.rows) return;
@@ -417,7 +427,9 @@ __global__ void __launch_bounds__(MAXT) k_gate_int8_ring(const so3lr_gate_int8_a
   extern __shared__ __align__(128) unsigned char smem[];
   const int hidden = int(a.hidden), t = threadIdx.x, size = blockDim.x;
   const uint32_t row_bytes = 2 * hidden * sizeof(T);
+  dependents_may_start();
   const RowRing ring(smem, row_bytes, stages, err);
+  wait_for_predecessors();
   const RowTeam<false> team;
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
   auto fetch = [&](int i) {
@@ -460,6 +472,8 @@ __global__ void __launch_bounds__(MAXT) k_gate_int8_ring(const so3lr_gate_int8_a
 
 template <class T, int VEC>
 __global__ void k_dequantize_int8(const so3lr_dequantize_int8_args a) {
+  dependents_may_start();
+  wait_for_predecessors();
   const long long per_row = a.width / VEC, total = a.rows * per_row;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
@@ -520,14 +534,13 @@ void norm_forward(const so3lr_rms_norm_args &a, cudaStream_t s) {
   const unsigned grid = unsigned(warp ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows);
   const int block = warp ? 32 * kWarpRows : threads;
   if (warp && a.codes)
-    k_rms_norm<T, W, VEC, N, true, true><<<grid, block, 0, s>>>(a);
+    launch(k_rms_norm<T, W, VEC, N, true, true>, grid, block, 0, s, a);
   else if (warp)
-    k_rms_norm<T, W, VEC, N, true, false><<<grid, block, 0, s>>>(a);
+    launch(k_rms_norm<T, W, VEC, N, true, false>, grid, block, 0, s, a);
   else if (a.codes)
-    k_rms_norm<T, W, VEC, N, false, true><<<grid, block, 0, s>>>(a);
+    launch(k_rms_norm<T, W, VEC, N, false, true>, grid, block, 0, s, a);
   else
-    k_rms_norm<T, W, VEC, N, false, false><<<grid, block, 0, s>>>(a);
-  SO3_LAUNCH("rms_norm");
+    launch(k_rms_norm<T, W, VEC, N, false, false>, grid, block, 0, s, a);
 }
 
 // Blocks of a kernel that walks over rows
@@ -571,13 +584,11 @@ template <class T, class W, int VEC, int N>
 void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int grid, cudaStream_t s) {
   const int threads = row_threads(a.width, VEC * N);
   if (threads == 32)
-    k_rms_norm_backward<T, W, VEC, N, 32 * kWarpRows>
-        <<<grid, 32 * kWarpRows, kWarpRows * a.width * sizeof(float), s>>>(a, partial);
+    launch(k_rms_norm_backward<T, W, VEC, N, 32 * kWarpRows>, grid, 32 * kWarpRows, kWarpRows * a.width * sizeof(float), s, a, partial);
   else if (threads <= 512)
-    k_rms_norm_backward<T, W, VEC, N, 512><<<grid, threads, 0, s>>>(a, partial);
+    launch(k_rms_norm_backward<T, W, VEC, N, 512>, grid, threads, 0, s, a, partial);
   else
-    k_rms_norm_backward<T, W, VEC, N, 1024><<<grid, threads, 0, s>>>(a, partial);
-  SO3_LAUNCH("rms_norm_backward");
+    launch(k_rms_norm_backward<T, W, VEC, N, 1024>, grid, threads, 0, s, a, partial);
 }
 template <class T, class W>
 void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, const RingPlan &r, cudaStream_t s) {
@@ -585,20 +596,18 @@ void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, c
   const int threads = row_threads(a.width, 16);
   auto run = [&](auto fn) {
     allow_dynamic_smem(reinterpret_cast<const void *>(fn), 227 * 1024 - 1024);
-    fn<<<r.grid, threads, r.smem, s>>>(a, partial, r.stages, gave_up_flag());
+    launch(fn, r.grid, threads, r.smem, s, a, partial, r.stages, gave_up_flag());
   };
   run(&k_rms_norm_backward_ring<T, W>);
-  SO3_LAUNCH("rms_norm_backward_ring");
 }
 
 template <class T, int VEC, int N>
 void gate(const so3lr_gate_int8_args &a, cudaStream_t s) {
   const int threads = row_threads(a.hidden, VEC * N);
   if (threads == 32)
-    k_gate_int8<T, VEC, N, true><<<unsigned((a.rows + kWarpRows - 1) / kWarpRows), 32 * kWarpRows, 0, s>>>(a);
+    launch(k_gate_int8<T, VEC, N, true>, unsigned((a.rows + kWarpRows - 1) / kWarpRows), 32 * kWarpRows, 0, s, a);
   else
-    k_gate_int8<T, VEC, N, false><<<unsigned(a.rows), threads, 0, s>>>(a);
-  SO3_LAUNCH("gate_int8");
+    launch(k_gate_int8<T, VEC, N, false>, unsigned(a.rows), threads, 0, s, a);
 }
 int ring_per_thread(long long hidden) { return hidden <= 4096 ? 16 : 32; }
 template <class T>
@@ -607,13 +616,12 @@ void gate_ring(const so3lr_gate_int8_args &a, const RingPlan &r, cudaStream_t s)
   const int threads = row_threads(a.hidden, ring_per_thread(a.hidden));
   auto run = [&](auto fn) {
     allow_dynamic_smem(reinterpret_cast<const void *>(fn), 227 * 1024 - 1024);
-    fn<<<r.grid, threads, r.smem, s>>>(a, r.stages, gave_up_flag());
+    launch(fn, r.grid, threads, r.smem, s, a, r.stages, gave_up_flag());
   };
   if (ring_per_thread(a.hidden) == 16)
     run(&k_gate_int8_ring<T, 16, 256>);
   else
     run(&k_gate_int8_ring<T, 32, 512>);
-  SO3_LAUNCH("gate_int8_ring");
 }
 
 }  // namespace
@@ -663,9 +671,7 @@ void launch_rms_norm_backward(const so3lr_rms_norm_backward_args &a, void *works
           wide ? norm_backward<T, W, V, 16 / V>(a, partial, parts, s)
                : norm_backward<T, W, 1, 16>(a, partial, parts, s);
       }
-      k_column_sum<W><<<unsigned((a.width + 31) / 32), dim3(32, 32), 0, s>>>(parts, int(a.width), partial,
-                                                                            static_cast<W *>(a.dweight));
-      SO3_LAUNCH("column_sum");
+      launch(k_column_sum<W>, unsigned((a.width + 31) / 32), dim3(32, 32), 0, s, parts, int(a.width), partial, static_cast<W *>(a.dweight));
     });
   });
 }
@@ -700,10 +706,9 @@ void launch_dequantize_int8(const so3lr_dequantize_int8_args &a, cudaStream_t s)
     const long long total = a.rows * (wide ? a.width / 16 : a.width);
     const unsigned grid = unsigned(std::min<long long>((total + 255) / 256, kSmCount * 64));
     if (wide)
-      k_dequantize_int8<T, 16><<<grid, 256, 0, s>>>(a);
+      launch(k_dequantize_int8<T, 16>, grid, 256, 0, s, a);
     else
-      k_dequantize_int8<T, 1><<<grid, 256, 0, s>>>(a);
-    SO3_LAUNCH("dequantize_int8");
+      launch(k_dequantize_int8<T, 1>, grid, 256, 0, s, a);
   });
 }
 
