@@ -101,8 +101,12 @@ __device__ __forceinline__ Item item_of(const Params &p, int it) {
   const int group = tile / (8 * q.tiles_n), rows = min(8, q.tiles_m - 8 * group), t = tile - group * 8 * q.tiles_n;
   w.m0 = (8 * group + t % rows) * kTileM;
   w.n0 = (t / rows) * Shape<MODE>::kColumns;
-  w.kb_begin = int((long long)q.kb * part / parts);
-  w.kb_end = int((long long)q.kb * (part + 1) / parts);
+  w.kb_begin = 0;
+  w.kb_end = q.kb;
+  if (parts > 1) {  // kb < 2^24 and parts < 2^7: the products fit 31 bits
+    w.kb_begin = q.kb * part / parts;
+    w.kb_end = q.kb * (part + 1) / parts;
+  }
   return w;
 }
 
@@ -144,9 +148,11 @@ __device__ __forceinline__ void store_rows(unsigned char *stage, int lane, const
   }
   __syncwarp();
 }
-template <class O, int N>
-__device__ __forceinline__ void put(Chunk<O, N> &chunk, int i, float v) {
-  chunk.e[i] = from_float<O>(v);
+// dg = dh u silu'(g), du = dh silu(g)
+__device__ __forceinline__ void gradients(float g, float u, float dh, float &dg, float &du) {
+  const float sg = sigmoid_f32(g);
+  du = dh * (g * sg);
+  dg = dh * u * (sg * fmaf(g, 1.0f - sg, 1.0f));
 }
 
 template <int MODE, class T, bool A_MN, bool B_MN>
@@ -318,7 +324,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       const int row0 = w.m0 + 128 * rank + 32 * quad, rows = min(32, q.m - row0);
       constexpr int kPer = 16 / sizeof(T);
       const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % 16 == 0;
-      if (MODE == kPlain || MODE == kInt8) {
+      if constexpr (MODE == kPlain || MODE == kInt8) {
         const bool split = w.partial != nullptr;
         const float sa = MODE == kInt8 && !split && lane < rows ? p.a_scales[row0 + lane] : 0.0f;
         for (int j = 0; j < 2; ++j) {
@@ -350,18 +356,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
             if (h * kCols >= 32) break;
             Chunk<T, kPer> v[4];
 #pragma unroll
-            for (int i = 0; i < kCols; ++i) {
-              const int k = (h * kCols + i) % 32;
-              float f = __uint_as_float(r[k]);
-              if (MODE == kInt8)
-                f = fmaf(float(int(r[k])) * sa, __shfl_sync(0xffffffffu, sb, k), __shfl_sync(0xffffffffu, bias, k));
-              put(v[i / kPer], i % kPer, f);
+            for (int i = 0; i < 4; ++i) {
+              float f[kPer];
+#pragma unroll
+              for (int e = 0; e < kPer; ++e) {
+                const int k = (h * kCols + i * kPer + e) % 32;
+                f[e] = __uint_as_float(r[k]);
+                if (MODE == kInt8)
+                  f[e] = fmaf(float(int(r[k])) * sa, __shfl_sync(0xffffffffu, sb, k),
+                              __shfl_sync(0xffffffffu, bias, k));
+              }
+              v[i] = to_chunk<T, kPer>(f);
             }
             store_rows<T>(stage, lane, v, static_cast<T *>(q.c) + row0 * q.ldc + c0 + h * kCols, q.ldc, rows,
                           q.n - c0 - h * kCols, wide);
           }
         }
-      } else if (MODE == kKeptBack) {
+      } else if constexpr (MODE == kKeptBack) {
         for (int j = 0; j < 2; ++j) {
           const int col = 64 * part + 32 * j, c0 = w.n0 + col;
           const bool live = rows > 0 && c0 < q.n;
@@ -389,10 +400,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
             tc::wait_ld(dh);
             if (j == 1 && h == 1) release();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float d = __uint_as_float(dh[i]), sg = sigmoid_f32(g[i]);
-              put(out2[2 * h + i / 8], i % 8, d * (g[i] * sg));
-              put(out[2 * h + i / 8], i % 8, d * u[i] * (sg * fmaf(g[i], 1.0f - sg, 1.0f)));
+            for (int k = 0; k < 2; ++k) {
+              float dg[8], du[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                gradients(g[8 * k + i], u[8 * k + i], __uint_as_float(dh[8 * k + i]), dg[i], du[i]);
+              out[2 * h + k] = to_chunk<T, 8>(dg);
+              out2[2 * h + k] = to_chunk<T, 8>(du);
             }
           }
           if (!live) continue;
@@ -404,7 +418,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
         const int col = 32 * part, c0 = w.n0 + col;
         const bool live = rows > 0 && c0 < q.n;
         const long long at = row0 * q.ldc + c0;
-        Chunk<T, 8> out[4], out2[4];
+        // only the 16-bit types have these modes
+        using H = typename std::conditional<sizeof(T) == 2, T, __half>::type;
+        Chunk<H, 8> out[4], out2[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t g[16], u[16], dh[16];
@@ -427,25 +443,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
               }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float gi = __uint_as_float(g[i]), ui = __uint_as_float(u[i]), sg = sigmoid_f32(gi);
-            if (MODE == kGated) {
-              put(out[2 * h + i / 8], i % 8, gi * sg * ui);
-            } else {
-              const float d = __uint_as_float(dh[i]);
-              put(out2[2 * h + i / 8], i % 8, d * (gi * sg));
-              put(out[2 * h + i / 8], i % 8, d * ui * (sg * fmaf(gi, 1.0f - sg, 1.0f)));
+          for (int k = 0; k < 2; ++k) {
+            float a[8], b[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float gi = __uint_as_float(g[8 * k + i]), ui = __uint_as_float(u[8 * k + i]);
+              if (MODE == kGated)
+                a[i] = silu_f32(gi) * ui;
+              else
+                gradients(gi, ui, __uint_as_float(dh[8 * k + i]), a[i], b[i]);
             }
+            out[2 * h + k] = to_chunk<H, 8>(a);
+            if (MODE == kGatedBack) out2[2 * h + k] = to_chunk<H, 8>(b);
           }
         }
         if (!live) continue;
-        // only the 16-bit types have these modes
-        using H = typename std::conditional<sizeof(T) == 2, T, __half>::type;
-        auto &o1 = reinterpret_cast<Chunk<H, 8>(&)[4]>(out);
-        auto &o2 = reinterpret_cast<Chunk<H, 8>(&)[4]>(out2);
-        store_rows<H>(stage, lane, o1, static_cast<H *>(q.c) + at, q.ldc, rows, q.n - c0, wide);
+        store_rows<H>(stage, lane, out, static_cast<H *>(q.c) + at, q.ldc, rows, q.n - c0, wide);
         if (MODE == kGatedBack)
-          store_rows<H>(stage, lane, o2, static_cast<H *>(p.c2) + at, q.ldc, rows, q.n - c0, wide);
+          store_rows<H>(stage, lane, out2, static_cast<H *>(p.c2) + at, q.ldc, rows, q.n - c0, wide);
       }
     }
   }

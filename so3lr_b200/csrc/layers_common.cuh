@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 #include <utility>
 
 #include "layers.hpp"
@@ -65,6 +66,26 @@ __device__ __forceinline__ Chunk<T, VEC> load_chunk(const T *p) {
 template <class T, int VEC>
 __device__ __forceinline__ void store_chunk(T *p, const Chunk<T, VEC> &c) {
   *reinterpret_cast<Chunk<T, VEC> *>(p) = c;
+}
+
+// VEC values rounded to T. Pairs go through one packed conversion: element by element
+// it is a conversion and a byte permutation each.
+template <class T, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> to_chunk(const float (&v)[VEC]) {
+  Chunk<T, VEC> c;
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2 *>(&c.e[i]) = __floats2half2_rn(v[i], v[i + 1]);
+      else
+        *reinterpret_cast<__nv_bfloat162 *>(&c.e[i]) = __floats2bfloat162_rn(v[i], v[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c.e[i] = from_float<T>(v[i]);
+  }
+  return c;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {

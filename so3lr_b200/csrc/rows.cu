@@ -93,8 +93,10 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
     if (c < width) {
       if (r) {
         // the stream is kept in the element type, and the norm is of what is kept
+        float sum[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) cx[j].e[i] = from_float<T>(to_float(cx[j].e[i]) + to_float(cr[j].e[i]));
+        for (int i = 0; i < VEC; ++i) sum[i] = to_float(cx[j].e[i]) + to_float(cr[j].e[i]);
+        cx[j] = to_chunk<T, VEC>(sum);
         store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx[j]);
       }
 #pragma unroll
@@ -110,17 +112,14 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
   for (int j = 0; j < N; ++j) {
     const int c = (j * team.size + team.t) * VEC;
     if (c < width) {
-      Chunk<T, VEC> out;
+      float y[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float y = v[j * VEC + i] * rstd * to_float(cw[j].e[i]);
-        v[j * VEC + i] = y;
-        if (QUANT)
-          top = max_abs(top, y);
-        else
-          out.e[i] = from_float<T>(y);
+        y[i] = v[j * VEC + i] * rstd * to_float(cw[j].e[i]);
+        v[j * VEC + i] = y[i];
+        if (QUANT) top = max_abs(top, y[i]);
       }
-      if (!QUANT) store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, out);
+      if (!QUANT) store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, to_chunk<T, VEC>(y));
     }
   }
   if (!QUANT) return;
@@ -192,16 +191,16 @@ __global__ void __launch_bounds__(MAXT) k_rms_norm_backward(const so3lr_rms_norm
     for (int j = 0; j < N; ++j) {
       const int c = (j * team.size + team.t) * VEC;
       if (c < width) {
-        Chunk<T, VEC> out;
+        float out[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float xh = to_float(cs[j].e[i]) * rstd, d = to_float(cd[j].e[i]);
           dw[j * VEC + i] = fmaf(d, xh, dw[j * VEC + i]);
           float g = rstd * (d * to_float(cw[j].e[i]) - xh * mean);
           if (ds) g += to_float(ce[j].e[i]);
-          out.e[i] = from_float<T>(g);
+          out[i] = g;
         }
-        store_chunk<T, VEC>(static_cast<T *>(a.dx) + row * a.dx_stride + c, out);
+        store_chunk<T, VEC>(static_cast<T *>(a.dx) + row * a.dx_stride + c, to_chunk<T, VEC>(out));
       }
     }
   }
@@ -332,15 +331,15 @@ __global__ void __launch_bounds__(512)
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
       if (c < width) {
-        Chunk<T, VEC> out;
+        float out[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float f = to_float(cs[j].e[i]), d = to_float(cd[j].e[i]);
           dw[j * VEC + i] = fmaf(d, f * rstd, dw[j * VEC + i]);
           const float rest = a.ds ? fmaf(f, back, to_float(ce[j].e[i])) : f * back;
-          out.e[i] = from_float<T>(fmaf(d * to_float(cw[j].e[i]), rstd, rest));
+          out[i] = fmaf(d * to_float(cw[j].e[i]), rstd, rest);
         }
-        store_chunk<T, VEC>(dx + c, out);
+        store_chunk<T, VEC>(dx + c, to_chunk<T, VEC>(out));
       }
     }
   }
@@ -486,12 +485,11 @@ __global__ void k_dequantize_int8(const so3lr_dequantize_int8_args a) {
       constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
       for (int j = 0; j < VEC; j += kPer) {
-        Chunk<T, kPer> out;
+        float out[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k)
-          out.e[k] = from_float<T>(
-              byte_to_float(reinterpret_cast<const uint32_t *>(&q)[(j + k) / 4] ^ 0x80808080u, (j + k) % 4) * scale);
-        store_chunk<T, kPer>(dst + j, out);
+          out[k] = byte_to_float(reinterpret_cast<const uint32_t *>(&q)[(j + k) / 4] ^ 0x80808080u, (j + k) % 4) * scale;
+        store_chunk<T, kPer>(dst + j, to_chunk<T, kPer>(out));
       }
     } else {
       dst[0] = from_float<T>(float(q.e[0]) * scale);
