@@ -36,6 +36,7 @@ constexpr uint32_t kOperand = 128 * 128;    // 128 rows of 128 bytes: one operan
 constexpr uint32_t kStaging = 2048;         // of an epilogue warp: 32 rows x 64 bytes
 constexpr int kBarBytes = 256;
 constexpr int kMaxMaps = 6, kMaxProblems = 3, kMaxStages = 6;
+constexpr int kItemTable = 32;              // work items of a pair worked out once, at its start
 
 // What the kernel computes.
 enum Mode {
@@ -175,6 +176,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(tc::cluster_rank());
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  // the pair's n-th work item: its divisions and parameter reads are not on the path of every tile
+  __shared__ Item table[kItemTable];
+  for (int i = threadIdx.x; i < kItemTable && pair + i * pairs < p.items; i += kThreads)
+    table[i] = item_of<MODE>(p, pair + i * pairs);
+  auto item = [&](int n) { return n < kItemTable ? table[n] : item_of<MODE>(p, pair + n * pairs); };
+  const int items = pair < p.items ? (p.items - 1 - pair) / pairs + 1 : 0;
 
   dependents_may_start();
   if (warp == 2 && lane < p.maps) tc::prefetch_map(&p.map[lane]);
@@ -208,8 +215,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
     if (lane == 0) {
       int n = 0;
       bool ok = true;
-      for (int it = pair; it < p.items && ok; it += pairs) {
-        const Item w = item_of<MODE>(p, it);
+      for (int it = 0; it < items && ok; ++it) {
+        const Item w = item(it);
         const Problem &q = p.prob[w.prob];
         for (int kb = w.kb_begin; kb < w.kb_end; ++kb, ++n) {
           const int s = n % S::kStages;
@@ -258,10 +265,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       constexpr uint32_t kAb = kI8 || std::is_same<T, __nv_bfloat16>::value ? 1 : 0;  // s8 / bf16, or f16
       constexpr uint32_t kId = tc::idesc(kI8 ? 2 : 1, kAb, A_MN, B_MN, 256);
       constexpr uint32_t kIdDh = tc::idesc(1, kAb, false, true, 128);
-      int n = 0, done = 0;
+      int n = 0;
       bool ok = true;
-      for (int it = pair; it < p.items && ok; it += pairs, ++done) {
-        const Item w = item_of<MODE>(p, it);
+      for (int done = 0; done < items && ok; ++done) {
+        const Item w = item(done);
         const int buf = done % S::kBuffers;
         ok = tc::mbar_wait(acc_empty(buf), ((done / S::kBuffers) & 1) ^ 1, abort_flag, p.err, 2);
         if (!ok) break;
@@ -307,9 +314,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
     const int quad = warp & 3, part = (warp - 2) >> 2;
     unsigned char *stage = staging + (warp - 2) * kStaging;
     const uint32_t lanes = tmem + (uint32_t(32 * quad) << 16);
-    int done = 0;
-    for (int it = pair; it < p.items; it += pairs, ++done) {
-      const Item w = item_of<MODE>(p, it);
+    for (int done = 0; done < items; ++done) {
+      const Item w = item(done);
       const Problem &q = p.prob[w.prob];
       const int buf = done % S::kBuffers;
       if (!__all_sync(0xffffffffu, tc::mbar_wait(acc_full(buf), (done / S::kBuffers) & 1, abort_flag, p.err, 5)))
