@@ -29,13 +29,13 @@ namespace so3lr_b200 {
 namespace {
 
 constexpr int kPairs = kSmCount / 2;
-constexpr int kTileM = 256, kTileN = 256;   // of a CTA pair
+constexpr int kTileM = 256;                 // rows of a CTA pair's tile
 constexpr int kEpiWarps = 16;  // four a scheduler: with two the epilogue's latencies show
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr uint32_t kOperand = 128 * 128;    // 128 rows of 128 bytes: one operand tile of a CTA, 16 KB
 constexpr uint32_t kStaging = 2048;         // of an epilogue warp: 32 rows x 64 bytes
 constexpr int kBarBytes = 256;
-constexpr int kMaxMaps = 6, kMaxProblems = 3, kMaxStages = 6;
+constexpr int kMaxMaps = 6, kMaxProblems = 3, kMaxStages = 8;
 constexpr int kItemTable = 32;              // work items of a pair worked out once, at its start
 
 // What the kernel computes.
@@ -46,14 +46,20 @@ enum Mode {
   kGatedBack, // g, u as above and dh = DY Wd: C = dg, C2 = du
   kKeptBack   // the same with g, u read from the forward pass: dh alone is computed
 };
-template <int MODE>
+// Accumulator columns of a tile, TN: 256, or 128 where 256 would leave most pairs
+// without a tile. A narrow tile takes half the time a K block, and there are twice as
+// many; it reads half as much again from L2 for each product.
+template <int MODE, int TN>
 struct Shape {
+  static constexpr uint32_t kOperandB = TN * 64;  // TN / 2 rows of 128 bytes
   // x, dy, one of Wg / Wu, 64 columns of Wd per CTA and K block, else A and B
-  static constexpr uint32_t kStage = MODE == kGatedBack ? 3 * kOperand + kOperand / 2 : 2 * kOperand;
-  static constexpr int kStages = MODE == kGatedBack ? 3 : 6;
-  static constexpr int kBuffers = MODE == kGatedBack ? 1 : 2;  // accumulators of 384 or 256 columns in 512
+  static constexpr uint32_t kStage = MODE == kGatedBack ? 3 * kOperand + kOperand / 2 : kOperand + kOperandB;
+  static constexpr int kStages = MODE == kGatedBack ? 3 : TN == 256 ? 6 : 8;
+  static constexpr int kBuffers = MODE == kGatedBack ? 1 : 2;  // accumulators of 384 or TN columns in 512
   static constexpr uint32_t kSmem = kStage * kStages + kEpiWarps * kStaging + kBarBytes + 1024;
-  static constexpr int kColumns = MODE == kGated || MODE == kGatedBack ? 128 : kTileN;  // result columns per tile
+  static constexpr int kColumns = MODE == kGated || MODE == kGatedBack ? TN / 2 : TN;  // result columns per tile
+  static constexpr int kChunks = kColumns / 32;             // epilogue chunks of 32 result columns
+  static constexpr int kWarpChunks = (kChunks + 3) / 4;     // of a warp (four warps share a TMEM quadrant)
 };
 
 struct Problem {
@@ -69,11 +75,12 @@ struct Params {
   CUtensorMap map[kMaxMaps];
   Problem prob[kMaxProblems];
   int problems, items, maps;
+  bool narrow;                   // tiles of 128 accumulator columns
   int whole, splits;             // tiles done by one work item each; parts of each tile after those
   void *c2;                      // du
   float *gu;                     // kept projections, see gu_index
   const float *a_scales, *b_scales, *bias;
-  uint32_t *partial;             // raw sums: [tile - whole][part][kTileM][kTileN]
+  uint32_t *partial;             // raw sums: [tile - whole][part][kTileM][TN]
   int *err;
 };
 
@@ -81,7 +88,7 @@ struct Item {
   int prob, m0, n0, kb_begin, kb_end;
   uint32_t *partial;  // where raw sums go; nullptr: the item is a whole tile
 };
-template <int MODE>
+template <int MODE, int TN>
 __device__ __forceinline__ Item item_of(const Params &p, int it) {
   Item w;
   int tile = it, part = 0, parts = 1;
@@ -90,7 +97,7 @@ __device__ __forceinline__ Item item_of(const Params &p, int it) {
     parts = p.splits;
     part = (it - p.whole) % parts;
     tile = p.whole + (it - p.whole) / parts;
-    if (parts > 1) w.partial = p.partial + (size_t)(it - p.whole) * (kTileM * kTileN);
+    if (parts > 1) w.partial = p.partial + (size_t)(it - p.whole) * (kTileM * TN);
   }
   w.prob = 0;
 #pragma unroll
@@ -101,7 +108,7 @@ __device__ __forceinline__ Item item_of(const Params &p, int it) {
   tile -= q.first;
   const int group = tile / (8 * q.tiles_n), rows = min(8, q.tiles_m - 8 * group), t = tile - group * 8 * q.tiles_n;
   w.m0 = (8 * group + t % rows) * kTileM;
-  w.n0 = (t / rows) * Shape<MODE>::kColumns;
+  w.n0 = (t / rows) * Shape<MODE, TN>::kColumns;
   w.kb_begin = 0;
   w.kb_end = q.kb;
   if (parts > 1) {  // kb < 2^24 and parts < 2^7: the products fit 31 bits
@@ -156,9 +163,9 @@ __device__ __forceinline__ void gradients(float g, float u, float dh, float &dg,
   dg = dh * u * (sg * fmaf(g, 1.0f - sg, 1.0f));
 }
 
-template <int MODE, class T, bool A_MN, bool B_MN>
+template <int MODE, class T, bool A_MN, bool B_MN, int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense(const __grid_constant__ Params p) {
-  using S = Shape<MODE>;
+  using S = Shape<MODE, TN>;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = tc::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char *sm = smem_raw + (base - raw);
@@ -179,8 +186,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   // the pair's n-th work item: its divisions and parameter reads are not on the path of every tile
   __shared__ Item table[kItemTable];
   for (int i = threadIdx.x; i < kItemTable && pair + i * pairs < p.items; i += kThreads)
-    table[i] = item_of<MODE>(p, pair + i * pairs);
-  auto item = [&](int n) { return n < kItemTable ? table[n] : item_of<MODE>(p, pair + n * pairs); };
+    table[i] = item_of<MODE, TN>(p, pair + i * pairs);
+  auto item = [&](int n) { return n < kItemTable ? table[n] : item_of<MODE, TN>(p, pair + n * pairs); };
   const int items = pair < p.items ? (p.items - 1 - pair) / pairs + 1 : 0;
 
   dependents_may_start();
@@ -236,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           } else {
             const int seg = kb >= q.kb0 ? 1 : 0, k = (kb - (seg ? q.kb0 : 0)) * kElems;
             const CUtensorMap *a = &p.map[q.a[seg]], *b = &p.map[q.b[seg]];
-            const int m = w.m0 + 128 * rank, c = w.n0 + 128 * rank;
+            const int m = w.m0 + 128 * rank, c = w.n0 + TN / 2 * rank;
             if (A_MN) {
               tc::tma_load(dst, a, m, k, bar);
               tc::tma_load(dst + kOperand / 2, a, m + 64, k, bar);
@@ -245,7 +252,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
             }
             if (B_MN) {
               tc::tma_load(dst + kOperand, b, c, k, bar);
-              tc::tma_load(dst + kOperand + kOperand / 2, b, c + 64, k, bar);
+              if (TN == 256) tc::tma_load(dst + kOperand + kOperand / 2, b, c + 64, k, bar);
             } else {
               tc::tma_load(dst + kOperand, b, k, c, bar);
             }
@@ -263,7 +270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
     if (rank == 0 && lane == 0) {
       constexpr bool kI8 = MODE == kInt8;
       constexpr uint32_t kAb = kI8 || std::is_same<T, __nv_bfloat16>::value ? 1 : 0;  // s8 / bf16, or f16
-      constexpr uint32_t kId = tc::idesc(kI8 ? 2 : 1, kAb, A_MN, B_MN, 256);
+      constexpr uint32_t kId = tc::idesc(kI8 ? 2 : 1, kAb, A_MN, B_MN, TN);
       constexpr uint32_t kIdDh = tc::idesc(1, kAb, false, true, 128);
       int n = 0;
       bool ok = true;
@@ -333,21 +340,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       if constexpr (MODE == kPlain || MODE == kInt8) {
         const bool split = w.partial != nullptr;
         const float sa = MODE == kInt8 && !split && lane < rows ? p.a_scales[row0 + lane] : 0.0f;
-        for (int j = 0; j < 2; ++j) {
-          const int col = 64 * part + 32 * j, c0 = w.n0 + col;
+        for (int j = 0; j < S::kWarpChunks; ++j) {
+          const int col = 32 * (S::kWarpChunks * part + j), c0 = w.n0 + col;
           uint32_t r[32];
           tc::tmem_ld32(acc + col, r);
           tc::wait_ld(r);
-          if (j == 1) release();
+          if (j == S::kWarpChunks - 1) release();
           if (rows <= 0 || c0 >= q.n) continue;
           if (split) {  // raw 32-bit sums, float or int
-            uint32_t *dst = w.partial + (128 * rank + 32 * quad) * kTileN + col;
+            uint32_t *dst = w.partial + (128 * rank + 32 * quad) * TN + col;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               Chunk<float, 4> v[4];
 #pragma unroll
               for (int i = 0; i < 16; ++i) v[i / 4].e[i % 4] = __uint_as_float(r[16 * h + i]);
-              store_rows<float>(stage, lane, v, reinterpret_cast<float *>(dst) + 16 * h, kTileN, rows, 16, true);
+              store_rows<float>(stage, lane, v, reinterpret_cast<float *>(dst) + 16 * h, TN, rows, 16, true);
             }
             continue;
           }
@@ -379,8 +386,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           }
         }
       } else if constexpr (MODE == kKeptBack) {
-        for (int j = 0; j < 2; ++j) {
-          const int col = 64 * part + 32 * j, c0 = w.n0 + col;
+        for (int j = 0; j < S::kWarpChunks; ++j) {
+          const int col = 32 * (S::kWarpChunks * part + j), c0 = w.n0 + col;
           const bool live = rows > 0 && c0 < q.n;
           Chunk<T, kPer> out[4], out2[4];
 #pragma unroll
@@ -404,7 +411,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
             }
             tc::tmem_ld16(acc + col + 16 * h, dh);
             tc::wait_ld(dh);
-            if (j == 1 && h == 1) release();
+            if (j == S::kWarpChunks - 1 && h == 1) release();
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               float dg[8], du[8];
@@ -422,16 +429,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
         }
       } else {
         const int col = 32 * part, c0 = w.n0 + col;
-        const bool live = rows > 0 && c0 < q.n;
+        const bool mine = part < S::kChunks, live = mine && rows > 0 && c0 < q.n;
+        if (!mine) release();
         const long long at = row0 * q.ldc + c0;
         // only the 16-bit types have these modes
         using H = typename std::conditional<sizeof(T) == 2, T, __half>::type;
         Chunk<H, 8> out[4], out2[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          if (!mine) break;
           uint32_t g[16], u[16], dh[16];
           tc::tmem_ld16(acc + col + 16 * h, g);
-          tc::tmem_ld16(acc + 128 + col + 16 * h, u);
+          tc::tmem_ld16(acc + TN / 2 + col + 16 * h, u);
           if (MODE == kGatedBack) tc::tmem_ld16(acc + 256 + col + 16 * h, dh);
           tc::wait_ld(g);
           tc::wait_ld(u);
@@ -478,25 +487,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
 }
 
 // C of the split tiles = the sum of their parts, in order; 8-bit products get their
-// scales here. A block does 16 rows of a tile, a thread 4 columns of 4 of them.
-template <int MODE, class T>
+// scales here. A block does 16 or 32 rows of a tile, a thread 4 columns of 4 of them.
+template <int MODE, class T, int TN>
 __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) {
   dependents_may_start();
   wait_for_predecessors();
-  const Item w = item_of<MODE>(p, p.whole + blockIdx.y * p.splits);
+  constexpr int kQuads = TN / 4;  // of columns
+  const Item w = item_of<MODE, TN>(p, p.whole + blockIdx.y * p.splits);
   const Problem &q = p.prob[w.prob];
-  const int col = w.n0 + 4 * (threadIdx.x & 63);
+  const int col = w.n0 + 4 * (threadIdx.x % kQuads);
   if (col >= q.n) return;
   const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % (4 * sizeof(T)) == 0 && col + 4 <= q.n;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = 16 * blockIdx.x + 4 * i + (threadIdx.x >> 6), row = w.m0 + r;
+    const int r = (4 * blockIdx.x + i) * (256 / kQuads) + threadIdx.x / kQuads, row = w.m0 + r;
     if (row >= q.m) break;
     float f[4] = {0, 0, 0, 0};
     int s[4] = {0, 0, 0, 0};
 #pragma unroll 4
     for (int k = 0; k < p.splits; ++k) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(w.partial + ((size_t)k * kTileM + r) * kTileN + col - w.n0);
+      const uint4 v = *reinterpret_cast<const uint4 *>(w.partial + ((size_t)k * kTileM + r) * TN + col - w.n0);
       const uint32_t e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -620,40 +630,56 @@ class Dense {
     return m;
   }
 
-  // Work items of the problems. The tiles after the last whole wave are split along K
+  // Work items of the problems. Tiles are narrow where 256 columns would give half of
+  // the pairs or fewer a tile. The tiles after the last whole wave are split along K
   // where that leaves no pair idle and saves more than the join costs: 24 K blocks
   // take a pair about 7 us, a join with its launch 4 to 5.
   template <int MODE>
   void plan(Params &p, bool may_split) {
-    long long tiles = 0;
+    long long tiles = count<MODE, 256>(p);
+    p.narrow = MODE != kGatedBack && 2 * tiles <= kPairs;
+    if (p.narrow) tiles = count<MODE, 128>(p);
     int kb = 1 << 30;
-    for (int i = 0; i < p.problems; ++i) {
-      Problem &q = p.prob[i];
-      q.tiles_m = (q.m - 1) / kTileM + 1;
-      q.tiles_n = (q.n - 1) / Shape<MODE>::kColumns + 1;
-      q.first = int(tiles);
-      tiles += (long long)q.tiles_m * q.tiles_n;
-      kb = std::min(kb, q.kb);
-      if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
-    }
+    for (int i = 0; i < p.problems; ++i) kb = std::min(kb, p.prob[i].kb);
+    if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
     const int rest = int(tiles % kPairs);
     p.splits = may_split && rest > 0 && kb >= 24 ? std::max(1, std::min(kPairs / rest, kb / 8)) : 1;
     p.whole = int(tiles) - (p.splits > 1 ? rest : 0);
     p.items = p.whole + (p.splits > 1 ? rest * p.splits : 0);
-    p.partial = p.splits > 1
-                    ? static_cast<uint32_t *>(scratch_.take((long long)rest * p.splits * kTileM * kTileN * 4))
-                    : nullptr;
+    p.partial = p.splits > 1 ? static_cast<uint32_t *>(scratch_.take((long long)rest * p.splits * kTileM *
+                                                                    (p.narrow ? 128 : 256) * 4))
+                             : nullptr;
+  }
+  template <int MODE, int TN>
+  static long long count(Params &p) {
+    long long tiles = 0;
+    for (int i = 0; i < p.problems; ++i) {
+      Problem &q = p.prob[i];
+      q.tiles_m = (q.m - 1) / kTileM + 1;
+      q.tiles_n = (q.n - 1) / Shape<MODE, TN>::kColumns + 1;
+      q.first = int(std::min<long long>(tiles, 1 << 30));
+      tiles += (long long)q.tiles_m * q.tiles_n;
+    }
+    return tiles;
   }
 
   template <int MODE, class T, bool A_MN, bool B_MN>
   void run(Params &p) {
-    const void *fn = reinterpret_cast<const void *>(&k_dense<MODE, T, A_MN, B_MN>);
-    allow_dynamic_smem(fn, Shape<MODE>::kSmem);
+    if constexpr (MODE != kGatedBack) {
+      if (p.narrow) return run_tiles<MODE, T, A_MN, B_MN, 128>(p);
+    }
+    run_tiles<MODE, T, A_MN, B_MN, 256>(p);
+  }
+  template <int MODE, class T, bool A_MN, bool B_MN, int TN>
+  void run_tiles(Params &p) {
+    using S = Shape<MODE, TN>;
+    allow_dynamic_smem(reinterpret_cast<const void *>(&k_dense<MODE, T, A_MN, B_MN, TN>), S::kSmem);
     p.err = gave_up_flag();
-    launch(k_dense<MODE, T, A_MN, B_MN>, 2 * std::min(kPairs, p.items), kThreads, Shape<MODE>::kSmem, stream_, p);
+    launch(k_dense<MODE, T, A_MN, B_MN, TN>, 2 * std::min(kPairs, p.items), kThreads, S::kSmem, stream_, p);
     if constexpr (MODE == kPlain || MODE == kInt8) {
       if (p.splits == 1) return;
-      launch(k_join<MODE, T>, dim3(kTileM / 16, (p.items - p.whole) / p.splits), 256, 0, stream_, p);
+      const int rows = 4 * (256 / (TN / 4));  // of a block
+      launch(k_join<MODE, T, TN>, dim3(kTileM / rows, (p.items - p.whole) / p.splits), 256, 0, stream_, p);
     }
   }
 
@@ -695,7 +721,7 @@ void int8_linear(Dense &d, const so3lr_int8_linear_args &a) {
   if (d.dry()) return;
   p.maps = 2;
   p.map[0] = d.map(x, 128);
-  p.map[1] = d.map(w, 128);
+  p.map[1] = d.map(w, p.narrow ? 64 : 128);
   d.run<kInt8, O, false, false>(p);
 }
 
@@ -730,8 +756,8 @@ void feed_forward(Dense &d, const so3lr_feed_forward_args &a) {
     if (!d.dry()) {
       p.maps = 3;
       p.map[0] = d.map(x, 128);
-      p.map[1] = d.map(g, 128);
-      p.map[2] = d.map(u, 128);
+      p.map[1] = d.map(g, p.narrow ? 64 : 128);
+      p.map[2] = d.map(u, p.narrow ? 64 : 128);
       d.run<kGated, T, false, false>(p);
     }
   }
@@ -750,7 +776,7 @@ void feed_forward(Dense &d, const so3lr_feed_forward_args &a) {
   if (d.dry()) return;
   p.maps = 2;
   p.map[0] = d.map(hr, 128);
-  p.map[1] = d.map(w, 128);
+  p.map[1] = d.map(w, p.narrow ? 64 : 128);
   d.run<kPlain, T, false, false>(p);
 }
 
