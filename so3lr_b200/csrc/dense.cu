@@ -906,11 +906,11 @@ void check_gave_up() {
 }
 
 long long int8_linear_bytes(const so3lr_int8_linear_args &a) {
-  if (a.rows <= kFewRows) return 0;
+  if (few_rows(a)) return 0;
   return dry_run(a, 1, [&](Dense &d) { int8_linear<float>(d, a); });
 }
 void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s) {
-  if (a.rows <= kFewRows) return launch_int8_linear_few(a, s);
+  if (few_rows(a)) return launch_int8_linear_few(a, s);
   Dense d(workspace, 1, s, false);
   if (a.out_dtype == SO3LR_FLOAT32)
     int8_linear<float>(d, a);
@@ -919,16 +919,18 @@ void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaSt
 }
 
 long long feed_forward_keep(const so3lr_feed_forward_args &a) {
-  return a.rows > kFewRows && keeps(a.width) ? (a.rows + 31) / 32 * 32 * a.hidden * 8 : 0;
+  so3lr_feed_forward_args plain = a;
+  plain.gu = nullptr;
+  return !few_rows(plain) && keeps(a.width) ? (a.rows + 31) / 32 * 32 * a.hidden * 8 : 0;
 }
 // rows of the hidden layer of a few rows, on 16-byte boundaries
 static long long few_stride(const so3lr_feed_forward_args &a) { return (a.hidden + 7) / 8 * 8; }
 long long feed_forward_bytes(const so3lr_feed_forward_args &a) {
-  if (a.rows <= kFewRows && !a.gu) return a.h ? 0 : a.rows * few_stride(a) * 2;
+  if (few_rows(a)) return a.h ? 0 : a.rows * few_stride(a) * 2;
   return dry_run(a, 2, [&](Dense &d) { feed_forward<__half>(d, a); });
 }
 void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s) {
-  if (a.rows <= kFewRows && !a.gu)
+  if (few_rows(a))
     return launch_feed_forward_few(a, a.h ? a.h : workspace, a.h ? a.hidden : few_stride(a), s);
   Dense d(workspace, 2, s, false);
   by_half(a.dtype, [&](auto t) { feed_forward<decltype(t)>(d, a); });

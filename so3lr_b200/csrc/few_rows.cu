@@ -1,5 +1,6 @@
-// Dense products of the feed-forward layers for up to kFewRows rows (single atoms or
-// tokens, small batches). All that counts is reading the weights once, at HBM's rate:
+// Dense products of the feed-forward layers for few rows (single atoms or tokens,
+// small batches; the rule is in layers.hpp). All that counts is reading the weights
+// once for each 16 rows, from HBM or, for small weights, from L2:
 // a block takes 8 output channels and its warps split the contraction, so that a
 // 4096 x 4096 weight has 512 blocks. The products run on warp-level MMAs
 // (m16n8k16 / m16n8k32, rows as M, channels as N) straight from registers: a tile of
@@ -83,10 +84,10 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   constexpr int kPer = 16 / sizeof(E), kUnroll = GATED ? 2 : 4, kOut = GATED ? 2 : 1;
   __shared__ Acc part[max_warps(TWO)][kOut][TWO ? 16 : 8][8];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n = blockIdx.x * 8 + g;
+  const int n = blockIdx.x * 8 + g, row0 = blockIdx.y * 16, rows = min(16, a.rows - row0);
   const E *w = static_cast<const E *>(a.w) + n * a.w_stride, *w2 = static_cast<const E *>(a.w2) + n * a.w2_stride;
-  const E *x0 = static_cast<const E *>(a.x) + g * a.x_stride, *x1 = x0 + 8 * a.x_stride;
-  const bool live_n = n < a.n, live0 = g < a.rows, live1 = TWO && g + 8 < a.rows;
+  const E *x0 = static_cast<const E *>(a.x) + (row0 + g) * a.x_stride, *x1 = x0 + 8 * a.x_stride;
+  const bool live_n = n < a.n, live0 = g < rows, live1 = TWO && g + 8 < rows;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer);
   const int begin = int((long long)steps * warp / warps), end = int((long long)steps * (warp + 1) / warps);
   dependents_may_start();
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 8 * a.rows; i += blockDim.x) {
+  for (int i = threadIdx.x; i < 8 * rows; i += blockDim.x) {
     const int row = i >> 3, c = blockIdx.x * 8 + (i & 7);
     if (c >= a.n) continue;
     Acc sum[kOut] = {};
@@ -140,12 +141,12 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
       for (int o = 0; o < kOut; ++o) sum[o] += part[k][o][row][i & 7];
     float y;
     if (kInt8)
-      y = fmaf(float(sum[0]) * a.a_scales[row], a.b_scales[c], a.bias ? a.bias[c] : 0.0f);
+      y = fmaf(float(sum[0]) * a.a_scales[row0 + row], a.b_scales[c], a.bias ? a.bias[c] : 0.0f);
     else if (GATED)
       y = silu_f32(float(sum[0])) * float(sum[kOut - 1]);
     else
       y = float(sum[0]);
-    static_cast<O *>(a.y)[row * a.y_stride + c] = from_float<O>(y);
+    static_cast<O *>(a.y)[(row0 + row) * a.y_stride + c] = from_float<O>(y);
   }
 }
 
@@ -162,8 +163,8 @@ void run(const FewArgs &a, cudaStream_t s) {
   // where the blocks alone would leave too few loads in flight. One row, 2048 channels
   // of 8192 bfloat16 (256 blocks): 12.3 us with 8, 9.3 us with 16; 4096 channels of
   // 4096 bytes (512 blocks): 5.6 us with 8, 7.0 us with 16.
-  const unsigned grid = unsigned((a.n + 7) / 8);
-  const int most = grid < 2 * kSmCount ? max_warps(a.rows > 8) : 8;
+  const dim3 grid(unsigned((a.n + 7) / 8), unsigned((a.rows + 15) / 16));
+  const int most = grid.x * grid.y < 2 * kSmCount ? max_warps(a.rows > 8) : 8;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer), warps = std::max(1, std::min(most, steps / 4));
   const unsigned block = unsigned(32 * warps);
   if (a.rows > 8)

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
 // dx = rstd (a - xh mean(a xh)) + ds with a = dy w, xh = s rstd; each block also
 // sums dy xh over its rows (a fixed set, in order) into one row of `partial`.
 template <class T, class W, int VEC, int N, int MAXT>
-__global__ void __launch_bounds__(MAXT) k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial) {
+__global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : 1) k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial) {
   constexpr bool WARP = MAXT == 32 * kWarpRows;
   __shared__ float2 slot[2][32];
   extern __shared__ float column[];  // WARP: kWarpRows x width
@@ -545,7 +545,7 @@ void norm_forward(const so3lr_rms_norm_args &a, cudaStream_t s) {
 int walking_blocks(long long rows, int threads) {
   const bool warp = threads == 32;
   const long long want = warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
-  const int per_sm = warp ? 4 : std::max(1, std::min(4, 1536 / threads));
+  const int per_sm = warp ? 4 : std::max(1, std::min(8, 1024 / threads));
   return int(std::min<long long>(want, (long long)kSmCount * per_sm));
 }
 

@@ -192,7 +192,8 @@ def _codes(seed, rows, k):
 INT8_SIZES = [(1, 1, 1), (1, 64, 64), (1, 1531, 4096), (2, 33, 17), (3, 100, 1000), (5, 513, 129), (8, 256, 2048),
               (9, 128, 128), (16, 136, 96), (17, 250, 384), (31, 1000, 1000), (33, 64, 8192), (64, 512, 512),
               (100, 128, 4097), (127, 129, 255), (128, 256, 256), (129, 257, 300), (333, 1531, 1000),
-              (1000, 72, 2048), (2500, 700, 130)]
+              (1000, 72, 2048), (2500, 700, 130), (257, 1, 1), (300, 129, 127),
+              (600, 256, 4096), (257, 64, 64), (512, 2100, 3200)]
 
 
 @pytest.mark.parametrize("rows, n, k", INT8_SIZES)
@@ -226,9 +227,9 @@ def test_int8_linear_extremes(layers):
 
 def test_int8_linear_layouts(layers):
     """Unaligned views and broadcast rows give what their copies give, bit for bit."""
-    wa, wb = _codes(1, 70, 600), _codes(2, 90, 600)
-    sa, sb = torch.rand(70, device="cuda"), torch.rand(90, device="cuda")
-    for rows in (1, 5, 30, 70):
+    wa, wb = _codes(1, 280, 600), _codes(2, 90, 600)
+    sa, sb = torch.rand(280, device="cuda"), torch.rand(90, device="cuda")
+    for rows in (1, 5, 30, 70, 280):
         for a, b in ((wa[:rows, 1:513], wb[:, 7:519]), (wa[:rows, :512], wb[:, 16:528]), (wa[:rows, 3:500], wb[:, 3:500]),
                      (wa[:1, :512].expand(rows, 512), wb[:, :512]), (wa[:rows, :512], wb[:1, :512].expand(90, 512))):
             y = layers.int8_linear(a, sa[:rows], b, sb, out_dtype=torch.float32)
@@ -238,7 +239,7 @@ def test_int8_linear_layouts(layers):
             assert torch.equal(y, y2)
     y = layers.int8_linear(wa[:0], sa[:0], wb, sb)
     assert y.shape == (0, 90)
-    y = layers.int8_linear(wa.view(7, 10, 600), sa, wb, sb, out_dtype=torch.float32)
+    y = layers.int8_linear(wa[:70].view(7, 10, 600), sa[:70], wb, sb, out_dtype=torch.float32)
     assert y.shape == (7, 10, 90)
 
 
@@ -321,7 +322,7 @@ def _ffn_ref(x, wg, wu, wd, dy, dtype):
 
 FFN_SIZES = [(1, 1, 1), (1, 64, 64), (1, 128, 512), (2, 33, 70), (3, 128, 300), (4, 256, 1024), (5, 7, 3), (8, 520, 1368),
              (9, 256, 256), (17, 100, 333), (33, 128, 512), (64, 64, 4096), (100, 136, 200), (128, 128, 128),
-             (129, 130, 131), (192, 256, 1024), (257, 264, 520), (777, 520, 1368), (3000, 256, 512), (5, 1024, 72), (40, 1024, 200),
+             (129, 130, 131), (192, 256, 1024), (257, 264, 520), (777, 520, 1368), (3000, 256, 512), (5, 1024, 72), (40, 1024, 200), (260, 64, 96), (400, 100, 90), (300, 72, 4100), (257, 1, 1),
              (333, 1032, 260), (300, 2048, 131)]
 
 
@@ -341,10 +342,10 @@ def test_feed_forward_and_gradients(layers, rows, width, hidden, dtype):
 
 
 def test_feed_forward_saved_of_another_call(layers):
-    x, wg, wu, wd, dy = _ffn_inputs(40, 1024, 64, torch.bfloat16)
+    x, wg, wu, wd, dy = _ffn_inputs(300, 1024, 64, torch.bfloat16)
     _, saved = layers.feed_forward_train(x, wg, wu, wd)
     assert saved[5] is not None
-    for wrong in (saved[:4] + (saved[4][:39], saved[5]), saved[:5] + (saved[5][:-1],), (x[:8],) + saved[1:]):
+    for wrong in (saved[:4] + (saved[4][:299], saved[5]), saved[:5] + (saved[5][:-1],), (x[:8],) + saved[1:]):
         with pytest.raises(ValueError):
             layers.feed_forward_backward(dy[:wrong[0].shape[0]], wrong)
     # without the kept projections they are computed again: the same gradients within their roundings
@@ -356,11 +357,12 @@ def test_feed_forward_saved_of_another_call(layers):
 def test_feed_forward_layouts(layers):
     """Unaligned and strided views, a broadcast row, leading dimensions, no rows."""
     dtype = torch.float16
-    big, dbig = _rand(1, 300, 200, dtype=dtype), _rand(6, 300, 200, dtype=dtype)
+    big, dbig = _rand(1, 600, 200, dtype=dtype), _rand(6, 600, 200, dtype=dtype)
     wgb, wub, wdb = (_rand(k, 300, 400, dtype=dtype, scale=0.1) for k in (2, 3, 4))
     for sl_x, sl_w in ((slice(0, 136), slice(0, 136)), (slice(1, 137), slice(5, 141)), (slice(3, 134), slice(8, 139))):
         width = sl_x.stop - sl_x.start
-        for x, dy in ((big[:150, sl_x], dbig[:150, sl_x]), (big[::2, sl_x], dbig[150:, sl_x]),
+        for x, dy in ((big[:300, sl_x], dbig[:300, sl_x]), (big[::2, sl_x], dbig[300:, sl_x]),
+                      (big[:150, sl_x], dbig[:150, sl_x]), (big[:1, sl_x].expand(270, width), dbig[:270, sl_x]),
                       (big[:1, sl_x].expand(40, width), dbig[:40, sl_x]), (big[:3, sl_x], dbig[:3, sl_x])):
             wg, wu, wd = wgb[:200, sl_w], wub[100:300, sl_w], wdb[:width, 7:207]
             ref = _ffn_ref(x, wg, wu, wd, dy, dtype)
@@ -376,7 +378,7 @@ def test_feed_forward_layouts(layers):
     assert y.shape == (0, 64) and grads[0].shape == (0, 64) and all(bool((g == 0).all()) for g in grads[1:])
 
 
-@pytest.mark.parametrize("rows", [2, 20, 150])
+@pytest.mark.parametrize("rows", [2, 20, 150, 300])
 def test_feed_forward_non_finite_rows_stay_apart(layers, rows):
     x, wg, wu, wd, _ = _ffn_inputs(rows, 96, 160, torch.bfloat16)
     clean = layers.feed_forward(x, wg, wu, wd)
@@ -388,7 +390,7 @@ def test_feed_forward_non_finite_rows_stay_apart(layers, rows):
 
 
 def test_feed_forward_repeats_streams_and_graphs(layers):
-    for rows in (1, 6, 40, 700):
+    for rows in (1, 6, 40, 260, 700):
         x, wg, wu, wd, dy = _ffn_inputs(rows, 256, 1024, torch.bfloat16)
 
         def step():

@@ -132,7 +132,7 @@ def test_feed_forward_refusals(lib, change, message):
 
 
 def test_workspaces_are_checked(lib):
-    a = _FeedForward(rows=200, width=64, hidden=128, dtype=1, x=4096, x_stride=64, w_gate=4096,
+    a = _FeedForward(rows=500, width=64, hidden=128, dtype=1, x=4096, x_stride=64, w_gate=4096,
                             w_gate_stride=64, w_up=4096, w_up_stride=64, w_down=4096, w_down_stride=128, y=4096,
                             y_stride=64)
     need = lib.so3lr_feed_forward_workspace(a)
@@ -146,11 +146,11 @@ def test_workspaces_are_checked(lib):
 
 def test_projections_are_kept_for_wide_layers(lib):
     """Nothing for narrow layers or a few rows; else whole blocks of 32 rows of two float32 values."""
-    a = _FeedForward(rows=100, width=4096, hidden=24, dtype=1)
-    assert lib.so3lr_feed_forward_keep(a) == 128 * 24 * 2 * 4
+    a = _FeedForward(rows=1000, width=4096, hidden=24, dtype=1)
+    assert lib.so3lr_feed_forward_keep(a) == 1024 * 24 * 2 * 4
     a.rows = 1
     assert lib.so3lr_feed_forward_keep(a) == 0
-    a.rows, a.width = 100, 64
+    a.rows, a.width = 1000, 64
     assert lib.so3lr_feed_forward_keep(a) == 0
     a.width = 0
     assert lib.so3lr_feed_forward_keep(a) == -1
