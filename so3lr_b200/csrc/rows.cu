@@ -581,12 +581,19 @@ int backward_parts(const so3lr_rms_norm_backward_args &a) {
 template <class T, class W, int VEC, int N>
 void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int grid, cudaStream_t s) {
   const int threads = row_threads(a.width, VEC * N);
-  if (threads == 32)
-    launch(k_rms_norm_backward<T, W, VEC, N, 32 * kWarpRows>, grid, 32 * kWarpRows, kWarpRows * a.width * sizeof(float), s, a, partial);
-  else if (threads <= 512)
-    launch(k_rms_norm_backward<T, W, VEC, N, 512>, grid, threads, 0, s, a, partial);
-  else
-    launch(k_rms_norm_backward<T, W, VEC, N, 1024>, grid, threads, 0, s, a, partial);
+  if (threads == 32) {
+    launch(k_rms_norm_backward<T, W, VEC, N, 32 * kWarpRows>, grid, 32 * kWarpRows,
+           kWarpRows * a.width * sizeof(float), s, a, partial);
+    return;
+  }
+  // rows of a block that do not go through the ring: unaligned ones, and those too long for it
+  if constexpr (VEC == 1 && N == 8) {
+    if (threads <= 512) {
+      launch(k_rms_norm_backward<T, W, VEC, N, 512>, grid, threads, 0, s, a, partial);
+      return;
+    }
+  }
+  launch(k_rms_norm_backward<T, W, VEC, N, 1024>, grid, threads, 0, s, a, partial);
 }
 template <class T, class W>
 void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, const RingPlan &r, cudaStream_t s) {
