@@ -85,14 +85,16 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   __shared__ Acc part[max_warps(TWO)][kOut][TWO ? 16 : 8][8];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n = blockIdx.x * 8 + g, row0 = blockIdx.y * 16, rows = min(16, a.rows - row0);
-  const E *w = static_cast<const E *>(a.w) + n * a.w_stride, *w2 = static_cast<const E *>(a.w2) + n * a.w2_stride;
-  const E *x0 = static_cast<const E *>(a.x) + (row0 + g) * a.x_stride, *x1 = x0 + 8 * a.x_stride;
-  const bool live_n = n < a.n, live0 = g < rows, live1 = TWO && g + 8 < rows;
+  // lanes beyond the last row or channel read it again; their results are not written
+  const int cn = min(n, a.n - 1);
+  const E *w = static_cast<const E *>(a.w) + cn * a.w_stride, *w2 = static_cast<const E *>(a.w2) + cn * a.w2_stride;
+  const E *x0 = static_cast<const E *>(a.x) + (row0 + min(g, rows - 1)) * a.x_stride;
+  const E *x1 = static_cast<const E *>(a.x) + (row0 + min(g + 8, rows - 1)) * a.x_stride;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer);
   const int begin = int((long long)steps * warp / warps), end = int((long long)steps * (warp + 1) / warps);
   dependents_may_start();
   // the first weights on their way to L2, which needs no order with the kernel before
-  if (ALIGNED && live_n) {
+  if (ALIGNED) {
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int k = ((begin + i) * 4 + t) * kPer;
@@ -104,23 +106,42 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   }
   wait_for_predecessors();
   Acc acc[kOut][4] = {};
-  for (int st = begin; st < end; st += kUnroll) {
-    uint4 vw[kUnroll], vw2[GATED ? kUnroll : 1], v0[kUnroll], v1[TWO ? kUnroll : 1];
-    const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  auto multiply = [&](const uint4 &v0, const uint4 &v1, const uint4 &vw, const uint4 &vw2) {
+    mma_step<E>(acc[0], v0, TWO ? v1 : zero, vw);
+    if (GATED) mma_step<E>(acc[kOut - 1], v0, TWO ? v1 : zero, vw2);
+  };
+  int st = begin;
+  if (ALIGNED) {  // whole groups of steps, all four lanes of a row inside it: loads at constant offsets
+    const int whole = min(end, a.k / (4 * kPer));
+    for (; st + kUnroll <= whole; st += kUnroll) {
+      const int k = (st * 4 + t) * kPer;
+      uint4 vw[kUnroll], vw2[GATED ? kUnroll : 1], v0[kUnroll], v1[TWO ? kUnroll : 1];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int k = ((st + i) * 4 + t) * kPer;
-      const bool in = st + i < end && k < a.k;
-      vw[i] = in && live_n ? load16<E, ALIGNED, true>(w, k, a.k) : zero;
-      if (GATED) vw2[i] = in && live_n ? load16<E, ALIGNED, true>(w2, k, a.k) : zero;
-      v0[i] = in && live0 ? load16<E, ALIGNED, false>(x0, k, a.k) : zero;
-      if (TWO) v1[i] = in && live1 ? load16<E, ALIGNED, false>(x1, k, a.k) : zero;
-    }
+      for (int i = 0; i < kUnroll; ++i) {
+        vw[i] = load16<E, true, true>(w, k + i * 4 * kPer, 1 << 30);
+        if (GATED) vw2[i] = load16<E, true, true>(w2, k + i * 4 * kPer, 1 << 30);
+      }
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      mma_step<E>(acc[0], v0[i], TWO ? v1[i] : zero, vw[i]);
-      if (GATED) mma_step<E>(acc[kOut - 1], v0[i], TWO ? v1[i] : zero, vw2[i]);
+      for (int i = 0; i < kUnroll; ++i) {
+        v0[i] = load16<E, true, false>(x0, k + i * 4 * kPer, 1 << 30);
+        if (TWO) v1[i] = load16<E, true, false>(x1, k + i * 4 * kPer, 1 << 30);
+      }
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) multiply(v0[i], TWO ? v1[i] : zero, vw[i], GATED ? vw2[i] : zero);
     }
+  }
+#pragma unroll 2
+  for (; st < end; ++st) {
+    const int k = (st * 4 + t) * kPer;
+    uint4 vw = zero, vw2 = zero, v0 = zero, v1 = zero;
+    if (k < a.k) {
+      vw = load16<E, ALIGNED, true>(w, k, a.k);
+      if (GATED) vw2 = load16<E, ALIGNED, true>(w2, k, a.k);
+      v0 = load16<E, ALIGNED, false>(x0, k, a.k);
+      if (TWO) v1 = load16<E, ALIGNED, false>(x1, k, a.k);
+    }
+    multiply(v0, v1, vw, vw2);
   }
 #pragma unroll
   for (int o = 0; o < kOut; ++o) {
