@@ -632,8 +632,8 @@ class Dense {
 
   // Work items of the problems. Tiles are narrow where 256 columns would give half of
   // the pairs or fewer a tile. The tiles after the last whole wave are split along K
-  // where that leaves no pair idle and saves more than the join costs: 24 K blocks
-  // take a pair about 7 us, a join with its launch 4 to 5.
+  // where that saves more than the join costs: 16 K blocks take a pair 5 us (28 of a
+  // narrow tile), a join with its launch 4 to 5.
   template <int MODE>
   void plan(Params &p, bool may_split) {
     long long tiles = count<MODE, 256>(p);
@@ -643,7 +643,9 @@ class Dense {
     for (int i = 0; i < p.problems; ++i) kb = std::min(kb, p.prob[i].kb);
     if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
     const int rest = int(tiles % kPairs);
-    p.splits = may_split && rest > 0 && kb >= 24 ? std::max(1, std::min(kPairs / rest, kb / 8)) : 1;
+    int splits = may_split && rest > 0 ? std::max(1, std::min(kPairs / rest, kb / 8)) : 1;
+    if (kb - kb / splits < (p.narrow ? 28 : 16)) splits = 1;
+    p.splits = splits;
     p.whole = int(tiles) - (p.splits > 1 ? rest : 0);
     p.items = p.whole + (p.splits > 1 ? rest * p.splits : 0);
     p.partial = p.splits > 1 ? static_cast<uint32_t *>(scratch_.take((long long)rest * p.splits * kTileM *

@@ -455,6 +455,31 @@ def test_blocks_train_and_serve(layers):
     assert off <= 4 * 3 ** 0.5 / (36 * 12 ** 0.5), off
 
 
+def test_autograd_hands_over_any_gradient(layers):
+    """Broadcast and transposed gradients, an output that nothing reads, leading dimensions."""
+    x, r = _rand(1, 2, 9, 64, dtype=torch.bfloat16), _rand(2, 2, 9, 64, dtype=torch.bfloat16)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for use in (lambda y, s: y.sum(), lambda y, s: s.sum(), lambda y, s: (y.transpose(1, 2) * 2).sum() + s.sum()):
+        leaf, other = x.clone().requires_grad_(), r.clone().requires_grad_()
+        w.grad = None
+        use(*layers.rms_norm(leaf, w, other)).backward()
+        xd, rd, wd = x.float().requires_grad_(), r.float().requires_grad_(), w.detach().clone().requires_grad_()
+        s = ((xd + rd).bfloat16().float() - (xd + rd)).detach() + (xd + rd)  # rounded, with the sum's gradient
+        y = s * torch.rsqrt(s.square().mean(-1, keepdim=True) + 1e-6) * wd
+        use(y, s).backward()
+        assert torch.equal(leaf.grad, other.grad)
+        _within(leaf.grad, xd.grad.double(), 2 * U[torch.bfloat16] * (xd.grad.double().abs() + 0.1), "dx")
+        if wd.grad is not None and bool((wd.grad != 0).any()):
+            _within(w.grad, wd.grad.double(), 1e-3 * (1 + wd.grad.double().abs()), "dweight")
+    ws = [t.requires_grad_() for t in _ffn_inputs(18, 64, 96, torch.bfloat16)[1:4]]
+    leaf = x.clone().requires_grad_()
+    layers.feed_forward(leaf, *ws).sum().backward()
+    _, saved = layers.feed_forward_train(x.view(18, 64), *(t.detach() for t in ws))
+    grads = layers.feed_forward_backward(torch.ones(18, 64, device="cuda", dtype=torch.bfloat16), saved)
+    for got, want in zip((leaf.grad.view(18, 64), *(t.grad for t in ws)), grads):
+        assert torch.equal(got, want)
+
+
 # --------------------------------------------------------------------- refusals
 def test_refusals(layers):
     from so3lr_b200 import So3lrError
