@@ -58,23 +58,25 @@ def main() -> None:
     residual = x.roll(1, 0)
     block = layers.FeedForwardBlock(WIDTH, HIDDEN)
     target = residual + torch.sin(2 * x.float() + x.float().roll(1, 1)).bfloat16()
-    master = [p.detach().float() for p in block.parameters()]  # float32 weights behind the block's own
+    master = [p.detach().float().requires_grad_() for p in block.parameters()]  # what the optimiser updates
+    adam = torch.optim.Adam(master, lr=2e-3)
 
-    def step(lr: float) -> float:
+    def step() -> float:
         out, stream = block(x, residual)
         loss = (out + stream - target - x).float().square().mean()
-        for p in block.parameters():
-            p.grad = None
+        block.zero_grad()
         loss.backward()
+        for p, m in zip(block.parameters(), master):
+            m.grad = p.grad.float()
+        adam.step()
         with torch.no_grad():
             for p, m in zip(block.parameters(), master):
-                m -= lr * p.grad.float()
                 p.copy_(m)
         return float(loss.detach())
 
-    first = step(20.0)
+    first = step()
     for _ in range(args.steps):
-        last = step(20.0)
+        last = step()
     served = layers.Int8FeedForwardBlock(block)
     with torch.no_grad():
         out, stream = block(x, residual)

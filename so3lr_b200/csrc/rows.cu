@@ -549,15 +549,17 @@ int walking_blocks(long long rows, int threads) {
   return int(std::min<long long>(want, (long long)kSmCount * per_sm));
 }
 
-// Ring of a kernel that walks over rows: two blocks an SM, shared memory for up to
-// kRingStages rows. stages < 2: the row is too long.
+// Ring of a kernel that walks over rows: as many blocks an SM as its registers hold
+// (`resident` threads), shared memory for up to kRingStages rows each. stages < 2: the
+// row is too long.
 struct RingPlan {
   int grid, stages, smem;
 };
-RingPlan ring_plan(long long rows, long long row_bytes) {
-  const long long room = 110 * 1024 - kRingHeader;
+RingPlan ring_plan(long long rows, int threads, int resident, long long row_bytes) {
+  const int per_sm = std::max(1, std::min(16, resident / threads));
+  const long long room = 220 * 1024 / per_sm - 2048 - kRingHeader;  // 2 KB: static and reserved shared memory
   RingPlan p;
-  p.grid = int(std::min<long long>(rows, 2LL * kSmCount));
+  p.grid = int(std::min<long long>(rows, (long long)kSmCount * per_sm));
   p.stages = int(std::min<long long>(kRingStages, room / row_bytes));
   p.smem = int(kRingHeader + p.stages * row_bytes);
   return p;
@@ -570,7 +572,7 @@ RingPlan backward_ring(const so3lr_rms_norm_backward_args &a) {
                     aligned(a.ds, a.ds_stride, e, 16) && aligned(a.dx, a.dx_stride, e, 16) &&
                     aligned(a.weight, 0, 1, 16);
   if (!wide || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
-  const RingPlan p = ring_plan(a.rows, 3 * a.width * e);
+  const RingPlan p = ring_plan(a.rows, row_threads(a.width, 16), 512, 3 * a.width * e);
   return p.stages < 2 ? RingPlan{0, 0, 0} : p;
 }
 int backward_parts(const so3lr_rms_norm_backward_args &a) {
@@ -690,7 +692,7 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s) {
     // up to 32 elements per thread: 32768 columns in a block of 1,024 threads
     const int per = a.hidden > 16384 ? 32 : per_thread(a.hidden);
     // the ring where a block has several rows to walk over, and a row needs a block
-    const RingPlan r = ring_plan(a.rows, 2 * a.hidden * e);
+    const RingPlan r = ring_plan(a.rows, row_threads(a.hidden, ring_per_thread(a.hidden)), 1024, 2 * a.hidden * e);
     if (wide && a.hidden > 512 && a.hidden <= 16384 && r.stages >= 2 && a.rows > 2 * r.grid)
       gate_ring<T>(a, r, s);
     else if (per == 32)
