@@ -88,12 +88,6 @@ __device__ __forceinline__ Chunk<T, VEC> to_chunk(const float (&v)[VEC]) {
   return c;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // 1 / (1 + exp(-g)) with the hardware's exponential and reciprocal (both within 2
 // units in the last place). exp(-g) overflows to infinity for g < -88, and the
 // result is then 0, as it should be to float32's range; the flushed denormals of
@@ -120,9 +114,9 @@ __device__ __forceinline__ float max_abs(float a, float b) {
 __device__ __forceinline__ float row_scale(uint32_t top_bits, float &inv) {
   inv = 0.0f;
   if (top_bits > 0x7f7fffffu) return __uint_as_float(0x7fc00000u);
-  const float scale = __uint_as_float(top_bits) / 127.0f;
+  const float scale = __uint_as_float(top_bits) * (1.0f / 127.0f);
   if (scale < 1.17549435e-38f) return 0.0f;
-  inv = 1.0f / scale;
+  inv = __fdividef(1.0f, scale);
   return scale;
 }
 // VEC codes of a row: v inv rounded to nearest even. Adding 1.5 2^23 leaves the

@@ -3,11 +3,12 @@
 // rows. All are bound by HBM: every input element is read once into registers,
 // every output written once; the row statistics are reduced between the two.
 //
-// A row belongs to one warp (up to 16 elements per lane, so that short rows need
-// no block barrier) or to one block. A thread holds N chunks of VEC elements:
-// 16-byte chunks where every row starts on a 16-byte boundary, single elements
-// otherwise (odd widths, views). Eight elements a thread keep the registers low and
-// so the bytes in flight high; sixteen only where a row would not fit otherwise.
+// A row belongs to 8, 16 or 32 lanes of a warp (rows of up to 1024 elements: no block
+// barrier) or to one block. A thread holds N chunks of VEC elements: 16-byte chunks
+// where every row starts on a 16-byte boundary, single elements otherwise (odd
+// widths, views). With 2-byte elements the kernels issue more than they load unless
+// a thread has many elements: a row's reduction, its reciprocal root and addresses
+// cost each thread about a hundred instructions, an element about ten.
 #include "layers_common.cuh"
 #include "model_host.hpp"
 #include "tensor_core.cuh"
@@ -15,18 +16,23 @@
 namespace so3lr_b200 {
 namespace {
 
-constexpr int kWarpRows = 8;     // rows of a block when a warp owns a row
+constexpr int kTeamThreads = 256;  // of a block whose rows belong to parts of a warp
 
-// The threads of one row: a warp or the whole block. Reductions run in a fixed
-// order and return the same value to every thread of the row.
-template <bool WARP>
+// The threads of one row: LANES of a warp, or the whole block (LANES = 0). Reductions
+// run in a fixed order and return the same value to every thread of the row.
+template <int LANES>
 struct RowTeam {
   int t, size;
-  __device__ RowTeam() : t(WARP ? threadIdx.x & 31 : threadIdx.x), size(WARP ? 32 : blockDim.x) {}
+  __device__ RowTeam() : t(LANES ? threadIdx.x % LANES : threadIdx.x), size(LANES ? LANES : blockDim.x) {}
+  static __device__ __forceinline__ float add(float v) {
+#pragma unroll
+    for (int o = (LANES ? LANES : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
   // slot: 32 floats of shared memory that no other pending reduction uses
   __device__ __forceinline__ float sum(float v, float *slot) const {
-    v = warp_sum(v);
-    if (WARP) return v;
+    v = add(v);
+    if (LANES) return v;
     const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -35,9 +41,9 @@ struct RowTeam {
     return total;
   }
   __device__ __forceinline__ float2 sum2(float a, float b, float2 *slot) const {
-    a = warp_sum(a);
-    b = warp_sum(b);
-    if (WARP) return make_float2(a, b);
+    a = add(a);
+    b = add(b);
+    if (LANES) return make_float2(a, b);
     const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
@@ -49,8 +55,13 @@ struct RowTeam {
     return total;
   }
   __device__ __forceinline__ uint32_t max(uint32_t v, uint32_t *slot) const {
+    if (LANES && LANES < 32) {
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) v = ::max(v, __shfl_xor_sync(0xffffffffu, v, o));
+      return v;
+    }
     v = __reduce_max_sync(0xffffffffu, v);
-    if (WARP) return v;
+    if (LANES) return v;
     const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -59,17 +70,27 @@ struct RowTeam {
     return top;
   }
 };
+// The row of this thread's team; `live`: it exists. A team past the last row goes
+// through the last one again without storing, so that whole warps stay together.
+template <int LANES>
+__device__ __forceinline__ long long team_row(long long rows, bool &live) {
+  const long long row = LANES ? (long long)blockIdx.x * (kTeamThreads / (LANES ? LANES : 1)) + threadIdx.x / (LANES ? LANES : 1)
+                              : blockIdx.x;
+  live = row < rows;
+  return live ? row : rows - 1;
+}
 
 // y = s w rstd, s = x + residual as stored. QUANT: y goes to 8 bits with the row's scale.
-template <class T, class W, int VEC, int N, bool WARP, bool QUANT>
-__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const so3lr_rms_norm_args a) {
+template <class T, class W, int VEC, int N, int LANES, bool QUANT>
+__global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
+    k_rms_norm(const so3lr_rms_norm_args a, const float inv_width, const float eps) {
   __shared__ float slot[32];
   __shared__ uint32_t slot_max[32];
   dependents_may_start();
   wait_for_predecessors();
-  const RowTeam<WARP> team;
-  const long long row = WARP ? (long long)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= a.rows) return;  // whole warps (WARP) only: a block row always exists
+  const RowTeam<LANES> team;
+  bool live;
+  const long long row = team_row<LANES>(a.rows, live);
   const int width = int(a.width);
   const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
   const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
@@ -97,7 +118,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum[i] = to_float(cx[j].e[i]) + to_float(cr[j].e[i]);
         cx[j] = to_chunk<T, VEC>(sum);
-        store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx[j]);
+        if (live) store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx[j]);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -106,7 +127,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
       }
     }
   }
-  const float rstd = 1.0f / sqrtf(team.sum(sq, slot) / float(width) + float(a.eps));
+  const float rstd = rsqrtf(fmaf(team.sum(sq, slot), inv_width, eps));
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -119,12 +140,13 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
         v[j * VEC + i] = y[i];
         if (QUANT) top = max_abs(top, y[i]);
       }
-      if (!QUANT) store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, to_chunk<T, VEC>(y));
+      if (!QUANT && live) store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, to_chunk<T, VEC>(y));
     }
   }
   if (!QUANT) return;
   float inv;
   const float scale = row_scale(team.max(__float_as_uint(top) & 0x7fffffffu, slot_max), inv);
+  if (!live) return;
   if (team.t == 0) a.scales[row] = scale;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -136,16 +158,18 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024) k_rms_norm(const
 
 // dx = rstd (a - xh mean(a xh)) + ds with a = dy w, xh = s rstd; each block also
 // sums dy xh over its rows (a fixed set, in order) into one row of `partial`.
-template <class T, class W, int VEC, int N, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : 1) k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial) {
-  constexpr bool WARP = MAXT == 32 * kWarpRows;
+template <class T, class W, int VEC, int N, int LANES, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ? 4 : 1)
+    k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, const float inv_width,
+                        const float eps) {
   __shared__ float2 slot[2][32];
-  extern __shared__ float column[];  // WARP: kWarpRows x width
+  extern __shared__ float column[];  // LANES: teams x width
   dependents_may_start();
   wait_for_predecessors();
-  const RowTeam<WARP> team;
+  const RowTeam<LANES> team;
   const int width = int(a.width);
-  const int teams = WARP ? kWarpRows : 1, team_id = WARP ? threadIdx.x >> 5 : 0;
+  constexpr int kTeams = LANES ? kTeamThreads / (LANES ? LANES : 1) : 1;
+  const int team_id = LANES ? threadIdx.x / (LANES ? LANES : 1) : 0;
   Chunk<W, VEC> cw[N];
   float dw[N * VEC];
 #pragma unroll
@@ -156,7 +180,10 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : 1) k_rms_norm_backward
     for (int i = 0; i < VEC; ++i) dw[j * VEC + i] = 0.0f;
   }
   int parity = 0;
-  for (long long row = (long long)blockIdx.x * teams + team_id; row < a.rows; row += (long long)gridDim.x * teams) {
+  // whole blocks walk together; a team past the last row goes through it again and adds nothing
+  for (long long first = (long long)blockIdx.x * kTeams; first < a.rows; first += (long long)gridDim.x * kTeams) {
+    const bool live = first + team_id < a.rows;
+    const long long row = live ? first + team_id : a.rows - 1;
     const T *s = static_cast<const T *>(a.s) + row * a.s_stride;
     const T *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
     const T *ds = a.ds ? static_cast<const T *>(a.ds) + row * a.ds_stride : nullptr;
@@ -185,8 +212,9 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : 1) k_rms_norm_backward
     }
     const float2 total = team.sum2(sq, dot, slot[parity]);
     parity ^= 1;
-    const float rstd = 1.0f / sqrtf(total.x / float(width) + float(a.eps));
-    const float mean = total.y * rstd / float(width);  // mean(a xh)
+    if (!live) continue;
+    const float rstd = rsqrtf(fmaf(total.x, inv_width, eps));
+    const float back = -(total.y * rstd * inv_width) * rstd * rstd;  // - mean(a xh) rstd^2, times s
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * team.size + team.t) * VEC;
@@ -194,17 +222,16 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : 1) k_rms_norm_backward
         float out[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float xh = to_float(cs[j].e[i]) * rstd, d = to_float(cd[j].e[i]);
-          dw[j * VEC + i] = fmaf(d, xh, dw[j * VEC + i]);
-          float g = rstd * (d * to_float(cw[j].e[i]) - xh * mean);
-          if (ds) g += to_float(ce[j].e[i]);
-          out[i] = g;
+          const float f = to_float(cs[j].e[i]), d = to_float(cd[j].e[i]);
+          dw[j * VEC + i] = fmaf(d, f * rstd, dw[j * VEC + i]);
+          const float rest = ds ? fmaf(f, back, to_float(ce[j].e[i])) : f * back;
+          out[i] = fmaf(d * to_float(cw[j].e[i]), rstd, rest);
         }
         store_chunk<T, VEC>(static_cast<T *>(a.dx) + row * a.dx_stride + c, to_chunk<T, VEC>(out));
       }
     }
   }
-  if (!WARP) {
+  if (!LANES) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * team.size + team.t) * VEC;
@@ -225,7 +252,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : 1) k_rms_norm_backward
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
     float total = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kWarpRows; ++k) total += column[k * width + c];
+    for (int k = 0; k < kTeams; ++k) total += column[k * width + c];
     partial[(size_t)blockIdx.x * width + c] = total;
   }
 }
@@ -271,7 +298,8 @@ constexpr int kRingHeader = 128, kRingStages = 8;
 // fuller warps are faster (8 elements a thread: 115 us at 16384 x 4096 bfloat16).
 template <class T, class W>
 __global__ void __launch_bounds__(512)
-    k_rms_norm_backward_ring(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, int stages, int *err) {
+    k_rms_norm_backward_ring(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, int stages, int *err,
+                             const float inv_width, const float eps) {
   constexpr int VEC = 16 / sizeof(T), N = 16 / VEC;
   __shared__ float2 slot[2][32];
   extern __shared__ __align__(128) unsigned char smem[];
@@ -280,7 +308,7 @@ __global__ void __launch_bounds__(512)
   dependents_may_start();
   const RowRing ring(smem, tensors * row_bytes, stages, err);
   wait_for_predecessors();
-  const RowTeam<false> team;
+  const RowTeam<0> team;
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
   auto fetch = [&](int i) {
     const long long row = blockIdx.x + (long long)i * gridDim.x;
@@ -301,7 +329,6 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j * VEC + i] = 0.0f;
   }
-  const float per = 1.0f / float(width);
   for (int k = 0; k < rows; ++k) {
     ring.wait(k);
     const T *s = reinterpret_cast<const T *>(ring.stage(k));
@@ -324,8 +351,8 @@ __global__ void __launch_bounds__(512)
     }
     const float2 total = team.sum2(sq, dot, slot[k & 1]);  // a barrier: every thread has read the stage
     if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
-    const float rstd = 1.0f / sqrtf(total.x * per + float(a.eps));
-    const float back = -(total.y * rstd * per) * rstd * rstd;  // - mean(a xh) rstd^2, times s
+    const float rstd = rsqrtf(fmaf(total.x, inv_width, eps));
+    const float back = -(total.y * rstd * inv_width) * rstd * rstd;  // - mean(a xh) rstd^2, times s
     T *dx = static_cast<T *>(a.dx) + (blockIdx.x + (long long)k * gridDim.x) * a.dx_stride;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -375,15 +402,14 @@ __global__ void k_column_sum(int nparts, int width, const float *__restrict__ pa
 }
 
 // 8-bit rows of silu(g) u
-template <class T, int VEC, int N, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024, VEC *N == 8 && !WARP ? 2 : 1)
-    k_gate_int8(const so3lr_gate_int8_args a) {
+template <class T, int VEC, int N, int LANES>
+__global__ void __launch_bounds__(LANES ? kTeamThreads : 1024) k_gate_int8(const so3lr_gate_int8_args a) {
   __shared__ uint32_t slot[32];
   dependents_may_start();
   wait_for_predecessors();
-  const RowTeam<WARP> team;
-  const long long row = WARP ? (long long)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= a.rows) return;
+  const RowTeam<LANES> team;
+  bool live;
+  const long long row = team_row<LANES>(a.rows, live);
   const int hidden = int(a.hidden);
   const T *g = static_cast<const T *>(a.gu) + row * a.gu_stride, *u = g + hidden;
   Chunk<T, VEC> cg[N], cu[N];
@@ -409,6 +435,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024, VEC *N == 8 && !
   }
   float inv;
   const float scale = row_scale(team.max(__float_as_uint(top) & 0x7fffffffu, slot), inv);
+  if (!live) return;
   if (team.t == 0) a.scales[row] = scale;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -418,10 +445,11 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024, VEC *N == 8 && !
   }
 }
 
-// k_gate_int8 for many rows on 16-byte boundaries: PER elements a thread, rows through a ring
-template <class T, int PER, int MAXT>
-__global__ void __launch_bounds__(MAXT) k_gate_int8_ring(const so3lr_gate_int8_args a, int stages, int *err) {
-  constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
+// k_gate_int8 for many rows on 16-byte boundaries: 32 elements a thread, rows through a ring
+constexpr int kGateRing = 32;
+template <class T>
+__global__ void __launch_bounds__(512) k_gate_int8_ring(const so3lr_gate_int8_args a, int stages, int *err) {
+  constexpr int VEC = 16 / sizeof(T), N = kGateRing / VEC;
   __shared__ uint32_t slot[2][32];
   extern __shared__ __align__(128) unsigned char smem[];
   const int hidden = int(a.hidden), t = threadIdx.x, size = blockDim.x;
@@ -429,7 +457,7 @@ __global__ void __launch_bounds__(MAXT) k_gate_int8_ring(const so3lr_gate_int8_a
   dependents_may_start();
   const RowRing ring(smem, row_bytes, stages, err);
   wait_for_predecessors();
-  const RowTeam<false> team;
+  const RowTeam<0> team;
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
   auto fetch = [&](int i) {
     const long long row = blockIdx.x + (long long)i * gridDim.x;
@@ -441,7 +469,7 @@ __global__ void __launch_bounds__(MAXT) k_gate_int8_ring(const so3lr_gate_int8_a
   for (int k = 0; k < rows; ++k) {
     ring.wait(k);
     const T *g = reinterpret_cast<const T *>(ring.stage(k)), *u = g + hidden;
-    float v[PER], top = 0.0f;
+    float v[kGateRing], top = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
@@ -502,11 +530,55 @@ bool aligned(const void *p, long long stride, int size, int bytes) {
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (stride * size) % bytes == 0);
 }
 
-// Threads that hold a row of `width` elements, `per` of them each: a warp where one
-// suffices, else a block of whole warps.
+// Threads that hold a row of `width` elements, `per` of them each.
 int row_threads(long long width, int per) { return int((width + 32LL * per - 1) / (32LL * per)) * 32; }
-// Elements a thread holds: 8, or 16 where that keeps the row in one warp or in one block.
-int per_thread(long long width) { return width <= 256 || (width > 512 && width <= 8192) ? 8 : 16; }
+
+// How a row is held: lanes of a warp (0: a block) and elements a thread. Rows on
+// 16-byte boundaries: in a warp where 16 elements a lane suffice, as few lanes as hold
+// them with 8 each. Longer rows whose results are 8 bits, which issue more than they
+// move, stay in a warp up to 1024 elements and take 16 a thread of a block above; the
+// others take 8 up to 4096 (1024 bfloat16: 5.4 TB/s, 3.4 with 32 in a warp; 2048 to 8
+// bits 2.6 with 8 and 2.9 with 16; 8192: 3.2 with 8 and 4.4 with 16). Rows on other boundaries move single
+// elements, 8 a thread (16 where the row would not fit otherwise).
+struct Hold {
+  int lanes, per;
+};
+Hold hold(long long width, bool wide, bool to_8_bits) {
+  if (wide) {
+    if (width <= 64) return {8, 8};
+    if (width <= 128) return {16, 8};
+    if (width <= 512) return {32, width <= 256 ? 8 : 16};
+    if (to_8_bits) return width <= 1024 ? Hold{32, 32} : Hold{0, 16};
+    return {0, width <= 4096 ? 8 : 16};
+  }
+  if (width <= 512) return {32, width <= 256 ? 8 : 16};
+  return {0, width <= 8192 ? 8 : 16};
+}
+// f(std::integral_constant lanes, std::integral_constant per) for each that hold() gives
+template <bool WIDE, class F>
+void by_hold(const Hold &h, F &&f) {
+  auto lanes_per = [&](auto lanes, auto per) {
+    if (h.lanes == lanes && h.per == per) f(lanes, per);
+  };
+  using std::integral_constant;
+  if constexpr (WIDE) {
+    lanes_per(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    lanes_per(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    lanes_per(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+  }
+  lanes_per(integral_constant<int, 0>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  lanes_per(integral_constant<int, 0>{}, integral_constant<int, 16>{});
+}
+// block and grid of one row a team
+dim3 team_block(const Hold &h, long long width) {
+  return h.lanes ? kTeamThreads : unsigned(row_threads(width, h.per));
+}
+dim3 team_grid(const Hold &h, long long rows) {
+  const long long teams = h.lanes ? kTeamThreads / h.lanes : 1;
+  return unsigned((rows + teams - 1) / teams);
+}
 
 template <class F>
 void by_type(int dtype, F &&f) {
@@ -525,28 +597,10 @@ void by_weight(int dtype, int weight_dtype, F &&f) {
     f(T{});
 }
 
-template <class T, class W, int VEC, int N>
-void norm_forward(const so3lr_rms_norm_args &a, cudaStream_t s) {
-  const int threads = row_threads(a.width, VEC * N);
-  const bool warp = threads == 32;
-  const unsigned grid = unsigned(warp ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows);
-  const int block = warp ? 32 * kWarpRows : threads;
-  if (warp && a.codes)
-    launch(k_rms_norm<T, W, VEC, N, true, true>, grid, block, 0, s, a);
-  else if (warp)
-    launch(k_rms_norm<T, W, VEC, N, true, false>, grid, block, 0, s, a);
-  else if (a.codes)
-    launch(k_rms_norm<T, W, VEC, N, false, true>, grid, block, 0, s, a);
-  else
-    launch(k_rms_norm<T, W, VEC, N, false, false>, grid, block, 0, s, a);
-}
-
 // Blocks of a kernel that walks over rows
-int walking_blocks(long long rows, int threads) {
-  const bool warp = threads == 32;
-  const long long want = warp ? (rows + kWarpRows - 1) / kWarpRows : rows;
-  const int per_sm = warp ? 4 : std::max(1, std::min(8, 1024 / threads));
-  return int(std::min<long long>(want, (long long)kSmCount * per_sm));
+int walking_blocks(const Hold &h, long long rows, long long width) {
+  const int per_sm = h.lanes ? 4 : std::max(1, std::min(8, 1024 / row_threads(width, h.per)));
+  return int(std::min<long long>(team_grid(h, rows).x, (long long)kSmCount * per_sm));
 }
 
 // Ring of a kernel that walks over rows: as many blocks an SM as its registers hold
@@ -556,7 +610,9 @@ struct RingPlan {
   int grid, stages, smem;
 };
 RingPlan ring_plan(long long rows, int threads, int resident, long long row_bytes) {
-  const int per_sm = std::max(1, std::min(16, resident / threads));
+  // not more blocks than have room for three rows each
+  const int per_sm = int(std::max<long long>(
+      1, std::min<long long>(std::min(16, resident / threads), 220 * 1024 / (3 * row_bytes + 2048 + kRingHeader))));
   const long long room = 220 * 1024 / per_sm - 2048 - kRingHeader;  // 2 KB: static and reserved shared memory
   RingPlan p;
   p.grid = int(std::min<long long>(rows, (long long)kSmCount * per_sm));
@@ -564,71 +620,60 @@ RingPlan ring_plan(long long rows, int threads, int resident, long long row_byte
   p.smem = int(kRingHeader + p.stages * row_bytes);
   return p;
 }
-// The ring kernel's blocks, 0 where the direct loads serve: rows of a warp, unaligned
-// rows, and rows too long for the ring
-RingPlan backward_ring(const so3lr_rms_norm_backward_args &a) {
+bool wide_backward(const so3lr_rms_norm_backward_args &a) {
   const int e = a.dtype == SO3LR_FLOAT32 ? 4 : 2;
-  const bool wide = a.width * e % 16 == 0 && aligned(a.dy, a.dy_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
-                    aligned(a.ds, a.ds_stride, e, 16) && aligned(a.dx, a.dx_stride, e, 16) &&
-                    aligned(a.weight, 0, 1, 16);
-  if (!wide || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
-  const RingPlan p = ring_plan(a.rows, row_threads(a.width, 16), 512, 3 * a.width * e);
+  return a.width * e % 16 == 0 && aligned(a.dy, a.dy_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
+         aligned(a.ds, a.ds_stride, e, 16) && aligned(a.dx, a.dx_stride, e, 16) && aligned(a.weight, 0, 1, 16);
+}
+// The ring kernel's blocks, no stages where the direct loads serve: rows of a warp,
+// unaligned rows, and rows too long for the ring
+RingPlan backward_ring(const so3lr_rms_norm_backward_args &a) {
+  if (!wide_backward(a) || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
+  const RingPlan p =
+      ring_plan(a.rows, row_threads(a.width, 16), 512, 3 * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
   return p.stages < 2 ? RingPlan{0, 0, 0} : p;
 }
 int backward_parts(const so3lr_rms_norm_backward_args &a) {
   const RingPlan r = backward_ring(a);
-  return r.stages ? r.grid : walking_blocks(a.rows, row_threads(a.width, per_thread(a.width)));
+  return r.stages ? r.grid : walking_blocks(hold(a.width, wide_backward(a), false), a.rows, a.width);
 }
 
-template <class T, class W, int VEC, int N>
+template <class T, class W, bool WIDE>
 void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int grid, cudaStream_t s) {
-  const int threads = row_threads(a.width, VEC * N);
-  if (threads == 32) {
-    launch(k_rms_norm_backward<T, W, VEC, N, 32 * kWarpRows>, grid, 32 * kWarpRows,
-           kWarpRows * a.width * sizeof(float), s, a, partial);
-    return;
-  }
-  // rows of a block that do not go through the ring: unaligned ones, and those too long for it
-  if constexpr (VEC == 1 && N == 8) {
-    if (threads <= 512) {
-      launch(k_rms_norm_backward<T, W, VEC, N, 512>, grid, threads, 0, s, a, partial);
-      return;
+  constexpr int V = WIDE ? 16 / int(sizeof(T)) : 1;
+  const Hold h = hold(a.width, WIDE, false);
+  by_hold<WIDE>(h, [&](auto lanes, auto per) {
+    constexpr int L = decltype(lanes)::value, N = decltype(per)::value / V;
+    const float inv = 1.0f / float(a.width), eps = float(a.eps);
+    if constexpr (L != 0 && decltype(per)::value <= 16) {
+      launch(k_rms_norm_backward<T, W, V, N, L, kTeamThreads>, grid, kTeamThreads,
+             kTeamThreads / L * a.width * sizeof(float), s, a, partial, inv, eps);
+    } else if constexpr (L == 0) {
+      // unaligned rows, and those too long for the ring
+      const int threads = row_threads(a.width, decltype(per)::value);
+      if constexpr (!WIDE && decltype(per)::value == 8) {
+        if (threads <= 512) {
+          launch(k_rms_norm_backward<T, W, V, N, 0, 512>, grid, threads, 0, s, a, partial, inv, eps);
+          return;
+        }
+      }
+      launch(k_rms_norm_backward<T, W, V, N, 0, 1024>, grid, threads, 0, s, a, partial, inv, eps);
     }
-  }
-  launch(k_rms_norm_backward<T, W, VEC, N, 1024>, grid, threads, 0, s, a, partial);
+  });
 }
 template <class T, class W>
 void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, const RingPlan &r, cudaStream_t s) {
   check_gave_up();
-  const int threads = row_threads(a.width, 16);
-  auto run = [&](auto fn) {
-    allow_dynamic_smem(reinterpret_cast<const void *>(fn), 227 * 1024 - 1024);
-    launch(fn, r.grid, threads, r.smem, s, a, partial, r.stages, gave_up_flag());
-  };
-  run(&k_rms_norm_backward_ring<T, W>);
+  allow_dynamic_smem(reinterpret_cast<const void *>(&k_rms_norm_backward_ring<T, W>), 227 * 1024 - 1024);
+  launch(k_rms_norm_backward_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, partial, r.stages,
+         gave_up_flag(), 1.0f / float(a.width), float(a.eps));
 }
 
-template <class T, int VEC, int N>
-void gate(const so3lr_gate_int8_args &a, cudaStream_t s) {
-  const int threads = row_threads(a.hidden, VEC * N);
-  if (threads == 32)
-    launch(k_gate_int8<T, VEC, N, true>, unsigned((a.rows + kWarpRows - 1) / kWarpRows), 32 * kWarpRows, 0, s, a);
-  else
-    launch(k_gate_int8<T, VEC, N, false>, unsigned(a.rows), threads, 0, s, a);
-}
-int ring_per_thread(long long hidden) { return hidden <= 4096 ? 16 : 32; }
 template <class T>
 void gate_ring(const so3lr_gate_int8_args &a, const RingPlan &r, cudaStream_t s) {
   check_gave_up();
-  const int threads = row_threads(a.hidden, ring_per_thread(a.hidden));
-  auto run = [&](auto fn) {
-    allow_dynamic_smem(reinterpret_cast<const void *>(fn), 227 * 1024 - 1024);
-    launch(fn, r.grid, threads, r.smem, s, a, r.stages, gave_up_flag());
-  };
-  if (ring_per_thread(a.hidden) == 16)
-    run(&k_gate_int8_ring<T, 16, 256>);
-  else
-    run(&k_gate_int8_ring<T, 32, 512>);
+  allow_dynamic_smem(reinterpret_cast<const void *>(&k_gate_int8_ring<T>), 227 * 1024 - 1024);
+  launch(k_gate_int8_ring<T>, r.grid, row_threads(a.hidden, kGateRing), r.smem, s, a, r.stages, gave_up_flag());
 }
 
 }  // namespace
@@ -644,10 +689,17 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
                         aligned(a.residual, a.residual_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
                         aligned(a.y, a.y_stride, e, 16) && aligned(a.codes, a.codes_stride, 1, V) &&
                         aligned(a.weight, 0, 1, 16);
-      if (per_thread(a.width) == 8)
-        wide ? norm_forward<T, W, V, 8 / V>(a, s) : norm_forward<T, W, 1, 8>(a, s);
-      else
-        wide ? norm_forward<T, W, V, 16 / V>(a, s) : norm_forward<T, W, 1, 16>(a, s);
+      const Hold h = hold(a.width, wide, a.codes != nullptr);
+      auto run = [&](auto is_wide) {
+        constexpr bool WIDE = decltype(is_wide)::value;
+        constexpr int VEC = WIDE ? V : 1;
+        by_hold<WIDE>(h, [&](auto lanes, auto per) {
+          constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
+          const auto fn = a.codes ? &k_rms_norm<T, W, VEC, N, L, true> : &k_rms_norm<T, W, VEC, N, L, false>;
+          launch(fn, team_grid(h, a.rows), team_block(h, a.width), 0, s, a, 1.0f / float(a.width), float(a.eps));
+        });
+      };
+      wide ? run(std::true_type{}) : run(std::false_type{});
     });
   });
 }
@@ -661,22 +713,16 @@ void launch_rms_norm_backward(const so3lr_rms_norm_backward_args &a, void *works
     using T = decltype(t);
     by_weight<T>(a.dtype, a.weight_dtype, [&](auto w) {
       using W = decltype(w);
-      constexpr int V = 16 / sizeof(T);
-      const int e = sizeof(T);
-      const bool wide = a.width % V == 0 && aligned(a.dy, a.dy_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
-                        aligned(a.ds, a.ds_stride, e, 16) && aligned(a.dx, a.dx_stride, e, 16) &&
-                        aligned(a.weight, 0, 1, 16);
       float *partial = static_cast<float *>(workspace);
       const RingPlan r = backward_ring(a);
       const int parts = backward_parts(a);
       if (parts > 0) {
         if (r.stages)
           norm_backward_ring<T, W>(a, partial, r, s);
-        else if (per_thread(a.width) == 8)
-          wide ? norm_backward<T, W, V, 8 / V>(a, partial, parts, s) : norm_backward<T, W, 1, 8>(a, partial, parts, s);
+        else if (wide_backward(a))
+          norm_backward<T, W, true>(a, partial, parts, s);
         else
-          wide ? norm_backward<T, W, V, 16 / V>(a, partial, parts, s)
-               : norm_backward<T, W, 1, 16>(a, partial, parts, s);
+          norm_backward<T, W, false>(a, partial, parts, s);
       }
       launch(k_column_sum<W>, unsigned((a.width + 31) / 32), dim3(32, 32), 0, s, parts, int(a.width), partial, static_cast<W *>(a.dweight));
     });
@@ -689,18 +735,26 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const int e = sizeof(T);
     const bool wide = a.hidden % V == 0 && aligned(a.gu, a.gu_stride, e, 16) && aligned(a.codes, a.codes_stride, 1, V);
-    // up to 32 elements per thread: 32768 columns in a block of 1,024 threads
-    const int per = a.hidden > 16384 ? 32 : per_thread(a.hidden);
-    // the ring where a block has several rows to walk over, and a row needs a block
-    const RingPlan r = ring_plan(a.rows, row_threads(a.hidden, ring_per_thread(a.hidden)), 1024, 2 * a.hidden * e);
-    if (wide && a.hidden > 512 && a.hidden <= 16384 && r.stages >= 2 && a.rows > 2 * r.grid)
+    // the ring for long rows, where a block has several to walk over (8192 bfloat16: 5.0
+    // TB/s, 4.6 without; 4096: 5.2, 5.6 without)
+    const RingPlan r = ring_plan(a.rows, row_threads(a.hidden, kGateRing), 1024, 2 * a.hidden * e);
+    if (wide && a.hidden > 4096 && a.hidden <= 16384 && r.stages >= 2 && a.rows > 2 * r.grid) {
       gate_ring<T>(a, r, s);
-    else if (per == 32)
-      wide ? gate<T, V, 32 / V>(a, s) : gate<T, 1, 32>(a, s);
-    else if (per == 8)
-      wide ? gate<T, V, 8 / V>(a, s) : gate<T, 1, 8>(a, s);
-    else
-      wide ? gate<T, V, 16 / V>(a, s) : gate<T, 1, 16>(a, s);
+      return;
+    }
+    const Hold h = a.hidden > 16384 ? Hold{0, 32} : hold(a.hidden, wide, true);
+    auto run = [&](auto is_wide) {
+      constexpr bool WIDE = decltype(is_wide)::value;
+      constexpr int VEC = WIDE ? V : 1;
+      if (h.per == 32 && h.lanes == 0)  // 32768 columns in a block of 1,024 threads
+        launch(k_gate_int8<T, VEC, 32 / VEC, 0>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
+      else
+        by_hold<WIDE>(h, [&](auto lanes, auto per) {
+          constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
+          launch(k_gate_int8<T, VEC, N, L>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
+        });
+    };
+    wide ? run(std::true_type{}) : run(std::false_type{});
   });
 }
 
