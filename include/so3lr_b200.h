@@ -457,7 +457,8 @@ typedef struct {
 int so3lr_dequantize_int8(const so3lr_dequantize_int8_args *args, void *stream, char *err, size_t errlen);
 
 /* Gated feed-forward block, bfloat16 or float16:
- *   h = silu(x Wg^T) * (x Wu^T)    (hidden wide; rounded to the element type between the products)
+ *   h = silu(x Wg^T) * (x Wu^T)    (hidden wide; rounded to the element type between the products, for
+ *                                   few rows to two such parts, so that the rounding does not show)
  *   y = h Wd^T
  * Weights are stored with output channels as rows. */
 typedef struct {

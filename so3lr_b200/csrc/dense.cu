@@ -925,15 +925,21 @@ long long feed_forward_keep(const so3lr_feed_forward_args &a) {
   plain.gu = nullptr;
   return !few_rows(plain) && keeps(a.width) ? (a.rows + 31) / 32 * 32 * a.hidden * 8 : 0;
 }
-// rows of the hidden layer of a few rows, on 16-byte boundaries
-static long long few_stride(const so3lr_feed_forward_args &a) { return (a.hidden + 7) / 8 * 8; }
+// The hidden layer of a few rows: its two parts with the same strides, on 16-byte
+// boundaries (or contiguous, where the first is the caller's).
+static long long few_stride(const so3lr_feed_forward_args &a) { return a.h ? a.hidden : (a.hidden + 7) / 8 * 8; }
+static long long few_part(const so3lr_feed_forward_args &a) {
+  return (a.rows * few_stride(a) * 2 + 255) / 256 * 256;
+}
 long long feed_forward_bytes(const so3lr_feed_forward_args &a) {
-  if (few_rows(a)) return a.h ? 0 : a.rows * few_stride(a) * 2;
+  if (few_rows(a)) return few_part(a) * (a.h ? 1 : 2);
   return dry_run(a, 2, [&](Dense &d) { feed_forward<__half>(d, a); });
 }
 void launch_feed_forward(const so3lr_feed_forward_args &a, void *workspace, cudaStream_t s) {
-  if (few_rows(a))
-    return launch_feed_forward_few(a, a.h ? a.h : workspace, a.h ? a.hidden : few_stride(a), s);
+  if (few_rows(a)) {
+    char *scratch = static_cast<char *>(workspace);
+    return launch_feed_forward_few(a, a.h ? a.h : scratch + few_part(a), few_stride(a), scratch, s);
+  }
   Dense d(workspace, 2, s, false);
   by_half(a.dtype, [&](auto t) { feed_forward<decltype(t)>(d, a); });
 }

@@ -74,14 +74,18 @@ struct FewArgs {
   void *y;
   long long y_stride;
   const float *a_scales, *b_scales, *bias;  // 8-bit products
+  void *rest;                    // GATED: what y's rounding leaves of the hidden layer; LO: the same of x
 };
 
-// y = x w^T (8 bits: scaled), or silu(x w^T) * (x w2^T). TWO: more than 8 rows.
-template <class E, class O, bool GATED, bool TWO, bool ALIGNED>
+// y = x w^T (8 bits: scaled), or silu(x w^T) * (x w2^T). TWO: more than 8 rows. LO: x is
+// the sum of x and a.rest (rows like x's). The hidden layer is handed over in two
+// 16-bit parts, so that its rounding does not show in y: with this few rows the second
+// MMA costs nothing beside the weights' loads.
+template <class E, class O, bool GATED, bool LO, bool TWO, bool ALIGNED>
 __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(const FewArgs a) {
   constexpr bool kInt8 = std::is_same<E, signed char>::value;
   using Acc = typename std::conditional<kInt8, int, float>::type;
-  constexpr int kPer = 16 / sizeof(E), kUnroll = GATED ? 2 : 4, kOut = GATED ? 2 : 1;
+  constexpr int kPer = 16 / sizeof(E), kUnroll = GATED ? 2 : LO ? (TWO ? 2 : 3) : 4, kOut = GATED ? 2 : 1;
   __shared__ Acc part[max_warps(TWO)][kOut][TWO ? 16 : 8][8];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n = blockIdx.x * 8 + g, row0 = blockIdx.y * 16, rows = min(16, a.rows - row0);
@@ -90,6 +94,8 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   const E *w = static_cast<const E *>(a.w) + cn * a.w_stride, *w2 = static_cast<const E *>(a.w2) + cn * a.w2_stride;
   const E *x0 = static_cast<const E *>(a.x) + (row0 + min(g, rows - 1)) * a.x_stride;
   const E *x1 = static_cast<const E *>(a.x) + (row0 + min(g + 8, rows - 1)) * a.x_stride;
+  const E *l0 = LO ? static_cast<const E *>(a.rest) + (x0 - static_cast<const E *>(a.x)) : nullptr;
+  const E *l1 = LO ? static_cast<const E *>(a.rest) + (x1 - static_cast<const E *>(a.x)) : nullptr;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer);
   const int begin = int((long long)steps * warp / warps), end = int((long long)steps * (warp + 1) / warps);
   dependents_may_start();
@@ -107,8 +113,10 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   wait_for_predecessors();
   Acc acc[kOut][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  auto multiply = [&](const uint4 &v0, const uint4 &v1, const uint4 &vw, const uint4 &vw2) {
+  auto multiply = [&](const uint4 &v0, const uint4 &v1, const uint4 &r0, const uint4 &r1, const uint4 &vw,
+                      const uint4 &vw2) {
     mma_step<E>(acc[0], v0, TWO ? v1 : zero, vw);
+    if (LO) mma_step<E>(acc[0], r0, TWO ? r1 : zero, vw);
     if (GATED) mma_step<E>(acc[kOut - 1], v0, TWO ? v1 : zero, vw2);
   };
   int st = begin;
@@ -117,6 +125,7 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
     for (; st + kUnroll <= whole; st += kUnroll) {
       const int k = (st * 4 + t) * kPer;
       uint4 vw[kUnroll], vw2[GATED ? kUnroll : 1], v0[kUnroll], v1[TWO ? kUnroll : 1];
+      uint4 r0[LO ? kUnroll : 1], r1[LO && TWO ? kUnroll : 1];
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
         vw[i] = load16<E, true, true>(w, k + i * 4 * kPer, 1 << 30);
@@ -126,22 +135,28 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
       for (int i = 0; i < kUnroll; ++i) {
         v0[i] = load16<E, true, false>(x0, k + i * 4 * kPer, 1 << 30);
         if (TWO) v1[i] = load16<E, true, false>(x1, k + i * 4 * kPer, 1 << 30);
+        if (LO) r0[i] = load16<E, true, false>(l0, k + i * 4 * kPer, 1 << 30);
+        if (LO && TWO) r1[i] = load16<E, true, false>(l1, k + i * 4 * kPer, 1 << 30);
       }
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) multiply(v0[i], TWO ? v1[i] : zero, vw[i], GATED ? vw2[i] : zero);
+      for (int i = 0; i < kUnroll; ++i)
+        multiply(v0[i], TWO ? v1[i] : zero, LO ? r0[i] : zero, LO && TWO ? r1[i] : zero, vw[i],
+                 GATED ? vw2[i] : zero);
     }
   }
 #pragma unroll 2
   for (; st < end; ++st) {
     const int k = (st * 4 + t) * kPer;
-    uint4 vw = zero, vw2 = zero, v0 = zero, v1 = zero;
+    uint4 vw = zero, vw2 = zero, v0 = zero, v1 = zero, r0 = zero, r1 = zero;
     if (k < a.k) {
       vw = load16<E, ALIGNED, true>(w, k, a.k);
       if (GATED) vw2 = load16<E, ALIGNED, true>(w2, k, a.k);
       v0 = load16<E, ALIGNED, false>(x0, k, a.k);
       if (TWO) v1 = load16<E, ALIGNED, false>(x1, k, a.k);
+      if (LO) r0 = load16<E, ALIGNED, false>(l0, k, a.k);
+      if (LO && TWO) r1 = load16<E, ALIGNED, false>(l1, k, a.k);
     }
-    multiply(v0, v1, vw, vw2);
+    multiply(v0, v1, r0, r1, vw, vw2);
   }
 #pragma unroll
   for (int o = 0; o < kOut; ++o) {
@@ -167,7 +182,12 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
       y = silu_f32(float(sum[0])) * float(sum[kOut - 1]);
     else
       y = float(sum[0]);
-    static_cast<O *>(a.y)[(row0 + row) * a.y_stride + c] = from_float<O>(y);
+    const O rounded = from_float<O>(y);
+    static_cast<O *>(a.y)[(row0 + row) * a.y_stride + c] = rounded;
+    if (GATED) {  // nothing is left of an infinity or a NaN
+      const float rest = y - to_float(rounded);
+      static_cast<O *>(a.rest)[(long long)(row0 + row) * a.y_stride + c] = from_float<O>(fabsf(rest) < 1e30f ? rest : 0.0f);
+    }
   }
 }
 
@@ -175,7 +195,7 @@ bool rows_aligned(const void *p, long long stride, long long rows, int size) {
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || stride * size % 16 == 0));
 }
 
-template <class E, class O, bool GATED>
+template <class E, class O, bool GATED, bool LO>
 void run(const FewArgs &a, cudaStream_t s) {
   constexpr int kPer = 16 / sizeof(E);
   const bool aligned = rows_aligned(a.x, a.x_stride, a.rows, sizeof(E)) && rows_aligned(a.w, a.w_stride, a.n, sizeof(E)) &&
@@ -189,37 +209,38 @@ void run(const FewArgs &a, cudaStream_t s) {
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer), warps = std::max(1, std::min(most, steps / 4));
   const unsigned block = unsigned(32 * warps);
   if (a.rows > 8)
-    aligned ? launch(k_few_rows<E, O, GATED, true, true>, grid, block, 0, s, a)
-            : launch(k_few_rows<E, O, GATED, true, false>, grid, block, 0, s, a);
+    aligned ? launch(k_few_rows<E, O, GATED, LO, true, true>, grid, block, 0, s, a)
+            : launch(k_few_rows<E, O, GATED, LO, true, false>, grid, block, 0, s, a);
   else
-    aligned ? launch(k_few_rows<E, O, GATED, false, true>, grid, block, 0, s, a)
-            : launch(k_few_rows<E, O, GATED, false, false>, grid, block, 0, s, a);
+    aligned ? launch(k_few_rows<E, O, GATED, LO, false, true>, grid, block, 0, s, a)
+            : launch(k_few_rows<E, O, GATED, LO, false, false>, grid, block, 0, s, a);
 }
 
 }  // namespace
 
 void launch_int8_linear_few(const so3lr_int8_linear_args &l, cudaStream_t s) {
   const FewArgs a{int(l.rows), int(l.n), int(l.k), l.a, l.a_stride, l.b, nullptr, l.b_stride, 0, l.y, l.y_stride,
-                  l.a_scales, l.b_scales, l.bias};
+                  l.a_scales, l.b_scales, l.bias, nullptr};
   if (l.out_dtype == SO3LR_FLOAT32)
-    run<signed char, float, false>(a, s);
+    run<signed char, float, false, false>(a, s);
   else if (l.out_dtype == SO3LR_BFLOAT16)
-    run<signed char, __nv_bfloat16, false>(a, s);
+    run<signed char, __nv_bfloat16, false, false>(a, s);
   else
-    run<signed char, __half, false>(a, s);
+    run<signed char, __half, false, false>(a, s);
 }
 
-void launch_feed_forward_few(const so3lr_feed_forward_args &f, void *h, long long h_stride, cudaStream_t s) {
+void launch_feed_forward_few(const so3lr_feed_forward_args &f, void *h, long long h_stride, void *h_rest,
+                             cudaStream_t s) {
   const FewArgs up{int(f.rows), int(f.hidden), int(f.width), f.x, f.x_stride, f.w_gate, f.w_up, f.w_gate_stride,
-                   f.w_up_stride, h, h_stride, nullptr, nullptr, nullptr};
+                   f.w_up_stride, h, h_stride, nullptr, nullptr, nullptr, h_rest};
   const FewArgs down{int(f.rows), int(f.width), int(f.hidden), h, h_stride, f.w_down, nullptr, f.w_down_stride, 0,
-                     f.y, f.y_stride, nullptr, nullptr, nullptr};
+                     f.y, f.y_stride, nullptr, nullptr, nullptr, h_rest};
   if (f.dtype == SO3LR_BFLOAT16) {
-    run<__nv_bfloat16, __nv_bfloat16, true>(up, s);
-    run<__nv_bfloat16, __nv_bfloat16, false>(down, s);
+    run<__nv_bfloat16, __nv_bfloat16, true, false>(up, s);
+    run<__nv_bfloat16, __nv_bfloat16, false, true>(down, s);
   } else {
-    run<__half, __half, true>(up, s);
-    run<__half, __half, false>(down, s);
+    run<__half, __half, true, false>(up, s);
+    run<__half, __half, false, true>(down, s);
   }
 }
 

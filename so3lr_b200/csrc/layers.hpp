@@ -44,6 +44,7 @@ inline bool few_rows(const so3lr_feed_forward_args &a) {
   return !a.gu && few_rows(a.rows, 6 * a.width * a.hidden, 48 << 20);
 }
 void launch_int8_linear_few(const so3lr_int8_linear_args &a, cudaStream_t s);
-void launch_feed_forward_few(const so3lr_feed_forward_args &a, void *h, long long h_stride, cudaStream_t s);
+void launch_feed_forward_few(const so3lr_feed_forward_args &a, void *h, long long h_stride, void *h_rest,
+                             cudaStream_t s);
 
 }  // namespace so3lr_b200
