@@ -631,20 +631,21 @@ class Dense {
   }
 
   // Work items of the problems. Tiles are narrow where 256 columns would give half of
-  // the pairs or fewer a tile. The tiles after the last whole wave are split along K
-  // where that saves more than the join costs: 16 K blocks take a pair 5 us (28 of a
-  // narrow tile), a join with its launch 4 to 5.
+  // the pairs or fewer a tile, unless the contraction is long enough to keep all pairs
+  // busy in parts (they then read a third less). The tiles after the last whole wave
+  // are split along K where that saves more than the join costs: a K block takes a pair
+  // 0.3 us, a join with its launch 5 (narrow tiles) to 7 us.
   template <int MODE>
   void plan(Params &p, bool may_split) {
     long long tiles = count<MODE, 256>(p);
-    p.narrow = MODE != kGatedBack && 2 * tiles <= kPairs;
-    if (p.narrow) tiles = count<MODE, 128>(p);
     int kb = 1 << 30;
     for (int i = 0; i < p.problems; ++i) kb = std::min(kb, p.prob[i].kb);
+    p.narrow = MODE != kGatedBack && 2 * tiles <= kPairs && (!may_split || tiles * kb < 24 * kPairs);
+    if (p.narrow) tiles = count<MODE, 128>(p);
     if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
     const int rest = int(tiles % kPairs);
     int splits = may_split && rest > 0 ? std::max(1, std::min(kPairs / rest, kb / 8)) : 1;
-    if (kb - kb / splits < (p.narrow ? 28 : 16)) splits = 1;
+    if (kb - kb / splits < (p.narrow ? 16 : 24)) splits = 1;
     p.splits = splits;
     p.whole = int(tiles) - (p.splits > 1 ? rest : 0);
     p.items = p.whole + (p.splits > 1 ? rest * p.splits : 0);
