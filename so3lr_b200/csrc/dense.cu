@@ -487,50 +487,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
 }
 
 // C of the split tiles = the sum of their parts, in order; 8-bit products get their
-// scales here. A block does 16 or 32 rows of a tile, a thread 4 columns of 4 of them.
+// scales here. A block does 4 or 8 rows of a tile, a thread 4 columns of one: latency
+// counts, so there are many blocks and all parts of a thread are loaded together.
 template <int MODE, class T, int TN>
 __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) {
   dependents_may_start();
-  wait_for_predecessors();
   constexpr int kQuads = TN / 4;  // of columns
   const Item w = item_of<MODE, TN>(p, p.whole + blockIdx.y * p.splits);
   const Problem &q = p.prob[w.prob];
   const int col = w.n0 + 4 * (threadIdx.x % kQuads);
-  if (col >= q.n) return;
-  const bool wide = (reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % (4 * sizeof(T)) == 0 && col + 4 <= q.n;
+  const int r = blockIdx.x * (256 / kQuads) + threadIdx.x / kQuads, row = w.m0 + r;
+  if (col >= q.n || row >= q.m) return;
+  wait_for_predecessors();
+  float f[4] = {0, 0, 0, 0};
+  int s[4] = {0, 0, 0, 0};
+  const uint32_t *part = w.partial + (size_t)r * TN + col - w.n0;
+  for (int k0 = 0; k0 < p.splits; k0 += 8) {
+    uint4 v[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = (4 * blockIdx.x + i) * (256 / kQuads) + threadIdx.x / kQuads, row = w.m0 + r;
-    if (row >= q.m) break;
-    float f[4] = {0, 0, 0, 0};
-    int s[4] = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int k = 0; k < p.splits; ++k) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(w.partial + ((size_t)k * kTileM + r) * TN + col - w.n0);
-      const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+    for (int k = 0; k < 8; ++k)
+      if (k0 + k < p.splits) v[k] = *reinterpret_cast<const uint4 *>(part + (size_t)(k0 + k) * (kTileM * TN));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (MODE == kInt8)
-          s[j] += int(e[j]);
-        else
-          f[j] += __uint_as_float(e[j]);
+    for (int k = 0; k < 8; ++k)
+      if (k0 + k < p.splits) {
+        const uint32_t e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (MODE == kInt8)
+            s[j] += int(e[j]);
+          else
+            f[j] += __uint_as_float(e[j]);
+        }
       }
-    }
-    Chunk<T, 4> out;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (MODE == kInt8 && col + j < q.n)
-        f[j] = fmaf(float(s[j]) * p.a_scales[row], p.b_scales[col + j], p.bias ? p.bias[col + j] : 0.0f);
-      out.e[j] = from_float<T>(f[j]);
-    }
-    T *dst = static_cast<T *>(q.c) + row * q.ldc + col;
-    if (wide)
-      store_chunk<T, 4>(dst, out);
-    else
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < q.n) dst[j] = out.e[j];
   }
+  if (MODE == kInt8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < q.n)
+        f[j] = fmaf(float(s[j]) * p.a_scales[row], p.b_scales[col + j], p.bias ? p.bias[col + j] : 0.0f);
+  }
+  const Chunk<T, 4> out = to_chunk<T, 4>(f);
+  T *dst = static_cast<T *>(q.c) + row * q.ldc + col;
+  if ((reinterpret_cast<uintptr_t>(q.c) | (q.ldc * sizeof(T))) % (4 * sizeof(T)) == 0 && col + 4 <= q.n)
+    store_chunk<T, 4>(dst, out);
+  else
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < q.n) dst[j] = out.e[j];
 }
 
 // rows copied to rows that start on 16-byte boundaries (the rest of a padded row is not read)
@@ -681,7 +684,7 @@ class Dense {
     launch(k_dense<MODE, T, A_MN, B_MN, TN>, 2 * std::min(kPairs, p.items), kThreads, S::kSmem, stream_, p);
     if constexpr (MODE == kPlain || MODE == kInt8) {
       if (p.splits == 1) return;
-      const int rows = 4 * (256 / (TN / 4));  // of a block
+      const int rows = 256 / (TN / 4);  // of a block
       launch(k_join<MODE, T, TN>, dim3(kTileM / rows, (p.items - p.whole) / p.splits), 256, 0, stream_, p);
     }
   }
