@@ -80,8 +80,55 @@ __device__ __forceinline__ long long team_row(long long rows, bool &live) {
   return live ? row : rows - 1;
 }
 
+// A chunk of a row of `width` elements at element c. SHIFT: c may be negative or the
+// chunk reach past the row; only what is inside is read or written.
+template <bool SHIFT, class T, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> load_part(const T *p, int c, int width) {
+  if (!SHIFT || (c >= 0 && c + VEC <= width)) return load_chunk<T, VEC>(p + c);
+  Chunk<T, VEC> v{};
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    if (c + i >= 0 && c + i < width) v.e[i] = p[c + i];
+  return v;
+}
+template <bool SHIFT, class T, int VEC>
+__device__ __forceinline__ void store_part(T *p, int c, int width, const Chunk<T, VEC> &v) {
+  if (!SHIFT || (c >= 0 && c + VEC <= width)) {
+    store_chunk<T, VEC>(p + c, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    if (c + i >= 0 && c + i < width) p[c + i] = v.e[i];
+}
+// the same for what lies on other boundaries than the row's: element by element
+template <bool SHIFT, class T, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> load_apart(const T *p, int c, int width) {
+  if (!SHIFT) return load_chunk<T, VEC>(p + c);
+  Chunk<T, VEC> v{};
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    if (c + i >= 0 && c + i < width) v.e[i] = p[c + i];
+  return v;
+}
+template <bool SHIFT, class T, int VEC>
+__device__ __forceinline__ void store_apart(T *p, int c, int width, const Chunk<T, VEC> &v) {
+  if (!SHIFT) {
+    store_chunk<T, VEC>(p + c, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    if (c + i >= 0 && c + i < width) p[c + i] = v.e[i];
+}
+// elements of a row past the last 16-byte boundary before it
+template <bool SHIFT, class T>
+__device__ __forceinline__ int phase(const T *row) {
+  return SHIFT ? int(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)) : 0;
+}
+
 // y = s w rstd, s = x + residual as stored. QUANT: y goes to 8 bits with the row's scale.
-template <class T, class W, int VEC, int N, int LANES, bool QUANT>
+template <class T, class W, int VEC, int N, int LANES, bool QUANT, bool SHIFT>
 __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
     k_rms_norm(const so3lr_rms_norm_args a, const float inv_width, const float eps) {
   __shared__ float slot[32];
@@ -95,22 +142,23 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
   const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
   const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
   const W *w = static_cast<const W *>(a.weight);
+  const int shift = phase<SHIFT>(x);
 
   Chunk<T, VEC> cx[N], cr[N];
   Chunk<W, VEC> cw[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
+    const int c = (j * team.size + team.t) * VEC - shift;
     if (c < width) {
-      cx[j] = load_chunk<T, VEC>(x + c);
-      if (r) cr[j] = load_chunk<T, VEC>(r + c);
-      cw[j] = load_chunk<W, VEC>(w + c);
+      cx[j] = load_part<SHIFT, T, VEC>(x, c, width);
+      if (r) cr[j] = load_part<SHIFT, T, VEC>(r, c, width);
+      cw[j] = load_apart<SHIFT, W, VEC>(w, c, width);
     }
   }
   float v[N * VEC], sq = 0.0f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
+    const int c = (j * team.size + team.t) * VEC - shift;
     if (c < width) {
       if (r) {
         // the stream is kept in the element type, and the norm is of what is kept
@@ -118,7 +166,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum[i] = to_float(cx[j].e[i]) + to_float(cr[j].e[i]);
         cx[j] = to_chunk<T, VEC>(sum);
-        if (live) store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx[j]);
+        if (live) store_part<SHIFT, T, VEC>(static_cast<T *>(a.s) + row * a.s_stride, c, width, cx[j]);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -131,7 +179,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
+    const int c = (j * team.size + team.t) * VEC - shift;
     if (c < width) {
       float y[VEC];
 #pragma unroll
@@ -140,7 +188,8 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
         v[j * VEC + i] = y[i];
         if (QUANT) top = max_abs(top, y[i]);
       }
-      if (!QUANT && live) store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, to_chunk<T, VEC>(y));
+      if (!QUANT && live)
+        store_part<SHIFT, T, VEC>(static_cast<T *>(a.y) + row * a.y_stride, c, width, to_chunk<T, VEC>(y));
     }
   }
   if (!QUANT) return;
@@ -150,15 +199,15 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
   if (team.t == 0) a.scales[row] = scale;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
+    const int c = (j * team.size + team.t) * VEC - shift;
     if (c < width)
-      store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
+      store_apart<SHIFT, signed char, VEC>(a.codes + row * a.codes_stride, c, width, to_codes<VEC>(v + j * VEC, inv));
   }
 }
 
 // dx = rstd (a - xh mean(a xh)) + ds with a = dy w, xh = s rstd; each block also
 // sums dy xh over its rows (a fixed set, in order) into one row of `partial`.
-template <class T, class W, int VEC, int N, int LANES, int MAXT>
+template <class T, class W, int VEC, int N, int LANES, int MAXT, bool SHIFT>
 __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ? 4 : 1)
     k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, const float inv_width,
                         const float eps) {
@@ -170,37 +219,40 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
   const int width = int(a.width);
   constexpr int kTeams = LANES ? kTeamThreads / (LANES ? LANES : 1) : 1;
   const int team_id = LANES ? threadIdx.x / (LANES ? LANES : 1) : 0;
+  // SHIFT: the grid's rows a step are a multiple of 8, so that a team's rows share their phase
+  const int shift = phase<SHIFT>(static_cast<const T *>(a.s) + ((long long)blockIdx.x * kTeams + team_id) * a.s_stride);
   Chunk<W, VEC> cw[N];
   float dw[N * VEC];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
-    if (c < width) cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
+    const int c = (j * team.size + team.t) * VEC - shift;
+    if (c < width) cw[j] = load_apart<SHIFT, W, VEC>(static_cast<const W *>(a.weight), c, width);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j * VEC + i] = 0.0f;
   }
   int parity = 0;
-  // whole blocks walk together; a team past the last row goes through it again and adds nothing
+  // whole blocks walk together; a team past the last row adds nothing
   for (long long first = (long long)blockIdx.x * kTeams; first < a.rows; first += (long long)gridDim.x * kTeams) {
     const bool live = first + team_id < a.rows;
-    const long long row = live ? first + team_id : a.rows - 1;
+    const long long row = live || SHIFT ? first + team_id : a.rows - 1;
     const T *s = static_cast<const T *>(a.s) + row * a.s_stride;
     const T *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
     const T *ds = a.ds ? static_cast<const T *>(a.ds) + row * a.ds_stride : nullptr;
     Chunk<T, VEC> cs[N], cd[N], ce[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC;
-      if (c < width) {
-        cs[j] = load_chunk<T, VEC>(s + c);
-        cd[j] = load_chunk<T, VEC>(dy + c);
-        if (ds) ce[j] = load_chunk<T, VEC>(ds + c);
+      const int c = (j * team.size + team.t) * VEC - shift;
+      if (SHIFT) cs[j] = cd[j] = ce[j] = Chunk<T, VEC>{};
+      if ((live || !SHIFT) && c < width) {  // the last row again, or (another phase) none
+        cs[j] = load_part<SHIFT, T, VEC>(s, c, width);
+        cd[j] = load_part<SHIFT, T, VEC>(dy, c, width);
+        if (ds) ce[j] = load_part<SHIFT, T, VEC>(ds, c, width);
       }
     }
     float sq = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC;
+      const int c = (j * team.size + team.t) * VEC - shift;
       if (c < width) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -217,7 +269,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
     const float back = -(total.y * rstd * inv_width) * rstd * rstd;  // - mean(a xh) rstd^2, times s
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC;
+      const int c = (j * team.size + team.t) * VEC - shift;
       if (c < width) {
         float out[VEC];
 #pragma unroll
@@ -227,26 +279,28 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
           const float rest = ds ? fmaf(f, back, to_float(ce[j].e[i])) : f * back;
           out[i] = fmaf(d * to_float(cw[j].e[i]), rstd, rest);
         }
-        store_chunk<T, VEC>(static_cast<T *>(a.dx) + row * a.dx_stride + c, to_chunk<T, VEC>(out));
+        store_part<SHIFT, T, VEC>(static_cast<T *>(a.dx) + row * a.dx_stride, c, width, to_chunk<T, VEC>(out));
       }
     }
   }
   if (!LANES) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC;
+      const int c = (j * team.size + team.t) * VEC - shift;
       if (c < width)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) partial[(size_t)blockIdx.x * width + c + i] = dw[j * VEC + i];
+        for (int i = 0; i < VEC; ++i)
+          if (!SHIFT || (c + i >= 0 && c + i < width)) partial[(size_t)blockIdx.x * width + c + i] = dw[j * VEC + i];
     }
     return;
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
+    const int c = (j * team.size + team.t) * VEC - shift;
     if (c < width)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) column[team_id * width + c + i] = dw[j * VEC + i];
+      for (int i = 0; i < VEC; ++i)
+        if (!SHIFT || (c + i >= 0 && c + i < width)) column[team_id * width + c + i] = dw[j * VEC + i];
   }
   __syncthreads();
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
@@ -497,30 +551,32 @@ __global__ void __launch_bounds__(512) k_gate_int8_ring(const so3lr_gate_int8_ar
   }
 }
 
-template <class T, int VEC>
+// WIDE: 16 codes a thread, rows of both on 16-byte boundaries. Otherwise a 16-byte chunk
+// of the result, counted from the boundary before its row, from single codes.
+template <class T, bool WIDE>
 __global__ void k_dequantize_int8(const so3lr_dequantize_int8_args a) {
   dependents_may_start();
   wait_for_predecessors();
-  const long long per_row = a.width / VEC, total = a.rows * per_row;
+  constexpr int kPer = 16 / sizeof(T), VEC = WIDE ? 16 : kPer;
+  const int width = int(a.width);
+  const long long per_row = WIDE ? a.width / VEC : (a.width + 2 * VEC - 2) / VEC, total = a.rows * per_row;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
     const long long row = total < (1LL << 31) ? uint32_t(i) / uint32_t(per_row) : i / per_row;
-    const long long c = (i - row * per_row) * VEC;
-    const Chunk<signed char, VEC> q = load_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c);
+    const signed char *codes = a.codes + row * a.codes_stride;
+    T *out = static_cast<T *>(a.out) + row * a.out_stride;
+    const int c = int(i - row * per_row) * VEC - phase<!WIDE>(out);
+    if (c >= width) continue;
     const float scale = a.scales[row];
-    T *dst = static_cast<T *>(a.out) + row * a.out_stride + c;
-    if (VEC == 16) {
-      constexpr int kPer = 16 / sizeof(T);
+    const Chunk<signed char, VEC> q = load_apart<!WIDE, signed char, VEC>(codes, c, width);
 #pragma unroll
-      for (int j = 0; j < VEC; j += kPer) {
-        float out[kPer];
+    for (int j = 0; j < VEC; j += kPer) {
+      float f[kPer];
 #pragma unroll
-        for (int k = 0; k < kPer; ++k)
-          out[k] = byte_to_float(reinterpret_cast<const uint32_t *>(&q)[(j + k) / 4] ^ 0x80808080u, (j + k) % 4) * scale;
-        store_chunk<T, kPer>(dst + j, to_chunk<T, kPer>(out));
-      }
-    } else {
-      dst[0] = from_float<T>(float(q.e[0]) * scale);
+      for (int k = 0; k < kPer; ++k)
+        f[k] = WIDE ? byte_to_float(reinterpret_cast<const uint32_t *>(&q)[(j + k) / 4] ^ 0x80808080u, (j + k) % 4) * scale
+                    : float(q.e[j + k]) * scale;
+      store_part<!WIDE, T, kPer>(out, c + j, width, to_chunk<T, kPer>(f));
     }
   }
 }
@@ -533,6 +589,30 @@ bool aligned(const void *p, long long stride, int size, int bytes) {
 // Threads that hold a row of `width` elements, `per` of them each.
 int row_threads(long long width, int per) { return int((width + 32LL * per - 1) / (32LL * per)) * 32; }
 
+// How a thread's chunks lie: 16-byte ones on the row's start (kWide), or counted from
+// the boundary before it (kShifted), or single elements.
+enum Path { kScalar, kWide, kShifted };
+struct RowTensors {  // of one row: all that is moved in chunks of the element type
+  int size;
+  bool any = false, same = true;
+  uintptr_t base = 0, step = 0;
+  void add(const void *p, long long stride) {
+    if (!p) return;
+    const uintptr_t b = reinterpret_cast<uintptr_t>(p) % 16, t = uintptr_t(stride * size) % 16;
+    if (any && (b != base || t != step)) same = false;
+    any = true;
+    base = b;
+    step = t;
+  }
+  // `rest_aligned`: what is moved beside them in chunks lies on its boundaries. A shifted
+  // row of the longest width would not fit a block.
+  Path path(long long width, bool rest_aligned) const {
+    if (!same) return kScalar;
+    if (base == 0 && step == 0 && width * size % 16 == 0 && rest_aligned) return kWide;
+    return width + 16 / size - 1 <= 16384 ? kShifted : kScalar;
+  }
+};
+
 // How a row is held: lanes of a warp (0: a block) and elements a thread. Rows on
 // 16-byte boundaries: in a warp where 16 elements a lane suffice, as few lanes as hold
 // them with 8 each. Longer rows whose results are 8 bits, which issue more than they
@@ -543,8 +623,9 @@ int row_threads(long long width, int per) { return int((width + 32LL * per - 1) 
 struct Hold {
   int lanes, per;
 };
-Hold hold(long long width, bool wide, bool to_8_bits) {
-  if (wide) {
+Hold hold(long long width, Path path, int vec, bool to_8_bits) {
+  if (path == kShifted) width += vec - 1;
+  if (path != kScalar) {
     if (width <= 64) return {8, 8};
     if (width <= 128) return {16, 8};
     if (width <= 512) return {32, width <= 256 ? 8 : 16};
@@ -555,13 +636,13 @@ Hold hold(long long width, bool wide, bool to_8_bits) {
   return {0, width <= 8192 ? 8 : 16};
 }
 // f(std::integral_constant lanes, std::integral_constant per) for each that hold() gives
-template <bool WIDE, class F>
+template <Path PATH, class F>
 void by_hold(const Hold &h, F &&f) {
   auto lanes_per = [&](auto lanes, auto per) {
     if (h.lanes == lanes && h.per == per) f(lanes, per);
   };
   using std::integral_constant;
-  if constexpr (WIDE) {
+  if constexpr (PATH != kScalar) {
     lanes_per(integral_constant<int, 8>{}, integral_constant<int, 8>{});
     lanes_per(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     lanes_per(integral_constant<int, 32>{}, integral_constant<int, 32>{});
@@ -570,6 +651,15 @@ void by_hold(const Hold &h, F &&f) {
   lanes_per(integral_constant<int, 32>{}, integral_constant<int, 8>{});
   lanes_per(integral_constant<int, 32>{}, integral_constant<int, 16>{});
   lanes_per(integral_constant<int, 0>{}, integral_constant<int, 16>{});
+}
+template <class F>
+void by_path(Path path, F &&f) {
+  if (path == kWide)
+    f(std::integral_constant<Path, kWide>{});
+  else if (path == kShifted)
+    f(std::integral_constant<Path, kShifted>{});
+  else
+    f(std::integral_constant<Path, kScalar>{});
 }
 // block and grid of one row a team
 dim3 team_block(const Hold &h, long long width) {
@@ -609,10 +699,10 @@ int walking_blocks(const Hold &h, long long rows, long long width) {
 struct RingPlan {
   int grid, stages, smem;
 };
-RingPlan ring_plan(long long rows, int threads, int resident, long long row_bytes) {
-  // not more blocks than have room for three rows each
+RingPlan ring_plan(long long rows, int threads, int resident, int depth, long long row_bytes) {
+  // not more blocks than have room for `depth` rows each
   const int per_sm = int(std::max<long long>(
-      1, std::min<long long>(std::min(16, resident / threads), 220 * 1024 / (3 * row_bytes + 2048 + kRingHeader))));
+      1, std::min<long long>(std::min(16, resident / threads), 220 * 1024 / (depth * row_bytes + 2048 + kRingHeader))));
   const long long room = 220 * 1024 / per_sm - 2048 - kRingHeader;  // 2 KB: static and reserved shared memory
   RingPlan p;
   p.grid = int(std::min<long long>(rows, (long long)kSmCount * per_sm));
@@ -620,44 +710,58 @@ RingPlan ring_plan(long long rows, int threads, int resident, long long row_byte
   p.smem = int(kRingHeader + p.stages * row_bytes);
   return p;
 }
-bool wide_backward(const so3lr_rms_norm_backward_args &a) {
-  const int e = a.dtype == SO3LR_FLOAT32 ? 4 : 2;
-  return a.width * e % 16 == 0 && aligned(a.dy, a.dy_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
-         aligned(a.ds, a.ds_stride, e, 16) && aligned(a.dx, a.dx_stride, e, 16) && aligned(a.weight, 0, 1, 16);
+Path backward_path(const so3lr_rms_norm_backward_args &a) {
+  RowTensors t{a.dtype == SO3LR_FLOAT32 ? 4 : 2};
+  t.add(a.dy, a.dy_stride);
+  t.add(a.s, a.s_stride);
+  t.add(a.ds, a.ds_stride);
+  t.add(a.dx, a.dx_stride);
+  return t.path(a.width, aligned(a.weight, 0, 1, 16));
+}
+Hold backward_hold(const so3lr_rms_norm_backward_args &a, Path path) {
+  const int vec = a.dtype == SO3LR_FLOAT32 ? 4 : 8;
+  // a block of 512 threads holds 4096 elements, 8 each
+  return hold(a.width, path, vec, false);
 }
 // The ring kernel's blocks, no stages where the direct loads serve: rows of a warp,
 // unaligned rows, and rows too long for the ring
 RingPlan backward_ring(const so3lr_rms_norm_backward_args &a) {
-  if (!wide_backward(a) || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
+  if (backward_path(a) != kWide || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
+  // two rows deep: float32, 2048 wide, 4.6 TB/s of inputs in four blocks an SM, 3.4 in three, three deep
   const RingPlan p =
-      ring_plan(a.rows, row_threads(a.width, 16), 512, 3 * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
+      ring_plan(a.rows, row_threads(a.width, 16), 512, 2, 3 * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
   return p.stages < 2 ? RingPlan{0, 0, 0} : p;
 }
 int backward_parts(const so3lr_rms_norm_backward_args &a) {
   const RingPlan r = backward_ring(a);
-  return r.stages ? r.grid : walking_blocks(hold(a.width, wide_backward(a), false), a.rows, a.width);
+  if (r.stages) return r.grid;
+  const Path path = backward_path(a);
+  const Hold h = backward_hold(a, path);
+  const int blocks = walking_blocks(h, a.rows, a.width);
+  return path == kShifted && h.lanes == 0 ? (blocks + 7) / 8 * 8 : blocks;
 }
 
-template <class T, class W, bool WIDE>
+template <class T, class W, Path PATH>
 void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int grid, cudaStream_t s) {
-  constexpr int V = WIDE ? 16 / int(sizeof(T)) : 1;
-  const Hold h = hold(a.width, WIDE, false);
-  by_hold<WIDE>(h, [&](auto lanes, auto per) {
-    constexpr int L = decltype(lanes)::value, N = decltype(per)::value / V;
+  constexpr int V = PATH == kScalar ? 1 : 16 / int(sizeof(T));
+  constexpr bool SHIFT = PATH == kShifted;
+  const Hold h = backward_hold(a, PATH);
+  by_hold<PATH>(h, [&](auto lanes, auto per) {
+    constexpr int L = decltype(lanes)::value, P = decltype(per)::value, N = P / V;
     const float inv = 1.0f / float(a.width), eps = float(a.eps);
-    if constexpr (L != 0 && decltype(per)::value <= 16) {
-      launch(k_rms_norm_backward<T, W, V, N, L, kTeamThreads>, grid, kTeamThreads,
+    if constexpr (L != 0 && P <= 16) {
+      launch(k_rms_norm_backward<T, W, V, N, L, kTeamThreads, SHIFT>, grid, kTeamThreads,
              kTeamThreads / L * a.width * sizeof(float), s, a, partial, inv, eps);
     } else if constexpr (L == 0) {
-      // unaligned rows, and those too long for the ring
-      const int threads = row_threads(a.width, decltype(per)::value);
-      if constexpr (!WIDE && decltype(per)::value == 8) {
+      // rows that start elsewhere than on 16-byte boundaries, and those too long for the ring
+      const int threads = row_threads(a.width + (SHIFT ? V - 1 : 0), P);
+      if constexpr (PATH != kWide && P == 8) {
         if (threads <= 512) {
-          launch(k_rms_norm_backward<T, W, V, N, 0, 512>, grid, threads, 0, s, a, partial, inv, eps);
+          launch(k_rms_norm_backward<T, W, V, N, 0, 512, SHIFT>, grid, threads, 0, s, a, partial, inv, eps);
           return;
         }
       }
-      launch(k_rms_norm_backward<T, W, V, N, 0, 1024>, grid, threads, 0, s, a, partial, inv, eps);
+      launch(k_rms_norm_backward<T, W, V, N, 0, 1024, SHIFT>, grid, threads, 0, s, a, partial, inv, eps);
     }
   });
 }
@@ -684,22 +788,27 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
     by_weight<T>(a.dtype, a.weight_dtype, [&](auto w) {
       using W = decltype(w);
       constexpr int V = 16 / sizeof(T);
-      const int e = sizeof(T);
-      const bool wide = a.width % V == 0 && aligned(a.x, a.x_stride, e, 16) &&
-                        aligned(a.residual, a.residual_stride, e, 16) && aligned(a.s, a.s_stride, e, 16) &&
-                        aligned(a.y, a.y_stride, e, 16) && aligned(a.codes, a.codes_stride, 1, V) &&
-                        aligned(a.weight, 0, 1, 16);
-      const Hold h = hold(a.width, wide, a.codes != nullptr);
-      auto run = [&](auto is_wide) {
-        constexpr bool WIDE = decltype(is_wide)::value;
-        constexpr int VEC = WIDE ? V : 1;
-        by_hold<WIDE>(h, [&](auto lanes, auto per) {
+      RowTensors t{int(sizeof(T))};
+      t.add(a.x, a.x_stride);
+      t.add(a.residual, a.residual_stride);
+      t.add(a.s, a.s_stride);
+      t.add(a.y, a.y_stride);
+      Path chosen = t.path(a.width, aligned(a.codes, a.codes_stride, 1, V) && aligned(a.weight, 0, 1, 16));
+      // 2-byte rows to codes on other boundaries: the codes' single stores undo what the chunks save (1003
+      // bfloat16: 1.25 TB/s in chunks, 1.4 in elements; float32 3.0 and 2.3)
+      if (chosen == kShifted && a.codes && sizeof(T) == 2) chosen = kScalar;
+      by_path(chosen, [&](auto path) {
+        constexpr Path PATH = decltype(path)::value;
+        constexpr int VEC = PATH == kScalar ? 1 : V;
+        const Hold h = hold(a.width, PATH, V, a.codes != nullptr);
+        by_hold<PATH>(h, [&](auto lanes, auto per) {
           constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
-          const auto fn = a.codes ? &k_rms_norm<T, W, VEC, N, L, true> : &k_rms_norm<T, W, VEC, N, L, false>;
-          launch(fn, team_grid(h, a.rows), team_block(h, a.width), 0, s, a, 1.0f / float(a.width), float(a.eps));
+          constexpr bool SHIFT = PATH == kShifted;
+          const auto fn = a.codes ? &k_rms_norm<T, W, VEC, N, L, true, SHIFT> : &k_rms_norm<T, W, VEC, N, L, false, SHIFT>;
+          launch(fn, team_grid(h, a.rows), team_block(h, a.width + (SHIFT ? V - 1 : 0)), 0, s, a,
+                 1.0f / float(a.width), float(a.eps));
         });
-      };
-      wide ? run(std::true_type{}) : run(std::false_type{});
+      });
     });
   });
 }
@@ -719,10 +828,10 @@ void launch_rms_norm_backward(const so3lr_rms_norm_backward_args &a, void *works
       if (parts > 0) {
         if (r.stages)
           norm_backward_ring<T, W>(a, partial, r, s);
-        else if (wide_backward(a))
-          norm_backward<T, W, true>(a, partial, parts, s);
         else
-          norm_backward<T, W, false>(a, partial, parts, s);
+          by_path(backward_path(a), [&](auto path) {
+            norm_backward<T, W, decltype(path)::value>(a, partial, parts, s);
+          });
       }
       launch(k_column_sum<W>, unsigned((a.width + 31) / 32), dim3(32, 32), 0, s, parts, int(a.width), partial, static_cast<W *>(a.dweight));
     });
@@ -737,24 +846,27 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s) {
     const bool wide = a.hidden % V == 0 && aligned(a.gu, a.gu_stride, e, 16) && aligned(a.codes, a.codes_stride, 1, V);
     // the ring for long rows, where a block has several to walk over (8192 bfloat16: 5.0
     // TB/s, 4.6 without; 4096: 5.2, 5.6 without)
-    const RingPlan r = ring_plan(a.rows, row_threads(a.hidden, kGateRing), 1024, 2 * a.hidden * e);
+    const RingPlan r = ring_plan(a.rows, row_threads(a.hidden, kGateRing), 1024, 3, 2 * a.hidden * e);
     if (wide && a.hidden > 4096 && a.hidden <= 16384 && r.stages >= 2 && a.rows > 2 * r.grid) {
       gate_ring<T>(a, r, s);
       return;
     }
-    const Hold h = a.hidden > 16384 ? Hold{0, 32} : hold(a.hidden, wide, true);
-    auto run = [&](auto is_wide) {
-      constexpr bool WIDE = decltype(is_wide)::value;
-      constexpr int VEC = WIDE ? V : 1;
+    const Hold h = a.hidden > 16384 ? Hold{0, 32} : hold(a.hidden, wide ? kWide : kScalar, V, true);
+    auto run = [&](auto path) {
+      constexpr Path PATH = decltype(path)::value;
+      constexpr int VEC = PATH == kWide ? V : 1;
       if (h.per == 32 && h.lanes == 0)  // 32768 columns in a block of 1,024 threads
         launch(k_gate_int8<T, VEC, 32 / VEC, 0>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
       else
-        by_hold<WIDE>(h, [&](auto lanes, auto per) {
+        by_hold<PATH>(h, [&](auto lanes, auto per) {
           constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
           launch(k_gate_int8<T, VEC, N, L>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
         });
     };
-    wide ? run(std::true_type{}) : run(std::false_type{});
+    if (wide)
+      run(std::integral_constant<Path, kWide>{});
+    else
+      run(std::integral_constant<Path, kScalar>{});
   });
 }
 
@@ -764,12 +876,9 @@ void launch_dequantize_int8(const so3lr_dequantize_int8_args &a, cudaStream_t s)
     const int e = sizeof(T);
     const bool wide =
         a.width % 16 == 0 && aligned(a.codes, a.codes_stride, 1, 16) && aligned(a.out, a.out_stride, e, 16);
-    const long long total = a.rows * (wide ? a.width / 16 : a.width);
+    const long long total = a.rows * (wide ? a.width / 16 : (a.width + 2 * (16 / e) - 2) / (16 / e));
     const unsigned grid = unsigned(std::min<long long>((total + 255) / 256, kSmCount * 64));
-    if (wide)
-      launch(k_dequantize_int8<T, 16>, grid, 256, 0, s, a);
-    else
-      launch(k_dequantize_int8<T, 1>, grid, 256, 0, s, a);
+    launch(wide ? &k_dequantize_int8<T, true> : &k_dequantize_int8<T, false>, grid, 256, 0, s, a);
   });
 }
 

@@ -146,6 +146,36 @@ def test_rms_norm_layouts(layers):
     assert dx.shape == (0, 264) and bool((dw == 0).all())
 
 
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("rows, width, offset", [(40, 63, 0), (19, 130, 1), (33, 257, 0), (50, 515, 3), (600, 1027, 2),
+                                                 (5, 4099, 5), (3, 8187, 1), (2, 16383, 1)])
+def test_rms_norm_rows_off_the_boundaries(layers, rows, width, offset, dtype):
+    """Rows that all start equally far past a boundary, and tensors that differ in it."""
+    def view(seed, apart=0):
+        return _rand(seed, rows * width + offset + apart, dtype=dtype)[offset + apart:].view(rows, width)
+
+    for apart in (0, 1):
+        x, r, dy, ds = view(1), view(2, apart), view(3), view(4, apart)
+        w = (1 + 0.1 * _rand(5, width + 1)[1:]).contiguous()
+        y, s = layers.rms_norm(x, w, r)
+        assert torch.equal(s, (x.float() + r.float()).to(dtype))
+        ref, rstd = _norm_ref(s.double(), w.double())
+        _within(y, ref, (U[dtype] + F32) * ref.abs() + TINY[dtype], "y")
+        codes, scales, s8 = layers.rms_norm_int8(x, w, r)
+        assert torch.equal(s8, s)
+        _check_codes(codes, scales, ref)
+        assert torch.equal(layers.dequantize_int8(codes, scales, dtype), (codes.float() * scales[:, None]).to(dtype))
+        sv = view(6)
+        dx, dw = layers.rms_norm_backward(dy, sv, w, ds)
+        _, rstd = _norm_ref(sv.double(), w.double())
+        xh, a = sv.double() * rstd, dy.double() * w.double()
+        want = rstd * (a - xh * (a * xh).mean(1, keepdim=True)) + ds.double()
+        size = rstd * (a.abs() + xh.abs() * (a * xh).abs().mean(1, keepdim=True)) + ds.double().abs()
+        _within(dx, want, U[dtype] * want.abs() + F32 * size + TINY[dtype], "dx")
+        want, size = (dy.double() * xh).sum(0), (dy.double() * xh).abs().sum(0)
+        _within(dw, want, U[torch.float32] * want.abs() + (rows * 2.0 ** -24 + F32) * size, "dweight")
+
+
 def test_rms_norm_repeats_and_streams(layers):
     """The same bits on every call, and on another stream than the tensors were made on."""
     x, r, w = (_rand(i, 3000, 256, dtype=torch.bfloat16) for i in (1, 2, 3))
