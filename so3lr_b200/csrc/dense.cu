@@ -536,17 +536,40 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) 
       if (col + j < q.n) dst[j] = out.e[j];
 }
 
-// rows copied to rows that start on 16-byte boundaries (the rest of a padded row is not read)
+// Operands copied to rows that start on 16-byte boundaries, all of a launch's in one
+// kernel: a thread gathers 16 bytes of a padded row.
+constexpr int kMaxRepack = 6;
+struct Repack {
+  struct Matrix {
+    const void *src;
+    void *dst;
+    long long stride, first;  // first: its first 16-byte piece among all
+    int cols, pieces;         // pieces of a row
+  } m[kMaxRepack];
+  int count;
+  long long total;
+};
 template <class T>
-__global__ void k_repack(long long rows, int cols, const T *__restrict__ src, long long stride, T *__restrict__ dst,
-                         int ld) {
+__global__ void k_repack(const __grid_constant__ Repack a) {
   dependents_may_start();
   wait_for_predecessors();
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * cols;
+  constexpr int kPer = 16 / sizeof(T);
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < a.total;
        i += (long long)gridDim.x * blockDim.x) {
-    const long long r = i / cols;
-    const int c = int(i - r * cols);
-    dst[r * ld + c] = src[r * stride + c];
+    int k = 0;
+#pragma unroll
+    for (int j = 1; j < kMaxRepack; ++j)
+      if (j < a.count && i >= a.m[j].first) k = j;
+    const Repack::Matrix &m = a.m[k];
+    const long long at = i - m.first;
+    const long long r = a.total < (1LL << 31) ? uint32_t(at) / uint32_t(m.pieces) : at / m.pieces;
+    const int c = int(at - r * m.pieces) * kPer;
+    const T *src = static_cast<const T *>(m.src) + r * m.stride;
+    Chunk<T, kPer> v{};
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (c + j < m.cols) v.e[j] = src[c + j];
+    store_chunk<T, kPer>(static_cast<T *>(m.dst) + (r * m.pieces * kPer + c), v);
   }
 }
 
@@ -599,23 +622,30 @@ class Dense {
   Scratch &scratch() { return scratch_; }
   bool dry() const { return dry_; }
 
-  // the operand as TMA reads it: in place, or copied to padded rows
+  // the operand as TMA reads it: in place, or copied to padded rows before the next run()
   Operand ready(Operand o) {
     const bool in_place = reinterpret_cast<uintptr_t>(o.data) % 16 == 0 &&
                           (o.rows == 1 || (o.stride * elem_ % 16 == 0 && o.stride >= o.cols));
     if (in_place) return o;
-    const int ld = int(padded(o.cols));
+    const long long ld = padded(o.cols);
     void *p = scratch_.take(o.rows * ld * elem_);
     if (!dry_) {
-      const unsigned grid = unsigned(std::min<long long>((o.rows * o.cols + 255) / 256, kSmCount * 32));
-      if (elem_ == 1)
-        launch(k_repack<uint8_t>, grid, 256, 0, stream_, o.rows, int(o.cols), static_cast<const uint8_t *>(o.data),
-               o.stride, static_cast<uint8_t *>(p), ld);
-      else
-        launch(k_repack<uint16_t>, grid, 256, 0, stream_, o.rows, int(o.cols), static_cast<const uint16_t *>(o.data),
-               o.stride, static_cast<uint16_t *>(p), ld);
+      if (repack_.count == kMaxRepack) flush();
+      const int pieces = int(ld * elem_ / 16);
+      repack_.m[repack_.count++] = Repack::Matrix{o.data, p, o.stride, repack_.total, int(o.cols), pieces};
+      repack_.total += o.rows * pieces;
     }
     return Operand{p, ld, o.rows, o.cols};
+  }
+  void flush() {
+    if (repack_.count == 0) return;
+    const unsigned grid = unsigned(std::min<long long>((repack_.total + 255) / 256, kSmCount * 32));
+    if (elem_ == 1)
+      launch(k_repack<uint8_t>, grid, 256, 0, stream_, repack_);
+    else
+      launch(k_repack<uint16_t>, grid, 256, 0, stream_, repack_);
+    repack_.count = 0;
+    repack_.total = 0;
   }
   long long padded(long long cols) const { return (cols * elem_ + 15) / 16 * 16 / elem_; }
 
@@ -671,6 +701,7 @@ class Dense {
 
   template <int MODE, class T, bool A_MN, bool B_MN>
   void run(Params &p) {
+    flush();
     if constexpr (MODE != kGatedBack) {
       if (p.narrow) return run_tiles<MODE, T, A_MN, B_MN, 128>(p);
     }
@@ -694,6 +725,7 @@ class Dense {
   int elem_;
   cudaStream_t stream_;
   bool dry_;
+  Repack repack_{};
 };
 
 int blocks_of(long long k, int per) { return int((k + per - 1) / per); }
