@@ -41,26 +41,39 @@ __device__ __forceinline__ void mma_step(Acc (&c)[4], const uint4 &x0, const uin
   mma_words(c, x0.z, x1.z, x0.w, x1.w, w.z, w.w, E{});
 }
 
-// 16 bytes of a row from element k on; elements past the row's end read as zero
-template <class E, bool ALIGNED, bool WEIGHT>
-__device__ __forceinline__ uint4 load16(const E *p, int k, int length) {
-  constexpr int kPer = 16 / sizeof(E);
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (ALIGNED && k + kPer <= length) {
-    if (WEIGHT)  // read once: not kept in L1
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                   : "l"(p + k));
-    else
-      v = *reinterpret_cast<const uint4 *>(p + k);
+// 16 bytes of a row from element k on. ALIGN: what rows start on (16 or 4 bytes, or 1).
+// With 1 the 4-byte words around them are read and shifted, so the caller sees to it
+// that the row has 4 bytes before and after.
+template <class E, int ALIGN, bool WEIGHT>
+__device__ __forceinline__ uint4 load_inside(const E *p, int k) {
+  uint4 v;
+  if (ALIGN == 16 && WEIGHT) {  // read once: not kept in L1
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p + k));
+  } else if (ALIGN == 16) {
+    v = *reinterpret_cast<const uint4 *>(p + k);
+  } else if (ALIGN == 4) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(p + k);
+    v = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
-    alignas(16) E e[kPer] = {};
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (k + i < length) e[i] = p[k + i];
-    v = *reinterpret_cast<const uint4 *>(e);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p + k), off = at % 4;
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(at - off);
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = w[4], bits = 8 * uint32_t(off);
+    v = make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                   __funnelshift_r(w3, w4, bits));
   }
   return v;
+}
+// the same anywhere in the row, element by element; those past its end read as zero
+template <class E>
+__device__ __forceinline__ uint4 load_anywhere(const E *p, int k, int length) {
+  constexpr int kPer = 16 / sizeof(E);
+  alignas(16) E e[kPer] = {};
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (k + i < length) e[i] = p[k + i];
+  return *reinterpret_cast<const uint4 *>(e);
 }
 
 constexpr int max_warps(bool two) { return two ? 8 : 16; }
@@ -81,11 +94,12 @@ struct FewArgs {
 // the sum of x and a.rest (rows like x's). The hidden layer is handed over in two
 // 16-bit parts, so that its rounding does not show in y: with this few rows the second
 // MMA costs nothing beside the weights' loads.
-template <class E, class O, bool GATED, bool LO, bool TWO, bool ALIGNED>
+template <class E, class O, bool GATED, bool LO, bool TWO, int ALIGN>
 __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(const FewArgs a) {
   constexpr bool kInt8 = std::is_same<E, signed char>::value;
   using Acc = typename std::conditional<kInt8, int, float>::type;
-  constexpr int kPer = 16 / sizeof(E), kUnroll = GATED ? 2 : LO ? (TWO ? 2 : 3) : 4, kOut = GATED ? 2 : 1;
+  constexpr int kPer = 16 / sizeof(E), kUnroll = ALIGN == 1 || GATED ? 2 : LO ? (TWO ? 2 : 3) : 4,
+                kOut = GATED ? 2 : 1;
   __shared__ Acc part[max_warps(TWO)][kOut][TWO ? 16 : 8][8];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n = blockIdx.x * 8 + g, row0 = blockIdx.y * 16, rows = min(16, a.rows - row0);
@@ -100,14 +114,12 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   const int begin = int((long long)steps * warp / warps), end = int((long long)steps * (warp + 1) / warps);
   dependents_may_start();
   // the first weights on their way to L2, which needs no order with the kernel before
-  if (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int k = ((begin + i) * 4 + t) * kPer;
-      if (begin + i < end && k < a.k) {
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(w + k));
-        if (GATED) asm volatile("prefetch.global.L2 [%0];" ::"l"(w2 + k));
-      }
+  for (int i = 0; i < kUnroll; ++i) {
+    const int k = ((begin + i) * 4 + t) * kPer;
+    if (begin + i < end && k < a.k) {
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(w + k));
+      if (GATED) asm volatile("prefetch.global.L2 [%0];" ::"l"(w2 + k));
     }
   }
   wait_for_predecessors();
@@ -119,45 +131,47 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
     if (LO) mma_step<E>(acc[0], r0, TWO ? r1 : zero, vw);
     if (GATED) mma_step<E>(acc[kOut - 1], v0, TWO ? v1 : zero, vw2);
   };
-  int st = begin;
-  if (ALIGNED) {  // whole groups of steps, all four lanes of a row inside it: loads at constant offsets
-    const int whole = min(end, a.k / (4 * kPer));
-    for (; st + kUnroll <= whole; st += kUnroll) {
-      const int k = (st * 4 + t) * kPer;
-      uint4 vw[kUnroll], vw2[GATED ? kUnroll : 1], v0[kUnroll], v1[TWO ? kUnroll : 1];
-      uint4 r0[LO ? kUnroll : 1], r1[LO && TWO ? kUnroll : 1];
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        vw[i] = load16<E, true, true>(w, k + i * 4 * kPer, 1 << 30);
-        if (GATED) vw2[i] = load16<E, true, true>(w2, k + i * 4 * kPer, 1 << 30);
-      }
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        v0[i] = load16<E, true, false>(x0, k + i * 4 * kPer, 1 << 30);
-        if (TWO) v1[i] = load16<E, true, false>(x1, k + i * 4 * kPer, 1 << 30);
-        if (LO) r0[i] = load16<E, true, false>(l0, k + i * 4 * kPer, 1 << 30);
-        if (LO && TWO) r1[i] = load16<E, true, false>(l1, k + i * 4 * kPer, 1 << 30);
-      }
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i)
-        multiply(v0[i], TWO ? v1[i] : zero, LO ? r0[i] : zero, LO && TWO ? r1[i] : zero, vw[i],
-                 GATED ? vw2[i] : zero);
-    }
-  }
-#pragma unroll 2
-  for (; st < end; ++st) {
+  auto step_anywhere = [&](int st) {
     const int k = (st * 4 + t) * kPer;
     uint4 vw = zero, vw2 = zero, v0 = zero, v1 = zero, r0 = zero, r1 = zero;
     if (k < a.k) {
-      vw = load16<E, ALIGNED, true>(w, k, a.k);
-      if (GATED) vw2 = load16<E, ALIGNED, true>(w2, k, a.k);
-      v0 = load16<E, ALIGNED, false>(x0, k, a.k);
-      if (TWO) v1 = load16<E, ALIGNED, false>(x1, k, a.k);
-      if (LO) r0 = load16<E, ALIGNED, false>(l0, k, a.k);
-      if (LO && TWO) r1 = load16<E, ALIGNED, false>(l1, k, a.k);
+      vw = load_anywhere(w, k, a.k);
+      if (GATED) vw2 = load_anywhere(w2, k, a.k);
+      v0 = load_anywhere(x0, k, a.k);
+      if (TWO) v1 = load_anywhere(x1, k, a.k);
+      if (LO) r0 = load_anywhere(l0, k, a.k);
+      if (LO && TWO) r1 = load_anywhere(l1, k, a.k);
     }
     multiply(v0, v1, r0, r1, vw, vw2);
-  }
+  };
+  auto steps_inside = [&](int st, auto count) {  // `count` steps, all four lanes of a row inside it
+    constexpr int C = decltype(count)::value;
+    const int k = (st * 4 + t) * kPer;
+    uint4 vw[C], vw2[GATED ? C : 1], v0[C], v1[TWO ? C : 1], r0[LO ? C : 1], r1[LO && TWO ? C : 1];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      vw[i] = load_inside<E, ALIGN, true>(w, k + i * 4 * kPer);
+      if (GATED) vw2[i] = load_inside<E, ALIGN, true>(w2, k + i * 4 * kPer);
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      v0[i] = load_inside<E, ALIGN, false>(x0, k + i * 4 * kPer);
+      if (TWO) v1[i] = load_inside<E, ALIGN, false>(x1, k + i * 4 * kPer);
+      if (LO) r0[i] = load_inside<E, ALIGN, false>(l0, k + i * 4 * kPer);
+      if (LO && TWO) r1[i] = load_inside<E, ALIGN, false>(l1, k + i * 4 * kPer);
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      multiply(v0[i], TWO ? v1[i] : zero, LO ? r0[i] : zero, LO && TWO ? r1[i] : zero, vw[i], GATED ? vw2[i] : zero);
+  };
+  // loads of 16 bytes where they are inside the row (and, off the boundaries, 4 bytes before and after them)
+  constexpr int kAround = ALIGN == 1 ? 4 / int(sizeof(E)) : 0;
+  int st = begin;
+  if (ALIGN == 1 && st == 0 && st < end) step_anywhere(st++);
+  const int whole = min(end, (a.k - kAround) / (4 * kPer));
+  for (; st + kUnroll <= whole; st += kUnroll) steps_inside(st, std::integral_constant<int, kUnroll>{});
+  for (; st < whole; ++st) steps_inside(st, std::integral_constant<int, 1>{});
+  for (; st < end; ++st) step_anywhere(st);
 #pragma unroll
   for (int o = 0; o < kOut; ++o) {
     part[warp][o][g][2 * t] = acc[o][0];
@@ -191,15 +205,18 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   }
 }
 
-bool rows_aligned(const void *p, long long stride, long long rows, int size) {
-  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || stride * size % 16 == 0));
+bool rows_on(int bytes, const void *p, long long stride, long long rows, int size) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (rows == 1 || stride * size % bytes == 0));
 }
 
 template <class E, class O, bool GATED, bool LO>
 void run(const FewArgs &a, cudaStream_t s) {
   constexpr int kPer = 16 / sizeof(E);
-  const bool aligned = rows_aligned(a.x, a.x_stride, a.rows, sizeof(E)) && rows_aligned(a.w, a.w_stride, a.n, sizeof(E)) &&
-                       rows_aligned(a.w2, a.w2_stride, a.n, sizeof(E));
+  auto all_on = [&](int bytes) {
+    constexpr int e = sizeof(E);
+    return rows_on(bytes, a.x, a.x_stride, a.rows, e) && rows_on(bytes, a.w, a.w_stride, a.n, e) &&
+           rows_on(bytes, a.w2, a.w2_stride, a.n, e) && (!LO || rows_on(bytes, a.rest, a.x_stride, a.rows, e));
+  };
   // Warps that split the contraction, four steps of 64 bytes or more to each: 8, or 16
   // where the blocks alone would leave too few loads in flight. One row, 2048 channels
   // of 8192 bfloat16 (256 blocks): 12.3 us with 8, 9.3 us with 16; 4096 channels of
@@ -208,12 +225,17 @@ void run(const FewArgs &a, cudaStream_t s) {
   const int most = grid.x * grid.y < 2 * kSmCount ? max_warps(a.rows > 8) : 8;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer), warps = std::max(1, std::min(most, steps / 4));
   const unsigned block = unsigned(32 * warps);
-  if (a.rows > 8)
-    aligned ? launch(k_few_rows<E, O, GATED, LO, true, true>, grid, block, 0, s, a)
-            : launch(k_few_rows<E, O, GATED, LO, true, false>, grid, block, 0, s, a);
+  auto go = [&](auto align) {
+    constexpr int A = decltype(align)::value;
+    launch(a.rows > 8 ? &k_few_rows<E, O, GATED, LO, true, A> : &k_few_rows<E, O, GATED, LO, false, A>, grid, block, 0,
+           s, a);
+  };
+  if (all_on(16))
+    go(std::integral_constant<int, 16>{});
+  else if (all_on(4))
+    go(std::integral_constant<int, 4>{});
   else
-    aligned ? launch(k_few_rows<E, O, GATED, LO, false, true>, grid, block, 0, s, a)
-            : launch(k_few_rows<E, O, GATED, LO, false, false>, grid, block, 0, s, a);
+    go(std::integral_constant<int, 1>{});
 }
 
 }  // namespace

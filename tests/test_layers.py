@@ -219,7 +219,7 @@ def _codes(seed, rows, k):
     return torch.randint(-127, 128, (rows, k), generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
 
 
-INT8_SIZES = [(1, 1, 1), (1, 64, 64), (1, 1531, 4096), (2, 33, 17), (3, 100, 1000), (5, 513, 129), (8, 256, 2048),
+INT8_SIZES = [(1, 1, 1), (1, 50, 900), (12, 70, 1004), (40, 33, 516), (1, 64, 64), (1, 1531, 4096), (2, 33, 17), (3, 100, 1000), (5, 513, 129), (8, 256, 2048),
               (9, 128, 128), (16, 136, 96), (17, 250, 384), (31, 1000, 1000), (33, 64, 8192), (64, 512, 512),
               (100, 128, 4097), (127, 129, 255), (128, 256, 256), (129, 257, 300), (333, 1531, 1000),
               (1000, 72, 2048), (2500, 700, 130), (257, 1, 1), (300, 129, 127),
@@ -350,7 +350,7 @@ def _ffn_ref(x, wg, wu, wd, dy, dtype):
     return out
 
 
-FFN_SIZES = [(1, 1, 1), (1, 64, 64), (1, 128, 512), (2, 33, 70), (3, 128, 300), (4, 256, 1024), (5, 7, 3), (8, 520, 1368),
+FFN_SIZES = [(1, 1, 1), (1, 70, 150), (3, 1498, 856), (20, 90, 202), (1, 64, 64), (1, 128, 512), (2, 33, 70), (3, 128, 300), (4, 256, 1024), (5, 7, 3), (8, 520, 1368),
              (9, 256, 256), (17, 100, 333), (33, 128, 512), (64, 64, 4096), (100, 136, 200), (128, 128, 128),
              (129, 130, 131), (192, 256, 1024), (257, 264, 520), (777, 520, 1368), (3000, 256, 512), (5, 1024, 72), (40, 1024, 200), (260, 64, 96), (400, 100, 90), (300, 72, 4100), (257, 1, 1),
              (333, 1032, 260), (300, 2048, 131)]
