@@ -29,7 +29,31 @@ struct RowTeam {
     for (int o = (LANES ? LANES : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }
-  // slot: 32 floats of shared memory that no other pending reduction uses
+  static __device__ __forceinline__ uint32_t largest(uint32_t v) {
+    if (!LANES || LANES == 32) return __reduce_max_sync(0xffffffffu, v);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = ::max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
+  // slot: 32 elements of shared memory that no other pending reduction uses
+  // the sum of v; bits becomes the row's largest
+  __device__ __forceinline__ float sum_and_max(float v, uint32_t &bits, float *slot, uint32_t *slot_max) const {
+    v = add(v);
+    bits = largest(bits);
+    if (LANES) return v;
+    const int warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+      slot[threadIdx.x >> 5] = v;
+      slot_max[threadIdx.x >> 5] = bits;
+    }
+    __syncthreads();
+    float total = 0.0f;
+    for (int i = 0; i < warps; ++i) {
+      total += slot[i];
+      bits = ::max(bits, slot_max[i]);
+    }
+    return total;
+  }
   __device__ __forceinline__ float sum(float v, float *slot) const {
     v = add(v);
     if (LANES) return v;
@@ -55,12 +79,7 @@ struct RowTeam {
     return total;
   }
   __device__ __forceinline__ uint32_t max(uint32_t v, uint32_t *slot) const {
-    if (LANES && LANES < 32) {
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) v = ::max(v, __shfl_xor_sync(0xffffffffu, v, o));
-      return v;
-    }
-    v = __reduce_max_sync(0xffffffffu, v);
+    v = largest(v);
     if (LANES) return v;
     const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
@@ -80,51 +99,41 @@ __device__ __forceinline__ long long team_row(long long rows, bool &live) {
   return live ? row : rows - 1;
 }
 
-// A chunk of a row of `width` elements at element c. SHIFT: c may be negative or the
-// chunk reach past the row; only what is inside is read or written.
-template <bool SHIFT, class T, int VEC>
-__device__ __forceinline__ Chunk<T, VEC> load_part(const T *p, int c, int width) {
-  if (!SHIFT || (c >= 0 && c + VEC <= width)) return load_chunk<T, VEC>(p + c);
-  Chunk<T, VEC> v{};
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (c + i >= 0 && c + i < width) v.e[i] = p[c + i];
-  return v;
-}
-template <bool SHIFT, class T, int VEC>
-__device__ __forceinline__ void store_part(T *p, int c, int width, const Chunk<T, VEC> &v) {
-  if (!SHIFT || (c >= 0 && c + VEC <= width)) {
-    store_chunk<T, VEC>(p + c, v);
-    return;
+// Which elements of a row a thread holds: chunks of VEC, from the row's start or (SHIFT)
+// from the first boundary of VEC elements in it; then what is left before the first and
+// after the last whole chunk, fewer than VEC elements each, goes one to a thread. So no
+// chunk is looked at element by element, and rows of any start and length cost little
+// more than those on the boundaries.
+template <bool SHIFT, int VEC>
+struct Span {
+  int first, width, edge;  // of the first chunk; edge: this thread's single element, -1 for none
+  template <class T>
+  __device__ Span(const T *row, int w, int t) : first(0), width(w), edge(-1) {
+    if (!SHIFT) return;
+    first = min(int((VEC - reinterpret_cast<uintptr_t>(row) / sizeof(T) % VEC) % VEC), w);
+    const int e = t < first ? t : t + (w - first) / VEC * VEC;
+    if (e < w && t < 2 * VEC) edge = e;
   }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (c + i >= 0 && c + i < width) p[c + i] = v.e[i];
-}
-// the same for what lies on other boundaries than the row's: element by element
+  __device__ __forceinline__ int at(int chunk) const { return first + chunk * VEC; }
+  __device__ __forceinline__ bool holds(int c) const { return SHIFT ? c + VEC <= width : c < width; }
+};
+// a chunk of what may lie on other boundaries than the row that the span is of
 template <bool SHIFT, class T, int VEC>
-__device__ __forceinline__ Chunk<T, VEC> load_apart(const T *p, int c, int width) {
-  if (!SHIFT) return load_chunk<T, VEC>(p + c);
-  Chunk<T, VEC> v{};
+__device__ __forceinline__ Chunk<T, VEC> load_apart(const T *p) {
+  if (!SHIFT) return load_chunk<T, VEC>(p);
+  Chunk<T, VEC> v;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (c + i >= 0 && c + i < width) v.e[i] = p[c + i];
+  for (int i = 0; i < VEC; ++i) v.e[i] = p[i];
   return v;
 }
 template <bool SHIFT, class T, int VEC>
-__device__ __forceinline__ void store_apart(T *p, int c, int width, const Chunk<T, VEC> &v) {
+__device__ __forceinline__ void store_apart(T *p, const Chunk<T, VEC> &v) {
   if (!SHIFT) {
-    store_chunk<T, VEC>(p + c, v);
+    store_chunk<T, VEC>(p, v);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (c + i >= 0 && c + i < width) p[c + i] = v.e[i];
-}
-// elements of a row past the last 16-byte boundary before it
-template <bool SHIFT, class T>
-__device__ __forceinline__ int phase(const T *row) {
-  return SHIFT ? int(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)) : 0;
+  for (int i = 0; i < VEC; ++i) p[i] = v.e[i];
 }
 
 // y = s w rstd, s = x + residual as stored. QUANT: y goes to 8 bits with the row's scale.
@@ -141,68 +150,95 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
   const int width = int(a.width);
   const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
   const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+  T *s = static_cast<T *>(a.s) + row * a.s_stride;
   const W *w = static_cast<const W *>(a.weight);
-  const int shift = phase<SHIFT>(x);
+  const Span<SHIFT, VEC> span(x, width, team.t);
 
   Chunk<T, VEC> cx[N], cr[N];
   Chunk<W, VEC> cw[N];
+  T ex{}, er{};
+  W ew{};
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC - shift;
-    if (c < width) {
-      cx[j] = load_part<SHIFT, T, VEC>(x, c, width);
-      if (r) cr[j] = load_part<SHIFT, T, VEC>(r, c, width);
-      cw[j] = load_apart<SHIFT, W, VEC>(w, c, width);
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) {
+      cx[j] = load_chunk<T, VEC>(x + c);
+      if (r) cr[j] = load_chunk<T, VEC>(r + c);
+      cw[j] = load_apart<SHIFT, W, VEC>(w + c);
     }
   }
-  float v[N * VEC], sq = 0.0f;
+  if (span.edge >= 0) {
+    ex = x[span.edge];
+    if (r) er = r[span.edge];
+    ew = w[span.edge];
+  }
+  float v[N * VEC], ve = 0.0f, sq = 0.0f, top = 0.0f;  // v: s, or (QUANT) s w
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC - shift;
-    if (c < width) {
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) {
       if (r) {
         // the stream is kept in the element type, and the norm is of what is kept
         float sum[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum[i] = to_float(cx[j].e[i]) + to_float(cr[j].e[i]);
         cx[j] = to_chunk<T, VEC>(sum);
-        if (live) store_part<SHIFT, T, VEC>(static_cast<T *>(a.s) + row * a.s_stride, c, width, cx[j]);
+        if (live) store_chunk<T, VEC>(s + c, cx[j]);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         v[j * VEC + i] = to_float(cx[j].e[i]);
         sq = fmaf(v[j * VEC + i], v[j * VEC + i], sq);
+        if (QUANT) {
+          v[j * VEC + i] *= to_float(cw[j].e[i]);
+          top = max_abs(top, v[j * VEC + i]);
+        }
       }
     }
+  }
+  if (span.edge >= 0) {
+    if (r) {
+      ex = from_float<T>(to_float(ex) + to_float(er));
+      if (live) s[span.edge] = ex;
+    }
+    ve = to_float(ex);
+    sq = fmaf(ve, ve, sq);
+    if (QUANT) {
+      ve *= to_float(ew);
+      top = max_abs(top, ve);
+    }
+  }
+  if (QUANT) {  // the largest y is that of s w: both statistics in one reduction
+    uint32_t bits = __float_as_uint(top) & 0x7fffffffu;
+    const float rstd = rsqrtf(fmaf(team.sum_and_max(sq, bits, slot, slot_max), inv_width, eps));
+    float inv;
+    const float scale = row_scale(__float_as_uint(__uint_as_float(bits) * rstd) & 0x7fffffffu, inv);
+    if (!live) return;
+    if (team.t == 0) a.scales[row] = scale;
+    if (inv != 0.0f) inv *= rstd;
+    signed char *codes = a.codes + row * a.codes_stride;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = span.at(j * team.size + team.t);
+      if (span.holds(c)) store_apart<SHIFT, signed char, VEC>(codes + c, to_codes<VEC>(v + j * VEC, inv));
+    }
+    if (span.edge >= 0) codes[span.edge] = to_codes<1>(&ve, inv).e[0];
+    return;
   }
   const float rstd = rsqrtf(fmaf(team.sum(sq, slot), inv_width, eps));
-  float top = 0.0f;
+  if (!live) return;
+  T *out = static_cast<T *>(a.y) + row * a.y_stride;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC - shift;
-    if (c < width) {
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) {
       float y[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        y[i] = v[j * VEC + i] * rstd * to_float(cw[j].e[i]);
-        v[j * VEC + i] = y[i];
-        if (QUANT) top = max_abs(top, y[i]);
-      }
-      if (!QUANT && live)
-        store_part<SHIFT, T, VEC>(static_cast<T *>(a.y) + row * a.y_stride, c, width, to_chunk<T, VEC>(y));
+      for (int i = 0; i < VEC; ++i) y[i] = v[j * VEC + i] * rstd * to_float(cw[j].e[i]);
+      store_chunk<T, VEC>(out + c, to_chunk<T, VEC>(y));
     }
   }
-  if (!QUANT) return;
-  float inv;
-  const float scale = row_scale(team.max(__float_as_uint(top) & 0x7fffffffu, slot_max), inv);
-  if (!live) return;
-  if (team.t == 0) a.scales[row] = scale;
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC - shift;
-    if (c < width)
-      store_apart<SHIFT, signed char, VEC>(a.codes + row * a.codes_stride, c, width, to_codes<VEC>(v + j * VEC, inv));
-  }
+  if (span.edge >= 0) out[span.edge] = from_float<T>(ve * rstd * to_float(ew));
 }
 
 // dx = rstd (a - xh mean(a xh)) + ds with a = dy w, xh = s rstd; each block also
@@ -219,14 +255,16 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
   const int width = int(a.width);
   constexpr int kTeams = LANES ? kTeamThreads / (LANES ? LANES : 1) : 1;
   const int team_id = LANES ? threadIdx.x / (LANES ? LANES : 1) : 0;
-  // SHIFT: the grid's rows a step are a multiple of 8, so that a team's rows share their phase
-  const int shift = phase<SHIFT>(static_cast<const T *>(a.s) + ((long long)blockIdx.x * kTeams + team_id) * a.s_stride);
+  // SHIFT: the grid's rows a step are a multiple of 8, so that a team's rows share their span
+  const Span<SHIFT, VEC> span(static_cast<const T *>(a.s) + ((long long)blockIdx.x * kTeams + team_id) * a.s_stride,
+                              width, team.t);
+  const W *w = static_cast<const W *>(a.weight);
   Chunk<W, VEC> cw[N];
-  float dw[N * VEC];
+  float dw[N * VEC], we = span.edge >= 0 ? to_float(w[span.edge]) : 0.0f, dwe = 0.0f;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC - shift;
-    if (c < width) cw[j] = load_apart<SHIFT, W, VEC>(static_cast<const W *>(a.weight), c, width);
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) cw[j] = load_apart<SHIFT, W, VEC>(w + c);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j * VEC + i] = 0.0f;
   }
@@ -239,21 +277,27 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
     const T *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
     const T *ds = a.ds ? static_cast<const T *>(a.ds) + row * a.ds_stride : nullptr;
     Chunk<T, VEC> cs[N], cd[N], ce[N];
+    T es{}, ed{}, ee{};
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC - shift;
+      const int c = span.at(j * team.size + team.t);
       if (SHIFT) cs[j] = cd[j] = ce[j] = Chunk<T, VEC>{};
-      if ((live || !SHIFT) && c < width) {  // the last row again, or (another phase) none
-        cs[j] = load_part<SHIFT, T, VEC>(s, c, width);
-        cd[j] = load_part<SHIFT, T, VEC>(dy, c, width);
-        if (ds) ce[j] = load_part<SHIFT, T, VEC>(ds, c, width);
+      if ((live || !SHIFT) && span.holds(c)) {  // the last row again, or (another span) none
+        cs[j] = load_chunk<T, VEC>(s + c);
+        cd[j] = load_chunk<T, VEC>(dy + c);
+        if (ds) ce[j] = load_chunk<T, VEC>(ds + c);
       }
+    }
+    const bool edge = live && span.edge >= 0;
+    if (edge) {
+      es = s[span.edge];
+      ed = dy[span.edge];
+      if (ds) ee = ds[span.edge];
     }
     float sq = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC - shift;
-      if (c < width) {
+      if (span.holds(span.at(j * team.size + team.t))) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float f = to_float(cs[j].e[i]);
@@ -262,15 +306,20 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
         }
       }
     }
+    if (SHIFT) {
+      sq = fmaf(to_float(es), to_float(es), sq);
+      dot = fmaf(to_float(es), to_float(ed) * we, dot);
+    }
     const float2 total = team.sum2(sq, dot, slot[parity]);
     parity ^= 1;
     if (!live) continue;
     const float rstd = rsqrtf(fmaf(total.x, inv_width, eps));
     const float back = -(total.y * rstd * inv_width) * rstd * rstd;  // - mean(a xh) rstd^2, times s
+    T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC - shift;
-      if (c < width) {
+      const int c = span.at(j * team.size + team.t);
+      if (span.holds(c)) {
         float out[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -279,29 +328,25 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
           const float rest = ds ? fmaf(f, back, to_float(ce[j].e[i])) : f * back;
           out[i] = fmaf(d * to_float(cw[j].e[i]), rstd, rest);
         }
-        store_part<SHIFT, T, VEC>(static_cast<T *>(a.dx) + row * a.dx_stride, c, width, to_chunk<T, VEC>(out));
+        store_chunk<T, VEC>(dx + c, to_chunk<T, VEC>(out));
       }
     }
-  }
-  if (!LANES) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * team.size + team.t) * VEC - shift;
-      if (c < width)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (!SHIFT || (c + i >= 0 && c + i < width)) partial[(size_t)blockIdx.x * width + c + i] = dw[j * VEC + i];
+    if (edge) {
+      const float f = to_float(es), d = to_float(ed);
+      dwe = fmaf(d, f * rstd, dwe);
+      dx[span.edge] = from_float<T>(fmaf(d * we, rstd, ds ? fmaf(f, back, to_float(ee)) : f * back));
     }
-    return;
   }
+  float *sums = LANES ? column + team_id * width : partial + (size_t)blockIdx.x * width;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC - shift;
-    if (c < width)
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c))
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (!SHIFT || (c + i >= 0 && c + i < width)) column[team_id * width + c + i] = dw[j * VEC + i];
+      for (int i = 0; i < VEC; ++i) sums[c + i] = dw[j * VEC + i];
   }
+  if (span.edge >= 0) sums[span.edge] = dwe;
+  if (!LANES) return;
   __syncthreads();
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
     float total = 0.0f;
@@ -456,7 +501,7 @@ __global__ void k_column_sum(int nparts, int width, const float *__restrict__ pa
 }
 
 // 8-bit rows of silu(g) u
-template <class T, int VEC, int N, int LANES>
+template <class T, int VEC, int N, int LANES, bool SHIFT>
 __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024) k_gate_int8(const so3lr_gate_int8_args a) {
   __shared__ uint32_t slot[32];
   dependents_may_start();
@@ -466,20 +511,24 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024) k_gate_int8(const
   const long long row = team_row<LANES>(a.rows, live);
   const int hidden = int(a.hidden);
   const T *g = static_cast<const T *>(a.gu) + row * a.gu_stride, *u = g + hidden;
+  const Span<SHIFT, VEC> span(g, hidden, team.t);
   Chunk<T, VEC> cg[N], cu[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
-    if (c < hidden) {
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) {
       cg[j] = load_chunk<T, VEC>(g + c);
-      cu[j] = load_chunk<T, VEC>(u + c);
+      cu[j] = load_apart<SHIFT, T, VEC>(u + c);
     }
   }
-  float v[N * VEC], top = 0.0f;
+  float v[N * VEC], ve = 0.0f, top = 0.0f;
+  if (span.edge >= 0) {
+    ve = silu_f32(to_float(g[span.edge])) * to_float(u[span.edge]);
+    top = max_abs(top, ve);
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
-    if (c < hidden) {
+    if (span.holds(span.at(j * team.size + team.t))) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         v[j * VEC + i] = silu_f32(to_float(cg[j].e[i])) * to_float(cu[j].e[i]);
@@ -491,12 +540,13 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024) k_gate_int8(const
   const float scale = row_scale(team.max(__float_as_uint(top) & 0x7fffffffu, slot), inv);
   if (!live) return;
   if (team.t == 0) a.scales[row] = scale;
+  signed char *codes = a.codes + row * a.codes_stride;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (j * team.size + team.t) * VEC;
-    if (c < hidden)
-      store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) store_apart<SHIFT, signed char, VEC>(codes + c, to_codes<VEC>(v + j * VEC, inv));
   }
+  if (span.edge >= 0) codes[span.edge] = to_codes<1>(&ve, inv).e[0];
 }
 
 // k_gate_int8 for many rows on 16-byte boundaries: 32 elements a thread, rows through a ring
@@ -565,10 +615,15 @@ __global__ void k_dequantize_int8(const so3lr_dequantize_int8_args a) {
     const long long row = total < (1LL << 31) ? uint32_t(i) / uint32_t(per_row) : i / per_row;
     const signed char *codes = a.codes + row * a.codes_stride;
     T *out = static_cast<T *>(a.out) + row * a.out_stride;
-    const int c = int(i - row * per_row) * VEC - phase<!WIDE>(out);
+    const int shift = WIDE ? 0 : int(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T));
+    const int c = int(i - row * per_row) * VEC - shift;
     if (c >= width) continue;
     const float scale = a.scales[row];
-    const Chunk<signed char, VEC> q = load_apart<!WIDE, signed char, VEC>(codes, c, width);
+    if (!WIDE && (c < 0 || c + VEC > width)) {
+      for (int k = max(c, 0); k < min(c + VEC, width); ++k) out[k] = from_float<T>(float(codes[k]) * scale);
+      continue;
+    }
+    const Chunk<signed char, VEC> q = load_apart<!WIDE, signed char, VEC>(codes + c);
 #pragma unroll
     for (int j = 0; j < VEC; j += kPer) {
       float f[kPer];
@@ -576,7 +631,7 @@ __global__ void k_dequantize_int8(const so3lr_dequantize_int8_args a) {
       for (int k = 0; k < kPer; ++k)
         f[k] = WIDE ? byte_to_float(reinterpret_cast<const uint32_t *>(&q)[(j + k) / 4] ^ 0x80808080u, (j + k) % 4) * scale
                     : float(q.e[j + k]) * scale;
-      store_part<!WIDE, T, kPer>(out, c + j, width, to_chunk<T, kPer>(f));
+      store_chunk<T, kPer>(out + c + j, to_chunk<T, kPer>(f));
     }
   }
 }
@@ -589,9 +644,10 @@ bool aligned(const void *p, long long stride, int size, int bytes) {
 // Threads that hold a row of `width` elements, `per` of them each.
 int row_threads(long long width, int per) { return int((width + 32LL * per - 1) / (32LL * per)) * 32; }
 
-// How a thread's chunks lie: 16-byte ones on the row's start (kWide), or counted from
-// the boundary before it (kShifted), or single elements.
+// How a thread's elements lie: 16-byte chunks from the row's start (kWide) or from the
+// first boundary in it (kShifted, see Span), or single elements.
 enum Path { kScalar, kWide, kShifted };
+constexpr int chunk_of(Path path, int size) { return path == kScalar ? 1 : 16 / size; }
 struct RowTensors {  // of one row: all that is moved in chunks of the element type
   int size;
   bool any = false, same = true;
@@ -604,12 +660,10 @@ struct RowTensors {  // of one row: all that is moved in chunks of the element t
     base = b;
     step = t;
   }
-  // `rest_aligned`: what is moved beside them in chunks lies on its boundaries. A shifted
-  // row of the longest width would not fit a block.
+  // `rest_aligned`: what is moved beside them in chunks lies on its boundaries
   Path path(long long width, bool rest_aligned) const {
     if (!same) return kScalar;
-    if (base == 0 && step == 0 && width * size % 16 == 0 && rest_aligned) return kWide;
-    return width + 16 / size - 1 <= 16384 ? kShifted : kScalar;
+    return base == 0 && step == 0 && width * size % 16 == 0 && rest_aligned ? kWide : kShifted;
   }
 };
 
@@ -623,10 +677,9 @@ struct RowTensors {  // of one row: all that is moved in chunks of the element t
 struct Hold {
   int lanes, per;
 };
-Hold hold(long long width, Path path, int vec, bool to_8_bits) {
-  if (path == kShifted) width += vec - 1;
+Hold hold(long long width, Path path, int size, bool to_8_bits) {
   if (path != kScalar) {
-    if (width <= 64) return {8, 8};
+    if (width <= 64 && (path == kWide || size == 4)) return {8, 8};  // the edges of a row: up to 14 threads
     if (width <= 128) return {16, 8};
     if (width <= 512) return {32, width <= 256 ? 8 : 16};
     if (to_8_bits) return width <= 1024 ? Hold{32, 32} : Hold{0, 16};
@@ -719,9 +772,7 @@ Path backward_path(const so3lr_rms_norm_backward_args &a) {
   return t.path(a.width, aligned(a.weight, 0, 1, 16));
 }
 Hold backward_hold(const so3lr_rms_norm_backward_args &a, Path path) {
-  const int vec = a.dtype == SO3LR_FLOAT32 ? 4 : 8;
-  // a block of 512 threads holds 4096 elements, 8 each
-  return hold(a.width, path, vec, false);
+  return hold(a.width, path, a.dtype == SO3LR_FLOAT32 ? 4 : 2, false);
 }
 // The ring kernel's blocks, no stages where the direct loads serve: rows of a warp,
 // unaligned rows, and rows too long for the ring
@@ -743,7 +794,7 @@ int backward_parts(const so3lr_rms_norm_backward_args &a) {
 
 template <class T, class W, Path PATH>
 void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int grid, cudaStream_t s) {
-  constexpr int V = PATH == kScalar ? 1 : 16 / int(sizeof(T));
+  constexpr int V = chunk_of(PATH, sizeof(T));
   constexpr bool SHIFT = PATH == kShifted;
   const Hold h = backward_hold(a, PATH);
   by_hold<PATH>(h, [&](auto lanes, auto per) {
@@ -754,7 +805,7 @@ void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int gr
              kTeamThreads / L * a.width * sizeof(float), s, a, partial, inv, eps);
     } else if constexpr (L == 0) {
       // rows that start elsewhere than on 16-byte boundaries, and those too long for the ring
-      const int threads = row_threads(a.width + (SHIFT ? V - 1 : 0), P);
+      const int threads = row_threads(a.width, P);
       if constexpr (PATH != kWide && P == 8) {
         if (threads <= 512) {
           launch(k_rms_norm_backward<T, W, V, N, 0, 512, SHIFT>, grid, threads, 0, s, a, partial, inv, eps);
@@ -793,19 +844,16 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
       t.add(a.residual, a.residual_stride);
       t.add(a.s, a.s_stride);
       t.add(a.y, a.y_stride);
-      Path chosen = t.path(a.width, aligned(a.codes, a.codes_stride, 1, V) && aligned(a.weight, 0, 1, 16));
-      // 2-byte rows to codes on other boundaries: the codes' single stores undo what the chunks save (1003
-      // bfloat16: 1.25 TB/s in chunks, 1.4 in elements; float32 3.0 and 2.3)
-      if (chosen == kShifted && a.codes && sizeof(T) == 2) chosen = kScalar;
+      const Path chosen = t.path(a.width, aligned(a.codes, a.codes_stride, 1, V) && aligned(a.weight, 0, 1, 16));
       by_path(chosen, [&](auto path) {
         constexpr Path PATH = decltype(path)::value;
-        constexpr int VEC = PATH == kScalar ? 1 : V;
-        const Hold h = hold(a.width, PATH, V, a.codes != nullptr);
+        constexpr int VEC = chunk_of(PATH, sizeof(T));
+        const Hold h = hold(a.width, PATH, sizeof(T), a.codes != nullptr);
         by_hold<PATH>(h, [&](auto lanes, auto per) {
           constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
           constexpr bool SHIFT = PATH == kShifted;
           const auto fn = a.codes ? &k_rms_norm<T, W, VEC, N, L, true, SHIFT> : &k_rms_norm<T, W, VEC, N, L, false, SHIFT>;
-          launch(fn, team_grid(h, a.rows), team_block(h, a.width + (SHIFT ? V - 1 : 0)), 0, s, a,
+          launch(fn, team_grid(h, a.rows), team_block(h, a.width), 0, s, a,
                  1.0f / float(a.width), float(a.eps));
         });
       });
@@ -851,22 +899,22 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s) {
       gate_ring<T>(a, r, s);
       return;
     }
-    const Hold h = a.hidden > 16384 ? Hold{0, 32} : hold(a.hidden, wide ? kWide : kScalar, V, true);
-    auto run = [&](auto path) {
+    const Path chosen = wide ? kWide : a.hidden <= 16384 ? kShifted : kScalar;
+    const Hold h = a.hidden > 16384 ? Hold{0, 32} : hold(a.hidden, chosen, e, true);
+    by_path(chosen, [&](auto path) {
       constexpr Path PATH = decltype(path)::value;
-      constexpr int VEC = PATH == kWide ? V : 1;
-      if (h.per == 32 && h.lanes == 0)  // 32768 columns in a block of 1,024 threads
-        launch(k_gate_int8<T, VEC, 32 / VEC, 0>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
-      else
-        by_hold<PATH>(h, [&](auto lanes, auto per) {
-          constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
-          launch(k_gate_int8<T, VEC, N, L>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
-        });
-    };
-    if (wide)
-      run(std::integral_constant<Path, kWide>{});
-    else
-      run(std::integral_constant<Path, kScalar>{});
+      constexpr int VEC = chunk_of(PATH, sizeof(T));
+      constexpr bool SHIFT = PATH == kShifted;
+      if constexpr (PATH != kShifted)
+        if (h.per == 32 && h.lanes == 0) {  // 32768 columns in a block of 1,024 threads
+          launch(k_gate_int8<T, VEC, 32 / VEC, 0, false>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
+          return;
+        }
+      by_hold<PATH>(h, [&](auto lanes, auto per) {
+        constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
+        launch(k_gate_int8<T, VEC, N, L, SHIFT>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
+      });
+    });
   });
 }
 
