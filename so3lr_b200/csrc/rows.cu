@@ -136,6 +136,49 @@ __device__ __forceinline__ void store_apart(T *p, const Chunk<T, VEC> &v) {
   for (int i = 0; i < VEC; ++i) p[i] = v.e[i];
 }
 
+// A ring of rows in shared memory, filled by bulk copies: what is in flight costs no
+// registers, so a block that walks over rows keeps the memory system busy while it
+// reduces and writes the current one. One block barrier after the last read of a
+// stage, thread 0 may refill it.
+struct RowRing {
+  uint32_t bars, buffer, stage_bytes;
+  int stages;
+  unsigned char *mem;
+  int *err;
+  volatile int *abort_flag;
+
+  __device__ RowRing(unsigned char *smem, uint32_t bytes, int nstages, int *error)
+      : stage_bytes(bytes), stages(nstages), mem(smem + 128), err(error) {
+    bars = tc::smem_u32(smem);
+    buffer = bars + 128;
+    abort_flag = reinterpret_cast<volatile int *>(smem + 120);
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) tc::mbar_init(bars + 8 * i, 1);
+      *abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+  }
+  __device__ const unsigned char *stage(int i) const { return mem + (i % stages) * stage_bytes; }
+  // waits for the i-th row of this block; after a wait that gave up (reported in *err) nothing waits again
+  __device__ void wait(int i) const { tc::mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, abort_flag, err, 7); }
+  // thread 0: the copies of the i-th row
+  __device__ uint32_t expect(int i, uint32_t bytes) const {
+    tc::mbar_expect_tx(bars + 8 * (i % stages), bytes);
+    return buffer + (i % stages) * stage_bytes;
+  }
+  __device__ uint32_t bar(int i) const { return bars + 8 * (i % stages); }
+};
+constexpr int kRingHeader = 128, kRingStages = 8;
+
+// The scale of a row of s w rstd from the bits of max|s w|; `inv` takes s w to codes.
+__device__ __forceinline__ float norm_scale(float mean_square, uint32_t top_bits, float &inv) {
+  const float rstd = rsqrtf(mean_square);
+  const float scale = row_scale(__float_as_uint(__uint_as_float(top_bits) * rstd) & 0x7fffffffu, inv);
+  if (inv != 0.0f) inv *= rstd;
+  return scale;
+}
+
 // y = s w rstd, s = x + residual as stored. QUANT: y goes to 8 bits with the row's scale.
 template <class T, class W, int VEC, int N, int LANES, bool QUANT, bool SHIFT>
 __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
@@ -210,12 +253,11 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
   }
   if (QUANT) {  // the largest y is that of s w: both statistics in one reduction
     uint32_t bits = __float_as_uint(top) & 0x7fffffffu;
-    const float rstd = rsqrtf(fmaf(team.sum_and_max(sq, bits, slot, slot_max), inv_width, eps));
+    const float sum = team.sum_and_max(sq, bits, slot, slot_max);
     float inv;
-    const float scale = row_scale(__float_as_uint(__uint_as_float(bits) * rstd) & 0x7fffffffu, inv);
+    const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv);
     if (!live) return;
     if (team.t == 0) a.scales[row] = scale;
-    if (inv != 0.0f) inv *= rstd;
     signed char *codes = a.codes + row * a.codes_stride;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -244,7 +286,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
 // dx = rstd (a - xh mean(a xh)) + ds with a = dy w, xh = s rstd; each block also
 // sums dy xh over its rows (a fixed set, in order) into one row of `partial`.
 template <class T, class W, int VEC, int N, int LANES, int MAXT, bool SHIFT>
-__global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ? 4 : 1)
+__global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ? 4 : LANES ? 2 : 1)
     k_rms_norm_backward(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, const float inv_width,
                         const float eps) {
   __shared__ float2 slot[2][32];
@@ -356,40 +398,78 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
   }
 }
 
-// A ring of rows in shared memory, filled by bulk copies: what is in flight costs no
-// registers, so a block that walks over rows keeps the memory system busy while it
-// reduces and writes the current one. One block barrier after the last read of a
-// stage, thread 0 may refill it.
-struct RowRing {
-  uint32_t bars, buffer, stage_bytes;
-  int stages;
-  unsigned char *mem;
-  int *err;
-  volatile int *abort_flag;
-
-  __device__ RowRing(unsigned char *smem, uint32_t bytes, int nstages, int *error)
-      : stage_bytes(bytes), stages(nstages), mem(smem + 128), err(error) {
-    bars = tc::smem_u32(smem);
-    buffer = bars + 128;
-    abort_flag = reinterpret_cast<volatile int *>(smem + 120);
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < stages; ++i) tc::mbar_init(bars + 8 * i, 1);
-      *abort_flag = 0;
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+// k_rms_norm to 8 bits for many rows on 16-byte boundaries: 16 elements a thread, rows
+// through a ring, the weight in registers
+template <class T, class W>
+__global__ void __launch_bounds__(512)
+    k_rms_norm_int8_ring(const so3lr_rms_norm_args a, int stages, int *err, const float inv_width, const float eps) {
+  constexpr int VEC = 16 / sizeof(T), N = 16 / VEC;
+  __shared__ float slot[2][32];
+  __shared__ uint32_t slot_max[2][32];
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
+  const uint32_t row_bytes = width * sizeof(T), tensors = a.residual ? 2 : 1;
+  dependents_may_start();
+  const RowRing ring(smem, tensors * row_bytes, stages, err);
+  wait_for_predecessors();
+  const RowTeam<0> team;
+  const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
+  auto fetch = [&](int i) {
+    const long long row = blockIdx.x + (long long)i * gridDim.x;
+    const uint32_t dst = ring.expect(i, tensors * row_bytes);
+    tc::bulk_load(dst, static_cast<const T *>(a.x) + row * a.x_stride, row_bytes, ring.bar(i));
+    if (a.residual)
+      tc::bulk_load(dst + row_bytes, static_cast<const T *>(a.residual) + row * a.residual_stride, row_bytes, ring.bar(i));
+  };
+  if (t == 0)
+    for (int i = 0; i < min(stages, rows); ++i) fetch(i);
+  Chunk<W, VEC> cw[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = (j * size + t) * VEC;
+    if (c < width) cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
+  }
+  for (int k = 0; k < rows; ++k) {
+    ring.wait(k);
+    const T *x = reinterpret_cast<const T *>(ring.stage(k));
+    const long long row = blockIdx.x + (long long)k * gridDim.x;
+    float v[16], sq = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        Chunk<T, VEC> cx = load_chunk<T, VEC>(x + c);
+        if (a.residual) {
+          const Chunk<T, VEC> cr = load_chunk<T, VEC>(x + width + c);
+          float sum[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum[i] = to_float(cx.e[i]) + to_float(cr.e[i]);
+          cx = to_chunk<T, VEC>(sum);
+          store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float f = to_float(cx.e[i]);
+          sq = fmaf(f, f, sq);
+          v[j * VEC + i] = f * to_float(cw[j].e[i]);
+          top = max_abs(top, v[j * VEC + i]);
+        }
+      }
     }
-    __syncthreads();
+    uint32_t bits = __float_as_uint(top) & 0x7fffffffu;
+    const float sum = team.sum_and_max(sq, bits, slot[k & 1], slot_max[k & 1]);  // every thread has read the stage
+    if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
+    float inv;
+    const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv);
+    if (t == 0) a.scales[row] = scale;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width)
+        store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
+    }
   }
-  __device__ const unsigned char *stage(int i) const { return mem + (i % stages) * stage_bytes; }
-  // waits for the i-th row of this block; after a wait that gave up (reported in *err) nothing waits again
-  __device__ void wait(int i) const { tc::mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, abort_flag, err, 7); }
-  // thread 0: the copies of the i-th row
-  __device__ uint32_t expect(int i, uint32_t bytes) const {
-    tc::mbar_expect_tx(bars + 8 * (i % stages), bytes);
-    return buffer + (i % stages) * stage_bytes;
-  }
-  __device__ uint32_t bar(int i) const { return bars + 8 * (i % stages); }
-};
-constexpr int kRingHeader = 128, kRingStages = 8;
+}
 
 // k_rms_norm_backward for rows on 16-byte boundaries that need a block: 16 elements a
 // thread, rows through a ring. Bound by instruction issue before it is bound by HBM:
@@ -549,58 +629,6 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024) k_gate_int8(const
   if (span.edge >= 0) codes[span.edge] = to_codes<1>(&ve, inv).e[0];
 }
 
-// k_gate_int8 for many rows on 16-byte boundaries: 32 elements a thread, rows through a ring
-constexpr int kGateRing = 32;
-template <class T>
-__global__ void __launch_bounds__(512) k_gate_int8_ring(const so3lr_gate_int8_args a, int stages, int *err) {
-  constexpr int VEC = 16 / sizeof(T), N = kGateRing / VEC;
-  __shared__ uint32_t slot[2][32];
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int hidden = int(a.hidden), t = threadIdx.x, size = blockDim.x;
-  const uint32_t row_bytes = 2 * hidden * sizeof(T);
-  dependents_may_start();
-  const RowRing ring(smem, row_bytes, stages, err);
-  wait_for_predecessors();
-  const RowTeam<0> team;
-  const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
-  auto fetch = [&](int i) {
-    const long long row = blockIdx.x + (long long)i * gridDim.x;
-    const uint32_t dst = ring.expect(i, row_bytes);
-    tc::bulk_load(dst, static_cast<const T *>(a.gu) + row * a.gu_stride, row_bytes, ring.bar(i));
-  };
-  if (t == 0)
-    for (int i = 0; i < min(stages, rows); ++i) fetch(i);
-  for (int k = 0; k < rows; ++k) {
-    ring.wait(k);
-    const T *g = reinterpret_cast<const T *>(ring.stage(k)), *u = g + hidden;
-    float v[kGateRing], top = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * size + t) * VEC;
-      if (c < hidden) {
-        const Chunk<T, VEC> cg = load_chunk<T, VEC>(g + c), cu = load_chunk<T, VEC>(u + c);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          v[j * VEC + i] = silu_f32(to_float(cg.e[i])) * to_float(cu.e[i]);
-          top = max_abs(top, v[j * VEC + i]);
-        }
-      }
-    }
-    float inv;
-    const uint32_t bits = team.max(__float_as_uint(top) & 0x7fffffffu, slot[k & 1]);  // every thread has read the stage
-    if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
-    const float scale = row_scale(bits, inv);
-    const long long row = blockIdx.x + (long long)k * gridDim.x;
-    if (t == 0) a.scales[row] = scale;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (j * size + t) * VEC;
-      if (c < hidden)
-        store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
-    }
-  }
-}
-
 // WIDE: 16 codes a thread, rows of both on 16-byte boundaries. Otherwise a 16-byte chunk
 // of the result, counted from the boundary before its row, from single codes.
 template <class T, bool WIDE>
@@ -667,26 +695,32 @@ struct RowTensors {  // of one row: all that is moved in chunks of the element t
   }
 };
 
-// How a row is held: lanes of a warp (0: a block) and elements a thread. Rows on
-// 16-byte boundaries: in a warp where 16 elements a lane suffice, as few lanes as hold
-// them with 8 each. Longer rows whose results are 8 bits, which issue more than they
-// move, stay in a warp up to 1024 elements and take 16 a thread of a block above; the
-// others take 8 up to 4096 (1024 bfloat16: 5.4 TB/s, 3.4 with 32 in a warp; 2048 to 8
-// bits 2.6 with 8 and 2.9 with 16; 8192: 3.2 with 8 and 4.4 with 16). Rows on other boundaries move single
-// elements, 8 a thread (16 where the row would not fit otherwise).
+// How a row is held: lanes of a warp (0: a block) and elements a thread. In a warp as
+// few lanes as hold it with 8 elements each, then 16; a block of 64 threads would be
+// bound by the rate at which blocks start (512 bfloat16 to 8 bits: 69 us, 31 in a warp).
+// Longer rows: their products 8 a thread where they are on the boundaries, 16 beyond 4096
+// and off the boundaries (1024: 41 us, 66 with 32 in a warp; 3001: 56 with 16, 63 with 8),
+// the gradient off them 8 (71 and 191). Rows that become 8 bits issue more than they
+// move and take fuller threads: 32 in a warp up to 1024 on the boundaries, above 32
+// in a block for the gate (2048: 27 us, 33 with 16), 16 for the norm (31, 42 with 32) and
+// for both off them (1003: 44 and 43 us, 49 and 52 in a warp). Bfloat16 rows, 33.5 M elements.
+enum RowOp { kNorm, kNormBack, kNorm8, kGate8 };
 struct Hold {
   int lanes, per;
 };
-Hold hold(long long width, Path path, int size, bool to_8_bits) {
+Hold hold(long long width, Path path, int size, RowOp op) {
   if (path != kScalar) {
-    if (width <= 64 && (path == kWide || size == 4)) return {8, 8};  // the edges of a row: up to 14 threads
+    // rows off the boundaries: their edges take up to 2 (16 / size - 1) threads
+    if (width <= 64 && (path == kWide || size == 4)) return {8, 8};
     if (width <= 128) return {16, 8};
-    if (width <= 512) return {32, width <= 256 ? 8 : 16};
-    if (to_8_bits) return width <= 1024 ? Hold{32, 32} : Hold{0, 16};
-    return {0, width <= 4096 ? 8 : 16};
   }
   if (width <= 512) return {32, width <= 256 ? 8 : 16};
-  return {0, width <= 8192 ? 8 : 16};
+  if (path == kScalar) return {0, width <= 8192 ? 8 : op == kGate8 && width > 16384 ? 32 : 16};
+  if (op == kNorm8 || op == kGate8) {
+    if (path == kShifted) return {0, 16};
+    return width <= 1024 ? Hold{32, 32} : Hold{0, op == kGate8 ? 32 : 16};
+  }
+  return {0, width <= (path == kShifted && op == kNorm ? 1024 : 4096) ? 8 : 16};
 }
 // f(std::integral_constant lanes, std::integral_constant per) for each that hold() gives
 template <Path PATH, class F>
@@ -772,7 +806,7 @@ Path backward_path(const so3lr_rms_norm_backward_args &a) {
   return t.path(a.width, aligned(a.weight, 0, 1, 16));
 }
 Hold backward_hold(const so3lr_rms_norm_backward_args &a, Path path) {
-  return hold(a.width, path, a.dtype == SO3LR_FLOAT32 ? 4 : 2, false);
+  return hold(a.width, path, a.dtype == SO3LR_FLOAT32 ? 4 : 2, kNormBack);
 }
 // The ring kernel's blocks, no stages where the direct loads serve: rows of a warp,
 // unaligned rows, and rows too long for the ring
@@ -817,18 +851,18 @@ void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int gr
   });
 }
 template <class T, class W>
+void norm_int8_ring(const so3lr_rms_norm_args &a, const RingPlan &r, cudaStream_t s) {
+  check_gave_up();
+  allow_dynamic_smem(reinterpret_cast<const void *>(&k_rms_norm_int8_ring<T, W>), 227 * 1024 - 1024);
+  launch(k_rms_norm_int8_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, r.stages, gave_up_flag(),
+         1.0f / float(a.width), float(a.eps));
+}
+template <class T, class W>
 void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, const RingPlan &r, cudaStream_t s) {
   check_gave_up();
   allow_dynamic_smem(reinterpret_cast<const void *>(&k_rms_norm_backward_ring<T, W>), 227 * 1024 - 1024);
   launch(k_rms_norm_backward_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, partial, r.stages,
          gave_up_flag(), 1.0f / float(a.width), float(a.eps));
-}
-
-template <class T>
-void gate_ring(const so3lr_gate_int8_args &a, const RingPlan &r, cudaStream_t s) {
-  check_gave_up();
-  allow_dynamic_smem(reinterpret_cast<const void *>(&k_gate_int8_ring<T>), 227 * 1024 - 1024);
-  launch(k_gate_int8_ring<T>, r.grid, row_threads(a.hidden, kGateRing), r.smem, s, a, r.stages, gave_up_flag());
 }
 
 }  // namespace
@@ -845,10 +879,15 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
       t.add(a.s, a.s_stride);
       t.add(a.y, a.y_stride);
       const Path chosen = t.path(a.width, aligned(a.codes, a.codes_stride, 1, V) && aligned(a.weight, 0, 1, 16));
+      const RingPlan r = ring_plan(a.rows, row_threads(a.width, 16), 2048, 2, (a.residual ? 2 : 1) * a.width * sizeof(T));
+      if (chosen == kWide && a.codes && a.width > 1024 && a.width <= 8192 && r.stages >= 2 && a.rows > 2 * r.grid) {
+        norm_int8_ring<T, W>(a, r, s);
+        return;
+      }
       by_path(chosen, [&](auto path) {
         constexpr Path PATH = decltype(path)::value;
         constexpr int VEC = chunk_of(PATH, sizeof(T));
-        const Hold h = hold(a.width, PATH, sizeof(T), a.codes != nullptr);
+        const Hold h = hold(a.width, PATH, sizeof(T), a.codes ? kNorm8 : kNorm);
         by_hold<PATH>(h, [&](auto lanes, auto per) {
           constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
           constexpr bool SHIFT = PATH == kShifted;
@@ -892,28 +931,18 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const int e = sizeof(T);
     const bool wide = a.hidden % V == 0 && aligned(a.gu, a.gu_stride, e, 16) && aligned(a.codes, a.codes_stride, 1, V);
-    // the ring for long rows, where a block has several to walk over (8192 bfloat16: 5.0
-    // TB/s, 4.6 without; 4096: 5.2, 5.6 without)
-    const RingPlan r = ring_plan(a.rows, row_threads(a.hidden, kGateRing), 1024, 3, 2 * a.hidden * e);
-    if (wide && a.hidden > 4096 && a.hidden <= 16384 && r.stages >= 2 && a.rows > 2 * r.grid) {
-      gate_ring<T>(a, r, s);
-      return;
-    }
     const Path chosen = wide ? kWide : a.hidden <= 16384 ? kShifted : kScalar;
-    const Hold h = a.hidden > 16384 ? Hold{0, 32} : hold(a.hidden, chosen, e, true);
+    const Hold h = hold(a.hidden, chosen, e, kGate8);
     by_path(chosen, [&](auto path) {
       constexpr Path PATH = decltype(path)::value;
       constexpr int VEC = chunk_of(PATH, sizeof(T));
-      constexpr bool SHIFT = PATH == kShifted;
-      if constexpr (PATH != kShifted)
-        if (h.per == 32 && h.lanes == 0) {  // 32768 columns in a block of 1,024 threads
-          launch(k_gate_int8<T, VEC, 32 / VEC, 0, false>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
-          return;
-        }
       by_hold<PATH>(h, [&](auto lanes, auto per) {
         constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
-        launch(k_gate_int8<T, VEC, N, L, SHIFT>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
+        launch(k_gate_int8<T, VEC, N, L, PATH == kShifted>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
       });
+      if constexpr (PATH != kShifted)
+        if (h.per == 32 && h.lanes == 0)
+          launch(k_gate_int8<T, VEC, 32 / VEC, 0, false>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
     });
   });
 }
