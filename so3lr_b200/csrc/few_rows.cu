@@ -1,8 +1,8 @@
 // Dense products of the feed-forward layers for few rows (single atoms or tokens,
 // small batches; the rule is in layers.hpp). All that counts is reading the weights
-// once for each 16 rows, from HBM or, for small weights, from L2:
-// a block takes 8 output channels and its warps split the contraction, so that a
-// 4096 x 4096 weight has 512 blocks. The products run on warp-level MMAs
+// once for each 16 rows, from HBM or, for small weights, from L2: a block takes 8
+// output channels and its warps split the contraction, so that a 4096 x 4096 weight has
+// 512 blocks; a long contraction to few channels is split over a cluster of blocks too. The products run on warp-level MMAs
 // (m16n8k16 / m16n8k32, rows as M, channels as N) straight from registers: a tile of
 // the tcgen05 kernel would be filled to a few of its 256 rows and would need its
 // operands in shared memory first.
@@ -13,6 +13,7 @@
 // same permutation of the contraction, so the sums are those of the formula.
 #include "layers_common.cuh"
 #include "model_host.hpp"
+#include "tensor_core.cuh"
 
 namespace so3lr_b200 {
 namespace {
@@ -102,7 +103,9 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
                 kOut = GATED ? 2 : 1;
   __shared__ Acc part[max_warps(TWO)][kOut][TWO ? 16 : 8][8];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n = blockIdx.x * 8 + g, row0 = blockIdx.y * 16, rows = min(16, a.rows - row0);
+  // the blocks of a cluster share its channels and split the contraction
+  const int splits = int(tc::cluster_size()), rank = int(tc::cluster_rank()), n0 = int(tc::cluster_index()) * 8;
+  const int n = n0 + g, row0 = blockIdx.y * 16, rows = min(16, a.rows - row0);
   // lanes beyond the last row or channel read it again; their results are not written
   const int cn = min(n, a.n - 1);
   const E *w = static_cast<const E *>(a.w) + cn * a.w_stride, *w2 = static_cast<const E *>(a.w2) + cn * a.w2_stride;
@@ -111,7 +114,8 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
   const E *l0 = LO ? static_cast<const E *>(a.rest) + (x0 - static_cast<const E *>(a.x)) : nullptr;
   const E *l1 = LO ? static_cast<const E *>(a.rest) + (x1 - static_cast<const E *>(a.x)) : nullptr;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer);
-  const int begin = int((long long)steps * warp / warps), end = int((long long)steps * (warp + 1) / warps);
+  const int which = rank * warps + warp, all = splits * warps;
+  const int begin = int((long long)steps * which / all), end = int((long long)steps * (which + 1) / all);
   dependents_may_start();
   // the first weights on their way to L2, which needs no order with the kernel before
 #pragma unroll
@@ -182,11 +186,35 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
     }
   }
   __syncthreads();
+  int parts = warps;
+  if (splits > 1) {  // all into the first part of the first block
+    parts = 1;
+    const int i = threadIdx.x, row = i >> 3, c = i & 7;  // 8 warps or more: a thread has one sum at most
+    if (i < 8 * rows)
+#pragma unroll
+      for (int o = 0; o < kOut; ++o) {
+        Acc sum{};
+        for (int k = 0; k < warps; ++k) sum += part[k][o][row][c];
+        part[0][o][row][c] = sum;
+      }
+    __syncwarp();
+    tc::cluster_sync();
+    if (rank == 0 && i < 8 * rows)
+#pragma unroll
+      for (int o = 0; o < kOut; ++o) {
+        Acc sum = part[0][o][row][c];
+        for (int k = 1; k < splits; ++k) sum += tc::load_of_rank(&part[0][o][row][c], k);
+        part[0][o][row][c] = sum;
+      }
+    __syncwarp();
+    tc::cluster_sync();  // no block leaves before its sums are read
+    if (rank != 0) return;
+  }
   for (int i = threadIdx.x; i < 8 * rows; i += blockDim.x) {
-    const int row = i >> 3, c = blockIdx.x * 8 + (i & 7);
+    const int row = i >> 3, c = n0 + (i & 7);
     if (c >= a.n) continue;
     Acc sum[kOut] = {};
-    for (int k = 0; k < warps; ++k)
+    for (int k = 0; k < parts; ++k)
 #pragma unroll
       for (int o = 0; o < kOut; ++o) sum[o] += part[k][o][row][i & 7];
     float y;
@@ -221,14 +249,18 @@ void run(const FewArgs &a, cudaStream_t s) {
   // where the blocks alone would leave too few loads in flight. One row, 2048 channels
   // of 8192 bfloat16 (256 blocks): 12.3 us with 8, 9.3 us with 16; 4096 channels of
   // 4096 bytes (512 blocks): 5.6 us with 8, 7.0 us with 16.
-  const dim3 grid(unsigned((a.n + 7) / 8), unsigned((a.rows + 15) / 16));
-  const int most = grid.x * grid.y < 2 * kSmCount ? max_warps(a.rows > 8) : 8;
+  const unsigned channels = unsigned((a.n + 7) / 8), groups = unsigned((a.rows + 15) / 16), blocks = channels * groups;
+  const int most = blocks < 2 * kSmCount ? max_warps(a.rows > 8) : 8;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer), warps = std::max(1, std::min(most, steps / 4));
-  const unsigned block = unsigned(32 * warps);
+  // Up to 8 blocks in a cluster split it too where SMs would be idle and each warp would have 12 steps or
+  // more (16 rows through the 64 x 8192 block: 16.7 us without, 7.6 with; where a warp has 8, 256 channels
+  // of 4096 bytes, a cluster costs what it gives: 3.0 and 3.2 us).
+  unsigned splits = 1;
+  while (splits < 8 && blocks * splits < kSmCount && steps >= 12 * int(splits) * warps) splits *= 2;
   auto go = [&](auto align) {
     constexpr int A = decltype(align)::value;
-    launch(a.rows > 8 ? &k_few_rows<E, O, GATED, LO, true, A> : &k_few_rows<E, O, GATED, LO, false, A>, grid, block, 0,
-           s, a);
+    launch_clusters(a.rows > 8 ? &k_few_rows<E, O, GATED, LO, true, A> : &k_few_rows<E, O, GATED, LO, false, A>,
+                    dim3(channels * splits, groups), unsigned(32 * warps), splits > 1 ? splits : 0, 0, s, a);
   };
   if (all_on(16))
     go(std::integral_constant<int, 16>{});

@@ -10,7 +10,6 @@
 
 namespace so3lr_b200 {
 
-
 // rows.cu
 void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s);
 long long rms_norm_backward_bytes(const so3lr_rms_norm_backward_args &a);
@@ -31,17 +30,21 @@ long long feed_forward_backward_bytes(const so3lr_feed_forward_backward_args &a)
 void launch_feed_forward_backward(const so3lr_feed_forward_backward_args &a, void *workspace, cudaStream_t s);
 
 // few_rows.cu: the forward products for few rows, any alignment, no workspace but the
-// hidden layer's. Its blocks read the weights once for every 16 rows, the tcgen05
-// tiles (dense.cu) once for 256 but with about 3 us more of set-up a launch. Measured
-// even: 64 rows of a 1.5 MB 8-bit weight (4.5 and 6.1 us; 96 rows 8.2 and 6.3), 128 rows
-// through a block of 6.3 MB (14.6 and 16.1 us), 32 through one of 25 MB (17 and 21).
+// hidden layer's. Its blocks read the weights once for every 16 rows, about 4 MB a
+// microsecond; the tcgen05 tiles (dense.cu) read them once for 256, but a launch takes 3
+// us or more, and longer the longer its contraction. Few rows are those where 16 or
+// fewer, or the weights times the groups of 16 below a limit that grows with the
+// contraction. Measured even (us in this kernel and that): 8-bit products of 64 to 8192
+// channels 64 rows (5.3, 5.0), 1024 to 4096 48 (6.2, 6.0), 4096 to 1024 80 (7.9, 7.7);
+// blocks of 64 x 8192 64 rows (13.0, 12.6), 256 x 4096 64 (13.0, 12.8), 1024 x 1024 96
+// (15.3, 15.9), 2048 x 2048 32 (19.2, 21.6).
 constexpr long long kFewRows = 16, kFewRowsMost = 256;
-inline bool few_rows(long long rows, long long weight_bytes, long long limit) {
-  return rows <= kFewRows || (rows <= kFewRowsMost && (rows + 15) / 16 * weight_bytes <= limit);
+inline bool few_rows(long long rows, long long weight_bytes, long long limit_mb) {
+  return rows <= kFewRows || (rows <= kFewRowsMost && (rows + 15) / 16 * weight_bytes <= limit_mb << 20);
 }
-inline bool few_rows(const so3lr_int8_linear_args &a) { return few_rows(a.rows, a.n * a.k, 8 << 20); }
+inline bool few_rows(const so3lr_int8_linear_args &a) { return few_rows(a.rows, a.n * a.k, 2 + a.k / 200); }
 inline bool few_rows(const so3lr_feed_forward_args &a) {
-  return !a.gu && few_rows(a.rows, 6 * a.width * a.hidden, 48 << 20);
+  return !a.gu && few_rows(a.rows, 6 * a.width * a.hidden, 12 + a.width / 40);
 }
 void launch_int8_linear_few(const so3lr_int8_linear_args &a, cudaStream_t s);
 void launch_feed_forward_few(const so3lr_feed_forward_args &a, void *h, long long h_stride, void *h_rest,

@@ -26,19 +26,27 @@ __device__ __forceinline__ void dependents_may_start() {
 }
 __device__ __forceinline__ void wait_for_predecessors() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class... P, class... A>
-void launch(void (*kernel)(P...), dim3 grid, dim3 block, std::size_t smem, cudaStream_t stream, A &&...args) {
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+void launch_clusters(void (*kernel)(P...), dim3 grid, dim3 block, unsigned cluster, std::size_t smem,
+                     cudaStream_t stream, A &&...args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = block;
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  config.attrs = &attr;
-  config.numAttrs = 1;
+  config.attrs = attr;
+  config.numAttrs = cluster ? 2 : 1;  // 0: as the kernel declares
   ++launch_counter();
   SO3_CUDA(cudaLaunchKernelEx(&config, kernel, std::forward<A>(args)...));
+}
+template <class... P, class... A>
+void launch(void (*kernel)(P...), dim3 grid, dim3 block, std::size_t smem, cudaStream_t stream, A &&...args) {
+  launch_clusters(kernel, grid, block, 0, smem, stream, std::forward<A>(args)...);
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }

@@ -26,6 +26,24 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ uint32_t cluster_index() {
+  uint32_t i;
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(i));
+  return i;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+// a 32-bit shared variable of another block of the cluster
+template <class T>
+__device__ __forceinline__ T load_of_rank(const T *own, uint32_t rank) {
+  uint32_t at, bits;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(own)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bits) : "r"(at) : "memory");
+  return reinterpret_cast<const T &>(bits);
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
