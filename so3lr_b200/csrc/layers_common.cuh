@@ -140,7 +140,8 @@ __device__ __forceinline__ Chunk<signed char, VEC> to_codes(const float *v, floa
     const uint32_t live = inv != 0.0f ? 0xffffffffu : 0u;
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
-      const uint32_t lo = __byte_perm(q[4 * i], q[4 * i + 1], 0x0040), hi = __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040);
+      const uint32_t lo = __byte_perm(q[4 * i], q[4 * i + 1], 0x0040);
+      const uint32_t hi = __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040);
       reinterpret_cast<uint32_t *>(&out)[i] = __byte_perm(lo, hi, 0x5410) & live;
     }
   } else {

@@ -4,11 +4,18 @@
 // every output written once; the row statistics are reduced between the two.
 //
 // A row belongs to 8, 16 or 32 lanes of a warp (rows of up to 1024 elements: no block
-// barrier) or to one block. A thread holds N chunks of VEC elements: 16-byte chunks
-// where every row starts on a 16-byte boundary, single elements otherwise (odd
-// widths, views). With 2-byte elements the kernels issue more than they load unless
-// a thread has many elements: a row's reduction, its reciprocal root and addresses
-// cost each thread about a hundred instructions, an element about ten.
+// barrier) or to one block. A thread holds N chunks of VEC elements: 16-byte chunks,
+// from the row's start where every row is on a 16-byte boundary, else from the first
+// boundary in the row (odd widths, views: Span), and single elements where the
+// tensors' rows lie differently. With 2-byte elements the kernels issue more than they
+// load unless a thread has many elements: a row's reduction, its reciprocal root and
+// addresses cost each thread about a hundred instructions, an element about ten. Long
+// 8-bit rows and gradients walk over their rows with a ring of copies in flight.
+//
+// Measured, 33.5 M bfloat16 elements, rows of 256 / 4096 / 1003: norm with residual 6.5 /
+// 6.3 / 5.1 TB/s (a copy: 6.5), 8-bit norm without 3.8 / 3.7 / 2.3, gradient 5.4 / 5.2 /
+// 3.8, 8-bit gate 5.8 / 6.1 / 3.9, reading back 5.9 / 6.2 / 4.0. The 8-bit norm issues 21
+// instructions an element at 0.8 of the issue rate, the gradient 29 at 0.6.
 #include "layers_common.cuh"
 #include "model_host.hpp"
 #include "tensor_core.cuh"
@@ -93,8 +100,9 @@ struct RowTeam {
 // through the last one again without storing, so that whole warps stay together.
 template <int LANES>
 __device__ __forceinline__ long long team_row(long long rows, bool &live) {
-  const long long row = LANES ? (long long)blockIdx.x * (kTeamThreads / (LANES ? LANES : 1)) + threadIdx.x / (LANES ? LANES : 1)
-                              : blockIdx.x;
+  constexpr int kLanes = LANES ? LANES : 1;
+  const long long row =
+      LANES ? (long long)blockIdx.x * (kTeamThreads / kLanes) + threadIdx.x / kLanes : (long long)blockIdx.x;
   live = row < rows;
   return live ? row : rows - 1;
 }
@@ -398,8 +406,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
   }
 }
 
-// k_rms_norm to 8 bits for many rows on 16-byte boundaries: 16 elements a thread, rows
-// through a ring, the weight in registers
+// k_rms_norm to 8 bits for many rows of 2-byte elements on 16-byte boundaries: 16
+// elements a thread, rows through a ring, the weight in registers
 template <class T, class W>
 __global__ void __launch_bounds__(512)
     k_rms_norm_int8_ring(const so3lr_rms_norm_args a, int stages, int *err, const float inv_width, const float eps) {
@@ -419,7 +427,8 @@ __global__ void __launch_bounds__(512)
     const uint32_t dst = ring.expect(i, tensors * row_bytes);
     tc::bulk_load(dst, static_cast<const T *>(a.x) + row * a.x_stride, row_bytes, ring.bar(i));
     if (a.residual)
-      tc::bulk_load(dst + row_bytes, static_cast<const T *>(a.residual) + row * a.residual_stride, row_bytes, ring.bar(i));
+      tc::bulk_load(dst + row_bytes, static_cast<const T *>(a.residual) + row * a.residual_stride, row_bytes,
+                    ring.bar(i));
   };
   if (t == 0)
     for (int i = 0; i < min(stages, rows); ++i) fetch(i);
@@ -457,7 +466,7 @@ __global__ void __launch_bounds__(512)
       }
     }
     uint32_t bits = __float_as_uint(top) & 0x7fffffffu;
-    const float sum = team.sum_and_max(sq, bits, slot[k & 1], slot_max[k & 1]);  // every thread has read the stage
+    const float sum = team.sum_and_max(sq, bits, slot[k & 1], slot_max[k & 1]);  // a barrier, as below
     if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
     float inv;
     const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv);
@@ -474,7 +483,7 @@ __global__ void __launch_bounds__(512)
 // k_rms_norm_backward for rows on 16-byte boundaries that need a block: 16 elements a
 // thread, rows through a ring. Bound by instruction issue before it is bound by HBM:
 // the row's reduction costs each warp about a hundred instructions, so fewer and
-// fuller warps are faster (8 elements a thread: 115 us at 16384 x 4096 bfloat16).
+// fuller warps are faster (16384 x 4096 bfloat16: 91 us, 115 with 8 elements a thread).
 template <class T, class W>
 __global__ void __launch_bounds__(512)
     k_rms_norm_backward_ring(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, int stages, int *err,
@@ -879,10 +888,17 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
       t.add(a.s, a.s_stride);
       t.add(a.y, a.y_stride);
       const Path chosen = t.path(a.width, aligned(a.codes, a.codes_stride, 1, V) && aligned(a.weight, 0, 1, 16));
-      const RingPlan r = ring_plan(a.rows, row_threads(a.width, 16), 2048, 2, (a.residual ? 2 : 1) * a.width * sizeof(T));
-      if (chosen == kWide && a.codes && a.width > 1024 && a.width <= 8192 && r.stages >= 2 && a.rows > 2 * r.grid) {
-        norm_int8_ring<T, W>(a, r, s);
-        return;
+      // The ring for many long rows of 2-byte elements (2048: 26 us, 31 without; 904: 34, 39; 768: 40, 33;
+      // with a residual 2048: 42, 47; 768: 52, 66; float32 2048: 18, 15), two rows deep and twice the
+      // blocks that fit, which evens out their ends (2048: 28 us with those that fit).
+      if constexpr (sizeof(T) == 2) {
+        const RingPlan r =
+            ring_plan(a.rows, row_threads(a.width, 16), 2048, 2, (a.residual ? 2 : 1) * a.width * sizeof(T));
+        if (chosen == kWide && a.codes && a.width > (a.residual ? 512 : 896) && a.width <= 8192 && r.stages >= 2 &&
+            a.rows > 2 * r.grid) {
+          norm_int8_ring<T, W>(a, r, s);
+          return;
+        }
       }
       by_path(chosen, [&](auto path) {
         constexpr Path PATH = decltype(path)::value;
@@ -891,7 +907,8 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
         by_hold<PATH>(h, [&](auto lanes, auto per) {
           constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
           constexpr bool SHIFT = PATH == kShifted;
-          const auto fn = a.codes ? &k_rms_norm<T, W, VEC, N, L, true, SHIFT> : &k_rms_norm<T, W, VEC, N, L, false, SHIFT>;
+          const auto fn =
+              a.codes ? &k_rms_norm<T, W, VEC, N, L, true, SHIFT> : &k_rms_norm<T, W, VEC, N, L, false, SHIFT>;
           launch(fn, team_grid(h, a.rows), team_block(h, a.width), 0, s, a,
                  1.0f / float(a.width), float(a.eps));
         });
@@ -920,7 +937,8 @@ void launch_rms_norm_backward(const so3lr_rms_norm_backward_args &a, void *works
             norm_backward<T, W, decltype(path)::value>(a, partial, parts, s);
           });
       }
-      launch(k_column_sum<W>, unsigned((a.width + 31) / 32), dim3(32, 32), 0, s, parts, int(a.width), partial, static_cast<W *>(a.dweight));
+      launch(k_column_sum<W>, unsigned((a.width + 31) / 32), dim3(32, 32), 0, s, parts, int(a.width), partial,
+             static_cast<W *>(a.dweight));
     });
   });
 }

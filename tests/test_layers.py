@@ -120,6 +120,30 @@ def test_rms_norm_special_rows(layers):
             assert bool(torch.isnan(y0[1]).all()) and bool(torch.isfinite(y0[0]).all())
 
 
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("rows, width, with_residual", [(2501, 904, False), (3001, 520, True), (2600, 4096, True),
+                                                        (2400, 8192, False), (5003, 1536, False)])
+def test_rms_norm_int8_of_many_rows(layers, rows, width, with_residual, dtype):
+    """Blocks that walk over rows, with rows of zeros, infinities and NaN, large and small ones among them."""
+    x, w = _rand(1, rows, width, dtype=dtype), 1 + 0.1 * _rand(3, width)
+    r = _rand(2, rows, width, dtype=dtype) if with_residual else None
+    kinds = torch.arange(rows, device="cuda") % 11
+    for t in (x,) if r is None else (x, r):
+        t[kinds == 3] = 0
+        t[kinds == 7] *= 2.0 ** 12 if dtype is torch.float16 else 2.0 ** 50
+        t[kinds == 8] *= 2.0 ** -9
+    x[kinds == 4, width - 1] = float("inf")
+    x[kinds == 5, 0] = float("nan")
+    codes, scales, s = layers.rms_norm_int8(x, w, r, eps=EPS)
+    want_s = x if r is None else (x.float() + r.float()).to(dtype)
+    assert torch.equal(s.nan_to_num(nan=1.0), want_s.nan_to_num(nan=1.0))
+    lost = (kinds == 4) | (kinds == 5)
+    assert bool(torch.isnan(scales[lost]).all()) and bool((codes[lost] == 0).all())
+    assert bool((scales[kinds == 3] == 0).all()) and bool((codes[kinds == 3] == 0).all())
+    ref, _ = _norm_ref(s[~lost].double(), w.double())
+    _check_codes(codes[~lost], scales[~lost], ref)
+
+
 def test_rms_norm_layouts(layers):
     """Views: odd offsets, row strides, broadcast rows, leading dimensions, no rows."""
     big = _rand(1, 20, 300, dtype=torch.bfloat16)
@@ -219,7 +243,8 @@ def _codes(seed, rows, k):
     return torch.randint(-127, 128, (rows, k), generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
 
 
-INT8_SIZES = [(1, 1, 1), (1, 50, 900), (12, 70, 1004), (40, 33, 516), (1, 64, 64), (1, 1531, 4096), (2, 33, 17), (3, 100, 1000), (5, 513, 129), (8, 256, 2048),
+INT8_SIZES = [(1, 1, 1), (1, 50, 900), (12, 70, 1004), (40, 33, 516), (1, 64, 64), (1, 1531, 4096), (2, 33, 17),
+              (3, 100, 1000), (5, 513, 129), (8, 256, 2048), (16, 64, 16384), (4, 40, 32757), (60, 24, 8188),
               (9, 128, 128), (16, 136, 96), (17, 250, 384), (31, 1000, 1000), (33, 64, 8192), (64, 512, 512),
               (100, 128, 4097), (127, 129, 255), (128, 256, 256), (129, 257, 300), (333, 1531, 1000),
               (1000, 72, 2048), (2500, 700, 130), (257, 1, 1), (300, 129, 127),
@@ -275,7 +300,8 @@ def test_int8_linear_layouts(layers):
 
 @pytest.mark.parametrize("dtype", list(U))
 @pytest.mark.parametrize("rows, hidden", [(1, 1), (1, 5632), (3, 7), (4, 256), (9, 512), (5, 513), (2, 8192), (3, 1003),
-                                          (2, 16392), (2, 32768), (1, 32767), (700, 1024)])
+                                          (2, 16392), (2, 32768), (1, 32767), (700, 1024),
+                                          (40, 100), (37, 63), (5, 2051), (9, 2056), (3, 16383), (6, 1030)])
 def test_gate_int8(layers, rows, hidden, dtype):
     gu = _rand(1, rows, 2 * hidden, dtype=dtype, scale=3.0)
     codes, scales = layers.gate_int8(gu)
@@ -350,10 +376,12 @@ def _ffn_ref(x, wg, wu, wd, dy, dtype):
     return out
 
 
-FFN_SIZES = [(1, 1, 1), (1, 70, 150), (3, 1498, 856), (20, 90, 202), (1, 64, 64), (1, 128, 512), (2, 33, 70), (3, 128, 300), (4, 256, 1024), (5, 7, 3), (8, 520, 1368),
-             (9, 256, 256), (17, 100, 333), (33, 128, 512), (64, 64, 4096), (100, 136, 200), (128, 128, 128),
-             (129, 130, 131), (192, 256, 1024), (257, 264, 520), (777, 520, 1368), (3000, 256, 512), (5, 1024, 72), (40, 1024, 200), (260, 64, 96), (400, 100, 90), (300, 72, 4100), (257, 1, 1),
-             (333, 1032, 260), (300, 2048, 131)]
+FFN_SIZES = [(1, 1, 1), (1, 70, 150), (3, 1498, 856), (20, 90, 202), (1, 64, 64), (1, 128, 512), (2, 33, 70),
+             (3, 128, 300), (4, 256, 1024), (5, 7, 3), (8, 520, 1368), (9, 256, 256), (16, 64, 8192), (6, 40, 8190),
+             (50, 24, 6147), (17, 100, 333), (33, 128, 512), (64, 64, 4096), (100, 136, 200), (128, 128, 128),
+             (129, 130, 131), (192, 256, 1024), (257, 264, 520), (777, 520, 1368), (3000, 256, 512), (5, 1024, 72),
+             (40, 1024, 200), (260, 64, 96), (400, 100, 90), (300, 72, 4100), (257, 1, 1), (333, 1032, 260),
+             (300, 2048, 131)]
 
 
 @pytest.mark.parametrize("dtype", HALF)
