@@ -576,3 +576,65 @@ def test_refusals(layers):
                            torch.zeros(1, 131072, dtype=torch.int8, device="cuda"), w[:1])
     with pytest.raises(So3lrError, match="eps"):
         layers.rms_norm(x, w, eps=-1.0)
+
+
+# ------------------------------------------------------------- past 32-bit offsets
+@pytest.mark.parametrize("off_boundary", [0, 1])
+@pytest.mark.parametrize("rows", [9, 300])
+def test_inputs_past_32_bit_offsets(layers, rows, off_boundary):
+    """Rows spread over more than 2^31 elements give what the same rows side by side give."""
+    stride = ((2 ** 31 + 2 ** 20) // (rows - 1) + 7) // 8 * 8 + off_boundary
+    big = torch.empty((rows - 1) * stride + 512, device="cuda", dtype=torch.bfloat16)
+
+    def spread(t):
+        view = big.as_strided(t.shape, (stride, 1))
+        view.copy_(t)
+        return view
+
+    x, w = _rand(1, rows, 256, dtype=torch.bfloat16), 1 + 0.1 * _rand(2, 256)
+    dy = _rand(3, rows, 256, dtype=torch.bfloat16)
+    y, s = layers.rms_norm(spread(x), w, dy)
+    _within(s, (x.float() + dy.float()).to(torch.bfloat16).double(), 0.0, "s")
+    ref, _ = _norm_ref(s.double(), w.double())
+    _within(y, ref, (U[torch.bfloat16] + F32) * ref.abs() + TINY[torch.bfloat16], "y")
+    dx, dw = layers.rms_norm_backward(dy, spread(x), w)
+    dx2, dw2 = layers.rms_norm_backward(dy, x, w)
+    _within(dx, dx2.double(), 2 * U[torch.bfloat16] * (dx2.double().abs() + 1e-3), "dx")
+    _within(dw, dw2.double(), 1e-4 * dw2.double().abs().max(), "dweight")
+    gate, _ = layers.gate_int8(spread(x))
+    assert torch.equal(gate, layers.gate_int8(x)[0])
+    wg, wu, wd = (_rand(i, *n, dtype=torch.bfloat16, scale=0.06) for i, n in ((4, (300, 256)), (5, (300, 256)), (6, (256, 300))))
+    assert torch.equal(layers.feed_forward(spread(x), wg, wu, wd), layers.feed_forward(x, wg, wu, wd))
+    _, saved = layers.feed_forward_train(spread(x), wg, wu, wd)
+    got = layers.feed_forward_backward(dy, saved)
+    _, saved = layers.feed_forward_train(x, wg, wu, wd)
+    assert all(torch.equal(a, b) for a, b in zip(got, layers.feed_forward_backward(dy, saved)))
+    b = _codes(7, 300, 512)
+    sa, sb = torch.ones(rows, device="cuda"), torch.ones(300, device="cuda")
+    a = _codes(8, rows, 512)
+    far = big.view(torch.int8).as_strided((rows, 512), (2 * stride, 1))
+    far.copy_(a)
+    want = layers.int8_linear(a, sa, b, sb, out_dtype=torch.float32)
+    assert torch.equal(layers.int8_linear(far, sa, b, sb, out_dtype=torch.float32), want)
+    assert torch.equal(layers.int8_linear(b, sb, far, sa, out_dtype=torch.float32), want.T)
+
+
+def test_results_past_32_bit_offsets(layers):
+    rows, width = 2 ** 31 // 4096 + 5, 4096
+    codes, scales = _codes(1, rows, width), 0.01 + torch.rand(rows, device="cuda")
+    x = layers.dequantize_int8(codes, scales)
+    for part in (slice(0, 3), slice(rows - 5, rows)):
+        assert torch.equal(x[part], (codes[part].float() * scales[part, None]).bfloat16())
+    w = 1 + 0.1 * _rand(2, width)
+    codes, scales, _ = layers.rms_norm_int8(x, w, eps=EPS)
+    ref, _ = _norm_ref(x[-5:].double(), w.double())
+    _check_codes(codes[-5:], scales[-5:], ref)
+    del codes
+    y, _ = layers.rms_norm(x, w, eps=EPS)
+    _within(y[-5:], ref, (U[torch.bfloat16] + F32) * ref.abs() + TINY[torch.bfloat16], "y")
+    del x, y
+    rows, n, k = 70001, 32768, 32
+    a, b = _codes(3, rows, k), _codes(4, n, k)
+    y = layers.int8_linear(a, torch.ones(rows, device="cuda"), b, torch.ones(n, device="cuda"))
+    want = (a[-40:].double() @ b.double().T).bfloat16()  # sums below 2^24: exact in float32
+    assert torch.equal(y[-40:], want)
