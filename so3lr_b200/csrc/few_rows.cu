@@ -49,10 +49,11 @@ __device__ __forceinline__ void mma_step(Acc (&c)[4], const uint4 &x0, const uin
 template <class E, int ALIGN, bool WEIGHT>
 __device__ __forceinline__ uint4 load_inside(const E *p, int k) {
   uint4 v;
-  if (ALIGN == 16 && WEIGHT) {  // read once: not kept in L1
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  if (ALIGN == 16 && WEIGHT) {  // read once: not kept in L1. The kernel before may still be writing them: no .nc
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p + k));
+                 : "l"(p + k)
+                 : "memory");
   } else if (ALIGN == 16) {
     v = *reinterpret_cast<const uint4 *>(p + k);
   } else if (ALIGN == 4) {
