@@ -568,9 +568,10 @@ __global__ void __launch_bounds__(512)
 }
 
 // column sums of `partial` (nparts x width) in a fixed order: 32 columns per
-// block, part k summed by thread row k % 32, then the 32 thread rows in order
+// block, part k summed by thread row k % 32, then the 32 thread rows in order. No
+// __restrict__: the kernel that writes `partial` may still run when this one starts.
 template <class W>
-__global__ void k_column_sum(int nparts, int width, const float *__restrict__ partial, W *__restrict__ out) {
+__global__ void k_column_sum(int nparts, int width, const float *partial, W *out) {
   __shared__ float part[32][33];
   dependents_may_start();
   wait_for_predecessors();

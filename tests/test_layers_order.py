@@ -43,3 +43,17 @@ def test_weights_of_few_rows_made_by_the_call_before(layers):
     for _ in range(20):
         for (y, z), (y1, z1) in zip([chain(codes) for codes in sets], apart):
             assert torch.equal(y, y1) and torch.equal(z, z1)
+
+
+def test_weight_gradient_follows_its_rows(layers):
+    """The norm's weight gradient is summed from what the kernel just before it wrote, in
+    scratch that the calls before used too: gradients of scaled rows are scaled."""
+    for rows, width in ((700, 96), (600, 1003), (3000, 2048)):
+        s, dy = (torch.randn(rows, width, device="cuda") for _ in range(2))
+        w = torch.ones(width, device="cuda")
+        one = layers.rms_norm_backward(dy, s, w)[1]
+        torch.cuda.synchronize()
+        scaled = [dy * 2.0 ** i for i in range(8)]
+        got = [layers.rms_norm_backward(d, s, w)[1] for _ in range(10) for d in scaled]
+        for i, dw in enumerate(got):
+            assert torch.equal(dw, one * 2.0 ** (i % 8))

@@ -13,7 +13,7 @@ def _code(name):
     return re.sub(r"//[^\n]*|/\*.*?\*/", "", text, flags=re.S)
 
 
-@pytest.mark.parametrize("name", ["few_rows.cu", "dense.cu", "tensor_core.cuh", "layers_common.cuh"])
+@pytest.mark.parametrize("name", ["few_rows.cu", "rows.cu", "dense.cu", "tensor_core.cuh", "layers_common.cuh"])
 def test_no_read_only_loads(name):
     """These kernels start while the kernel before them may still write what they read
     (programmatic dependent launch), so nothing of theirs is read-only for their
