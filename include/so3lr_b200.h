@@ -351,12 +351,23 @@ void so3lr_destroy(so3lr_handle *h);
  *     function returns for the same arguments (-1: invalid sizes), 256-byte
  *     aligned; its contents mean nothing between calls. Calls that may overlap
  *     need workspaces of their own.
+ *   - Waits inside the kernels are bounded. A kernel whose wait gives up (a GPU that
+ *     stands still for seconds under it) leaves results that are not valid, and
+ *     every later call that would queue work on that device is refused until
+ *     so3lr_layers_status has reported it. A caller that must know of the last
+ *     calls too asks so3lr_layers_status after synchronising with them.
  *   - Elements are SO3LR_FLOAT32, SO3LR_BFLOAT16 or SO3LR_FLOAT16. Sums, norms and
  *     activations are computed in float32 (8-bit products: int32) in a fixed
  *     order: repeated calls return the same bits. */
 #define SO3LR_FLOAT32 0
 #define SO3LR_BFLOAT16 1
 #define SO3LR_FLOAT16 2
+
+/* 0, or 1 with a message when a kernel of these layers on the calling thread's
+ * current device has given up waiting since the last call of this function (the
+ * results of its call and of those after it are not valid). Reports each such event
+ * once; calls on that device are accepted again. Does not synchronise. */
+int so3lr_layers_status(char *err, size_t errlen);
 
 /* RMS norm with the residual's addition, width <= 16384:
  *   s = x + residual, rounded to the element type (x itself without a residual)

@@ -386,6 +386,14 @@ PyObject *feed_forward_backward(Args o) {
   return tuple(wrap(dx), wrap(dwg), wrap(dwu), wrap(dwd));
 }
 
+// status(device index) -> None
+PyObject *status(Args o) {
+  const c10::cuda::CUDAGuard guard(c10::Device(c10::kCUDA, c10::DeviceIndex(PyLong_AsLong(o[0]))));
+  char err[1024] = "";
+  check(so3lr_layers_status(err, sizeof err), err);
+  return none();
+}
+
 // No C++ exception leaves the module: refusals become ValueError, failures of the
 // library So3lrError, torch's own errors RuntimeError.
 template <PyObject *(*F)(Args), int N>
@@ -417,7 +425,7 @@ PyObject *method(PyObject *, PyObject *const *args, Py_ssize_t n) {
   { #f, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&method<f, n>)), METH_FASTCALL, nullptr }
 PyMethodDef g_methods[] = {METHOD(rms_norm, 5),        METHOD(rms_norm_backward, 5), METHOD(int8_linear, 6),
                            METHOD(gate_int8, 1),       METHOD(dequantize_int8, 3),   METHOD(feed_forward, 5),
-                           METHOD(feed_forward_backward, 7), {nullptr, nullptr, 0, nullptr}};
+                           METHOD(feed_forward_backward, 7), METHOD(status, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_layers", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

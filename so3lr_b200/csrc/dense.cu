@@ -19,7 +19,8 @@
 // Tiles beyond the last whole wave (one tile a CTA pair) of a long contraction are
 // split along K, so that they fill the pairs too: each part writes raw 32-bit sums,
 // k_join adds them in order.
-#include <mutex>
+#include <cstring>
+#include <string>
 
 #include "layers_common.cuh"
 #include "model_host.hpp"
@@ -616,9 +617,7 @@ struct Operand {
 class Dense {
  public:
   Dense(void *workspace, int elem, cudaStream_t stream, bool dry)
-      : scratch_(workspace), elem_(elem), stream_(stream), dry_(dry) {
-    if (!dry) check_gave_up();
-  }
+      : scratch_(workspace), elem_(elem), stream_(stream), dry_(dry) {}
   Scratch &scratch() { return scratch_; }
   bool dry() const { return dry_; }
 
@@ -920,27 +919,34 @@ long long dry_run(const A &a, int elem, F &&f) {
 
 }  // namespace
 
-// Where a kernel whose wait gave up says so (page-locked host memory that every
-// device writes); looked at before the next call queues work.
+// Where a kernel whose wait gave up says so: a word for each device in page-locked host
+// memory that all of them can write.
 int *gave_up_flag() {
-  static int *flag = [] {
+  constexpr int kMaxDevices = 64;
+  static int *flags = [] {
     // allowed while another stream of the thread is being captured: it is no stream operation
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     SO3_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
     void *p = nullptr;
-    const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    const cudaError_t e = cudaHostAlloc(&p, kMaxDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
     cudaThreadExchangeStreamCaptureMode(&mode);
     SO3_CUDA(e);
-    *static_cast<volatile int *>(p) = 0;
+    std::memset(p, 0, kMaxDevices * sizeof(int));
     return static_cast<int *>(p);
   }();
-  return flag;
+  int device = 0;
+  SO3_CUDA(cudaGetDevice(&device));
+  if (device >= kMaxDevices) throw Error("feed-forward layers: more than 64 devices");
+  return flags + device;
 }
 void check_gave_up() {
   const int where = *static_cast<volatile int *>(gave_up_flag());
-  if (where)
-    throw Error("feed-forward layers: a kernel of an earlier call gave up waiting (stage " + std::to_string(where) +
-                "); its results are not valid");
+  if (where) throw Error(gave_up_message(where) + "; so3lr_layers_status clears this");
+}
+int take_gave_up() { return __atomic_exchange_n(gave_up_flag(), 0, __ATOMIC_SEQ_CST); }
+std::string gave_up_message(int where) {
+  return "feed-forward layers: a kernel of an earlier call on this device gave up waiting (stage " +
+         std::to_string(where) + "); the results of that call and of those after it are not valid";
 }
 
 long long int8_linear_bytes(const so3lr_int8_linear_args &a) {

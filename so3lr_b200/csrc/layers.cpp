@@ -212,10 +212,18 @@ void check(const so3lr_feed_forward_backward_args *a) {
 
 extern "C" {
 
+int so3lr_layers_status(char *err, size_t errlen) {
+  return guarded(err, errlen, [&] {
+    if (const int where = so3lr_b200::take_gave_up()) throw Error(so3lr_b200::gave_up_message(where));
+  });
+}
+
 int so3lr_rms_norm(const so3lr_rms_norm_args *args, void *stream, char *err, size_t errlen) {
   return guarded(err, errlen, [&] {
     check(args);
-    if (args->rows > 0) so3lr_b200::launch_rms_norm(*args, static_cast<cudaStream_t>(stream));
+    if (args->rows == 0) return;
+    so3lr_b200::check_gave_up();
+    so3lr_b200::launch_rms_norm(*args, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -230,6 +238,7 @@ int so3lr_rms_norm_backward(const so3lr_rms_norm_backward_args *args, void *work
   return guarded(err, errlen, [&] {
     check(args);
     workspace_is("so3lr_rms_norm_backward", workspace, workspace_bytes, so3lr_b200::rms_norm_backward_bytes(*args));
+    so3lr_b200::check_gave_up();
     so3lr_b200::launch_rms_norm_backward(*args, workspace, static_cast<cudaStream_t>(stream));
   });
 }
@@ -245,21 +254,27 @@ int so3lr_int8_linear(const so3lr_int8_linear_args *args, void *workspace, long 
   return guarded(err, errlen, [&] {
     check(args);
     workspace_is("so3lr_int8_linear", workspace, workspace_bytes, so3lr_b200::int8_linear_bytes(*args));
-    if (args->rows > 0) so3lr_b200::launch_int8_linear(*args, workspace, static_cast<cudaStream_t>(stream));
+    if (args->rows == 0) return;
+    so3lr_b200::check_gave_up();
+    so3lr_b200::launch_int8_linear(*args, workspace, static_cast<cudaStream_t>(stream));
   });
 }
 
 int so3lr_gate_int8(const so3lr_gate_int8_args *args, void *stream, char *err, size_t errlen) {
   return guarded(err, errlen, [&] {
     check(args);
-    if (args->rows > 0) so3lr_b200::launch_gate_int8(*args, static_cast<cudaStream_t>(stream));
+    if (args->rows == 0) return;
+    so3lr_b200::check_gave_up();
+    so3lr_b200::launch_gate_int8(*args, static_cast<cudaStream_t>(stream));
   });
 }
 
 int so3lr_dequantize_int8(const so3lr_dequantize_int8_args *args, void *stream, char *err, size_t errlen) {
   return guarded(err, errlen, [&] {
     check(args);
-    if (args->rows > 0) so3lr_b200::launch_dequantize_int8(*args, static_cast<cudaStream_t>(stream));
+    if (args->rows == 0) return;
+    so3lr_b200::check_gave_up();
+    so3lr_b200::launch_dequantize_int8(*args, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -280,7 +295,9 @@ int so3lr_feed_forward(const so3lr_feed_forward_args *args, void *workspace, lon
   return guarded(err, errlen, [&] {
     check(args);
     workspace_is("so3lr_feed_forward", workspace, workspace_bytes, so3lr_b200::feed_forward_bytes(*args));
-    if (args->rows > 0) so3lr_b200::launch_feed_forward(*args, workspace, static_cast<cudaStream_t>(stream));
+    if (args->rows == 0) return;
+    so3lr_b200::check_gave_up();
+    so3lr_b200::launch_feed_forward(*args, workspace, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -296,6 +313,7 @@ int so3lr_feed_forward_backward(const so3lr_feed_forward_backward_args *args, vo
     check(args);
     workspace_is("so3lr_feed_forward_backward", workspace, workspace_bytes,
                  so3lr_b200::feed_forward_backward_bytes(*args));
+    so3lr_b200::check_gave_up();
     so3lr_b200::launch_feed_forward_backward(*args, workspace, static_cast<cudaStream_t>(stream));
   });
 }

@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cstddef>
+#include <string>
 
 #include "../../include/so3lr_b200.h"
 #include "common.cuh"
@@ -18,9 +19,12 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s);
 void launch_dequantize_int8(const so3lr_dequantize_int8_args &a, cudaStream_t s);
 
 // dense.cu
-// Where a kernel whose bounded wait gave up says so, and the refusal of further calls after that.
+// Where a kernel whose bounded wait gave up on the current device says so (which wait, 0: none), the
+// refusal of further calls after that, and reading and clearing it.
 int *gave_up_flag();
 void check_gave_up();
+int take_gave_up();
+std::string gave_up_message(int where);
 long long int8_linear_bytes(const so3lr_int8_linear_args &a);
 void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s);
 long long feed_forward_keep(const so3lr_feed_forward_args &a);

@@ -862,14 +862,12 @@ void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int gr
 }
 template <class T, class W>
 void norm_int8_ring(const so3lr_rms_norm_args &a, const RingPlan &r, cudaStream_t s) {
-  check_gave_up();
   allow_dynamic_smem(reinterpret_cast<const void *>(&k_rms_norm_int8_ring<T, W>), 227 * 1024 - 1024);
   launch(k_rms_norm_int8_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, r.stages, gave_up_flag(),
          1.0f / float(a.width), float(a.eps));
 }
 template <class T, class W>
 void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, const RingPlan &r, cudaStream_t s) {
-  check_gave_up();
   allow_dynamic_smem(reinterpret_cast<const void *>(&k_rms_norm_backward_ring<T, W>), 227 * 1024 - 1024);
   launch(k_rms_norm_backward_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, partial, r.stages,
          gave_up_flag(), 1.0f / float(a.width), float(a.eps));

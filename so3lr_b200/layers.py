@@ -19,7 +19,8 @@ in 8 bits.
 The calls are the entry points of include/so3lr_b200.h ("Row-wise feed-forward
 layers") through the compiled module ``so3lr_b200._layers``
 (binding/layers_binding.cpp): they queue kernels on the current torch stream of the
-tensors' GPU and return; outputs and scratch come from torch's allocator. Rows are
+tensors' GPU and return; outputs and scratch come from torch's allocator. A kernel
+whose wait gives up is reported by the next call on that GPU and by ``check_status``. Rows are
 all leading dimensions; the last dimension must be contiguous, rows may have any
 stride. A refused argument raises ValueError, a failure of the library So3lrError.
 There is no CPU path: a tensor that is not on a GPU is refused.
@@ -39,7 +40,16 @@ except (ImportError, So3lrError) as e:
 
 __all__ = ["rms_norm", "rms_norm_int8", "rms_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
            "quantize_weight", "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock",
-           "Int8FeedForwardBlock"]
+           "Int8FeedForwardBlock", "check_status"]
+
+
+def check_status(device=None) -> None:
+    """Raises So3lrError if a kernel of an earlier call on `device` (the current one by
+    default) gave up waiting: the results of that call and of those after it are not
+    valid. Calls on the device are refused from then on until this has said so, once.
+    It does not synchronise: ask after doing so to know about the last calls too."""
+    index = None if device is None else torch.device(device).index
+    _layers.status(torch.cuda.current_device() if index is None else index)
 
 
 def _dense_rows(t):

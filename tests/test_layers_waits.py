@@ -1,0 +1,66 @@
+"""Bounded waits of the row-wise feed-forward kernels: what a call says when a wait of
+an earlier one has given up."""
+import ctypes as C
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def layers():
+    from so3lr_b200 import layers
+    return layers
+
+
+def _calls(layers):
+    """One call of each kind that queues work: dense and few-row products, row kernels with and without a ring."""
+    half = lambda *n: torch.randn(*n, device="cuda").bfloat16()  # noqa: E731
+    ones = lambda n: torch.ones(n, device="cuda")  # noqa: E731
+    x, w, d = half(300, 64), half(96, 64), half(64, 96)
+    big = half(4000, 1024)
+    _, saved = layers.feed_forward_train(x, w, w, d)
+    c = torch.ones(300, 64, dtype=torch.int8, device="cuda")
+    return {
+        "feed_forward": lambda: layers.feed_forward(x, w, w, d),
+        "feed_forward, few rows": lambda: layers.feed_forward(x[:2], w, w, d),
+        "feed_forward_backward": lambda: layers.feed_forward_backward(x, saved),
+        "int8_linear": lambda: layers.int8_linear(c, ones(300), c, ones(300)),
+        "int8_linear, few rows": lambda: layers.int8_linear(c[:2], ones(2), c, ones(300)),
+        "rms_norm": lambda: layers.rms_norm(x, ones(64)),
+        "rms_norm_backward": lambda: layers.rms_norm_backward(x, x, ones(64)),
+        "rms_norm_backward, ring": lambda: layers.rms_norm_backward(big, big, ones(1024)),
+        "rms_norm_int8": lambda: layers.rms_norm_int8(x, ones(64)),
+        "rms_norm_int8, ring": lambda: layers.rms_norm_int8(big, ones(1024)),
+        "gate_int8": lambda: layers.gate_int8(x),
+        "dequantize_int8": lambda: layers.dequantize_int8(c, ones(300)),
+    }
+
+
+def test_a_wait_that_gave_up_is_reported_once(layers):
+    """The word that a kernel writes, written here by the host: every kind of call is refused until
+    check_status has said so, and accepted afterwards."""
+    from so3lr_b200 import So3lrError, load_library
+    word = getattr(load_library(), "_ZN10so3lr_b20012gave_up_flagEv")
+    word.restype = C.POINTER(C.c_int)
+    calls = _calls(layers)
+    layers.check_status()
+    for name, call in calls.items():
+        call()
+        torch.cuda.synchronize()
+        word()[0] = 3
+        for _ in range(2):
+            with pytest.raises(So3lrError, match="gave up waiting .stage 3.*so3lr_layers_status"):
+                call()
+        with pytest.raises(So3lrError, match="gave up waiting .stage 3"):
+            layers.check_status("cuda:0")
+        layers.check_status()
+        call()
+    torch.cuda.synchronize()
+    layers.check_status(torch.device("cuda"))
+    # what queues nothing is not refused, and takes nothing from the report
+    word()[0] = 5
+    assert layers.rms_norm(torch.zeros(0, 64, device="cuda"), torch.ones(64, device="cuda"))[0].shape == (0, 64)
+    with pytest.raises(So3lrError, match="stage 5"):
+        layers.check_status()
