@@ -368,6 +368,10 @@ void so3lr_destroy(so3lr_handle *h);
  * results of its call and of those after it are not valid). Reports each such event
  * once; calls on that device are accepted again. Does not synchronise. */
 int so3lr_layers_status(char *err, size_t errlen);
+/* About how many clock cycles of an SM a wait inside the kernels that are queued from
+ * now on may take (process-wide); 0 or less: the default of 4e9, about 2 s. A GPU that
+ * is shared in time slices of seconds, or stopped in a debugger, needs more. */
+void so3lr_layers_wait_limit(long long cycles);
 
 /* RMS norm with the residual's addition, width <= 16384:
  *   s = x + residual, rounded to the element type (x itself without a residual)

@@ -394,6 +394,12 @@ PyObject *status(Args o) {
   return none();
 }
 
+// set_wait_limit(cycles) -> None
+PyObject *set_wait_limit(Args o) {
+  so3lr_layers_wait_limit(PyLong_AsLongLong(o[0]));
+  return none();
+}
+
 // No C++ exception leaves the module: refusals become ValueError, failures of the
 // library So3lrError, torch's own errors RuntimeError.
 template <PyObject *(*F)(Args), int N>
@@ -425,7 +431,7 @@ PyObject *method(PyObject *, PyObject *const *args, Py_ssize_t n) {
   { #f, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&method<f, n>)), METH_FASTCALL, nullptr }
 PyMethodDef g_methods[] = {METHOD(rms_norm, 5),        METHOD(rms_norm_backward, 5), METHOD(int8_linear, 6),
                            METHOD(gate_int8, 1),       METHOD(dequantize_int8, 3),   METHOD(feed_forward, 5),
-                           METHOD(feed_forward_backward, 7), METHOD(status, 1), {nullptr, nullptr, 0, nullptr}};
+                           METHOD(feed_forward_backward, 7), METHOD(status, 1), METHOD(set_wait_limit, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_layers", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

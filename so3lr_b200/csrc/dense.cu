@@ -19,6 +19,7 @@
 // Tiles beyond the last whole wave (one tile a CTA pair) of a long contraction are
 // split along K, so that they fill the pairs too: each part writes raw 32-bit sums,
 // k_join adds them in order.
+#include <atomic>
 #include <cstring>
 #include <string>
 
@@ -944,6 +945,9 @@ void check_gave_up() {
   if (where) throw Error(gave_up_message(where) + "; so3lr_layers_status clears this");
 }
 int take_gave_up() { return __atomic_exchange_n(gave_up_flag(), 0, __ATOMIC_SEQ_CST); }
+static std::atomic<long long> g_wait_cycles{tc::kWaitCycles};
+WaitLimit wait_limit() { return WaitLimit{gave_up_flag(), g_wait_cycles.load(std::memory_order_relaxed)}; }
+void set_wait_limit(long long cycles) { g_wait_cycles = cycles > 0 ? cycles : tc::kWaitCycles; }
 std::string gave_up_message(int where) {
   return "feed-forward layers: a kernel of an earlier call on this device gave up waiting (stage " +
          std::to_string(where) + "); the results of that call and of those after it are not valid";

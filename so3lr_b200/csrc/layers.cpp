@@ -218,6 +218,8 @@ int so3lr_layers_status(char *err, size_t errlen) {
   });
 }
 
+void so3lr_layers_wait_limit(long long cycles) { so3lr_b200::set_wait_limit(cycles); }
+
 int so3lr_rms_norm(const so3lr_rms_norm_args *args, void *stream, char *err, size_t errlen) {
   return guarded(err, errlen, [&] {
     check(args);

@@ -25,6 +25,13 @@ int *gave_up_flag();
 void check_gave_up();
 int take_gave_up();
 std::string gave_up_message(int where);
+// How long a kernel's wait may take, and where it says that it gave up; the limit of kernels queued from now on.
+struct WaitLimit {
+  int *err;
+  long long cycles;
+};
+WaitLimit wait_limit();
+void set_wait_limit(long long cycles);
 long long int8_linear_bytes(const so3lr_int8_linear_args &a);
 void launch_int8_linear(const so3lr_int8_linear_args &a, void *workspace, cudaStream_t s);
 long long feed_forward_keep(const so3lr_feed_forward_args &a);

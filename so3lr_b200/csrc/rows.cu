@@ -147,16 +147,18 @@ __device__ __forceinline__ void store_apart(T *p, const Chunk<T, VEC> &v) {
 // A ring of rows in shared memory, filled by bulk copies: what is in flight costs no
 // registers, so a block that walks over rows keeps the memory system busy while it
 // reduces and writes the current one. One block barrier after the last read of a
-// stage, thread 0 may refill it.
+// stage, thread 0 may refill it. A wait that gives up marks its row; the block leaves
+// its loop after that row's barrier, where every thread sees the mark, and not before
+// the copies in flight have landed.
 struct RowRing {
   uint32_t bars, buffer, stage_bytes;
   int stages;
   unsigned char *mem;
-  int *err;
-  volatile int *abort_flag;
+  WaitLimit limit;
+  volatile int *abort_flag;  // 1 + the row of this block at which a wait gave up
 
-  __device__ RowRing(unsigned char *smem, uint32_t bytes, int nstages, int *error)
-      : stage_bytes(bytes), stages(nstages), mem(smem + 128), err(error) {
+  __device__ RowRing(unsigned char *smem, uint32_t bytes, int nstages, const WaitLimit &l)
+      : stage_bytes(bytes), stages(nstages), mem(smem + 128), limit(l) {
     bars = tc::smem_u32(smem);
     buffer = bars + 128;
     abort_flag = reinterpret_cast<volatile int *>(smem + 120);
@@ -168,8 +170,21 @@ struct RowRing {
     __syncthreads();
   }
   __device__ const unsigned char *stage(int i) const { return mem + (i % stages) * stage_bytes; }
-  // waits for the i-th row of this block; after a wait that gave up (reported in *err) nothing waits again
-  __device__ void wait(int i) const { tc::mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, abort_flag, err, 7); }
+  // waits for the i-th row of this block
+  __device__ void wait(int i) const {
+    tc::mbar_wait(bar(i), (i / stages) & 1, abort_flag, limit.err, 7, limit.cycles, i + 1);
+  }
+  // after the barrier of the i-th row: whether a thread gave up waiting for it (a later row's mark does not count,
+  // so all threads agree)
+  __device__ bool gave_up(int i) const {
+    const int at = *abort_flag;
+    return at != 0 && at <= i + 1;
+  }
+  // thread 0, at the loop's end: the copies of rows i and on, of `rows`, have landed
+  __device__ void settle(int i, int rows) const {
+    const long long t0 = clock64();
+    for (const int end = min(i + stages, rows); i < end; ++i) tc::mbar_settle(bar(i), (i / stages) & 1, t0);
+  }
   // thread 0: the copies of the i-th row
   __device__ uint32_t expect(int i, uint32_t bytes) const {
     tc::mbar_expect_tx(bars + 8 * (i % stages), bytes);
@@ -410,7 +425,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : VEC *N == 8 && LANES ?
 // elements a thread, rows through a ring, the weight in registers
 template <class T, class W>
 __global__ void __launch_bounds__(512)
-    k_rms_norm_int8_ring(const so3lr_rms_norm_args a, int stages, int *err, const float inv_width, const float eps) {
+    k_rms_norm_int8_ring(const so3lr_rms_norm_args a, int stages, const WaitLimit limit, const float inv_width,
+                         const float eps) {
   constexpr int VEC = 16 / sizeof(T), N = 16 / VEC;
   __shared__ float slot[2][32];
   __shared__ uint32_t slot_max[2][32];
@@ -418,7 +434,7 @@ __global__ void __launch_bounds__(512)
   const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
   const uint32_t row_bytes = width * sizeof(T), tensors = a.residual ? 2 : 1;
   dependents_may_start();
-  const RowRing ring(smem, tensors * row_bytes, stages, err);
+  const RowRing ring(smem, tensors * row_bytes, stages, limit);
   wait_for_predecessors();
   const RowTeam<0> team;
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
@@ -438,7 +454,8 @@ __global__ void __launch_bounds__(512)
     const int c = (j * size + t) * VEC;
     if (c < width) cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
   }
-  for (int k = 0; k < rows; ++k) {
+  int k = 0;
+  for (; k < rows; ++k) {
     ring.wait(k);
     const T *x = reinterpret_cast<const T *>(ring.stage(k));
     const long long row = blockIdx.x + (long long)k * gridDim.x;
@@ -467,7 +484,8 @@ __global__ void __launch_bounds__(512)
     }
     uint32_t bits = __float_as_uint(top) & 0x7fffffffu;
     const float sum = team.sum_and_max(sq, bits, slot[k & 1], slot_max[k & 1]);  // a barrier, as below
-    if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
+    if (ring.gave_up(k)) break;
+    if (t == 0 && k + stages < rows) fetch(k + stages);
     float inv;
     const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv);
     if (t == 0) a.scales[row] = scale;
@@ -478,6 +496,7 @@ __global__ void __launch_bounds__(512)
         store_chunk<signed char, VEC>(a.codes + row * a.codes_stride + c, to_codes<VEC>(v + j * VEC, inv));
     }
   }
+  if (t == 0) ring.settle(k, rows);
 }
 
 // k_rms_norm_backward for rows on 16-byte boundaries that need a block: 16 elements a
@@ -486,15 +505,15 @@ __global__ void __launch_bounds__(512)
 // fuller warps are faster (16384 x 4096 bfloat16: 91 us, 115 with 8 elements a thread).
 template <class T, class W>
 __global__ void __launch_bounds__(512)
-    k_rms_norm_backward_ring(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, int stages, int *err,
-                             const float inv_width, const float eps) {
+    k_rms_norm_backward_ring(const so3lr_rms_norm_backward_args a, float *__restrict__ partial, int stages,
+                             const WaitLimit limit, const float inv_width, const float eps) {
   constexpr int VEC = 16 / sizeof(T), N = 16 / VEC;
   __shared__ float2 slot[2][32];
   extern __shared__ __align__(128) unsigned char smem[];
   const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
   const uint32_t row_bytes = width * sizeof(T), tensors = a.ds ? 3 : 2;
   dependents_may_start();
-  const RowRing ring(smem, tensors * row_bytes, stages, err);
+  const RowRing ring(smem, tensors * row_bytes, stages, limit);
   wait_for_predecessors();
   const RowTeam<0> team;
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
@@ -517,7 +536,8 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j * VEC + i] = 0.0f;
   }
-  for (int k = 0; k < rows; ++k) {
+  int k = 0;
+  for (; k < rows; ++k) {
     ring.wait(k);
     const T *s = reinterpret_cast<const T *>(ring.stage(k));
     Chunk<T, VEC> cs[N], cd[N], ce[N];
@@ -538,7 +558,8 @@ __global__ void __launch_bounds__(512)
       }
     }
     const float2 total = team.sum2(sq, dot, slot[k & 1]);  // a barrier: every thread has read the stage
-    if (t == 0 && k + stages < rows && !*ring.abort_flag) fetch(k + stages);
+    if (ring.gave_up(k)) break;
+    if (t == 0 && k + stages < rows) fetch(k + stages);
     const float rstd = rsqrtf(fmaf(total.x, inv_width, eps));
     const float back = -(total.y * rstd * inv_width) * rstd * rstd;  // - mean(a xh) rstd^2, times s
     T *dx = static_cast<T *>(a.dx) + (blockIdx.x + (long long)k * gridDim.x) * a.dx_stride;
@@ -558,6 +579,7 @@ __global__ void __launch_bounds__(512)
       }
     }
   }
+  if (t == 0) ring.settle(k, rows);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = (j * size + t) * VEC;
@@ -863,14 +885,14 @@ void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int gr
 template <class T, class W>
 void norm_int8_ring(const so3lr_rms_norm_args &a, const RingPlan &r, cudaStream_t s) {
   allow_dynamic_smem(reinterpret_cast<const void *>(&k_rms_norm_int8_ring<T, W>), 227 * 1024 - 1024);
-  launch(k_rms_norm_int8_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, r.stages, gave_up_flag(),
+  launch(k_rms_norm_int8_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, r.stages, wait_limit(),
          1.0f / float(a.width), float(a.eps));
 }
 template <class T, class W>
 void norm_backward_ring(const so3lr_rms_norm_backward_args &a, float *partial, const RingPlan &r, cudaStream_t s) {
   allow_dynamic_smem(reinterpret_cast<const void *>(&k_rms_norm_backward_ring<T, W>), 227 * 1024 - 1024);
   launch(k_rms_norm_backward_ring<T, W>, r.grid, row_threads(a.width, 16), r.smem, s, a, partial, r.stages,
-         gave_up_flag(), 1.0f / float(a.width), float(a.eps));
+         wait_limit(), 1.0f / float(a.width), float(a.eps));
 }
 
 }  // namespace

@@ -17,6 +17,7 @@ namespace so3lr_b200 {
 namespace tc {
 
 constexpr long long kWaitCycles = 4000000000LL;  // about 2 s at 1.9 GHz
+constexpr long long kPolled = 20000;             // limits below it: a blocking try alone takes 8,000 cycles
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -77,21 +78,39 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// Waits for the phase of the given parity, at most kWaitCycles; false (and *err =
-// where) when it gives up or another thread of the CTA already gave up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err,
-                                          int where) {
-  if (mbar_try(bar, parity)) return true;
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {  // without blocking
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Waits for the phase of the given parity, about `limit` cycles at most; false (with
+// *abort_flag = mark and *err = where) when it gives up or another thread of the CTA
+// already gave up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err, int where,
+                                          long long limit = kWaitCycles, int mark = 1) {
+  const bool polled = limit < kPolled;
+  if (polled ? mbar_test(bar, parity) : mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!mbar_try(bar, parity)) {
+  while (!(polled ? mbar_test(bar, parity) : mbar_try(bar, parity))) {
     if (*abort_flag) return false;
-    if (clock64() - t0 > kWaitCycles) {
-      *abort_flag = 1;
+    if (clock64() - t0 > limit) {
+      *abort_flag = mark;
       *reinterpret_cast<volatile int *>(err) = where;
       return false;
     }
   }
   return true;
+}
+// After a wait that gave up: waits for what is still under way into this block's
+// memory, whoever gave up, until kWaitCycles after t0.
+__device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity, long long t0) {
+  while (!mbar_try(bar, parity) && clock64() - t0 < kWaitCycles) {
+  }
 }
 
 // `bytes` (a multiple of 16) from 16-byte aligned global memory, completed on `bar`

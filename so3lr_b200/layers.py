@@ -40,7 +40,7 @@ except (ImportError, So3lrError) as e:
 
 __all__ = ["rms_norm", "rms_norm_int8", "rms_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
            "quantize_weight", "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock",
-           "Int8FeedForwardBlock", "check_status"]
+           "Int8FeedForwardBlock", "check_status", "set_wait_limit"]
 
 
 def check_status(device=None) -> None:
@@ -50,6 +50,12 @@ def check_status(device=None) -> None:
     It does not synchronise: ask after doing so to know about the last calls too."""
     index = None if device is None else torch.device(device).index
     _layers.status(torch.cuda.current_device() if index is None else index)
+
+
+def set_wait_limit(cycles: int = 0) -> None:
+    """About how many clock cycles of an SM a wait inside the kernels that are queued
+    from now on may take; 0: the default of 4e9, about 2 s."""
+    _layers.set_wait_limit(cycles)
 
 
 def _dense_rows(t):

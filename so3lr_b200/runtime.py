@@ -30,7 +30,7 @@ EXPORTED = (
     "so3lr_destroy",
     "so3lr_nccl_unique_id", "so3lr_comm_init", "so3lr_owned_atoms", "so3lr_partition",
     # row-wise feed-forward layers (bound in layers.py)
-    "so3lr_layers_status", "so3lr_rms_norm", "so3lr_rms_norm_backward_workspace", "so3lr_rms_norm_backward", "so3lr_int8_linear_workspace",
+    "so3lr_layers_status", "so3lr_layers_wait_limit", "so3lr_rms_norm", "so3lr_rms_norm_backward_workspace", "so3lr_rms_norm_backward", "so3lr_int8_linear_workspace",
     "so3lr_int8_linear", "so3lr_gate_int8", "so3lr_dequantize_int8", "so3lr_feed_forward_workspace",
     "so3lr_feed_forward_keep", "so3lr_feed_forward", "so3lr_feed_forward_backward_workspace", "so3lr_feed_forward_backward",
 )

@@ -19,7 +19,7 @@ def _calls(layers):
     half = lambda *n: torch.randn(*n, device="cuda").bfloat16()  # noqa: E731
     ones = lambda n: torch.ones(n, device="cuda")  # noqa: E731
     x, w, d = half(300, 64), half(96, 64), half(64, 96)
-    big = half(4000, 1024)
+    big = half(6000, 1024)
     _, saved = layers.feed_forward_train(x, w, w, d)
     c = torch.ones(300, 64, dtype=torch.int8, device="cuda")
     return {
@@ -64,3 +64,39 @@ def test_a_wait_that_gave_up_is_reported_once(layers):
     assert layers.rms_norm(torch.zeros(0, 64, device="cuda"), torch.ones(64, device="cuda"))[0].shape == (0, 64)
     with pytest.raises(So3lrError, match="stage 5"):
         layers.check_status()
+
+
+def _rows(rows, width, dtype):
+    g = torch.Generator(device="cuda").manual_seed(rows + width)
+    return [torch.randn(rows, width, generator=g, device="cuda").to(dtype) for _ in range(3)]
+
+
+@pytest.mark.parametrize("rows, width", [(6000, 1024), (2600, 4096), (2400, 8192), (5003, 1536)])
+def test_ring_kernels_end_when_a_wait_runs_out(layers, rows, width):
+    """Rows come from HBM in about 1,500 cycles: with shorter limits blocks give up at their first rows
+    or later ones, with their copies in flight. The kernel ends, the host hears of it, and the next
+    calls are right, in the same memory."""
+    from so3lr_b200 import So3lrError
+    x, r, dy = _rows(rows, width, torch.bfloat16)
+    w = torch.ones(width, device="cuda")
+    calls = (lambda: layers.rms_norm_int8(x, w), lambda: layers.rms_norm_int8(x, w, r),
+             lambda: layers.rms_norm_backward(dy, x, w), lambda: layers.rms_norm_backward(dy, x, w, r))
+    for call in calls:
+        want = call()
+        gave_up = 0
+        try:
+            for limit in (1, 300, 700, 1500, 3000):
+                layers.set_wait_limit(limit)
+                got = call()
+                torch.cuda.synchronize()
+                try:
+                    layers.check_status()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))  # no wait was too long
+                except So3lrError as e:
+                    assert "stage 7" in str(e)
+                    gave_up += 1
+                layers.set_wait_limit()
+                assert all(torch.equal(a, b) for a, b in zip(call(), want))
+        finally:
+            layers.set_wait_limit()
+        assert gave_up >= 1
