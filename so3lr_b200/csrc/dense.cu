@@ -83,7 +83,7 @@ struct Params {
   float *gu;                     // kept projections, see gu_index
   const float *a_scales, *b_scales, *bias;
   uint32_t *partial;             // raw sums: [tile - whole][part][kTileM][TN]
-  int *err;
+  WaitLimit wait;
 };
 
 struct Item {
@@ -181,7 +181,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   const uint32_t drain = bars + 8u * (2 * kMaxStages + 4);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar_mem + 8 * (2 * kMaxStages + 5));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  volatile int *issued = reinterpret_cast<volatile int *>(tmem_slot + 2);
+  // for the end after a wait that gave up: K blocks that this CTA has fetched, and (leader) those that have been
+  // multiplied and the items whose accumulator is complete
+  volatile int *fetched = reinterpret_cast<volatile int *>(tmem_slot + 2);
+  volatile int *multiplied = reinterpret_cast<volatile int *>(tmem_slot + 3);
+  volatile int *finished = reinterpret_cast<volatile int *>(tmem_slot + 4);
+  auto wait = [&](uint32_t bar, int parity, int where) {
+    return tc::mbar_wait(bar, parity, abort_flag, p.wait.err, where, p.wait.cycles);
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(tc::cluster_rank());
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -205,7 +212,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
     }
     tc::mbar_init(drain, 1);
     *abort_flag = 0;
-    *issued = 0;
+    *fetched = *multiplied = *finished = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -219,6 +226,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   const uint32_t tmem = *tmem_slot;
   wait_for_predecessors();
 
+  // one thread of each CTA: its parts of the pair's n-th K block, which is K block kb of item w
+  auto fetch = [&](int n, const Item &w, int kb) {
+    const Problem &q = p.prob[w.prob];
+    const int s = n % S::kStages;
+    if (rank == 0) tc::mbar_expect_tx(full(s), 2 * S::kStage);
+    const uint32_t bar = tc::at_leader(full(s)), dst = base + s * S::kStage;
+    constexpr int kElems = MODE == kInt8 ? 128 : 64;  // of a K block
+    if (MODE == kGated || MODE == kGatedBack) {
+      const int k = kb * 64;
+      tc::tma_load(dst, &p.map[0], k, w.m0 + 128 * rank, bar);                  // x
+      tc::tma_load(dst + kOperand, &p.map[1 + rank], k, w.n0, bar);             // Wg | Wu
+      if (MODE == kGatedBack) {
+        tc::tma_load(dst + 2 * kOperand, &p.map[3], k, w.m0 + 128 * rank, bar); // dy
+        tc::tma_load(dst + 3 * kOperand, &p.map[4], w.n0 + 64 * rank, k, bar);  // Wd
+      }
+    } else {
+      const int seg = kb >= q.kb0 ? 1 : 0, k = (kb - (seg ? q.kb0 : 0)) * kElems;
+      const CUtensorMap *a = &p.map[q.a[seg]], *b = &p.map[q.b[seg]];
+      const int m = w.m0 + 128 * rank, c = w.n0 + TN / 2 * rank;
+      if (A_MN) {
+        tc::tma_load(dst, a, m, k, bar);
+        tc::tma_load(dst + kOperand / 2, a, m + 64, k, bar);
+      } else {
+        tc::tma_load(dst, a, k, m, bar);
+      }
+      if (B_MN) {
+        tc::tma_load(dst + kOperand, b, c, k, bar);
+        if (TN == 256) tc::tma_load(dst + kOperand + kOperand / 2, b, c + 64, k, bar);
+      } else {
+        tc::tma_load(dst + kOperand, b, k, c, bar);
+      }
+    }
+    *fetched = n + 1;
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------------- loads
     if (lane == 0) {
@@ -226,45 +268,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       bool ok = true;
       for (int it = 0; it < items && ok; ++it) {
         const Item w = item(it);
-        const Problem &q = p.prob[w.prob];
         for (int kb = w.kb_begin; kb < w.kb_end; ++kb, ++n) {
-          const int s = n % S::kStages;
-          ok = tc::mbar_wait(empty(s), ((n / S::kStages) & 1) ^ 1, abort_flag, p.err, 1);
+          ok = wait(empty(n % S::kStages), ((n / S::kStages) & 1) ^ 1, 1);
           if (!ok) break;
-          if (rank == 0) tc::mbar_expect_tx(full(s), 2 * S::kStage);
-          const uint32_t bar = tc::at_leader(full(s)), dst = base + s * S::kStage;
-          constexpr int kElems = MODE == kInt8 ? 128 : 64;  // of a K block
-          if (MODE == kGated || MODE == kGatedBack) {
-            const int k = kb * 64;
-            tc::tma_load(dst, &p.map[0], k, w.m0 + 128 * rank, bar);                  // x
-            tc::tma_load(dst + kOperand, &p.map[1 + rank], k, w.n0, bar);             // Wg | Wu
-            if (MODE == kGatedBack) {
-              tc::tma_load(dst + 2 * kOperand, &p.map[3], k, w.m0 + 128 * rank, bar); // dy
-              tc::tma_load(dst + 3 * kOperand, &p.map[4], w.n0 + 64 * rank, k, bar);  // Wd
-            }
-          } else {
-            const int seg = kb >= q.kb0 ? 1 : 0, k = (kb - (seg ? q.kb0 : 0)) * kElems;
-            const CUtensorMap *a = &p.map[q.a[seg]], *b = &p.map[q.b[seg]];
-            const int m = w.m0 + 128 * rank, c = w.n0 + TN / 2 * rank;
-            if (A_MN) {
-              tc::tma_load(dst, a, m, k, bar);
-              tc::tma_load(dst + kOperand / 2, a, m + 64, k, bar);
-            } else {
-              tc::tma_load(dst, a, k, m, bar);
-            }
-            if (B_MN) {
-              tc::tma_load(dst + kOperand, b, c, k, bar);
-              if (TN == 256) tc::tma_load(dst + kOperand + kOperand / 2, b, c + 64, k, bar);
-            } else {
-              tc::tma_load(dst + kOperand, b, k, c, bar);
-            }
-          }
-          *issued = n + 1;
+          fetch(n, w, kb);
         }
       }
       // every release of a K block has reached this CTA before it may leave
       for (int i = max(0, n - S::kStages); i < n && ok; ++i)
-        ok = tc::mbar_wait(empty(i % S::kStages), (i / S::kStages) & 1, abort_flag, p.err, 6);
+        ok = wait(empty(i % S::kStages), (i / S::kStages) & 1, 6);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -279,13 +291,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       for (int done = 0; done < items && ok; ++done) {
         const Item w = item(done);
         const int buf = done % S::kBuffers;
-        ok = tc::mbar_wait(acc_empty(buf), ((done / S::kBuffers) & 1) ^ 1, abort_flag, p.err, 2);
+        ok = wait(acc_empty(buf), ((done / S::kBuffers) & 1) ^ 1, 2);
         if (!ok) break;
         tc::fence_after();
         const uint32_t d = tmem + 256u * buf;
         for (int kb = w.kb_begin; kb < w.kb_end; ++kb, ++n) {
           const int s = n % S::kStages;
-          ok = tc::mbar_wait(full(s), (n / S::kStages) & 1, abort_flag, p.err, 3);
+          ok = wait(full(s), (n / S::kStages) & 1, 3);
           if (!ok) break;
           tc::fence_after();
           const uint32_t a = base + s * S::kStage, b = a + kOperand;
@@ -303,18 +315,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
         }
         if (!ok) break;
         tc::commit_pair(acc_full(buf));
+        *finished = done + 1;
       }
-      // every MMA has completed and, after a wait that gave up, so have the copies in flight (bounded)
+      // every MMA has completed
+      *multiplied = n;
       tc::commit_pair(drain);
-      tc::mbar_wait(drain, 0, abort_flag, p.err, 4);
-      if (!ok) {
-        const long long t0 = clock64();
-        for (int i = n; i < *issued; ++i)
-          while (!tc::mbar_try(full(i % S::kStages), (i / S::kStages) & 1) && clock64() - t0 < tc::kWaitCycles) {
-          }
-      }
+      wait(drain, 0, 4);
     } else if (lane == 0) {
-      tc::mbar_wait(drain, 0, abort_flag, p.err, 4);
+      wait(drain, 0, 4);
     }
     __syncwarp();
   } else {
@@ -327,8 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       const Item w = item(done);
       const Problem &q = p.prob[w.prob];
       const int buf = done % S::kBuffers;
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(acc_full(buf), (done / S::kBuffers) & 1, abort_flag, p.err, 5)))
-        break;
+      if (!__all_sync(0xffffffffu, wait(acc_full(buf), (done / S::kBuffers) & 1, 5))) break;
       tc::fence_after();
       const uint32_t acc = lanes + 256u * buf;
       auto release = [&] {  // this warp has read its part of the accumulator
@@ -483,8 +490,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   }
   tc::fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) tc::store_of_rank(abort_flag, rank ^ 1, 1);
   tc::cluster_sync();  // neither CTA leaves while the other may still signal it
   tc::fence_after();
+  if (*abort_flag) {
+    // A wait of either CTA gave up. All that the pair has started ends (with a limit) before TMEM is handed back
+    // and shared memory is left: copies, MMAs and the signals of both. A K block's barrier completes when both CTAs
+    // have fetched their parts, so the CTA that is behind fetches as many (any block of the right size; the release
+    // of their stages has reached the other CTA, so their MMAs are through with both).
+    if (threadIdx.x == 0) {
+      const Item w = item(0);
+      const int all = max(*fetched, tc::load_of_rank(fetched, rank ^ 1));
+      for (int n = *fetched; n < all; ++n) fetch(n, w, w.kb_begin);
+    }
+    __syncwarp();
+    tc::cluster_sync();
+    if (threadIdx.x == 0) {
+      const long long t0 = clock64();
+      const int through = tc::load_of_rank(multiplied, 0), tiles = tc::load_of_rank(finished, 0);
+      if (rank == 0)
+        for (int i = through; i < *fetched; ++i) tc::mbar_settle(full(i % S::kStages), (i / S::kStages) & 1, t0);
+      for (int i = max(0, through - S::kStages); i < through; ++i)
+        tc::mbar_settle(empty(i % S::kStages), (i / S::kStages) & 1, t0);
+      for (int i = max(0, tiles - S::kBuffers); i < tiles; ++i)
+        tc::mbar_settle(acc_full(i % S::kBuffers), (i / S::kBuffers) & 1, t0);
+      tc::mbar_settle(drain, 0, t0);
+    }
+    __syncwarp();
+    tc::cluster_sync();
+    tc::fence_after();
+  }
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
@@ -711,7 +746,7 @@ class Dense {
   void run_tiles(Params &p) {
     using S = Shape<MODE, TN>;
     allow_dynamic_smem(reinterpret_cast<const void *>(&k_dense<MODE, T, A_MN, B_MN, TN>), S::kSmem);
-    p.err = gave_up_flag();
+    p.wait = wait_limit();
     launch(k_dense<MODE, T, A_MN, B_MN, TN>, 2 * std::min(kPairs, p.items), kThreads, S::kSmem, stream_, p);
     if constexpr (MODE == kPlain || MODE == kInt8) {
       if (p.splits == 1) return;

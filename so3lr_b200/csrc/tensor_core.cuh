@@ -19,8 +19,8 @@ namespace tc {
 constexpr long long kWaitCycles = 4000000000LL;  // about 2 s at 1.9 GHz
 constexpr long long kPolled = 20000;             // limits below it: a blocking try alone takes 8,000 cycles
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+__device__ __forceinline__ uint32_t smem_u32(const volatile void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(const_cast<const void *>(p)));
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -39,11 +39,16 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 // a 32-bit shared variable of another block of the cluster
 template <class T>
-__device__ __forceinline__ T load_of_rank(const T *own, uint32_t rank) {
+__device__ __forceinline__ T load_of_rank(const volatile T *own, uint32_t rank) {
   uint32_t at, bits;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(own)), "r"(rank));
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bits) : "r"(at) : "memory");
   return reinterpret_cast<const T &>(bits);
+}
+__device__ __forceinline__ void store_of_rank(volatile int *own, uint32_t rank, int v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(own)), "r"(rank));
+  asm volatile("st.volatile.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -100,3 +100,54 @@ def test_ring_kernels_end_when_a_wait_runs_out(layers, rows, width):
         finally:
             layers.set_wait_limit()
         assert gave_up >= 1
+
+
+def _product(layers, kind):
+    g = torch.Generator(device="cuda").manual_seed(5)
+    half = lambda *n: torch.randn(*n, generator=g, device="cuda").mul_(n[-1] ** -0.5).bfloat16()  # noqa: E731
+    if kind.startswith("int8"):
+        rows, n, k = {"int8 ragged": (333, 1531, 1000), "int8 split": (600, 256, 16384), "int8 waves": (3000, 4096, 512)}[kind]
+        a, b = (torch.randint(-127, 128, s, generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
+                for s in ((rows, k), (n, k)))
+        sa, sb = torch.rand(rows, device="cuda"), torch.rand(n, device="cuda")
+        return lambda: (layers.int8_linear(a, sa, b, sb),)
+    rows, width, hidden = {"narrow": (3000, 256, 1024), "wide": (700, 1032, 1368), "unaligned": (300, 91, 251)}[kind]
+    x, dy, wg, wu, wd = half(rows, width), half(rows, width), half(hidden, width), half(hidden, width), half(width, hidden)
+
+    def step():
+        y, saved = layers.feed_forward_train(x, wg, wu, wd)
+        return (y, *layers.feed_forward_backward(dy, saved))
+    return step
+
+
+@pytest.mark.parametrize("kind", ["int8 ragged", "int8 split", "int8 waves", "narrow", "wide", "unaligned"])
+def test_products_end_when_a_wait_runs_out(layers, kind):
+    """The first K block takes about 1,500 cycles to come, a tile's accumulator some thousands: with
+    these limits CTA pairs give up at loads, products or epilogues, with copies and products in flight,
+    one CTA before the other. The kernels end, the host hears of it, and the next calls are right."""
+    from so3lr_b200 import So3lrError
+    step = _product(layers, kind)
+    want = step()
+    gave_up = 0
+    try:
+        for limit in (1, 200, 500, 1000, 1500, 2000, 3000, 5000, 8000, 15000):
+            layers.set_wait_limit(limit)
+            for _ in range(3):
+                try:
+                    got = step()
+                    torch.cuda.synchronize()
+                    layers.check_status()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))  # no wait was too long
+                except So3lrError as e:
+                    assert "gave up waiting (stage " in str(e) and 1 <= int(str(e).split("stage ")[1][0]) <= 6
+                    gave_up += 1
+                    torch.cuda.synchronize()  # a call of the step was refused: the one before it has ended
+                    try:
+                        layers.check_status()
+                    except So3lrError:
+                        pass
+            layers.set_wait_limit()
+            assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    finally:
+        layers.set_wait_limit()
+    assert gave_up >= 1
