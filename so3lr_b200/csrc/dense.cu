@@ -277,6 +277,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       // every release of a K block has reached this CTA before it may leave
       for (int i = max(0, n - S::kStages); i < n && ok; ++i)
         ok = wait(empty(i % S::kStages), (i / S::kStages) & 1, 6);
+      // in the odd CTA also the leader's last signal. Not before: each wait is for one step of the pipeline, so that
+      // its limit does not bound the whole kernel
+      if (rank != 0 && ok) wait(drain, 0, 4);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -320,8 +323,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       // every MMA has completed
       *multiplied = n;
       tc::commit_pair(drain);
-      wait(drain, 0, 4);
-    } else if (lane == 0) {
       wait(drain, 0, 4);
     }
     __syncwarp();

@@ -151,3 +151,25 @@ def test_products_end_when_a_wait_runs_out(layers, kind):
     finally:
         layers.set_wait_limit()
     assert gave_up >= 1
+
+
+def test_the_limit_is_a_waits_and_not_a_kernels(layers):
+    """Products of 0.8 ms and more under a limit of 0.2 ms: a tile takes 10 to 40 us, and every wait is for one
+    step of the pipeline."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    a, b = (torch.randint(-127, 128, s, generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
+            for s in ((32768, 4096), (8192, 4096)))
+    sa, sb = torch.rand(32768, device="cuda"), torch.rand(8192, device="cuda")
+    x, wg, wu, wd = (torch.randn(*s, generator=g, device="cuda").mul_(s[-1] ** -0.5).bfloat16()
+                     for s in ((65536, 1024), (4096, 1024), (4096, 1024), (1024, 4096)))
+    for call in (lambda: layers.int8_linear(a, sa, b, sb), lambda: layers.feed_forward(x, wg, wu, wd)):
+        want = call()
+        torch.cuda.synchronize()
+        try:
+            layers.set_wait_limit(400_000)
+            got = call()
+            torch.cuda.synchronize()
+            layers.check_status()
+        finally:
+            layers.set_wait_limit()
+        assert torch.equal(got, want)
