@@ -59,7 +59,10 @@ int float_type(at::ScalarType t, const char *what, bool half_only = false) {
 
 const Tensor &tensor(PyObject *o, const char *what) {
   if (!THPVariable_Check(o)) refuse(what, " must be a tensor");
-  return THPVariable_Unpack(o);
+  const Tensor &t = THPVariable_Unpack(o);
+  // the results would be without a tangent of their own, and what is computed from them wrong
+  if (t._fw_grad(0).defined()) refuse(what, " has a forward-mode tangent, which these calls do not carry on");
+  return t;
 }
 
 // A matrix of rows: all leading dimensions of a tensor, with one row stride

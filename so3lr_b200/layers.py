@@ -11,8 +11,8 @@ The row-wise half of a transformer block over per-atom (or per-token) features:
 * ``feed_forward``, the gated block y = (silu(x Wg^T) * (x Wu^T)) Wd^T, with
   ``feed_forward_train`` and ``feed_forward_backward`` for training.
 
-``rms_norm`` and ``feed_forward`` record themselves for autograd when an argument
-requires a gradient. ``FeedForwardBlock`` and ``Int8FeedForwardBlock`` run them
+``rms_norm`` and ``feed_forward`` record themselves for reverse-mode autograd when an
+argument requires a gradient; tensors with a forward-mode tangent are refused. ``FeedForwardBlock`` and ``Int8FeedForwardBlock`` run them
 together: the pre-norm sublayer as it is trained, and the same weights served
 in 8 bits.
 

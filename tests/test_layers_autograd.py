@@ -1,0 +1,58 @@
+"""What the row-wise feed-forward layers do with derivatives that they do not compute."""
+import pytest
+
+torch = pytest.importorskip("torch")
+import torch.autograd.forward_ad as fwd  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def layers():
+    from so3lr_b200 import layers
+    return layers
+
+
+def _calls(layers, device):
+    """Each call by name, as a function of its first floating tensor, and that tensor."""
+    x, w = torch.randn(4, 64, device=device).bfloat16(), torch.ones(64, device=device)
+    m = torch.randn(64, 64, device=device).bfloat16()
+    c, one = torch.ones(4, 64, dtype=torch.int8, device=device), torch.ones(4, device=device)
+    return {
+        "rms_norm": (lambda t: layers.rms_norm(t, w), x),
+        "rms_norm weight": (lambda t: layers.rms_norm(x, t), w),
+        "rms_norm residual": (lambda t: layers.rms_norm(x, w, t), x),
+        "rms_norm_int8": (lambda t: layers.rms_norm_int8(t, w), x),
+        "rms_norm_backward": (lambda t: layers.rms_norm_backward(t, x, w), x),
+        "feed_forward": (lambda t: layers.feed_forward(t, m, m, m), x),
+        "feed_forward weight": (lambda t: layers.feed_forward(x, m, m, t), m),
+        "feed_forward_train": (lambda t: layers.feed_forward_train(x, t, m, m), m),
+        "gate_int8": (lambda t: layers.gate_int8(t), x),
+        "int8_linear": (lambda t: layers.int8_linear(c, t, c, one), one),
+        "int8_linear bias": (lambda t: layers.int8_linear(c, one, c, one, t), one),
+        "dequantize_int8": (lambda t: layers.dequantize_int8(c, t), one),
+    }
+
+
+def test_forward_mode_is_refused(layers):
+    """Also where the tensor is elsewhere than on a GPU: the tangent is looked at first."""
+    for name, (call, t) in _calls(layers, "cpu").items():
+        with fwd.dual_level():
+            with pytest.raises(ValueError, match="forward-mode tangent|there is no CPU path|on cpu"):
+                call(fwd.make_dual(t, torch.ones_like(t)))
+    with fwd.dual_level(), pytest.raises(ValueError, match="x has a forward-mode tangent"):
+        x = torch.zeros(4, 64, dtype=torch.bfloat16)
+        layers.rms_norm(fwd.make_dual(x, x), torch.ones(64))
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_the_gpu(layers):
+    for name, (call, t) in _calls(layers, "cuda").items():
+        call(t)
+        with fwd.dual_level():
+            with pytest.raises(ValueError, match="forward-mode tangent"):
+                call(fwd.make_dual(t, torch.ones_like(t)))
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+    # with a gradient in reverse mode as well, autograd itself refuses
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    with fwd.dual_level(), pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+        layers.rms_norm(fwd.make_dual(x, torch.ones_like(x)), torch.ones(64, device="cuda"))
