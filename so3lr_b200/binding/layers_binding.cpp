@@ -7,6 +7,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -412,6 +413,8 @@ PyObject *method(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return nullptr;
   }
   try {
+    // it would record the results as constants
+    if (at::tracer::impl::is_dispatch_enabled()) refuse("torch.jit.trace cannot record the feed-forward layers");
     PyObject *r = F(args);
     if (PyErr_Occurred()) {
       Py_XDECREF(r);

@@ -12,7 +12,8 @@ The row-wise half of a transformer block over per-atom (or per-token) features:
   ``feed_forward_train`` and ``feed_forward_backward`` for training.
 
 ``rms_norm`` and ``feed_forward`` record themselves for reverse-mode autograd when an
-argument requires a gradient; tensors with a forward-mode tangent are refused. ``FeedForwardBlock`` and ``Int8FeedForwardBlock`` run them
+argument requires a gradient; tensors with a forward-mode tangent and
+``torch.jit.trace`` are refused. ``FeedForwardBlock`` and ``Int8FeedForwardBlock`` run them
 together: the pre-norm sublayer as it is trained, and the same weights served
 in 8 bits.
 

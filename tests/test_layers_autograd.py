@@ -56,3 +56,26 @@ def test_forward_mode_is_refused_on_the_gpu(layers):
     x = torch.randn(4, 64, device="cuda", requires_grad=True)
     with fwd.dual_level(), pytest.raises((ValueError, RuntimeError, NotImplementedError)):
         layers.rms_norm(fwd.make_dual(x, torch.ones_like(x)), torch.ones(64, device="cuda"))
+
+
+def _traced(call, t):
+    with pytest.raises(Exception, match="torch.jit.trace cannot record"), torch.no_grad():
+        torch.jit.trace(call, (t,), check_trace=False)
+
+
+def test_tracing_is_refused(layers):
+    """A trace would hold the results of the traced call as constants."""
+    x = torch.zeros(4, 64)
+    _traced(lambda t: layers.rms_norm(t, torch.ones(64))[0], x)
+    _traced(lambda t: layers.feed_forward(t, x, x, x), x)
+    _traced(lambda t: layers.gate_int8(t)[1], x)
+
+
+@pytest.mark.gpu
+def test_tracing_is_refused_on_the_gpu(layers):
+    for name, (call, t) in _calls(layers, "cuda").items():
+        _traced(lambda v: torch.zeros(1, device="cuda") + (call(v) if torch.is_tensor(call(v)) else call(v)[1]).sum(), t)
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    with pytest.raises(Exception, match="torch.jit.trace cannot record"):
+        torch.jit.trace(lambda t: layers.rms_norm(t, torch.ones(64, device="cuda"))[0], (x,), check_trace=False)
+    layers.rms_norm(x, torch.ones(64, device="cuda"))
