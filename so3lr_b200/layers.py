@@ -13,7 +13,9 @@ The row-wise half of a transformer block over per-atom (or per-token) features:
 
 ``rms_norm`` and ``feed_forward`` record themselves for reverse-mode autograd when an
 argument requires a gradient; tensors with a forward-mode tangent and
-``torch.jit.trace`` are refused. ``FeedForwardBlock`` and ``Int8FeedForwardBlock`` run them
+``torch.jit.trace`` are refused. All other calls record nothing: their results, the
+stream of ``rms_norm_int8`` among them, are detached from arguments that require a
+gradient. ``FeedForwardBlock`` and ``Int8FeedForwardBlock`` run them
 together: the pre-norm sublayer as it is trained, and the same weights served
 in 8 bits.
 
@@ -85,20 +87,22 @@ class _NormFunction(torch.autograd.Function):
 
 
 def rms_norm(x, weight, residual=None, *, eps: float = 1e-6):
-    """(y, s): s = x + residual rounded to x's type (x itself without a
-    residual), y = s * weight / sqrt(mean(s^2) + eps). weight: x's type or float32."""
+    """(y, s): s = x + residual rounded to x's type (x itself, detached under no_grad,
+    without a residual), y = s * weight / sqrt(mean(s^2) + eps). weight: x's type or float32."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     (residual is not None and residual.requires_grad)):
         return _NormFunction.apply(x, weight, residual, eps)
     y, _, s = _layers.rms_norm(x, weight, residual, eps, False)
-    return y, s
+    return y, s.detach() if s.requires_grad else s
 
 
 def rms_norm_int8(x, weight, residual=None, *, eps: float = 1e-6):
     """(codes, scales, s): rms_norm's y in 8 bits, one row for each row of x:
     y ~ codes * scales[:, None] with scales = max|y| / 127 of each row (float32).
-    Row starts of `codes` are 16-byte aligned."""
-    return _layers.rms_norm(x, weight, residual, eps, True)
+    Row starts of `codes` are 16-byte aligned. Records nothing for autograd: s is
+    detached with a residual and without one."""
+    codes, scales, s = _layers.rms_norm(x, weight, residual, eps, True)
+    return codes, scales, s.detach() if s.requires_grad else s
 
 
 def rms_norm_backward(dy, s, weight, ds=None, *, eps: float = 1e-6):

@@ -79,3 +79,27 @@ def test_tracing_is_refused_on_the_gpu(layers):
     with pytest.raises(Exception, match="torch.jit.trace cannot record"):
         torch.jit.trace(lambda t: layers.rms_norm(t, torch.ones(64, device="cuda"))[0], (x,), check_trace=False)
     layers.rms_norm(x, torch.ones(64, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_eight_bit_calls_are_detached(layers):
+    """The stream with a residual and without one alike, whatever requires a gradient."""
+    x, r = (torch.randn(4, 64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for residual in (None, r, r.detach()):
+        codes, scales, s = layers.rms_norm_int8(x, w, residual)
+        assert not s.requires_grad and not scales.requires_grad
+        if residual is None:
+            assert s.data_ptr() == x.data_ptr() and torch.equal(s, x)
+    assert layers.rms_norm_int8(r.detach(), w)[2] is not None
+    plain = r.detach()
+    assert layers.rms_norm_int8(plain, w)[2] is plain  # nothing to detach
+    b, one = codes[:2], torch.ones(2, device="cuda", requires_grad=True)
+    assert not layers.int8_linear(codes, scales, b, one, one).requires_grad
+    assert not layers.dequantize_int8(codes, torch.ones(4, device="cuda", requires_grad=True)).requires_grad
+    assert not layers.gate_int8(x)[1].requires_grad
+    y, _ = layers.rms_norm(x, w, r)
+    assert y.requires_grad
+    with torch.no_grad():
+        for residual in (None, r):
+            assert not any(t.requires_grad for t in layers.rms_norm(x, w, residual))
