@@ -194,11 +194,23 @@ struct RowRing {
 };
 constexpr int kRingHeader = 128, kRingStages = 8;
 
-// The scale of a row of s w rstd from the bits of max|s w|; `inv` takes s w to codes.
-__device__ __forceinline__ float norm_scale(float mean_square, uint32_t top_bits, float &inv) {
-  const float rstd = rsqrtf(mean_square);
-  const float scale = row_scale(__float_as_uint(__uint_as_float(top_bits) * rstd) & 0x7fffffffu, inv);
-  if (inv != 0.0f) inv *= rstd;
+// The scale of a row of s w rstd from the bits of max|s w|; `inv` takes v and ve, the row's
+// s w, to codes. inv is 127 / max|s w|, which overflows below 2^-121: rows of less than 2^-100
+// are lifted by 2^64 first.
+template <int COUNT>
+__device__ __forceinline__ float norm_scale(float mean_square, uint32_t top_bits, float &inv, float (&v)[COUNT],
+                                            float &ve) {
+  const float rstd = rsqrtf(mean_square), top = __uint_as_float(top_bits);
+  const float scale = row_scale(__float_as_uint(top * rstd) & 0x7fffffffu, inv);
+  if (inv != 0.0f) {
+    if (top < 0x1p-100f) {
+      inv *= 0x1p-64f;
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) v[i] *= 0x1p64f;
+      ve *= 0x1p64f;
+    }
+    inv *= rstd;
+  }
   return scale;
 }
 
@@ -278,7 +290,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
     uint32_t bits = __float_as_uint(top) & 0x7fffffffu;
     const float sum = team.sum_and_max(sq, bits, slot, slot_max);
     float inv;
-    const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv);
+    const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv, v, ve);
     if (!live) return;
     if (team.t == 0) a.scales[row] = scale;
     signed char *codes = a.codes + row * a.codes_stride;
@@ -486,8 +498,8 @@ __global__ void __launch_bounds__(512)
     const float sum = team.sum_and_max(sq, bits, slot[k & 1], slot_max[k & 1]);  // a barrier, as below
     if (ring.gave_up(k)) break;
     if (t == 0 && k + stages < rows) fetch(k + stages);
-    float inv;
-    const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv);
+    float inv, none = 0.0f;
+    const float scale = norm_scale(fmaf(sum, inv_width, eps), bits, inv, v, none);
     if (t == 0) a.scales[row] = scale;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
