@@ -98,9 +98,11 @@ def rms_norm(x, weight, residual=None, *, eps: float = 1e-6):
 
 def rms_norm_int8(x, weight, residual=None, *, eps: float = 1e-6):
     """(codes, scales, s): rms_norm's y in 8 bits, one row for each row of x:
-    y ~ codes * scales[:, None] with scales = max|y| / 127 of each row (float32).
-    Row starts of `codes` are 16-byte aligned. Records nothing for autograd: s is
-    detached with a residual and without one."""
+    y ~ codes * scales[:, None] with scales = max|y| / 127 of each row (float32) and
+    codes = y / scale rounded to nearest; the quotient is formed with a reciprocal, so
+    that a y within a few float32 units of a tie may fall on its other side. Row starts
+    of `codes` are 16-byte aligned. Records nothing for autograd: s is detached with a
+    residual and without one."""
     codes, scales, s = _layers.rms_norm(x, weight, residual, eps, True)
     return codes, scales, s.detach() if s.requires_grad else s
 
@@ -130,14 +132,17 @@ def dequantize_int8(codes, scales, dtype=torch.bfloat16):
 
 def quantize_weight(w):
     """(codes, scales) of a weight [n, k], a scale for each output channel: done
-    once when a model is loaded, with the same rounding as rms_norm_int8. Row
-    starts of `codes` are 16-byte aligned."""
+    once when a model is loaded. codes = w / scale rounded to nearest, ties to even;
+    channels of zeros get scale 0, channels with an infinity or a NaN scale NaN, both
+    codes 0. Row starts of `codes` are 16-byte aligned."""
     f = w.detach().float()
     n, k = f.shape
     scales = f.abs().amax(1) / 127.0
+    live = scales.isfinite() & (scales > 0)
+    quotients = torch.where(live[:, None], f / torch.where(live, scales, 1.0)[:, None], 0.0)
     codes = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.int8, device=f.device)[:, :k]
-    codes.copy_(torch.round(f / torch.where(scales > 0, scales, 1.0)[:, None]).clamp_(-127, 127))
-    return codes, scales
+    codes.copy_(torch.round(quotients).clamp_(-127, 127))
+    return codes, torch.where(scales.isfinite(), scales, torch.nan)
 
 
 # ----------------------------------------------------------------- feed-forward
