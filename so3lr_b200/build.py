@@ -8,8 +8,8 @@ Every translation unit is compiled with
 translation units whose code depends on the model width are compiled once per
 supported width (``-DSO3LR_FEATURES=128`` and ``=256``; the mixed-precision
 filter kernels exist for F = 128 only). Object files are cached under
-``so3lr_b200/_build`` and rebuilt when a source or header is newer. Where torch is
-installed, the Python module of the row-wise feed-forward layers is compiled
+``so3lr_b200/_build`` and rebuilt when a source or header is newer. Where a torch with
+CUDA is installed, the Python module of the row-wise feed-forward layers is compiled
 against it and linked to the library.
 """
 from __future__ import annotations
@@ -80,11 +80,21 @@ def _compile(unit, newest_header: float, force: bool, verbose: bool) -> pathlib.
     return obj
 
 
+def torch_root() -> pathlib.Path | None:
+    """The folder of the torch that `import torch` would take, without importing it."""
+    spec = importlib.util.find_spec("torch")
+    return pathlib.Path(spec.origin).parent if spec is not None and spec.origin else None
+
+
 def torch_module() -> pathlib.Path | None:
     """The Python module of the feed-forward layers (binding/layers_binding.cpp),
-    compiled against the torch that is installed; None without torch (the rest of
-    the package does not need it)."""
-    if importlib.util.find_spec("torch") is None:
+    compiled against the torch that is installed. None where it cannot be: without
+    torch, with one for CPUs only, or without Python's headers (the rest of the package
+    needs none of them)."""
+    root = torch_root()
+    if root is None or not (root / "lib" / "libtorch_cuda.so").exists():
+        return None
+    if not (pathlib.Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
         return None
     return HERE / ("_layers" + sysconfig.get_config_var("EXT_SUFFIX"))
 

@@ -39,7 +39,7 @@ try:
     from . import _layers
 except (ImportError, So3lrError) as e:
     raise ImportError(f"the feed-forward layers' module is missing or does not fit the installed torch ({e}): build it "
-                      "with `python -m so3lr_b200.build`") from e
+                      "with `python -m so3lr_b200.build`, which needs a torch with CUDA and Python's headers") from e
 
 __all__ = ["rms_norm", "rms_norm_int8", "rms_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
            "quantize_weight", "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock",

@@ -2,6 +2,10 @@
 import pytest
 
 torch = pytest.importorskip("torch")
+from so3lr_b200.build import torch_module  # noqa: E402
+
+if torch_module() is None:
+    pytest.skip("the layers' module is not built here", allow_module_level=True)
 import torch.autograd.forward_ad as fwd  # noqa: E402
 
 
