@@ -105,7 +105,10 @@ def build_torch_module(force: bool = False) -> pathlib.Path | None:
         return None
     src, header = HERE / "binding" / "layers_binding.cpp", INCLUDE / "so3lr_b200.h"
     newest = max(f.stat().st_mtime for f in (src, header, pathlib.Path(__file__)))
-    if not force and out.exists() and out.stat().st_mtime >= newest:
+    # what the module was compiled against: its binary interface is that of one torch build
+    stamp, version = BUILD / "layers_module.txt", (torch_root() / "version.py").read_text()
+    current = stamp.exists() and stamp.read_text() == version
+    if not force and current and out.exists() and out.stat().st_mtime >= newest:
         return out
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
@@ -118,6 +121,8 @@ def build_torch_module(force: bool = False) -> pathlib.Path | None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    BUILD.mkdir(exist_ok=True)
+    stamp.write_text(version)
     return out
 
 

@@ -45,3 +45,30 @@ def test_no_torch_and_no_python_headers(monkeypatch, torch_of, tmp_path):
         assert build.build_torch_module(force=True) is None
     monkeypatch.setattr(build.importlib.util, "find_spec", lambda name, *a: None)
     assert build.build_torch_module(force=True) is None
+
+
+def test_the_module_is_built_again_for_another_torch(monkeypatch, torch_of, tmp_path):
+    """The same sources, older than the module, and a torch of another version."""
+    pytest.importorskip("torch.utils.cpp_extension")
+    calls = []
+
+    def run(cmd, **k):
+        calls.append(cmd)
+        out.write_bytes(b"module")
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "BUILD", tmp_path / "_build")
+    out = tmp_path / "_layers.so"
+    monkeypatch.setattr(build, "torch_module", lambda: out)
+    torch_of(version="__version__ = '2.0'")
+    for _ in range(3):
+        assert build.build_torch_module() == out
+    assert len(calls) == 1
+    torch_of(version="__version__ = '2.1'")
+    for _ in range(3):
+        build.build_torch_module()
+    assert len(calls) == 2
+    out.unlink()
+    build.build_torch_module()
+    assert len(calls) == 3
