@@ -381,7 +381,8 @@ void so3lr_layers_wait_limit(long long cycles);
  * when `codes` is given instead, into 8 bits with a scale for each row:
  *   scale = max|y| / 127, code = y / scale rounded to nearest (ties to even)
  * A row of zeros gets scale 0 and codes 0; a row that holds an infinity or a NaN
- * gets scale NaN and codes 0. s, y may be the memory of x or residual. */
+ * gets scale NaN and codes 0. s and y may each be the memory of x or of residual,
+ * row for row (not both the same). */
 typedef struct {
   long long rows, width;
   int dtype;                  /* x, residual, s, y */
@@ -418,7 +419,7 @@ typedef struct {
   const void *weight;
   const void *ds;             /* optional */
   long long ds_stride;
-  void *dx;                   /* may be the memory of dy or ds */
+  void *dx;                   /* may be the memory of dy or ds, row for row */
   long long dx_stride;
   void *dweight;              /* width */
 } so3lr_rms_norm_backward_args;
