@@ -752,7 +752,7 @@ enum RowOp { kNorm, kNormBack, kNorm8, kGate8 };
 struct Hold {
   int lanes, per;
 };
-Hold hold(long long width, Path path, int size, RowOp op) {
+constexpr Hold hold(long long width, Path path, int size, RowOp op) {
   if (path != kScalar) {
     // rows off the boundaries: their edges take up to 2 (16 / size - 1) threads
     if (width <= 64 && (path == kWide || size == 4)) return {8, 8};
@@ -766,22 +766,40 @@ Hold hold(long long width, Path path, int size, RowOp op) {
   }
   return {0, width <= (path == kShifted && op == kNorm ? 1024 : 4096) ? 8 : 16};
 }
-// f(std::integral_constant lanes, std::integral_constant per) for each that hold() gives
-template <Path PATH, class F>
+// Whether a call reaches the kernels that hold a row so. The widths are those at which
+// hold() changes, each the widest of its kind.
+constexpr bool reached(Path path, int size, RowOp op, int lanes, int per) {
+  for (const int width : {64, 128, 256, 512, 1024, 4096, 8192, 16384, 32768}) {
+    if (width > (op == kGate8 ? 32768 : 16384)) continue;
+    if (op == kGate8 && path != kWide && (path == kScalar) != (width > 16384)) continue;  // launch_gate_int8
+    if (op == kNormBack && path == kWide && width > 512 && width <= 8192) continue;       // backward_ring
+    const Hold h = hold(width, path, size, op);
+    if (h.lanes == lanes && h.per == per) return true;
+  }
+  return false;
+}
+// f(std::integral_constant lanes, std::integral_constant per) for h; kernels are compiled
+// for those that a call reaches
+template <Path PATH, int SIZE, RowOp OP, class F>
 void by_hold(const Hold &h, F &&f) {
+  bool found = false;
   auto lanes_per = [&](auto lanes, auto per) {
-    if (h.lanes == lanes && h.per == per) f(lanes, per);
+    if constexpr (reached(PATH, SIZE, OP, decltype(lanes)::value, decltype(per)::value))
+      if (h.lanes == lanes && h.per == per) {
+        found = true;
+        f(lanes, per);
+      }
   };
   using std::integral_constant;
-  if constexpr (PATH != kScalar) {
-    lanes_per(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-    lanes_per(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    lanes_per(integral_constant<int, 32>{}, integral_constant<int, 32>{});
-  }
-  lanes_per(integral_constant<int, 0>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 16>{}, integral_constant<int, 8>{});
   lanes_per(integral_constant<int, 32>{}, integral_constant<int, 8>{});
   lanes_per(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  lanes_per(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+  lanes_per(integral_constant<int, 0>{}, integral_constant<int, 8>{});
   lanes_per(integral_constant<int, 0>{}, integral_constant<int, 16>{});
+  lanes_per(integral_constant<int, 0>{}, integral_constant<int, 32>{});
+  if (!found) throw Error("feed-forward layers: no kernel holds such a row");
 }
 template <class F>
 void by_path(Path path, F &&f) {
@@ -853,13 +871,12 @@ Hold backward_hold(const so3lr_rms_norm_backward_args &a, Path path) {
   return hold(a.width, path, a.dtype == SO3LR_FLOAT32 ? 4 : 2, kNormBack);
 }
 // The ring kernel's blocks, no stages where the direct loads serve: rows of a warp,
-// unaligned rows, and rows too long for the ring
+// rows off the boundaries, and rows too long for the ring
 RingPlan backward_ring(const so3lr_rms_norm_backward_args &a) {
   if (backward_path(a) != kWide || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
   // two rows deep: float32, 2048 wide, 4.6 TB/s of inputs in four blocks an SM, 3.4 in three, three deep
-  const RingPlan p =
-      ring_plan(a.rows, row_threads(a.width, 16), 512, 2, 3 * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
-  return p.stages < 2 ? RingPlan{0, 0, 0} : p;
+  // (8192 wide, the longest: 96 KB a row, two of them in one)
+  return ring_plan(a.rows, row_threads(a.width, 16), 512, 2, 3 * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
 }
 int backward_parts(const so3lr_rms_norm_backward_args &a) {
   const RingPlan r = backward_ring(a);
@@ -875,22 +892,23 @@ void norm_backward(const so3lr_rms_norm_backward_args &a, float *partial, int gr
   constexpr int V = chunk_of(PATH, sizeof(T));
   constexpr bool SHIFT = PATH == kShifted;
   const Hold h = backward_hold(a, PATH);
-  by_hold<PATH>(h, [&](auto lanes, auto per) {
+  by_hold<PATH, sizeof(T), kNormBack>(h, [&](auto lanes, auto per) {
     constexpr int L = decltype(lanes)::value, P = decltype(per)::value, N = P / V;
     const float inv = 1.0f / float(a.width), eps = float(a.eps);
-    if constexpr (L != 0 && P <= 16) {
+    if constexpr (L != 0) {
       launch(k_rms_norm_backward<T, W, V, N, L, kTeamThreads, SHIFT>, grid, kTeamThreads,
              kTeamThreads / L * a.width * sizeof(float), s, a, partial, inv, eps);
-    } else if constexpr (L == 0) {
+    } else {
       // rows that start elsewhere than on 16-byte boundaries, and those too long for the ring
       const int threads = row_threads(a.width, P);
-      if constexpr (PATH != kWide && P == 8) {
-        if (threads <= 512) {
+      if constexpr (P == 8) {
+        if (PATH == kShifted || threads <= 512) {  // shifted: up to 4096 elements, see hold()
           launch(k_rms_norm_backward<T, W, V, N, 0, 512, SHIFT>, grid, threads, 0, s, a, partial, inv, eps);
           return;
         }
       }
-      launch(k_rms_norm_backward<T, W, V, N, 0, 1024, SHIFT>, grid, threads, 0, s, a, partial, inv, eps);
+      if constexpr (PATH != kShifted || P != 8)
+        launch(k_rms_norm_backward<T, W, V, N, 0, 1024, SHIFT>, grid, threads, 0, s, a, partial, inv, eps);
     }
   });
 }
@@ -936,15 +954,19 @@ void launch_rms_norm(const so3lr_rms_norm_args &a, cudaStream_t s) {
       by_path(chosen, [&](auto path) {
         constexpr Path PATH = decltype(path)::value;
         constexpr int VEC = chunk_of(PATH, sizeof(T));
-        const Hold h = hold(a.width, PATH, sizeof(T), a.codes ? kNorm8 : kNorm);
-        by_hold<PATH>(h, [&](auto lanes, auto per) {
-          constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
-          constexpr bool SHIFT = PATH == kShifted;
-          const auto fn =
-              a.codes ? &k_rms_norm<T, W, VEC, N, L, true, SHIFT> : &k_rms_norm<T, W, VEC, N, L, false, SHIFT>;
-          launch(fn, team_grid(h, a.rows), team_block(h, a.width), 0, s, a,
-                 1.0f / float(a.width), float(a.eps));
-        });
+        auto run = [&](auto op) {
+          constexpr RowOp OP = decltype(op)::value;
+          const Hold h = hold(a.width, PATH, sizeof(T), OP);
+          by_hold<PATH, sizeof(T), OP>(h, [&](auto lanes, auto per) {
+            constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
+            launch(k_rms_norm<T, W, VEC, N, L, OP == kNorm8, PATH == kShifted>, team_grid(h, a.rows),
+                   team_block(h, a.width), 0, s, a, 1.0f / float(a.width), float(a.eps));
+          });
+        };
+        if (a.codes)
+          run(std::integral_constant<RowOp, kNorm8>{});
+        else
+          run(std::integral_constant<RowOp, kNorm>{});
       });
     });
   });
@@ -987,13 +1009,10 @@ void launch_gate_int8(const so3lr_gate_int8_args &a, cudaStream_t s) {
     by_path(chosen, [&](auto path) {
       constexpr Path PATH = decltype(path)::value;
       constexpr int VEC = chunk_of(PATH, sizeof(T));
-      by_hold<PATH>(h, [&](auto lanes, auto per) {
+      by_hold<PATH, sizeof(T), kGate8>(h, [&](auto lanes, auto per) {
         constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
         launch(k_gate_int8<T, VEC, N, L, PATH == kShifted>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
       });
-      if constexpr (PATH != kShifted)
-        if (h.per == 32 && h.lanes == 0)
-          launch(k_gate_int8<T, VEC, 32 / VEC, 0, false>, team_grid(h, a.rows), team_block(h, a.hidden), 0, s, a);
     });
   });
 }
