@@ -66,6 +66,15 @@ const Tensor &tensor(PyObject *o, const char *what) {
   return t;
 }
 
+double number(PyObject *o, const char *what) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(what, " must be a number");
+  }
+  return v;
+}
+
 // A matrix of rows: all leading dimensions of a tensor, with one row stride
 struct Rows {
   void *data;
@@ -166,7 +175,7 @@ PyObject *rms_norm(Args o) {
   a.rows = r.rows;
   a.width = r.width;
   a.dtype = float_type(r.type, "x");
-  a.eps = PyFloat_AsDouble(o[3]);
+  a.eps = number(o[3], "eps");
   a.x = r.data;
   a.x_stride = r.stride;
   a.weight = vector_of(w, "weight", r, r.width, r.type, at::kFloat);
@@ -213,7 +222,7 @@ PyObject *rms_norm_backward(Args o) {
   a.rows = r.rows;
   a.width = r.width;
   a.dtype = float_type(r.type, "s");
-  a.eps = PyFloat_AsDouble(o[4]);
+  a.eps = number(o[4], "eps");
   a.s = r.data;
   a.s_stride = r.stride;
   a.weight = vector_of(w, "weight", r, r.width, r.type, at::kFloat);

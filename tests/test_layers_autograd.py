@@ -107,3 +107,14 @@ def test_eight_bit_calls_are_detached(layers):
     with torch.no_grad():
         for residual in (None, r):
             assert not any(t.requires_grad for t in layers.rms_norm(x, w, residual))
+
+
+@pytest.mark.gpu
+def test_eps_that_is_no_number(layers):
+    x, w = torch.zeros(2, 64, device="cuda"), torch.ones(64, device="cuda")
+    for wrong in ("1e-6", None, [1e-6]):
+        with pytest.raises(ValueError, match="eps must be a number"):
+            layers.rms_norm(x, w, eps=wrong)
+        with pytest.raises(ValueError, match="eps must be a number"):
+            layers.rms_norm_backward(x, x, w, eps=wrong)
+    layers.rms_norm(x, w, eps=torch.tensor(1e-6))
