@@ -340,7 +340,8 @@ void so3lr_destroy(so3lr_handle *h);
  *   - No handle. Every pointer is device memory of the calling thread's current
  *     CUDA device; `stream` is a cudaStream_t of that device (NULL: the default
  *     stream). The work is asynchronous on `stream`: a call returns when its
- *     kernels are queued, allocates nothing and may be captured in a graph.
+ *     kernels are queued, allocates nothing and may be captured in a graph. (The
+ *     first call of a process allocates a few words of page-locked host memory.)
  *   - A matrix is row-major with unit column stride and a row stride in elements
  *     (inputs: any stride >= 0, so a row may be broadcast; outputs: at least the
  *     row's length). Any alignment of the element type is accepted; rows that
@@ -379,9 +380,12 @@ void so3lr_layers_wait_limit(long long cycles);
  * The norm is of s as stored, so so3lr_rms_norm_backward, which has only the
  * stored s, returns the gradient of exactly what ran. The result goes to `y`, or,
  * when `codes` is given instead, into 8 bits with a scale for each row:
- *   scale = max|y| / 127, code = y / scale rounded to nearest (ties to even)
- * A row of zeros gets scale 0 and codes 0; a row that holds an infinity or a NaN
- * gets scale NaN and codes 0. s and y may each be the memory of x or of residual,
+ *   scale = max|y| / 127, code = y / scale rounded to nearest (ties to even; the
+ *   quotient within a few float32 units, so a y that near a tie may go either way)
+ * A row of zeros, or of values whose scale is below float32's normal numbers, gets
+ * scale 0 and codes 0; a row that holds an infinity or a NaN gets scale NaN and codes
+ * 0. Squares and products s * weight are float32: a row must stay below 1.8e19 in
+ * root of its sum of squares, else y is 0, and |s * weight| below 3.4e38 for codes. s and y may each be the memory of x or of residual,
  * row for row (not both the same). */
 typedef struct {
   long long rows, width;
@@ -476,6 +480,8 @@ int so3lr_dequantize_int8(const so3lr_dequantize_int8_args *args, void *stream, 
  *   h = silu(x Wg^T) * (x Wu^T)    (hidden wide; rounded to the element type between the products, for
  *                                   few rows to two such parts, so that the rounding does not show)
  *   y = h Wd^T
+ * Few rows are 16 or fewer, and up to 256 where the weights are small. The same row of
+ * x can therefore have results that differ in their last bits in calls of few and of many rows.
  * Weights are stored with output channels as rows. */
 typedef struct {
   long long rows, width, hidden;
@@ -493,7 +499,8 @@ typedef struct {
   void *h;                    /* optional: rows x hidden, contiguous; h as the second product reads it,
                                  which so3lr_feed_forward_backward needs */
   float *gu;                  /* optional: so3lr_feed_forward_keep bytes, 16-byte aligned; the two projections
-                                 in float32 for so3lr_feed_forward_backward, which otherwise computes them again */
+                                 in float32 for so3lr_feed_forward_backward, which otherwise computes them again
+                                 (8 bytes for each element of h: most of what a training step saves) */
 } so3lr_feed_forward_args;
 /* Bytes of `gu` worth keeping for the backward pass: 0 where computing the
  * projections again is cheaper than writing and reading them (narrow layers). */
@@ -505,7 +512,8 @@ int so3lr_feed_forward(const so3lr_feed_forward_args *args, void *workspace, lon
 /* Gradients of so3lr_feed_forward for dy: with g, u the two projections (kept by
  * the forward pass, or computed again), sg = 1 / (1 + exp(-g)),
  *   dh = dy Wd,  du = dh g sg,  dg = dh u sg (1 + g (1 - sg))
- *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h */
+ *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
+ * dg and du are rounded to the element type between the products, as h is. */
 typedef struct {
   long long rows, width, hidden;
   int dtype;

@@ -19,6 +19,18 @@
 // Tiles beyond the last whole wave (one tile a CTA pair) of a long contraction are
 // split along K, so that they fill the pairs too: each part writes raw 32-bit sums,
 // k_join adds them in order.
+//
+// Sums are float32 (int32 for 8-bit operands). What goes from one product to the next is
+// rounded to the element type, because the tensor core takes 16-bit operands: h = silu(g) u
+// in the forward pass, dg and du in the gradient, each from float32 accumulators and
+// rounded once. Two independent roundings instead of one: a training step's results are
+// 1.4 times as far from 64-bit ones as a float32 chain's that is rounded at its end (2-norm:
+// bfloat16 0.0023 and 0.0017 at 24000 x 256 x 1024, float16 0.00029 and 0.00021 at 8190 x
+// 2048 x 8200). Keeping h, dg and du in two parts would add two thirds
+// to the products.
+//
+// Every wait is bounded (layers.hpp, WaitLimit) and waits for one step of the pipeline.
+// After one that gives up, the pair ends what it has started before it leaves.
 #include <atomic>
 #include <cstring>
 #include <string>

@@ -6,7 +6,8 @@
 // The products run on warp-level MMAs (m16n8k16 / m16n8k32, rows as M, channels as N)
 // straight from registers: a tile of the tcgen05 kernel would be filled to a few of its
 // 256 rows and would need its operands in shared memory first. One row through the
-// 2048 x 8192 block takes 20 us, 5.0 TB/s of weights, bound by the latency of their loads.
+// 2048 x 8192 block takes 21 us, 4.7 TB/s of weights: two or three 16-byte loads a lane, held
+// in registers, do not keep HBM busy.
 //
 // Contraction order: an MMA takes two 4-byte words of each lane's operands. A lane
 // loads 16 contiguous bytes (words 0..3) of its row and of its channel at the same
@@ -251,7 +252,7 @@ void run(const FewArgs &a, cudaStream_t s) {
   // Warps that split the contraction, four steps of 64 bytes or more to each: 8, or 16
   // where the blocks alone would leave too few loads in flight. One row, 2048 channels
   // of 8192 bfloat16 (256 blocks): 12.3 us with 8, 9.3 us with 16; 4096 channels of
-  // 4096 bytes (512 blocks): 5.6 us with 8, 7.0 us with 16.
+  // 4096 bytes (512 blocks): 4.4 us with 8, 6.5 us with 16.
   const unsigned channels = unsigned((a.n + 7) / 8), groups = unsigned((a.rows + 15) / 16), blocks = channels * groups;
   const int most = blocks < 2 * kSmCount ? max_warps(a.rows > 8) : 8;
   const int steps = (a.k + 4 * kPer - 1) / (4 * kPer), warps = std::max(1, std::min(most, steps / 4));

@@ -96,10 +96,12 @@ __device__ __forceinline__ Chunk<T, VEC> to_chunk(const float (&v)[VEC]) {
   return c;
 }
 
-// 1 / (1 + exp(-g)) with the hardware's exponential and reciprocal (both within 2
-// units in the last place). exp(-g) overflows to infinity for g < -88, and the
-// result is then 0, as it should be to float32's range; the flushed denormals of
-// either do not show beside 1.
+// 1 / (1 + exp(-g)) with the hardware's exponential and reciprocal, within 2 units in the
+// last place each, besides the rounding of the exponential's argument: up to 0.6 |g| units
+// of exp(-g), which show where it is not small beside 1 (g = -10: 6 units of a sigmoid of
+// 4e-5; g = -80: 50 of one of 2e-35). exp(-g) overflows to infinity for g < -88, and the
+// result is then 0, as it should be to float32's range; the flushed denormals of either do
+// not show beside 1.
 __device__ __forceinline__ float sigmoid_f32(float g) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));

@@ -12,10 +12,11 @@
 // addresses cost each thread about a hundred instructions, an element about ten. Long
 // 8-bit rows and gradients walk over their rows with a ring of copies in flight.
 //
-// Measured, 33.5 M bfloat16 elements, rows of 256 / 4096 / 1003: norm with residual 6.5 /
-// 6.3 / 5.1 TB/s (a copy: 6.5), 8-bit norm without 3.8 / 3.7 / 2.3, gradient 5.4 / 5.2 /
-// 3.8, 8-bit gate 5.8 / 6.1 / 3.9, reading back 5.9 / 6.2 / 4.0. The 8-bit norm issues 21
-// instructions an element at 0.8 of the issue rate, the gradient 29 at 0.6.
+// Measured, 33.5 M bfloat16 elements, float32 weights, rows of 256 / 4096 / 1003: norm with
+// residual 6.5 / 6.5 / 4.5 TB/s (a copy: 6.5), 8-bit norm without 3.4 / 3.7 / 1.8 (bfloat16
+// weights 3.7 / 3.7 / 2.2), gradient with ds 5.5 / 5.3 / 3.8, 8-bit gate 5.9 / 6.3 / 4.0,
+// reading back 5.9 / 6.2 / 3.9. The 8-bit norm issues 21 instructions an element at 0.8 of
+// the issue rate, the gradient 29 at 0.6.
 #include "layers_common.cuh"
 #include "model_host.hpp"
 #include "tensor_core.cuh"
@@ -196,7 +197,9 @@ constexpr int kRingHeader = 128, kRingStages = 8;
 
 // The scale of a row of s w rstd from the bits of max|s w|; `inv` takes v and ve, the row's
 // s w, to codes. inv is 127 / max|s w|, which overflows below 2^-121: rows of less than 2^-100
-// are lifted by 2^64 first.
+// are lifted by 2^64 first (four instructions a row: 131072 x 256 bfloat16 29.8 -> 30.5 us).
+// Against y / scale the codes' quotient carries the roundings of s w, the reciprocal and
+// rstd, a few float32 units: a y that near a tie may fall on its other side.
 template <int COUNT>
 __device__ __forceinline__ float norm_scale(float mean_square, uint32_t top_bits, float &inv, float (&v)[COUNT],
                                             float &ve) {

@@ -23,10 +23,11 @@ The calls are the entry points of include/so3lr_b200.h ("Row-wise feed-forward
 layers") through the compiled module ``so3lr_b200._layers``
 (binding/layers_binding.cpp): they queue kernels on the current torch stream of the
 tensors' GPU and return; outputs and scratch come from torch's allocator. A kernel
-whose wait gives up is reported by the next call on that GPU and by ``check_status``. Rows are
-all leading dimensions; the last dimension must be contiguous, rows may have any
-stride. A refused argument raises ValueError, a failure of the library So3lrError.
-There is no CPU path: a tensor that is not on a GPU is refused.
+whose wait gives up is reported by the next call on that GPU and by ``check_status``.
+Rows are all leading dimensions; the last dimension must be contiguous, rows may have
+any stride. Arguments that do not fit one another raise ValueError; a length or an eps
+outside the library's range, and failures of the library, So3lrError. There is no CPU
+path: a tensor that is not on a GPU is refused.
 """
 from __future__ import annotations
 
@@ -161,7 +162,15 @@ class _FeedForwardFunction(torch.autograd.Function):
 
 def feed_forward(x, w_gate, w_up, w_down):
     """y = (silu(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T, bfloat16 or float16:
-    x [..., width], w_gate and w_up [hidden, width], w_down [width, hidden]."""
+    x [..., width], w_gate and w_up [hidden, width], w_down [width, hidden].
+
+    The hidden layer is rounded to x's type between the products, in calls of few rows
+    (16, or up to 256 through small weights) to two such parts: a row's result can
+    differ in its last bits between calls of few and of many rows. With autograd the
+    operands and the hidden layer are kept, and for widths of 1024 and more and many
+    rows the two projections in float32, 8 bytes for each element of the hidden layer
+    (537 MB for 8190 rows of 8200). The backward pass computes the gradients of all
+    four operands, whichever are asked for."""
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
                                     w_down.requires_grad):
         return _FeedForwardFunction.apply(x, w_gate, w_up, w_down)
@@ -188,7 +197,7 @@ class FeedForwardBlock(torch.nn.Module):
         y, s = rms_norm(x, norm, residual);  out = feed_forward(y, w_gate, w_up, w_down)
 
     forward(x, residual) returns (out, s): the next block adds `out` to the
-    stream `s`. Trains through autograd."""
+    stream `s`. Trains through autograd (see feed_forward for what that keeps)."""
 
     def __init__(self, width: int, hidden: int, *, eps: float = 1e-6, dtype=torch.bfloat16, device="cuda"):
         super().__init__()
