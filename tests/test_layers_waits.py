@@ -1,6 +1,9 @@
 """Bounded waits of the row-wise feed-forward kernels: what a call says when a wait of
 an earlier one has given up."""
 import ctypes as C
+import pathlib
+import subprocess
+import sys
 
 import pytest
 
@@ -173,3 +176,30 @@ def test_the_limit_is_a_waits_and_not_a_kernels(layers):
         finally:
             layers.set_wait_limit()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("call", ["layers.rms_norm(x, w)", "layers.rms_norm_int8(big, w)", "layers.gate_int8(x)",
+                                  "layers.feed_forward(x[:2], m, m, m)", "layers.feed_forward(big, m, m, m)",
+                                  "layers.int8_linear(c, s, c, s)"])
+def test_the_first_call_of_a_process_may_be_captured(call):
+    """It makes the words that waits which give up are reported in, and sets up kernels and tensor maps."""
+    program = f"""
+import torch
+from so3lr_b200 import layers
+x, big, m, w = (torch.randn(n, 1024, device="cuda").bfloat16() for n in (40, 6000, 1024, 1))
+w, c, s = w[0].float(), torch.ones(300, 64, dtype=torch.int8, device="cuda"), torch.ones(300, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = {call}
+graph.replay()
+torch.cuda.synchronize()
+want = {call}
+pairs = zip(got, want) if isinstance(got, tuple) else [(got, want)]
+assert all(torch.equal(a, b) for a, b in pairs)
+layers.check_status()
+print("captured")
+"""
+    root = pathlib.Path(__file__).resolve().parents[1]
+    res = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=120, cwd=root)
+    assert res.returncode == 0 and "captured" in res.stdout, res.stdout + res.stderr
