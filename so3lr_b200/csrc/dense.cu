@@ -193,16 +193,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   const uint32_t drain = bars + 8u * (2 * kMaxStages + 4);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar_mem + 8 * (2 * kMaxStages + 5));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(tc::cluster_rank());
   // for the end after a wait that gave up: K blocks that this CTA has fetched, and (leader) those that have been
   // multiplied and the items whose accumulator is complete
   volatile int *fetched = reinterpret_cast<volatile int *>(tmem_slot + 2);
   volatile int *multiplied = reinterpret_cast<volatile int *>(tmem_slot + 3);
   volatile int *finished = reinterpret_cast<volatile int *>(tmem_slot + 4);
-  auto wait = [&](uint32_t bar, int parity, int where) {
-    return tc::mbar_wait(bar, parity, abort_flag, p.wait.err, where, p.wait.cycles);
+  auto wait = [&](uint32_t bar, int parity, int where) {  // both CTAs learn of one that gives up
+    const bool ok = tc::mbar_wait(bar, parity, abort_flag, p.wait.err, where, p.wait.cycles);
+    if (!ok) tc::store_of_rank(abort_flag, rank ^ 1, 1);
+    return ok;
   };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = int(tc::cluster_rank());
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   // the pair's n-th work item: its divisions and parameter reads are not on the path of every tile
   __shared__ Item table[kItemTable];
@@ -503,10 +505,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   }
   tc::fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) tc::store_of_rank(abort_flag, rank ^ 1, 1);
   tc::cluster_sync();  // neither CTA leaves while the other may still signal it
   tc::fence_after();
-  if (*abort_flag) {
+  if (__builtin_expect(*abort_flag, 0)) {
     // A wait of either CTA gave up. All that the pair has started ends (with a limit) before TMEM is handed back
     // and shared memory is left: copies, MMAs and the signals of both. A K block's barrier completes when both CTAs
     // have fetched their parts, so the CTA that is behind fetches as many (any block of the right size; the release
