@@ -240,41 +240,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   const uint32_t tmem = *tmem_slot;
   wait_for_predecessors();
 
-  // one thread of each CTA: its parts of the pair's n-th K block, which is K block kb of item w
-  auto fetch = [&](int n, const Item &w, int kb) {
-    const Problem &q = p.prob[w.prob];
-    const int s = n % S::kStages;
-    if (rank == 0) tc::mbar_expect_tx(full(s), 2 * S::kStage);
-    const uint32_t bar = tc::at_leader(full(s)), dst = base + s * S::kStage;
-    constexpr int kElems = MODE == kInt8 ? 128 : 64;  // of a K block
-    if (MODE == kGated || MODE == kGatedBack) {
-      const int k = kb * 64;
-      tc::tma_load(dst, &p.map[0], k, w.m0 + 128 * rank, bar);                  // x
-      tc::tma_load(dst + kOperand, &p.map[1 + rank], k, w.n0, bar);             // Wg | Wu
-      if (MODE == kGatedBack) {
-        tc::tma_load(dst + 2 * kOperand, &p.map[3], k, w.m0 + 128 * rank, bar); // dy
-        tc::tma_load(dst + 3 * kOperand, &p.map[4], w.n0 + 64 * rank, k, bar);  // Wd
-      }
-    } else {
-      const int seg = kb >= q.kb0 ? 1 : 0, k = (kb - (seg ? q.kb0 : 0)) * kElems;
-      const CUtensorMap *a = &p.map[q.a[seg]], *b = &p.map[q.b[seg]];
-      const int m = w.m0 + 128 * rank, c = w.n0 + TN / 2 * rank;
-      if (A_MN) {
-        tc::tma_load(dst, a, m, k, bar);
-        tc::tma_load(dst + kOperand / 2, a, m + 64, k, bar);
-      } else {
-        tc::tma_load(dst, a, k, m, bar);
-      }
-      if (B_MN) {
-        tc::tma_load(dst + kOperand, b, c, k, bar);
-        if (TN == 256) tc::tma_load(dst + kOperand + kOperand / 2, b, c + 64, k, bar);
-      } else {
-        tc::tma_load(dst + kOperand, b, k, c, bar);
-      }
-    }
-    *fetched = n + 1;
-  };
-
   if (warp == 0) {
     // ------------------------------------------------------------------- loads
     if (lane == 0) {
@@ -282,10 +247,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       bool ok = true;
       for (int it = 0; it < items && ok; ++it) {
         const Item w = item(it);
+        const Problem &q = p.prob[w.prob];
         for (int kb = w.kb_begin; kb < w.kb_end; ++kb, ++n) {
-          ok = wait(empty(n % S::kStages), ((n / S::kStages) & 1) ^ 1, 1);
+          const int s = n % S::kStages;
+          ok = wait(empty(s), ((n / S::kStages) & 1) ^ 1, 1);
           if (!ok) break;
-          fetch(n, w, kb);
+          if (rank == 0) tc::mbar_expect_tx(full(s), 2 * S::kStage);
+          const uint32_t bar = tc::at_leader(full(s)), dst = base + s * S::kStage;
+          constexpr int kElems = MODE == kInt8 ? 128 : 64;  // of a K block
+          if (MODE == kGated || MODE == kGatedBack) {
+            const int k = kb * 64;
+            tc::tma_load(dst, &p.map[0], k, w.m0 + 128 * rank, bar);                  // x
+            tc::tma_load(dst + kOperand, &p.map[1 + rank], k, w.n0, bar);             // Wg | Wu
+            if (MODE == kGatedBack) {
+              tc::tma_load(dst + 2 * kOperand, &p.map[3], k, w.m0 + 128 * rank, bar); // dy
+              tc::tma_load(dst + 3 * kOperand, &p.map[4], w.n0 + 64 * rank, k, bar);  // Wd
+            }
+          } else {
+            const int seg = kb >= q.kb0 ? 1 : 0, k = (kb - (seg ? q.kb0 : 0)) * kElems;
+            const CUtensorMap *a = &p.map[q.a[seg]], *b = &p.map[q.b[seg]];
+            const int m = w.m0 + 128 * rank, c = w.n0 + TN / 2 * rank;
+            if (A_MN) {
+              tc::tma_load(dst, a, m, k, bar);
+              tc::tma_load(dst + kOperand / 2, a, m + 64, k, bar);
+            } else {
+              tc::tma_load(dst, a, k, m, bar);
+            }
+            if (B_MN) {
+              tc::tma_load(dst + kOperand, b, c, k, bar);
+              if (TN == 256) tc::tma_load(dst + kOperand + kOperand / 2, b, c + 64, k, bar);
+            } else {
+              tc::tma_load(dst + kOperand, b, k, c, bar);
+            }
+          }
+          *fetched = n + 1;
         }
       }
       // every release of a K block has reached this CTA before it may leave
@@ -509,26 +504,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
   tc::fence_after();
   if (__builtin_expect(*abort_flag, 0)) {
     // A wait of either CTA gave up. All that the pair has started ends (with a limit) before TMEM is handed back
-    // and shared memory is left: copies, MMAs and the signals of both. A K block's barrier completes when both CTAs
-    // have fetched their parts, so the CTA that is behind fetches as many (any block of the right size; the release
-    // of their stages has reached the other CTA, so their MMAs are through with both).
+    // and shared memory is left: copies, MMAs and the signals of both. A K block's barrier counts the parts of both
+    // CTAs, so the CTA that is behind answers for the parts that it has not fetched.
+    int all = 0;  // K blocks that either has fetched
     if (threadIdx.x == 0) {
-      const Item w = item(0);
-      const int all = max(*fetched, tc::load_of_rank(fetched, rank ^ 1));
-      for (int n = *fetched; n < all; ++n) fetch(n, w, w.kb_begin);
+      const int mine = *fetched;
+      all = max(mine, tc::load_of_rank(fetched, rank ^ 1));
+#pragma unroll 1
+      for (int n = mine; n < all; ++n) {
+        const uint32_t bar = full(n % S::kStages);
+        if (rank == 0)
+          tc::mbar_expect_tx(bar, S::kStage);
+        else
+          tc::mbar_complete_tx(tc::at_leader(bar), S::kStage);
+      }
     }
     __syncwarp();
     tc::cluster_sync();
     if (threadIdx.x == 0) {
       const long long t0 = clock64();
       const int through = tc::load_of_rank(multiplied, 0), tiles = tc::load_of_rank(finished, 0);
-      if (rank == 0)
-        for (int i = through; i < *fetched; ++i) tc::mbar_settle(full(i % S::kStages), (i / S::kStages) & 1, t0);
-      for (int i = max(0, through - S::kStages); i < through; ++i)
-        tc::mbar_settle(empty(i % S::kStages), (i / S::kStages) & 1, t0);
-      for (int i = max(0, tiles - S::kBuffers); i < tiles; ++i)
-        tc::mbar_settle(acc_full(i % S::kBuffers), (i / S::kBuffers) & 1, t0);
-      tc::mbar_settle(drain, 0, t0);
+      auto settle = [&](uint32_t first, int begin, int end, int ring) {
+#pragma unroll 1
+        for (int i = max(0, begin); i < end; ++i) tc::mbar_settle(first + 8u * (i % ring), (i / ring) & 1, t0);
+      };
+      if (rank == 0) settle(full(0), through, all, S::kStages);
+      settle(empty(0), through - S::kStages, through, S::kStages);
+      settle(acc_full(0), tiles - S::kBuffers, tiles, S::kBuffers);
+      settle(drain, 0, 1, 1);
     }
     __syncwarp();
     tc::cluster_sync();
