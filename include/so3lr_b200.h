@@ -539,6 +539,131 @@ long long so3lr_feed_forward_backward_workspace(const so3lr_feed_forward_backwar
 int so3lr_feed_forward_backward(const so3lr_feed_forward_backward_args *args, void *workspace,
                                 long long workspace_bytes, void *stream, char *err, size_t errlen);
 
+/* The norms on both sides of a block's boundary, width <= 16384: the block's output x is
+ * normalised, gated and added to the scaled residual stream, and the stream is normalised
+ * for the next block,
+ *   s = residual * residual_scale + gate * x * weight / sqrt(mean(x^2) + eps)   (rounded to the element type)
+ *   y = s * next_weight / sqrt(mean(s^2) + eps)
+ * gate is an element for each element of x (a row stride of 0: one gate for all rows), the
+ * weights and residual_scale one for each column; without gate or residual_scale they are 1.
+ * The second norm is of s as stored. Squares are float32, as in so3lr_rms_norm. s and y may
+ * each be the memory of x, residual or gate, row for row (not both the same). */
+typedef struct {
+  long long rows, width;
+  int dtype;                  /* x, residual, gate, s, y */
+  int weight_dtype;           /* weight, next_weight, residual_scale: dtype or SO3LR_FLOAT32 */
+  double eps;                 /* >= 0 */
+  const void *x;
+  long long x_stride;
+  const void *residual;
+  long long residual_stride;
+  const void *gate;           /* optional */
+  long long gate_stride;
+  const void *weight;         /* width */
+  const void *next_weight;    /* width */
+  const void *residual_scale; /* width, optional */
+  void *s;
+  long long s_stride;
+  void *y;
+  long long y_stride;
+} so3lr_sandwich_norm_args;
+int so3lr_sandwich_norm(const so3lr_sandwich_norm_args *args, void *stream, char *err, size_t errlen);
+
+/* Gradients of so3lr_sandwich_norm: with rx, rs the two reciprocal roots, xh = x rx, sh = s rs,
+ *   g = rs (dy next_weight - sh mean(dy next_weight sh)) + ds,   q = g gate
+ *   dx = rx (q weight - xh mean(q weight xh)),  dresidual = g residual_scale,  dgate = g xh weight
+ *   dweight = sum over rows of q xh,  dnext_weight = sum dy sh,  dresidual_scale = sum g residual
+ * ds is the gradient that reaches s directly; optional. Results must not overlap the inputs. */
+typedef struct {
+  long long rows, width;
+  int dtype;
+  int weight_dtype;           /* the weights and their gradients */
+  double eps;
+  const void *dy;
+  long long dy_stride;
+  const void *ds;             /* optional */
+  long long ds_stride;
+  const void *s;              /* from the forward pass */
+  long long s_stride;
+  const void *x;
+  long long x_stride;
+  const void *residual;       /* read with residual_scale only */
+  long long residual_stride;
+  const void *gate;           /* as in the forward pass */
+  long long gate_stride;
+  const void *weight;
+  const void *next_weight;
+  const void *residual_scale; /* as in the forward pass */
+  void *dx;
+  long long dx_stride;
+  void *dresidual;
+  long long dresidual_stride;
+  void *dgate;                /* with gate */
+  long long dgate_stride;
+  void *dweight;
+  void *dnext_weight;
+  void *dresidual_scale;      /* with residual_scale */
+} so3lr_sandwich_norm_backward_args;
+long long so3lr_sandwich_norm_backward_workspace(const so3lr_sandwich_norm_backward_args *args);
+int so3lr_sandwich_norm_backward(const so3lr_sandwich_norm_backward_args *args, void *workspace,
+                                 long long workspace_bytes, void *stream, char *err, size_t errlen);
+
+/* One AdamW step of many tensors at once:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * t is the tensor's step counter, on the GPU, to which the call adds 1: a captured graph
+ * counts its replays. Arithmetic is float32 (the corrections float64). A 16-bit parameter
+ * may have a float32 master, which is then what is updated, and the parameter its rounding;
+ * without one the updated parameter is rounded to its type, so that updates below half a
+ * unit of it are lost.
+ * Moments are float32 or, where the two scale arrays are given, 8 bits: a code for each
+ * element and a float32 scale for each 256 of the tensor (the last of fewer), the largest
+ * magnitude among them:
+ *   m = scale c |c| / 127^2, c int8;   v = scale (c / 255)^4, c uint8
+ * each code rounded to nearest (the share of the scale within a few float32 units, so a
+ * value that near a tie may go either way), that of a v above zero 1 at least. 256 moments
+ * whose largest is below float32's normal numbers get scale 0 and codes 0; 256 that hold an
+ * infinity or a NaN scale NaN and codes 0, so that in 8 bits one such gradient makes 256
+ * moments NaN, for good.
+ * `tensors` is host memory, read before the call returns, and holds device pointers.
+ * Buffers are contiguous and must not overlap; parameters or counters that do are refused. */
+typedef struct {
+  void *param;                /* n */
+  const void *grad;           /* n */
+  float *master;              /* n, or NULL */
+  void *exp_avg;              /* m: n float, or n int8 with scales */
+  void *exp_avg_sq;           /* v: n float, or n uint8 with scales */
+  float *exp_avg_scale;       /* (n + 255) / 256, or NULL */
+  float *exp_avg_sq_scale;
+  long long *step;            /* 1: steps taken so far */
+  long long n;                /* may be 0: the step is counted */
+  int dtype;                  /* param */
+  int grad_dtype;             /* dtype or SO3LR_FLOAT32 */
+} so3lr_adamw_tensor;
+typedef struct {
+  long long count;
+  const so3lr_adamw_tensor *tensors;
+  double lr;                  /* >= 0 */
+  const float *lr_device;     /* optional: read on the GPU instead of lr */
+  double beta1, beta2;        /* in 0..1, below 1 */
+  double eps;                 /* in 1e-30..1e30 */
+  double weight_decay;        /* >= 0 */
+} so3lr_adamw_args;
+long long so3lr_adamw_workspace(const so3lr_adamw_args *args);
+int so3lr_adamw(const so3lr_adamw_args *args, void *workspace, long long workspace_bytes, void *stream, char *err,
+                size_t errlen);
+
+/* What the codes of an 8-bit moment stand for. */
+typedef struct {
+  long long n;
+  int is_signed;              /* exp_avg, else exp_avg_sq */
+  int dtype;
+  const void *codes;          /* n */
+  const float *scales;        /* (n + 255) / 256 */
+  void *values;               /* n, of dtype */
+} so3lr_moment_values_args;
+int so3lr_moment_values(const so3lr_moment_values_args *args, void *stream, char *err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif

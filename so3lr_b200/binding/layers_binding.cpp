@@ -21,6 +21,7 @@
 #include <stdexcept>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "so3lr_b200.h"
 
@@ -46,6 +47,8 @@ const char *name_of(at::ScalarType t) {
     case at::kBFloat16: return "torch.bfloat16";
     case at::kHalf: return "torch.float16";
     case at::kChar: return "torch.int8";
+    case at::kByte: return "torch.uint8";
+    case at::kLong: return "torch.int64";
     default: return c10::toString(t);
   }
 }
@@ -399,6 +402,229 @@ PyObject *feed_forward_backward(Args o) {
   return tuple(wrap(dx), wrap(dwg), wrap(dwu), wrap(dwd));
 }
 
+// x, residual, weight, next_weight, gate | None, residual_scale | None of either sandwich call
+template <class A>
+Rows sandwich_operands(A &a, Args o, PyObject *eps) {
+  const Tensor &x = tensor(o[0], "x"), &residual = tensor(o[1], "residual"), &w = tensor(o[2], "weight");
+  const Rows r = rows_of(x, "x");
+  a.rows = r.rows;
+  a.width = r.width;
+  a.dtype = float_type(r.type, "x");
+  a.eps = number(eps, "eps");
+  a.x = r.data;
+  a.x_stride = r.stride;
+  if (residual.sizes() != x.sizes())
+    refuse("residual must have the shape of x, got ", residual.sizes(), " and ", x.sizes());
+  const Rows q = rows_like(residual, "residual", r, r.type, r.rows, r.width);
+  a.residual = q.data;
+  a.residual_stride = q.stride;
+  a.weight = vector_of(w, "weight", r, r.width, r.type, at::kFloat);
+  a.weight_dtype = w.scalar_type() == at::kFloat ? SO3LR_FLOAT32 : a.dtype;
+  a.next_weight = vector_of(tensor(o[3], "next_weight"), "next_weight", r, r.width, w.scalar_type());
+  if (o[4] != Py_None) {
+    const Tensor &gate = tensor(o[4], "gate");
+    if (gate.sizes() != x.sizes()) refuse("gate must have the shape of x, got ", gate.sizes(), " and ", x.sizes());
+    const Rows g = rows_like(gate, "gate", r, r.type, r.rows, r.width);
+    a.gate = g.data;
+    a.gate_stride = g.stride;
+  }
+  if (o[5] != Py_None)
+    a.residual_scale = vector_of(tensor(o[5], "residual_scale"), "residual_scale", r, r.width, w.scalar_type());
+  return r;
+}
+
+// sandwich_norm(x, residual, weight, next_weight, gate | None, residual_scale | None, eps) -> (y, s)
+PyObject *sandwich_norm(Args o) {
+  so3lr_sandwich_norm_args a{};
+  const Rows r = sandwich_operands(a, o, o[6]);
+  const c10::cuda::CUDAGuard guard(r.device);
+  const Tensor &x = tensor(o[0], "x");
+  Tensor y = empty(x.sizes(), r.type, r.device), s = empty(x.sizes(), r.type, r.device);
+  a.y = y.data_ptr();
+  a.s = s.data_ptr();
+  a.y_stride = a.s_stride = r.width;
+  char err[1024] = "";
+  check(so3lr_sandwich_norm(&a, stream_of(r.device), err, sizeof err), err);
+  return tuple(wrap(y), wrap(s));
+}
+
+// sandwich_norm_backward(x, residual, weight, next_weight, gate | None, residual_scale | None, dy, ds | None, s, eps)
+// -> (dx, dresidual, dweight, dnext_weight, dgate | None, dresidual_scale | None)
+PyObject *sandwich_norm_backward(Args o) {
+  so3lr_sandwich_norm_backward_args a{};
+  const Rows r = sandwich_operands(a, o, o[9]);
+  const c10::cuda::CUDAGuard guard(r.device);
+  const Tensor &x = tensor(o[0], "x"), &w = tensor(o[2], "weight");
+  const Rows d = rows_like(tensor(o[6], "dy"), "dy", r, r.type, r.rows, r.width);
+  a.dy = d.data;
+  a.dy_stride = d.stride;
+  if (o[7] != Py_None) {
+    const Rows e = rows_like(tensor(o[7], "ds"), "ds", r, r.type, r.rows, r.width);
+    a.ds = e.data;
+    a.ds_stride = e.stride;
+  }
+  const Rows s = rows_like(tensor(o[8], "s"), "s", r, r.type, r.rows, r.width);
+  a.s = s.data;
+  a.s_stride = s.stride;
+  Tensor dx = empty(x.sizes(), r.type, r.device), dresidual = empty(x.sizes(), r.type, r.device), dgate, dscale,
+         dw = empty({r.width}, w.scalar_type(), r.device), dnext = empty({r.width}, w.scalar_type(), r.device);
+  a.dx = dx.data_ptr();
+  a.dresidual = dresidual.data_ptr();
+  a.dx_stride = a.dresidual_stride = r.width;
+  a.dweight = dw.data_ptr();
+  a.dnext_weight = dnext.data_ptr();
+  if (o[4] != Py_None) {
+    dgate = empty(x.sizes(), r.type, r.device);
+    a.dgate = dgate.data_ptr();
+    a.dgate_stride = r.width;
+  }
+  if (a.residual_scale) {
+    dscale = empty({r.width}, w.scalar_type(), r.device);
+    a.dresidual_scale = dscale.data_ptr();
+  }
+  with_workspace(a, r.device, so3lr_sandwich_norm_backward_workspace, so3lr_sandwich_norm_backward);
+  return tuple(wrap(dx), wrap(dresidual), wrap(dw), wrap(dnext), dgate.defined() ? wrap(dgate) : none(),
+               dscale.defined() ? wrap(dscale) : none());
+}
+
+// A list of tensors (or of None) as borrowed references; the list object must outlive it
+struct List {
+  PyObject *fast;
+  List(PyObject *o, const char *what) : fast(PySequence_Fast(o, "")) {
+    if (!fast) {
+      PyErr_Clear();
+      refuse(what, " must be a list of tensors");
+    }
+  }
+  ~List() { Py_DECREF(fast); }
+  List(const List &) = delete;
+  Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(fast); }
+  PyObject *operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(fast, i); }
+};
+// one tensor of a list, contiguous, with `n` elements of one of two types
+const Tensor &element(const List &list, Py_ssize_t i, const char *what, c10::Device device, int64_t n,
+                      at::ScalarType type, std::optional<at::ScalarType> or_type = std::nullopt) {
+  const Tensor &t = tensor(list[i], what);
+  if (t.layout() != at::kStrided) refuse(what, "[", i, "] must be a dense tensor");
+  if (t.device() != device) refuse(what, "[", i, "] is on ", t.device().str(), ", the other tensors are on ", device.str());
+  if (t.scalar_type() != type && t.scalar_type() != or_type)
+    refuse(what, "[", i, "] must be ", name_of(type), or_type ? " or " : "", or_type ? name_of(*or_type) : "", ", got ",
+           name_of(t.scalar_type()));
+  if (t.numel() != n) refuse(what, "[", i, "] must have ", n, " elements, got ", t.numel());
+  if (!t.is_contiguous()) refuse(what, "[", i, "] must be contiguous");
+  return t;
+}
+
+constexpr int64_t kScaleBlock = 256;
+
+// adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales | None, exp_avg_sq_scales | None,
+//            masters | None, lr, beta1, beta2, eps, weight_decay) -> None
+PyObject *adamw_step(Args o) {
+  const List params(o[0], "params"), grads(o[1], "grads"), ms(o[2], "exp_avgs"), vs(o[3], "exp_avg_sqs");
+  const Py_ssize_t count = params.size();
+  std::optional<List> m_scales, v_scales, masters, counters;
+  if (o[5] != Py_None) m_scales.emplace(o[5], "exp_avg_scales");
+  if (o[6] != Py_None) v_scales.emplace(o[6], "exp_avg_sq_scales");
+  if (o[7] != Py_None) masters.emplace(o[7], "masters");
+  if (!THPVariable_Check(o[4])) counters.emplace(o[4], "steps");
+  auto same = [&](const List &l, const char *what) {
+    if (l.size() != count) refuse(what, " must have as many tensors as params, ", count, ", got ", l.size());
+  };
+  same(grads, "grads");
+  same(ms, "exp_avgs");
+  same(vs, "exp_avg_sqs");
+  if (m_scales) same(*m_scales, "exp_avg_scales");
+  if (v_scales) same(*v_scales, "exp_avg_sq_scales");
+  if (masters) same(*masters, "masters");
+  if (counters) same(*counters, "steps");
+  so3lr_adamw_args a{};
+  a.beta1 = number(o[9], "betas");
+  a.beta2 = number(o[10], "betas");
+  a.eps = number(o[11], "eps");
+  a.weight_decay = number(o[12], "weight_decay");
+  a.count = count;
+  if (count == 0) return none();
+  const Tensor &first = tensor(params[0], "params");
+  const c10::Device device = first.device();
+  if (!first.is_cuda()) refuse("params must be on a CUDA device, got ", device.str(), " (there is no CPU path)");
+  const c10::cuda::CUDAGuard guard(device);
+  if (THPVariable_Check(o[8])) {
+    const Tensor &lr = tensor(o[8], "lr");
+    if (lr.device() != device || lr.scalar_type() != at::kFloat || lr.numel() != 1)
+      refuse("lr must be a number or a torch.float32 tensor of one element on ", device.str());
+    a.lr_device = static_cast<const float *>(lr.data_ptr());
+  } else {
+    a.lr = number(o[8], "lr");
+  }
+  long long *steps = nullptr;
+  if (!counters) {
+    const Tensor &t = tensor(o[4], "steps");
+    if (t.dim() != 1 || t.size(0) != count || t.device() != device || t.scalar_type() != at::kLong || !t.is_contiguous())
+      refuse("steps must be a contiguous 1-D torch.int64 tensor of ", count, " elements on ", device.str(),
+             ", or a list of tensors of one");
+    steps = reinterpret_cast<long long *>(t.data_ptr());
+  }
+  std::vector<so3lr_adamw_tensor> tensors(count);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    so3lr_adamw_tensor &e = tensors[i];
+    const Tensor &p = tensor(params[i], "params");
+    e.n = p.numel();
+    const at::ScalarType t = p.scalar_type();
+    e.dtype = float_type(t, "params");
+    e.param = element(params, i, "params", device, e.n, t).data_ptr();
+    const Tensor &g = element(grads, i, "grads", device, e.n, t, at::kFloat);
+    e.grad = g.data_ptr();
+    e.grad_dtype = g.scalar_type() == at::kFloat ? SO3LR_FLOAT32 : e.dtype;
+    const bool eight = m_scales && (*m_scales)[i] != Py_None;
+    if (eight != (v_scales && (*v_scales)[i] != Py_None))
+      refuse("exp_avg_scales[", i, "] and exp_avg_sq_scales[", i, "] must be given together");
+    e.exp_avg = element(ms, i, "exp_avgs", device, e.n, eight ? at::kChar : at::kFloat).data_ptr();
+    e.exp_avg_sq = element(vs, i, "exp_avg_sqs", device, e.n, eight ? at::kByte : at::kFloat).data_ptr();
+    if (eight) {
+      const int64_t blocks = (e.n + kScaleBlock - 1) / kScaleBlock;
+      e.exp_avg_scale = static_cast<float *>(element(*m_scales, i, "exp_avg_scales", device, blocks, at::kFloat).data_ptr());
+      e.exp_avg_sq_scale =
+          static_cast<float *>(element(*v_scales, i, "exp_avg_sq_scales", device, blocks, at::kFloat).data_ptr());
+    }
+    if (masters && (*masters)[i] != Py_None)
+      e.master = static_cast<float *>(element(*masters, i, "masters", device, e.n, at::kFloat).data_ptr());
+    e.step = counters ? reinterpret_cast<long long *>(element(*counters, i, "steps", device, 1, at::kLong).data_ptr())
+                      : steps + i;
+  }
+  a.tensors = tensors.data();
+  with_workspace(a, device, so3lr_adamw_workspace, so3lr_adamw);
+  // what autograd has kept of the parameters for a backward pass to come is no longer what it was
+  for (Py_ssize_t i = 0; i < count; ++i)
+    if (const Tensor &p = THPVariable_Unpack(params[i]); !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  return none();
+}
+
+// moment_values(codes, scales, dtype) -> values
+PyObject *moment_values(Args o) {
+  const Tensor &codes = tensor(o[0], "codes"), &scales = tensor(o[1], "scales");
+  if (!codes.is_cuda()) refuse("codes must be on a CUDA device, got ", codes.device().str(), " (there is no CPU path)");
+  if (codes.scalar_type() != at::kChar && codes.scalar_type() != at::kByte)
+    refuse("codes must be torch.int8 or torch.uint8, got ", name_of(codes.scalar_type()));
+  if (!codes.is_contiguous()) refuse("codes must be contiguous");
+  const int64_t blocks = (codes.numel() + kScaleBlock - 1) / kScaleBlock;
+  if (scales.device() != codes.device() || scales.scalar_type() != at::kFloat || scales.numel() != blocks ||
+      !scales.is_contiguous())
+    refuse("scales must be a contiguous torch.float32 tensor of ", blocks, " elements on ", codes.device().str());
+  const c10::cuda::CUDAGuard guard(codes.device());
+  const at::ScalarType out = dtype_of(o[2], "dtype");
+  so3lr_moment_values_args a{};
+  a.n = codes.numel();
+  a.is_signed = codes.scalar_type() == at::kChar;
+  a.dtype = float_type(out, "dtype");
+  a.codes = codes.data_ptr();
+  a.scales = static_cast<const float *>(scales.data_ptr());
+  Tensor y = empty(codes.sizes(), out, codes.device());
+  a.values = y.data_ptr();
+  char err[1024] = "";
+  check(so3lr_moment_values(&a, stream_of(codes.device()), err, sizeof err), err);
+  return wrap(y);
+}
+
 // status(device index) -> None
 PyObject *status(Args o) {
   const c10::cuda::CUDAGuard guard(c10::Device(c10::kCUDA, c10::DeviceIndex(PyLong_AsLong(o[0]))));
@@ -446,7 +672,9 @@ PyObject *method(PyObject *, PyObject *const *args, Py_ssize_t n) {
   { #f, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&method<f, n>)), METH_FASTCALL, nullptr }
 PyMethodDef g_methods[] = {METHOD(rms_norm, 5),        METHOD(rms_norm_backward, 5), METHOD(int8_linear, 6),
                            METHOD(gate_int8, 1),       METHOD(dequantize_int8, 3),   METHOD(feed_forward, 5),
-                           METHOD(feed_forward_backward, 7), METHOD(status, 1), METHOD(set_wait_limit, 1), {nullptr, nullptr, 0, nullptr}};
+                           METHOD(feed_forward_backward, 7), METHOD(sandwich_norm, 7),
+                           METHOD(sandwich_norm_backward, 10), METHOD(adamw_step, 13),
+                           METHOD(moment_values, 3),   METHOD(status, 1), METHOD(set_wait_limit, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_layers", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

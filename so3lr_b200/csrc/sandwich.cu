@@ -1,0 +1,495 @@
+// The norms on both sides of a block's boundary, in one pass over the rows:
+//
+//   s = residual scale + gate norm(x) weight,  y = norm(s) next_weight
+//   norm(v) = v / sqrt(mean(v^2) + eps), of s as stored
+//
+// and their gradients: with rx, rs the reciprocal roots, xh = x rx, sh = s rs,
+//
+//   g = rs (dy next_weight - sh mean(dy next_weight sh)) + ds,  dnext_weight = sum dy sh
+//   dresidual = g scale,  dscale = sum g residual,  dgate = g xh weight
+//   q = g gate,  dweight = sum q xh,  dx = rx (q weight - xh mean(q weight xh))
+//
+// Bound by HBM: the forward pass moves 5 elements for each of a row, the backward pass 9;
+// apart, the two norms, the gate and the sums would move 11 and 20. A row belongs to
+// lanes of a warp or to a block as in rows.cu. The backward kernels walk over their rows
+// and hold the three column sums; each block writes one row of them, and k_column_sums
+// adds those in order.
+#include "row_team.cuh"
+
+namespace so3lr_b200 {
+namespace {
+
+template <class T, class W>
+struct SandwichRow {  // pointers to one row
+  const T *x, *residual, *gate;
+  T *s, *y;
+  __device__ SandwichRow(const so3lr_sandwich_norm_args &a, long long row)
+      : x(static_cast<const T *>(a.x) + row * a.x_stride),
+        residual(static_cast<const T *>(a.residual) + row * a.residual_stride),
+        gate(a.gate ? static_cast<const T *>(a.gate) + row * a.gate_stride : nullptr),
+        s(static_cast<T *>(a.s) + row * a.s_stride),
+        y(static_cast<T *>(a.y) + row * a.y_stride) {}
+};
+
+template <class T, class W, int VEC, int N, int LANES, bool SHIFT>
+__global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
+    k_sandwich(const so3lr_sandwich_norm_args a, const float inv_width, const float eps) {
+  __shared__ float slot[2][32];
+  dependents_may_start();
+  wait_for_predecessors();
+  const RowTeam<LANES> team;
+  bool live;
+  const SandwichRow<T, W> row(a, team_row<LANES>(a.rows, live));
+  const W *w = static_cast<const W *>(a.weight), *next = static_cast<const W *>(a.next_weight),
+          *scale = static_cast<const W *>(a.residual_scale);
+  const Span<SHIFT, VEC> span(row.x, int(a.width), team.t);
+  Chunk<T, VEC> cx[N], cr[N], cg[N];
+  T ex{}, er{}, eg{};
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) {
+      cx[j] = load_chunk<T, VEC>(row.x + c);
+      cr[j] = load_chunk<T, VEC>(row.residual + c);
+      if (row.gate) cg[j] = load_chunk<T, VEC>(row.gate + c);
+    }
+  }
+  if (span.edge >= 0) {
+    ex = row.x[span.edge];
+    er = row.residual[span.edge];
+    if (row.gate) eg = row.gate[span.edge];
+  }
+  float sq = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (span.holds(span.at(j * team.size + team.t)))
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
+  sq = fmaf(to_float(ex), to_float(ex), sq);
+  const float rx = rsqrtf(fmaf(team.sum(sq, slot[0]), inv_width, eps));
+  // what is kept of the stream is rounded, and the second norm is of what is kept
+  auto stream = [&](T x, T r, T g, W wi, int c) {
+    const float added = to_float(x) * rx * to_float(wi), kept = to_float(r);
+    return fmaf(row.gate ? to_float(g) : 1.0f, added, scale ? kept * to_float(scale[c]) : kept);
+  };
+  sq = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) {
+      const Chunk<W, VEC> cw = load_apart<SHIFT, W, VEC>(w + c);
+      float f[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[i] = stream(cx[j].e[i], cr[j].e[i], cg[j].e[i], cw.e[i], c + i);
+      cx[j] = to_chunk<T, VEC>(f);
+      if (live) store_chunk<T, VEC>(row.s + c, cx[j]);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
+    }
+  }
+  if (span.edge >= 0) {
+    ex = from_float<T>(stream(ex, er, eg, w[span.edge], span.edge));
+    if (live) row.s[span.edge] = ex;
+    sq = fmaf(to_float(ex), to_float(ex), sq);
+  }
+  const float rs = rsqrtf(fmaf(team.sum(sq, slot[1]), inv_width, eps));
+  if (!live) return;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = span.at(j * team.size + team.t);
+    if (span.holds(c)) {
+      const Chunk<W, VEC> cn = load_apart<SHIFT, W, VEC>(next + c);
+      float f[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[i] = to_float(cx[j].e[i]) * rs * to_float(cn.e[i]);
+      store_chunk<T, VEC>(row.y + c, to_chunk<T, VEC>(f));
+    }
+  }
+  if (span.edge >= 0) row.y[span.edge] = from_float<T>(to_float(ex) * rs * to_float(next[span.edge]));
+}
+
+template <class T, class W>
+struct SandwichBackRow {
+  const T *dy, *ds, *s, *x, *residual, *gate;
+  T *dx, *dresidual, *dgate;
+  __device__ SandwichBackRow(const so3lr_sandwich_norm_backward_args &a, long long row)
+      : dy(static_cast<const T *>(a.dy) + row * a.dy_stride),
+        ds(a.ds ? static_cast<const T *>(a.ds) + row * a.ds_stride : nullptr),
+        s(static_cast<const T *>(a.s) + row * a.s_stride),
+        x(static_cast<const T *>(a.x) + row * a.x_stride),
+        residual(a.residual_scale ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr),
+        gate(a.gate ? static_cast<const T *>(a.gate) + row * a.gate_stride : nullptr),
+        dx(static_cast<T *>(a.dx) + row * a.dx_stride),
+        dresidual(static_cast<T *>(a.dresidual) + row * a.dresidual_stride),
+        dgate(a.gate ? static_cast<T *>(a.dgate) + row * a.dgate_stride : nullptr) {}
+};
+// One element of the gradient, all in float32. The row's first statistics give g and what
+// follows from it; its last one, sum(a x), is there after them.
+struct SandwichElement {
+  float dres, dgate, a, sum_w, sum_next, sum_scale;
+  __device__ __forceinline__ SandwichElement(float x, float s, float dy, float ds, float r, float gate, float w,
+                                             float next, float scale, float rx, float rs, float back) {
+    const float g = fmaf(dy * next, rs, fmaf(s, back, ds)), xh = x * rx, q = g * gate;
+    dres = g * scale;
+    dgate = g * (xh * w);
+    a = q * w;
+    sum_w = q * xh;
+    sum_next = dy * (s * rs);
+    sum_scale = g * r;
+  }
+};
+
+// Rows in registers, 8 or 16 elements a thread.
+template <class T, class W, int VEC, int N, int LANES, bool SHIFT>
+__global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N == 8 ? 2 : 1)
+    k_sandwich_backward(const so3lr_sandwich_norm_backward_args a, float *partial, const float inv_width,
+                        const float eps) {
+  __shared__ float2 slot2[32];
+  __shared__ float slot[2][32];
+  extern __shared__ float column[];  // LANES: teams x width
+  dependents_may_start();
+  wait_for_predecessors();
+  const RowTeam<LANES> team;
+  const int width = int(a.width);
+  constexpr int kTeams = LANES ? kTeamThreads / (LANES ? LANES : 1) : 1;
+  const int team_id = LANES ? threadIdx.x / (LANES ? LANES : 1) : 0;
+  // SHIFT: the grid's rows a step are a multiple of 8, so that a team's rows share their span
+  const Span<SHIFT, VEC> span(static_cast<const T *>(a.s) + ((long long)blockIdx.x * kTeams + team_id) * a.s_stride,
+                              width, team.t);
+  const W *w = static_cast<const W *>(a.weight), *next = static_cast<const W *>(a.next_weight),
+          *scale = static_cast<const W *>(a.residual_scale);
+  float sums[3][N * VEC] = {}, edge_sums[3] = {};
+  // whole blocks walk together; a team past the last row adds nothing
+  for (long long first = (long long)blockIdx.x * kTeams; first < a.rows; first += (long long)gridDim.x * kTeams) {
+    const bool live = first + team_id < a.rows;
+    const SandwichBackRow<T, W> row(a, live ? first + team_id : a.rows - 1);
+    Chunk<T, VEC> cs[N], cd[N], ce[N], cx[N], cr[N], cg[N];
+    T es{}, ed{}, ee{}, ex{}, er{}, eg{};
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = span.at(j * team.size + team.t);
+      cs[j] = cd[j] = ce[j] = cx[j] = cr[j] = cg[j] = Chunk<T, VEC>{};
+      if (live && span.holds(c)) {
+        cs[j] = load_chunk<T, VEC>(row.s + c);
+        cd[j] = load_chunk<T, VEC>(row.dy + c);
+        cx[j] = load_chunk<T, VEC>(row.x + c);
+        if (row.ds) ce[j] = load_chunk<T, VEC>(row.ds + c);
+        if (row.residual) cr[j] = load_chunk<T, VEC>(row.residual + c);
+        if (row.gate) cg[j] = load_chunk<T, VEC>(row.gate + c);
+      }
+    }
+    const bool edge = live && span.edge >= 0;
+    if (edge) {
+      es = row.s[span.edge];
+      ed = row.dy[span.edge];
+      ex = row.x[span.edge];
+      if (row.ds) ee = row.ds[span.edge];
+      if (row.residual) er = row.residual[span.edge];
+      if (row.gate) eg = row.gate[span.edge];
+    }
+    float sx = 0.0f, ss = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = span.at(j * team.size + team.t);
+      if (span.holds(c)) {
+        const Chunk<W, VEC> cn = load_apart<SHIFT, W, VEC>(next + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float f = to_float(cs[j].e[i]), x = to_float(cx[j].e[i]);
+          sx = fmaf(x, x, sx);
+          ss = fmaf(f, f, ss);
+          dot = fmaf(f, to_float(cd[j].e[i]) * to_float(cn.e[i]), dot);
+        }
+      }
+    }
+    if (edge) {
+      sx = fmaf(to_float(ex), to_float(ex), sx);
+      ss = fmaf(to_float(es), to_float(es), ss);
+      dot = fmaf(to_float(es), to_float(ed) * to_float(next[span.edge]), dot);
+    }
+    const float2 total = team.sum2(ss, dot, slot2);
+    const float rx = rsqrtf(fmaf(team.sum(sx, slot[0]), inv_width, eps));
+    const float rs = rsqrtf(fmaf(total.x, inv_width, eps));
+    const float back = -(total.y * rs * inv_width) * rs * rs;
+    float av[N * VEC], ae = 0.0f, last = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = span.at(j * team.size + team.t);
+      if (span.holds(c)) {
+        const Chunk<W, VEC> cw = load_apart<SHIFT, W, VEC>(w + c), cn = load_apart<SHIFT, W, VEC>(next + c);
+        Chunk<W, VEC> cc{};
+        if (scale) cc = load_apart<SHIFT, W, VEC>(scale + c);
+        float dres[VEC], dgate[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float x = to_float(cx[j].e[i]);
+          const SandwichElement e(x, to_float(cs[j].e[i]), to_float(cd[j].e[i]), to_float(ce[j].e[i]),
+                                  to_float(cr[j].e[i]), row.gate ? to_float(cg[j].e[i]) : 1.0f, to_float(cw.e[i]),
+                                  to_float(cn.e[i]), scale ? to_float(cc.e[i]) : 1.0f, rx, rs, back);
+          dres[i] = e.dres;
+          dgate[i] = e.dgate;
+          av[j * VEC + i] = e.a;
+          last = fmaf(e.a, x, last);
+          if (live) {
+            sums[0][j * VEC + i] += e.sum_w;
+            sums[1][j * VEC + i] += e.sum_next;
+            sums[2][j * VEC + i] += e.sum_scale;
+          }
+        }
+        if (live) {
+          store_chunk<T, VEC>(row.dresidual + c, to_chunk<T, VEC>(dres));
+          if (row.dgate) store_chunk<T, VEC>(row.dgate + c, to_chunk<T, VEC>(dgate));
+        }
+      }
+    }
+    if (edge) {
+      const int c = span.edge;
+      const SandwichElement e(to_float(ex), to_float(es), to_float(ed), to_float(ee), to_float(er),
+                              row.gate ? to_float(eg) : 1.0f, to_float(w[c]), to_float(next[c]),
+                              scale ? to_float(scale[c]) : 1.0f, rx, rs, back);
+      row.dresidual[c] = from_float<T>(e.dres);
+      if (row.dgate) row.dgate[c] = from_float<T>(e.dgate);
+      ae = e.a;
+      last = fmaf(ae, to_float(ex), last);
+      edge_sums[0] += e.sum_w;
+      edge_sums[1] += e.sum_next;
+      edge_sums[2] += e.sum_scale;
+    }
+    const float back_x = -(team.sum(last, slot[1]) * rx * inv_width) * rx * rx;
+    if (!live) continue;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = span.at(j * team.size + team.t);
+      if (span.holds(c)) {
+        float dx[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) dx[i] = fmaf(av[j * VEC + i], rx, to_float(cx[j].e[i]) * back_x);
+        store_chunk<T, VEC>(row.dx + c, to_chunk<T, VEC>(dx));
+      }
+    }
+    if (edge) row.dx[span.edge] = from_float<T>(fmaf(ae, rx, to_float(ex) * back_x));
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    float *mine = partial + ((size_t)blockIdx.x * 3 + k) * width;
+    float *out = LANES ? column + team_id * width : mine;
+    if (LANES) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = span.at(j * team.size + team.t);
+      if (span.holds(c))
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[c + i] = sums[k][j * VEC + i];
+    }
+    if (span.edge >= 0) out[span.edge] = edge_sums[k];
+    if (!LANES) continue;
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += blockDim.x) {
+      float total = 0.0f;
+#pragma unroll
+      for (int t = 0; t < kTeams; ++t) total += column[t * width + c];
+      mine[c] = total;
+    }
+  }
+}
+
+// Any row, a block each: elements are read again for each statistic (from L2, mostly), the
+// column sums stand in shared memory.
+template <class T, class W>
+__global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sandwich_norm_backward_args a,
+                                                                float *partial, const float inv_width,
+                                                                const float eps) {
+  __shared__ float2 slot2[32];
+  __shared__ float slot[2][32];
+  extern __shared__ float column[];  // 3 x width
+  dependents_may_start();
+  wait_for_predecessors();
+  const RowTeam<0> team;
+  const int width = int(a.width);
+  const W *w = static_cast<const W *>(a.weight), *next = static_cast<const W *>(a.next_weight),
+          *scale = static_cast<const W *>(a.residual_scale);
+  for (int c = team.t; c < 3 * width; c += team.size) column[c] = 0.0f;
+  __syncthreads();
+  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const SandwichBackRow<T, W> row(a, r);
+    float sx = 0.0f, ss = 0.0f, dot = 0.0f;
+#pragma unroll 4
+    for (int c = team.t; c < width; c += team.size) {
+      const float x = to_float(row.x[c]), s = to_float(row.s[c]);
+      sx = fmaf(x, x, sx);
+      ss = fmaf(s, s, ss);
+      dot = fmaf(s, to_float(row.dy[c]) * to_float(next[c]), dot);
+    }
+    const float2 total = team.sum2(ss, dot, slot2);
+    const float rx = rsqrtf(fmaf(team.sum(sx, slot[0]), inv_width, eps));
+    const float rs = rsqrtf(fmaf(total.x, inv_width, eps));
+    const float back = -(total.y * rs * inv_width) * rs * rs;
+    auto element = [&](int c) {
+      return SandwichElement(to_float(row.x[c]), to_float(row.s[c]), to_float(row.dy[c]),
+                             row.ds ? to_float(row.ds[c]) : 0.0f, row.residual ? to_float(row.residual[c]) : 0.0f,
+                             row.gate ? to_float(row.gate[c]) : 1.0f, to_float(w[c]), to_float(next[c]),
+                             scale ? to_float(scale[c]) : 1.0f, rx, rs, back);
+    };
+    float last = 0.0f;
+#pragma unroll 2
+    for (int c = team.t; c < width; c += team.size) {
+      const SandwichElement e = element(c);
+      row.dresidual[c] = from_float<T>(e.dres);
+      if (row.dgate) row.dgate[c] = from_float<T>(e.dgate);
+      last = fmaf(e.a, to_float(row.x[c]), last);
+      column[c] += e.sum_w;
+      column[width + c] += e.sum_next;
+      column[2 * width + c] += e.sum_scale;
+    }
+    const float back_x = -(team.sum(last, slot[1]) * rx * inv_width) * rx * rx;
+#pragma unroll 2
+    for (int c = team.t; c < width; c += team.size)
+      row.dx[c] = from_float<T>(fmaf(element(c).a, rx, to_float(row.x[c]) * back_x));
+  }
+  for (int c = team.t; c < 3 * width; c += team.size) partial[(size_t)blockIdx.x * 3 * width + c] = column[c];
+}
+
+// Column sums of `partial` (nparts x 3 x width) in a fixed order, one output for each y of the grid
+template <class W>
+struct Sums {
+  W *out[3];
+};
+template <class W>
+__global__ void k_column_sums(int nparts, int width, const float *partial, const Sums<W> sums) {
+  __shared__ float part[32][33];
+  dependents_may_start();
+  wait_for_predecessors();
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float total = 0.0f;
+  if (c < width)
+#pragma unroll 8
+    for (int k = threadIdx.y; k < nparts; k += 32) total += partial[((size_t)k * 3 + blockIdx.y) * width + c];
+  part[threadIdx.y][threadIdx.x] = total;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < width) {
+    total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) total += part[k][threadIdx.x];
+    sums.out[blockIdx.y][c] = from_float<W>(total);
+  }
+}
+
+// -------------------------------------------------------------------- dispatch
+// How a row is held, lanes of a warp (0: a block) and elements a thread. The backward pass
+// holds rows of up to 4096 elements; per = 0: longer ones.
+constexpr Hold sandwich_hold(long long width, Path path, int size, bool backward) {
+  if (path != kScalar) {
+    // rows off the boundaries: their edges take up to 2 (16 / size - 1) threads
+    if (width <= 64 && (path == kWide || size == 4)) return {8, 8};
+    if (width <= 128) return {16, 8};
+  }
+  if (width <= 512) return {32, width <= 256 ? 8 : 16};
+  if (backward && width > 4096) return {0, 0};
+  return {0, width <= 8192 ? 8 : 16};
+}
+template <class F>
+void by_sandwich_hold(const Hold &h, F &&f) {
+  using std::integral_constant;
+  if (h.lanes == 8) return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+  if (h.lanes == 16) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  if (h.lanes == 32 && h.per == 8) return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+  if (h.lanes == 32) return f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  if (h.per == 8) return f(integral_constant<int, 0>{}, integral_constant<int, 8>{});
+  return f(integral_constant<int, 0>{}, integral_constant<int, 16>{});
+}
+
+struct BackPlan {
+  Path path;
+  Hold hold;
+  int grid, threads;
+};
+BackPlan back_plan(const so3lr_sandwich_norm_backward_args &a) {
+  RowTensors t{a.dtype == SO3LR_FLOAT32 ? 4 : 2};
+  t.add(a.dy, a.dy_stride);
+  t.add(a.ds, a.ds_stride);
+  t.add(a.s, a.s_stride);
+  t.add(a.x, a.x_stride);
+  if (a.residual_scale) t.add(a.residual, a.residual_stride);
+  t.add(a.gate, a.gate_stride);
+  t.add(a.dx, a.dx_stride);
+  t.add(a.dresidual, a.dresidual_stride);
+  t.add(a.dgate, a.dgate_stride);
+  BackPlan p;
+  p.path = t.path(a.width, aligned(a.weight, 0, 1, 16) && aligned(a.next_weight, 0, 1, 16) &&
+                               aligned(a.residual_scale, 0, 1, 16));
+  p.hold = sandwich_hold(a.width, p.path, t.size, true);
+  if (p.hold.per == 0) {
+    p.threads = 512;
+    p.grid = int(std::min<long long>(a.rows, kSmCount));
+    return p;
+  }
+  p.threads = p.hold.lanes ? kTeamThreads : row_threads(a.width, p.hold.per);
+  const int per_sm = p.hold.lanes ? 2 : std::max(1, 512 / p.threads);
+  p.grid = int(std::min<long long>(team_grid(p.hold, a.rows).x, (long long)kSmCount * per_sm));
+  if (p.path == kShifted && p.hold.lanes == 0) p.grid = (p.grid + 7) / 8 * 8;
+  return p;
+}
+
+}  // namespace
+
+void launch_sandwich_norm(const so3lr_sandwich_norm_args &a, cudaStream_t s) {
+  by_type(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    by_weight<T>(a.dtype, a.weight_dtype, [&](auto w) {
+      using W = decltype(w);
+      RowTensors t{int(sizeof(T))};
+      t.add(a.x, a.x_stride);
+      t.add(a.residual, a.residual_stride);
+      t.add(a.gate, a.gate_stride);
+      t.add(a.s, a.s_stride);
+      t.add(a.y, a.y_stride);
+      by_path(t.path(a.width, aligned(a.weight, 0, 1, 16) && aligned(a.next_weight, 0, 1, 16)), [&](auto path) {
+        constexpr Path PATH = decltype(path)::value;
+        constexpr int VEC = chunk_of(PATH, sizeof(T));
+        const Hold h = sandwich_hold(a.width, PATH, sizeof(T), false);
+        by_sandwich_hold(h, [&](auto lanes, auto per) {
+          constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
+          launch(k_sandwich<T, W, VEC, N, L, PATH == kShifted>, team_grid(h, a.rows), team_block(h, a.width), 0, s, a,
+                 1.0f / float(a.width), float(a.eps));
+        });
+      });
+    });
+  });
+}
+
+long long sandwich_norm_backward_bytes(const so3lr_sandwich_norm_backward_args &a) {
+  return (long long)back_plan(a).grid * 3 * a.width * 4;
+}
+
+void launch_sandwich_norm_backward(const so3lr_sandwich_norm_backward_args &a, void *workspace, cudaStream_t s) {
+  by_type(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    by_weight<T>(a.dtype, a.weight_dtype, [&](auto w) {
+      using W = decltype(w);
+      const BackPlan p = back_plan(a);
+      float *partial = static_cast<float *>(workspace);
+      const float inv = 1.0f / float(a.width), eps = float(a.eps);
+      if (p.grid > 0 && p.hold.per == 0) {
+        allow_dynamic_smem(reinterpret_cast<const void *>(&k_sandwich_backward_long<T, W>), 3 * 16384 * sizeof(float));
+        launch(k_sandwich_backward_long<T, W>, p.grid, p.threads, 3 * a.width * sizeof(float), s, a, partial, inv, eps);
+      } else if (p.grid > 0) {
+        by_path(p.path, [&](auto path) {
+          constexpr Path PATH = decltype(path)::value;
+          constexpr int VEC = chunk_of(PATH, sizeof(T));
+          by_sandwich_hold(p.hold, [&](auto lanes, auto per) {
+            constexpr int L = decltype(lanes)::value, P = decltype(per)::value, N = P / VEC;
+            if constexpr (L != 0 || P == 8)
+              launch(k_sandwich_backward<T, W, VEC, N, L, PATH == kShifted>, p.grid, p.threads,
+                     L ? kTeamThreads / (L ? L : 1) * a.width * sizeof(float) : 0, s, a, partial, inv, eps);
+          });
+        });
+      }
+      const Sums<W> sums{{static_cast<W *>(a.dweight), static_cast<W *>(a.dnext_weight),
+                          static_cast<W *>(a.dresidual_scale)}};
+      launch(k_column_sums<W>, dim3(unsigned((a.width + 31) / 32), a.residual_scale ? 3 : 2), dim3(32, 32), 0, s,
+             p.grid, int(a.width), partial, sums);
+    });
+  });
+}
+
+}  // namespace so3lr_b200

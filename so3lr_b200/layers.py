@@ -42,7 +42,7 @@ except (ImportError, So3lrError) as e:
     raise ImportError(f"the feed-forward layers' module is missing or does not fit the installed torch ({e}): build it "
                       "with `python -m so3lr_b200.build`, which needs a torch with CUDA and Python's headers") from e
 
-__all__ = ["rms_norm", "rms_norm_int8", "rms_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
+__all__ = ["rms_norm", "rms_norm_int8", "rms_norm_backward", "sandwich_norm", "sandwich_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
            "quantize_weight", "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock",
            "Int8FeedForwardBlock", "check_status", "set_wait_limit"]
 
@@ -112,6 +112,52 @@ def rms_norm_backward(dy, s, weight, ds=None, *, eps: float = 1e-6):
     """(dx, dweight) of rms_norm for the gradient dy of y and, optionally, ds that
     of s; dx is also the residual's gradient."""
     return _layers.rms_norm_backward(dy, s, weight, ds, eps)
+
+
+# --------------------------------------------------- norms on both sides of a block
+class _SandwichFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, next_weight, gate, residual_scale, eps):
+        y, s = _layers.sandwich_norm(x, residual, weight, next_weight, gate, residual_scale, eps)
+        ctx.set_materialize_grads(False)  # an output that nothing reads has no gradient, rather than zeros
+        ctx.save_for_backward(x, residual, weight, next_weight, gate, residual_scale, s)
+        ctx.eps = eps
+        return y, s
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, ds):
+        if dy is None and ds is None:
+            return (None,) * 7
+        *operands, s = ctx.saved_tensors
+        dy = torch.zeros_like(s) if dy is None else _dense_rows(dy)
+        dx, dresidual, dweight, dnext, dgate, dscale = _layers.sandwich_norm_backward(*operands, dy, _dense_rows(ds), s,
+                                                                                      ctx.eps)
+        return dx, dresidual, dweight, dnext, dgate, dscale, None
+
+
+def sandwich_norm(x, residual, weight, next_weight, gate=None, residual_scale=None, *, eps: float = 1e-6):
+    """(y, s), the norms on both sides of a block's boundary in one pass: the block's output
+    x is normalised, gated and added to the scaled stream, which is normalised for the next
+    block:
+
+        s = residual * residual_scale + gate * x * weight / sqrt(mean(x^2) + eps), rounded to x's type
+        y = s * next_weight / sqrt(mean(s^2) + eps)
+
+    residual and gate have x's shape and type (a gate may be expanded over rows), the weights
+    and residual_scale are vectors of x's type or all three float32. Without gate or
+    residual_scale they are 1."""
+    args = x, residual, weight, next_weight, gate, residual_scale
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        return _SandwichFunction.apply(*args, eps)
+    return _layers.sandwich_norm(*args, eps)
+
+
+def sandwich_norm_backward(dy, ds, s, x, residual, weight, next_weight, gate=None, residual_scale=None, *,
+                           eps: float = 1e-6):
+    """(dx, dresidual, dweight, dnext_weight, dgate, dresidual_scale) of sandwich_norm for the
+    gradient dy of y and, optionally, ds that of s; the last two None without gate or scale."""
+    return _layers.sandwich_norm_backward(x, residual, weight, next_weight, gate, residual_scale, dy, ds, s, eps)
 
 
 # ----------------------------------------------------------------------- 8 bits

@@ -1,0 +1,118 @@
+"""AdamW on torch CUDA tensors: one call updates every tensor of a model.
+
+* ``AdamW``, a ``torch.optim.Optimizer``: 16-bit parameters keep a float32 master, the
+  moments are float32 or 8 bits (``moment_bits=8``);
+* ``adamw_step``, the step by itself on lists of tensors, and ``moment_values``, what the
+  codes of an 8-bit moment stand for.
+
+The calls are the entry points so3lr_adamw and so3lr_moment_values of
+include/so3lr_b200.h, which has the formulas, through the compiled module of the
+feed-forward layers; its conventions hold here: kernels are queued on the current torch
+stream of the tensors' GPU, arguments that do not fit one another raise ValueError, a
+value outside the library's range So3lrError, and there is no CPU path. The step
+counters are on the GPU, so a step may be captured in a graph and replayed.
+"""
+from __future__ import annotations
+
+import torch
+
+from .layers import _layers
+
+__all__ = ["AdamW", "adamw_step", "moment_values", "SCALE_BLOCK"]
+
+SCALE_BLOCK = 256  # elements of a tensor that share the scale of an 8-bit moment
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, exp_avg_scales=None, exp_avg_sq_scales=None,
+               masters=None, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2) -> None:
+    """One AdamW step of lists of contiguous tensors, in place:
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+
+    params: float32, bfloat16 or float16; grads: the parameter's type or float32. steps: the
+    counters t, to which the call adds 1: an int64 tensor of one element for each parameter,
+    or a list of one-element tensors. masters: for each parameter a float32 tensor that is
+    updated in its place, the parameter being its rounding, or None. Moments are float32; with
+    a tensor of scales for a parameter, one for each 256 elements, 8 bits (exp_avgs int8,
+    exp_avg_sqs uint8). lr: a number, or a float32 tensor of one element on the GPU, which is
+    read there. Zero codes and scales are zero moments. Nothing in the call may overlap;
+    parameters or counters that do are refused."""
+    _layers.adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales, exp_avg_sq_scales, masters, lr,
+                       *betas, eps, weight_decay)
+
+
+def moment_values(codes, scales, dtype=torch.float32):
+    """What an 8-bit moment's codes stand for, rounded to dtype: scales[i / 256] c |c| / 127^2
+    for int8 codes (the first moment), scales[i / 256] (c / 255)^4 for uint8 (the second)."""
+    return _layers.moment_values(codes, scales, dtype)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over all parameters of a group in one call.
+
+    moment_bits: 32, or 8 (a quarter of the memory; tensors of fewer than 4096 elements keep
+    32). master: keep a float32 copy of each 16-bit parameter, made at its first step, and
+    update that; the parameter is its rounding, so what is written into a parameter after
+    that step is lost. Each may be set for a group. lr may be a float32 tensor of one
+    element on the GPU, for graphs. The first step allocates the state: take it before a
+    capture."""
+
+    SMALL = 4096
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 moment_bits: int = 32, master: bool = True):
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, moment_bits=moment_bits,
+                                      master=master))
+
+    def add_param_group(self, param_group):
+        bits = param_group.get("moment_bits", self.defaults["moment_bits"])
+        if bits not in (8, 32):
+            raise ValueError(f"moment_bits must be 8 or 32, got {bits}")
+        super().add_param_group(param_group)
+
+    def _start(self, p, group):
+        state = self.state[p]
+        state["step"] = torch.zeros((), dtype=torch.int64, device=p.device)
+        flat = dict(device=p.device, memory_format=torch.contiguous_format)
+        if group["moment_bits"] == 8 and p.numel() >= self.SMALL:
+            blocks = (p.numel() + SCALE_BLOCK - 1) // SCALE_BLOCK
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.int8, **flat)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.uint8, **flat)
+            state["exp_avg_scale"], state["exp_avg_sq_scale"] = (torch.zeros(blocks, device=p.device) for _ in range(2))
+        else:
+            state["exp_avg"], state["exp_avg_sq"] = (torch.zeros_like(p, dtype=torch.float32, **flat) for _ in range(2))
+        if group["master"] and p.dtype != torch.float32:
+            state["master"] = p.detach().float().clone(memory_format=torch.contiguous_format)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            grads = [p.grad if p.grad.is_sparse or p.grad.is_contiguous() else p.grad.contiguous() for p in params]
+            states = [self.state[p] or self._start(p, group) for p in params]
+            pick = lambda key: [s.get(key) for s in states]  # noqa: E731
+            adamw_step(params, grads, pick("exp_avg"), pick("exp_avg_sq"), pick("step"),
+                       exp_avg_scales=pick("exp_avg_scale"), exp_avg_sq_scales=pick("exp_avg_sq_scale"),
+                       masters=pick("master"), lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"])
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch.optim.Optimizer's, with each state tensor in its own type: the base class
+        would cast masters, moments and scales to the parameter's."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, params):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.to(p.device, copy=True) if torch.is_tensor(v) else v
+                                 for k, v in state_dict["state"][i].items()}
