@@ -72,10 +72,10 @@ __global__ void k_adamw_steps(const __grid_constant__ Steps<MOST> a) {
                           float(1.0 - lr * a.decay), 0.0f);
 }
 
-// kPer consecutive elements as float, or `left` of them one by one
-template <class T>
-__device__ __forceinline__ void read(const T *p, bool whole, int left, float (&f)[kPer]) {
-  if (whole) {
+// kPer consecutive elements as float; not WHOLE: the `left` first of them one by one, zeros for the others
+template <bool WHOLE, class T>
+__device__ __forceinline__ void read(const T *p, int left, float (&f)[kPer]) {
+  if (WHOLE) {
     const Chunk<T, kPer> c = load_chunk<T, kPer>(p);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) f[i] = to_float(c.e[i]);
@@ -84,10 +84,10 @@ __device__ __forceinline__ void read(const T *p, bool whole, int left, float (&f
     for (int i = 0; i < kPer; ++i) f[i] = i < left ? to_float(p[i]) : 0.0f;
   }
 }
-template <class T>
-__device__ __forceinline__ void write(T *p, bool whole, int left, const float (&f)[kPer]) {
+template <bool WHOLE, class T>
+__device__ __forceinline__ void write(T *p, int left, const float (&f)[kPer]) {
   const Chunk<T, kPer> c = to_chunk<T, kPer>(f);
-  if (whole) {
+  if (WHOLE) {
     store_chunk<T, kPer>(p, c);
   } else {
 #pragma unroll
@@ -95,154 +95,219 @@ __device__ __forceinline__ void write(T *p, bool whole, int left, const float (&
       if (i < left) p[i] = c.e[i];
   }
 }
-using Codes = Chunk<unsigned char, kPer>;
-__device__ __forceinline__ Codes read_codes(const void *p, bool whole, int left) {
-  if (whole) return load_chunk<unsigned char, kPer>(static_cast<const unsigned char *>(p));
+// kPer codes, in words: bytes by themselves would take a register and an instruction each
+struct Codes {
+  uint32_t word[kPer / 4];
+};
+template <bool WHOLE>
+__device__ __forceinline__ Codes read_codes(const void *from, int left) {
+  const unsigned char *p = static_cast<const unsigned char *>(from);
   Codes c{};
+  if (WHOLE) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    c.word[0] = v.x;
+    c.word[1] = v.y;
+  } else {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (i < left) c.e[i] = static_cast<const unsigned char *>(p)[i];
+    for (int i = 0; i < kPer; ++i)
+      if (i < left) c.word[i / 4] |= uint32_t(p[i]) << 8 * (i % 4);
+  }
   return c;
 }
-__device__ __forceinline__ void write_codes(void *p, bool whole, int left, const Codes &c) {
-  if (whole) return store_chunk<unsigned char, kPer>(static_cast<unsigned char *>(p), c);
+template <bool WHOLE>
+__device__ __forceinline__ void write_codes(void *to, int left, const Codes &c) {
+  unsigned char *p = static_cast<unsigned char *>(to);
+  if (WHOLE) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(c.word[0], c.word[1]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (i < left) static_cast<unsigned char *>(p)[i] = c.e[i];
+    for (int i = 0; i < kPer; ++i)
+      if (i < left) p[i] = static_cast<unsigned char>(c.word[i / 4] >> 8 * (i % 4));
+  }
 }
 
-// What a code stands for. SIGNED: m, else v.
+// What a code stands for. SIGNED: m, else v. Each product is rounded by itself: what a state
+// stands for must not depend on how a compiler contracts.
+__device__ __forceinline__ float of_m(float code, float top) {
+  const float t = __fmul_rn(code, 1.0f / 127.0f);
+  return __fmul_rn(__fmul_rn(t, fabsf(t)), top);
+}
+__device__ __forceinline__ float of_v(float code, float top) {
+  const float t = __fmul_rn(code, 1.0f / 255.0f), square = __fmul_rn(t, t);
+  return __fmul_rn(__fmul_rn(square, square), top);
+}
+// kPer values of codes, without the slow int-to-float conversion: a byte in the low bits of 2^23
 template <bool SIGNED>
-__device__ __forceinline__ float value_of(unsigned char code, float top) {
-  if (SIGNED) {
-    const float t = float(static_cast<signed char>(code)) * (1.0f / 127.0f);
-    return t * fabsf(t) * top;
+__device__ __forceinline__ void values_of(const Codes &codes, float top, float (&f)[kPer]) {
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t word = codes.word[i / 4];
+    if (SIGNED)
+      f[i] = of_m(byte_to_float(word ^ 0x80808080u, i % 4), top);
+    else
+      f[i] = of_v(__uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 + i % 4)) - 8388608.0f, top);
   }
-  const float t = float(code) * (1.0f / 255.0f), square = t * t;
-  return square * square * top;
 }
 __device__ __forceinline__ float root(float v) {
   float r;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// The warp's 256 elements to codes; returns their scale. A block that holds an infinity
-// or a NaN gets scale NaN and codes 0, one whose largest is below float32's normal
-// numbers (its reciprocal could overflow) scale 0 and codes 0.
-template <bool SIGNED>
-__device__ __forceinline__ float encode(const float (&f)[kPer], Codes &codes) {
+// The square root of x in 2^-126..1 as correctly rounded (but for one in a million, which is a
+// unit off): Heron's step on x times the hardware's reciprocal root. With the approximate
+// root alone one code in 30,000 would fall on the other side of a tie.
+__device__ __forceinline__ float root_of_share(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  const float s = x * y;
+  return fmaf(fmaf(-s, s, x), 0.5f * y, s);
+}
+// The largest magnitude of the warp's 256 elements, for a scale; `live`: codes can be made
+// with it. Not of a block that holds an infinity or a NaN (scale NaN, codes 0), nor of one
+// whose largest is below float32's normal numbers (scale 0, codes 0: its reciprocal could
+// overflow).
+__device__ __forceinline__ float scale_of(const float (&f)[kPer], bool &live) {
   float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) top = max_abs(top, f[i]);
   const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
-  top = __uint_as_float(bits);
-  if (bits > 0x7f7fffffu || bits < 0x00800000u) {
-    codes = Codes{};
-    return bits > 0x7f7fffffu ? __uint_as_float(0x7fc00000u) : 0.0f;
-  }
-  const float inv = 1.0f / top;
-  // adding 1.5 2^23 leaves the rounded integer in the low bits of the sum
+  live = bits <= 0x7f7fffffu && bits >= 0x00800000u;
+  return live ? __uint_as_float(bits) : bits > 0x7f7fffffu ? __uint_as_float(0x7fc00000u) : 0.0f;
+}
+// The shares of the scale, 2^-126 at least: smaller ones get code 0 (or 1) either way.
+__device__ __forceinline__ float share_of(float f, float inv) { return fmaxf(fabsf(f) * inv, 0x1p-126f); }
+// Codes from their values: adding 1.5 2^23 leaves the rounded integer in the low bits of the sum.
+__device__ __forceinline__ Codes pack(const float (&code)[kPer]) {
+  Codes codes;
   uint32_t q[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (SIGNED) {
-      q[i] = __float_as_uint(fmaf(copysignf(root(fabsf(f[i]) * inv), f[i]), 127.0f, 12582912.0f));
-    } else {
-      const float code = root(root(f[i] * inv)) * 255.0f;
-      q[i] = __float_as_uint((f[i] > 0.0f ? fmaxf(code, 1.0f) : 0.0f) + 12582912.0f);
-    }
-  }
+  for (int i = 0; i < kPer; ++i) q[i] = __float_as_uint(__fadd_rn(code[i], 12582912.0f));
 #pragma unroll
   for (int i = 0; i < kPer / 4; ++i) {
     const uint32_t lo = __byte_perm(q[4 * i], q[4 * i + 1], 0x0040), hi = __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040);
-    reinterpret_cast<uint32_t *>(&codes)[i] = __byte_perm(lo, hi, 0x5410);
+    codes.word[i] = __byte_perm(lo, hi, 0x5410);
   }
-  return top;
+  return codes;
+}
+__device__ __forceinline__ float reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-template <class P, class G, bool EIGHT, int MOST>
-__device__ __forceinline__ void update(const Table<MOST> &a, const Entry &e, bool wide, long long chunk, const float4 &coef) {
-  const long long at = chunk * kChunk + threadIdx.x * kPer;
-  const int left = int(min((long long)kPer, e.n - at));  // may be negative; a warp past the end has nothing to do
-  const bool whole = wide && left == kPer;
-  if (at - (threadIdx.x & 31) * kPer >= e.n) return;
+// What of a tensor a block needs, and the coefficients of its step
+struct Work {
+  const Entry &e;
+  float4 coef;
+  float b1, c1, b2, c2, eps;
+};
+// WHOLE: all of the warp's elements are there and on 16-byte boundaries
+template <class P, class G, bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void update(const Work &a, long long at) {
+  const Entry &e = a.e;
+  const float4 coef = a.coef;
+  const int left = WHOLE ? kPer : int(min((long long)kPer, e.n - at));  // may be negative
   float g[kPer], p[kPer], m[kPer], v[kPer];
-  read(static_cast<const G *>(e.g) + at, whole, left, g);
+  read<WHOLE>(static_cast<const G *>(e.g) + at, left, g);
   if (e.master)
-    read(e.master + at, whole, left, p);
+    read<WHOLE>(e.master + at, left, p);
   else
-    read(static_cast<const P *>(e.p) + at, whole, left, p);
+    read<WHOLE>(static_cast<const P *>(e.p) + at, left, p);
   const long long block = at / kScaleBlock;
   if (EIGHT) {
-    const Codes cm = read_codes(static_cast<unsigned char *>(e.m) + at, whole, left);
-    const Codes cv = read_codes(static_cast<unsigned char *>(e.v) + at, whole, left);
-    const float m_top = e.m_top[block], v_top = e.v_top[block];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      m[i] = value_of<true>(cm.e[i], m_top);
-      v[i] = value_of<false>(cv.e[i], v_top);
-    }
+    const Codes cm = read_codes<WHOLE>(static_cast<unsigned char *>(e.m) + at, left);
+    const Codes cv = read_codes<WHOLE>(static_cast<unsigned char *>(e.v) + at, left);
+    // what is behind the end stays zero, and so does not count in the scale
+    values_of<true>(cm, e.m_top[block], m);
+    values_of<false>(cv, e.v_top[block], v);
   } else {
-    read(static_cast<const float *>(e.m) + at, whole, left, m);
-    read(static_cast<const float *>(e.v) + at, whole, left, v);
+    read<WHOLE>(static_cast<const float *>(e.m) + at, left, m);
+    read<WHOLE>(static_cast<const float *>(e.v) + at, left, v);
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    m[i] = fmaf(a.b1, m[i], a.c1 * g[i]);
-    v[i] = fmaf(a.b2, v[i], a.c2 * (g[i] * g[i]));
-    // the denominator is at least eps and far below 2^126, where the fast division is exact to 2 units
-    p[i] = fmaf(p[i], coef.z, -coef.x * __fdividef(m[i], fmaf(root(v[i]), coef.y, a.eps)));
+    m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
+    v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(a.c2, __fmul_rn(g[i], g[i])));
   }
+  // the denominator is at least eps, a normal number, and below 2^126
+  auto move = [&](int i, float denominator) { p[i] = fmaf(p[i], coef.z, -coef.x * (m[i] * reciprocal(denominator))); };
   if (EIGHT) {
-    if (left < kPer) {  // what is behind the end does not count in the scale
+    bool m_live, v_live;
+    const float m_top = scale_of(m, m_live), v_top = scale_of(v, v_live);
+    float code[kPer];
+    Codes cm{}, cv{};
+    if (v_live) {  // the root of v is that of its share, which its code needs too
+      const float inv = __frcp_rn(v_top), back = root(v_top) * coef.y;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i >= left) m[i] = v[i] = 0.0f;
+      for (int i = 0; i < kPer; ++i) {
+        const float half = root_of_share(share_of(v[i], inv));
+        move(i, fmaf(half, back, a.eps));
+        code[i] = __fmul_rn(root_of_share(half), 255.0f);
+        if (v[i] > 0.0f) code[i] = fmaxf(code[i], 1.0f);
+      }
+      cv = pack(code);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) move(i, fmaf(root(v[i]), coef.y, a.eps));
     }
-    Codes cm, cv;
-    const float m_top = encode<true>(m, cm), v_top = encode<false>(v, cv);
-    write_codes(static_cast<unsigned char *>(e.m) + at, whole, left, cm);
-    write_codes(static_cast<unsigned char *>(e.v) + at, whole, left, cv);
+    if (m_live) {
+      const float inv = __frcp_rn(m_top);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) code[i] = copysignf(__fmul_rn(root_of_share(share_of(m[i], inv)), 127.0f), m[i]);
+      cm = pack(code);
+    }
+    write_codes<WHOLE>(static_cast<unsigned char *>(e.m) + at, left, cm);
+    write_codes<WHOLE>(static_cast<unsigned char *>(e.v) + at, left, cv);
     if ((threadIdx.x & 31) == 0) {
       e.m_top[block] = m_top;
       e.v_top[block] = v_top;
     }
   } else {
-    write(static_cast<float *>(e.m) + at, whole, left, m);
-    write(static_cast<float *>(e.v) + at, whole, left, v);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) move(i, fmaf(root(v[i]), coef.y, a.eps));
+    write<WHOLE>(static_cast<float *>(e.m) + at, left, m);
+    write<WHOLE>(static_cast<float *>(e.v) + at, left, v);
   }
-  if (e.master) write(e.master + at, whole, left, p);
-  write(static_cast<P *>(e.p) + at, whole, left, p);
+  if (e.master) write<WHOLE>(e.master + at, left, p);
+  write<WHOLE>(static_cast<P *>(e.p) + at, left, p);
+}
+
+template <class P, class G, bool EIGHT>
+__device__ __forceinline__ void update_chunk(const Work &a, long long chunk, bool wide) {
+  const long long at = chunk * kChunk + threadIdx.x * kPer, warp_at = at - (threadIdx.x & 31) * kPer;
+  if (wide && warp_at + 32 * kPer <= a.e.n)
+    update<P, G, EIGHT, true>(a, at);
+  else if (warp_at < a.e.n)
+    update<P, G, EIGHT, false>(a, at);
 }
 
 template <int MOST>
-__global__ void __launch_bounds__(kAdamThreads) k_adamw(const __grid_constant__ Table<MOST> a) {
+__global__ void __launch_bounds__(kAdamThreads) k_adamw(const __grid_constant__ Table<MOST> t) {
   dependents_may_start();
-  int lo = 0, hi = a.count - 1;  // the last tensor whose first chunk is not behind this block's
+  int lo = 0, hi = t.count - 1;  // the last tensor whose first chunk is not behind this block's
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (a.first[mid] <= int(blockIdx.x))
+    if (t.first[mid] <= int(blockIdx.x))
       lo = mid;
     else
       hi = mid - 1;
   }
-  const Entry &e = a.e[lo];
-  const int kind = a.kind[lo];
-  const long long chunk = blockIdx.x - a.first[lo];
+  const int kind = t.kind[lo];
+  const long long chunk = blockIdx.x - t.first[lo];
   const bool wide = kind & kWide;
   wait_for_predecessors();
-  const float4 coef = a.coef[lo];
+  const Work a{t.e[lo], t.coef[lo], t.b1, t.c1, t.b2, t.c2, t.eps};
   switch (kind & (kParamMask | kGradFloat | kEight)) {
-    case SO3LR_FLOAT32 | kGradFloat: return update<float, float, false>(a, e, wide, chunk, coef);
-    case SO3LR_FLOAT32 | kGradFloat | kEight: return update<float, float, true>(a, e, wide, chunk, coef);
-    case SO3LR_BFLOAT16: return update<__nv_bfloat16, __nv_bfloat16, false>(a, e, wide, chunk, coef);
-    case SO3LR_BFLOAT16 | kEight: return update<__nv_bfloat16, __nv_bfloat16, true>(a, e, wide, chunk, coef);
-    case SO3LR_BFLOAT16 | kGradFloat: return update<__nv_bfloat16, float, false>(a, e, wide, chunk, coef);
-    case SO3LR_BFLOAT16 | kGradFloat | kEight: return update<__nv_bfloat16, float, true>(a, e, wide, chunk, coef);
-    case SO3LR_FLOAT16: return update<__half, __half, false>(a, e, wide, chunk, coef);
-    case SO3LR_FLOAT16 | kEight: return update<__half, __half, true>(a, e, wide, chunk, coef);
-    case SO3LR_FLOAT16 | kGradFloat: return update<__half, float, false>(a, e, wide, chunk, coef);
-    case SO3LR_FLOAT16 | kGradFloat | kEight: return update<__half, float, true>(a, e, wide, chunk, coef);
+    case SO3LR_FLOAT32 | kGradFloat: return update_chunk<float, float, false>(a, chunk, wide);
+    case SO3LR_FLOAT32 | kGradFloat | kEight: return update_chunk<float, float, true>(a, chunk, wide);
+    case SO3LR_BFLOAT16: return update_chunk<__nv_bfloat16, __nv_bfloat16, false>(a, chunk, wide);
+    case SO3LR_BFLOAT16 | kEight: return update_chunk<__nv_bfloat16, __nv_bfloat16, true>(a, chunk, wide);
+    case SO3LR_BFLOAT16 | kGradFloat: return update_chunk<__nv_bfloat16, float, false>(a, chunk, wide);
+    case SO3LR_BFLOAT16 | kGradFloat | kEight: return update_chunk<__nv_bfloat16, float, true>(a, chunk, wide);
+    case SO3LR_FLOAT16: return update_chunk<__half, __half, false>(a, chunk, wide);
+    case SO3LR_FLOAT16 | kEight: return update_chunk<__half, __half, true>(a, chunk, wide);
+    case SO3LR_FLOAT16 | kGradFloat: return update_chunk<__half, float, false>(a, chunk, wide);
+    case SO3LR_FLOAT16 | kGradFloat | kEight: return update_chunk<__half, float, true>(a, chunk, wide);
   }
 }
 
@@ -255,13 +320,15 @@ __global__ void k_moment_values(const so3lr_moment_values_args a, bool wide) {
   for (long long at = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * kPer; at < a.n;
        at += (long long)gridDim.x * blockDim.x * kPer) {
     const int left = int(min((long long)kPer, a.n - at));
-    const bool whole = wide && left == kPer;
-    const Codes c = read_codes(codes + at, whole, left);
     const float top = a.scales[at / kScaleBlock];
     float f[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) f[i] = value_of<SIGNED>(c.e[i], top);
-    write(static_cast<O *>(a.values) + at, whole, left, f);
+    if (wide && left == kPer) {
+      values_of<SIGNED>(read_codes<true>(codes + at, left), top, f);
+      write<true>(static_cast<O *>(a.values) + at, left, f);
+    } else {
+      values_of<SIGNED>(read_codes<false>(codes + at, left), top, f);
+      write<false>(static_cast<O *>(a.values) + at, left, f);
+    }
   }
 }
 
