@@ -28,6 +28,7 @@ namespace so3lr_b200 {
 namespace {
 
 constexpr int kChunk = 2048, kScaleBlock = 256, kPer = 8, kAdamThreads = kChunk / kPer;
+constexpr int kAhead = 4 * kSmCount;  // chunks
 
 struct Entry {
   void *p;
@@ -126,26 +127,55 @@ __device__ __forceinline__ void write_codes(void *to, int left, const Codes &c) 
   }
 }
 
-// What a code stands for. SIGNED: m, else v. Each product is rounded by itself: what a state
-// stands for must not depend on how a compiler contracts.
-__device__ __forceinline__ float of_m(float code, float top) {
-  const float t = __fmul_rn(code, 1.0f / 127.0f);
-  return __fmul_rn(__fmul_rn(t, fabsf(t)), top);
+// Two floats in one register pair: products and multiply-adds of pairs issue as one
+// instruction, each half rounded by itself (268 M elements 735 -> 692 us). Sums of products
+// that codes depend on are taken half by half: the assembler contracts add.rn.f32x2 with a
+// product, which a float32 of the formula is not.
+struct Pair {
+  uint64_t bits;
+  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
+  __device__ __forceinline__ Pair(uint64_t b, int) : bits(b) {}
+  __device__ __forceinline__ void get(float &a, float &b) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits));
+  }
+};
+__device__ __forceinline__ Pair operator*(const Pair &a, const Pair &b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits), "l"(b.bits));
+  return Pair(r, 0);
 }
-__device__ __forceinline__ float of_v(float code, float top) {
-  const float t = __fmul_rn(code, 1.0f / 255.0f), square = __fmul_rn(t, t);
-  return __fmul_rn(__fmul_rn(square, square), top);
+__device__ __forceinline__ Pair operator+(const Pair &a, const Pair &b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits), "l"(b.bits));
+  return Pair(r, 0);
 }
-// kPer values of codes, without the slow int-to-float conversion: a byte in the low bits of 2^23
+__device__ __forceinline__ Pair fma(const Pair &a, const Pair &b, const Pair &c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return Pair(r, 0);
+}
+
+// What codes stand for. SIGNED: m, else v. Bytes become floats without the slow conversion: a
+// byte in the low bits of 2^23.
 template <bool SIGNED>
 __device__ __forceinline__ void values_of(const Codes &codes, float top, float (&f)[kPer]) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const uint32_t word = codes.word[i / 4];
-    if (SIGNED)
-      f[i] = of_m(byte_to_float(word ^ 0x80808080u, i % 4), top);
-    else
-      f[i] = of_v(__uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 + i % 4)) - 8388608.0f, top);
+  for (int i = 0; i < kPer; i += 2) {
+    const uint32_t word = SIGNED ? codes.word[i / 4] ^ 0x80808080u : codes.word[i / 4];
+    const Pair code = Pair(__uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 + i % 4)),
+                           __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7441 + i % 4))) +
+                      Pair(SIGNED ? -8388736.0f : -8388608.0f);
+    const Pair t = code * Pair(SIGNED ? 1.0f / 127.0f : 1.0f / 255.0f), square = t * t;
+    if (SIGNED) {
+      float a, b;
+      t.get(a, b);
+      (square * Pair(top)).get(f[i], f[i + 1]);
+      f[i] = copysignf(f[i], a);
+      f[i + 1] = copysignf(f[i + 1], b);
+    } else {
+      (square * square * Pair(top)).get(f[i], f[i + 1]);
+    }
   }
 }
 __device__ __forceinline__ float root(float v) {
@@ -153,14 +183,16 @@ __device__ __forceinline__ float root(float v) {
   asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// The square root of x in 2^-126..1 as correctly rounded (but for one in a million, which is a
-// unit off): Heron's step on x times the hardware's reciprocal root. With the approximate
-// root alone one code in 30,000 would fall on the other side of a tie.
-__device__ __forceinline__ float root_of_share(float x) {
-  float y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  const float s = x * y;
-  return fmaf(fmaf(-s, s, x), 0.5f * y, s);
+// The square roots of two numbers in 2^-126..1 as correctly rounded (but for one in a million,
+// which is a unit off): Heron's step on x times the hardware's reciprocal root. With the
+// approximate root alone one code in 30,000 would fall on the other side of a tie.
+__device__ __forceinline__ Pair roots_of_shares(const Pair &x) {
+  float a, b, ya, yb;
+  x.get(a, b);
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(ya) : "f"(a));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(yb) : "f"(b));
+  const Pair y(ya, yb), s = x * y;
+  return fma(fma(s * Pair(-1.0f), s, x), y * Pair(0.5f), s);
 }
 // The largest magnitude of the warp's 256 elements, for a scale; `live`: codes can be made
 // with it. Not of a block that holds an infinity or a NaN (scale NaN, codes 0), nor of one
@@ -175,7 +207,11 @@ __device__ __forceinline__ float scale_of(const float (&f)[kPer], bool &live) {
   return live ? __uint_as_float(bits) : bits > 0x7f7fffffu ? __uint_as_float(0x7fc00000u) : 0.0f;
 }
 // The shares of the scale, 2^-126 at least: smaller ones get code 0 (or 1) either way.
-__device__ __forceinline__ float share_of(float f, float inv) { return fmaxf(fabsf(f) * inv, 0x1p-126f); }
+__device__ __forceinline__ Pair shares_of(float a, float b, float inv) {
+  float x, y;
+  (Pair(a, b) * Pair(inv)).get(x, y);
+  return Pair(fmaxf(fabsf(x), 0x1p-126f), fmaxf(fabsf(y), 0x1p-126f));
+}
 // Codes from their values: adding 1.5 2^23 leaves the rounded integer in the low bits of the sum.
 __device__ __forceinline__ Codes pack(const float (&code)[kPer]) {
   Codes codes;
@@ -224,13 +260,30 @@ __device__ __forceinline__ void update(const Work &a, long long at) {
     read<WHOLE>(static_cast<const float *>(e.m) + at, left, m);
     read<WHOLE>(static_cast<const float *>(e.v) + at, left, v);
   }
+  auto sum = [](const Pair &x, const Pair &y, float &a, float &b) {
+    float c, d;
+    x.get(a, b);
+    y.get(c, d);
+    a = __fadd_rn(a, c);
+    b = __fadd_rn(b, d);
+  };
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
-    v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(a.c2, __fmul_rn(g[i], g[i])));
+  for (int i = 0; i < kPer; i += 2) {
+    const Pair gi(g[i], g[i + 1]);
+    sum(Pair(a.b1) * Pair(m[i], m[i + 1]), Pair(a.c1) * gi, m[i], m[i + 1]);
+    sum(Pair(a.b2) * Pair(v[i], v[i + 1]), Pair(a.c2) * (gi * gi), v[i], v[i + 1]);
   }
-  // the denominator is at least eps, a normal number, and below 2^126
-  auto move = [&](int i, float denominator) { p[i] = fmaf(p[i], coef.z, -coef.x * (m[i] * reciprocal(denominator))); };
+  // the denominators are at least eps, a normal number, and below 2^126
+  auto move = [&](int i, const Pair &denominators) {
+    float d, e;
+    denominators.get(d, e);
+    const Pair ratio = Pair(m[i], m[i + 1]) * Pair(reciprocal(d), reciprocal(e));
+    fma(Pair(p[i], p[i + 1]), Pair(coef.z), ratio * Pair(-coef.x)).get(p[i], p[i + 1]);
+  };
+  auto move_by_root = [&] {
+#pragma unroll
+    for (int i = 0; i < kPer; i += 2) move(i, fma(Pair(root(v[i]), root(v[i + 1])), Pair(coef.y), Pair(a.eps)));
+  };
   if (EIGHT) {
     bool m_live, v_live;
     const float m_top = scale_of(m, m_live), v_top = scale_of(v, v_live);
@@ -239,21 +292,25 @@ __device__ __forceinline__ void update(const Work &a, long long at) {
     if (v_live) {  // the root of v is that of its share, which its code needs too
       const float inv = __frcp_rn(v_top), back = root(v_top) * coef.y;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const float half = root_of_share(share_of(v[i], inv));
-        move(i, fmaf(half, back, a.eps));
-        code[i] = __fmul_rn(root_of_share(half), 255.0f);
+      for (int i = 0; i < kPer; i += 2) {
+        const Pair half = roots_of_shares(shares_of(v[i], v[i + 1], inv));
+        move(i, fma(half, Pair(back), Pair(a.eps)));
+        (roots_of_shares(half) * Pair(255.0f)).get(code[i], code[i + 1]);
         if (v[i] > 0.0f) code[i] = fmaxf(code[i], 1.0f);
+        if (v[i + 1] > 0.0f) code[i + 1] = fmaxf(code[i + 1], 1.0f);
       }
       cv = pack(code);
     } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) move(i, fmaf(root(v[i]), coef.y, a.eps));
+      move_by_root();
     }
     if (m_live) {
       const float inv = __frcp_rn(m_top);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) code[i] = copysignf(__fmul_rn(root_of_share(share_of(m[i], inv)), 127.0f), m[i]);
+      for (int i = 0; i < kPer; i += 2) {
+        (roots_of_shares(shares_of(m[i], m[i + 1], inv)) * Pair(127.0f)).get(code[i], code[i + 1]);
+        code[i] = copysignf(code[i], m[i]);
+        code[i + 1] = copysignf(code[i + 1], m[i + 1]);
+      }
       cm = pack(code);
     }
     write_codes<WHOLE>(static_cast<unsigned char *>(e.m) + at, left, cm);
@@ -263,8 +320,7 @@ __device__ __forceinline__ void update(const Work &a, long long at) {
       e.v_top[block] = v_top;
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) move(i, fmaf(root(v[i]), coef.y, a.eps));
+    move_by_root();
     write<WHOLE>(static_cast<float *>(e.m) + at, left, m);
     write<WHOLE>(static_cast<float *>(e.v) + at, left, v);
   }
@@ -282,7 +338,7 @@ __device__ __forceinline__ void update_chunk(const Work &a, long long chunk, boo
 }
 
 template <int MOST>
-__global__ void __launch_bounds__(kAdamThreads) k_adamw(const __grid_constant__ Table<MOST> t) {
+__global__ void __launch_bounds__(kAdamThreads, 5) k_adamw(const __grid_constant__ Table<MOST> t) {
   dependents_may_start();
   int lo = 0, hi = t.count - 1;  // the last tensor whose first chunk is not behind this block's
   while (lo < hi) {
@@ -297,6 +353,17 @@ __global__ void __launch_bounds__(kAdamThreads) k_adamw(const __grid_constant__ 
   const bool wide = kind & kWide;
   wait_for_predecessors();
   const Work a{t.e[lo], t.coef[lo], t.b1, t.c1, t.b2, t.c2, t.eps};
+  // The 8-bit step computes for a third of the time that it loads: what a later block reads is on
+  // its way to L2 meanwhile (268 M elements 692 -> 640 us with five blocks an SM; the 32-bit
+  // step, bound by HBM, has nothing of it: 1096 and 1110 us).
+  const long long ahead = (chunk + kAhead) * kChunk;
+  if ((kind & kEight) && wide && threadIdx.x < 4 && ahead + kChunk <= a.e.n) {
+    const bool g = threadIdx.x == 0, p = threadIdx.x == 1;
+    const void *from = g ? a.e.g : p ? (a.e.master ? a.e.master : a.e.p) : threadIdx.x == 2 ? a.e.m : a.e.v;
+    const bool four = g ? kind & kGradFloat : a.e.master || (kind & kParamMask) == SO3LR_FLOAT32;
+    const int size = g || p ? (four ? 4 : 2) : 1;
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char *>(from) + ahead * size), "r"(kChunk * size) : "memory");
+  }
   switch (kind & (kParamMask | kGradFloat | kEight)) {
     case SO3LR_FLOAT32 | kGradFloat: return update_chunk<float, float, false>(a, chunk, wide);
     case SO3LR_FLOAT32 | kGradFloat | kEight: return update_chunk<float, float, true>(a, chunk, wide);
@@ -311,24 +378,30 @@ __global__ void __launch_bounds__(kAdamThreads) k_adamw(const __grid_constant__ 
   }
 }
 
-// values = what an 8-bit moment's codes stand for
+// values = what an 8-bit moment's codes stand for, 16 a thread
 template <class O, bool SIGNED>
-__global__ void k_moment_values(const so3lr_moment_values_args a, bool wide) {
+__global__ void __launch_bounds__(256) k_moment_values(const so3lr_moment_values_args a, bool wide) {
   dependents_may_start();
+  const long long at = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 2 * kPer;
+  if (at >= a.n) return;
+  const unsigned char *codes = static_cast<const unsigned char *>(a.codes) + at;
+  O *values = static_cast<O *>(a.values) + at;
   wait_for_predecessors();
-  const unsigned char *codes = static_cast<const unsigned char *>(a.codes);
-  for (long long at = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * kPer; at < a.n;
-       at += (long long)gridDim.x * blockDim.x * kPer) {
-    const int left = int(min((long long)kPer, a.n - at));
-    const float top = a.scales[at / kScaleBlock];
-    float f[kPer];
-    if (wide && left == kPer) {
-      values_of<SIGNED>(read_codes<true>(codes + at, left), top, f);
-      write<true>(static_cast<O *>(a.values) + at, left, f);
-    } else {
-      values_of<SIGNED>(read_codes<false>(codes + at, left), top, f);
-      write<false>(static_cast<O *>(a.values) + at, left, f);
-    }
+  const float top = a.scales[at / kScaleBlock];
+  float f[2][kPer];
+  if (wide && at + 2 * kPer <= a.n) {
+    const uint4 w = *reinterpret_cast<const uint4 *>(codes);
+    values_of<SIGNED>(Codes{{w.x, w.y}}, top, f[0]);
+    values_of<SIGNED>(Codes{{w.z, w.w}}, top, f[1]);
+    write<true>(values, kPer, f[0]);
+    write<true>(values + kPer, kPer, f[1]);
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int left = int(min((long long)kPer, a.n - at - h * kPer));  // may be negative
+    values_of<SIGNED>(read_codes<false>(codes + h * kPer, left), top, f[h]);
+    write<false>(values + h * kPer, left, f[h]);
   }
 }
 
@@ -365,9 +438,8 @@ void launch_step(const so3lr_adamw_args &a, float4 *coef, cudaStream_t s) {
     if (t.count == 0) t.coef = coef + i;
     t.e[t.count] = Entry{x.param, x.grad, x.master, x.exp_avg, x.exp_avg_sq, x.exp_avg_scale, x.exp_avg_sq_scale, x.n};
     const std::size_t e = x.dtype == SO3LR_FLOAT32 ? 4 : 2, ge = x.grad_dtype == SO3LR_FLOAT32 ? 4 : 2;
-    const std::size_t moment = x.exp_avg_scale ? 8 : 16;
-    const bool wide = on(x.param, std::min<std::size_t>(16, e * kPer)) && on(x.grad, std::min<std::size_t>(16, ge * kPer)) &&
-                      on(x.master, 16) && on(x.exp_avg, moment) && on(x.exp_avg_sq, moment);
+      const bool wide = on(x.param, std::min<std::size_t>(16, e * kPer)) && on(x.grad, std::min<std::size_t>(16, ge * kPer)) &&
+                      on(x.master, 16) && on(x.exp_avg, 16) && on(x.exp_avg_sq, 16);
     t.kind[t.count] = static_cast<unsigned char>(x.dtype | (x.grad_dtype == SO3LR_FLOAT32 ? kGradFloat : 0) |
                                                  (x.exp_avg_scale ? kEight : 0) | (wide ? kWide : 0));
     t.first[t.count + 1] = int(t.first[t.count] + chunks);
@@ -391,8 +463,8 @@ void launch_adamw(const so3lr_adamw_args &a, void *workspace, cudaStream_t s) {
 }
 
 void launch_moment_values(const so3lr_moment_values_args &a, cudaStream_t s) {
-  const bool wide = on(a.codes, 8) && on(a.values, 16);
-  const unsigned grid = unsigned(std::min<long long>((a.n + 256 * kPer - 1) / (256 * kPer), kSmCount * 32));
+  const bool wide = on(a.codes, 16) && on(a.values, 16);
+  const unsigned grid = unsigned((a.n + 512 * kPer - 1) / (512 * kPer));  // n <= 2^40: 2^28 blocks at most
   auto go = [&](auto t) {
     using O = decltype(t);
     launch(a.is_signed ? &k_moment_values<O, true> : &k_moment_values<O, false>, grid, 256, 0, s, a, wide);
