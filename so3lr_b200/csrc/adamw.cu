@@ -44,15 +44,17 @@ enum Kind : unsigned char { kParamMask = 3, kGradFloat = 4, kEight = 8, kWide = 
 template <int MOST>
 struct Table {
   Entry e[MOST];
-  int first[MOST + 1];  // first chunk of each tensor, and their number
   unsigned char kind[MOST];
-  int count;
-  const float4 *coef;   // of the first tensor: lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr decay
+  int count, chunks;
+  const float4 *coef;   // of the first tensor, as the steps' kernel left it
   float b1, c1, b2, c2, eps;
 };
+// For each tensor lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr decay and, as an integer,
+// its first chunk in its launch of k_adamw
 template <int MOST>
 struct Steps {
   long long *step[MOST];
+  int first[MOST];
   int count;
   float4 *coef;
   double lr;
@@ -70,7 +72,7 @@ __global__ void k_adamw_steps(const __grid_constant__ Steps<MOST> a) {
   *a.step[i] = t;
   const double lr = a.lr_device ? double(*a.lr_device) : a.lr;
   a.coef[i] = make_float4(float(lr / (1.0 - pow(a.beta1, double(t)))), float(1.0 / sqrt(1.0 - pow(a.beta2, double(t)))),
-                          float(1.0 - lr * a.decay), 0.0f);
+                          float(1.0 - lr * a.decay), __int_as_float(a.first[i]));
 }
 
 // kPer consecutive elements as float; not WHOLE: the `left` first of them one by one, zeros for the others
@@ -337,33 +339,45 @@ __device__ __forceinline__ void update_chunk(const Work &a, long long chunk, boo
     update<P, G, EIGHT, false>(a, at);
 }
 
+// The tensor of a chunk, the last whose first chunk is not behind it: the warp's lanes look at
+// every `every`-th, then at those up to the next.
+template <int MOST>
+__device__ __forceinline__ int tensor_of(const Table<MOST> &t, int chunk) {
+  const int lane = threadIdx.x & 31, every = (t.count + 31) / 32;
+  auto starts = [&](int i) { return i < t.count && __float_as_int(t.coef[i].w) <= chunk; };
+  int lo = every * (31 - __clz(__ballot_sync(0xffffffffu, starts(lane * every))));
+  if (MOST > 32 && every > 1) lo += 31 - __clz(__ballot_sync(0xffffffffu, lane < every && starts(lo + lane)));
+  return lo;
+}
+
 template <int MOST>
 __global__ void __launch_bounds__(kAdamThreads, 5) k_adamw(const __grid_constant__ Table<MOST> t) {
   dependents_may_start();
-  int lo = 0, hi = t.count - 1;  // the last tensor whose first chunk is not behind this block's
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t.first[mid] <= int(blockIdx.x))
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int kind = t.kind[lo];
-  const long long chunk = blockIdx.x - t.first[lo];
-  const bool wide = kind & kWide;
   wait_for_predecessors();
-  const Work a{t.e[lo], t.coef[lo], t.b1, t.c1, t.b2, t.c2, t.eps};
-  // The 8-bit step computes for a third of the time that it loads: what a later block reads is on
-  // its way to L2 meanwhile (268 M elements 692 -> 640 us with five blocks an SM; the 32-bit
-  // step, bound by HBM, has nothing of it: 1096 and 1110 us).
-  const long long ahead = (chunk + kAhead) * kChunk;
-  if ((kind & kEight) && wide && threadIdx.x < 4 && ahead + kChunk <= a.e.n) {
-    const bool g = threadIdx.x == 0, p = threadIdx.x == 1;
-    const void *from = g ? a.e.g : p ? (a.e.master ? a.e.master : a.e.p) : threadIdx.x == 2 ? a.e.m : a.e.v;
-    const bool four = g ? kind & kGradFloat : a.e.master || (kind & kParamMask) == SO3LR_FLOAT32;
-    const int size = g || p ? (four ? 4 : 2) : 1;
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char *>(from) + ahead * size), "r"(kChunk * size) : "memory");
+  const int block = int(blockIdx.x);
+  const int lo = tensor_of(t, block);
+  const float4 coef = t.coef[lo];
+  const int kind = t.kind[lo];
+  // The 8-bit step computes for longer than it loads: what a block of the next wave reads is on
+  // its way to L2 meanwhile (317 M elements in 256 tensors 957 us without; the 32-bit step,
+  // bound by HBM, has nothing of it: 1096 us without, 1110 with).
+  if (threadIdx.x < 32 && block + kAhead < t.chunks) {
+    const int then = tensor_of(t, block + kAhead), what = t.kind[then];
+    const Entry &e = t.e[then];
+    const long long at = (long long)(block + kAhead - __float_as_int(t.coef[then].w)) * kChunk;
+    if ((what & kEight) && (what & kWide) && threadIdx.x < 4 && at + kChunk <= e.n) {
+      const bool g = threadIdx.x == 0, p = threadIdx.x == 1;
+      const void *from = g ? e.g : p ? (e.master ? e.master : e.p) : threadIdx.x == 2 ? e.m : e.v;
+      const bool four = g ? what & kGradFloat : e.master || (what & kParamMask) == SO3LR_FLOAT32;
+      const int size = g || p ? (four ? 4 : 2) : 1;
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char *>(from) + at * size),
+                   "r"(kChunk * size)
+                   : "memory");
+    }
   }
+  const long long chunk = block - __float_as_int(coef.w);
+  const bool wide = kind & kWide;
+  const Work a{t.e[lo], coef, t.b1, t.c1, t.b2, t.c2, t.eps};
   switch (kind & (kParamMask | kGradFloat | kEight)) {
     case SO3LR_FLOAT32 | kGradFloat: return update_chunk<float, float, false>(a, chunk, wide);
     case SO3LR_FLOAT32 | kGradFloat | kEight: return update_chunk<float, float, true>(a, chunk, wide);
@@ -409,18 +423,13 @@ bool on(const void *p, std::size_t bytes) { return reinterpret_cast<uintptr_t>(p
 
 template <int MOST>
 void launch_step(const so3lr_adamw_args &a, float4 *coef, cudaStream_t s) {
-  for (long long begin = 0; begin < a.count; begin += MOST) {
-    Steps<MOST> steps{};
-    steps.count = int(std::min<long long>(MOST, a.count - begin));
-    steps.coef = coef + begin;
-    steps.lr = a.lr;
-    steps.lr_device = a.lr_device;
-    steps.beta1 = a.beta1;
-    steps.beta2 = a.beta2;
-    steps.decay = a.weight_decay;
-    for (int i = 0; i < steps.count; ++i) steps.step[i] = a.tensors[begin + i].step;
-    launch(k_adamw_steps<MOST>, unsigned((steps.count + 31) / 32), 32, 0, s, steps);
-  }
+  static_assert(MOST <= 32 * 32, "a block's search takes two steps");
+  Steps<MOST> steps{};
+  steps.lr = a.lr;
+  steps.lr_device = a.lr_device;
+  steps.beta1 = a.beta1;
+  steps.beta2 = a.beta2;
+  steps.decay = a.weight_decay;
   Table<MOST> t{};
   t.b1 = float(a.beta1);
   t.c1 = float(1.0 - a.beta1);
@@ -428,21 +437,27 @@ void launch_step(const so3lr_adamw_args &a, float4 *coef, cudaStream_t s) {
   t.c2 = float(1.0 - a.beta2);
   t.eps = float(a.eps);
   auto flush = [&] {
-    if (t.count && t.first[t.count]) launch(k_adamw<MOST>, unsigned(t.first[t.count]), kAdamThreads, 0, s, t);
-    t.count = 0;
+    if (t.count) {
+      t.coef = steps.coef = coef;
+      steps.count = t.count;
+      launch(k_adamw_steps<MOST>, unsigned((t.count + 31) / 32), 32, 0, s, steps);
+      if (t.chunks) launch(k_adamw<MOST>, unsigned(t.chunks), kAdamThreads, 0, s, t);
+    }
+    coef += t.count;
+    t.count = t.chunks = 0;
   };
   for (long long i = 0; i < a.count; ++i) {
     const so3lr_adamw_tensor &x = a.tensors[i];
-    const long long chunks = (x.n + kChunk - 1) / kChunk;  // 2^30 at most
-    if (t.count == MOST || (t.count && t.first[t.count] + chunks > 0x7fffffffLL)) flush();
-    if (t.count == 0) t.coef = coef + i;
+    const long long chunks = (x.n + kChunk - 1) / kChunk;  // 2^29 at most
+    if (t.count == MOST || t.chunks + chunks > 0x7fffffffLL) flush();
     t.e[t.count] = Entry{x.param, x.grad, x.master, x.exp_avg, x.exp_avg_sq, x.exp_avg_scale, x.exp_avg_sq_scale, x.n};
-    const std::size_t e = x.dtype == SO3LR_FLOAT32 ? 4 : 2, ge = x.grad_dtype == SO3LR_FLOAT32 ? 4 : 2;
-      const bool wide = on(x.param, std::min<std::size_t>(16, e * kPer)) && on(x.grad, std::min<std::size_t>(16, ge * kPer)) &&
+    const bool wide = on(x.param, 16) && on(x.grad, 16) &&
                       on(x.master, 16) && on(x.exp_avg, 16) && on(x.exp_avg_sq, 16);
     t.kind[t.count] = static_cast<unsigned char>(x.dtype | (x.grad_dtype == SO3LR_FLOAT32 ? kGradFloat : 0) |
                                                  (x.exp_avg_scale ? kEight : 0) | (wide ? kWide : 0));
-    t.first[t.count + 1] = int(t.first[t.count] + chunks);
+    steps.step[t.count] = x.step;
+    steps.first[t.count] = t.chunks;
+    t.chunks += int(chunks);
     ++t.count;
   }
   flush();
