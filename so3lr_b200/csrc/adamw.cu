@@ -3,8 +3,11 @@
 //   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
 //   p = p (1 - lr decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
 //
-// Bound by HBM: an element is read and written once (28 bytes with 32-bit moments, 16
-// with 8-bit ones and a float32 master). Every tensor is cut into chunks of 2048
+// Bound by HBM: an element is read and written once (28 bytes with 32-bit moments, 14
+// with 8-bit ones and a float32 master). With 32-bit moments 268 M elements take 1090 us, 6.9
+// TB/s; with 8-bit ones 317 M take 850 us, 5.2 TB/s, and under the power limit of a long run
+// 930. There neither fewer instructions (a third fewer: 870 us), nor five blocks an SM (845,
+// and the 32-bit step 1130), nor blocks of 2 or 4 times the elements (960 to 1300) help. Every tensor is cut into chunks of 2048
 // elements, a chunk is a block's work, and one launch covers all tensors: a block finds
 // its tensor in a table that travels as the kernel's argument, so that nothing is
 // copied to the GPU before it and a captured graph holds its own table. The step
@@ -351,7 +354,7 @@ __device__ __forceinline__ int tensor_of(const Table<MOST> &t, int chunk) {
 }
 
 template <int MOST>
-__global__ void __launch_bounds__(kAdamThreads, 5) k_adamw(const __grid_constant__ Table<MOST> t) {
+__global__ void __launch_bounds__(kAdamThreads, 4) k_adamw(const __grid_constant__ Table<MOST> t) {
   dependents_may_start();
   wait_for_predecessors();
   const int block = int(blockIdx.x);
@@ -359,8 +362,8 @@ __global__ void __launch_bounds__(kAdamThreads, 5) k_adamw(const __grid_constant
   const float4 coef = t.coef[lo];
   const int kind = t.kind[lo];
   // The 8-bit step computes for longer than it loads: what a block of the next wave reads is on
-  // its way to L2 meanwhile (317 M elements in 256 tensors 957 us without; the 32-bit step,
-  // bound by HBM, has nothing of it: 1096 us without, 1110 with).
+  // its way to L2 meanwhile (67 M elements 219 us without, 190 with; the 32-bit step, bound by
+  // HBM, has nothing of it: 268 M elements 1096 us without, 1110 with).
   if (threadIdx.x < 32 && block + kAhead < t.chunks) {
     const int then = tensor_of(t, block + kAhead), what = t.kind[then];
     const Entry &e = t.e[then];
