@@ -539,6 +539,63 @@ long long so3lr_feed_forward_backward_workspace(const so3lr_feed_forward_backwar
 int so3lr_feed_forward_backward(const so3lr_feed_forward_backward_args *args, void *workspace,
                                 long long workspace_bytes, void *stream, char *err, size_t errlen);
 
+/* Dense layer, bfloat16 or float16:
+ *   z = x W^T + bias,   y = act(z) + residual
+ * Sums, bias, activation and residual are float32, y is rounded once. gelu is z Phi(z) with the
+ * normal distribution's Phi, gelu_tanh z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2. y may
+ * be the memory of residual, row for row. A training step with an activation passes `z`, which
+ * the gradient reads: z rounded to the element type and kept finite. */
+#define SO3LR_NO_ACTIVATION 0
+#define SO3LR_SILU 1
+#define SO3LR_GELU 2
+#define SO3LR_GELU_TANH 3
+#define SO3LR_RELU 4
+typedef struct {
+  long long rows, n, k;       /* n, k <= 2^20 */
+  int dtype;                  /* x, w, residual, y, z */
+  int bias_dtype;             /* dtype or SO3LR_FLOAT32 */
+  int activation;
+  const void *x;              /* rows x k */
+  long long x_stride;
+  const void *w;              /* n x k: output channels are rows */
+  long long w_stride;
+  const void *bias;           /* n, optional */
+  const void *residual;       /* rows x n, optional */
+  long long residual_stride;
+  void *y;                    /* rows x n */
+  long long y_stride;
+  void *z;                    /* rows x n, optional */
+  long long z_stride;
+} so3lr_linear_args;
+long long so3lr_linear_workspace(const so3lr_linear_args *args);
+int so3lr_linear(const so3lr_linear_args *args, void *workspace, long long workspace_bytes, void *stream, char *err,
+                 size_t errlen);
+
+/* Gradients of so3lr_linear for dy, each optional (the residual's is dy):
+ *   dz = dy act'(z),  dx = dz W,  dw = dz^T x,  dbias = sum over rows of dz
+ * dz is rounded to the element type for the products, not for dbias. */
+typedef struct {
+  long long rows, n, k;
+  int dtype;                  /* dy, x, w, z, dx, dw */
+  int bias_dtype;             /* dbias: dtype or SO3LR_FLOAT32 */
+  int activation;
+  const void *dy;             /* rows x n */
+  long long dy_stride;
+  const void *x;              /* read for dw */
+  long long x_stride;
+  const void *w;              /* read for dx */
+  long long w_stride;
+  const void *z;              /* from the forward pass; not read without an activation */
+  long long z_stride;
+  void *dx;                   /* rows x k, or NULL */
+  long long dx_stride;
+  void *dw;                   /* n x k, contiguous, or NULL */
+  void *dbias;                /* n, or NULL */
+} so3lr_linear_backward_args;
+long long so3lr_linear_backward_workspace(const so3lr_linear_backward_args *args);
+int so3lr_linear_backward(const so3lr_linear_backward_args *args, void *workspace, long long workspace_bytes,
+                          void *stream, char *err, size_t errlen);
+
 /* The norms on both sides of a block's boundary, width <= 16384: the block's output x is
  * normalised, gated and added to the scaled residual stream, and the stream is normalised
  * for the next block,

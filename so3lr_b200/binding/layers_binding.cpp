@@ -402,6 +402,112 @@ PyObject *feed_forward_backward(Args o) {
   return tuple(wrap(dx), wrap(dwg), wrap(dwu), wrap(dwd));
 }
 
+// a whole number of a Python int
+int whole(PyObject *o, const char *what) {
+  const long v = PyLong_AsLong(o);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(what, " must be a whole number");
+  }
+  return int(v);
+}
+
+// linear(x, weight, bias | None, residual | None, activation, keep) -> y, or with keep (y, z | None)
+PyObject *linear(Args o) {
+  const Tensor &x = tensor(o[0], "x");
+  const Rows r = rows_of(x, "x");
+  so3lr_linear_args a{};
+  a.dtype = a.bias_dtype = float_type(r.type, "x", true);
+  const Rows w = rows_like(tensor(o[1], "weight"), "weight", r, r.type, -1, r.width);
+  if (w.rows < 1) refuse("weight must have at least one row");
+  const bool keep = PyObject_IsTrue(o[5]);
+  const c10::cuda::CUDAGuard guard(r.device);
+  a.rows = r.rows;
+  a.n = w.rows;
+  a.k = r.width;
+  a.activation = whole(o[4], "activation");
+  a.x = r.data;
+  a.x_stride = r.stride;
+  a.w = w.data;
+  a.w_stride = w.stride;
+  if (o[2] != Py_None) {
+    const Tensor &bias = tensor(o[2], "bias");
+    a.bias = vector_of(bias, "bias", r, w.rows, r.type, at::kFloat);
+    if (bias.scalar_type() == at::kFloat) a.bias_dtype = SO3LR_FLOAT32;
+  }
+  const at::DimVector shape = shaped(x, w.rows);
+  if (o[3] != Py_None) {
+    const Tensor &residual = tensor(o[3], "residual");
+    if (residual.sizes() != at::IntArrayRef(shape))
+      refuse("residual must have the shape of the result, ", at::IntArrayRef(shape), ", got ", residual.sizes());
+    const Rows q = rows_like(residual, "residual", r, r.type, r.rows, w.rows);
+    a.residual = q.data;
+    a.residual_stride = q.stride;
+  }
+  Tensor y = empty(shape, r.type, r.device), z;
+  a.y = y.data_ptr();
+  a.y_stride = w.rows;
+  if (keep && a.activation != SO3LR_NO_ACTIVATION) {  // rows on 16-byte boundaries
+    const int64_t padded = (w.rows + 7) / 8 * 8;
+    z = empty({r.rows, padded}, r.type, r.device);
+    a.z = z.data_ptr();
+    a.z_stride = padded;
+    if (padded != w.rows) z = z.narrow(1, 0, w.rows);
+  }
+  with_workspace(a, r.device, so3lr_linear_workspace, so3lr_linear);
+  if (!keep) return wrap(y);
+  return tuple(wrap(y), z.defined() ? wrap(z) : none());
+}
+
+// linear_backward(dy, x, weight, z | None, activation, bias dtype | None, dx wanted, dweight wanted)
+// -> (dx | None, dweight | None, dbias | None)
+PyObject *linear_backward(Args o) {
+  const Tensor &x = tensor(o[1], "x");
+  const Rows r = rows_of(x, "x");
+  so3lr_linear_backward_args a{};
+  a.dtype = a.bias_dtype = float_type(r.type, "x", true);
+  const Rows w = rows_like(tensor(o[2], "weight"), "weight", r, r.type, -1, r.width);
+  if (w.rows < 1) refuse("weight must have at least one row");
+  const c10::cuda::CUDAGuard guard(r.device);
+  const Rows d = rows_like(tensor(o[0], "dy"), "dy", r, r.type, r.rows, w.rows);
+  a.rows = r.rows;
+  a.n = w.rows;
+  a.k = r.width;
+  a.activation = whole(o[4], "activation");
+  a.dy = d.data;
+  a.dy_stride = d.stride;
+  a.x = r.data;
+  a.x_stride = r.stride;
+  a.w = w.data;
+  a.w_stride = w.stride;
+  if (a.activation != SO3LR_NO_ACTIVATION) {
+    if (o[3] == Py_None) refuse("saved does not come from linear_train on these tensors");
+    const Rows z = rows_like(tensor(o[3], "saved"), "saved", r, r.type, r.rows, w.rows);
+    a.z = z.data;
+    a.z_stride = z.stride;
+  }
+  Tensor dx, dw, dbias;
+  if (PyObject_IsTrue(o[6])) {
+    dx = empty(x.sizes(), r.type, r.device);
+    a.dx = dx.data_ptr();
+    a.dx_stride = r.width;
+  }
+  if (PyObject_IsTrue(o[7])) {
+    dw = empty({w.rows, r.width}, r.type, r.device);
+    a.dw = dw.data_ptr();
+  }
+  if (o[5] != Py_None) {
+    const at::ScalarType t = dtype_of(o[5], "bias");
+    if (t != r.type && t != at::kFloat) refuse("bias must be ", name_of(r.type), " or torch.float32, got ", name_of(t));
+    if (t == at::kFloat) a.bias_dtype = SO3LR_FLOAT32;
+    dbias = empty({w.rows}, t, r.device);
+    a.dbias = dbias.data_ptr();
+  }
+  with_workspace(a, r.device, so3lr_linear_backward_workspace, so3lr_linear_backward);
+  return tuple(dx.defined() ? wrap(dx) : none(), dw.defined() ? wrap(dw) : none(),
+               dbias.defined() ? wrap(dbias) : none());
+}
+
 // x, residual, weight, next_weight, gate | None, residual_scale | None of either sandwich call
 template <class A>
 Rows sandwich_operands(A &a, Args o, PyObject *eps) {
@@ -672,7 +778,8 @@ PyObject *method(PyObject *, PyObject *const *args, Py_ssize_t n) {
   { #f, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&method<f, n>)), METH_FASTCALL, nullptr }
 PyMethodDef g_methods[] = {METHOD(rms_norm, 5),        METHOD(rms_norm_backward, 5), METHOD(int8_linear, 6),
                            METHOD(gate_int8, 1),       METHOD(dequantize_int8, 3),   METHOD(feed_forward, 5),
-                           METHOD(feed_forward_backward, 7), METHOD(sandwich_norm, 7),
+                           METHOD(feed_forward_backward, 7), METHOD(linear, 6),          METHOD(linear_backward, 8),
+                           METHOD(sandwich_norm, 7),
                            METHOD(sandwich_norm_backward, 10), METHOD(adamw_step, 13),
                            METHOD(moment_values, 3),   METHOD(status, 1), METHOD(set_wait_limit, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_layers", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

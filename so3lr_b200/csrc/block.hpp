@@ -12,4 +12,19 @@ void launch_sandwich_norm(const so3lr_sandwich_norm_args &a, cudaStream_t s);
 long long sandwich_norm_backward_bytes(const so3lr_sandwich_norm_backward_args &a);
 void launch_sandwich_norm_backward(const so3lr_sandwich_norm_backward_args &a, void *workspace, cudaStream_t s);
 
+// dense.cu
+long long linear_bytes(const so3lr_linear_args &a);
+void launch_linear(const so3lr_linear_args &a, void *workspace, cudaStream_t s);
+long long linear_backward_bytes(const so3lr_linear_backward_args &a);
+void launch_linear_backward(const so3lr_linear_backward_args &a, void *workspace, cudaStream_t s);
+
+// linear.cu: dz (where dz is not dy itself) and, with `partial`, the bias gradient
+long long linear_elementwise_bytes(const so3lr_linear_backward_args &a);
+void launch_linear_elementwise(const so3lr_linear_backward_args &a, void *dz, long long dz_stride, float *partial,
+                               cudaStream_t s);
+
+// few_rows.cu
+inline bool few_rows(const so3lr_linear_args &a) { return few_rows(a.rows, 2 * a.n * a.k, 4 + a.k / 100); }
+void launch_linear_few(const so3lr_linear_args &a, cudaStream_t s);
+
 }  // namespace so3lr_b200

@@ -1,6 +1,6 @@
-// Dense products of the feed-forward layers on the tcgen05 tensor cores: 8-bit
-// products with row and channel scales, the gated block's forward pass and its
-// gradients.
+// Dense products of the layers on the tcgen05 tensor cores: 8-bit products with row
+// and channel scales, the gated block's forward pass and its gradients, the dense layer
+// with bias, activation and residual in its epilogue and its gradients.
 //
 // One persistent kernel. A CTA pair computes a tile of 256 rows x 256 accumulator
 // columns; each CTA stages its 128 rows of A and its 128 rows of B (half the
@@ -35,6 +35,8 @@
 #include <cstring>
 #include <string>
 
+#include "activation.cuh"
+#include "block.hpp"
 #include "layers_common.cuh"
 #include "model_host.hpp"
 #include "tensor_core.cuh"
@@ -58,7 +60,8 @@ enum Mode {
   kInt8,      // C = (A B^T) a_scale b_scale + bias
   kGated,     // C = silu(A G^T) * (A U^T): 128 columns of G and 128 of U per tile
   kGatedBack, // g, u as above and dh = DY Wd: C = dg, C2 = du
-  kKeptBack   // the same with g, u read from the forward pass: dh alone is computed
+  kKeptBack,  // the same with g, u read from the forward pass: dh alone is computed
+  kLinear     // C = act(A B^T + bias) + residual, C2 = A B^T + bias where it is kept
 };
 // Accumulator columns of a tile, TN: 256, or 128 where 256 would leave most pairs
 // without a tile. A narrow tile takes half the time a K block, and there are twice as
@@ -96,6 +99,11 @@ struct Params {
   const float *a_scales, *b_scales, *bias;
   uint32_t *partial;             // raw sums: [tile - whole][part][kTileM][TN]
   WaitLimit wait;
+  // kLinear (c2, ldc2: z, optional)
+  const void *bias16;            // a bias of the element type (`bias`: of float32)
+  const void *residual;
+  long long ldr, ldc2;
+  int act;
 };
 
 struct Item {
@@ -169,6 +177,58 @@ __device__ __forceinline__ void store_rows(unsigned char *stage, int lane, const
       for (int r = r0; r < rows; r += kRows, c += kRows * ldc) *c = slot(r, e / kPer)[e % kPer];
   }
   __syncwarp();
+}
+// The counterpart: 32 columns of each of the warp's rows through its staging, a row to a lane.
+// In two halves, so that the loads are under way while the accumulator is waited for.
+template <class T>
+__device__ __forceinline__ void fetch_rows(uint4 (&v)[4], int lane, const T *c, long long ldc, int rows) {
+  c += (lane >> 2) * ldc + (lane & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (8 * i + (lane >> 2) < rows) v[i] = *reinterpret_cast<const uint4 *>(c + 8 * i * ldc);
+}
+template <class T>
+__device__ __forceinline__ void spread_rows(unsigned char *stage, int lane, const uint4 (&v)[4],
+                                            Chunk<T, 8> (&out)[4]) {
+  auto slot = [&](int r, int piece) { return stage + 64 * r + 16 * (piece ^ ((r >> 1) & 3)); };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(slot(8 * i + (lane >> 2), lane & 3)) = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = *reinterpret_cast<const Chunk<T, 8> *>(slot(lane, i));
+  __syncwarp();
+}
+// the same for rows off the boundaries or past the last column, a column to a lane
+template <class T>
+__device__ __forceinline__ void gather_rows(unsigned char *stage, int lane, const T *c, long long ldc, int rows,
+                                            int cols, Chunk<T, 8> (&out)[4]) {
+  auto slot = [&](int r, int piece) { return reinterpret_cast<T *>(stage + 64 * r + 16 * (piece ^ ((r >> 1) & 3))); };
+  if (lane < cols)
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) slot(r, lane / 8)[lane % 8] = c[r * ldc + lane];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = *reinterpret_cast<const Chunk<T, 8> *>(slot(lane, i));
+  __syncwarp();
+}
+// the bias of 8 columns from c on; the same for all lanes
+template <class T>
+__device__ __forceinline__ void bias_of(const Params &p, int c, int n, float (&b)[8]) {
+  const T *half = static_cast<const T *>(p.bias16);
+  const bool on = (reinterpret_cast<uintptr_t>(p.bias) | reinterpret_cast<uintptr_t>(half)) % 16 == 0 && c + 8 <= n;
+  if (p.bias && on) {
+    const Chunk<float, 8> v = load_chunk<float, 8>(p.bias + c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = v.e[i];
+  } else if (half && on) {
+    const Chunk<T, 8> v = load_chunk<T, 8>(half + c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = to_float(v.e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      b[i] = c + i >= n ? 0.0f : p.bias ? p.bias[c + i] : half ? to_float(half[c + i]) : 0.0f;
+  }
 }
 // dg = dh u silu'(g), du = dh silu(g)
 __device__ __forceinline__ void gradients(float g, float u, float dh, float &dg, float &du) {
@@ -345,6 +405,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
       const Item w = item(done);
       const Problem &q = p.prob[w.prob];
       const int buf = done % S::kBuffers;
+      // only the 16-bit types have the other modes than kPlain and kInt8
+      using H = typename std::conditional<sizeof(T) == 2, T, __half>::type;
+      uint4 ahead[4];  // kLinear: the residual of the next 32 columns, the first loaded under the MMAs
+      auto fetch_residual = [&](int j) {
+        const int r0 = w.m0 + 128 * rank + 32 * quad, c = w.n0 + 32 * (S::kWarpChunks * part + j);
+        if (p.residual && w.partial == nullptr && (reinterpret_cast<uintptr_t>(p.residual) | (p.ldr * 2)) % 16 == 0 &&
+            c + 32 <= q.n) {
+          fetch_rows<H>(ahead, lane, static_cast<const H *>(p.residual) + r0 * p.ldr + c, p.ldr, q.m - r0);
+          return true;
+        }
+        return false;
+      };
+      bool fetched_ahead = false;
+      if constexpr (MODE == kLinear) fetched_ahead = fetch_residual(0);
       if (!__all_sync(0xffffffffu, wait(acc_full(buf), (done / S::kBuffers) & 1, 5))) break;
       tc::fence_after();
       const uint32_t acc = lanes + 256u * buf;
@@ -404,6 +478,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
                           q.n - c0 - h * kCols, wide);
           }
         }
+      } else if constexpr (MODE == kLinear) {
+#pragma unroll
+        for (int j = 0; j < S::kWarpChunks; ++j) {
+          const int col = 32 * (S::kWarpChunks * part + j), c0 = w.n0 + col;
+          uint32_t r[32];
+          tc::tmem_ld32(acc + col, r);
+          tc::wait_ld(r);
+          if (j == S::kWarpChunks - 1) release();
+          if (rows <= 0 || c0 >= q.n) continue;
+          if (w.partial) {  // raw sums: k_join has the rest
+            uint32_t *dst = w.partial + (128 * rank + 32 * quad) * TN + col;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              Chunk<float, 4> v[4];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i / 4].e[i % 4] = __uint_as_float(r[16 * h + i]);
+              store_rows<float>(stage, lane, v, reinterpret_cast<float *>(dst) + 16 * h, TN, rows, 16, true);
+            }
+            continue;
+          }
+          Chunk<H, 8> v[4];
+          if (p.bias || p.bias16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float b[8];
+              bias_of<H>(p, c0 + 8 * i, q.n, b);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) r[8 * i + e] = __float_as_uint(__uint_as_float(r[8 * i + e]) + b[e]);
+            }
+          }
+          if (p.c2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float z[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) z[e] = kept<H>(__uint_as_float(r[8 * i + e]));
+              v[i] = to_chunk<H, 8>(z);
+            }
+            store_rows<H>(stage, lane, v, static_cast<H *>(p.c2) + row0 * p.ldc2 + c0, p.ldc2, rows, q.n - c0,
+                          (reinterpret_cast<uintptr_t>(p.c2) | (p.ldc2 * 2)) % 16 == 0);
+          }
+          by_activation(p.act, [&](auto act) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(activate<decltype(act)::value>(__uint_as_float(r[i])));
+          });
+          if (p.residual) {
+            if (fetched_ahead)
+              spread_rows<H>(stage, lane, ahead, v);
+            else
+              gather_rows<H>(stage, lane, static_cast<const H *>(p.residual) + row0 * p.ldr + c0, p.ldr, rows,
+                             q.n - c0, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + to_float(v[i / 8].e[i % 8]));
+            if (j + 1 < S::kWarpChunks) fetched_ahead = fetch_residual(j + 1);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(r[8 * i + e]);
+            v[i] = to_chunk<H, 8>(y);
+          }
+          store_rows<H>(stage, lane, v, static_cast<H *>(q.c) + row0 * q.ldc + c0, q.ldc, rows, q.n - c0, wide);
+        }
       } else if constexpr (MODE == kKeptBack) {
         for (int j = 0; j < S::kWarpChunks; ++j) {
           const int col = 32 * (S::kWarpChunks * part + j), c0 = w.n0 + col;
@@ -451,8 +589,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
         const bool mine = part < S::kChunks, live = mine && rows > 0 && c0 < q.n;
         if (!mine) release();
         const long long at = row0 * q.ldc + c0;
-        // only the 16-bit types have these modes
-        using H = typename std::conditional<sizeof(T) == 2, T, __half>::type;
         Chunk<H, 8> out[4], out2[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -579,6 +715,23 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) 
     for (int j = 0; j < 4; ++j)
       if (col + j < q.n)
         f[j] = fmaf(float(s[j]) * p.a_scales[row], p.b_scales[col + j], p.bias ? p.bias[col + j] : 0.0f);
+  }
+  if constexpr (MODE == kLinear) {
+    const T *half = static_cast<const T *>(p.bias16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < q.n) {
+        f[j] += p.bias ? p.bias[col + j] : half ? to_float(half[col + j]) : 0.0f;
+        if (p.c2) static_cast<T *>(p.c2)[row * p.ldc2 + col + j] = from_float<T>(kept<T>(f[j]));
+      }
+    by_activation(p.act, [&](auto act) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = activate<decltype(act)::value>(f[j]);
+    });
+    if (p.residual)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < q.n) f[j] += to_float(static_cast<const T *>(p.residual)[row * p.ldr + col + j]);
   }
   const Chunk<T, 4> out = to_chunk<T, 4>(f);
   T *dst = static_cast<T *>(q.c) + row * q.ldc + col;
@@ -765,7 +918,7 @@ class Dense {
     allow_dynamic_smem(reinterpret_cast<const void *>(&k_dense<MODE, T, A_MN, B_MN, TN>), S::kSmem);
     p.wait = wait_limit();
     launch(k_dense<MODE, T, A_MN, B_MN, TN>, 2 * std::min(kPairs, p.items), kThreads, S::kSmem, stream_, p);
-    if constexpr (MODE == kPlain || MODE == kInt8) {
+    if constexpr (MODE == kPlain || MODE == kInt8 || MODE == kLinear) {
       if (p.splits == 1) return;
       const int rows = 256 / (TN / 4);  // of a block
       launch(k_join<MODE, T, TN>, dim3(kTileM / rows, (p.items - p.whole) / p.splits), 256, 0, stream_, p);
@@ -962,6 +1115,91 @@ void feed_forward_backward(Dense &d, const so3lr_feed_forward_backward_args &a) 
   d.run<kPlain, T, true, true>(p);
 }
 
+// ------------------------------------------------------------------- dense layer
+template <class T>
+void linear(Dense &d, const so3lr_linear_args &a) {
+  Params p{};
+  const Operand x = d.ready(Operand{a.x, a.x_stride, a.rows, a.k}), w = d.ready(Operand{a.w, a.w_stride, a.n, a.k});
+  p.problems = 1;
+  Problem &q = p.prob[0];
+  q.a[0] = 0;
+  q.b[0] = 1;
+  q.kb = q.kb0 = blocks_of(a.k, 64);
+  q.m = int(a.rows);
+  q.n = int(a.n);
+  q.c = a.y;
+  q.ldc = a.y_stride;
+  if (a.bias_dtype == SO3LR_FLOAT32)
+    p.bias = static_cast<const float *>(a.bias);
+  else
+    p.bias16 = a.bias;
+  p.residual = a.residual;
+  p.ldr = a.residual_stride;
+  p.c2 = a.z;
+  p.ldc2 = a.z_stride;
+  p.act = a.activation;
+  d.plan<kLinear>(p, true);
+  if (d.dry()) return;
+  p.maps = 2;
+  p.map[0] = d.map(x, 128);
+  p.map[1] = d.map(w, p.narrow ? 64 : 128);
+  d.run<kLinear, T, false, false>(p);
+}
+
+template <class T>
+void linear_backward(Dense &d, const so3lr_linear_backward_args &a, cudaStream_t s) {
+  const bool act = a.activation != SO3LR_NO_ACTIVATION;
+  Operand dz{a.dy, a.dy_stride, a.rows, a.n};
+  if (act) {
+    dz.stride = d.padded(a.n);
+    dz.data = d.scratch().take(a.rows * dz.stride * 2);
+  }
+  float *partial = a.dbias ? static_cast<float *>(d.scratch().take(linear_elementwise_bytes(a))) : nullptr;
+  if (!d.dry() && (act || partial))
+    launch_linear_elementwise(a, act ? const_cast<void *>(dz.data) : nullptr, dz.stride, partial, s);
+  if (!act && (a.dx || a.dw)) dz = d.ready(dz);
+  if (a.dx) {  // dz W
+    const Operand w = d.ready(Operand{a.w, a.w_stride, a.n, a.k});
+    Params p{};
+    p.problems = 1;
+    Problem &q = p.prob[0];
+    q.a[0] = 0;
+    q.b[0] = 1;
+    q.kb = q.kb0 = blocks_of(a.n, 64);
+    q.m = int(a.rows);
+    q.n = int(a.k);
+    q.c = a.dx;
+    q.ldc = a.dx_stride;
+    d.plan<kPlain>(p, true);
+    if (!d.dry()) {
+      p.maps = 2;
+      p.map[0] = d.map(dz, 128);
+      p.map[1] = d.map(w, 64);
+      d.run<kPlain, T, false, true>(p);
+    }
+  }
+  if (a.dw) {  // dz^T x
+    const Operand x = d.ready(Operand{a.x, a.x_stride, a.rows, a.k});
+    Params p{};
+    p.problems = 1;
+    Problem &q = p.prob[0];
+    q.a[0] = 0;
+    q.b[0] = 1;
+    q.kb = q.kb0 = blocks_of(a.rows, 64);
+    q.m = int(a.n);
+    q.n = int(a.k);
+    q.c = a.dw;
+    q.ldc = a.k;
+    d.plan<kPlain>(p, true);
+    if (!d.dry()) {
+      p.maps = 2;
+      p.map[0] = d.map(dz, 64);
+      p.map[1] = d.map(x, 64);
+      d.run<kPlain, T, true, true>(p);
+    }
+  }
+}
+
 template <class A, class F>
 long long dry_run(const A &a, int elem, F &&f) {
   if (a.rows == 0) return 0;
@@ -1053,6 +1291,29 @@ void launch_feed_forward_backward(const so3lr_feed_forward_backward_args &a, voi
   }
   Dense d(workspace, 2, s, false);
   by_half(a.dtype, [&](auto t) { feed_forward_backward<decltype(t)>(d, a); });
+}
+
+long long linear_bytes(const so3lr_linear_args &a) {
+  if (few_rows(a)) return 0;
+  return dry_run(a, 2, [&](Dense &d) { linear<__half>(d, a); });
+}
+void launch_linear(const so3lr_linear_args &a, void *workspace, cudaStream_t s) {
+  if (few_rows(a)) return launch_linear_few(a, s);
+  Dense d(workspace, 2, s, false);
+  by_half(a.dtype, [&](auto t) { linear<decltype(t)>(d, a); });
+}
+
+long long linear_backward_bytes(const so3lr_linear_backward_args &a) {
+  return dry_run(a, 2, [&](Dense &d) { linear_backward<__half>(d, a, nullptr); });
+}
+void launch_linear_backward(const so3lr_linear_backward_args &a, void *workspace, cudaStream_t s) {
+  if (a.rows == 0) {
+    if (a.dw) SO3_CUDA(cudaMemsetAsync(a.dw, 0, std::size_t(a.n) * a.k * 2, s));
+    if (a.dbias) SO3_CUDA(cudaMemsetAsync(a.dbias, 0, std::size_t(a.n) * (a.bias_dtype == SO3LR_FLOAT32 ? 4 : 2), s));
+    return;
+  }
+  Dense d(workspace, 2, s, false);
+  by_half(a.dtype, [&](auto t) { linear_backward<decltype(t)>(d, a, s); });
 }
 
 }  // namespace so3lr_b200

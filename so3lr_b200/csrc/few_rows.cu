@@ -13,6 +13,8 @@
 // loads 16 contiguous bytes (words 0..3) of its row and of its channel at the same
 // place, feeds words 0, 1 to one MMA and 2, 3 to the next; both operands use the
 // same permutation of the contraction, so the sums are those of the formula.
+#include "activation.cuh"
+#include "block.hpp"
 #include "layers_common.cuh"
 #include "model_host.hpp"
 #include "tensor_core.cuh"
@@ -92,13 +94,19 @@ struct FewArgs {
   long long y_stride;
   const float *a_scales, *b_scales, *bias;  // 8-bit products
   void *rest;                    // GATED: what y's rounding leaves of the hidden layer; LO: the same of x
+  // LAYER
+  const void *bias16, *residual; // a bias of the element type (`bias`: of float32)
+  long long residual_stride;
+  void *z;                       // optional: act's argument
+  long long z_stride;
+  int act;
 };
 
 // y = x w^T (8 bits: scaled), or silu(x w^T) * (x w2^T). TWO: more than 8 rows. LO: x is
 // the sum of x and a.rest (rows like x's). The hidden layer is handed over in two
 // 16-bit parts, so that its rounding does not show in y: with this few rows the second
-// MMA costs nothing beside the weights' loads.
-template <class E, class O, bool GATED, bool LO, bool TWO, int ALIGN>
+// MMA costs nothing beside the weights' loads. LAYER: y = act(x w^T + bias) + residual.
+template <class E, class O, bool GATED, bool LO, bool TWO, int ALIGN, bool LAYER>
 __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(const FewArgs a) {
   constexpr bool kInt8 = std::is_same<E, signed char>::value;
   using Acc = typename std::conditional<kInt8, int, float>::type;
@@ -227,6 +235,12 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
       y = silu_f32(float(sum[0])) * float(sum[kOut - 1]);
     else
       y = float(sum[0]);
+    if constexpr (LAYER) {
+      y += a.bias ? a.bias[c] : a.bias16 ? to_float(static_cast<const O *>(a.bias16)[c]) : 0.0f;
+      if (a.z) static_cast<O *>(a.z)[(row0 + row) * a.z_stride + c] = from_float<O>(kept<O>(y));
+      by_activation(a.act, [&](auto act) { y = activate<decltype(act)::value>(y); });
+      if (a.residual) y += to_float(static_cast<const O *>(a.residual)[(row0 + row) * a.residual_stride + c]);
+    }
     const O rounded = from_float<O>(y);
     static_cast<O *>(a.y)[(row0 + row) * a.y_stride + c] = rounded;
     if (GATED) {  // nothing is left of an infinity or a NaN
@@ -241,7 +255,7 @@ bool rows_on(int bytes, const void *p, long long stride, long long rows, int siz
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (rows == 1 || stride * size % bytes == 0));
 }
 
-template <class E, class O, bool GATED, bool LO>
+template <class E, class O, bool GATED, bool LO, bool LAYER = false>
 void run(const FewArgs &a, cudaStream_t s) {
   constexpr int kPer = 16 / sizeof(E);
   auto all_on = [&](int bytes) {
@@ -263,7 +277,7 @@ void run(const FewArgs &a, cudaStream_t s) {
   while (splits < 8 && blocks * splits < kSmCount && steps >= 12 * int(splits) * warps) splits *= 2;
   auto go = [&](auto align) {
     constexpr int A = decltype(align)::value;
-    launch_clusters(a.rows > 8 ? &k_few_rows<E, O, GATED, LO, true, A> : &k_few_rows<E, O, GATED, LO, false, A>,
+    launch_clusters(a.rows > 8 ? &k_few_rows<E, O, GATED, LO, true, A, LAYER> : &k_few_rows<E, O, GATED, LO, false, A, LAYER>,
                     dim3(channels * splits, groups), unsigned(32 * warps), splits > 1 ? splits : 0, 0, s, a);
   };
   if (all_on(16))
@@ -300,6 +314,23 @@ void launch_feed_forward_few(const so3lr_feed_forward_args &f, void *h, long lon
     run<__half, __half, true, false>(up, s);
     run<__half, __half, false, true>(down, s);
   }
+}
+
+void launch_linear_few(const so3lr_linear_args &l, cudaStream_t s) {
+  FewArgs a{int(l.rows), int(l.n), int(l.k), l.x, l.x_stride, l.w, nullptr, l.w_stride, 0, l.y, l.y_stride};
+  if (l.bias_dtype == SO3LR_FLOAT32)
+    a.bias = static_cast<const float *>(l.bias);
+  else
+    a.bias16 = l.bias;
+  a.residual = l.residual;
+  a.residual_stride = l.residual_stride;
+  a.z = l.z;
+  a.z_stride = l.z_stride;
+  a.act = l.activation;
+  if (l.dtype == SO3LR_BFLOAT16)
+    run<__nv_bfloat16, __nv_bfloat16, false, false, true>(a, s);
+  else
+    run<__half, __half, false, false, true>(a, s);
 }
 
 }  // namespace so3lr_b200

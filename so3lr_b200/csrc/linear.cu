@@ -1,0 +1,161 @@
+// Elementwise part of the dense layer's gradient: dz = dy act'(z) in the element type, as the
+// products after it read it, and the bias gradient, its column sums in float32 before that
+// rounding.
+//
+// Bound by HBM (dy and z in, dz out). A warp takes 256 columns of a row, or several rows of
+// narrow ones, 8 columns a lane; a block walks down its share of the rows and writes one row
+// of sums, which k_bias_sum adds in order.
+#include <algorithm>
+
+#include "activation.cuh"
+#include "block.hpp"
+
+namespace so3lr_b200 {
+namespace {
+
+constexpr int kVec = 8, kWarps = 8;
+
+struct BackArgs {
+  long long rows, rows_per_block;
+  int n, lanes;               // lanes: of a warp that share a row, a power of two
+  const void *dy, *z;
+  long long dy_stride, z_stride;
+  void *dz;                   // nullptr: dy itself is dz
+  long long dz_stride;
+  float *partial;             // [blocks of a column strip][n], or nullptr
+  bool dy_wide, z_wide;       // rows on 16-byte boundaries
+};
+
+template <class T>
+__device__ __forceinline__ Chunk<T, kVec> load_part(const T *p, bool wide, int left) {
+  if (wide && left >= kVec) return load_chunk<T, kVec>(p);
+  Chunk<T, kVec> c;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) c.e[i] = i < left ? p[i] : from_float<T>(0.0f);
+  return c;
+}
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs a) {
+  __shared__ float sums[kWarps * 32][kVec + 1];
+  dependents_may_start();
+  wait_for_predecessors();
+  const int lane = threadIdx.x & 31, t = lane % a.lanes, rows_of_warp = 32 / a.lanes;
+  const int c = (blockIdx.x * a.lanes + t) * kVec, left = a.n - c;
+  const int step = kWarps * rows_of_warp;
+  const long long begin = blockIdx.y * a.rows_per_block, end = min(a.rows, begin + a.rows_per_block);
+  float total[kVec] = {};
+  auto one = [&](const Chunk<T, kVec> &dy, const Chunk<T, kVec> &z, long long row) {
+    float d[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      d[i] = to_float(dy.e[i]);
+      if (ACT != SO3LR_NO_ACTIVATION) d[i] *= slope<ACT>(to_float(z.e[i]));
+      total[i] += d[i];
+    }
+    if (ACT == SO3LR_NO_ACTIVATION) return;
+    T *dz = static_cast<T *>(a.dz) + row * a.dz_stride + c;  // rows are padded to whole chunks
+    store_chunk<T, kVec>(dz, to_chunk<T, kVec>(d));
+  };
+  if (left > 0) {
+    const T *dy = static_cast<const T *>(a.dy) + c, *z = static_cast<const T *>(a.z) + c;
+    long long row = begin + (threadIdx.x >> 5) * rows_of_warp + lane / a.lanes;
+    constexpr int kAtOnce = 4;
+    for (; row < end; row += kAtOnce * step) {
+      Chunk<T, kVec> cd[kAtOnce], cz[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (row + k * step < end) {
+          cd[k] = load_part(dy + (row + k * step) * a.dy_stride, a.dy_wide, left);
+          if (ACT != SO3LR_NO_ACTIVATION) cz[k] = load_part(z + (row + k * step) * a.z_stride, a.z_wide, left);
+        }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (row + k * step < end) one(cd[k], cz[k], row + k * step);
+    }
+  }
+  if (!a.partial) return;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) sums[threadIdx.x][i] = total[i];
+  __syncthreads();
+  // thread: one column of the strip; the rows' owners in order
+  for (int i = threadIdx.x; i < a.lanes * kVec; i += blockDim.x) {
+    const int column = blockIdx.x * a.lanes * kVec + i;
+    if (column >= a.n) break;
+    float all = 0.0f;
+    for (int k = i / kVec; k < kWarps * 32; k += a.lanes) all += sums[k][i % kVec];
+    a.partial[(size_t)blockIdx.y * a.n + column] = all;
+  }
+}
+
+template <class B>
+__global__ void k_bias_sum(int parts, int n, const float *partial, B *out) {
+  __shared__ float part[32][33];
+  dependents_may_start();
+  wait_for_predecessors();
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float total = 0.0f;
+  if (c < n)
+#pragma unroll 8
+    for (int k = threadIdx.y; k < parts; k += 32) total += partial[(size_t)k * n + c];
+  part[threadIdx.y][threadIdx.x] = total;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < n) {
+    total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) total += part[k][threadIdx.x];
+    out[c] = from_float<B>(total);
+  }
+}
+
+struct Plan {
+  int lanes, strips, parts;
+  long long rows_per_block;
+};
+Plan plan(long long rows, long long n) {
+  Plan p;
+  p.lanes = 1;
+  while (p.lanes < 32 && p.lanes * kVec < n) p.lanes *= 2;
+  p.strips = int((n + p.lanes * kVec - 1) / (p.lanes * kVec));
+  // about four blocks an SM in all, 32 rows of a warp or more
+  const long long least = 4LL * kWarps * (32 / p.lanes);
+  const long long want = std::max<long long>(1, 8LL * kSmCount / p.strips);
+  p.rows_per_block = std::max(least, (rows + want - 1) / want);
+  p.parts = int((rows + p.rows_per_block - 1) / p.rows_per_block);
+  return p;
+}
+bool wide(const void *p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0; }
+
+}  // namespace
+
+long long linear_elementwise_bytes(const so3lr_linear_backward_args &a) {
+  return a.dbias && a.rows > 0 ? (long long)plan(a.rows, a.n).parts * a.n * 4 : 0;
+}
+
+void launch_linear_elementwise(const so3lr_linear_backward_args &a, void *dz, long long dz_stride, float *partial,
+                               cudaStream_t s) {
+  const Plan p = plan(a.rows, a.n);
+  const BackArgs b{a.rows, p.rows_per_block, int(a.n), p.lanes, a.dy, a.z, a.dy_stride, a.z_stride, dz, dz_stride,
+                   partial, wide(a.dy, a.dy_stride), wide(a.z, a.z_stride)};
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    void (*kernel)(BackArgs) = a.activation == SO3LR_SILU        ? &k_linear_backward<T, SO3LR_SILU>
+                               : a.activation == SO3LR_GELU      ? &k_linear_backward<T, SO3LR_GELU>
+                               : a.activation == SO3LR_GELU_TANH ? &k_linear_backward<T, SO3LR_GELU_TANH>
+                               : a.activation == SO3LR_RELU      ? &k_linear_backward<T, SO3LR_RELU>
+                                                                 : &k_linear_backward<T, SO3LR_NO_ACTIVATION>;
+    launch(kernel, dim3(p.strips, p.parts), 32 * kWarps, 0, s, b);
+    if (!partial) return;
+    const dim3 grid(unsigned((a.n + 31) / 32)), block(32, 32);
+    if (a.bias_dtype == SO3LR_FLOAT32)
+      launch(k_bias_sum<float>, grid, block, 0, s, p.parts, int(a.n), partial, static_cast<float *>(a.dbias));
+    else
+      launch(k_bias_sum<T>, grid, block, 0, s, p.parts, int(a.n), partial, static_cast<T *>(a.dbias));
+  };
+  if (a.dtype == SO3LR_BFLOAT16)
+    go(__nv_bfloat16{});
+  else
+    go(__half{});
+}
+
+}  // namespace so3lr_b200

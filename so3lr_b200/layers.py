@@ -42,7 +42,7 @@ except (ImportError, So3lrError) as e:
     raise ImportError(f"the feed-forward layers' module is missing or does not fit the installed torch ({e}): build it "
                       "with `python -m so3lr_b200.build`, which needs a torch with CUDA and Python's headers") from e
 
-__all__ = ["rms_norm", "rms_norm_int8", "rms_norm_backward", "sandwich_norm", "sandwich_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
+__all__ = ["linear", "linear_train", "linear_backward", "rms_norm", "rms_norm_int8", "rms_norm_backward", "sandwich_norm", "sandwich_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
            "quantize_weight", "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock",
            "Int8FeedForwardBlock", "check_status", "set_wait_limit"]
 
@@ -112,6 +112,63 @@ def rms_norm_backward(dy, s, weight, ds=None, *, eps: float = 1e-6):
     """(dx, dweight) of rms_norm for the gradient dy of y and, optionally, ds that
     of s; dx is also the residual's gradient."""
     return _layers.rms_norm_backward(dy, s, weight, ds, eps)
+
+
+# ----------------------------------------------------------------------- dense layer
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
+
+
+def _activation(name):
+    try:
+        return _ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation must be one of {', '.join(map(repr, _ACTIVATIONS))}, got {name!r}") from None
+
+
+class _LinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        y, z = _layers.linear(x, weight, bias, residual, act, True)
+        ctx.save_for_backward(x, weight, z)
+        ctx.act, ctx.bias = act, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dweight = dbias = None
+        if any(need[:3]):
+            dx, dweight, dbias = _layers.linear_backward(_dense_rows(dy), x, weight, z, ctx.act,
+                                                         ctx.bias if need[2] else None, need[0], need[1])
+        return dx, dweight, dbias, dy if need[3] else None, None
+
+
+def linear(x, weight, bias=None, residual=None, *, activation=None):
+    """y = act(x @ weight.T + bias) + residual, bfloat16 or float16: x [..., k], weight [n, k],
+    bias [n] of x's type or float32, residual [..., n]. activation: None, "silu", "gelu"
+    (z Phi(z)), "gelu_tanh" or "relu". Sums and everything after them are float32, y is
+    rounded once. For the gradients of an activation its argument is kept in x's type."""
+    act = _activation(activation)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearFunction.apply(x, weight, bias, residual, act)
+    return _layers.linear(x, weight, bias, residual, act, False)
+
+
+def linear_train(x, weight, bias=None, residual=None, *, activation=None):
+    """(y, saved): linear, and what linear_backward needs of it: x, weight and, with an
+    activation, its argument rounded to x's type."""
+    act = _activation(activation)
+    y, z = _layers.linear(x, weight, bias, residual, act, True)
+    return y, (x, weight, z, act, None if bias is None else bias.dtype)
+
+
+def linear_backward(dy, saved):
+    """(dx, dweight, dbias) for the gradient dy of linear_train's y, dbias None without a
+    bias; the residual's gradient is dy."""
+    x, weight, z, act, bias = saved
+    return _layers.linear_backward(dy, x, weight, z, act, bias, True, True)
 
 
 # --------------------------------------------------- norms on both sides of a block
