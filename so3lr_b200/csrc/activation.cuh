@@ -42,11 +42,20 @@ __device__ __forceinline__ float slope(float z) {
 }
 // z as it is kept for the backward pass, rounded to the element type: its derivative is then off
 // by at most half a unit of z, as much as the rounding of dz itself. Kept finite, where every
-// derivative has its limit (of a NaN nothing is left to keep).
+// derivative has its limit; a NaN stays one.
 template <class T>
-__device__ __forceinline__ float kept(float z) {
-  const float most = std::is_same<T, __half>::value ? 65504.0f : 3.3895314e38f;
-  return z != z ? z : fminf(fmaxf(z, -most), most);
+__device__ __forceinline__ uint32_t kept(float a, float b) {
+  uint32_t r;
+  if (std::is_same<T, __half>::value)
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ T kept(float z) {
+  const uint32_t r = kept<T>(z, 0.0f);
+  return *reinterpret_cast<const T *>(&r);
 }
 // f(std::integral_constant activation)
 template <class F>

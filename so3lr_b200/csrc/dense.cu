@@ -211,24 +211,26 @@ __device__ __forceinline__ void gather_rows(unsigned char *stage, int lane, cons
   for (int i = 0; i < 4; ++i) out[i] = *reinterpret_cast<const Chunk<T, 8> *>(slot(lane, i));
   __syncwarp();
 }
-// the bias of 8 columns from c on; the same for all lanes
+// the bias of column c
 template <class T>
-__device__ __forceinline__ void bias_of(const Params &p, int c, int n, float (&b)[8]) {
-  const T *half = static_cast<const T *>(p.bias16);
-  const bool on = (reinterpret_cast<uintptr_t>(p.bias) | reinterpret_cast<uintptr_t>(half)) % 16 == 0 && c + 8 <= n;
-  if (p.bias && on) {
-    const Chunk<float, 8> v = load_chunk<float, 8>(p.bias + c);
+__device__ __forceinline__ float bias_of(const Params &p, int c, int n) {
+  if (c >= n) return 0.0f;
+  return p.bias ? p.bias[c] : p.bias16 ? to_float(static_cast<const T *>(p.bias16)[c]) : 0.0f;
+}
+// r[i] += the value of lane i, through the warp's staging
+__device__ __forceinline__ void add_columns(unsigned char *stage, int lane, float v, uint32_t (&r)[32]) {
+  float *column = reinterpret_cast<float *>(stage);
+  column[lane] = v;
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = v.e[i];
-  } else if (half && on) {
-    const Chunk<T, 8> v = load_chunk<T, 8>(half + c);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = to_float(v.e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      b[i] = c + i >= n ? 0.0f : p.bias ? p.bias[c + i] : half ? to_float(half[c + i]) : 0.0f;
+  for (int i = 0; i < 32; i += 4) {
+    const float4 b = *reinterpret_cast<const float4 *>(column + i);
+    r[i] = __float_as_uint(__uint_as_float(r[i]) + b.x);
+    r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) + b.y);
+    r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) + b.z);
+    r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) + b.w);
   }
+  __syncwarp();
 }
 // dg = dh u silu'(g), du = dh silu(g)
 __device__ __forceinline__ void gradients(float g, float u, float dh, float &dg, float &du) {
@@ -418,7 +420,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
         return false;
       };
       bool fetched_ahead = false;
-      if constexpr (MODE == kLinear) fetched_ahead = fetch_residual(0);
+      float bias = 0.0f;
+      if constexpr (MODE == kLinear) {
+        fetched_ahead = fetch_residual(0);
+        bias = bias_of<H>(p, w.n0 + 32 * S::kWarpChunks * part + lane, q.n);
+      }
       if (!__all_sync(0xffffffffu, wait(acc_full(buf), (done / S::kBuffers) & 1, 5))) break;
       tc::fence_after();
       const uint32_t acc = lanes + 256u * buf;
@@ -479,7 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           }
         }
       } else if constexpr (MODE == kLinear) {
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < S::kWarpChunks; ++j) {
           const int col = 32 * (S::kWarpChunks * part + j), c0 = w.n0 + col;
           uint32_t r[32];
@@ -500,21 +506,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           }
           Chunk<H, 8> v[4];
           if (p.bias || p.bias16) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float b[8];
-              bias_of<H>(p, c0 + 8 * i, q.n, b);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) r[8 * i + e] = __float_as_uint(__uint_as_float(r[8 * i + e]) + b[e]);
-            }
+            add_columns(stage, lane, bias, r);
+            if (j + 1 < S::kWarpChunks) bias = bias_of<H>(p, c0 + 32 + lane, q.n);
           }
           if (p.c2) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float z[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) z[e] = kept<H>(__uint_as_float(r[8 * i + e]));
-              v[i] = to_chunk<H, 8>(z);
+              for (int e = 0; e < 8; e += 2)
+                *reinterpret_cast<uint32_t *>(&v[i].e[e]) =
+                    kept<H>(__uint_as_float(r[8 * i + e]), __uint_as_float(r[8 * i + e + 1]));
             }
             store_rows<H>(stage, lane, v, static_cast<H *>(p.c2) + row0 * p.ldc2 + c0, p.ldc2, rows, q.n - c0,
                           (reinterpret_cast<uintptr_t>(p.c2) | (p.ldc2 * 2)) % 16 == 0);
@@ -722,7 +723,7 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Params p) 
     for (int j = 0; j < 4; ++j)
       if (col + j < q.n) {
         f[j] += p.bias ? p.bias[col + j] : half ? to_float(half[col + j]) : 0.0f;
-        if (p.c2) static_cast<T *>(p.c2)[row * p.ldc2 + col + j] = from_float<T>(kept<T>(f[j]));
+        if (p.c2) static_cast<T *>(p.c2)[row * p.ldc2 + col + j] = kept<T>(f[j]);
       }
     by_activation(p.act, [&](auto act) {
 #pragma unroll

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(32 * max_warps(TWO), TWO ? 3 : 2) k_few_rows(c
       y = float(sum[0]);
     if constexpr (LAYER) {
       y += a.bias ? a.bias[c] : a.bias16 ? to_float(static_cast<const O *>(a.bias16)[c]) : 0.0f;
-      if (a.z) static_cast<O *>(a.z)[(row0 + row) * a.z_stride + c] = from_float<O>(kept<O>(y));
+      if (a.z) static_cast<O *>(a.z)[(row0 + row) * a.z_stride + c] = kept<O>(y);
       by_activation(a.act, [&](auto act) { y = activate<decltype(act)::value>(y); });
       if (a.residual) y += to_float(static_cast<const O *>(a.residual)[(row0 + row) * a.residual_stride + c]);
     }

@@ -26,8 +26,9 @@ struct BackArgs {
   bool dy_wide, z_wide;       // rows on 16-byte boundaries
 };
 
-template <class T>
+template <bool WIDE, class T>
 __device__ __forceinline__ Chunk<T, kVec> load_part(const T *p, bool wide, int left) {
+  if (WIDE) return load_chunk<T, kVec>(p);
   if (wide && left >= kVec) return load_chunk<T, kVec>(p);
   Chunk<T, kVec> c;
 #pragma unroll
@@ -35,7 +36,8 @@ __device__ __forceinline__ Chunk<T, kVec> load_part(const T *p, bool wide, int l
   return c;
 }
 
-template <class T, int ACT>
+// WIDE: all rows on 16-byte boundaries and of whole chunks
+template <class T, int ACT, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs a) {
   __shared__ float sums[kWarps * 32][kVec + 1];
   dependents_may_start();
@@ -60,18 +62,22 @@ __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs 
   if (left > 0) {
     const T *dy = static_cast<const T *>(a.dy) + c, *z = static_cast<const T *>(a.z) + c;
     long long row = begin + (threadIdx.x >> 5) * rows_of_warp + lane / a.lanes;
-    constexpr int kAtOnce = 4;
-    for (; row < end; row += kAtOnce * step) {
+    constexpr int kAtOnce = WIDE ? 4 : 1;
+    for (; row + (kAtOnce - 1) * step < end; row += kAtOnce * step) {
       Chunk<T, kVec> cd[kAtOnce], cz[kAtOnce];
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
-        if (row + k * step < end) {
-          cd[k] = load_part(dy + (row + k * step) * a.dy_stride, a.dy_wide, left);
-          if (ACT != SO3LR_NO_ACTIVATION) cz[k] = load_part(z + (row + k * step) * a.z_stride, a.z_wide, left);
-        }
+      for (int k = 0; k < kAtOnce; ++k) {
+        cd[k] = load_part<WIDE>(dy + (row + k * step) * a.dy_stride, a.dy_wide, left);
+        if (ACT != SO3LR_NO_ACTIVATION) cz[k] = load_part<WIDE>(z + (row + k * step) * a.z_stride, a.z_wide, left);
+      }
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
-        if (row + k * step < end) one(cd[k], cz[k], row + k * step);
+      for (int k = 0; k < kAtOnce; ++k) one(cd[k], cz[k], row + k * step);
+    }
+    for (; row < end; row += step) {
+      const Chunk<T, kVec> cd = load_part<WIDE>(dy + row * a.dy_stride, a.dy_wide, left);
+      Chunk<T, kVec> cz{};
+      if (ACT != SO3LR_NO_ACTIVATION) cz = load_part<WIDE>(z + row * a.z_stride, a.z_wide, left);
+      one(cd, cz, row);
     }
   }
   if (!a.partial) return;
@@ -139,11 +145,17 @@ void launch_linear_elementwise(const so3lr_linear_backward_args &a, void *dz, lo
                    partial, wide(a.dy, a.dy_stride), wide(a.z, a.z_stride)};
   auto go = [&](auto t) {
     using T = decltype(t);
-    void (*kernel)(BackArgs) = a.activation == SO3LR_SILU        ? &k_linear_backward<T, SO3LR_SILU>
-                               : a.activation == SO3LR_GELU      ? &k_linear_backward<T, SO3LR_GELU>
-                               : a.activation == SO3LR_GELU_TANH ? &k_linear_backward<T, SO3LR_GELU_TANH>
-                               : a.activation == SO3LR_RELU      ? &k_linear_backward<T, SO3LR_RELU>
-                                                                 : &k_linear_backward<T, SO3LR_NO_ACTIVATION>;
+    auto by_width = [&](auto act) {
+      constexpr int A = decltype(act)::value;
+      return b.dy_wide && (A == SO3LR_NO_ACTIVATION || b.z_wide) && a.n % kVec == 0 ? &k_linear_backward<T, A, true>
+                                                                                   : &k_linear_backward<T, A, false>;
+    };
+    using std::integral_constant;
+    void (*kernel)(BackArgs) = a.activation == SO3LR_SILU        ? by_width(integral_constant<int, SO3LR_SILU>{})
+                               : a.activation == SO3LR_GELU      ? by_width(integral_constant<int, SO3LR_GELU>{})
+                               : a.activation == SO3LR_GELU_TANH ? by_width(integral_constant<int, SO3LR_GELU_TANH>{})
+                               : a.activation == SO3LR_RELU      ? by_width(integral_constant<int, SO3LR_RELU>{})
+                                                                 : by_width(integral_constant<int, SO3LR_NO_ACTIVATION>{});
     launch(kernel, dim3(p.strips, p.parts), 32 * kWarps, 0, s, b);
     if (!partial) return;
     const dim3 grid(unsigned((a.n + 31) / 32)), block(32, 32);
