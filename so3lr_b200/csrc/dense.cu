@@ -204,8 +204,16 @@ __device__ __forceinline__ void gather_rows(unsigned char *stage, int lane, cons
                                             int cols, Chunk<T, 8> (&out)[4]) {
   auto slot = [&](int r, int piece) { return reinterpret_cast<T *>(stage + 64 * r + 16 * (piece ^ ((r >> 1) & 3))); };
   if (lane < cols)
-#pragma unroll 8
-    for (int r = 0; r < rows; ++r) slot(r, lane / 8)[lane % 8] = c[r * ldc + lane];
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 16) {
+      T v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (r0 + i < rows) v[i] = c[(r0 + i) * ldc + lane];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (r0 + i < rows) slot(r0 + i, lane / 8)[lane % 8] = v[i];
+    }
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 4; ++i) out[i] = *reinterpret_cast<const Chunk<T, 8> *>(slot(lane, i));
@@ -875,11 +883,20 @@ class Dense {
   // are split along K where that saves more than the join costs: a K block takes a pair
   // 0.3 us, a join with its launch 5 (narrow tiles) to 7 us.
   template <int MODE>
-  void plan(Params &p, bool may_split) {
+  void plan(Params &p, bool may_split, bool deep = false) {
     long long tiles = count<MODE, 256>(p);
     int kb = 1 << 30;
     for (int i = 0; i < p.problems; ++i) kb = std::min(kb, p.prob[i].kb);
     p.narrow = MODE != kGatedBack && 2 * tiles <= kPairs && (!may_split || tiles * kb < 24 * kPairs);
+    // The dense layer's epilogue bounds it where the contraction is short: half tiles that make
+    // fewer rounds (24000 x 256 -> 1024 with silu 38.3 -> 35.7 us). A weight gradient contracted
+    // over many rows wants wide ones however few (24000 rows, 256 x 256: 29.1 -> 24.6).
+    if (MODE == kLinear && kb <= 8 && !p.narrow) {
+      const long long rounds = (tiles - 1) / kPairs + 1, half = (count<MODE, 128>(p) - 1) / kPairs + 1;
+      p.narrow = half < 2 * rounds;
+      if (!p.narrow) count<MODE, 256>(p);
+    }
+    if (deep && kb >= 128) p.narrow = false;
     if (p.narrow) tiles = count<MODE, 128>(p);
     if (tiles > (1LL << 30)) throw Error("feed-forward layers: the product has too many tiles");
     const int rest = int(tiles % kPairs);
@@ -1191,7 +1208,7 @@ void linear_backward(Dense &d, const so3lr_linear_backward_args &a, cudaStream_t
     q.n = int(a.k);
     q.c = a.dw;
     q.ldc = a.k;
-    d.plan<kPlain>(p, true);
+    d.plan<kPlain>(p, true, true);
     if (!d.dry()) {
       p.maps = 2;
       p.map[0] = d.map(dz, 64);

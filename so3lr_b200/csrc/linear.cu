@@ -123,8 +123,8 @@ Plan plan(long long rows, long long n) {
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes * kVec < n) p.lanes *= 2;
   p.strips = int((n + p.lanes * kVec - 1) / (p.lanes * kVec));
-  // about four blocks an SM in all, 32 rows of a warp or more
-  const long long least = 4LL * kWarps * (32 / p.lanes);
+  // about eight blocks an SM in all, a row for each warp at least
+  const long long least = (long long)kWarps * (32 / p.lanes);
   const long long want = std::max<long long>(1, 8LL * kSmCount / p.strips);
   p.rows_per_block = std::max(least, (rows + want - 1) / want);
   p.parts = int((rows + p.rows_per_block - 1) / p.rows_per_block);
