@@ -74,6 +74,25 @@ struct RowTeam {
     }
     return total;
   }
+  __device__ __forceinline__ float3 sum3(float a, float b, float c, float *slot, float2 *slot2) const {
+    a = add(a);
+    b = add(b);
+    c = add(c);
+    if (LANES) return make_float3(a, b, c);
+    const int warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+      slot[threadIdx.x >> 5] = a;
+      slot2[threadIdx.x >> 5] = make_float2(b, c);
+    }
+    __syncthreads();
+    float3 total = make_float3(0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < warps; ++i) {
+      total.x += slot[i];
+      total.y += slot2[i].x;
+      total.z += slot2[i].y;
+    }
+    return total;
+  }
   __device__ __forceinline__ uint32_t max(uint32_t v, uint32_t *slot) const {
     v = largest(v);
     if (LANES) return v;

@@ -207,10 +207,9 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
       ss = fmaf(to_float(es), to_float(es), ss);
       dot = fmaf(to_float(es), to_float(ed) * to_float(next[span.edge]), dot);
     }
-    const float2 total = team.sum2(ss, dot, slot2);
-    const float rx = rsqrtf(fmaf(team.sum(sx, slot[0]), inv_width, eps));
-    const float rs = rsqrtf(fmaf(total.x, inv_width, eps));
-    const float back = -(total.y * rs * inv_width) * rs * rs;
+    const float3 total = team.sum3(sx, ss, dot, slot[0], slot2);
+    const float rx = rsqrtf(fmaf(total.x, inv_width, eps)), rs = rsqrtf(fmaf(total.y, inv_width, eps));
+    const float back = -(total.z * rs * inv_width) * rs * rs;
     float av[N * VEC], ae = 0.0f, last = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -293,6 +292,222 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
   }
 }
 
+// k_sandwich for many long rows on 16-byte boundaries: rows through a ring, weights in
+// registers. The stream's statistics need the first norm's, so a row goes through two block
+// barriers; the copies of the next ones run on meanwhile.
+template <class T, class W, int PER>
+__global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
+    k_sandwich_ring(const so3lr_sandwich_norm_args a, int stages, const WaitLimit limit, const float inv_width,
+                    const float eps) {
+  constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
+  __shared__ float slot[2][32];
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
+  const uint32_t row_bytes = width * sizeof(T), tensors = a.gate ? 3 : 2;
+  dependents_may_start();
+  const RowRing ring(smem, tensors * row_bytes, stages, limit);
+  wait_for_predecessors();
+  const RowTeam<0> team;
+  const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
+  auto fetch = [&](int i) {
+    const long long row = blockIdx.x + (long long)i * gridDim.x;
+    const uint32_t dst = ring.expect(i, tensors * row_bytes), bar = ring.bar(i);
+    tc::bulk_load(dst, static_cast<const T *>(a.x) + row * a.x_stride, row_bytes, bar);
+    tc::bulk_load(dst + row_bytes, static_cast<const T *>(a.residual) + row * a.residual_stride, row_bytes, bar);
+    if (a.gate) tc::bulk_load(dst + 2 * row_bytes, static_cast<const T *>(a.gate) + row * a.gate_stride, row_bytes, bar);
+  };
+  if (t == 0)
+    for (int i = 0; i < min(stages, rows); ++i) fetch(i);
+  Chunk<W, VEC> cw[N], cn[N], cc[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = (j * size + t) * VEC;
+    if (c < width) {
+      cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
+      cn[j] = load_chunk<W, VEC>(static_cast<const W *>(a.next_weight) + c);
+      if (a.residual_scale) cc[j] = load_chunk<W, VEC>(static_cast<const W *>(a.residual_scale) + c);
+    }
+  }
+  int k = 0;
+  for (; k < rows; ++k) {
+    ring.wait(k);
+    const T *x = reinterpret_cast<const T *>(ring.stage(k));
+    const long long row = blockIdx.x + (long long)k * gridDim.x;
+    Chunk<T, VEC> cx[N];
+    float sq = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        cx[j] = load_chunk<T, VEC>(x + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
+      }
+    }
+    const float rx = rsqrtf(fmaf(team.sum(sq, slot[0]), inv_width, eps));
+    if (ring.gave_up(k)) break;
+    sq = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        const Chunk<T, VEC> cr = load_chunk<T, VEC>(x + width + c);
+        Chunk<T, VEC> cg;
+        if (a.gate) cg = load_chunk<T, VEC>(x + 2 * width + c);
+        float f[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float added = to_float(cx[j].e[i]) * rx * to_float(cw[j].e[i]), kept = to_float(cr.e[i]);
+          f[i] = fmaf(a.gate ? to_float(cg.e[i]) : 1.0f, added, a.residual_scale ? kept * to_float(cc[j].e[i]) : kept);
+        }
+        cx[j] = to_chunk<T, VEC>(f);
+        store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx[j]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
+      }
+    }
+    const float rs = rsqrtf(fmaf(team.sum(sq, slot[1]), inv_width, eps));
+    if (t == 0 && k + stages < rows) fetch(k + stages);  // every thread has read the stage
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        float f[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = to_float(cx[j].e[i]) * rs * to_float(cn[j].e[i]);
+        store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, to_chunk<T, VEC>(f));
+      }
+    }
+  }
+  if (t == 0) ring.settle(k, rows);
+}
+
+// k_sandwich_backward for rows on 16-byte boundaries that need a block, through a ring
+template <class T, class W, int PER>
+__global__ void __launch_bounds__(512)
+    k_sandwich_backward_ring(const so3lr_sandwich_norm_backward_args a, float *partial, int stages,
+                             const WaitLimit limit, const float inv_width, const float eps) {
+  constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
+  __shared__ float2 slot2[32];
+  __shared__ float slot[2][32];
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
+  const uint32_t row_bytes = width * sizeof(T);
+  // where each tensor of a row lies in its stage: s, dy, x, then those that there are
+  const int ds_at = 3, gate_at = ds_at + (a.ds ? 1 : 0), residual_at = gate_at + (a.gate ? 1 : 0),
+            tensors = residual_at + (a.residual_scale ? 1 : 0);
+  dependents_may_start();
+  const RowRing ring(smem, tensors * row_bytes, stages, limit);
+  wait_for_predecessors();
+  const RowTeam<0> team;
+  const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
+  auto fetch = [&](int i) {
+    const long long row = blockIdx.x + (long long)i * gridDim.x;
+    const uint32_t dst = ring.expect(i, tensors * row_bytes), bar = ring.bar(i);
+    auto copy = [&](const void *from, long long stride, int at) {
+      tc::bulk_load(dst + at * row_bytes, static_cast<const T *>(from) + row * stride, row_bytes, bar);
+    };
+    copy(a.s, a.s_stride, 0);
+    copy(a.dy, a.dy_stride, 1);
+    copy(a.x, a.x_stride, 2);
+    if (a.ds) copy(a.ds, a.ds_stride, ds_at);
+    if (a.gate) copy(a.gate, a.gate_stride, gate_at);
+    if (a.residual_scale) copy(a.residual, a.residual_stride, residual_at);
+  };
+  if (t == 0)
+    for (int i = 0; i < min(stages, rows); ++i) fetch(i);
+  Chunk<W, VEC> cw[N], cn[N], cc[N];
+  float sums[3][PER] = {};
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int c = (j * size + t) * VEC;
+    if (c < width) {
+      cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
+      cn[j] = load_chunk<W, VEC>(static_cast<const W *>(a.next_weight) + c);
+      if (a.residual_scale) cc[j] = load_chunk<W, VEC>(static_cast<const W *>(a.residual_scale) + c);
+    }
+  }
+  int k = 0;
+  for (; k < rows; ++k) {
+    ring.wait(k);
+    const T *stage = reinterpret_cast<const T *>(ring.stage(k));
+    const SandwichBackRow<T, W> row(a, blockIdx.x + (long long)k * gridDim.x);
+    Chunk<T, VEC> cs[N], cd[N], cx[N];
+    float sx = 0.0f, ss = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        cs[j] = load_chunk<T, VEC>(stage + c);
+        cd[j] = load_chunk<T, VEC>(stage + width + c);
+        cx[j] = load_chunk<T, VEC>(stage + 2 * width + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float f = to_float(cs[j].e[i]), x = to_float(cx[j].e[i]);
+          sx = fmaf(x, x, sx);
+          ss = fmaf(f, f, ss);
+          dot = fmaf(f, to_float(cd[j].e[i]) * to_float(cn[j].e[i]), dot);
+        }
+      }
+    }
+    const float3 total = team.sum3(sx, ss, dot, slot[0], slot2);
+    if (ring.gave_up(k)) break;
+    const float rx = rsqrtf(fmaf(total.x, inv_width, eps)), rs = rsqrtf(fmaf(total.y, inv_width, eps));
+    const float back = -(total.z * rs * inv_width) * rs * rs;
+    float av[PER], last = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        Chunk<T, VEC> ce{}, cg{}, cr{};
+        if (a.ds) ce = load_chunk<T, VEC>(stage + ds_at * width + c);
+        if (a.gate) cg = load_chunk<T, VEC>(stage + gate_at * width + c);
+        if (a.residual_scale) cr = load_chunk<T, VEC>(stage + residual_at * width + c);
+        float dres[VEC], dgate[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float x = to_float(cx[j].e[i]);
+          const SandwichElement e(x, to_float(cs[j].e[i]), to_float(cd[j].e[i]), to_float(ce.e[i]), to_float(cr.e[i]),
+                                  a.gate ? to_float(cg.e[i]) : 1.0f, to_float(cw[j].e[i]), to_float(cn[j].e[i]),
+                                  a.residual_scale ? to_float(cc[j].e[i]) : 1.0f, rx, rs, back);
+          dres[i] = e.dres;
+          dgate[i] = e.dgate;
+          av[j * VEC + i] = e.a;
+          last = fmaf(e.a, x, last);
+          sums[0][j * VEC + i] += e.sum_w;
+          sums[1][j * VEC + i] += e.sum_next;
+          sums[2][j * VEC + i] += e.sum_scale;
+        }
+        store_chunk<T, VEC>(row.dresidual + c, to_chunk<T, VEC>(dres));
+        if (a.gate) store_chunk<T, VEC>(row.dgate + c, to_chunk<T, VEC>(dgate));
+      }
+    }
+    const float back_x = -(team.sum(last, slot[1]) * rx * inv_width) * rx * rx;
+    if (t == 0 && k + stages < rows) fetch(k + stages);  // every thread has read the stage
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width) {
+        float dx[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) dx[i] = fmaf(av[j * VEC + i], rx, to_float(cx[j].e[i]) * back_x);
+        store_chunk<T, VEC>(row.dx + c, to_chunk<T, VEC>(dx));
+      }
+    }
+  }
+  if (t == 0) ring.settle(k, rows);
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (j * size + t) * VEC;
+      if (c < width)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          partial[((size_t)blockIdx.x * 3 + q) * width + c + i] = sums[q][j * VEC + i];
+    }
+}
+
 // Any row, a block each: elements are read again for each statistic (from L2, mostly), the
 // column sums stand in shared memory.
 template <class T, class W>
@@ -320,10 +535,9 @@ __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sand
       ss = fmaf(s, s, ss);
       dot = fmaf(s, to_float(row.dy[c]) * to_float(next[c]), dot);
     }
-    const float2 total = team.sum2(ss, dot, slot2);
-    const float rx = rsqrtf(fmaf(team.sum(sx, slot[0]), inv_width, eps));
-    const float rs = rsqrtf(fmaf(total.x, inv_width, eps));
-    const float back = -(total.y * rs * inv_width) * rs * rs;
+    const float3 total = team.sum3(sx, ss, dot, slot[0], slot2);
+    const float rx = rsqrtf(fmaf(total.x, inv_width, eps)), rs = rsqrtf(fmaf(total.y, inv_width, eps));
+    const float back = -(total.z * rs * inv_width) * rs * rs;
     auto element = [&](int c) {
       return SandwichElement(to_float(row.x[c]), to_float(row.s[c]), to_float(row.dy[c]),
                              row.ds ? to_float(row.ds[c]) : 0.0f, row.residual ? to_float(row.residual[c]) : 0.0f,
@@ -398,10 +612,19 @@ void by_sandwich_hold(const Hold &h, F &&f) {
   return f(integral_constant<int, 0>{}, integral_constant<int, 16>{});
 }
 
+// The rings: rows that need a block, up to what a ring of two holds.
+int ring_per(long long width) { return width <= 4096 ? 8 : 16; }
+RingPlan forward_ring(const so3lr_sandwich_norm_args &a, Path path) {
+  if (path != kWide || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
+  const int per = ring_per(a.width);
+  return ring_plan(a.rows, row_threads(a.width, per), per == 8 ? 1024 : 512, 2,
+                   (a.gate ? 3 : 2) * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
+}
 struct BackPlan {
   Path path;
   Hold hold;
   int grid, threads;
+  RingPlan ring;
 };
 BackPlan back_plan(const so3lr_sandwich_norm_backward_args &a) {
   RowTensors t{a.dtype == SO3LR_FLOAT32 ? 4 : 2};
@@ -418,6 +641,18 @@ BackPlan back_plan(const so3lr_sandwich_norm_backward_args &a) {
   p.path = t.path(a.width, aligned(a.weight, 0, 1, 16) && aligned(a.next_weight, 0, 1, 16) &&
                                aligned(a.residual_scale, 0, 1, 16));
   p.hold = sandwich_hold(a.width, p.path, t.size, true);
+  p.ring = RingPlan{0, 0, 0};
+  if (p.path == kWide && a.width > 512 && a.width <= 8192) {
+    const int per = ring_per(a.width), threads = row_threads(a.width, per);
+    const RingPlan r = ring_plan(a.rows, threads, 512, 2,
+                                 (3 + (a.ds ? 1 : 0) + (a.gate ? 1 : 0) + (a.residual_scale ? 1 : 0)) * a.width * t.size);
+    if (r.stages >= 2) {
+      p.ring = r;
+      p.grid = r.grid;
+      p.threads = threads;
+      return p;
+    }
+  }
   if (p.hold.per == 0) {
     p.threads = 512;
     p.grid = int(std::min<long long>(a.rows, kSmCount));
@@ -443,7 +678,22 @@ void launch_sandwich_norm(const so3lr_sandwich_norm_args &a, cudaStream_t s) {
       t.add(a.gate, a.gate_stride);
       t.add(a.s, a.s_stride);
       t.add(a.y, a.y_stride);
-      by_path(t.path(a.width, aligned(a.weight, 0, 1, 16) && aligned(a.next_weight, 0, 1, 16)), [&](auto path) {
+      const Path chosen = t.path(a.width, aligned(a.weight, 0, 1, 16) && aligned(a.next_weight, 0, 1, 16) &&
+                                              aligned(a.residual_scale, 0, 1, 16));
+      const RingPlan r = forward_ring(a, chosen);
+      if (r.stages >= 2 && a.rows > 2 * r.grid) {
+        auto go = [&](auto kernel) {
+          allow_dynamic_smem(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
+          launch(kernel, r.grid, row_threads(a.width, ring_per(a.width)), r.smem, s, a, r.stages, wait_limit(),
+                 1.0f / float(a.width), float(a.eps));
+        };
+        if (ring_per(a.width) == 8)
+          go(&k_sandwich_ring<T, W, 8>);
+        else
+          go(&k_sandwich_ring<T, W, 16>);
+        return;
+      }
+      by_path(chosen, [&](auto path) {
         constexpr Path PATH = decltype(path)::value;
         constexpr int VEC = chunk_of(PATH, sizeof(T));
         const Hold h = sandwich_hold(a.width, PATH, sizeof(T), false);
@@ -469,7 +719,16 @@ void launch_sandwich_norm_backward(const so3lr_sandwich_norm_backward_args &a, v
       const BackPlan p = back_plan(a);
       float *partial = static_cast<float *>(workspace);
       const float inv = 1.0f / float(a.width), eps = float(a.eps);
-      if (p.grid > 0 && p.hold.per == 0) {
+      if (p.grid > 0 && p.ring.stages) {
+        auto go = [&](auto kernel) {
+          allow_dynamic_smem(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
+          launch(kernel, p.grid, p.threads, p.ring.smem, s, a, partial, p.ring.stages, wait_limit(), inv, eps);
+        };
+        if (ring_per(a.width) == 8)
+          go(&k_sandwich_backward_ring<T, W, 8>);
+        else
+          go(&k_sandwich_backward_ring<T, W, 16>);
+      } else if (p.grid > 0 && p.hold.per == 0) {
         allow_dynamic_smem(reinterpret_cast<const void *>(&k_sandwich_backward_long<T, W>), 3 * 16384 * sizeof(float));
         launch(k_sandwich_backward_long<T, W>, p.grid, p.threads, 3 * a.width * sizeof(float), s, a, partial, inv, eps);
       } else if (p.grid > 0) {
