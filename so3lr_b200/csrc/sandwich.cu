@@ -292,6 +292,28 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
   }
 }
 
+// Sums over a block of up to 16 warps, the same value to every thread; `slot` starts as zeros.
+// The warps' parts are read four at a time: one by one they would cost a row more than its
+// arithmetic.
+template <int K>
+__device__ __forceinline__ void block_sums(float (&v)[K], float (*slot)[16]) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = RowTeam<0>::add(v[k]);
+    if ((threadIdx.x & 31) == 0) slot[k][threadIdx.x >> 5] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float4 p = *reinterpret_cast<const float4 *>(&slot[k][i]);
+      v[k] += (p.x + p.y) + (p.z + p.w);
+    }
+  }
+}
+
 // k_sandwich for many long rows on 16-byte boundaries: rows through a ring, weights in
 // registers. The stream's statistics need the first norm's, so a row goes through two block
 // barriers; the copies of the next ones run on meanwhile.
@@ -300,14 +322,15 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
     k_sandwich_ring(const so3lr_sandwich_norm_args a, int stages, const WaitLimit limit, const float inv_width,
                     const float eps) {
   constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
-  __shared__ float slot[2][32];
+  __shared__ __align__(16) float slot[2][16];
   extern __shared__ __align__(128) unsigned char smem[];
   const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
   const uint32_t row_bytes = width * sizeof(T), tensors = a.gate ? 3 : 2;
   dependents_may_start();
   const RowRing ring(smem, tensors * row_bytes, stages, limit);
   wait_for_predecessors();
-  const RowTeam<0> team;
+  if (t < 32) slot[t / 16][t % 16] = 0.0f;
+  __syncthreads();
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
   auto fetch = [&](int i) {
     const long long row = blockIdx.x + (long long)i * gridDim.x;
@@ -334,19 +357,20 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
     const T *x = reinterpret_cast<const T *>(ring.stage(k));
     const long long row = blockIdx.x + (long long)k * gridDim.x;
     Chunk<T, VEC> cx[N];
-    float sq = 0.0f;
+    float sq[1] = {};
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
       if (c < width) {
         cx[j] = load_chunk<T, VEC>(x + c);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
+        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq[0]);
       }
     }
-    const float rx = rsqrtf(fmaf(team.sum(sq, slot[0]), inv_width, eps));
+    block_sums(sq, &slot[0]);
+    const float rx = rsqrtf(fmaf(sq[0], inv_width, eps));
     if (ring.gave_up(k)) break;
-    sq = 0.0f;
+    sq[0] = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
@@ -363,10 +387,11 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
         cx[j] = to_chunk<T, VEC>(f);
         store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx[j]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
+        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq[0]);
       }
     }
-    const float rs = rsqrtf(fmaf(team.sum(sq, slot[1]), inv_width, eps));
+    block_sums(sq, &slot[1]);
+    const float rs = rsqrtf(fmaf(sq[0], inv_width, eps));
     if (t == 0 && k + stages < rows) fetch(k + stages);  // every thread has read the stage
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -388,8 +413,7 @@ __global__ void __launch_bounds__(512)
     k_sandwich_backward_ring(const so3lr_sandwich_norm_backward_args a, float *partial, int stages,
                              const WaitLimit limit, const float inv_width, const float eps) {
   constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
-  __shared__ float2 slot2[32];
-  __shared__ float slot[2][32];
+  __shared__ __align__(16) float slot[4][16];
   extern __shared__ __align__(128) unsigned char smem[];
   const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
   const uint32_t row_bytes = width * sizeof(T);
@@ -399,7 +423,8 @@ __global__ void __launch_bounds__(512)
   dependents_may_start();
   const RowRing ring(smem, tensors * row_bytes, stages, limit);
   wait_for_predecessors();
-  const RowTeam<0> team;
+  if (t < 64) slot[t / 16][t % 16] = 0.0f;
+  __syncthreads();
   const int rows = a.rows > blockIdx.x ? int((a.rows - 1 - blockIdx.x) / gridDim.x) + 1 : 0;
   auto fetch = [&](int i) {
     const long long row = blockIdx.x + (long long)i * gridDim.x;
@@ -433,7 +458,7 @@ __global__ void __launch_bounds__(512)
     const T *stage = reinterpret_cast<const T *>(ring.stage(k));
     const SandwichBackRow<T, W> row(a, blockIdx.x + (long long)k * gridDim.x);
     Chunk<T, VEC> cs[N], cd[N], cx[N];
-    float sx = 0.0f, ss = 0.0f, dot = 0.0f;
+    float first[3] = {};  // sums of x^2, s^2, s dy next
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
@@ -444,17 +469,17 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float f = to_float(cs[j].e[i]), x = to_float(cx[j].e[i]);
-          sx = fmaf(x, x, sx);
-          ss = fmaf(f, f, ss);
-          dot = fmaf(f, to_float(cd[j].e[i]) * to_float(cn[j].e[i]), dot);
+          first[0] = fmaf(x, x, first[0]);
+          first[1] = fmaf(f, f, first[1]);
+          first[2] = fmaf(f, to_float(cd[j].e[i]) * to_float(cn[j].e[i]), first[2]);
         }
       }
     }
-    const float3 total = team.sum3(sx, ss, dot, slot[0], slot2);
+    block_sums(first, &slot[0]);
     if (ring.gave_up(k)) break;
-    const float rx = rsqrtf(fmaf(total.x, inv_width, eps)), rs = rsqrtf(fmaf(total.y, inv_width, eps));
-    const float back = -(total.z * rs * inv_width) * rs * rs;
-    float av[PER], last = 0.0f;
+    const float rx = rsqrtf(fmaf(first[0], inv_width, eps)), rs = rsqrtf(fmaf(first[1], inv_width, eps));
+    const float back = -(first[2] * rs * inv_width) * rs * rs;
+    float av[PER], last[1] = {};
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
@@ -473,7 +498,7 @@ __global__ void __launch_bounds__(512)
           dres[i] = e.dres;
           dgate[i] = e.dgate;
           av[j * VEC + i] = e.a;
-          last = fmaf(e.a, x, last);
+          last[0] = fmaf(e.a, x, last[0]);
           sums[0][j * VEC + i] += e.sum_w;
           sums[1][j * VEC + i] += e.sum_next;
           sums[2][j * VEC + i] += e.sum_scale;
@@ -482,7 +507,8 @@ __global__ void __launch_bounds__(512)
         if (a.gate) store_chunk<T, VEC>(row.dgate + c, to_chunk<T, VEC>(dgate));
       }
     }
-    const float back_x = -(team.sum(last, slot[1]) * rx * inv_width) * rx * rx;
+    block_sums(last, &slot[3]);
+    const float back_x = -(last[0] * rx * inv_width) * rx * rx;
     if (t == 0 && k + stages < rows) fetch(k + stages);  // every thread has read the stage
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -508,59 +534,87 @@ __global__ void __launch_bounds__(512)
     }
 }
 
-// Any row, a block each: elements are read again for each statistic (from L2, mostly), the
-// column sums stand in shared memory.
-template <class T, class W>
+// Any row, a block each, VEC elements at a time: elements are read again for each statistic
+// (from L2, mostly), the column sums stand in shared memory, each thread's own.
+template <class T, class W, int VEC>
 __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sandwich_norm_backward_args a,
                                                                 float *partial, const float inv_width,
                                                                 const float eps) {
-  __shared__ float2 slot2[32];
-  __shared__ float slot[2][32];
-  extern __shared__ float column[];  // 3 x width
+  __shared__ __align__(16) float slot[4][16];
+  extern __shared__ __align__(16) float column[];  // 3 x width
   dependents_may_start();
+  const int width = int(a.width), t = threadIdx.x, step = blockDim.x * VEC;
+  if (t < 64) slot[t / 16][t % 16] = 0.0f;
+  for (int c = t; c < 3 * width; c += blockDim.x) column[c] = 0.0f;
+  __syncthreads();
   wait_for_predecessors();
-  const RowTeam<0> team;
-  const int width = int(a.width);
   const W *w = static_cast<const W *>(a.weight), *next = static_cast<const W *>(a.next_weight),
           *scale = static_cast<const W *>(a.residual_scale);
-  for (int c = team.t; c < 3 * width; c += team.size) column[c] = 0.0f;
-  __syncthreads();
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const SandwichBackRow<T, W> row(a, r);
-    float sx = 0.0f, ss = 0.0f, dot = 0.0f;
-#pragma unroll 4
-    for (int c = team.t; c < width; c += team.size) {
-      const float x = to_float(row.x[c]), s = to_float(row.s[c]);
-      sx = fmaf(x, x, sx);
-      ss = fmaf(s, s, ss);
-      dot = fmaf(s, to_float(row.dy[c]) * to_float(next[c]), dot);
+    float first[3] = {};  // sums of x^2, s^2, s dy next
+#pragma unroll 2
+    for (int c = t * VEC; c < width; c += step) {
+      const Chunk<T, VEC> cx = load_chunk<T, VEC>(row.x + c), cs = load_chunk<T, VEC>(row.s + c),
+                          cd = load_chunk<T, VEC>(row.dy + c);
+      const Chunk<W, VEC> cn = load_chunk<W, VEC>(next + c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float x = to_float(cx.e[i]), f = to_float(cs.e[i]);
+        first[0] = fmaf(x, x, first[0]);
+        first[1] = fmaf(f, f, first[1]);
+        first[2] = fmaf(f, to_float(cd.e[i]) * to_float(cn.e[i]), first[2]);
+      }
     }
-    const float3 total = team.sum3(sx, ss, dot, slot[0], slot2);
-    const float rx = rsqrtf(fmaf(total.x, inv_width, eps)), rs = rsqrtf(fmaf(total.y, inv_width, eps));
-    const float back = -(total.z * rs * inv_width) * rs * rs;
-    auto element = [&](int c) {
-      return SandwichElement(to_float(row.x[c]), to_float(row.s[c]), to_float(row.dy[c]),
-                             row.ds ? to_float(row.ds[c]) : 0.0f, row.residual ? to_float(row.residual[c]) : 0.0f,
-                             row.gate ? to_float(row.gate[c]) : 1.0f, to_float(w[c]), to_float(next[c]),
-                             scale ? to_float(scale[c]) : 1.0f, rx, rs, back);
+    block_sums(first, &slot[0]);
+    const float rx = rsqrtf(fmaf(first[0], inv_width, eps)), rs = rsqrtf(fmaf(first[1], inv_width, eps));
+    const float back = -(first[2] * rs * inv_width) * rs * rs;
+    // f(c, i, the element) over the row
+    auto elements = [&](auto f) {
+      for (int c = t * VEC; c < width; c += step) {
+        const Chunk<T, VEC> cx = load_chunk<T, VEC>(row.x + c), cs = load_chunk<T, VEC>(row.s + c),
+                            cd = load_chunk<T, VEC>(row.dy + c);
+        const Chunk<W, VEC> cw = load_chunk<W, VEC>(w + c), cn = load_chunk<W, VEC>(next + c);
+        Chunk<T, VEC> ce{}, cr{}, cg{};
+        Chunk<W, VEC> cc{};
+        if (row.ds) ce = load_chunk<T, VEC>(row.ds + c);
+        if (row.residual) cr = load_chunk<T, VEC>(row.residual + c);
+        if (row.gate) cg = load_chunk<T, VEC>(row.gate + c);
+        if (scale) cc = load_chunk<W, VEC>(scale + c);
+        auto element = [&](int i) {
+          return SandwichElement(to_float(cx.e[i]), to_float(cs.e[i]), to_float(cd.e[i]), to_float(ce.e[i]),
+                                 to_float(cr.e[i]), row.gate ? to_float(cg.e[i]) : 1.0f, to_float(cw.e[i]),
+                                 to_float(cn.e[i]), scale ? to_float(cc.e[i]) : 1.0f, rx, rs, back);
+        };
+        f(c, cx, element);
+      }
     };
-    float last = 0.0f;
-#pragma unroll 2
-    for (int c = team.t; c < width; c += team.size) {
-      const SandwichElement e = element(c);
-      row.dresidual[c] = from_float<T>(e.dres);
-      if (row.dgate) row.dgate[c] = from_float<T>(e.dgate);
-      last = fmaf(e.a, to_float(row.x[c]), last);
-      column[c] += e.sum_w;
-      column[width + c] += e.sum_next;
-      column[2 * width + c] += e.sum_scale;
-    }
-    const float back_x = -(team.sum(last, slot[1]) * rx * inv_width) * rx * rx;
-#pragma unroll 2
-    for (int c = team.t; c < width; c += team.size)
-      row.dx[c] = from_float<T>(fmaf(element(c).a, rx, to_float(row.x[c]) * back_x));
+    float last[1] = {};
+    elements([&](int c, const Chunk<T, VEC> &cx, auto element) {
+      float dres[VEC], dgate[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const SandwichElement e = element(i);
+        dres[i] = e.dres;
+        dgate[i] = e.dgate;
+        last[0] = fmaf(e.a, to_float(cx.e[i]), last[0]);
+        column[c + i] += e.sum_w;
+        column[width + c + i] += e.sum_next;
+        column[2 * width + c + i] += e.sum_scale;
+      }
+      store_chunk<T, VEC>(row.dresidual + c, to_chunk<T, VEC>(dres));
+      if (row.dgate) store_chunk<T, VEC>(row.dgate + c, to_chunk<T, VEC>(dgate));
+    });
+    block_sums(last, &slot[3]);
+    const float back_x = -(last[0] * rx * inv_width) * rx * rx;
+    elements([&](int c, const Chunk<T, VEC> &cx, auto element) {
+      float dx[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dx[i] = fmaf(element(i).a, rx, to_float(cx.e[i]) * back_x);
+      store_chunk<T, VEC>(row.dx + c, to_chunk<T, VEC>(dx));
+    });
   }
-  for (int c = team.t; c < 3 * width; c += team.size) partial[(size_t)blockIdx.x * 3 * width + c] = column[c];
+  for (int c = t; c < 3 * width; c += blockDim.x) partial[(size_t)blockIdx.x * 3 * width + c] = column[c];
 }
 
 // Column sums of `partial` (nparts x 3 x width) in a fixed order, one output for each y of the grid
@@ -729,8 +783,14 @@ void launch_sandwich_norm_backward(const so3lr_sandwich_norm_backward_args &a, v
         else
           go(&k_sandwich_backward_ring<T, W, 16>);
       } else if (p.grid > 0 && p.hold.per == 0) {
-        allow_dynamic_smem(reinterpret_cast<const void *>(&k_sandwich_backward_long<T, W>), 3 * 16384 * sizeof(float));
-        launch(k_sandwich_backward_long<T, W>, p.grid, p.threads, 3 * a.width * sizeof(float), s, a, partial, inv, eps);
+        auto go = [&](auto kernel) {
+          allow_dynamic_smem(reinterpret_cast<const void *>(kernel), 3 * 16384 * sizeof(float));
+          launch(kernel, p.grid, p.threads, 3 * a.width * sizeof(float), s, a, partial, inv, eps);
+        };
+        if (p.path == kWide)
+          go(&k_sandwich_backward_long<T, W, 16 / sizeof(T)>);
+        else
+          go(&k_sandwich_backward_long<T, W, 1>);
       } else if (p.grid > 0) {
         by_path(p.path, [&](auto path) {
           constexpr Path PATH = decltype(path)::value;
