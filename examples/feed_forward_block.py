@@ -1,6 +1,6 @@
 """A feed-forward sublayer over per-atom features, trained and then served in 8 bits.
 
-    python examples/feed_forward_block.py [--molecules 8000] [--steps 60]
+    python examples/feed_forward_block.py [--molecules 8000] [--steps 60] [--moment-bits 8]
 
 Rows are the atoms of a water box, columns 256 features (the wider shipped
 model's width). The features are a random embedding of each atom's element and of
@@ -18,7 +18,7 @@ sys.path.insert(0, str(pathlib.Path(__file__).resolve().parents[1]))
 
 import torch  # noqa: E402
 
-from so3lr_b200 import layers  # noqa: E402
+from so3lr_b200 import layers, optim  # noqa: E402
 from so3lr_b200.systems import water_box  # noqa: E402
 
 WIDTH, HIDDEN = 256, 1024
@@ -52,26 +52,21 @@ def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--molecules", type=int, default=8000)
     ap.add_argument("--steps", type=int, default=60)
+    ap.add_argument("--moment-bits", type=int, choices=(8, 32), default=32, help="of the optimiser's moments")
     args = ap.parse_args()
     torch.manual_seed(0)
     x = atom_features(args.molecules)
     residual = x.roll(1, 0)
     block = layers.FeedForwardBlock(WIDTH, HIDDEN)
     target = residual + torch.sin(2 * x.float() + x.float().roll(1, 1)).bfloat16()
-    master = [p.detach().float().requires_grad_() for p in block.parameters()]  # what the optimiser updates
-    adam = torch.optim.Adam(master, lr=2e-3)
+    adam = optim.AdamW(block.parameters(), lr=2e-3, weight_decay=0.0, moment_bits=args.moment_bits)
 
     def step() -> float:
         out, stream = block(x, residual)
         loss = (out + stream - target - x).float().square().mean()
-        block.zero_grad()
+        adam.zero_grad()
         loss.backward()
-        for p, m in zip(block.parameters(), master):
-            m.grad = p.grad.float()
         adam.step()
-        with torch.no_grad():
-            for p, m in zip(block.parameters(), master):
-                p.copy_(m)
         return float(loss.detach())
 
     first = step()

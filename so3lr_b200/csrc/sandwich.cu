@@ -14,6 +14,12 @@
 // lanes of a warp or to a block as in rows.cu. The backward kernels walk over their rows
 // and hold the three column sums; each block writes one row of them, and k_column_sums
 // adds those in order.
+//
+// Measured, 33.5 M elements with gate and scale, forward and backward (TB/s): bfloat16 rows of
+// 256 5.5 and 4.6, of 1024 5.4 and 4.8, of 4096 5.4 and 4.2, of 1003 3.6 and 2.8, of 16384 3.4 and
+// 1.8; float32 rows (half as many) 6.5 and 6.0, 5.8 and 5.5, 5.9 and 5.3, 5.7 and 5.3, 4.5 and 3.0.
+// With 2-byte elements a row's two reductions, about 50 instructions a thread, and one block of
+// 512 threads an SM (the column sums fill the registers) hold the backward pass back.
 #include "row_team.cuh"
 
 namespace so3lr_b200 {
@@ -666,10 +672,13 @@ void by_sandwich_hold(const Hold &h, F &&f) {
   return f(integral_constant<int, 0>{}, integral_constant<int, 16>{});
 }
 
-// The rings: rows that need a block, up to what a ring of two holds.
+// The rings: rows too long for a warp with 8 elements a lane, up to what a ring of two holds. 65536
+// rows of 512 bfloat16: 67 us forward and 133 back, 73 and 192 in a warp with 16 elements a lane;
+// 32768 rows of 512 float32: 63 and 115, 53 and 102 in a warp.
+bool ring_takes(long long width, int size) { return width > (size == 2 ? 256 : 512) && width <= 8192; }
 int ring_per(long long width) { return width <= 4096 ? 8 : 16; }
 RingPlan forward_ring(const so3lr_sandwich_norm_args &a, Path path) {
-  if (path != kWide || a.width <= 512 || a.width > 8192) return RingPlan{0, 0, 0};
+  if (path != kWide || !ring_takes(a.width, a.dtype == SO3LR_FLOAT32 ? 4 : 2)) return RingPlan{0, 0, 0};
   const int per = ring_per(a.width);
   return ring_plan(a.rows, row_threads(a.width, per), per == 8 ? 1024 : 512, 2,
                    (a.gate ? 3 : 2) * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
@@ -696,7 +705,7 @@ BackPlan back_plan(const so3lr_sandwich_norm_backward_args &a) {
                                aligned(a.residual_scale, 0, 1, 16));
   p.hold = sandwich_hold(a.width, p.path, t.size, true);
   p.ring = RingPlan{0, 0, 0};
-  if (p.path == kWide && a.width > 512 && a.width <= 8192) {
+  if (p.path == kWide && ring_takes(a.width, t.size)) {
     const int per = ring_per(a.width), threads = row_threads(a.width, per);
     const RingPlan r = ring_plan(a.rows, threads, 512, 2,
                                  (3 + (a.ds ? 1 : 0) + (a.gate ? 1 : 0) + (a.residual_scale ? 1 : 0)) * a.width * t.size);
@@ -797,7 +806,8 @@ void launch_sandwich_norm_backward(const so3lr_sandwich_norm_backward_args &a, v
           constexpr int VEC = chunk_of(PATH, sizeof(T));
           by_sandwich_hold(p.hold, [&](auto lanes, auto per) {
             constexpr int L = decltype(lanes)::value, P = decltype(per)::value, N = P / VEC;
-            if constexpr (L != 0 || P == 8)
+            // rows on the boundaries that the rings take are not held in registers
+            if constexpr (PATH == kWide ? L != 0 && (P == 8 || sizeof(T) == 4) : L != 0 || P == 8)
               launch(k_sandwich_backward<T, W, VEC, N, L, PATH == kShifted>, p.grid, p.threads,
                      L ? kTeamThreads / (L ? L : 1) * a.width * sizeof(float) : 0, s, a, partial, inv, eps);
           });

@@ -4,6 +4,10 @@ The row-wise half of a transformer block over per-atom (or per-token) features:
 
 * ``rms_norm`` (with the residual's addition), ``rms_norm_int8`` and the gradient
   ``rms_norm_backward``;
+* ``sandwich_norm``, the norms on both sides of a block's boundary with gate and
+  residual scale between them, and ``sandwich_norm_backward``;
+* ``linear``, a dense layer with bias, activation and residual in one kernel, with
+  ``linear_train`` and ``linear_backward`` for training;
 * ``int8_linear``, a product of 8-bit integers with a scale for each row of the
   activations and for each output channel, and ``gate_int8``, which stands
   between two of them in a feed-forward block; ``quantize_weight`` lays a weight
@@ -11,13 +15,14 @@ The row-wise half of a transformer block over per-atom (or per-token) features:
 * ``feed_forward``, the gated block y = (silu(x Wg^T) * (x Wu^T)) Wd^T, with
   ``feed_forward_train`` and ``feed_forward_backward`` for training.
 
-``rms_norm`` and ``feed_forward`` record themselves for reverse-mode autograd when an
-argument requires a gradient; tensors with a forward-mode tangent and
+``rms_norm``, ``sandwich_norm``, ``linear`` and ``feed_forward`` record themselves for
+reverse-mode autograd when an argument requires a gradient; tensors with a forward-mode tangent and
 ``torch.jit.trace`` are refused. All other calls record nothing: their results, the
 stream of ``rms_norm_int8`` among them, are detached from arguments that require a
 gradient. ``FeedForwardBlock`` and ``Int8FeedForwardBlock`` run them
 together: the pre-norm sublayer as it is trained, and the same weights served
-in 8 bits.
+in 8 bits; ``SandwichBlock`` is a sublayer of dense layers between norms on both
+sides. ``so3lr_b200.optim`` updates their weights.
 
 The calls are the entry points of include/so3lr_b200.h ("Row-wise feed-forward
 layers") through the compiled module ``so3lr_b200._layers``
@@ -44,7 +49,7 @@ except (ImportError, So3lrError) as e:
 
 __all__ = ["linear", "linear_train", "linear_backward", "rms_norm", "rms_norm_int8", "rms_norm_backward", "sandwich_norm", "sandwich_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
            "quantize_weight", "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock",
-           "Int8FeedForwardBlock", "check_status", "set_wait_limit"]
+           "SandwichBlock", "Int8FeedForwardBlock", "check_status", "set_wait_limit"]
 
 
 def check_status(device=None) -> None:
@@ -313,6 +318,38 @@ class FeedForwardBlock(torch.nn.Module):
     def forward(self, x, residual=None):
         y, s = rms_norm(x, self.norm, residual, eps=self.eps)
         return feed_forward(y, self.w_gate, self.w_up, self.w_down), s
+
+
+class SandwichBlock(torch.nn.Module):
+    """Feed-forward sublayer between a norm before and a norm after it, with a learned gate
+    and residual scale:
+
+        h = linear(y, w_up, b_up, activation);  out = linear(h, w_down, b_down)
+        y', s' = sandwich_norm(out, s, norm, next_norm, linear(y, w_gate, b_gate), residual_scale)
+
+    forward(y, s) takes the normalised stream and the stream and returns both for the next
+    block; the first block gets them from rms_norm. gated=False leaves the gate out. Starts
+    with gates and residual scales of 1. Trains through autograd."""
+
+    def __init__(self, width: int, hidden: int, *, activation="silu", gated: bool = True, eps: float = 1e-6,
+                 dtype=torch.bfloat16, device="cuda"):
+        super().__init__()
+        _activation(activation)
+        self.activation, self.eps = activation, eps
+        parameter = torch.nn.Parameter
+        weight = lambda n, k: parameter(torch.randn(n, k, device=device).mul_(k ** -0.5).to(dtype))  # noqa: E731
+        vector = lambda n, value, dtype=dtype: parameter(torch.full((n,), value, device=device, dtype=dtype))  # noqa: E731
+        self.w_up, self.b_up = weight(hidden, width), vector(hidden, 0.0)
+        self.w_down, self.b_down = weight(width, hidden), vector(width, 0.0)
+        self.w_gate = parameter(torch.zeros(width, width, device=device, dtype=dtype)) if gated else None
+        self.b_gate = vector(width, 1.0) if gated else None
+        self.norm, self.next_norm, self.residual_scale = (vector(width, 1.0, torch.float32) for _ in range(3))
+
+    def forward(self, y, s):
+        h = linear(y, self.w_up, self.b_up, activation=self.activation)
+        out = linear(h, self.w_down, self.b_down)
+        gate = None if self.w_gate is None else linear(y, self.w_gate, self.b_gate)
+        return sandwich_norm(out, s, self.norm, self.next_norm, gate, self.residual_scale, eps=self.eps)
 
 
 class Int8FeedForwardBlock:
