@@ -25,7 +25,7 @@
 #include <algorithm>
 
 #include "adamw.hpp"
-#include "layers_common.cuh"
+#include "pairs.cuh"
 
 namespace so3lr_b200 {
 namespace {
@@ -132,35 +132,6 @@ __device__ __forceinline__ void write_codes(void *to, int left, const Codes &c) 
   }
 }
 
-// Two floats in one register pair: products and multiply-adds of pairs issue as one
-// instruction, each half rounded by itself (268 M elements 735 -> 692 us). Sums of products
-// that codes depend on are taken half by half: the assembler contracts add.rn.f32x2 with a
-// product, which a float32 of the formula is not.
-struct Pair {
-  uint64_t bits;
-  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
-  __device__ __forceinline__ Pair(uint64_t b, int) : bits(b) {}
-  __device__ __forceinline__ void get(float &a, float &b) const {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits));
-  }
-};
-__device__ __forceinline__ Pair operator*(const Pair &a, const Pair &b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits), "l"(b.bits));
-  return Pair(r, 0);
-}
-__device__ __forceinline__ Pair operator+(const Pair &a, const Pair &b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.bits), "l"(b.bits));
-  return Pair(r, 0);
-}
-__device__ __forceinline__ Pair fma(const Pair &a, const Pair &b, const Pair &c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
-  return Pair(r, 0);
-}
-
 // What codes stand for. SIGNED: m, else v. Bytes become floats without the slow conversion: a
 // byte in the low bits of 2^23.
 template <bool SIGNED>
@@ -197,7 +168,7 @@ __device__ __forceinline__ Pair roots_of_shares(const Pair &x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(ya) : "f"(a));
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(yb) : "f"(b));
   const Pair y(ya, yb), s = x * y;
-  return fma(fma(s * Pair(-1.0f), s, x), y * Pair(0.5f), s);
+  return madd(madd(s * Pair(-1.0f), s, x), y * Pair(0.5f), s);
 }
 // The largest magnitude of the warp's 256 elements, for a scale; `live`: codes can be made
 // with it. Not of a block that holds an infinity or a NaN (scale NaN, codes 0), nor of one
@@ -265,6 +236,8 @@ __device__ __forceinline__ void update(const Work &a, long long at) {
     read<WHOLE>(static_cast<const float *>(e.m) + at, left, m);
     read<WHOLE>(static_cast<const float *>(e.v) + at, left, v);
   }
+  // Pairs take an instruction for two elements (268 M elements in 8 bits 735 -> 692 us). Sums that
+  // codes depend on are taken half by half: a contracted one is not the formula's in float32.
   auto sum = [](const Pair &x, const Pair &y, float &a, float &b) {
     float c, d;
     x.get(a, b);
@@ -283,11 +256,11 @@ __device__ __forceinline__ void update(const Work &a, long long at) {
     float d, e;
     denominators.get(d, e);
     const Pair ratio = Pair(m[i], m[i + 1]) * Pair(reciprocal(d), reciprocal(e));
-    fma(Pair(p[i], p[i + 1]), Pair(coef.z), ratio * Pair(-coef.x)).get(p[i], p[i + 1]);
+    madd(Pair(p[i], p[i + 1]), Pair(coef.z), ratio * Pair(-coef.x)).get(p[i], p[i + 1]);
   };
   auto move_by_root = [&] {
 #pragma unroll
-    for (int i = 0; i < kPer; i += 2) move(i, fma(Pair(root(v[i]), root(v[i + 1])), Pair(coef.y), Pair(a.eps)));
+    for (int i = 0; i < kPer; i += 2) move(i, madd(Pair(root(v[i]), root(v[i + 1])), Pair(coef.y), Pair(a.eps)));
   };
   if (EIGHT) {
     bool m_live, v_live;
@@ -299,7 +272,7 @@ __device__ __forceinline__ void update(const Work &a, long long at) {
 #pragma unroll
       for (int i = 0; i < kPer; i += 2) {
         const Pair half = roots_of_shares(shares_of(v[i], v[i + 1], inv));
-        move(i, fma(half, Pair(back), Pair(a.eps)));
+        move(i, madd(half, Pair(back), Pair(a.eps)));
         (roots_of_shares(half) * Pair(255.0f)).get(code[i], code[i + 1]);
         if (v[i] > 0.0f) code[i] = fmaxf(code[i], 1.0f);
         if (v[i + 1] > 0.0f) code[i + 1] = fmaxf(code[i + 1], 1.0f);

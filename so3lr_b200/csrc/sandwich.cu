@@ -20,6 +20,7 @@
 // 1.8; float32 rows (half as many) 6.5 and 6.0, 5.8 and 5.5, 5.9 and 5.3, 5.7 and 5.3, 4.5 and 3.0.
 // With 2-byte elements a row's two reductions, about 50 instructions a thread, and one block of
 // 512 threads an SM (the column sums fill the registers) hold the backward pass back.
+#include "pairs.cuh"
 #include "row_team.cuh"
 
 namespace so3lr_b200 {
@@ -37,6 +38,33 @@ struct SandwichRow {  // pointers to one row
         y(static_cast<T *>(a.y) + row * a.y_stride) {}
 };
 
+// The stream as it is kept, and its squares: residual scale + gate (x rx weight), rounded.
+template <class T, class W, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> stream_of(const Chunk<T, VEC> &cx, const Chunk<T, VEC> &cr,
+                                                   const Chunk<T, VEC> &cg, const Chunk<W, VEC> &cw,
+                                                   const Chunk<W, VEC> &cc, float rx, typename Floats<VEC>::V &squares) {
+  using F = Floats<VEC>;
+  using V = typename F::V;
+  const F x = floats_of(cx), r = floats_of(cr), g = floats_of(cg), w = floats_of(cw), scale = floats_of(cc);
+  F s;
+#pragma unroll
+  for (int i = 0; i < F::kCount; ++i) s.v[i] = madd(g.v[i], x.v[i] * V(rx) * w.v[i], r.v[i] * scale.v[i]);
+  const Chunk<T, VEC> kept = chunk_of_floats<T, VEC>(s);
+  s = floats_of(kept);
+#pragma unroll
+  for (int i = 0; i < F::kCount; ++i) squares = madd(s.v[i], s.v[i], squares);
+  return kept;
+}
+template <class T, class W, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> normed(const Chunk<T, VEC> &cs, const Chunk<W, VEC> &cn, float rs) {
+  using F = Floats<VEC>;
+  const F s = floats_of(cs), next = floats_of(cn);
+  F y;
+#pragma unroll
+  for (int i = 0; i < F::kCount; ++i) y.v[i] = s.v[i] * typename F::V(rs) * next.v[i];
+  return chunk_of_floats<T, VEC>(y);
+}
+
 template <class T, class W, int VEC, int N, int LANES, bool SHIFT>
 __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
     k_sandwich(const so3lr_sandwich_norm_args a, const float inv_width, const float eps) {
@@ -50,10 +78,11 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
           *scale = static_cast<const W *>(a.residual_scale);
   const Span<SHIFT, VEC> span(row.x, int(a.width), team.t);
   Chunk<T, VEC> cx[N], cr[N], cg[N];
-  T ex{}, er{}, eg{};
+  T ex{}, er{}, eg = from_float<T>(1.0f);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = span.at(j * team.size + team.t);
+    cg[j] = ones<T, VEC>();
     if (span.holds(c)) {
       cx[j] = load_chunk<T, VEC>(row.x + c);
       cr[j] = load_chunk<T, VEC>(row.residual + c);
@@ -65,51 +94,45 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
     er = row.residual[span.edge];
     if (row.gate) eg = row.gate[span.edge];
   }
-  float sq = 0.0f;
+  using F = Floats<VEC>;
+  using V = typename F::V;
+  V squares(0.0f);
 #pragma unroll
   for (int j = 0; j < N; ++j)
-    if (span.holds(span.at(j * team.size + team.t)))
+    if (span.holds(span.at(j * team.size + team.t))) {
+      const F x = floats_of(cx[j]);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
-  sq = fmaf(to_float(ex), to_float(ex), sq);
+      for (int i = 0; i < F::kCount; ++i) squares = madd(x.v[i], x.v[i], squares);
+    }
+  float sq = fmaf(to_float(ex), to_float(ex), total(squares));
   const float rx = rsqrtf(fmaf(team.sum(sq, slot[0]), inv_width, eps));
   // what is kept of the stream is rounded, and the second norm is of what is kept
-  auto stream = [&](T x, T r, T g, W wi, int c) {
-    const float added = to_float(x) * rx * to_float(wi), kept = to_float(r);
-    return fmaf(row.gate ? to_float(g) : 1.0f, added, scale ? kept * to_float(scale[c]) : kept);
-  };
-  sq = 0.0f;
+  squares = V(0.0f);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = span.at(j * team.size + team.t);
     if (span.holds(c)) {
-      const Chunk<W, VEC> cw = load_apart<SHIFT, W, VEC>(w + c);
-      float f[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = stream(cx[j].e[i], cr[j].e[i], cg[j].e[i], cw.e[i], c + i);
-      cx[j] = to_chunk<T, VEC>(f);
+      cx[j] = stream_of(cx[j], cr[j], cg[j], load_apart<SHIFT, W, VEC>(w + c),
+                        scale ? load_apart<SHIFT, W, VEC>(scale + c) : ones<W, VEC>(), rx, squares);
       if (live) store_chunk<T, VEC>(row.s + c, cx[j]);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sq = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq);
     }
   }
+  sq = total(squares);
   if (span.edge >= 0) {
-    ex = from_float<T>(stream(ex, er, eg, w[span.edge], span.edge));
-    if (live) row.s[span.edge] = ex;
-    sq = fmaf(to_float(ex), to_float(ex), sq);
+    const int c = span.edge;
+    float one = 0.0f;
+    ex = stream_of(Chunk<T, 1>{{ex}}, Chunk<T, 1>{{er}}, Chunk<T, 1>{{eg}}, Chunk<W, 1>{{w[c]}},
+                   Chunk<W, 1>{{scale ? scale[c] : from_float<W>(1.0f)}}, rx, one)
+             .e[0];
+    if (live) row.s[c] = ex;
+    sq += one;
   }
   const float rs = rsqrtf(fmaf(team.sum(sq, slot[1]), inv_width, eps));
   if (!live) return;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = span.at(j * team.size + team.t);
-    if (span.holds(c)) {
-      const Chunk<W, VEC> cn = load_apart<SHIFT, W, VEC>(next + c);
-      float f[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = to_float(cx[j].e[i]) * rs * to_float(cn.e[i]);
-      store_chunk<T, VEC>(row.y + c, to_chunk<T, VEC>(f));
-    }
+    if (span.holds(c)) store_chunk<T, VEC>(row.y + c, normed(cx[j], load_apart<SHIFT, W, VEC>(next + c), rs));
   }
   if (span.edge >= 0) row.y[span.edge] = from_float<T>(to_float(ex) * rs * to_float(next[span.edge]));
 }
@@ -129,21 +152,49 @@ struct SandwichBackRow {
         dresidual(static_cast<T *>(a.dresidual) + row * a.dresidual_stride),
         dgate(a.gate ? static_cast<T *>(a.dgate) + row * a.dgate_stride : nullptr) {}
 };
-// One element of the gradient, all in float32. The row's first statistics give g and what
-// follows from it; its last one, sum(a x), is there after them.
+// The gradient's elements (V: a float or a pair), all in float32. The row's first statistics give
+// g and what follows from it; its last one, sum(a x), is there after them.
+template <class V>
+__device__ __forceinline__ void add_squares(const V &x, const V &s, const V &dy, const V &next, V (&sums)[3]) {
+  sums[0] = madd(x, x, sums[0]);
+  sums[1] = madd(s, s, sums[1]);
+  sums[2] = madd(s, dy * next, sums[2]);
+}
+template <class V>
 struct SandwichElement {
-  float dres, dgate, a, sum_w, sum_next, sum_scale;
-  __device__ __forceinline__ SandwichElement(float x, float s, float dy, float ds, float r, float gate, float w,
-                                             float next, float scale, float rx, float rs, float back) {
-    const float g = fmaf(dy * next, rs, fmaf(s, back, ds)), xh = x * rx, q = g * gate;
+  V dres, dgate, a;
+  // adds to the column sums of q xh, dy sh and g residual, and to the row's of a x
+  __device__ __forceinline__ SandwichElement(const V &x, const V &s, const V &dy, const V &ds, const V &r,
+                                             const V &gate, const V &w, const V &next, const V &scale, float rx,
+                                             float rs, float back, V &sum_w, V &sum_next, V &sum_scale, V &row_sum) {
+    const V g = madd(dy * next, V(rs), madd(s, V(back), ds)), xh = x * V(rx), q = g * gate;
     dres = g * scale;
     dgate = g * (xh * w);
     a = q * w;
-    sum_w = q * xh;
-    sum_next = dy * (s * rs);
-    sum_scale = g * r;
+    sum_w = madd(q, xh, sum_w);
+    sum_next = madd(dy, s * V(rs), sum_next);
+    sum_scale = madd(g, r, sum_scale);
+    row_sum = madd(a, x, row_sum);
   }
 };
+// dx from a and the row's last statistic
+template <class T, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> dx_of(const Floats<VEC> &a, const Chunk<T, VEC> &cx, float rx, float back_x) {
+  using F = Floats<VEC>;
+  using V = typename F::V;
+  const F x = floats_of(cx);
+  F dx;
+#pragma unroll
+  for (int i = 0; i < F::kCount; ++i) dx.v[i] = madd(a.v[i], V(rx), x.v[i] * V(back_x));
+  return chunk_of_floats<T, VEC>(dx);
+}
+
+template <int VEC>
+__device__ __forceinline__ void write_floats(float *p, const Floats<VEC> &f) {
+  const Chunk<float, VEC> c = chunk_of_floats<float, VEC>(f);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) p[i] = c.e[i];
+}
 
 // Rows in registers, 8 or 16 elements a thread.
 template <class T, class W, int VEC, int N, int LANES, bool SHIFT>
@@ -164,17 +215,27 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
                               width, team.t);
   const W *w = static_cast<const W *>(a.weight), *next = static_cast<const W *>(a.next_weight),
           *scale = static_cast<const W *>(a.residual_scale);
-  float sums[3][N * VEC] = {}, edge_sums[3] = {};
+  using F = Floats<VEC>;
+  using V = typename F::V;
+  F sums[3][N];
+  float edge_sums[3] = {};
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int i = 0; i < F::kCount; ++i) sums[k][j].v[i] = V(0.0f);
   // whole blocks walk together; a team past the last row adds nothing
   for (long long first = (long long)blockIdx.x * kTeams; first < a.rows; first += (long long)gridDim.x * kTeams) {
     const bool live = first + team_id < a.rows;
     const SandwichBackRow<T, W> row(a, live ? first + team_id : a.rows - 1);
     Chunk<T, VEC> cs[N], cd[N], ce[N], cx[N], cr[N], cg[N];
-    T es{}, ed{}, ee{}, ex{}, er{}, eg{};
+    T es{}, ed{}, ee{}, ex{}, er{}, eg = from_float<T>(1.0f);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = span.at(j * team.size + team.t);
-      cs[j] = cd[j] = ce[j] = cx[j] = cr[j] = cg[j] = Chunk<T, VEC>{};
+      cs[j] = cd[j] = ce[j] = cx[j] = cr[j] = Chunk<T, VEC>{};
+      cg[j] = ones<T, VEC>();
       if (live && span.holds(c)) {
         cs[j] = load_chunk<T, VEC>(row.s + c);
         cd[j] = load_chunk<T, VEC>(row.dy + c);
@@ -193,84 +254,64 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
       if (row.residual) er = row.residual[span.edge];
       if (row.gate) eg = row.gate[span.edge];
     }
-    float sx = 0.0f, ss = 0.0f, dot = 0.0f;
+    V squares[3] = {V(0.0f), V(0.0f), V(0.0f)};
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = span.at(j * team.size + team.t);
       if (span.holds(c)) {
-        const Chunk<W, VEC> cn = load_apart<SHIFT, W, VEC>(next + c);
+        const F x = floats_of(cx[j]), s = floats_of(cs[j]), dy = floats_of(cd[j]),
+                n = floats_of(load_apart<SHIFT, W, VEC>(next + c));
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float f = to_float(cs[j].e[i]), x = to_float(cx[j].e[i]);
-          sx = fmaf(x, x, sx);
-          ss = fmaf(f, f, ss);
-          dot = fmaf(f, to_float(cd[j].e[i]) * to_float(cn.e[i]), dot);
-        }
+        for (int i = 0; i < F::kCount; ++i) add_squares(x.v[i], s.v[i], dy.v[i], n.v[i], squares);
       }
     }
-    if (edge) {
-      sx = fmaf(to_float(ex), to_float(ex), sx);
-      ss = fmaf(to_float(es), to_float(es), ss);
-      dot = fmaf(to_float(es), to_float(ed) * to_float(next[span.edge]), dot);
-    }
-    const float3 total = team.sum3(sx, ss, dot, slot[0], slot2);
-    const float rx = rsqrtf(fmaf(total.x, inv_width, eps)), rs = rsqrtf(fmaf(total.y, inv_width, eps));
-    const float back = -(total.z * rs * inv_width) * rs * rs;
-    float av[N * VEC], ae = 0.0f, last = 0.0f;
+    float three[3] = {total(squares[0]), total(squares[1]), total(squares[2])};
+    if (edge) add_squares(to_float(ex), to_float(es), to_float(ed), to_float(next[span.edge]), three);
+    const float3 all = team.sum3(three[0], three[1], three[2], slot[0], slot2);
+    const float rx = rsqrtf(fmaf(all.x, inv_width, eps)), rs = rsqrtf(fmaf(all.y, inv_width, eps));
+    const float back = -(all.z * rs * inv_width) * rs * rs;
+    F av[N];
+    V row_sum(0.0f);
+    float ae = 0.0f, last = 0.0f;
+    if (live) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = span.at(j * team.size + team.t);
-      if (span.holds(c)) {
-        const Chunk<W, VEC> cw = load_apart<SHIFT, W, VEC>(w + c), cn = load_apart<SHIFT, W, VEC>(next + c);
-        Chunk<W, VEC> cc{};
-        if (scale) cc = load_apart<SHIFT, W, VEC>(scale + c);
-        float dres[VEC], dgate[VEC];
+      for (int j = 0; j < N; ++j) {
+        const int c = span.at(j * team.size + team.t);
+        if (span.holds(c)) {
+          const F x = floats_of(cx[j]), s = floats_of(cs[j]), dy = floats_of(cd[j]), ds = floats_of(ce[j]),
+                  r = floats_of(cr[j]), g = floats_of(cg[j]), wf = floats_of(load_apart<SHIFT, W, VEC>(w + c)),
+                  n = floats_of(load_apart<SHIFT, W, VEC>(next + c)),
+                  f = floats_of(scale ? load_apart<SHIFT, W, VEC>(scale + c) : ones<W, VEC>());
+          F dres, dgate;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float x = to_float(cx[j].e[i]);
-          const SandwichElement e(x, to_float(cs[j].e[i]), to_float(cd[j].e[i]), to_float(ce[j].e[i]),
-                                  to_float(cr[j].e[i]), row.gate ? to_float(cg[j].e[i]) : 1.0f, to_float(cw.e[i]),
-                                  to_float(cn.e[i]), scale ? to_float(cc.e[i]) : 1.0f, rx, rs, back);
-          dres[i] = e.dres;
-          dgate[i] = e.dgate;
-          av[j * VEC + i] = e.a;
-          last = fmaf(e.a, x, last);
-          if (live) {
-            sums[0][j * VEC + i] += e.sum_w;
-            sums[1][j * VEC + i] += e.sum_next;
-            sums[2][j * VEC + i] += e.sum_scale;
+          for (int i = 0; i < F::kCount; ++i) {
+            const SandwichElement<V> e(x.v[i], s.v[i], dy.v[i], ds.v[i], r.v[i], g.v[i], wf.v[i], n.v[i], f.v[i], rx, rs,
+                                       back, sums[0][j].v[i], sums[1][j].v[i], sums[2][j].v[i], row_sum);
+            dres.v[i] = e.dres;
+            dgate.v[i] = e.dgate;
+            av[j].v[i] = e.a;
           }
-        }
-        if (live) {
-          store_chunk<T, VEC>(row.dresidual + c, to_chunk<T, VEC>(dres));
-          if (row.dgate) store_chunk<T, VEC>(row.dgate + c, to_chunk<T, VEC>(dgate));
+          store_chunk<T, VEC>(row.dresidual + c, chunk_of_floats<T, VEC>(dres));
+          if (row.dgate) store_chunk<T, VEC>(row.dgate + c, chunk_of_floats<T, VEC>(dgate));
         }
       }
+      last = total(row_sum);
     }
     if (edge) {
       const int c = span.edge;
-      const SandwichElement e(to_float(ex), to_float(es), to_float(ed), to_float(ee), to_float(er),
-                              row.gate ? to_float(eg) : 1.0f, to_float(w[c]), to_float(next[c]),
-                              scale ? to_float(scale[c]) : 1.0f, rx, rs, back);
+      const SandwichElement<float> e(to_float(ex), to_float(es), to_float(ed), to_float(ee), to_float(er), to_float(eg),
+                                     to_float(w[c]), to_float(next[c]), scale ? to_float(scale[c]) : 1.0f, rx, rs, back,
+                                     edge_sums[0], edge_sums[1], edge_sums[2], last);
       row.dresidual[c] = from_float<T>(e.dres);
       if (row.dgate) row.dgate[c] = from_float<T>(e.dgate);
       ae = e.a;
-      last = fmaf(ae, to_float(ex), last);
-      edge_sums[0] += e.sum_w;
-      edge_sums[1] += e.sum_next;
-      edge_sums[2] += e.sum_scale;
     }
     const float back_x = -(team.sum(last, slot[1]) * rx * inv_width) * rx * rx;
     if (!live) continue;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = span.at(j * team.size + team.t);
-      if (span.holds(c)) {
-        float dx[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) dx[i] = fmaf(av[j * VEC + i], rx, to_float(cx[j].e[i]) * back_x);
-        store_chunk<T, VEC>(row.dx + c, to_chunk<T, VEC>(dx));
-      }
+      if (span.holds(c)) store_chunk<T, VEC>(row.dx + c, dx_of(av[j], cx[j], rx, back_x));
     }
     if (edge) row.dx[span.edge] = from_float<T>(fmaf(ae, rx, to_float(ex) * back_x));
   }
@@ -282,9 +323,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = span.at(j * team.size + team.t);
-      if (span.holds(c))
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) out[c + i] = sums[k][j * VEC + i];
+      if (span.holds(c)) write_floats(out + c, sums[k][j]);
     }
     if (span.edge >= 0) out[span.edge] = edge_sums[k];
     if (!LANES) continue;
@@ -299,8 +338,8 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
 }
 
 // Sums over a block of up to 16 warps, the same value to every thread; `slot` starts as zeros.
-// The warps' parts are read four at a time: one by one they would cost a row more than its
-// arithmetic.
+// The warps' parts are added by twos in every warp: each thread adding all 16 would cost a row of 8
+// elements a thread a tenth of its instructions.
 template <int K>
 __device__ __forceinline__ void block_sums(float (&v)[K], float (*slot)[16]) {
 #pragma unroll
@@ -311,12 +350,9 @@ __device__ __forceinline__ void block_sums(float (&v)[K], float (*slot)[16]) {
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    v[k] = 0.0f;
+    v[k] = slot[k][threadIdx.x & 15];
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const float4 p = *reinterpret_cast<const float4 *>(&slot[k][i]);
-      v[k] += (p.x + p.y) + (p.z + p.w);
-    }
+    for (int o = 8; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   }
 }
 
@@ -328,6 +364,8 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
     k_sandwich_ring(const so3lr_sandwich_norm_args a, int stages, const WaitLimit limit, const float inv_width,
                     const float eps) {
   constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
+  using F = Floats<VEC>;
+  using V = typename F::V;
   __shared__ __align__(16) float slot[2][16];
   extern __shared__ __align__(128) unsigned char smem[];
   const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
@@ -351,6 +389,7 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = (j * size + t) * VEC;
+    cc[j] = ones<W, VEC>();
     if (c < width) {
       cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
       cn[j] = load_chunk<W, VEC>(static_cast<const W *>(a.next_weight) + c);
@@ -363,51 +402,39 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
     const T *x = reinterpret_cast<const T *>(ring.stage(k));
     const long long row = blockIdx.x + (long long)k * gridDim.x;
     Chunk<T, VEC> cx[N];
-    float sq[1] = {};
+    V squares(0.0f);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
       if (c < width) {
         cx[j] = load_chunk<T, VEC>(x + c);
+        const F f = floats_of(cx[j]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq[0]);
+        for (int i = 0; i < F::kCount; ++i) squares = madd(f.v[i], f.v[i], squares);
       }
     }
+    float sq[1] = {total(squares)};
     block_sums(sq, &slot[0]);
     const float rx = rsqrtf(fmaf(sq[0], inv_width, eps));
     if (ring.gave_up(k)) break;
-    sq[0] = 0.0f;
+    squares = V(0.0f);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
       if (c < width) {
-        const Chunk<T, VEC> cr = load_chunk<T, VEC>(x + width + c);
-        Chunk<T, VEC> cg;
-        if (a.gate) cg = load_chunk<T, VEC>(x + 2 * width + c);
-        float f[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float added = to_float(cx[j].e[i]) * rx * to_float(cw[j].e[i]), kept = to_float(cr.e[i]);
-          f[i] = fmaf(a.gate ? to_float(cg.e[i]) : 1.0f, added, a.residual_scale ? kept * to_float(cc[j].e[i]) : kept);
-        }
-        cx[j] = to_chunk<T, VEC>(f);
+        const Chunk<T, VEC> cg = a.gate ? load_chunk<T, VEC>(x + 2 * width + c) : ones<T, VEC>();
+        cx[j] = stream_of(cx[j], load_chunk<T, VEC>(x + width + c), cg, cw[j], cc[j], rx, squares);
         store_chunk<T, VEC>(static_cast<T *>(a.s) + row * a.s_stride + c, cx[j]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(to_float(cx[j].e[i]), to_float(cx[j].e[i]), sq[0]);
       }
     }
+    sq[0] = total(squares);
     block_sums(sq, &slot[1]);
     const float rs = rsqrtf(fmaf(sq[0], inv_width, eps));
     if (t == 0 && k + stages < rows) fetch(k + stages);  // every thread has read the stage
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
-      if (c < width) {
-        float f[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = to_float(cx[j].e[i]) * rs * to_float(cn[j].e[i]);
-        store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, to_chunk<T, VEC>(f));
-      }
+      if (c < width) store_chunk<T, VEC>(static_cast<T *>(a.y) + row * a.y_stride + c, normed(cx[j], cn[j], rs));
     }
   }
   if (t == 0) ring.settle(k, rows);
@@ -419,6 +446,8 @@ __global__ void __launch_bounds__(512)
     k_sandwich_backward_ring(const so3lr_sandwich_norm_backward_args a, float *partial, int stages,
                              const WaitLimit limit, const float inv_width, const float eps) {
   constexpr int VEC = 16 / sizeof(T), N = PER / VEC;
+  using F = Floats<VEC>;
+  using V = typename F::V;
   __shared__ __align__(16) float slot[4][16];
   extern __shared__ __align__(128) unsigned char smem[];
   const int width = int(a.width), t = threadIdx.x, size = blockDim.x;
@@ -448,10 +477,13 @@ __global__ void __launch_bounds__(512)
   if (t == 0)
     for (int i = 0; i < min(stages, rows); ++i) fetch(i);
   Chunk<W, VEC> cw[N], cn[N], cc[N];
-  float sums[3][PER] = {};
+  F sums[3][N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = (j * size + t) * VEC;
+    cc[j] = ones<W, VEC>();
+#pragma unroll
+    for (int i = 0; i < F::kCount; ++i) sums[0][j].v[i] = sums[1][j].v[i] = sums[2][j].v[i] = V(0.0f);
     if (c < width) {
       cw[j] = load_chunk<W, VEC>(static_cast<const W *>(a.weight) + c);
       cn[j] = load_chunk<W, VEC>(static_cast<const W *>(a.next_weight) + c);
@@ -464,7 +496,7 @@ __global__ void __launch_bounds__(512)
     const T *stage = reinterpret_cast<const T *>(ring.stage(k));
     const SandwichBackRow<T, W> row(a, blockIdx.x + (long long)k * gridDim.x);
     Chunk<T, VEC> cs[N], cd[N], cx[N];
-    float first[3] = {};  // sums of x^2, s^2, s dy next
+    V squares[3] = {V(0.0f), V(0.0f), V(0.0f)};
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
@@ -472,59 +504,48 @@ __global__ void __launch_bounds__(512)
         cs[j] = load_chunk<T, VEC>(stage + c);
         cd[j] = load_chunk<T, VEC>(stage + width + c);
         cx[j] = load_chunk<T, VEC>(stage + 2 * width + c);
+        const F x = floats_of(cx[j]), s = floats_of(cs[j]), dy = floats_of(cd[j]), n = floats_of(cn[j]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float f = to_float(cs[j].e[i]), x = to_float(cx[j].e[i]);
-          first[0] = fmaf(x, x, first[0]);
-          first[1] = fmaf(f, f, first[1]);
-          first[2] = fmaf(f, to_float(cd[j].e[i]) * to_float(cn[j].e[i]), first[2]);
-        }
+        for (int i = 0; i < F::kCount; ++i) add_squares(x.v[i], s.v[i], dy.v[i], n.v[i], squares);
       }
     }
+    float first[3] = {total(squares[0]), total(squares[1]), total(squares[2])};
     block_sums(first, &slot[0]);
     if (ring.gave_up(k)) break;
     const float rx = rsqrtf(fmaf(first[0], inv_width, eps)), rs = rsqrtf(fmaf(first[1], inv_width, eps));
     const float back = -(first[2] * rs * inv_width) * rs * rs;
-    float av[PER], last[1] = {};
+    F av[N];
+    V row_sum(0.0f);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
       if (c < width) {
-        Chunk<T, VEC> ce{}, cg{}, cr{};
-        if (a.ds) ce = load_chunk<T, VEC>(stage + ds_at * width + c);
-        if (a.gate) cg = load_chunk<T, VEC>(stage + gate_at * width + c);
-        if (a.residual_scale) cr = load_chunk<T, VEC>(stage + residual_at * width + c);
-        float dres[VEC], dgate[VEC];
+        const F x = floats_of(cx[j]), s = floats_of(cs[j]), dy = floats_of(cd[j]),
+                ds = floats_of(a.ds ? load_chunk<T, VEC>(stage + ds_at * width + c) : Chunk<T, VEC>{}),
+                g = floats_of(a.gate ? load_chunk<T, VEC>(stage + gate_at * width + c) : ones<T, VEC>()),
+                r = floats_of(a.residual_scale ? load_chunk<T, VEC>(stage + residual_at * width + c) : Chunk<T, VEC>{}),
+                w = floats_of(cw[j]), n = floats_of(cn[j]), f = floats_of(cc[j]);
+        F dres, dgate;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float x = to_float(cx[j].e[i]);
-          const SandwichElement e(x, to_float(cs[j].e[i]), to_float(cd[j].e[i]), to_float(ce.e[i]), to_float(cr.e[i]),
-                                  a.gate ? to_float(cg.e[i]) : 1.0f, to_float(cw[j].e[i]), to_float(cn[j].e[i]),
-                                  a.residual_scale ? to_float(cc[j].e[i]) : 1.0f, rx, rs, back);
-          dres[i] = e.dres;
-          dgate[i] = e.dgate;
-          av[j * VEC + i] = e.a;
-          last[0] = fmaf(e.a, x, last[0]);
-          sums[0][j * VEC + i] += e.sum_w;
-          sums[1][j * VEC + i] += e.sum_next;
-          sums[2][j * VEC + i] += e.sum_scale;
+        for (int i = 0; i < F::kCount; ++i) {
+          const SandwichElement<V> e(x.v[i], s.v[i], dy.v[i], ds.v[i], r.v[i], g.v[i], w.v[i], n.v[i], f.v[i], rx, rs,
+                                     back, sums[0][j].v[i], sums[1][j].v[i], sums[2][j].v[i], row_sum);
+          dres.v[i] = e.dres;
+          dgate.v[i] = e.dgate;
+          av[j].v[i] = e.a;
         }
-        store_chunk<T, VEC>(row.dresidual + c, to_chunk<T, VEC>(dres));
-        if (a.gate) store_chunk<T, VEC>(row.dgate + c, to_chunk<T, VEC>(dgate));
+        store_chunk<T, VEC>(row.dresidual + c, chunk_of_floats<T, VEC>(dres));
+        if (a.gate) store_chunk<T, VEC>(row.dgate + c, chunk_of_floats<T, VEC>(dgate));
       }
     }
+    float last[1] = {total(row_sum)};
     block_sums(last, &slot[3]);
     const float back_x = -(last[0] * rx * inv_width) * rx * rx;
     if (t == 0 && k + stages < rows) fetch(k + stages);  // every thread has read the stage
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
-      if (c < width) {
-        float dx[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) dx[i] = fmaf(av[j * VEC + i], rx, to_float(cx[j].e[i]) * back_x);
-        store_chunk<T, VEC>(row.dx + c, to_chunk<T, VEC>(dx));
-      }
+      if (c < width) store_chunk<T, VEC>(row.dx + c, dx_of(av[j], cx[j], rx, back_x));
     }
   }
   if (t == 0) ring.settle(k, rows);
@@ -533,10 +554,7 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int c = (j * size + t) * VEC;
-      if (c < width)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          partial[((size_t)blockIdx.x * 3 + q) * width + c + i] = sums[q][j * VEC + i];
+      if (c < width) write_floats(partial + ((size_t)blockIdx.x * 3 + q) * width + c, sums[q][j]);
     }
 }
 
@@ -566,10 +584,7 @@ __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sand
       const Chunk<W, VEC> cn = load_chunk<W, VEC>(next + c);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float x = to_float(cx.e[i]), f = to_float(cs.e[i]);
-        first[0] = fmaf(x, x, first[0]);
-        first[1] = fmaf(f, f, first[1]);
-        first[2] = fmaf(f, to_float(cd.e[i]) * to_float(cn.e[i]), first[2]);
+        add_squares(to_float(cx.e[i]), to_float(cs.e[i]), to_float(cd.e[i]), to_float(cn.e[i]), first);
       }
     }
     block_sums(first, &slot[0]);
@@ -587,10 +602,11 @@ __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sand
         if (row.residual) cr = load_chunk<T, VEC>(row.residual + c);
         if (row.gate) cg = load_chunk<T, VEC>(row.gate + c);
         if (scale) cc = load_chunk<W, VEC>(scale + c);
-        auto element = [&](int i) {
-          return SandwichElement(to_float(cx.e[i]), to_float(cs.e[i]), to_float(cd.e[i]), to_float(ce.e[i]),
-                                 to_float(cr.e[i]), row.gate ? to_float(cg.e[i]) : 1.0f, to_float(cw.e[i]),
-                                 to_float(cn.e[i]), scale ? to_float(cc.e[i]) : 1.0f, rx, rs, back);
+        auto element = [&](int i, float &sum_w, float &sum_next, float &sum_scale, float &row_sum) {
+          return SandwichElement<float>(to_float(cx.e[i]), to_float(cs.e[i]), to_float(cd.e[i]), to_float(ce.e[i]),
+                                        to_float(cr.e[i]), row.gate ? to_float(cg.e[i]) : 1.0f, to_float(cw.e[i]),
+                                        to_float(cn.e[i]), scale ? to_float(cc.e[i]) : 1.0f, rx, rs, back, sum_w,
+                                        sum_next, sum_scale, row_sum);
         };
         f(c, cx, element);
       }
@@ -600,13 +616,10 @@ __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sand
       float dres[VEC], dgate[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const SandwichElement e = element(i);
+        const SandwichElement<float> e =
+            element(i, column[c + i], column[width + c + i], column[2 * width + c + i], last[0]);
         dres[i] = e.dres;
         dgate[i] = e.dgate;
-        last[0] = fmaf(e.a, to_float(cx.e[i]), last[0]);
-        column[c + i] += e.sum_w;
-        column[width + c + i] += e.sum_next;
-        column[2 * width + c + i] += e.sum_scale;
       }
       store_chunk<T, VEC>(row.dresidual + c, to_chunk<T, VEC>(dres));
       if (row.dgate) store_chunk<T, VEC>(row.dgate + c, to_chunk<T, VEC>(dgate));
@@ -616,7 +629,10 @@ __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sand
     elements([&](int c, const Chunk<T, VEC> &cx, auto element) {
       float dx[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) dx[i] = fmaf(element(i).a, rx, to_float(cx.e[i]) * back_x);
+      for (int i = 0; i < VEC; ++i) {
+        float none[4] = {};
+        dx[i] = fmaf(element(i, none[0], none[1], none[2], none[3]).a, rx, to_float(cx.e[i]) * back_x);
+      }
       store_chunk<T, VEC>(row.dx + c, to_chunk<T, VEC>(dx));
     });
   }
