@@ -26,6 +26,13 @@
 namespace so3lr_b200 {
 namespace {
 
+// 1 / sqrt(a): a Newton step on the hardware's root, within a unit. The root's error is the whole
+// row's, and shows in how many elements of the stream round to the other side.
+__device__ __forceinline__ float inverse_root(float a) {
+  const float y = rsqrtf(a), e = fmaf(-a * y, y, 1.0f);
+  return fabsf(e) < 1.0f ? fmaf(0.5f * y, e, y) : y;  // 0, infinities and NaN as they are
+}
+
 template <class T, class W>
 struct SandwichRow {  // pointers to one row
   const T *x, *residual, *gate;
@@ -105,7 +112,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
       for (int i = 0; i < F::kCount; ++i) squares = madd(x.v[i], x.v[i], squares);
     }
   float sq = fmaf(to_float(ex), to_float(ex), total(squares));
-  const float rx = rsqrtf(fmaf(team.sum(sq, slot[0]), inv_width, eps));
+  const float rx = inverse_root(fmaf(team.sum(sq, slot[0]), inv_width, eps));
   // what is kept of the stream is rounded, and the second norm is of what is kept
   squares = V(0.0f);
 #pragma unroll
@@ -127,7 +134,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
     if (live) row.s[c] = ex;
     sq += one;
   }
-  const float rs = rsqrtf(fmaf(team.sum(sq, slot[1]), inv_width, eps));
+  const float rs = inverse_root(fmaf(team.sum(sq, slot[1]), inv_width, eps));
   if (!live) return;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
@@ -268,7 +275,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
     float three[3] = {total(squares[0]), total(squares[1]), total(squares[2])};
     if (edge) add_squares(to_float(ex), to_float(es), to_float(ed), to_float(next[span.edge]), three);
     const float3 all = team.sum3(three[0], three[1], three[2], slot[0], slot2);
-    const float rx = rsqrtf(fmaf(all.x, inv_width, eps)), rs = rsqrtf(fmaf(all.y, inv_width, eps));
+    const float rx = inverse_root(fmaf(all.x, inv_width, eps)), rs = inverse_root(fmaf(all.y, inv_width, eps));
     const float back = -(all.z * rs * inv_width) * rs * rs;
     F av[N];
     V row_sum(0.0f);
@@ -415,7 +422,7 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
     }
     float sq[1] = {total(squares)};
     block_sums(sq, &slot[0]);
-    const float rx = rsqrtf(fmaf(sq[0], inv_width, eps));
+    const float rx = inverse_root(fmaf(sq[0], inv_width, eps));
     if (ring.gave_up(k)) break;
     squares = V(0.0f);
 #pragma unroll
@@ -429,7 +436,7 @@ __global__ void __launch_bounds__(512, PER == 8 ? 2 : 1)
     }
     sq[0] = total(squares);
     block_sums(sq, &slot[1]);
-    const float rs = rsqrtf(fmaf(sq[0], inv_width, eps));
+    const float rs = inverse_root(fmaf(sq[0], inv_width, eps));
     if (t == 0 && k + stages < rows) fetch(k + stages);  // every thread has read the stage
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -512,7 +519,7 @@ __global__ void __launch_bounds__(512)
     float first[3] = {total(squares[0]), total(squares[1]), total(squares[2])};
     block_sums(first, &slot[0]);
     if (ring.gave_up(k)) break;
-    const float rx = rsqrtf(fmaf(first[0], inv_width, eps)), rs = rsqrtf(fmaf(first[1], inv_width, eps));
+    const float rx = inverse_root(fmaf(first[0], inv_width, eps)), rs = inverse_root(fmaf(first[1], inv_width, eps));
     const float back = -(first[2] * rs * inv_width) * rs * rs;
     F av[N];
     V row_sum(0.0f);
@@ -588,7 +595,7 @@ __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sand
       }
     }
     block_sums(first, &slot[0]);
-    const float rx = rsqrtf(fmaf(first[0], inv_width, eps)), rs = rsqrtf(fmaf(first[1], inv_width, eps));
+    const float rx = inverse_root(fmaf(first[0], inv_width, eps)), rs = inverse_root(fmaf(first[1], inv_width, eps));
     const float back = -(first[2] * rs * inv_width) * rs * rs;
     // f(c, i, the element) over the row
     auto elements = [&](auto f) {
