@@ -233,10 +233,13 @@ __device__ __forceinline__ void add_columns(unsigned char *stage, int lane, floa
 #pragma unroll
   for (int i = 0; i < 32; i += 4) {
     const float4 b = *reinterpret_cast<const float4 *>(column + i);
-    r[i] = __float_as_uint(__uint_as_float(r[i]) + b.x);
-    r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) + b.y);
-    r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) + b.z);
-    r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) + b.w);
+    float u, w;
+    (Pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])) + Pair(b.x, b.y)).get(u, w);
+    r[i] = __float_as_uint(u);
+    r[i + 1] = __float_as_uint(w);
+    (Pair(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])) + Pair(b.z, b.w)).get(u, w);
+    r[i + 2] = __float_as_uint(u);
+    r[i + 3] = __float_as_uint(w);
   }
   __syncwarp();
 }
@@ -530,7 +533,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
           }
           by_activation(p.act, [&](auto act) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(activate<decltype(act)::value>(__uint_as_float(r[i])));
+            for (int i = 0; i < 32; i += 2) {
+              float a, b;
+              activate<decltype(act)::value>(Pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1]))).get(a, b);
+              r[i] = __float_as_uint(a);
+              r[i + 1] = __float_as_uint(b);
+            }
           });
           if (p.residual) {
             if (fetched_ahead)
@@ -539,7 +547,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_dense
               gather_rows<H>(stage, lane, static_cast<const H *>(p.residual) + row0 * p.ldr + c0, p.ldr, rows,
                              q.n - c0, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + to_float(v[i / 8].e[i % 8]));
+            for (int i = 0; i < 32; i += 2) {
+              const Floats<8> f = floats_of(v[i / 8]);
+              float a, b;
+              (Pair(__uint_as_float(r[i]), __uint_as_float(r[i + 1])) + f.v[i % 8 / 2]).get(a, b);
+              r[i] = __float_as_uint(a);
+              r[i + 1] = __float_as_uint(b);
+            }
             if (j + 1 < S::kWarpChunks) fetched_ahead = fetch_residual(j + 1);
           }
 #pragma unroll

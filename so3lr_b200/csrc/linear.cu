@@ -46,18 +46,20 @@ __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs 
   const int c = (blockIdx.x * a.lanes + t) * kVec, left = a.n - c;
   const int step = kWarps * rows_of_warp;
   const long long begin = blockIdx.y * a.rows_per_block, end = min(a.rows, begin + a.rows_per_block);
-  float total[kVec] = {};
-  auto one = [&](const Chunk<T, kVec> &dy, const Chunk<T, kVec> &z, long long row) {
-    float d[kVec];
+  Floats<kVec> sum;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      d[i] = to_float(dy.e[i]);
-      if (ACT != SO3LR_NO_ACTIVATION) d[i] *= slope<ACT>(to_float(z.e[i]));
-      total[i] += d[i];
+  for (int i = 0; i < kVec / 2; ++i) sum.v[i] = Pair(0.0f);
+  auto one = [&](const Chunk<T, kVec> &dy, const Chunk<T, kVec> &z, long long row) {
+    Floats<kVec> d = floats_of(dy);
+    const Floats<kVec> zf = floats_of(z);
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) {
+      if (ACT != SO3LR_NO_ACTIVATION) d.v[i] = d.v[i] * slope<ACT>(zf.v[i]);
+      sum.v[i] = sum.v[i] + d.v[i];
     }
     if (ACT == SO3LR_NO_ACTIVATION) return;
     T *dz = static_cast<T *>(a.dz) + row * a.dz_stride + c;  // rows are padded to whole chunks
-    store_chunk<T, kVec>(dz, to_chunk<T, kVec>(d));
+    store_chunk<T, kVec>(dz, chunk_of_floats<T, kVec>(d));
   };
   if (left > 0) {
     const T *dy = static_cast<const T *>(a.dy) + c, *z = static_cast<const T *>(a.z) + c;
@@ -81,8 +83,9 @@ __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs 
     }
   }
   if (!a.partial) return;
+  const Chunk<float, kVec> total = chunk_of_floats<float, kVec>(sum);
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) sums[threadIdx.x][i] = total[i];
+  for (int i = 0; i < kVec; ++i) sums[threadIdx.x][i] = total.e[i];
   __syncthreads();
   // thread: one column of the strip; the rows' owners in order
   for (int i = threadIdx.x; i < a.lanes * kVec; i += blockDim.x) {
