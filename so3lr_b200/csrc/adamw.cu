@@ -425,7 +425,7 @@ void launch_step(const so3lr_adamw_args &a, float4 *coef, cudaStream_t s) {
   for (long long i = 0; i < a.count; ++i) {
     const so3lr_adamw_tensor &x = a.tensors[i];
     const long long chunks = (x.n + kChunk - 1) / kChunk;  // 2^29 at most
-    if (t.count == MOST || t.chunks + chunks > 0x7fffffffLL) flush();
+    if (t.count == MOST || t.chunks + chunks > 0x7fffffffLL - kAhead) flush();
     t.e[t.count] = Entry{x.param, x.grad, x.master, x.exp_avg, x.exp_avg_sq, x.exp_avg_scale, x.exp_avg_sq_scale, x.n};
     const bool wide = on(x.param, 16) && on(x.grad, 16) &&
                       on(x.master, 16) && on(x.exp_avg, 16) && on(x.exp_avg_sq, 16);

@@ -391,6 +391,22 @@ def test_optimizer_groups_schedules_and_missing_gradients(optim):
     assert float(adam.step(closure).detach()) > 0
 
 
+def test_optimizer_rate_on_the_gpu(optim):
+    """A rate that is a tensor, and a schedule that writes into it, do what numbers do."""
+    runs = []
+    for lr in (HYPER["lr"], torch.tensor(HYPER["lr"], device="cuda")):
+        model = _model()
+        adam = optim.AdamW(model.parameters(), **{**HYPER, "lr": lr})
+        schedule = torch.optim.lr_scheduler.StepLR(adam, 1, gamma=0.5)
+        for k in range(3):
+            _backward(model, k)
+            adam.step()
+            schedule.step()
+        runs.append([adam.state[p]["master"] for p in model.parameters()])
+    for a, b in zip(*runs):  # the rate itself is rounded to float32: 2^-24 of three updates of at most 2 lr
+        assert bool(((a - b).abs() <= 2.0 ** -23 * (a.abs() + 6 * HYPER["lr"])).all())
+
+
 def test_optimizer_marks_parameters_as_changed(optim):
     """A backward pass that kept a parameter from before the step is refused, as after torch's own steps."""
     w = torch.nn.Parameter(torch.ones(8, device="cuda"))
