@@ -684,21 +684,42 @@ constexpr Hold sandwich_hold(long long width, Path path, int size, bool backward
   if (backward && width > 4096) return {0, 0};
   return {0, width <= 8192 ? 8 : 16};
 }
-template <class F>
-void by_sandwich_hold(const Hold &h, F &&f) {
-  using std::integral_constant;
-  if (h.lanes == 8) return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-  if (h.lanes == 16) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-  if (h.lanes == 32 && h.per == 8) return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-  if (h.lanes == 32) return f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
-  if (h.per == 8) return f(integral_constant<int, 0>{}, integral_constant<int, 8>{});
-  return f(integral_constant<int, 0>{}, integral_constant<int, 16>{});
-}
-
 // The rings: rows too long for a warp with 8 elements a lane, up to what a ring of two holds. 65536
 // rows of 512 bfloat16: 67 us forward and 133 back, 73 and 192 in a warp with 16 elements a lane;
 // 32768 rows of 512 float32: 63 and 115, 53 and 102 in a warp.
-bool ring_takes(long long width, int size) { return width > (size == 2 ? 256 : 512) && width <= 8192; }
+constexpr bool ring_takes(long long width, int size) { return width > (size == 2 ? 256 : 512) && width <= 8192; }
+// Whether a call reaches the kernels that hold a row so: the widths are those at which
+// sandwich_hold changes, each the widest of its kind.
+constexpr bool held_so(Path path, int size, bool backward, int lanes, int per) {
+  for (const int width : {64, 128, 256, 512, 4096, 8192, 16384}) {
+    if (backward && path == kWide && ring_takes(width, size)) continue;
+    const Hold h = sandwich_hold(width, path, size, backward);
+    if (h.lanes == lanes && h.per == per) return true;
+  }
+  return false;
+}
+// f(std::integral_constant lanes, std::integral_constant per) for h; kernels are compiled for those
+// that a call reaches
+template <Path PATH, int SIZE, bool BACKWARD, class F>
+void by_sandwich_hold(const Hold &h, F &&f) {
+  bool found = false;
+  auto lanes_per = [&](auto lanes, auto per) {
+    if constexpr (held_so(PATH, SIZE, BACKWARD, decltype(lanes)::value, decltype(per)::value))
+      if (h.lanes == lanes && h.per == per) {
+        found = true;
+        f(lanes, per);
+      }
+  };
+  using std::integral_constant;
+  lanes_per(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  lanes_per(integral_constant<int, 0>{}, integral_constant<int, 8>{});
+  lanes_per(integral_constant<int, 0>{}, integral_constant<int, 16>{});
+  if (!found) throw Error("sandwich norm: no kernel holds such a row");
+}
+
 int ring_per(long long width) { return width <= 4096 ? 8 : 16; }
 RingPlan forward_ring(const so3lr_sandwich_norm_args &a, Path path) {
   if (path != kWide || !ring_takes(a.width, a.dtype == SO3LR_FLOAT32 ? 4 : 2)) return RingPlan{0, 0, 0};
@@ -783,7 +804,7 @@ void launch_sandwich_norm(const so3lr_sandwich_norm_args &a, cudaStream_t s) {
         constexpr Path PATH = decltype(path)::value;
         constexpr int VEC = chunk_of(PATH, sizeof(T));
         const Hold h = sandwich_hold(a.width, PATH, sizeof(T), false);
-        by_sandwich_hold(h, [&](auto lanes, auto per) {
+        by_sandwich_hold<PATH, sizeof(T), false>(h, [&](auto lanes, auto per) {
           constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
           launch(k_sandwich<T, W, VEC, N, L, PATH == kShifted>, team_grid(h, a.rows), team_block(h, a.width), 0, s, a,
                  1.0f / float(a.width), float(a.eps));
@@ -827,12 +848,10 @@ void launch_sandwich_norm_backward(const so3lr_sandwich_norm_backward_args &a, v
         by_path(p.path, [&](auto path) {
           constexpr Path PATH = decltype(path)::value;
           constexpr int VEC = chunk_of(PATH, sizeof(T));
-          by_sandwich_hold(p.hold, [&](auto lanes, auto per) {
-            constexpr int L = decltype(lanes)::value, P = decltype(per)::value, N = P / VEC;
-            // rows on the boundaries that the rings take are not held in registers
-            if constexpr (PATH == kWide ? L != 0 && (P == 8 || sizeof(T) == 4) : L != 0 || P == 8)
-              launch(k_sandwich_backward<T, W, VEC, N, L, PATH == kShifted>, p.grid, p.threads,
-                     L ? kTeamThreads / (L ? L : 1) * a.width * sizeof(float) : 0, s, a, partial, inv, eps);
+          by_sandwich_hold<PATH, sizeof(T), true>(p.hold, [&](auto lanes, auto per) {
+            constexpr int L = decltype(lanes)::value, N = decltype(per)::value / VEC;
+            launch(k_sandwich_backward<T, W, VEC, N, L, PATH == kShifted>, p.grid, p.threads,
+                   L ? kTeamThreads / (L ? L : 1) * a.width * sizeof(float) : 0, s, a, partial, inv, eps);
           });
         });
       }

@@ -33,6 +33,10 @@ EXPORTED = (
     "so3lr_layers_status", "so3lr_layers_wait_limit", "so3lr_rms_norm", "so3lr_rms_norm_backward_workspace", "so3lr_rms_norm_backward", "so3lr_int8_linear_workspace",
     "so3lr_int8_linear", "so3lr_gate_int8", "so3lr_dequantize_int8", "so3lr_feed_forward_workspace",
     "so3lr_feed_forward_keep", "so3lr_feed_forward", "so3lr_feed_forward_backward_workspace", "so3lr_feed_forward_backward",
+    # dense layer, norms on both sides of a block (bound in layers.py), AdamW (bound in optim.py)
+    "so3lr_linear_workspace", "so3lr_linear", "so3lr_linear_backward_workspace", "so3lr_linear_backward",
+    "so3lr_sandwich_norm", "so3lr_sandwich_norm_backward_workspace", "so3lr_sandwich_norm_backward",
+    "so3lr_adamw_workspace", "so3lr_adamw", "so3lr_moment_values",
 )
 
 _dp = C.POINTER(C.c_double)
