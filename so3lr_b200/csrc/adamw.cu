@@ -17,8 +17,8 @@
 // An 8-bit moment is a code for each element and, for each 256 of them, the largest
 // magnitude `top`: m = top t |t| with t = code / 127, v = top t^4 with t = code / 255.
 // The roots spread the codes over the magnitudes that a block mixes: m down to 6e-5 of
-// the largest, the root of v to 1.5e-5, both with steps of at most 1.6 % (v: 1.6 %) near
-// the largest, and the largest itself is kept exactly, so that a block decays as its
+// the largest, the root of v to 1.5e-5, both in steps of 1.6 % of the value near the
+// largest, and the largest itself is kept exactly, so that a block decays as its
 // moments do. Codes are rounded to nearest. A v that is not zero never becomes zero
 // (its code is 1 at least): m / sqrt(v) would otherwise run away. One warp holds the 256
 // elements of a scale, eight to a lane.

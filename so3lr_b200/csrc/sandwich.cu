@@ -16,8 +16,8 @@
 // adds those in order.
 //
 // Measured, 33.5 M elements with gate and scale, forward and backward (TB/s): bfloat16 rows of
-// 256 5.5 and 4.6, of 1024 5.4 and 4.8, of 4096 5.4 and 4.2, of 1003 3.6 and 2.8, of 16384 3.4 and
-// 1.8; float32 rows (half as many) 6.5 and 6.0, 5.8 and 5.5, 5.9 and 5.3, 5.7 and 5.3, 4.5 and 3.0.
+// 256 5.9 and 5.0, of 1024 5.8 and 5.2, of 4096 6.0 and 4.6, of 1003 4.0 and 3.3, of 16384 4.1 and
+// 1.8; float32 rows (half as many) 6.5 and 6.0, 6.5 and 6.1, 6.2 and 5.3, 5.7 and 5.3, 4.7 and 3.0.
 // With 2-byte elements a row's two reductions, about 50 instructions a thread, and one block of
 // 512 threads an SM (the column sums fill the registers) hold the backward pass back.
 #include "pairs.cuh"
@@ -684,15 +684,18 @@ constexpr Hold sandwich_hold(long long width, Path path, int size, bool backward
   if (backward && width > 4096) return {0, 0};
   return {0, width <= 8192 ? 8 : 16};
 }
-// The rings: rows too long for a warp with 8 elements a lane, up to what a ring of two holds. 65536
-// rows of 512 bfloat16: 67 us forward and 133 back, 73 and 192 in a warp with 16 elements a lane;
-// 32768 rows of 512 float32: 63 and 115, 53 and 102 in a warp.
-constexpr bool ring_takes(long long width, int size) { return width > (size == 2 ? 256 : 512) && width <= 8192; }
+// The rings take rows on the boundaries from these widths on, up to what a ring of two holds (us, 33.5
+// M elements, in registers and through the ring). Forward, bfloat16 512: 52 and 61, 768: 65 and 59,
+// 4096: 83 and 56; float32 (half as many) 1024: 51 and 59, 4096: 55 and 58, 8192: 71 and 58. Backward,
+// bfloat16 512: 132 and 121, 4096: 188 and 132; float32 2048: 104 and 110, 4096: 121 and 114.
+constexpr bool ring_takes(long long width, int size, bool backward) {
+  return width > (backward ? (size == 2 ? 256 : 2048) : (size == 2 ? 512 : 4096)) && width <= 8192;
+}
 // Whether a call reaches the kernels that hold a row so: the widths are those at which
-// sandwich_hold changes, each the widest of its kind.
+// sandwich_hold or ring_takes changes, each the widest of its kind.
 constexpr bool held_so(Path path, int size, bool backward, int lanes, int per) {
-  for (const int width : {64, 128, 256, 512, 4096, 8192, 16384}) {
-    if (backward && path == kWide && ring_takes(width, size)) continue;
+  for (const int width : {64, 128, 256, 512, 2048, 4096, 8192, 16384}) {
+    if (backward && path == kWide && ring_takes(width, size, true)) continue;
     const Hold h = sandwich_hold(width, path, size, backward);
     if (h.lanes == lanes && h.per == per) return true;
   }
@@ -722,7 +725,7 @@ void by_sandwich_hold(const Hold &h, F &&f) {
 
 int ring_per(long long width) { return width <= 4096 ? 8 : 16; }
 RingPlan forward_ring(const so3lr_sandwich_norm_args &a, Path path) {
-  if (path != kWide || !ring_takes(a.width, a.dtype == SO3LR_FLOAT32 ? 4 : 2)) return RingPlan{0, 0, 0};
+  if (path != kWide || !ring_takes(a.width, a.dtype == SO3LR_FLOAT32 ? 4 : 2, false)) return RingPlan{0, 0, 0};
   const int per = ring_per(a.width);
   return ring_plan(a.rows, row_threads(a.width, per), per == 8 ? 1024 : 512, 2,
                    (a.gate ? 3 : 2) * a.width * (a.dtype == SO3LR_FLOAT32 ? 4 : 2));
@@ -749,7 +752,7 @@ BackPlan back_plan(const so3lr_sandwich_norm_backward_args &a) {
                                aligned(a.residual_scale, 0, 1, 16));
   p.hold = sandwich_hold(a.width, p.path, t.size, true);
   p.ring = RingPlan{0, 0, 0};
-  if (p.path == kWide && ring_takes(a.width, t.size)) {
+  if (p.path == kWide && ring_takes(a.width, t.size, true)) {
     const int per = ring_per(a.width), threads = row_threads(a.width, per);
     const RingPlan r = ring_plan(a.rows, threads, 512, 2,
                                  (3 + (a.ds ? 1 : 0) + (a.gate ? 1 : 0) + (a.residual_scale ? 1 : 0)) * a.width * t.size);
@@ -794,10 +797,13 @@ void launch_sandwich_norm(const so3lr_sandwich_norm_args &a, cudaStream_t s) {
           launch(kernel, r.grid, row_threads(a.width, ring_per(a.width)), r.smem, s, a, r.stages, wait_limit(),
                  1.0f / float(a.width), float(a.eps));
         };
-        if (ring_per(a.width) == 8)
-          go(&k_sandwich_ring<T, W, 8>);
-        else
-          go(&k_sandwich_ring<T, W, 16>);
+        if constexpr (sizeof(T) == 2) {
+          if (ring_per(a.width) == 8) {
+            go(&k_sandwich_ring<T, W, 8>);
+            return;
+          }
+        }
+        go(&k_sandwich_ring<T, W, 16>);
         return;
       }
       by_path(chosen, [&](auto path) {

@@ -36,14 +36,15 @@ def _expected():
                 lanes, per = _hold(width, path, size, False)
                 out.add(f"k_sandwich<{t}, {w}, {vec}, {per // vec}, {lanes}, {shift}>")
                 lanes, per = _hold(width, path, size, True)
-                ring = path == "wide" and (256 if size == 2 else 512) < width <= 8192
+                ring = path == "wide" and (256 if size == 2 else 2048) < width <= 8192
                 if per and not ring:
                     out.add(f"k_sandwich_backward<{t}, {w}, {vec}, {per // vec}, {lanes}, {shift}>")
                 if not per:
                     out.add(f"k_sandwich_backward_long<{t}, {w}, {vec if path == 'wide' else 1}>")
                 if ring:
-                    for name in ("k_sandwich_ring", "k_sandwich_backward_ring"):
-                        out.add(f"{name}<{t}, {w}, {8 if width <= 4096 else 16}>")
+                    out.add(f"k_sandwich_backward_ring<{t}, {w}, {8 if width <= 4096 else 16}>")
+                if path == "wide" and (512 if size == 2 else 4096) < width <= 8192:
+                    out.add(f"k_sandwich_ring<{t}, {w}, {8 if width <= 4096 else 16}>")
     return out
 
 
