@@ -156,7 +156,9 @@ def linear(x, weight, bias=None, residual=None, *, activation=None):
     (z Phi(z)), "gelu_tanh" or "relu". Sums and everything after them are float32, y is
     rounded once. For the gradients of an activation its argument is kept in x's type."""
     act = _activation(activation)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
         return _LinearFunction.apply(x, weight, bias, residual, act)
     return _layers.linear(x, weight, bias, residual, act, False)
 
@@ -209,10 +211,12 @@ def sandwich_norm(x, residual, weight, next_weight, gate=None, residual_scale=No
     residual and gate have x's shape and type (a gate may be expanded over rows), the weights
     and residual_scale are vectors of x's type or all three float32. Without gate or
     residual_scale they are 1."""
-    args = x, residual, weight, next_weight, gate, residual_scale
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        return _SandwichFunction.apply(*args, eps)
-    return _layers.sandwich_norm(*args, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad) or
+                                    weight.requires_grad or next_weight.requires_grad or
+                                    (gate is not None and gate.requires_grad) or
+                                    (residual_scale is not None and residual_scale.requires_grad)):
+        return _SandwichFunction.apply(x, residual, weight, next_weight, gate, residual_scale, eps)
+    return _layers.sandwich_norm(x, residual, weight, next_weight, gate, residual_scale, eps)
 
 
 def sandwich_norm_backward(dy, ds, s, x, residual, weight, next_weight, gate=None, residual_scale=None, *,

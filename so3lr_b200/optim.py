@@ -23,7 +23,6 @@ __all__ = ["AdamW", "adamw_step", "moment_values", "SCALE_BLOCK"]
 SCALE_BLOCK = 256  # elements of a tensor that share the scale of an 8-bit moment
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, exp_avg_scales=None, exp_avg_sq_scales=None,
                masters=None, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2) -> None:
     """One AdamW step of lists of contiguous tensors, in place:
