@@ -29,7 +29,10 @@ struct BackArgs {
 
 template <bool WIDE, class T>
 __device__ __forceinline__ Chunk<T, kVec> load_part(const T *p, bool wide, int left) {
-  if (WIDE) return load_chunk<T, kVec>(p);
+  if (WIDE) {
+    const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(p));
+    return *reinterpret_cast<const Chunk<T, kVec> *>(&v);
+  }
   if (wide && left >= kVec) return load_chunk<T, kVec>(p);
   Chunk<T, kVec> c;
 #pragma unroll
