@@ -47,9 +47,10 @@ except (ImportError, So3lrError) as e:
     raise ImportError(f"the feed-forward layers' module is missing or does not fit the installed torch ({e}): build it "
                       "with `python -m so3lr_b200.build`, which needs a torch with CUDA and Python's headers") from e
 
-__all__ = ["linear", "linear_train", "linear_backward", "rms_norm", "rms_norm_int8", "rms_norm_backward", "sandwich_norm", "sandwich_norm_backward", "int8_linear", "gate_int8", "dequantize_int8",
-           "quantize_weight", "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock",
-           "SandwichBlock", "Int8FeedForwardBlock", "check_status", "set_wait_limit"]
+__all__ = ["linear", "linear_train", "linear_backward", "rms_norm", "rms_norm_int8", "rms_norm_backward",
+           "sandwich_norm", "sandwich_norm_backward", "int8_linear", "gate_int8", "dequantize_int8", "quantize_weight",
+           "feed_forward", "feed_forward_train", "feed_forward_backward", "FeedForwardBlock", "SandwichBlock",
+           "Int8FeedForwardBlock", "check_status", "set_wait_limit"]
 
 
 def check_status(device=None) -> None:
