@@ -542,7 +542,8 @@ int so3lr_feed_forward_backward(const so3lr_feed_forward_backward_args *args, vo
 /* Dense layer, bfloat16 or float16:
  *   z = x W^T + bias,   y = act(z) + residual
  * Sums, bias, activation and residual are float32, y is rounded once. gelu is z Phi(z) with the
- * normal distribution's Phi, gelu_tanh z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2. y may
+ * normal distribution's Phi (formed within 2e-7, and within 2e-5 of its value for z >= -12), gelu_tanh
+ * z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2. y may
  * be the memory of residual, row for row. A training step with an activation passes `z`, which
  * the gradient reads: z rounded to the element type and kept finite. */
 #define SO3LR_NO_ACTIVATION 0

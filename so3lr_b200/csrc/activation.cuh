@@ -11,8 +11,7 @@ constexpr float kTanhSlope = 1.5957691f, kTanhCube = 0.044715f;  // 2 sqrt(2 / p
 
 template <int ACT>
 __device__ __forceinline__ Pair activate(const Pair &z);
-// gelu: z Phi(z), Phi(-|z|) = t poly(t) exp(-z^2 / 2) / 2, t = 1 / (1 + p |z| / sqrt 2) (Abramowitz and
-// Stegun 7.1.26, off by 1.5e-7 at most; with erff 24000 x 256 -> 1024 takes 49 us, so 37).
+// gelu: z Phi(z), see normal_cdf.
 // gelu_tanh: z (1 + tanh(u)) / 2 = z sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3). relu keeps a NaN.
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
@@ -64,10 +63,16 @@ __device__ __forceinline__ Pair tanh_sigmoid(const Pair &z) {  // sigmoid(2 u) o
   const Pair cube = z * Pair(kTanhCube) * z;
   return sigmoid_pair(madd(cube, z, z) * Pair(-kTanhSlope * kLog2E));
 }
+// Phi(z) and e = exp(-z^2 / 2). Phi(-|z|) = t poly(t) e with t = 1 / (1 + 0.35 |z|), the form of
+// Hastings' approximations of erf. The coefficients were fitted here (a linear program over 6000 points of
+// |z| <= 14) so that the largest of the relative error / 5e-6 and the absolute error / 3e-8 is least, 1.04: far
+// out, where z Phi(z) is small, it keeps its leading digits too. In float32 arithmetic 2e-7 and, up to |z| = 12,
+// 2e-5 of the value. (Abramowitz and Stegun's 7.1.26, of two terms fewer, is off by 1 % at z = -8 for the same
+// absolute error.)
 __device__ __forceinline__ Pair normal_cdf(const Pair &z, Pair &e) {
   float a, b, ta, tb, ea, eb;
   z.get(a, b);
-  madd(Pair(fabsf(a), fabsf(b)), Pair(0.3275911f * 0.70710678f), Pair(1.0f)).get(ta, tb);
+  madd(Pair(fabsf(a), fabsf(b)), Pair(0.35f), Pair(1.0f)).get(ta, tb);
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(ta));
   asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(tb));
   (z * z * Pair(-0.5f * kLog2E)).get(ea, eb);
@@ -75,10 +80,12 @@ __device__ __forceinline__ Pair normal_cdf(const Pair &z, Pair &e) {
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(eb));
   const Pair t(ta, tb);
   e = Pair(ea, eb);
-  Pair q = madd(t, Pair(0.5f * 1.061405429f), Pair(0.5f * -1.453152027f));
-  q = madd(q, t, Pair(0.5f * 1.421413741f));
-  q = madd(q, t, Pair(0.5f * -0.284496736f));
-  q = madd(q, t, Pair(0.5f * 0.254829592f)) * (t * e);
+  Pair q = madd(t, Pair(0.0441702157f), Pair(-0.182627589f));
+  q = madd(q, t, Pair(0.208162174f));
+  q = madd(q, t, Pair(0.0113299619f));
+  q = madd(q, t, Pair(0.142112911f));
+  q = madd(q, t, Pair(0.137093723f));
+  q = madd(q, t, Pair(0.139758632f)) * (t * e);
   float qa, qb;
   q.get(qa, qb);
   return Pair(a < 0.0f ? qa : 1.0f - qa, b < 0.0f ? qb : 1.0f - qb);
