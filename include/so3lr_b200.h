@@ -707,6 +707,9 @@ typedef struct {
   double eps;                 /* in 1e-30..1e30 */
   double weight_decay;        /* >= 0 */
 } so3lr_adamw_args;
+/* Whether so3lr_adamw refuses the arguments, without a launch: for a step that takes several calls
+ * and is to be taken as a whole or not at all. */
+int so3lr_adamw_check(const so3lr_adamw_args *args, char *err, size_t errlen);
 long long so3lr_adamw_workspace(const so3lr_adamw_args *args);
 int so3lr_adamw(const so3lr_adamw_args *args, void *workspace, long long workspace_bytes, void *stream, char *err,
                 size_t errlen);

@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdio>
+#include <deque>
 #include <optional>
 #include <sstream>
 #include <stdexcept>
@@ -623,10 +624,24 @@ const Tensor &element(const List &list, Py_ssize_t i, const char *what, c10::Dev
 
 constexpr int64_t kScaleBlock = 256;
 
-// adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales | None, exp_avg_sq_scales | None,
-//            masters | None, lr, beta1, beta2, eps, weight_decay) -> None
-PyObject *adamw_step(Args o) {
-  const List params(o[0], "params"), grads(o[1], "grads"), ms(o[2], "exp_avgs"), vs(o[3], "exp_avg_sqs");
+// One AdamW call: its arguments as the library takes them. The Python objects must outlive it.
+struct AdamwCall {
+  List params;
+  so3lr_adamw_args a{};
+  std::vector<so3lr_adamw_tensor> tensors;
+  c10::Device device{c10::kCUDA};
+  explicit AdamwCall(Args o);
+  AdamwCall(const AdamwCall &) = delete;
+  void check_arguments() const {
+    char err[1024] = "";
+    check(so3lr_adamw_check(&a, err, sizeof err), err);
+  }
+  void run() const;
+};
+// params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales | None, exp_avg_sq_scales | None, masters | None, lr,
+// beta1, beta2, eps, weight_decay
+AdamwCall::AdamwCall(Args o) : params(o[0], "params") {
+  const List grads(o[1], "grads"), ms(o[2], "exp_avgs"), vs(o[3], "exp_avg_sqs");
   const Py_ssize_t count = params.size();
   std::optional<List> m_scales, v_scales, masters, counters;
   if (o[5] != Py_None) m_scales.emplace(o[5], "exp_avg_scales");
@@ -643,17 +658,15 @@ PyObject *adamw_step(Args o) {
   if (v_scales) same(*v_scales, "exp_avg_sq_scales");
   if (masters) same(*masters, "masters");
   if (counters) same(*counters, "steps");
-  so3lr_adamw_args a{};
   a.beta1 = number(o[9], "betas");
   a.beta2 = number(o[10], "betas");
   a.eps = number(o[11], "eps");
   a.weight_decay = number(o[12], "weight_decay");
   a.count = count;
-  if (count == 0) return none();
+  if (count == 0) return;
   const Tensor &first = tensor(params[0], "params");
-  const c10::Device device = first.device();
+  device = first.device();
   if (!first.is_cuda()) refuse("params must be on a CUDA device, got ", device.str(), " (there is no CPU path)");
-  const c10::cuda::CUDAGuard guard(device);
   if (THPVariable_Check(o[8])) {
     const Tensor &lr = tensor(o[8], "lr");
     if (lr.device() != device || lr.scalar_type() != at::kFloat || lr.numel() != 1)
@@ -670,7 +683,7 @@ PyObject *adamw_step(Args o) {
              ", or a list of tensors of one");
     steps = reinterpret_cast<long long *>(t.data_ptr());
   }
-  std::vector<so3lr_adamw_tensor> tensors(count);
+  tensors.resize(count);
   for (Py_ssize_t i = 0; i < count; ++i) {
     so3lr_adamw_tensor &e = tensors[i];
     const Tensor &p = tensor(params[i], "params");
@@ -698,10 +711,34 @@ PyObject *adamw_step(Args o) {
                       : steps + i;
   }
   a.tensors = tensors.data();
+}
+void AdamwCall::run() const {
+  if (a.count == 0) return;
+  const c10::cuda::CUDAGuard guard(device);
   with_workspace(a, device, so3lr_adamw_workspace, so3lr_adamw);
   // what autograd has kept of the parameters for a backward pass to come is no longer what it was
-  for (Py_ssize_t i = 0; i < count; ++i)
+  for (Py_ssize_t i = 0; i < a.count; ++i)
     if (const Tensor &p = THPVariable_Unpack(params[i]); !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+}
+
+// adamw_step(an AdamwCall's arguments) -> None
+PyObject *adamw_step(Args o) {
+  AdamwCall(o).run();
+  return none();
+}
+
+// adamw_steps(a list of tuples of such arguments) -> None: nothing is launched before the last call's arguments
+// have been checked
+PyObject *adamw_steps(Args o) {
+  const List list(o[0], "calls");
+  std::deque<AdamwCall> calls;
+  for (Py_ssize_t i = 0; i < list.size(); ++i) {
+    if (!PyTuple_Check(list[i]) || PyTuple_GET_SIZE(list[i]) != 13) refuse("calls must be tuples of 13 arguments");
+    calls.emplace_back(&PyTuple_GET_ITEM(list[i], 0));
+  }
+  if (calls.size() > 1)
+    for (const AdamwCall &c : calls) c.check_arguments();
+  for (const AdamwCall &c : calls) c.run();
   return none();
 }
 
@@ -780,7 +817,7 @@ PyMethodDef g_methods[] = {METHOD(rms_norm, 5),        METHOD(rms_norm_backward,
                            METHOD(gate_int8, 1),       METHOD(dequantize_int8, 3),   METHOD(feed_forward, 5),
                            METHOD(feed_forward_backward, 7), METHOD(linear, 6),          METHOD(linear_backward, 8),
                            METHOD(sandwich_norm, 7),
-                           METHOD(sandwich_norm_backward, 10), METHOD(adamw_step, 13),
+                           METHOD(sandwich_norm_backward, 10), METHOD(adamw_step, 13),   METHOD(adamw_steps, 1),
                            METHOD(moment_values, 3),   METHOD(status, 1), METHOD(set_wait_limit, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_layers", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

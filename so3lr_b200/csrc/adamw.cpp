@@ -88,6 +88,9 @@ long long so3lr_adamw_workspace(const so3lr_adamw_args *args) {
     return so3lr_b200::adamw_bytes(*args);
   });
 }
+int so3lr_adamw_check(const so3lr_adamw_args *args, char *err, size_t errlen) {
+  return guarded(err, errlen, [&] { check(args); });
+}
 int so3lr_adamw(const so3lr_adamw_args *args, void *workspace, long long workspace_bytes, void *stream, char *err,
                 size_t errlen) {
   return guarded(err, errlen, [&] {

@@ -86,23 +86,32 @@ class AdamW(torch.optim.Optimizer):
             state["master"] = p.detach().float().clone(memory_format=torch.contiguous_format)
         return state
 
+    def _call(self, group, params, fresh):
+        """The arguments of the group's adamw_step; parameters whose state is made for it are added to fresh."""
+        grads = [g if g.is_sparse or g.is_contiguous() else g.contiguous() for g in [p.grad for p in params]]
+        states = [self.state[p] or fresh.append(p) or self._start(p, group) for p in params]
+        pick = lambda key: [s.get(key) for s in states]  # noqa: E731
+        return (params, grads, pick("exp_avg"), pick("exp_avg_sq"), pick("step"), pick("exp_avg_scale"),
+                pick("exp_avg_sq_scale"), pick("master"), group["lr"], *group["betas"], group["eps"], group["weight_decay"])
+
     @torch.no_grad()
     def step(self, closure=None):
+        """One step of every group, or none: what a group's call would refuse is refused before any is queued."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            params = [p for p in group["params"] if p.grad is not None]
-            if not params:
-                continue
-            grads = [p.grad if p.grad.is_sparse or p.grad.is_contiguous() else p.grad.contiguous() for p in params]
-            states = [self.state[p] or self._start(p, group) for p in params]
-            pick = lambda key: [s.get(key) for s in states]  # noqa: E731
-            adamw_step(params, grads, pick("exp_avg"), pick("exp_avg_sq"), pick("step"),
-                       exp_avg_scales=pick("exp_avg_scale"), exp_avg_sq_scales=pick("exp_avg_sq_scale"),
-                       masters=pick("master"), lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                       weight_decay=group["weight_decay"])
+        calls, fresh = [], []
+        try:
+            for group in self.param_groups:
+                params = [p for p in group["params"] if p.grad is not None]
+                if params:
+                    calls.append(self._call(group, params, fresh))
+            _layers.adamw_steps(calls)
+        except Exception:
+            for p in fresh:  # a master made now would be stale if the weights change before the next step
+                self.state.pop(p, None)
+            raise
         return loss
 
     def load_state_dict(self, state_dict):

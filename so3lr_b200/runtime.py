@@ -36,7 +36,7 @@ EXPORTED = (
     # dense layer, norms on both sides of a block (bound in layers.py), AdamW (bound in optim.py)
     "so3lr_linear_workspace", "so3lr_linear", "so3lr_linear_backward_workspace", "so3lr_linear_backward",
     "so3lr_sandwich_norm", "so3lr_sandwich_norm_backward_workspace", "so3lr_sandwich_norm_backward",
-    "so3lr_adamw_workspace", "so3lr_adamw", "so3lr_moment_values",
+    "so3lr_adamw_check", "so3lr_adamw_workspace", "so3lr_adamw", "so3lr_moment_values",
 )
 
 _dp = C.POINTER(C.c_double)
