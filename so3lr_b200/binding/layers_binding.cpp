@@ -742,6 +742,16 @@ PyObject *adamw_steps(Args o) {
   return none();
 }
 
+// uniform(a list of tensors) -> whether the dense ones are contiguous and all are on one device
+PyObject *uniform(Args o) {
+  const List list(o[0], "tensors");
+  for (Py_ssize_t i = 0; i < list.size(); ++i) {
+    const Tensor &t = tensor(list[i], "tensors");
+    if ((t.layout() == at::kStrided && !t.is_contiguous()) || t.device() != tensor(list[0], "tensors").device()) Py_RETURN_FALSE;
+  }
+  Py_RETURN_TRUE;
+}
+
 // moment_values(codes, scales, dtype) -> values
 PyObject *moment_values(Args o) {
   const Tensor &codes = tensor(o[0], "codes"), &scales = tensor(o[1], "scales");
@@ -818,6 +828,7 @@ PyMethodDef g_methods[] = {METHOD(rms_norm, 5),        METHOD(rms_norm_backward,
                            METHOD(feed_forward_backward, 7), METHOD(linear, 6),          METHOD(linear_backward, 8),
                            METHOD(sandwich_norm, 7),
                            METHOD(sandwich_norm_backward, 10), METHOD(adamw_step, 13),   METHOD(adamw_steps, 1),
+                           METHOD(uniform, 1),
                            METHOD(moment_values, 3),   METHOD(status, 1), METHOD(set_wait_limit, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_layers", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

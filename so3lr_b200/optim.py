@@ -48,6 +48,18 @@ def moment_values(codes, scales, dtype=torch.float32):
     return _layers.moment_values(codes, scales, dtype)
 
 
+def _copied(p, copies):
+    """A contiguous copy of a parameter of another layout, noted in copies."""
+    reach = 1  # of the dimensions so far, from the shortest stride on
+    for stride, size in sorted((t, n) for t, n in zip(p.stride(), p.shape) if n > 1):
+        if stride < reach:
+            raise ValueError(f"params: elements of a parameter share memory (shape {tuple(p.shape)}, strides {p.stride()})")
+        reach = stride * size
+    copy = p.contiguous()
+    copies.append((p, copy))
+    return copy
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW over all parameters of a group in one call.
 
@@ -56,7 +68,9 @@ class AdamW(torch.optim.Optimizer):
     update that; the parameter is its rounding, so what is written into a parameter after
     that step is lost. Each may be set for a group. lr may be a float32 tensor of one
     element on the GPU, for graphs. The first step allocates the state: take it before a
-    capture."""
+    capture. Parameters of a layout that is not contiguous are updated in a contiguous copy
+    and written back, which costs a copy each way; their state is contiguous. A group may span
+    several GPUs (with a rate that is a number)."""
 
     SMALL = 4096
 
@@ -101,17 +115,24 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls, fresh = [], []
+        calls, fresh, copies = [], [], []
         try:
             for group in self.param_groups:
                 params = [p for p in group["params"] if p.grad is not None]
-                if params:
-                    calls.append(self._call(group, params, fresh))
+                if _layers.uniform(params):
+                    calls += [self._call(group, params, fresh)] if params else []
+                else:
+                    for device in sorted({p.device for p in params}, key=str):
+                        there = [p for p in params if p.device == device]
+                        call = self._call(group, there, fresh)
+                        calls.append(([p if p.is_contiguous() else _copied(p, copies) for p in there], *call[1:]))
             _layers.adamw_steps(calls)
         except Exception:
             for p in fresh:  # a master made now would be stale if the weights change before the next step
                 self.state.pop(p, None)
             raise
+        for p, updated in copies:
+            p.copy_(updated)
         return loss
 
     def load_state_dict(self, state_dict):
