@@ -3,9 +3,11 @@
 // rounding.
 //
 // Bound by HBM (dy and z in, dz out): 8192 x 8192 bfloat16 70 us, 5.8 TB/s; rows off the boundaries, dy
-// one element at a time, 3.4 to 4.2 TB/s. What is read here is not read again and is not kept in L2 for
-// it: dz is, and the two products that follow find it there (a whole step of 24000 x 256 -> 1024 114 us
-// without, 107 with). A warp takes 256 columns of a row, or several rows of
+// one element at a time, 3.4 to 4.2 TB/s. With an activation what is read here is not read again and is not
+// kept in L2 for it: dz is, and the two products that follow find it there (a whole step of 24000 x 256 -> 1024
+// 114 us without, 107 with). Without one dy is dz, and only its column sums are formed here: its loads are
+// ordinary (24000 x 256 -> 1024 with a bias, backward, 62 us marked as first to be evicted, 61 so; 8192 x 4096 ->
+// 4096 after a kernel that wrote dy 392 and 381). A warp takes 256 columns of a row, or several rows of
 // narrow ones, 8 columns a lane; a block walks down its share of the rows and writes one row
 // of sums, which k_bias_sum adds in order.
 #include <algorithm>
@@ -29,13 +31,14 @@ struct BackArgs {
   bool dy_wide, z_wide;       // rows on 16-byte boundaries
 };
 
-template <bool WIDE, class T>
+// ONCE: no kernel after this one reads it
+template <bool WIDE, bool ONCE, class T>
 __device__ __forceinline__ Chunk<T, kVec> load_part(const T *p, bool wide, int left) {
-  if (WIDE) {
+  if (WIDE && ONCE) {
     const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(p));
     return *reinterpret_cast<const Chunk<T, kVec> *>(&v);
   }
-  if (wide && left >= kVec) return load_chunk<T, kVec>(p);
+  if (WIDE || (wide && left >= kVec)) return load_chunk<T, kVec>(p);
   Chunk<T, kVec> c;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) c.e[i] = i < left ? p[i] : from_float<T>(0.0f);
@@ -45,6 +48,7 @@ __device__ __forceinline__ Chunk<T, kVec> load_part(const T *p, bool wide, int l
 // WIDE: all rows on 16-byte boundaries and of whole chunks
 template <class T, int ACT, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs a) {
+  constexpr bool kOnce = ACT != SO3LR_NO_ACTIVATION;  // else dy is dz, which the products read next
   __shared__ float sums[kWarps * 32][kVec + 1];
   dependents_may_start();
   wait_for_predecessors();
@@ -75,16 +79,16 @@ __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs 
       Chunk<T, kVec> cd[kAtOnce], cz[kAtOnce];
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
-        cd[k] = load_part<WIDE>(dy + (row + k * step) * a.dy_stride, a.dy_wide, left);
-        if (ACT != SO3LR_NO_ACTIVATION) cz[k] = load_part<WIDE>(z + (row + k * step) * a.z_stride, a.z_wide, left);
+        cd[k] = load_part<WIDE, kOnce>(dy + (row + k * step) * a.dy_stride, a.dy_wide, left);
+        if (ACT != SO3LR_NO_ACTIVATION) cz[k] = load_part<WIDE, kOnce>(z + (row + k * step) * a.z_stride, a.z_wide, left);
       }
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) one(cd[k], cz[k], row + k * step);
     }
     for (; row < end; row += step) {
-      const Chunk<T, kVec> cd = load_part<WIDE>(dy + row * a.dy_stride, a.dy_wide, left);
+      const Chunk<T, kVec> cd = load_part<WIDE, kOnce>(dy + row * a.dy_stride, a.dy_wide, left);
       Chunk<T, kVec> cz{};
-      if (ACT != SO3LR_NO_ACTIVATION) cz = load_part<WIDE>(z + row * a.z_stride, a.z_wide, left);
+      if (ACT != SO3LR_NO_ACTIVATION) cz = load_part<WIDE, kOnce>(z + row * a.z_stride, a.z_wide, left);
       one(cd, cz, row);
     }
   }
