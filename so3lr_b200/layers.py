@@ -185,7 +185,8 @@ class _SandwichFunction(torch.autograd.Function):
     def forward(ctx, x, residual, weight, next_weight, gate, residual_scale, eps):
         y, s = _layers.sandwich_norm(x, residual, weight, next_weight, gate, residual_scale, eps)
         ctx.set_materialize_grads(False)  # an output that nothing reads has no gradient, rather than zeros
-        ctx.save_for_backward(x, residual, weight, next_weight, gate, residual_scale, s)
+        # the gradients read the residual with a scale only: without one it is not kept
+        ctx.save_for_backward(x, None if residual_scale is None else residual, weight, next_weight, gate, residual_scale, s)
         ctx.eps = eps
         return y, s
 
@@ -194,10 +195,10 @@ class _SandwichFunction(torch.autograd.Function):
     def backward(ctx, dy, ds):
         if dy is None and ds is None:
             return (None,) * 7
-        *operands, s = ctx.saved_tensors
+        x, residual, *operands, s = ctx.saved_tensors
         dy = torch.zeros_like(s) if dy is None else _dense_rows(dy)
-        dx, dresidual, dweight, dnext, dgate, dscale = _layers.sandwich_norm_backward(*operands, dy, _dense_rows(ds), s,
-                                                                                      ctx.eps)
+        dx, dresidual, dweight, dnext, dgate, dscale = _layers.sandwich_norm_backward(
+            x, x if residual is None else residual, *operands, dy, _dense_rows(ds), s, ctx.eps)
         return dx, dresidual, dweight, dnext, dgate, dscale, None
 
 
