@@ -138,10 +138,21 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch.optim.Optimizer's, with each state tensor in its own type: the base class
         would cast masters, moments and scales to the parameter's."""
-        super().load_state_dict(state_dict)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(saved, params):
-            if i in state_dict["state"]:
-                self.state[p] = {k: v.to(p.device, copy=True) if torch.is_tensor(v) else v
-                                 for k, v in state_dict["state"][i].items()}
+        loaded = {}
+
+        def restore(optimizer):
+            saved = [i for g in loaded["param_groups"] for i in g["params"]]
+            params = [p for g in optimizer.param_groups for p in g["params"]]
+            for i, p in zip(saved, params):
+                if i in loaded["state"]:
+                    optimizer.state[p] = {k: v.to(p.device, copy=True) if torch.is_tensor(v) else v
+                                          for k, v in loaded["state"][i].items()}
+
+        # after the caller's hooks before the load, which may replace the dictionary, and before those after it
+        hooks = (self.register_load_state_dict_pre_hook(lambda optimizer, given: loaded.update(given)),
+                 self.register_load_state_dict_post_hook(restore, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
