@@ -208,13 +208,6 @@ __device__ __forceinline__ float reciprocal(float v) {
   return r;
 }
 
-// An infinity becomes the largest number of its sign.
-__device__ __forceinline__ float at_most_largest(float v) {
-  float r;
-  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(3.402823466e38f));
-  return r;
-}
-
 // What of a tensor a block needs, and the coefficients of its step
 struct Work {
   const Entry &e;
@@ -259,17 +252,18 @@ __device__ __forceinline__ void update(const Work &a, long long at) {
     sum(Pair(a.b1) * Pair(m[i], m[i + 1]), Pair(a.c1) * gi, m[i], m[i + 1]);
     sum(Pair(a.b2) * Pair(v[i], v[i + 1]), Pair(a.c2) * (gi * gi), v[i], v[i + 1]);
   }
-  // 1 - lr decay in two floats, so that p is rounded once. An infinite p stays what it is: inf 0 would
-  // be NaN, so the second's product is with the largest number instead. (268 M elements in 8 bits 675 us
-  // with one float, 680 with two, 688 with infinities kept; 1092 with 32-bit moments in each form.)
-  const float keep = __fsub_rn(1.0f, coef.z), keep_low = __fsub_rn(__fsub_rn(1.0f, keep), coef.z);
+  // 1 - lr decay in two floats, so that p is rounded once. The second has the first's sign and is not 0,
+  // so that an infinite p stays infinite: inf 0 and inf - inf would be NaN. (268 M elements in 8 bits 675
+  // us with one float, 680 with two; 1092 with 32-bit moments in both forms.)
+  const float keep = __fmul_rn(__fsub_rn(1.0f, coef.z), 1.0f - 0x1p-23f);
+  const float keep_low = __fsub_rn(__fsub_rn(1.0f, keep), coef.z);
   // the denominators are at least eps, a normal number, and below 2^126
   auto move = [&](int i, const Pair &denominators) {
     float d, e;
     denominators.get(d, e);
     const Pair ratio = Pair(m[i], m[i + 1]) * Pair(reciprocal(d), reciprocal(e));
-    const Pair finite(at_most_largest(p[i]), at_most_largest(p[i + 1]));
-    madd(Pair(p[i], p[i + 1]), Pair(keep), madd(finite, Pair(keep_low), ratio * Pair(-coef.x))).get(p[i], p[i + 1]);
+    const Pair old(p[i], p[i + 1]);
+    madd(old, Pair(keep), madd(old, Pair(keep_low), ratio * Pair(-coef.x))).get(p[i], p[i + 1]);
   };
   auto move_by_root = [&] {
 #pragma unroll
