@@ -3,11 +3,11 @@
 //   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
 //   p = p (1 - lr decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
 //
-// Bound by HBM: an element is read and written once (28 bytes with 32-bit moments, 14
-// with 8-bit ones and a float32 master). With 32-bit moments 268 M elements take 1090 us, 6.9
-// TB/s; with 8-bit ones 317 M take 850 us, 5.2 TB/s, and under the power limit of a long run
-// 930. There neither fewer instructions (a third fewer: 870 us), nor five blocks an SM (845,
-// and the 32-bit step 1130), nor blocks of 2 or 4 times the elements (960 to 1300) help. Every tensor is cut into chunks of 2048
+// Bound by HBM: an element is read and written once (with a 16-bit parameter and a float32 master 28
+// bytes with 32-bit moments, 16 with 8-bit ones). With 32-bit moments 268 M elements take 1090 us, 6.9
+// TB/s; with 8-bit ones 317 M take 840 us, 6.0 TB/s, and under the power limit of a long run 957, 5.3.
+// There neither fewer instructions (a third fewer: 850 -> 870 us), nor five blocks an SM (845, and the
+// 32-bit step 1130), nor blocks of 2 or 4 times the elements (960 to 1300) help. Every tensor is cut into chunks of 2048
 // elements, a chunk is a block's work, and one launch covers all tensors: a block finds
 // its tensor in a table that travels as the kernel's argument, so that nothing is
 // copied to the GPU before it and a captured graph holds its own table. The step
@@ -450,8 +450,8 @@ void launch_step(const so3lr_adamw_args &a, float4 *coef, cudaStream_t s) {
 
 long long adamw_bytes(const so3lr_adamw_args &a) { return a.count * (long long)sizeof(float4); }
 
-// A table of 24 tensors (1.8 KB of arguments) where they fit: the driver copies the
-// whole argument at every launch, 28 KB for 400 tensors.
+// A table of 24 tensors (1.6 KB of arguments) where they fit: the driver copies the
+// whole argument at every launch, 26 KB for 400 tensors.
 void launch_adamw(const so3lr_adamw_args &a, void *workspace, cudaStream_t s) {
   float4 *coef = static_cast<float4 *>(workspace);
   if (a.count <= 24)

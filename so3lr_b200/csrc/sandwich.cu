@@ -18,6 +18,8 @@
 // Measured, 33.5 M elements with gate and scale, forward and backward (TB/s): bfloat16 rows of
 // 256 5.9 and 5.0, of 1024 5.8 and 5.2, of 4096 6.0 and 4.6, of 1003 4.0 and 3.3, of 16384 4.1 and
 // 1.8; float32 rows (half as many) 6.5 and 6.0, 6.5 and 6.1, 6.2 and 5.3, 5.7 and 5.3, 4.7 and 3.0.
+// Rows off the boundaries past 4096 elements go one element at a time in the backward pass: bfloat16 of
+// 8191 2.2 and 0.75 (803 us), float32 3.5 and 1.5.
 // With 2-byte elements a row's two reductions, about 50 instructions a thread, and one block of
 // 512 threads an SM (the column sums fill the registers) hold the backward pass back.
 #include "pairs.cuh"
@@ -33,7 +35,7 @@ __device__ __forceinline__ float inverse_root(float a) {
   return fabsf(e) < 1.0f ? fmaf(0.5f * y, e, y) : y;  // 0, infinities and NaN as they are
 }
 
-template <class T, class W>
+template <class T>
 struct SandwichRow {  // pointers to one row
   const T *x, *residual, *gate;
   T *s, *y;
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
   wait_for_predecessors();
   const RowTeam<LANES> team;
   bool live;
-  const SandwichRow<T, W> row(a, team_row<LANES>(a.rows, live));
+  const SandwichRow<T> row(a, team_row<LANES>(a.rows, live));
   const W *w = static_cast<const W *>(a.weight), *next = static_cast<const W *>(a.next_weight),
           *scale = static_cast<const W *>(a.residual_scale);
   const Span<SHIFT, VEC> span(row.x, int(a.width), team.t);
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 1024)
   if (span.edge >= 0) row.y[span.edge] = from_float<T>(to_float(ex) * rs * to_float(next[span.edge]));
 }
 
-template <class T, class W>
+template <class T>
 struct SandwichBackRow {
   const T *dy, *ds, *s, *x, *residual, *gate;
   T *dx, *dresidual, *dgate;
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(LANES ? kTeamThreads : 512, LANES && VEC *N ==
   // whole blocks walk together; a team past the last row adds nothing
   for (long long first = (long long)blockIdx.x * kTeams; first < a.rows; first += (long long)gridDim.x * kTeams) {
     const bool live = first + team_id < a.rows;
-    const SandwichBackRow<T, W> row(a, live ? first + team_id : a.rows - 1);
+    const SandwichBackRow<T> row(a, live ? first + team_id : a.rows - 1);
     Chunk<T, VEC> cs[N], cd[N], ce[N], cx[N], cr[N], cg[N];
     T es{}, ed{}, ee{}, ex{}, er{}, eg = from_float<T>(1.0f);
 #pragma unroll
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(512)
   for (; k < rows; ++k) {
     ring.wait(k);
     const T *stage = reinterpret_cast<const T *>(ring.stage(k));
-    const SandwichBackRow<T, W> row(a, blockIdx.x + (long long)k * gridDim.x);
+    const SandwichBackRow<T> row(a, blockIdx.x + (long long)k * gridDim.x);
     Chunk<T, VEC> cs[N], cd[N], cx[N];
     V squares[3] = {V(0.0f), V(0.0f), V(0.0f)};
 #pragma unroll
@@ -582,7 +584,7 @@ __global__ void __launch_bounds__(512) k_sandwich_backward_long(const so3lr_sand
   const W *w = static_cast<const W *>(a.weight), *next = static_cast<const W *>(a.next_weight),
           *scale = static_cast<const W *>(a.residual_scale);
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const SandwichBackRow<T, W> row(a, r);
+    const SandwichBackRow<T> row(a, r);
     float first[3] = {};  // sums of x^2, s^2, s dy next
 #pragma unroll 2
     for (int c = t * VEC; c < width; c += step) {
