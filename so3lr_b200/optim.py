@@ -60,6 +60,39 @@ def _copied(p, copies):
     return copy
 
 
+def _share_memory(a, b):
+    """Whether tensors share memory: whether k_i elements of each stride, as many as they have, make up the distance
+    between them."""
+    sizes = {}  # stride in bytes -> how far a and b go along it
+    for side, t in enumerate((a, b)):
+        for stride, n in ((1, t.element_size()), *((s * t.element_size(), n) for s, n in zip(t.stride(), t.shape))):
+            if n > 1:
+                sizes.setdefault(stride, [0, 0])[side] += n - 1
+    strides = sorted(sizes, reverse=True)
+    reach = [[sum(s * sizes[s][side] for s in strides[i:]) for side in (0, 1)] for i in range(len(strides) + 1)]
+
+    def found(i, distance):
+        if i == len(strides):
+            return distance == 0
+        s, (up, down) = strides[i], sizes[strides[i]]
+        least, most = max(-down, -((reach[i + 1][0] - distance) // s)), min(up, (distance + reach[i + 1][1]) // s)
+        return any(found(i + 1, distance - k * s) for k in range(least, most + 1))
+
+    return found(0, b.data_ptr() - a.data_ptr())
+
+
+def _check_apart(params):
+    """Refuses parameters that share memory where one is updated in a copy: it would be written over the other's step."""
+    size = lambda p: (1 + sum((n - 1) * s for n, s in zip(p.shape, p.stride()))) * p.element_size()  # noqa: E731
+    before = []  # those whose memory may reach the next one's
+    for p in sorted((p for p in params if p.numel()), key=lambda p: p.data_ptr()):
+        before = [q for q in before if q.data_ptr() + size(q) > p.data_ptr()]
+        for q in before:
+            if not (p.is_contiguous() and q.is_contiguous()) and _share_memory(q, p):
+                raise ValueError(f"params: parameters of shapes {tuple(q.shape)} and {tuple(p.shape)} share memory")
+        before.append(p)
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW over all parameters of a group in one call.
 
@@ -126,6 +159,8 @@ class AdamW(torch.optim.Optimizer):
                         there = [p for p in params if p.device == device]
                         call = self._call(group, there, fresh)
                         calls.append(([p if p.is_contiguous() else _copied(p, copies) for p in there], *call[1:]))
+            if copies:
+                _check_apart([p for group in self.param_groups for p in group["params"] if p.grad is not None])
             _layers.adamw_steps(calls)
         except Exception:
             for p in fresh:  # a master made now would be stale if the weights change before the next step

@@ -118,3 +118,57 @@ def test_a_call_for_each_device(optim, monkeypatch):
         lists = [x for x in c[:8] if isinstance(x, list)]
         assert len({t.device for x in lists for t in x if t is not None}) == 1
         assert all(len(x) == len(c[0]) for x in lists)
+
+
+def test_share_memory(optim):
+    """Against the elements' addresses, over random layouts of one storage. No GPU."""
+    import random
+    rng, storage = random.Random(0), torch.zeros(4000, dtype=torch.uint8)
+    seen = [0, 0]
+
+    def draw():
+        dtype = rng.choice((torch.uint8, torch.int16, torch.float32))
+        dims = [(rng.choice((1, 2, 3, 5, 8, 21, 40)), rng.randint(1, 5)) for _ in range(rng.randint(0, 3))]
+        base = storage[:4000 // 4 * 4].view(dtype)
+        return base.as_strided([n for _, n in dims], [s for s, _ in dims], rng.randint(0, 200) // dtype.itemsize)
+
+    def addresses(t):
+        at = torch.zeros((), dtype=torch.int64)
+        for n, s in zip(t.shape, t.stride()):
+            at = at[..., None] + torch.arange(n) * s
+        first = (t.data_ptr() - storage.data_ptr() + at.reshape(-1, 1) * t.element_size())
+        return set((first + torch.arange(t.element_size())).flatten().tolist())
+
+    for _ in range(3000):
+        a, b = draw(), draw()
+        want = bool(addresses(a) & addresses(b))
+        assert optim._share_memory(a, b) == want, (a.shape, a.stride(), a.data_ptr(), b.shape, b.stride(), b.data_ptr())
+        seen[want] += 1
+    assert min(seen) > 300
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [1, 2])
+def test_parameters_within_one_matrix(optim, groups):
+    """Columns of one matrix are parameters of their own; a matrix and its transpose are refused, in one group or in two."""
+    split = lambda params: params if groups == 1 else [dict(params=params[:1]), dict(params=params[1:])]  # noqa: E731
+    whole = _draw(1, 40, 30)
+    parts = [torch.nn.Parameter(whole[:, :11]), torch.nn.Parameter(whole[:, 11:])]
+    twins = [torch.nn.Parameter(p.detach().contiguous()) for p in parts]
+    adams = [optim.AdamW(split(p), lr=1e-2) for p in (parts, twins)]
+    for k in range(3):
+        for p, q in zip(parts, twins):
+            p.grad = _draw(5 + k, *p.shape)
+            q.grad = p.grad.clone()
+        for a in adams:
+            a.step()
+    for p, q in zip(parts, twins):
+        assert torch.equal(p, q)
+    both = [torch.nn.Parameter(whole), torch.nn.Parameter(whole.t())]
+    kept = whole.clone()
+    for p in both:
+        p.grad = torch.ones_like(p)
+    adam = optim.AdamW(split(both))
+    with pytest.raises(ValueError, match="share memory"):
+        adam.step()
+    assert torch.equal(whole, kept) and not any(adam.state.get(p) for p in both)
