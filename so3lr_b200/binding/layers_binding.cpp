@@ -747,7 +747,8 @@ PyObject *uniform(Args o) {
   const List list(o[0], "tensors");
   for (Py_ssize_t i = 0; i < list.size(); ++i) {
     const Tensor &t = tensor(list[i], "tensors");
-    if ((t.layout() == at::kStrided && !t.is_contiguous()) || t.device() != tensor(list[0], "tensors").device()) Py_RETURN_FALSE;
+    if (t.layout() == at::kStrided && !t.is_contiguous()) Py_RETURN_FALSE;
+    if (t.device() != tensor(list[0], "tensors").device()) Py_RETURN_FALSE;
   }
   Py_RETURN_TRUE;
 }

@@ -48,7 +48,7 @@ __device__ __forceinline__ Chunk<T, kVec> load_part(const T *p, bool wide, int l
 // WIDE: all rows on 16-byte boundaries and of whole chunks
 template <class T, int ACT, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs a) {
-  constexpr bool kOnce = ACT != SO3LR_NO_ACTIVATION;  // else dy is dz, which the products read next
+  constexpr bool kOnce = ACT != SO3LR_NO_ACTIVATION;  // else there is no z, and dy is dz, which the products read next
   __shared__ float sums[kWarps * 32][kVec + 1];
   dependents_may_start();
   wait_for_predecessors();
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs 
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
         cd[k] = load_part<WIDE, kOnce>(dy + (row + k * step) * a.dy_stride, a.dy_wide, left);
-        if (ACT != SO3LR_NO_ACTIVATION) cz[k] = load_part<WIDE, kOnce>(z + (row + k * step) * a.z_stride, a.z_wide, left);
+        if (kOnce) cz[k] = load_part<WIDE, kOnce>(z + (row + k * step) * a.z_stride, a.z_wide, left);
       }
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) one(cd[k], cz[k], row + k * step);
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_linear_backward(const BackArgs 
     for (; row < end; row += step) {
       const Chunk<T, kVec> cd = load_part<WIDE, kOnce>(dy + row * a.dy_stride, a.dy_wide, left);
       Chunk<T, kVec> cz{};
-      if (ACT != SO3LR_NO_ACTIVATION) cz = load_part<WIDE, kOnce>(z + row * a.z_stride, a.z_wide, left);
+      if (kOnce) cz = load_part<WIDE, kOnce>(z + row * a.z_stride, a.z_wide, left);
       one(cd, cz, row);
     }
   }
